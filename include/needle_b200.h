@@ -266,6 +266,131 @@ int needle_ffn_plan_forward(NeedleFfnPlan *plan, const float *x, size_t T, int a
 int needle_ffn_plan_status(NeedleFfnPlan *plan);
 void needle_ffn_plan_free(NeedleFfnPlan *plan);
 
+/* ── serving operators on device pointers (no counterpart in the reference) ──
+ * Building blocks for callers that assemble their own layers beside the INT4
+ * and MLP calls above: an 8-bit product, the norms around a block with its
+ * gate and residual, and cross attention to encoder states.  They run on the
+ * device that holds their first operand (a plan's calls on the plan's
+ * device), whatever device is current, and restore the current one.  `stream`
+ * (cudaStream_t or NULL) must belong to that device.  Every call but the
+ * plans' creation is asynchronous, allocates nothing and can be captured into
+ * a CUDA graph.  Sizes of zero are refused unless a comment says otherwise. */
+
+/* Element types of the operands below. */
+#define NEEDLE_F32 0
+#define NEEDLE_F16 1
+#define NEEDLE_BF16 2
+#define NEEDLE_I8 3
+
+/* 8-bit rows: [rows][needle_int8_row_bytes(K)] int8, K rounded up to 16, with
+ * one f32 scale for each row; element k of a row stands for value * scale.
+ * The bytes past K are zero where the library writes them and never read.
+ * A row is quantised as
+ *   top = max|x|, scale = top / 127, value = rint(x * (127 / top)),
+ * each operation rounded to f32 and rint to even, |value| <= 127; a row whose
+ * top is below 127 * 2^-126 becomes zeros with scale 0, and one that holds an
+ * infinity or NaN becomes zeros with scale NaN (its products are NaN). */
+size_t needle_int8_row_bytes(size_t K);
+
+/* x[M][ldx] (f32, f16 or bf16; ldx >= K elements) -> q [M][row_bytes(K)] and
+ * scales[M]: one scale for each token.  A weight stored [out][in] is packed by
+ * the same call, one scale for each output channel. */
+int needle_int8_quantize_tokens(const void *x, int x_dtype, size_t M, size_t K, size_t ldx, int8_t *q, float *scales,
+                                void *stream);
+/* w[K][N] (in-features by out-features, as needle_int4_quantize takes it) ->
+ * data [N][row_bytes(K)] and scales[N]: one scale for each output channel. */
+int needle_int8_quantize_weight(const void *w, int w_dtype, size_t K, size_t N, int8_t *data, float *scales,
+                                void *stream);
+
+/* A prepared 8-bit weight (data [N][row_bytes(K)], 16-byte aligned, and
+ * scales[N], both kept by the caller while the plan lives) for
+ *   y[m][n] = (sum_k q[m][k] w[n][k]) * (q_scales[m] * w_scales[n]) + bias[n]
+ * with an exact 32-bit integer sum (K <= 131,071), rounded once to y_dtype
+ * (f32, f16 or bf16).  needle_int8_plan_matmul quantises the tokens
+ * x[M][ldx] first (the same values as needle_int8_quantize_tokens), into the
+ * plan's workspace of max_m rows; needle_int8_plan_matmul_quantized takes rows
+ * that are quantised already (q 16-byte aligned).  M <= max_m; bias (f32[N])
+ * may be NULL; ldy >= N elements; y must not overlap the inputs.  Calls on one
+ * plan share its workspace and must be ordered (one stream), and so must the
+ * replays of graphs that captured them.  needle_int8_plan_status synchronises
+ * the device and returns -1 if a bounded wait inside a launch expired since
+ * the last check. */
+typedef struct NeedleInt8Plan NeedleInt8Plan;
+NeedleInt8Plan *needle_int8_plan_create(const int8_t *w_data, const float *w_scales, size_t K, size_t N, size_t max_m,
+                                        void *stream);
+int needle_int8_plan_matmul(NeedleInt8Plan *plan, const void *x, int x_dtype, size_t M, size_t ldx, const float *bias,
+                            void *y, int y_dtype, size_t ldy, void *stream);
+int needle_int8_plan_matmul_quantized(NeedleInt8Plan *plan, const int8_t *q, const float *q_scales, size_t M,
+                                      const float *bias, void *y, int y_dtype, size_t ldy, void *stream);
+int needle_int8_plan_status(NeedleInt8Plan *plan);
+void needle_int8_plan_free(NeedleInt8Plan *plan);
+
+/* The step between two blocks, for M rows of d elements (d <= 32,768):
+ *   r = residual_scale * x + g * post(y)     h = pre(r)
+ * with the model's ZCRMSNorm (crates/needle-core/src/norm.rs:23-30)
+ *   norm(v; s) = (1 + s) * v / sqrt(mean(v^2) + 1e-6).
+ * x: the residual stream, y: the block's output, post(y) = norm(y;
+ * post_scale), or y itself where post_scale is NULL; h: the next block's
+ * input, norm(r; pre_scale), taken from r before r is rounded to its type.
+ * The gate g is 1 (gate_flags 0, gate NULL), one f32 (NEEDLE_GATE_SCALAR), f32[d]
+ * (NEEDLE_GATE_CHANNEL) or a [M][ldg] matrix of y's type
+ * (NEEDLE_GATE_TOKEN); with NEEDLE_GATE_SIGMOID added, the logistic function
+ * of that.  All arithmetic is f32.
+ *   y NULL: r is x * residual_scale and only h is written (r must be NULL):
+ *     the norm before the first block; post_scale and gate must be NULL.
+ *   h NULL: only r is written; pre_scale must be NULL then.
+ * Types: x and r share x_dtype, y and a token gate share y_dtype; x_dtype is
+ * NEEDLE_F32 or y_dtype (both f32, f16 or bf16).  h is y_dtype, or NEEDLE_I8:
+ * rows of needle_int8_row_bytes(d) (ldh at least that, 16-byte aligned) with
+ * their scales in h_scales[M], ready for needle_int8_plan_matmul_quantized
+ * when ldh is that row size.  Strides are in elements.  r may be x and h may
+ * be y (same strides and, for h, type); else the outputs must not overlap the
+ * inputs or each other. */
+#define NEEDLE_GATE_SCALAR 1u
+#define NEEDLE_GATE_CHANNEL 2u
+#define NEEDLE_GATE_TOKEN 3u
+#define NEEDLE_GATE_SIGMOID 8u
+int needle_residual_norm(const void *x, int x_dtype, size_t ldx, const void *y, int y_dtype, size_t ldy, size_t M,
+                         size_t d, const float *post_scale, const void *gate, uint32_t gate_flags, size_t ldg,
+                         float residual_scale, const float *pre_scale, void *r, size_t ldr, void *h, int h_dtype,
+                         size_t ldh, float *h_scales, void *stream);
+
+/* Cross attention of n_seq requests to encoder states of other lengths:
+ * request i has query rows [q_start[i], q_start[i] + q_len[i]) of q and
+ * reads K and V rows [k_start[i], k_start[i] + k_len[i]), all of them
+ * (host arrays; lengths may be zero).  Key ranges may overlap or be the same
+ * (several drafts over one prompt); query ranges may not.  Query head h reads KV
+ * head h / (num_heads / num_kv_heads).  For every query row and head
+ *   s_j = scale * q . k_j,  out = sum_j exp(s_j) v_j / sum_j exp(s_j)
+ * over the request's keys j whose key_mask byte (one for each row of K, or NULL)
+ * is not zero; what masked keys and rows outside the request hold, NaN
+ * and infinity included, changes nothing.  A row without keys gives zeros.
+ * dtype: f16 or bf16 for q, k, v and out (sums in f32; the weights are rounded
+ * to dtype for the product with V); head_dim a multiple of 8 up to 128.
+ * The plan holds the split of the requests over the device and the
+ * workspace: lengths stay fixed while a prompt is decoded, so one plan serves
+ * every layer and step. */
+typedef struct NeedleCrossAttnPlan NeedleCrossAttnPlan;
+NeedleCrossAttnPlan *needle_cross_attn_plan_create(const uint64_t *q_start, const uint64_t *q_len,
+                                                   const uint64_t *k_start, const uint64_t *k_len, size_t n_seq,
+                                                   size_t num_heads, size_t num_kv_heads, size_t head_dim, int dtype,
+                                                   void *stream);
+/* Row r of head h of q is at q + r * q_row + h * q_head (elements), likewise
+ * k, v and out: token-major and head-major layouts, and parts of fused rows.
+ * Bases must be 16-byte aligned and strides multiples of 8 elements.  out must
+ * not overlap the inputs or itself; rows outside the requests are left as
+ * they were.  lse, if not NULL, is f32 [rows][num_heads], rows as in q, and
+ * receives log(sum_j exp(s_j)) (-infinity for a row without keys).  scale
+ * must be positive.  Calls on one plan share its workspace and must be ordered
+ * (one stream), and so must the replays of graphs that captured them. */
+int needle_cross_attn_plan_run(NeedleCrossAttnPlan *plan, const void *q, size_t q_row, size_t q_head, const void *k,
+                               size_t k_row, size_t k_head, const void *v, size_t v_row, size_t v_head,
+                               const uint8_t *key_mask, float scale, void *out, size_t out_row, size_t out_head,
+                               float *lse, void *stream);
+/* As needle_int8_plan_status. */
+int needle_cross_attn_plan_status(NeedleCrossAttnPlan *plan);
+void needle_cross_attn_plan_free(NeedleCrossAttnPlan *plan);
+
 /* ── SafeTensors reader (crates/needle-infer/src/safetensors.rs:43-128) ── */
 /* The weight-file reader needle_load uses, on a host buffer: header JSON with
  * a string-valued __metadata__ object, dtypes F32 / BF16 / F16 / I8 and the

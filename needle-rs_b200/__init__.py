@@ -109,6 +109,19 @@ def lib():
             "needle_ffn_plan_forward": (I, [P, P, S, I, P, P]),
             "needle_ffn_plan_status": (I, [P]),
             "needle_ffn_plan_free": (None, [P]),
+            "needle_int8_row_bytes": (S, [S]),
+            "needle_int8_quantize_tokens": (I, [P, I, S, S, S, P, P, P]),
+            "needle_int8_quantize_weight": (I, [P, I, S, S, P, P, P]),
+            "needle_int8_plan_create": (P, [P, P, S, S, S, P]),
+            "needle_int8_plan_matmul": (I, [P, P, I, S, S, P, P, I, S, P]),
+            "needle_int8_plan_matmul_quantized": (I, [P, P, P, S, P, P, I, S, P]),
+            "needle_int8_plan_status": (I, [P]),
+            "needle_int8_plan_free": (None, [P]),
+            "needle_residual_norm": (I, [P, I, S, P, I, S, S, S, P, P, U32, S, C.c_float, P, P, S, P, I, S, P, P]),
+            "needle_cross_attn_plan_create": (P, [P, P, P, P, S, S, S, S, I, P]),
+            "needle_cross_attn_plan_run": (I, [P, P, S, S, P, S, S, P, S, S, P, C.c_float, P, S, S, P, P]),
+            "needle_cross_attn_plan_status": (I, [P]),
+            "needle_cross_attn_plan_free": (None, [P]),
             "needle_safetensors_parse": (P, [P, S]),
             "needle_safetensors_metadata": (C.c_char_p, [P, C.c_char_p]),
             "needle_safetensors_get_f32": (S, [P, C.c_char_p, P, S]),
@@ -453,6 +466,117 @@ class FfnPlan:
     def close(self):
         if getattr(self, "_h", None):
             lib().needle_ffn_plan_free(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+# ── serving operators: 8-bit product, residual norm, cross attention ──
+F32, F16, BF16, I8 = 0, 1, 2, 3
+GATE_SCALAR, GATE_CHANNEL, GATE_TOKEN, GATE_SIGMOID = 1, 2, 3, 8
+
+
+def int8_row_bytes(K):
+    """Bytes of a quantised row of K elements (K rounded up to 16)."""
+    return lib().needle_int8_row_bytes(K)
+
+
+def int8_quantize_tokens(x_ptr, M, K, q_ptr, scales_ptr, dtype=F32, ldx=None, stream=None):
+    """x[M][ldx] -> int8 rows [M][int8_row_bytes(K)] and one f32 scale for each."""
+    _check(lib().needle_int8_quantize_tokens(x_ptr, dtype, M, K, K if ldx is None else ldx, q_ptr, scales_ptr, stream))
+
+
+def int8_quantize_weight(w_ptr, K, N, data_ptr, scales_ptr, dtype=F32, stream=None):
+    """w[K][N] -> int8 rows [N][int8_row_bytes(K)] and one f32 scale for each output channel."""
+    _check(lib().needle_int8_quantize_weight(w_ptr, dtype, K, N, data_ptr, scales_ptr, stream))
+
+
+class Int8Plan:
+    """A prepared 8-bit weight (device pointers: rows [N][int8_row_bytes(K)]
+    and N f32 scales, which must outlive the plan) for asynchronous products
+    of up to max_m tokens."""
+
+    def __init__(self, w_ptr, s_ptr, K, N, max_m, stream=None):
+        self.K, self.N, self.max_m = K, N, max_m
+        self._h = lib().needle_int8_plan_create(w_ptr, s_ptr, K, N, max_m, stream)
+        if not self._h:
+            raise NeedleError(last_error() or "needle_int8_plan_create failed")
+
+    def matmul(self, x_ptr, M, y_ptr, x_dtype=F32, y_dtype=F32, ldx=None, ldy=None, bias_ptr=None, stream=None):
+        """Quantises the tokens x[M][ldx] and multiplies."""
+        _check(_lib.needle_int8_plan_matmul(self._h, x_ptr, x_dtype, M, self.K if ldx is None else ldx, bias_ptr, y_ptr,
+                                            y_dtype, self.N if ldy is None else ldy, stream))
+
+    def matmul_quantized(self, q_ptr, q_scales_ptr, M, y_ptr, y_dtype=F32, ldy=None, bias_ptr=None, stream=None):
+        """Multiplies tokens that are quantised already."""
+        _check(_lib.needle_int8_plan_matmul_quantized(self._h, q_ptr, q_scales_ptr, M, bias_ptr, y_ptr, y_dtype,
+                                                      self.N if ldy is None else ldy, stream))
+
+    def status(self):
+        _check(lib().needle_int8_plan_status(self._h))
+
+    def close(self):
+        if getattr(self, "_h", None):
+            lib().needle_int8_plan_free(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def residual_norm(x_ptr, x_dtype, y_ptr, y_dtype, M, d, pre_scale_ptr, r_ptr, h_ptr, h_dtype, post_scale_ptr=None,
+                  gate_ptr=None, gate_flags=0, residual_scale=1.0, h_scales_ptr=None, ldx=None, ldy=None, ldg=None,
+                  ldr=None, ldh=None, stream=None):
+    """r = residual_scale * x + g * post(y) and h = pre(r) (needle_residual_norm).
+    Row strides default to d, that of an 8-bit h to int8_row_bytes(d)."""
+    if ldh is None:
+        ldh = (d + 15) // 16 * 16 if h_dtype == I8 else d
+    _check(lib().needle_residual_norm(x_ptr, x_dtype, d if ldx is None else ldx, y_ptr, y_dtype, d if ldy is None else ldy,
+                                      M, d, post_scale_ptr, gate_ptr, gate_flags, d if ldg is None else ldg,
+                                      residual_scale, pre_scale_ptr, r_ptr, d if ldr is None else ldr, h_ptr, h_dtype, ldh,
+                                      h_scales_ptr, stream))
+
+
+class CrossAttnPlan:
+    """Cross attention of ragged query rows to encoder states (needle_cross_attn_plan_*):
+    request i has q_len[i] query rows from q_start[i] on and reads k_len[i] K / V
+    rows from k_start[i] on.  run() is asynchronous and allocates nothing."""
+
+    def __init__(self, q_start, q_len, k_start, k_len, num_heads, num_kv_heads, head_dim, dtype=BF16, stream=None):
+        a = [np.ascontiguousarray(v, np.uint64) for v in (q_start, q_len, k_start, k_len)]
+        if any(v.ndim != 1 or v.size != a[0].size for v in a):
+            raise ValueError("q_start, q_len, k_start and k_len differ in length")
+        self.num_heads, self.num_kv_heads, self.head_dim = num_heads, num_kv_heads, head_dim
+        self._qs = (num_heads * head_dim, head_dim)
+        self._ks = (num_kv_heads * head_dim, head_dim)
+        self._h = lib().needle_cross_attn_plan_create(_p(a[0]), _p(a[1]), _p(a[2]), _p(a[3]), a[0].size, num_heads,
+                                                      num_kv_heads, head_dim, dtype, stream)
+        if not self._h:
+            raise NeedleError(last_error() or "needle_cross_attn_plan_create failed")
+
+    def run(self, q_ptr, k_ptr, v_ptr, out_ptr, scale, q_strides=None, k_strides=None, v_strides=None, out_strides=None,
+            key_mask_ptr=None, lse_ptr=None, stream=None):
+        """Strides are (row, head) in elements; by default [rows][heads][head_dim]."""
+        qr, qh = q_strides or self._qs
+        kr, kh = k_strides or self._ks
+        vr, vh = v_strides or self._ks
+        orow, oh = out_strides or self._qs
+        _check(_lib.needle_cross_attn_plan_run(self._h, q_ptr, qr, qh, k_ptr, kr, kh, v_ptr, vr, vh, key_mask_ptr, scale,
+                                               out_ptr, orow, oh, lse_ptr, stream))
+
+    def status(self):
+        _check(lib().needle_cross_attn_plan_status(self._h))
+
+    def close(self):
+        if getattr(self, "_h", None):
+            lib().needle_cross_attn_plan_free(self._h)
             self._h = None
 
     def __del__(self):

@@ -1,0 +1,182 @@
+"""The residual norm on the GPU against 64-bit arithmetic."""
+import pytest
+
+from conftest import load_pkg
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+nb = load_pkg()
+TYPES = {nb.F32: torch.float32, nb.F16: torch.float16, nb.BF16: torch.bfloat16}
+U = 2.0 ** -24
+KINDS = {"none": 0, "scalar": nb.GATE_SCALAR, "channel": nb.GATE_CHANNEL, "token": nb.GATE_TOKEN}
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _cuda():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    torch.cuda.init()
+
+
+def reference(x, y, post, gate, sigmoid, scale, pre):
+    """(r, h, tolerance of r, tolerance of h) before rounding to a type.
+
+    A statistic sums d squares: a thread up to 32 of them one after another,
+    then 10 levels of a tree, so it is off by at most 45 U relative and the
+    factor 1/sqrt by half of that and 4 roundings; gates and products add
+    under 12.  r: 40 U of each summand.  h: r's error times the factor, the
+    factor's own error (from r's errors and from its sum), 4 roundings."""
+    x = x.double()
+    if y is None:
+        r, er = scale * x, 2 * U * (scale * x).abs()
+    else:
+        y = y.double()
+        if post is not None:
+            y = (1 + post.double()) * y / torch.sqrt(y.pow(2).mean(-1, keepdim=True) + 1e-6)
+        if gate is not None:
+            g = gate.double()
+            y = y * (torch.sigmoid(g) if sigmoid else g)
+        r = scale * x + y
+        er = 40 * U * ((scale * x).abs() + y.abs())
+    if pre is None:
+        return r, None, er, None
+    inv = 1 / torch.sqrt(r.pow(2).mean(-1, keepdim=True) + 1e-6)
+    h = (1 + pre.double()) * r * inv
+    off = torch.sqrt(er.pow(2).mean(-1, keepdim=True)) * inv
+    eh = er * (1 + pre.double()).abs() * inv + h.abs() * (off + 40 * U)
+    return r, h, er, eh
+
+
+def rounded(e, v, dtype):
+    f = torch.finfo(TYPES[dtype])
+    return e + f.eps / 2 * (v.abs() + e) + f.tiny * f.eps / 2
+
+
+def close(got, want, tol):
+    got = got.double().cpu()
+    assert torch.isfinite(got).all()
+    assert ((got - want).abs() <= tol).all(), float(((got - want).abs() / tol).max())
+
+
+def inputs(M, d, tx, ty, gate, post, seed):
+    g = torch.Generator().manual_seed(seed)
+    rnd = lambda *s: torch.randn(s, generator=g)  # noqa: E731
+    x, y = (rnd(M, d) * 2).to(TYPES[tx]), (rnd(M, d) * 0.7).to(TYPES[ty])
+    gates = {"none": None, "scalar": rnd(1), "channel": rnd(d), "token": rnd(M, d).to(TYPES[ty])}[gate]
+    return x, y, gates, rnd(d) * 0.1 if post else None, rnd(d) * 0.1
+
+
+def cuda(*a):
+    return [None if t is None else t.cuda() for t in a]
+
+
+def p(t):
+    return None if t is None else t.data_ptr()
+
+
+CASES = [(1, 512, nb.F32, nb.F32, "scalar", True, False, 1.0), (1, 1, nb.F32, nb.BF16, "none", False, True, 1.0),
+         (5, 7, nb.F16, nb.F16, "token", True, True, 0.5), (9, 33, nb.BF16, nb.BF16, "channel", False, True, 1.0),
+         (17, 256, nb.F32, nb.F16, "token", False, False, 0.7), (3, 264, nb.F32, nb.F32, "channel", True, True, -1.5),
+         (4, 1000, nb.F32, nb.BF16, "channel", True, True, 1.0), (2, 1531, nb.F16, nb.F16, "scalar", False, True, 1.0),
+         (6, 2048, nb.BF16, nb.BF16, "none", False, False, 1.0), (3, 4096, nb.F32, nb.BF16, "token", True, True, 0.5),
+         (2, 4104, nb.F32, nb.F32, "token", True, True, 1.0), (2, 8191, nb.BF16, nb.BF16, "token", False, True, 1.0),
+         (2, 16384, nb.F32, nb.F16, "channel", True, True, 1.0), (1, 32768, nb.F32, nb.F32, "none", False, True, 1.0),
+         (1, 32767, nb.F16, nb.F16, "token", True, True, 1.0), (1000, 512, nb.F32, nb.F32, "scalar", True, True, 1.0)]
+
+
+@pytest.mark.parametrize("M,d,tx,ty,gate,sigmoid,post,scale", CASES)
+def test_against_64_bits(M, d, tx, ty, gate, sigmoid, post, scale):
+    x, y, g, ps, pre = inputs(M, d, tx, ty, gate, post, M + d)
+    r, h, er, eh = reference(x, y, ps, g, sigmoid, scale, pre)
+    flags = KINDS[gate] | (nb.GATE_SIGMOID if gate != "none" and sigmoid else 0)
+    xd, yd, gd, pd, prd = cuda(x, y, g, ps, pre)
+    rd, hd = torch.full_like(xd, float("nan")), torch.full_like(yd, float("nan"))
+    common = dict(post_scale_ptr=p(pd), gate_ptr=p(gd), gate_flags=flags, residual_scale=scale)
+    nb.residual_norm(p(xd), tx, p(yd), ty, M, d, p(prd), p(rd), p(hd), ty, **common)
+    close(rd, r, rounded(er, r, tx))
+    close(hd, h, rounded(eh, h, ty))
+    # 8-bit rows: the scale is max|h| / 127, each value within half a step
+    Kp = nb.int8_row_bytes(d)
+    q, s = torch.full((M, Kp), 9, dtype=torch.int8, device="cuda"), torch.empty(M, device="cuda")
+    r2 = torch.empty_like(rd)
+    nb.residual_norm(p(xd), tx, p(yd), ty, M, d, p(prd), p(r2), p(q), nb.I8, h_scales_ptr=p(s), **common)
+    assert torch.equal(r2, rd) and not q[:, d:].any()
+    s, q = s.double().cpu(), q[:, :d].double().cpu()
+    top = h.abs().max(dim=1).values
+    etop = eh.max(dim=1).values
+    assert ((s - top / 127).abs() <= etop / 127 + 2 * U * s).all()
+    # the quotient is rounded to f32 twice (127 / top and the product), up to 127 steps from zero
+    close(q * s[:, None], h, eh + s[:, None] * (0.5 + 4 * 127 * U) + etop[:, None])
+    assert (q.abs().max(dim=1).values == 127).all()
+    # r alone, in place; h in the place of y
+    nb.residual_norm(p(xd), tx, p(yd), ty, M, d, None, p(xd), None, ty, **common)
+    assert torch.equal(xd, rd)
+    xd = x.cuda()
+    nb.residual_norm(p(xd), tx, p(yd), ty, M, d, p(prd), p(xd), p(yd), ty, **common)
+    assert torch.equal(xd, rd) and torch.equal(yd, hd)
+
+
+@pytest.mark.parametrize("M,d,tx,ty", [(3, 512, nb.F32, nb.BF16), (2, 77, nb.F32, nb.F32), (1, 8200, nb.F16, nb.F16)])
+def test_norm_before_the_first_block(M, d, tx, ty):
+    x, _, _, _, pre = inputs(M, d, tx, ty, "none", False, 3)
+    _, h, _, eh = reference(x, None, None, None, False, 0.25, pre)
+    xd, prd = cuda(x, pre)
+    hd = torch.empty((M, d), dtype=TYPES[ty], device="cuda")
+    nb.residual_norm(p(xd), tx, None, ty, M, d, p(prd), None, p(hd), ty, residual_scale=0.25)
+    close(hd, h, rounded(eh, h, ty))
+
+
+@pytest.mark.parametrize("d", [40, 1000, 37])
+@pytest.mark.parametrize("off", [0, 1])
+def test_strides_and_alignment(d, off):
+    """Rows inside wider rows, on and off 16-byte boundaries; what lies between them stays."""
+    M, ty = 6, nb.BF16
+    x, y, g, ps, pre = inputs(M, d, nb.F32, ty, "token", True, d)
+    r, h, er, eh = reference(x, y, ps, g, True, 1.0, pre)
+    ld = (d + 7) // 8 * 8 + 8 * (1 - off) + 3 * off
+
+    def wide(t, dtype):
+        b = torch.full((M * ld + 16,), 5.0, dtype=TYPES[dtype], device="cuda")
+        v = b[off:off + M * ld].view(M, ld)
+        if t is not None:
+            v[:, :d] = t.cuda()
+        return v
+
+    xd, yd, gd, rd, hd = wide(x, nb.F32), wide(y, ty), wide(g, ty), wide(None, nb.F32), wide(None, ty)
+    pd, prd = cuda(ps, pre)
+    nb.residual_norm(p(xd), nb.F32, p(yd), ty, M, d, p(prd), p(rd), p(hd), ty, post_scale_ptr=p(pd), gate_ptr=p(gd),
+                     gate_flags=nb.GATE_TOKEN | nb.GATE_SIGMOID, ldx=ld, ldy=ld, ldg=ld, ldr=ld, ldh=ld)
+    close(rd[:, :d], r, rounded(er, r, nb.F32))
+    close(hd[:, :d], h, rounded(eh, h, ty))
+    assert (rd[:, d:] == 5).all() and (hd[:, d:] == 5).all()
+
+
+def test_zero_rows_infinities_and_nan():
+    M, d = 4, 96
+    x, y, _, ps, pre = inputs(M, d, nb.F32, nb.F32, "none", True, 1)
+    x[0], y[0] = 0, 0
+    x[1, 4], y[2, 7] = float("inf"), float("nan")
+    xd, yd, pd, prd = cuda(x, y, ps, pre)
+    rd, q, s = torch.empty_like(xd), torch.empty((M, 96), dtype=torch.int8, device="cuda"), torch.empty(M, device="cuda")
+    nb.residual_norm(p(xd), nb.F32, p(yd), nb.F32, M, d, p(prd), p(rd), p(q), nb.I8, post_scale_ptr=p(pd), h_scales_ptr=p(s))
+    s, q = s.cpu(), q.cpu()
+    assert s[0] == 0 and not q[0].any() and torch.isnan(s[1]) and torch.isnan(s[2]) and s[3] > 0
+    assert not q[1].any() and not q[2].any()
+
+
+def test_graph_on_another_stream():
+    M, d = 33, 512
+    x, y, g, ps, pre = inputs(M, d, nb.F32, nb.BF16, "scalar", True, 8)
+    xd, yd, gd, pd, prd = cuda(x, y, g, ps, pre)
+    rd, hd = torch.empty_like(xd), torch.empty_like(yd)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr, stream=torch.cuda.Stream()):
+        nb.residual_norm(p(xd), nb.F32, p(yd), nb.BF16, M, d, p(prd), p(rd), p(hd), nb.BF16, post_scale_ptr=p(pd), gate_ptr=p(gd),
+                         gate_flags=nb.GATE_SCALAR | nb.GATE_SIGMOID, stream=torch.cuda.current_stream().cuda_stream)
+    x2 = x + 1
+    xd.copy_(x2)
+    gr.replay()
+    r, h, er, eh = reference(x2, y, ps, g, True, 1.0, pre)
+    close(rd, r, rounded(er, r, nb.F32))
+    close(hd, h, rounded(eh, h, nb.BF16))
