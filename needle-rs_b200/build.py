@@ -17,7 +17,7 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 CU = ["int4_matmul.cu", "attention.cu", "head.cu", "tc_gemm.cu", "tc_attn.cu", "ffn_noalloc.cu", "measure.cu",
       "int8_matmul.cu", "residual_norm.cu", "cross_attn.cu"]
-CPP = ["safetensors.cpp", "frontend.cpp", "engine.cpp", "capi.cpp", "ops.cpp"]
+CPP = ["safetensors.cpp", "frontend.cpp", "engine.cpp", "capi.cpp", "ops.cpp", "tma_encode.cpp"]
 
 
 def sources():

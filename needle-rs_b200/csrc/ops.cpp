@@ -121,7 +121,7 @@ void free_buffer(int device, void *buf) {
 
 struct NeedleInt8Plan {
   int device = 0;
-  const int8_t *w = nullptr;
+  CUtensorMap w_map;
   const float *w_scales = nullptr;
   int K = 0, N = 0, max_m = 0;
   void *buf = nullptr;
@@ -141,9 +141,9 @@ struct NeedleCrossAttnPlan {
 namespace {
 
 bool int8_product(NeedleInt8Plan *p, const int8_t *q, const float *qs, size_t M, const float *bias, void *y, int y_dtype,
-                  size_t ldy, cudaStream_t st) {
-  Int8Args a{q, p->w, qs, p->w_scales, bias, y, (int64_t)ldy, (int)M, p->N, p->K, y_dtype};
-  return ok(int8_matmul(a, p->flag, st));
+                  size_t ldy, bool pdl, cudaStream_t st) {
+  Int8Args a{q, &p->w_map, qs, p->w_scales, bias, y, (int64_t)ldy, (int)M, p->N, p->K, y_dtype};
+  return ok(int8_matmul(a, pdl, p->flag, st));
 }
 
 }  // namespace
@@ -196,7 +196,7 @@ NeedleInt8Plan *needle_int8_plan_create(const int8_t *w, const float *s, size_t 
     if (!on.good()) return false;
     plan = new NeedleInt8Plan();
     plan->device = device;
-    plan->w = w;
+    if (!ok(int8_weight_map(&plan->w_map, w, (int64_t)N, (int)K))) return false;
     plan->w_scales = s;
     plan->K = (int)K;
     plan->N = (int)N;
@@ -225,7 +225,7 @@ int needle_int8_plan_matmul(NeedleInt8Plan *p, const void *x, int x_dtype, size_
     if (!on.good() || !all_on(p->device, {{"x", x}, {"y", y}, {"bias", bias}})) return false;
     cudaStream_t st = (cudaStream_t)stream;
     return ok(int8_quantize_rows(x, x_dtype, (int64_t)M, p->K, (int64_t)ldx, p->q, p->q_scales, st)) &&
-           int8_product(p, p->q, p->q_scales, M, bias, y, y_dtype, ldy, st);
+           int8_product(p, p->q, p->q_scales, M, bias, y, y_dtype, ldy, true, st);
   }) ? 0 : -1;
 }
 
@@ -238,7 +238,7 @@ int needle_int8_plan_matmul_quantized(NeedleInt8Plan *p, const int8_t *q, const 
       return fail("invalid plan matmul arguments");
     OnDevice on(p->device);
     if (!on.good() || !all_on(p->device, {{"q", q}, {"q_scales", q_scales}, {"y", y}, {"bias", bias}})) return false;
-    return int8_product(p, q, q_scales, M, bias, y, y_dtype, ldy, (cudaStream_t)stream);
+    return int8_product(p, q, q_scales, M, bias, y, y_dtype, ldy, false, (cudaStream_t)stream);
   }) ? 0 : -1;
 }
 

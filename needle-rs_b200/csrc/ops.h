@@ -4,6 +4,7 @@
 // All pointers are device pointers unless a name says host.  Launchers enqueue
 // on `st` and return the launch status.
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
@@ -27,14 +28,20 @@ cudaError_t int8_quantize_rows(const void *x, int dtype, int64_t M, int64_t K, i
 cudaError_t int8_quantize_cols(const void *w, int dtype, int64_t K, int64_t N, int8_t *data, float *scales,
                                cudaStream_t st);
 struct Int8Args {
-  const int8_t *q, *w;               // [M][Kp], [N][Kp]
+  const int8_t *q;                   // [M][Kp]
+  const CUtensorMap *w_map;          // of the weight [N][Kp] (host)
   const float *q_scales, *w_scales;  // [M], [N]
   const float *bias;                 // [N] or NULL
   void *y;                           // [M][ldy] of y_dtype
   int64_t ldy;
   int M, N, K, y_dtype;
 };
-cudaError_t int8_matmul(const Int8Args &a, int *err, cudaStream_t st);
+// TMA descriptor of a weight [N][Kp], 16-byte aligned.
+cudaError_t int8_weight_map(CUtensorMap *map, const int8_t *w, int64_t N, int K);
+// *err is set if a bounded wait inside the kernel expired.  pdl: the kernel
+// before it in the stream is int8_quantize_rows of the same tokens, which it
+// may overlap (programmatic dependent launch).
+cudaError_t int8_matmul(const Int8Args &a, bool pdl, int *err, cudaStream_t st);
 
 // ── residual norm ──
 struct ResidualNormArgs {

@@ -11,14 +11,12 @@
 // statistics is one reduction over the row's threads, in f32.  Up to 1,024
 // elements a warp owns a row and reduces with shuffles alone; above, a block
 // does.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
 #include <algorithm>
 
 #include "common.cuh"
 #include "ops.h"
 #include "quant8.cuh"
+#include "rowio.cuh"
 
 namespace ndl {
 namespace {
@@ -26,66 +24,15 @@ namespace {
 constexpr float kEps = 1e-6f;
 constexpr int kWarpRows = 8;  // rows of a block whose warps own a row each
 
-template <typename T>
-__device__ __forceinline__ float to_f32(T v) {
-  return (float)v;
-}
-template <typename T>
-__device__ __forceinline__ T from_f32(float v);
-template <>
-__device__ __forceinline__ float from_f32<float>(float v) {
-  return v;
-}
-template <>
-__device__ __forceinline__ __half from_f32<__half>(float v) {
-  return __float2half_rn(v);
-}
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
-  return __float2bfloat16_rn(v);
-}
-
-// VEC consecutive elements as f32 (16-byte accesses for VEC = 8).
-template <int VEC, typename T>
-__device__ __forceinline__ void load(const T *p, float *v) {
-  if constexpr (VEC == 1) {
-    v[0] = to_f32(*p);
-  } else {
-    constexpr int N = VEC * (int)sizeof(T) / 16;
-    uint4 raw[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) raw[i] = reinterpret_cast<const uint4 *>(p)[i];
-    const T *e = reinterpret_cast<const T *>(raw);
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = to_f32(e[i]);
-  }
-}
-template <int VEC, typename T>
-__device__ __forceinline__ void store(T *p, const float *v) {
-  if constexpr (VEC == 1) {
-    *p = from_f32<T>(v[0]);
-  } else {
-    constexpr int N = VEC * (int)sizeof(T) / 16;
-    alignas(16) T e[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) e[i] = from_f32<T>(v[i]);
-#pragma unroll
-    for (int i = 0; i < N; ++i) reinterpret_cast<uint4 *>(p)[i] = reinterpret_cast<const uint4 *>(e)[i];
-  }
-}
-
-// Sum (or maximum) over the threads of a row; `warps` of them when the block
-// owns the row, else one.  `sm` holds a value for each warp and is free again
-// when every thread has passed the next reduction's barrier.
-template <bool MAX>
-__device__ __forceinline__ float row_reduce(float v, int warps, float *sm) {
-  v = MAX ? warp_max(v) : warp_sum(v);
+// Sum over the threads of a row; `warps` of them when the block owns the row,
+// else one.  sm: a word for each warp.
+__device__ __forceinline__ float row_sum(float v, int warps, float *sm) {
+  v = warp_sum(v);
   if (warps == 1) return v;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (lane == 0) sm[warp] = v;
   __syncthreads();
-  v = lane < warps ? sm[lane] : 0.0f;
-  return MAX ? warp_max(v) : warp_sum(v);
+  return warp_sum(lane < warps ? sm[lane] : 0.0f);
 }
 
 // Threads of a block: up to 256 with 8 or 16 elements each in whole vectors
@@ -117,7 +64,7 @@ __global__ void __launch_bounds__(kMaxThreads<VEC, CH>) residual_norm_kernel(Res
       for (int j = 0; j < VEC; ++j) ss += r[c][j] * r[c][j];
     }
     float inv = 1.0f;
-    if (a.post) inv = 1.0f / sqrtf(row_reduce<false>(ss, warps, sm[0]) / (float)d + kEps);
+    if (a.post) inv = 1.0f / sqrtf(row_sum(ss, warps, sm[0]) / (float)d + kEps);
     float g = 1.0f;
     if (a.gate_kind == 1) {
       g = *(const float *)a.gate;
@@ -167,7 +114,7 @@ __global__ void __launch_bounds__(kMaxThreads<VEC, CH>) residual_norm_kernel(Res
   for (int c = 0; c < CH; ++c)
 #pragma unroll
     for (int j = 0; j < VEC; ++j) ss += r[c][j] * r[c][j];
-  const float inv = 1.0f / sqrtf(row_reduce<false>(ss, warps, sm[1]) / (float)d + kEps);
+  const float inv = 1.0f / sqrtf(row_sum(ss, warps, sm[1]) / (float)d + kEps);
   uint32_t top = 0;  // largest |h| as bits: infinities and NaN order above every number
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
@@ -184,17 +131,7 @@ __global__ void __launch_bounds__(kMaxThreads<VEC, CH>) residual_norm_kernel(Res
     }
   }
   if (a.h_dtype != DT_I8) return;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (warps > 1) {
-    uint32_t *smu = reinterpret_cast<uint32_t *>(sm[2]);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (lane == 0) smu[warp] = top;
-    __syncthreads();
-    top = lane < warps ? smu[lane] : 0u;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  }
+  top = row_max_bits(top, warps, reinterpret_cast<uint32_t *>(sm[2]));
   const RowScale rs = int8_row_scale(top);
   int8_t *h = (int8_t *)a.h + row * a.ldh;
   const int dp = (d + 15) / 16 * 16;  // the row's bytes past d are zero
