@@ -2,6 +2,21 @@
 // lengths:
 //   s_j = scale * q . k_j     out = sum_j e^(s_j) v_j / sum_j e^(s_j)
 // over a request's keys, masked ones left out.
+//
+// The query heads that share a KV head are rows of one matrix: row r of a
+// request and KV head is token r / G, head kvh * G + r % G (G = H / KVH), so K
+// and V are read once for all of them.  One pass over the keys keeps a running
+// maximum m and sum l for each row (f32); weights are e^(s - m), rounded to the
+// operands' type for the product with V, whose sums are f32.
+//
+// Two kernels.  Up to 32 rows read K and V from HBM faster than any tensor
+// core needs them: xattn_few_kernel streams them through a ring for each warp
+// and multiplies with mma.sync (16 rows an instruction).  More rows are bound by the
+// exponentials and the products: xattn_tile_kernel runs both on tcgen05 with
+// 128-row tiles in TMEM.
+//
+// Long key ranges are cut so that all SMs work; the cuts' partial results
+// (unnormalised sums, m in units of log2, l) meet in xattn_join_kernel.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -9,76 +24,909 @@
 
 #include "common.cuh"
 #include "ops.h"
+#include "rowio.cuh"
+#include "tc_common.cuh"
+#include "tma_encode.h"
 
 namespace ndl {
 namespace {
 
-constexpr int kRows = 8;
+using namespace tc;
 
-// A warp for each packed row: 32 keys at a time, a lane for each key's score,
-// then a lane for each 4 dimensions of the sum.
+// 2^x by the PTX base-2 exponential (a few ulp; results below 2^-126 become 0).
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 template <typename T>
-__global__ void cross_attn_rows_kernel(XAttnWork w, XAttnCall c) {
-  const XAttnItem it = w.items[blockIdx.x];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = w.s.H / w.s.KVH, D = w.s.D;
-  if (warp >= it.rows) return;
-  const int r = it.r0 + warp, h = it.kvh * G + r % G;
-  const int64_t qrow = it.q0 + r / G;
-  const T *q = (const T *)c.q + qrow * c.q_row + (int64_t)h * c.q_head;
-  float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int j0 = 0; j0 < it.klen; j0 += 32) {
-    const int64_t key = it.k0 + j0 + lane;
-    const bool seen = j0 + lane < it.klen && (!c.mask || c.mask[key]);
-    float s = -INFINITY;
-    if (seen) {
-      const T *k = (const T *)c.k + key * c.k_row + (int64_t)it.kvh * c.k_head;
-      s = 0.0f;
-      for (int i = 0; i < D; ++i) s += (float)q[i] * (float)k[i];
-      s *= c.scale;
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// Partial results of split `s` of an item's rows: [rows][DP] sums, then m and
+// l of each row, in a piece of rows * (DP + 4) floats (16-byte multiples).
+__device__ __forceinline__ float *partial(const XAttnWork &w, const XAttnItem &it, int s, int DP) {
+  return w.ws + it.ws + (int64_t)s * it.rows * (DP + 4);
+}
+
+// ── few rows ────────────────────────────────────────────────────────────────
+
+constexpr int kFewWarps = 4, kFewKeys = 16, kFewStages = 3;
+
+template <int DP>
+constexpr int kFewStageBytes = 2 * kFewKeys * DP * 2;  // K and V rows of 16 keys
+template <int DP>
+constexpr int kFewSmem = kFewWarps * kFewStages * kFewStageBytes<DP> + kFewWarps * kFewStages * 4;
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool take) {
+  const int n = take ? 16 : 0;  // 0: the 16 bytes become zero and src is not read
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void ldm4(uint32_t *r, uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a)
+               : "memory");
+}
+__device__ __forceinline__ void ldm4t(uint32_t *r, uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a)
+               : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma16(float *d, const uint32_t *a, uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16<__half>(float *d, const uint32_t *a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16<__nv_bfloat16>(float *d, const uint32_t *a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Up to 16 * MT rows of one request and KV head.  Each of four warps takes
+// every fourth block of 16 keys through its own ring of cp.async stages, with
+// its own running maxima: no barrier until the warps' results meet in shared
+// memory at the end.  Rows of masked keys, of keys past the item and dimensions
+// past D are written as zeros by the copies themselves, so nothing that they
+// hold can reach a product.  Ring rows are swizzled (16-byte chunk c of row r
+// at c ^ (r & 7)): ldmatrix reads them without bank conflicts.
+template <typename T, int DP, int MT>
+__global__ void __launch_bounds__(kFewWarps * 32) xattn_few_kernel(const XAttnItem *items, XAttnWork w, XAttnCall c) {
+  constexpr int CH = DP / 8, KS = DP / 16;  // 16-byte chunks of a row, MMA steps over the dimensions
+  extern __shared__ __align__(128) uint8_t sm[];
+  uint32_t *live_of = reinterpret_cast<uint32_t *>(sm + kFewWarps * kFewStages * kFewStageBytes<DP>);
+  pdl_trigger();
+  const XAttnItem it = items[blockIdx.x];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int G = w.s.H / w.s.KVH, D = w.s.D;
+  const int nblk = (it.klen + kFewKeys - 1) / kFewKeys;
+  const T *kb = (const T *)c.k + it.k0 * c.k_row + (int64_t)it.kvh * c.k_head;
+  const T *vb = (const T *)c.v + it.k0 * c.v_row + (int64_t)it.kvh * c.v_head;
+  const uint8_t *mask = c.mask ? c.mask + it.k0 : nullptr;
+  const uint32_t ring = smem_u32(sm) + warp * kFewStages * kFewStageBytes<DP>;
+
+  // lane j < 16: whether key j of block b is attended to
+  auto look = [&](int b) -> bool {
+    const int j = b * kFewKeys + lane;
+    return lane < kFewKeys && j < it.klen && (!mask || mask[j] != 0);
+  };
+  auto issue = [&](int b, int stage, bool seen) {
+    const uint32_t live = __ballot_sync(0xffffffffu, seen);
+    if (lane == 0) live_of[warp * kFewStages + stage] = live;
+    const uint32_t dst = ring + stage * kFewStageBytes<DP>;
+#pragma unroll
+    for (int i = 0; i < CH / 2; ++i) {
+      const int id = lane + 32 * i, row = id / CH, ch = id % CH;
+      const bool take = ((live >> row) & 1) && ch * 8 < D;
+      const int64_t key = b * kFewKeys + row;
+      const uint32_t at = dst + row * (DP * 2) + ((ch ^ (row & 7)) << 4);
+      cp16(at, take ? kb + key * c.k_row + ch * 8 : kb, take);
+      cp16(at + kFewKeys * DP * 2, take ? vb + key * c.v_row + ch * 8 : vb, take);
     }
-    const float mn = fmaxf(m, warp_max(s));
-    if (mn == -INFINITY) continue;
-    const float p = s == -INFINITY ? 0.0f : expf(s - mn), f = expf(m - mn);
-    l = l * f + warp_sum(p);
-    for (int i = 0; i < 4; ++i) o[i] *= f;
-    m = mn;
-    const unsigned live = __ballot_sync(0xffffffffu, seen);
-    for (int j = 0; j < 32; ++j) {
-      const float pj = __shfl_sync(0xffffffffu, p, j);
-      if (!((live >> j) & 1)) continue;
-      const T *v = (const T *)c.v + (it.k0 + j0 + j) * c.v_row + (int64_t)it.kvh * c.v_head;
-      for (int i = 0; i < 4; ++i)
-        if (4 * lane + i < D) o[i] += pj * (float)v[4 * lane + i];
+  };
+
+  bool seen = look(warp);
+#pragma unroll
+  for (int s = 0; s < kFewStages - 1; ++s) {
+    const int b = warp + s * kFewWarps;
+    const bool next = look(b + kFewWarps);
+    if (b < nblk) issue(b, s, seen);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    seen = next;
+  }
+
+  // Q as MMA fragments (rows g and g + 8 of each 16)
+  uint32_t qf[MT][KS][4];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int i = mt * 16 + h * 8 + g, r = it.r0 + i;
+      const T *q = (const T *)c.q + (it.q0 + r / G) * c.q_row + (int64_t)(it.kvh * G + r % G) * c.q_head;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int d = ks * 16 + u * 8 + 2 * t;
+          qf[mt][ks][2 * u + h] = i < it.rows && d < D ? *reinterpret_cast<const uint32_t *>(q + d) : 0u;
+        }
+    }
+
+  const float sc = c.scale * kLog2e;
+  float o[MT][DP / 8][4], m[MT][2], l[MT][2];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+    for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[mt][n][i] = 0.0f;
+    m[mt][0] = m[mt][1] = -INFINITY;
+    l[mt][0] = l[mt][1] = 0.0f;
+  }
+
+  int stage = 0;
+  for (int b = warp; b < nblk; b += kFewWarps) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kFewStages - 2) : "memory");
+    __syncwarp();  // every lane's copies of this stage, and the reads of the stage refilled next
+    {
+      const int nb = b + (kFewStages - 1) * kFewWarps, ns = stage == 0 ? kFewStages - 1 : stage - 1;
+      const bool next = look(nb + kFewWarps);
+      if (nb < nblk) issue(nb, ns, seen);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      seen = next;
+    }
+    const uint32_t live = live_of[warp * kFewStages + stage];
+    const uint32_t K = ring + stage * kFewStageBytes<DP>, V = K + kFewKeys * DP * 2;
+    if (++stage == kFewStages) stage = 0;
+    if (!live) continue;
+    float s[MT][2][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[mt][i >> 2][i & 3] = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      uint32_t kf[4];
+      const int row = (lane >> 4) * 8 + (lane & 7), ch = 2 * ks + ((lane >> 3) & 1);
+      ldm4(kf, K + row * (DP * 2) + ((ch ^ (row & 7)) << 4));
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        mma16<T>(s[mt][0], qf[mt][ks], kf[0], kf[1]);
+        mma16<T>(s[mt][1], qf[mt][ks], kf[2], kf[3]);
+      }
+    }
+    uint32_t pf[MT][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {  // row g, then g + 8
+        float mx = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            float &x = s[mt][n][2 * h + u];
+            if (!((live >> (n * 8 + 2 * t + u)) & 1)) x = -INFINITY;
+            mx = fmaxf(mx, x);
+          }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        if (mx > m[mt][h]) {
+          const float f = ex2((m[mt][h] - mx) * sc);
+          m[mt][h] = mx;
+          l[mt][h] *= f;
+#pragma unroll
+          for (int n = 0; n < DP / 8; ++n) {
+            o[mt][n][2 * h] *= f;
+            o[mt][n][2 * h + 1] *= f;
+          }
+        }
+        const float base = m[mt][h] == -INFINITY ? 0.0f : m[mt][h] * sc;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const float p0 = ex2(fmaf(s[mt][n][2 * h], sc, -base)), p1 = ex2(fmaf(s[mt][n][2 * h + 1], sc, -base));
+          l[mt][h] += p0 + p1;
+          pf[mt][2 * n + h] = pack2<T>(p0, p1);
+        }
+      }
+#pragma unroll
+    for (int nb = 0; nb < KS; ++nb) {
+      uint32_t vf[4];
+      const int row = ((lane >> 3) & 1) * 8 + (lane & 7), ch = 2 * nb + (lane >> 4);
+      ldm4t(vf, V + row * (DP * 2) + ((ch ^ (row & 7)) << 4));
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        mma16<T>(o[mt][2 * nb], pf[mt], vf[0], vf[1]);
+        mma16<T>(o[mt][2 * nb + 1], pf[mt], vf[2], vf[3]);
+      }
     }
   }
-  T *out = (T *)c.out + qrow * c.o_row + (int64_t)h * c.o_head;
-  for (int i = 0; i < 4; ++i)
-    if (4 * lane + i < D) out[4 * lane + i] = (T)(l > 0.0f ? o[i] / l : (l == 0.0f ? 0.0f : l));
-  if (c.lse && lane == 0) c.lse[qrow * w.s.H + h] = l == 0.0f ? -INFINITY : m + logf(l);
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();  // the rings are free
+
+  // the four warps' results: sums [warp][row][DP], m and l [warp][row]
+  constexpr int R = 16 * MT;
+  float *so = reinterpret_cast<float *>(sm), *smm = so + kFewWarps * R * DP, *sl = smm + kFewWarps * R;
+  static_assert(kFewWarps * R * (DP + 2) * 4 <= kFewWarps * kFewStages * kFewStageBytes<DP>, "the rings hold the results");
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int i = mt * 16 + h * 8 + g;
+      float lr = l[mt][h];
+      lr += __shfl_xor_sync(0xffffffffu, lr, 1);
+      lr += __shfl_xor_sync(0xffffffffu, lr, 2);
+      if (t == 0) {
+        smm[warp * R + i] = m[mt][h] * sc;
+        sl[warp * R + i] = lr;
+      }
+#pragma unroll
+      for (int n = 0; n < DP / 8; ++n)
+        *reinterpret_cast<float2 *>(so + (warp * R + i) * DP + n * 8 + 2 * t) =
+            make_float2(o[mt][n][2 * h], o[mt][n][2 * h + 1]);
+    }
+  __syncthreads();
+  for (int u = threadIdx.x; u < it.rows * (DP / 2); u += kFewWarps * 32) {
+    const int i = u / (DP / 2), d = u % (DP / 2) * 2;
+    if (d >= D) continue;
+    float M = -INFINITY, L = 0.0f, x0 = 0.0f, x1 = 0.0f;
+#pragma unroll
+    for (int a = 0; a < kFewWarps; ++a) M = fmaxf(M, smm[a * R + i]);
+    const float base = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+    for (int a = 0; a < kFewWarps; ++a) {
+      const float f = ex2(smm[a * R + i] - base);
+      const float2 v = *reinterpret_cast<const float2 *>(so + (a * R + i) * DP + d);
+      L += f * sl[a * R + i];
+      x0 += f * v.x;
+      x1 += f * v.y;
+    }
+    if (it.nsplit > 1) {
+      float *p = partial(w, it, it.split, DP);
+      *reinterpret_cast<float2 *>(p + i * DP + d) = make_float2(x0, x1);
+      if (d == 0) {
+        p[it.rows * DP + i] = M;
+        p[it.rows * (DP + 1) + i] = L;
+      }
+      continue;
+    }
+    const int r = it.r0 + i, h = it.kvh * G + r % G;
+    const int64_t row = it.q0 + r / G;
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;  // no key: zeros
+    *reinterpret_cast<uint32_t *>((T *)c.out + row * c.o_row + (int64_t)h * c.o_head + d) = pack2<T>(x0 * inv, x1 * inv);
+    if (d == 0 && c.lse) c.lse[row * w.s.H + h] = L == 0.0f ? -INFINITY : fmaf(M, kLn2, logf(L));
+  }
+}
+
+// ── many rows ───────────────────────────────────────────────────────────────
+
+constexpr int kRows = 128, kKeys = 128, kTileThreads = 384;
+// Registers a thread, as the launch gives them and after setmaxnreg.
+constexpr int kRegLaunch = 168, kRegOther = 56, kRegSoftmax = 224;
+static_assert(128 * kRegOther + 256 * kRegSoftmax == kTileThreads * kRegLaunch, "the split adds up to the launch's");
+
+template <int DP>
+struct Tile {
+  static constexpr int kAtoms = DP / 64;                    // 64-dimension halves of a row (128 bytes each)
+  static constexpr int kAtom = kKeys * 128;                 // bytes of 128 rows of one half
+  static constexpr int kBytes = kAtoms * kAtom;             // a tile of Q, K or V
+  static constexpr int kStages = DP == 64 ? 4 : 2;          // K tiles, and V tiles, in flight
+  static constexpr int kQ = 0, kK = 2 * kBytes, kV = kK + kStages * kBytes, kBar = kV + kStages * kBytes;
+  static constexpr int kSmem = kBar + 256 + 1024;
+  // TMEM columns: S of both slots, their O; P beside them where there is room, else over S
+  static constexpr int kO = 256;
+  static constexpr bool kOwnP = DP == 64;
+  __host__ __device__ static constexpr int p_col(int x) { return kOwnP ? 384 + 64 * x : 128 * x; }
+};
+
+template <typename T>
+__host__ __device__ constexpr uint32_t f16_idesc(int n, bool b_mn) {
+  const uint32_t t = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  return (1u << 4) | (t << 7) | (t << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(kRows >> 4) << 24);
+}
+
+__device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, uint64_t *bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+          smem_u32(dst)),
+      "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld32_raw(uint32_t taddr, uint32_t *r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ float fmax3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// Which keys of tile j of an item are attended to: bit i of word i / 32
+// (the whole warp calls it).
+struct Live {
+  uint32_t w[4];
+};
+__device__ __forceinline__ Live live_keys(const uint8_t *mask, int klen, int j, int lane) {
+  Live v;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int i = j * kKeys + 32 * q + lane;
+    v.w[q] = __ballot_sync(0xffffffffu, i < klen && (!mask || mask[i] != 0));
+  }
+  return v;
+}
+
+// The 128 weights of a row: p = 2^(s c - m c), packed into P's TMEM columns, and
+// their sum.
+template <typename T>
+__device__ __forceinline__ float weights(const uint32_t *s, float c, float mc, uint32_t tP) {
+  const uint64_t cc = f2pack(c, c), nm = f2pack(-mc, -mc);
+  uint64_t sum = f2pack(0.0f, 0.0f);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    uint32_t w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int e = 32 * q + 2 * i;
+      float t0, t1;
+      f2unpack(ffma2(f2pack(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), cc, nm), t0, t1);
+      const float p0 = ex2(t0), p1 = ex2(t1);
+      sum = fadd2(sum, f2pack(p0, p1));
+      w[i] = pack2<T>(p0, p1);
+    }
+    tmem_st16(tP + 16 * q, w);
+  }
+  float a, b;
+  f2unpack(sum, a, b);
+  return a + b;
+}
+
+// Up to 256 rows (two slots of 128) of one request and KV head.  Warp 0
+// loads K and V tiles of 128 keys (TMA, a ring each), warp 1 issues the MMAs,
+// warp 2 zeroes the V rows of keys that are not attended to (their weights are
+// zero, but zero times NaN is not), and a warpgroup for each slot turns scores
+// into weights, a thread a row.  For slot x and tile j:
+//   S_x = Q_x K_j^T   M128 N128, both K-major in shared memory
+//   P_x = weights     TMEM, 16 bits
+//   O_x += P_x V_j    M128 N DP, P from TMEM, V MN-major
+// m moves only when a row's maximum passes it by 2^8, and O_x is rescaled
+// then: a weight is at most 256.  With D <= 64 P has TMEM columns of its own and
+// S_x(j+1) is issued as soon as the softmax has read S_x(j); with D > 64 P lies over S
+// and S_x(j+1) follows PV_x(j), while the other slot's softmax runs.
+template <typename T, int DP>
+__global__ void __launch_bounds__(kTileThreads, 1)
+    xattn_tile_kernel(const XAttnItem *items, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+                      XAttnWork w, XAttnCall c, int *err) {
+  using L = Tile<DP>;
+  constexpr int ST = L::kStages;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t *sm = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t *k_full = (uint64_t *)(sm + L::kBar), *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST;
+  uint64_t *v_ok = v_empty + ST, *q_full = v_ok + ST;
+  uint64_t *s_full = q_full + 1, *s_free = s_full + 2, *p_full = s_free + 2, *pv_done = p_full + 2;
+  uint32_t *tmem_slot = (uint32_t *)(pv_done + 2);
+  pdl_trigger();
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const XAttnItem it = items[blockIdx.x];
+  const int nt = (it.klen + kKeys - 1) / kKeys;
+  const bool two = it.rows > kRows;
+  const uint8_t *mask = c.mask ? c.mask + it.k0 : nullptr;
+  // keys of tile j that the MMAs cover: a multiple of 16
+  auto covered = [&](int j) { return min(kKeys, (it.klen - j * kKeys + 15) & ~15); };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_empty[s], 1);
+      mbar_init(&v_ok[s], 1);
+    }
+    mbar_init(q_full, 8);
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&s_full[x], 1);
+      mbar_init(&s_free[x], 4);
+      mbar_init(&p_full[x], 4);
+      mbar_init(&pv_done[x], 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const uint32_t tmem = *(volatile uint32_t *)tmem_slot;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegOther));
+    if (warp == 0) {
+      if (lane == 0) {
+        int k_done = 0, v_done = 0;
+        bool ok = true;
+        for (int j = 0; j < nt && ok; ++j) {
+          const int s = j % ST, row = (int)it.k0 + j * kKeys;
+          const uint32_t ph = (uint32_t)((j / ST) & 1) ^ 1;
+          if (!(ok = mbar_wait(&k_empty[s], ph, err))) break;
+          mbar_expect_tx(&k_full[s], L::kBytes);
+          for (int a = 0; a < L::kAtoms; ++a)
+            tma_load_3d(sm + L::kK + s * L::kBytes + a * L::kAtom, &mk, &k_full[s], 64 * a, it.kvh, row);
+          ++k_done;
+          if (!(ok = mbar_wait(&v_empty[s], ph, err))) break;
+          mbar_expect_tx(&v_full[s], L::kBytes);
+          for (int a = 0; a < L::kAtoms; ++a)
+            tma_load_3d(sm + L::kV + s * L::kBytes + a * L::kAtom, &mv, &v_full[s], 64 * a, it.kvh, row);
+          ++v_done;
+        }
+        // no copy may be in flight when the CTA leaves
+        for (int j = max(0, k_done - ST); j < k_done; ++j) mbar_drain(&k_full[j % ST], (uint32_t)((j / ST) & 1));
+        for (int j = max(0, v_done - ST); j < v_done; ++j) mbar_drain(&v_full[j % ST], (uint32_t)((j / ST) & 1));
+      }
+      __syncwarp();
+    } else if (warp == 1 && nt > 0) {
+      // descriptors share their high word; the low one is the address / 16
+      // (and, MN-major, the distance of the 64-dimension halves)
+      const uint32_t s16 = smem_u32(sm) >> 4;
+      const uint64_t hi = umma_desc(sm) & 0xFFFFFFFF00000000ull;
+      auto kmaj = [&](uint32_t a16) { return hi | (uint64_t)(a16 | (1u << 16)); };
+      auto mnmaj = [&](uint32_t a16) { return hi | (uint64_t)(a16 | ((uint32_t)(L::kAtom >> 4) << 16)); };
+      const int steps = (w.s.D + 15) / 16;
+      auto issue_s = [&](int x, int j) {
+        const int s = j % ST;
+        const uint32_t id = f16_idesc<T>(covered(j), false), d = tmem + 128u * x;
+        const uint32_t q = s16 + (uint32_t)((L::kQ + x * L::kBytes) >> 4), k = s16 + (uint32_t)((L::kK + s * L::kBytes) >> 4);
+#pragma unroll 1
+        for (int i = 0; i < steps; ++i) {
+          const uint32_t at = (uint32_t)((i >> 2) * (L::kAtom >> 4) + (i & 3) * 2);
+          umma_bf16_e(d, kmaj(q + at), kmaj(k + at), id, i ? 1u : 0u);
+        }
+        umma_commit_e(&s_full[x]);
+      };
+      auto issue_pv = [&](int x, int j) {
+        const int s = j % ST, n = covered(j) >> 4;
+        const uint32_t id = f16_idesc<T>(DP, true), d = tmem + (uint32_t)(L::kO + DP * x);
+        const uint32_t v = s16 + (uint32_t)((L::kV + s * L::kBytes) >> 4), p = tmem + (uint32_t)L::p_col(x);
+#pragma unroll 1
+        for (int i = 0; i < n; ++i) umma_bf16_ts_e(d, p + 8 * i, mnmaj(v + 128 * i), id, (j | i) ? 1u : 0u);
+        umma_commit_e(&pv_done[x]);
+      };
+      // S_x(j), once S_x(j-1) has been read and, where P lies over S, used
+      auto next_s = [&](int x, int j) -> bool {
+        if (j > 0) {
+          if (L::kOwnP ? !warp_wait(&s_free[x], (uint32_t)(j - 1) & 1, err) : !warp_wait(&pv_done[x], (uint32_t)(j - 1) & 1, err))
+            return false;
+        }
+        if (x == 0 && !warp_wait(&k_full[j % ST], (uint32_t)((j / ST) & 1), err)) return false;
+        tc_after();
+        issue_s(x, j);
+        if (x == (two ? 1 : 0)) umma_commit_e(&k_empty[j % ST]);
+        return true;
+      };
+      auto next_pv = [&](int x, int j) -> bool {
+        if (!warp_wait(&p_full[x], (uint32_t)j & 1, err)) return false;
+        if (x == 0 && (!warp_wait(&v_full[j % ST], (uint32_t)((j / ST) & 1), err) ||
+                       !warp_wait(&v_ok[j % ST], (uint32_t)((j / ST) & 1), err)))
+          return false;
+        tc_after();
+        issue_pv(x, j);
+        if (x == (two ? 1 : 0)) umma_commit_e(&v_empty[j % ST]);
+        return true;
+      };
+      bool ok = warp_wait(q_full, 0, err) && next_s(0, 0) && (!two || next_s(1, 0));
+      for (int j = 0; j < nt && ok; ++j) {
+        const bool more = j + 1 < nt;
+        if (L::kOwnP) {
+          ok = (!more || next_s(0, j + 1)) && (!more || !two || next_s(1, j + 1)) && next_pv(0, j) &&
+               (!two || next_pv(1, j));
+        } else {
+          ok = next_pv(0, j) && (!more || next_s(0, j + 1)) && (!two || next_pv(1, j)) &&
+               (!more || !two || next_s(1, j + 1));
+        }
+      }
+    } else if (warp == 2) {
+      for (int j = 0; j < nt; ++j) {
+        const int s = j % ST;
+        const bool whole = !mask && (j + 1) * kKeys <= it.klen;
+        Live live{};
+        if (!whole) live = live_keys(mask, it.klen, j, lane);
+        if (!warp_wait(&v_full[s], (uint32_t)((j / ST) & 1), err)) break;
+        if (!whole) {
+          const int n = covered(j);
+          // 8 lanes a row and half, 4 rows at a time
+          for (int r0 = 0; r0 < n; r0 += 4) {
+            const int r = r0 + (lane >> 3);
+            if ((live.w[r >> 5] >> (r & 31)) & 1) continue;
+#pragma unroll
+            for (int a = 0; a < L::kAtoms; ++a)
+              *reinterpret_cast<uint4 *>(sm + L::kV + s * L::kBytes + a * L::kAtom + r * 128 + (lane & 7) * 16) =
+                  make_uint4(0, 0, 0, 0);
+          }
+          fence_async_smem();
+          __syncwarp();
+        }
+        if (lane == 0) mbar_arrive(&v_ok[s]);
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegSoftmax));
+    const int quarter = warp & 3, x = (warp - 4) >> 2;
+    const int i = x * kRows + quarter * 32 + lane, r = it.r0 + i;  // this thread's row
+    const int G = w.s.H / w.s.KVH, D = w.s.D;
+    const int h = it.kvh * G + r % G;
+    const int64_t row = it.q0 + r / G;
+    const bool mine = i < it.rows, slot = x == 0 || two;
+    if (slot) {  // the row of Q, K-major with the 128-byte swizzle
+      const T *q = (const T *)c.q + row * c.q_row + (int64_t)h * c.q_head;
+      uint8_t *dst = sm + L::kQ + x * L::kBytes + (quarter * 32 + lane) * 128;
+#pragma unroll
+      for (int ch = 0; ch < DP / 8; ++ch) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (mine && ch * 8 < D) v = *reinterpret_cast<const uint4 *>(q + ch * 8);
+        *reinterpret_cast<uint4 *>(dst + (ch >> 3) * L::kAtom + (((ch & 7) ^ (lane & 7)) << 4)) = v;
+      }
+      fence_async_smem();
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(q_full);
+    if (slot) {
+      const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+      const uint32_t tS = tmem + lanes + 128u * x, tP = tmem + lanes + (uint32_t)L::p_col(x);
+      const uint32_t tO = tmem + lanes + (uint32_t)(L::kO + DP * x);
+      const float sc = c.scale * kLog2e;
+      float m = -INFINITY, l = 0.0f;
+      bool ok = true;
+      for (int j = 0; j < nt; ++j) {
+        const bool whole = !mask && (j + 1) * kKeys <= it.klen;
+        Live live{};
+        if (!whole) live = live_keys(mask, it.klen, j, lane);
+        if (!(ok = warp_wait(&s_full[x], (uint32_t)j & 1, err))) break;
+        tc_after();
+        uint32_t s[128];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) tmem_ld32_raw(tS + 32 * q, s + 32 * q);
+        tmem_wait_ld();
+        if (L::kOwnP) {
+          tc_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_free[x]);
+        }
+        if (!whole) {
+#pragma unroll
+          for (int e = 0; e < 128; ++e)
+            if (!((live.w[e >> 5] >> (e & 31)) & 1)) s[e] = 0xff800000u;
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < 128; e += 2)
+          mx[(e >> 1) & 3] = fmax3(mx[(e >> 1) & 3], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        const bool move = (top - m) * sc > 8.0f;  // also at the first attended key (m = -inf)
+        float f = 1.0f;
+        if (move) {
+          f = ex2((m - top) * sc);
+          m = top;
+          l *= f;
+        }
+        // P_x and O_x are free once PV_x(j-1) is done
+        if (j > 0 && !(ok = warp_wait(&pv_done[x], (uint32_t)(j - 1) & 1, err))) break;
+        tc_after();
+        if (j > 0 && __any_sync(0xffffffffu, move)) {
+#pragma unroll 1
+          for (int q = 0; q < DP / 16; ++q) {
+            uint32_t o[16];
+            asm volatile(
+                "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+                "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]), "=r"(o[4]), "=r"(o[5]), "=r"(o[6]), "=r"(o[7]),
+                  "=r"(o[8]), "=r"(o[9]), "=r"(o[10]), "=r"(o[11]), "=r"(o[12]), "=r"(o[13]), "=r"(o[14]), "=r"(o[15])
+                : "r"(tO + 16 * q));
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tmem_st16(tO + 16 * q, o);
+          }
+        }
+        l += weights<T>(s, sc, m == -INFINITY ? 0.0f : m * sc, tP);
+        tmem_wait_st();
+        tc_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[x]);
+      }
+      if (ok && nt > 0) ok = warp_wait(&pv_done[x], (uint32_t)(nt - 1) & 1, err);
+      if (ok) {
+        tc_after();
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
+        T *out = (T *)c.out + row * c.o_row + (int64_t)h * c.o_head;
+        float *p = partial(w, it, it.split, DP);
+#pragma unroll
+        for (int q = 0; q < DP / 32; ++q) {
+          uint32_t o[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0;
+          if (nt > 0) {
+            tmem_ld32_raw(tO + 32 * q, o);
+            tmem_wait_ld();
+          }
+          if (!mine) continue;
+          if (it.nsplit > 1) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<uint4 *>(p + (int64_t)i * DP + 32 * q + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              if (32 * q + e >= D) break;
+              uint32_t u[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                u[k] = pack2<T>(__uint_as_float(o[e + 2 * k]) * inv, __uint_as_float(o[e + 2 * k + 1]) * inv);
+              *reinterpret_cast<uint4 *>(out + 32 * q + e) = make_uint4(u[0], u[1], u[2], u[3]);
+            }
+          }
+        }
+        if (mine) {
+          if (it.nsplit > 1) {
+            p[it.rows * DP + i] = m * sc;
+            p[it.rows * (DP + 1) + i] = l;
+          } else if (c.lse) {
+            c.lse[row * w.s.H + h] = l == 0.0f ? -INFINITY : fmaf(m * sc, kLn2, logf(l));
+          }
+        }
+      }
+    }
+  }
+  __syncwarp();
+  tc_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  }
+}
+
+// ── joining split ranges ────────────────────────────────────────────────────
+
+// A warp for each row of a group (blockIdx.x) of items on the same rows:
+// out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s, in the order of the splits.
+template <typename T>
+__global__ void xattn_join_kernel(const XAttnItem *groups, XAttnWork w, XAttnCall c, int DP) {
+  pdl_wait();
+  const XAttnItem it = groups[blockIdx.x];
+  const int lane = threadIdx.x & 31, i = blockIdx.y * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (i >= it.rows) return;
+  const int G = w.s.H / w.s.KVH, D = w.s.D, r = it.r0 + i, h = it.kvh * G + r % G;
+  const int64_t row = it.q0 + r / G, stride = (int64_t)it.rows * (DP + 4);
+  const float *p = partial(w, it, 0, DP), *pm = p + it.rows * DP + i, *pl = pm + it.rows;
+  float M = -INFINITY;
+  for (int s = lane; s < it.nsplit; s += 32) M = fmaxf(M, pm[s * stride]);
+  M = warp_max(M);
+  const float base = M == -INFINITY ? 0.0f : M;
+  float L = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  const bool own = 4 * lane < D;
+  for (int s = 0; s < it.nsplit; ++s) {
+    const float f = ex2(pm[s * stride] - base);
+    L += f * pl[s * stride];
+    if (own) {
+      const float4 v = *reinterpret_cast<const float4 *>(p + s * stride + (int64_t)i * DP + 4 * lane);
+      o[0] += f * v.x;
+      o[1] += f * v.y;
+      o[2] += f * v.z;
+      o[3] += f * v.w;
+    }
+  }
+  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+  if (own)
+    *reinterpret_cast<uint2 *>((T *)c.out + row * c.o_row + (int64_t)h * c.o_head + 4 * lane) =
+        make_uint2(pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv));
+  if (lane == 0 && c.lse) c.lse[row * w.s.H + h] = L == 0.0f ? -INFINITY : fmaf(M, kLn2, logf(L));
+}
+
+// ── launches ────────────────────────────────────────────────────────────────
+
+template <typename T, int DP, int MT>
+cudaError_t launch_few(const XAttnItem *items, int n, const XAttnWork &w, const XAttnCall &c, cudaStream_t st) {
+  if (n == 0) return cudaSuccess;
+  auto *kernel = xattn_few_kernel<T, DP, MT>;
+  static thread_local int ready = -1;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && ready != dev) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem<DP>);
+    if (e == cudaSuccess) ready = dev;
+  }
+  if (e != cudaSuccess) return e;
+  kernel<<<n, kFewWarps * 32, kFewSmem<DP>, st>>>(items, w, c);
+  return cudaGetLastError();
+}
+
+cudaError_t kv_map(CUtensorMap *map, const void *p, const XAttnShape &s, int64_t row, int64_t head) {
+  const uint64_t dims[3] = {(uint64_t)s.D, (uint64_t)s.KVH, (uint64_t)s.k_rows};
+  const uint64_t strides[2] = {(uint64_t)head * 2, (uint64_t)row * 2};
+  const uint32_t box[3] = {64, 1, kKeys};
+  return tma_map_tiled(map, s.dtype == DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, p,
+                       dims, strides, box);
+}
+
+template <typename T, int DP>
+cudaError_t launch_tile(const XAttnItem *items, int n, const XAttnWork &w, const XAttnCall &c, int *err, cudaStream_t st) {
+  if (n == 0) return cudaSuccess;
+  auto *kernel = xattn_tile_kernel<T, DP>;
+  static thread_local int ready = -1;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && ready != dev) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<DP>::kSmem);
+    if (e == cudaSuccess) ready = dev;
+  }
+  CUtensorMap mk, mv;
+  XAttnShape s = w.s;
+  s.k_rows = std::max<int64_t>(s.k_rows, 1);  // no keys at all: nothing is loaded
+  if (e == cudaSuccess) e = kv_map(&mk, c.k, s, c.k_row, c.k_head);
+  if (e == cudaSuccess) e = kv_map(&mv, c.v, s, c.v_row, c.v_head);
+  if (e != cudaSuccess) return e;
+  kernel<<<n, kTileThreads, Tile<DP>::kSmem, st>>>(items, mk, mv, w, c, err);
+  return cudaGetLastError();
+}
+
+template <typename T, int DP>
+cudaError_t run(const XAttnWork &w, const XAttnCall &c, int *err, cudaStream_t st) {
+  const XAttnItem *i16 = w.items, *i32 = i16 + w.n16, *it = i32 + w.n32, *groups = it + w.n_tile;
+  cudaError_t e = launch_tile<T, DP>(it, w.n_tile, w, c, err, st);
+  if (e == cudaSuccess) e = launch_few<T, DP, 1>(i16, w.n16, w, c, st);
+  if (e == cudaSuccess) e = launch_few<T, DP, 2>(i32, w.n32, w, c, st);
+  if (e != cudaSuccess || w.n_groups == 0) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)w.n_groups, (unsigned)((w.group_rows + 7) / 8));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, xattn_join_kernel<T>, groups, w, c, DP);
+}
+
+// Keys of an item (a multiple of `unit`) for ranges of `keys` each, run by
+// `slots` CTAs at a time: the length with the least estimated finish.  An item costs
+// its units and `fixed` more; with no more items than slots the longest
+// decides, else the sum over the slots and half an item of imbalance.  Splitting
+// costs the join.
+int64_t choose_chunk(const std::vector<int64_t> &keys, int unit, double fixed, double join, int slots) {
+  int64_t longest = 1, total = 0;
+  std::vector<int64_t> units;
+  for (int64_t k : keys) {
+    units.push_back(std::max<int64_t>(1, (k + unit - 1) / unit));
+    longest = std::max(longest, units.back());
+    total += units.back();
+  }
+  double best = 1e300;
+  int64_t chunk = longest;
+  for (int64_t c = longest;; c = std::min(c - 1, c * 9 / 10)) {
+    if (c < 2 && c != longest) break;
+    int64_t n = 0;
+    for (int64_t u : units) n += (u + c - 1) / c;
+    double t = (double)c + fixed;
+    if (n > slots) t = std::max(t, (total + n * fixed) / slots + t / 2);
+    if (c < longest) t += join;
+    if (t < best) best = t, chunk = c;
+    if (c <= 1 || n > 8 * (int64_t)slots + (int64_t)units.size()) break;
+  }
+  return chunk * unit;
 }
 
 }  // namespace
 
-std::vector<XAttnItem> cross_attn_split(const XAttnShape &s, const uint64_t *q_start, const uint64_t *q_len,
-                                        const uint64_t *k_start, const uint64_t *k_len, size_t n_seq, int sms) {
-  std::vector<XAttnItem> items;
+XAttnSplit cross_attn_split(const XAttnShape &s, const uint64_t *q_start, const uint64_t *q_len, const uint64_t *k_start,
+                            const uint64_t *k_len, size_t n_seq, int sms) {
+  const int G = s.H / s.KVH, DP = s.D <= 64 ? 64 : 128;
+  std::vector<XAttnItem> whole[3];  // up to 16 rows, up to 32, tiles
   for (size_t i = 0; i < n_seq; ++i) {
-    const int64_t rows = (int64_t)q_len[i] * (s.H / s.KVH);
-    for (int g = 0; g < s.KVH; ++g)
-      for (int64_t r0 = 0; r0 < rows; r0 += kRows)
-        items.push_back(XAttnItem{(int64_t)q_start[i], (int64_t)k_start[i], (int)k_len[i], (int)r0,
-                                  (int)std::min<int64_t>(kRows, rows - r0), g, 0, 1, 0, 0});
+    const int64_t rows = (int64_t)q_len[i] * G;
+    const int kind = rows <= 16 ? 0 : rows <= 32 ? 1 : 2, step = kind == 2 ? 2 * kRows : 32;
+    for (int64_t r0 = 0; r0 < rows; r0 += step)
+      for (int g = 0; g < s.KVH; ++g) {
+        XAttnItem it{};
+        it.q0 = (int64_t)q_start[i];
+        it.k0 = (int64_t)k_start[i];
+        it.klen = (int)k_len[i];
+        it.r0 = (int)r0;
+        it.rows = (int)std::min<int64_t>(step, rows - r0);
+        it.kvh = g;
+        it.nsplit = 1;
+        whole[kind].push_back(it);
+      }
   }
-  return items;
+  XAttnSplit out;
+  std::vector<XAttnItem> groups;
+  for (int kind = 0; kind < 3; ++kind) {
+    std::vector<int64_t> keys;
+    for (const XAttnItem &it : whole[kind]) keys.push_back(it.klen);
+    std::vector<XAttnItem> items;
+    if (!keys.empty()) {
+      // few rows: a unit is 64 keys (16 a warp); a CTA's start and end cost
+      // about as much as 8 of them, a join as 8.  Tiles: units of 128 keys, 2 each.
+      const int occ = DP == 64 ? 4 : 2;
+      const int64_t chunk = kind < 2 ? choose_chunk(keys, 64, 8.0, 8.0, sms * occ) : choose_chunk(keys, kKeys, 2.0, 3.0, sms);
+      for (XAttnItem it : whole[kind]) {
+        const int klen = it.klen, unit = kind < 2 ? 64 : kKeys;
+        it.nsplit = (int)std::max<int64_t>(1, (klen + chunk - 1) / chunk);
+        if (it.nsplit > 1) {
+          it.ws = out.ws_floats;
+          out.ws_floats += (int64_t)it.nsplit * it.rows * (DP + 4);
+          groups.push_back(it);
+          out.group_rows = std::max(out.group_rows, it.rows);
+        }
+        const int64_t units = (klen + unit - 1) / unit, k0 = it.k0;
+        for (int q = 0; q < it.nsplit; ++q) {
+          const int64_t a = units * q / it.nsplit * unit, b = std::min<int64_t>(units * (q + 1) / it.nsplit * unit, klen);
+          it.split = q;
+          it.k0 = k0 + a;
+          it.klen = (int)(b - a);
+          items.push_back(it);
+        }
+      }
+      // the longest first
+      std::stable_sort(items.begin(), items.end(), [](const XAttnItem &a, const XAttnItem &b) {
+        return (int64_t)a.klen * (a.rows > kRows ? 2 : 1) > (int64_t)b.klen * (b.rows > kRows ? 2 : 1);
+      });
+    }
+    (kind == 0 ? out.n16 : kind == 1 ? out.n32 : out.n_tile) = (int64_t)items.size();
+    out.items.insert(out.items.end(), items.begin(), items.end());
+  }
+  out.n_groups = (int64_t)groups.size();
+  out.items.insert(out.items.end(), groups.begin(), groups.end());
+  return out;
 }
 
 cudaError_t cross_attn(const XAttnWork &w, const XAttnCall &c, int *err, cudaStream_t st) {
-  if (w.n_items == 0) return cudaSuccess;
-  if (w.s.dtype == DT_F16)
-    cross_attn_rows_kernel<__half><<<w.n_items, 32 * kRows, 0, st>>>(w, c);
-  else
-    cross_attn_rows_kernel<__nv_bfloat16><<<w.n_items, 32 * kRows, 0, st>>>(w, c);
-  return cudaGetLastError();
+  if (w.s.dtype == DT_F16) return w.s.D <= 64 ? run<__half, 64>(w, c, err, st) : run<__half, 128>(w, c, err, st);
+  return w.s.D <= 64 ? run<__nv_bfloat16, 64>(w, c, err, st) : run<__nv_bfloat16, 128>(w, c, err, st);
 }
 
 }  // namespace ndl

@@ -348,15 +348,21 @@ NeedleCrossAttnPlan *needle_cross_attn_plan_create(const uint64_t *q_start, cons
         !ok(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, plan->device)))
       return false;
     plan->work.s = XAttnShape{(int)H, (int)KVH, (int)D, dtype, k_rows};
-    const std::vector<XAttnItem> items = cross_attn_split(plan->work.s, q_start, q_len, k_start, k_len, n_seq, sms);
-    if (items.size() > kMaxRows) return fail("cross attention: too many rows for one plan");
-    const size_t ib = (items.size() * sizeof(XAttnItem) + 255) / 256 * 256;
-    if (!ok(cudaMalloc(&plan->buf, ib + 256))) return false;
+    const XAttnSplit split = cross_attn_split(plan->work.s, q_start, q_len, k_start, k_len, n_seq, sms);
+    if (split.items.size() > kMaxRows) return fail("cross attention: too many rows for one plan");
+    const size_t ib = (split.items.size() * sizeof(XAttnItem) + 255) / 256 * 256;
+    if (!ok(cudaMalloc(&plan->buf, ib + (size_t)split.ws_floats * sizeof(float) + 256))) return false;
     plan->flag = (int *)((char *)plan->buf + ib);
     plan->work.items = (const XAttnItem *)plan->buf;
-    plan->work.n_items = (int)items.size();
+    plan->work.ws = (float *)((char *)plan->flag + 256);
+    plan->work.n16 = (int)split.n16;
+    plan->work.n32 = (int)split.n32;
+    plan->work.n_tile = (int)split.n_tile;
+    plan->work.n_groups = (int)split.n_groups;
+    plan->work.group_rows = split.group_rows;
     cudaStream_t st = (cudaStream_t)stream;
-    return ok(cudaMemcpyAsync(plan->buf, items.data(), items.size() * sizeof(XAttnItem), cudaMemcpyHostToDevice, st)) &&
+    return (split.items.empty() || ok(cudaMemcpyAsync(plan->buf, split.items.data(), split.items.size() * sizeof(XAttnItem),
+                                                      cudaMemcpyHostToDevice, st))) &&
            ok(cudaMemsetAsync(plan->flag, 0, 256, st)) && ok(cudaStreamSynchronize(st));
   });
   if (good) return plan;

@@ -62,17 +62,14 @@ cudaError_t residual_norm(const ResidualNormArgs &a, cudaStream_t st);
 
 // ── cross attention ──
 // One unit of work: `rows` packed query rows of one request and KV head
-// against keys [k0, k0 + klen).  A packed row r0 + i is query token (r0 + i) /
-// G, head kvh * G + (r0 + i) % G of the request, G = H / KVH.
+// against keys [k0, k0 + klen).  Packed row r is query token r / G, head
+// kvh * G + r % G of the request, G = H / KVH; the item's are r0 ..
 struct XAttnItem {
-  int64_t q0;   // first query row of the request
-  int64_t k0;   // first key row
-  int klen;     // keys of this item
-  int r0, rows; // packed rows
-  int kvh;
-  int split, nsplit;  // this item's place among the items of the same rows
-  int ws;             // first partial of those items in the workspace (nsplit > 1)
-  int group;          // counter of those items
+  int64_t q0;         // first query row of the request
+  int64_t k0;         // first key row
+  int64_t ws;         // workspace (floats) of the items on these rows, when there are several
+  int klen, r0, rows, kvh;
+  int split, nsplit;  // this item among those on the same rows
 };
 struct XAttnShape {
   int H, KVH, D, dtype;
@@ -86,14 +83,23 @@ struct XAttnCall {
   int64_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head;
   float scale;
 };
-// The items of a plan on the device, and what they need.
+// A plan's work (host): items of up to 16 rows, up to 32 and up to 256, then
+// one entry for each group of items that share rows, to be joined.
+struct XAttnSplit {
+  std::vector<XAttnItem> items;
+  int64_t n16 = 0, n32 = 0, n_tile = 0, n_groups = 0;
+  int64_t ws_floats = 0;
+  int group_rows = 0;  // most rows of a group
+};
+XAttnSplit cross_attn_split(const XAttnShape &s, const uint64_t *q_start, const uint64_t *q_len, const uint64_t *k_start,
+                            const uint64_t *k_len, size_t n_seq, int sms);
+// The same on the device, with its workspace.
 struct XAttnWork {
   XAttnShape s;
   const XAttnItem *items = nullptr;
-  int n_items = 0;
+  float *ws = nullptr;
+  int n16 = 0, n32 = 0, n_tile = 0, n_groups = 0, group_rows = 0;
 };
-std::vector<XAttnItem> cross_attn_split(const XAttnShape &s, const uint64_t *q_start, const uint64_t *q_len,
-                                        const uint64_t *k_start, const uint64_t *k_len, size_t n_seq, int sms);
 cudaError_t cross_attn(const XAttnWork &w, const XAttnCall &c, int *err, cudaStream_t st);
 
 }  // namespace ndl
