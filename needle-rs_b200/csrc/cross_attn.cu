@@ -64,6 +64,8 @@ __device__ __forceinline__ float *partial(const XAttnWork &w, const XAttnItem &i
 // ── few rows ────────────────────────────────────────────────────────────────
 
 constexpr int kFewWarps = 4, kFewKeys = 16, kFewStages = 3;
+// Rows of an item, and of a request and KV head that this kernel takes.
+constexpr int kFewRows = 32, kFewMaxRows = 64;
 
 template <int DP>
 constexpr int kFewStageBytes = 2 * kFewKeys * DP * 2;  // K and V rows of 16 keys
@@ -120,39 +122,56 @@ __global__ void __launch_bounds__(kFewWarps * 32) xattn_few_kernel(const XAttnIt
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int G = w.s.H / w.s.KVH, D = w.s.D;
   const int nblk = (it.klen + kFewKeys - 1) / kFewKeys;
-  const T *kb = (const T *)c.k + it.k0 * c.k_row + (int64_t)it.kvh * c.k_head;
-  const T *vb = (const T *)c.v + it.k0 * c.v_row + (int64_t)it.kvh * c.v_head;
   const uint8_t *mask = c.mask ? c.mask + it.k0 : nullptr;
   const uint32_t ring = smem_u32(sm) + warp * kFewStages * kFewStageBytes<DP>;
+  // this lane's 16-byte chunk of the first rows of the warp's next block: the
+  // other rows follow RS rows apart, the next block 64 rows on
+  constexpr int RS = 32 / CH;
+  const int ch0 = lane % CH, row0 = lane / CH;
+  const T *kp = (const T *)c.k + (it.k0 + warp * kFewKeys + row0) * c.k_row + (int64_t)it.kvh * c.k_head + ch0 * 8;
+  const T *vp = (const T *)c.v + (it.k0 + warp * kFewKeys + row0) * c.v_row + (int64_t)it.kvh * c.v_head + ch0 * 8;
+  const int64_t k_step = RS * c.k_row, v_step = RS * c.v_row;
+  const bool have = ch0 * 8 < D;
 
-  // lane j < 16: whether key j of block b is attended to
-  auto look = [&](int b) -> bool {
-    const int j = b * kFewKeys + lane;
-    return lane < kFewKeys && j < it.klen && (!mask || mask[j] != 0);
+  // The 16 attended bits of the warp's n-th block, from a window of 32 blocks
+  // (lane i holds block i's): the mask's bytes are fetched for 32 blocks at once, all
+  // loads in flight together.
+  uint32_t window = 0;
+  auto live_block = [&](int n) -> uint32_t {
+    if ((n & 31) == 0) {
+      const int j = ((n + lane) * kFewWarps + warp) * kFewKeys, left = min(max(it.klen - j, 0), kFewKeys);
+      window = (1u << left) - 1;
+      if (mask) {
+        uint32_t seen = 0;
+#pragma unroll
+        for (int i = 0; i < kFewKeys; ++i)
+          if (i < left) seen |= (mask[j + i] != 0 ? 1u : 0u) << i;
+        window = seen;
+      }
+    }
+    return __shfl_sync(0xffffffffu, window, n & 31);
   };
-  auto issue = [&](int b, int stage, bool seen) {
-    const uint32_t live = __ballot_sync(0xffffffffu, seen);
+  auto issue = [&](int n, int stage) {  // the warp's n-th block, in order
+    const uint32_t live = live_block(n);
     if (lane == 0) live_of[warp * kFewStages + stage] = live;
     const uint32_t dst = ring + stage * kFewStageBytes<DP>;
 #pragma unroll
     for (int i = 0; i < CH / 2; ++i) {
-      const int id = lane + 32 * i, row = id / CH, ch = id % CH;
-      const bool take = ((live >> row) & 1) && ch * 8 < D;
-      const int64_t key = b * kFewKeys + row;
-      const uint32_t at = dst + row * (DP * 2) + ((ch ^ (row & 7)) << 4);
-      cp16(at, take ? kb + key * c.k_row + ch * 8 : kb, take);
-      cp16(at + kFewKeys * DP * 2, take ? vb + key * c.v_row + ch * 8 : vb, take);
+      const int row = row0 + RS * i;
+      const bool take = ((live >> row) & 1) && have;
+      const uint32_t at = dst + row * (DP * 2) + ((ch0 ^ (row & 7)) << 4);
+      cp16(at, take ? kp + i * k_step : (const T *)c.k, take);
+      cp16(at + kFewKeys * DP * 2, take ? vp + i * v_step : (const T *)c.v, take);
     }
+    kp += kFewWarps * kFewKeys * c.k_row;
+    vp += kFewWarps * kFewKeys * c.v_row;
   };
+  const int mine = (nblk - warp + kFewWarps - 1) / kFewWarps;  // blocks of this warp
 
-  bool seen = look(warp);
 #pragma unroll
-  for (int s = 0; s < kFewStages - 1; ++s) {
-    const int b = warp + s * kFewWarps;
-    const bool next = look(b + kFewWarps);
-    if (b < nblk) issue(b, s, seen);
+  for (int n = 0; n < kFewStages - 1; ++n) {
+    if (n < mine) issue(n, n);
     asm volatile("cp.async.commit_group;" ::: "memory");
-    seen = next;
   }
 
   // Q as MMA fragments (rows g and g + 8 of each 16)
@@ -185,16 +204,11 @@ __global__ void __launch_bounds__(kFewWarps * 32) xattn_few_kernel(const XAttnIt
   }
 
   int stage = 0;
-  for (int b = warp; b < nblk; b += kFewWarps) {
+  for (int n = 0; n < mine; ++n) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kFewStages - 2) : "memory");
     __syncwarp();  // every lane's copies of this stage, and the reads of the stage refilled next
-    {
-      const int nb = b + (kFewStages - 1) * kFewWarps, ns = stage == 0 ? kFewStages - 1 : stage - 1;
-      const bool next = look(nb + kFewWarps);
-      if (nb < nblk) issue(nb, ns, seen);
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      seen = next;
-    }
+    if (n + kFewStages - 1 < mine) issue(n + kFewStages - 1, stage == 0 ? kFewStages - 1 : stage - 1);
+    asm volatile("cp.async.commit_group;" ::: "memory");
     const uint32_t live = live_of[warp * kFewStages + stage];
     const uint32_t K = ring + stage * kFewStageBytes<DP>, V = K + kFewKeys * DP * 2;
     if (++stage == kFewStages) stage = 0;
@@ -276,6 +290,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) xattn_few_kernel(const XAttnIt
       float lr = l[mt][h];
       lr += __shfl_xor_sync(0xffffffffu, lr, 1);
       lr += __shfl_xor_sync(0xffffffffu, lr, 2);
+      if (i >= it.rows) continue;
       if (t == 0) {
         smm[warp * R + i] = m[mt][h] * sc;
         sl[warp * R + i] = lr;
@@ -398,29 +413,28 @@ __device__ __forceinline__ Live live_keys(const uint8_t *mask, int klen, int j, 
   return v;
 }
 
-// The 128 weights of a row: p = 2^(s c - m c), packed into P's TMEM columns, and
-// their sum.
+// 32 weights of a row: p = 2^(s c - m c), rounded and packed into w, their sum
+// added to `sum`.
 template <typename T>
-__device__ __forceinline__ float weights(const uint32_t *s, float c, float mc, uint32_t tP) {
-  const uint64_t cc = f2pack(c, c), nm = f2pack(-mc, -mc);
-  uint64_t sum = f2pack(0.0f, 0.0f);
+__device__ __forceinline__ void weights(const uint32_t *s, uint64_t cc, uint64_t nm, uint32_t *w, uint64_t &sum) {
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    uint32_t w[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int e = 32 * q + 2 * i;
-      float t0, t1;
-      f2unpack(ffma2(f2pack(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), cc, nm), t0, t1);
-      const float p0 = ex2(t0), p1 = ex2(t1);
-      sum = fadd2(sum, f2pack(p0, p1));
-      w[i] = pack2<T>(p0, p1);
-    }
-    tmem_st16(tP + 16 * q, w);
+  for (int i = 0; i < 16; ++i) {
+    float t0, t1;
+    f2unpack(ffma2(f2pack(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), cc, nm), t0, t1);
+    const float p0 = ex2(t0), p1 = ex2(t1);
+    sum = fadd2(sum, f2pack(p0, p1));
+    w[i] = pack2<T>(p0, p1);
   }
-  float a, b;
-  f2unpack(sum, a, b);
-  return a + b;
+}
+
+// Bounded wait of a converged warp through one lane: 32 lanes polling one
+// barrier take about 200 clocks even when its phase is complete.
+__device__ __forceinline__ bool one_wait(uint64_t *b, uint32_t parity, int *err, int lane) {
+  bool ok = true;
+  if (lane == 0) ok = mbar_wait(b, parity, err);
+  ok = __all_sync(0xffffffffu, ok);
+  __syncwarp();  // orders what lane 0 has seen before the other lanes' reads
+  return ok;
 }
 
 // Up to 256 rows (two slots of 128) of one request and KV head.  Warp 0
@@ -538,26 +552,26 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       // S_x(j), once S_x(j-1) has been read and, where P lies over S, used
       auto next_s = [&](int x, int j) -> bool {
         if (j > 0) {
-          if (L::kOwnP ? !warp_wait(&s_free[x], (uint32_t)(j - 1) & 1, err) : !warp_wait(&pv_done[x], (uint32_t)(j - 1) & 1, err))
+          if (L::kOwnP ? !one_wait(&s_free[x], (uint32_t)(j - 1) & 1, err, lane) : !one_wait(&pv_done[x], (uint32_t)(j - 1) & 1, err, lane))
             return false;
         }
-        if (x == 0 && !warp_wait(&k_full[j % ST], (uint32_t)((j / ST) & 1), err)) return false;
+        if (x == 0 && !one_wait(&k_full[j % ST], (uint32_t)((j / ST) & 1), err, lane)) return false;
         tc_after();
         issue_s(x, j);
         if (x == (two ? 1 : 0)) umma_commit_e(&k_empty[j % ST]);
         return true;
       };
       auto next_pv = [&](int x, int j) -> bool {
-        if (!warp_wait(&p_full[x], (uint32_t)j & 1, err)) return false;
-        if (x == 0 && (!warp_wait(&v_full[j % ST], (uint32_t)((j / ST) & 1), err) ||
-                       !warp_wait(&v_ok[j % ST], (uint32_t)((j / ST) & 1), err)))
+        if (!one_wait(&p_full[x], (uint32_t)j & 1, err, lane)) return false;
+        if (x == 0 && (!one_wait(&v_full[j % ST], (uint32_t)((j / ST) & 1), err, lane) ||
+                       !one_wait(&v_ok[j % ST], (uint32_t)((j / ST) & 1), err, lane)))
           return false;
         tc_after();
         issue_pv(x, j);
         if (x == (two ? 1 : 0)) umma_commit_e(&v_empty[j % ST]);
         return true;
       };
-      bool ok = warp_wait(q_full, 0, err) && next_s(0, 0) && (!two || next_s(1, 0));
+      bool ok = one_wait(q_full, 0, err, lane) && next_s(0, 0) && (!two || next_s(1, 0));
       for (int j = 0; j < nt && ok; ++j) {
         const bool more = j + 1 < nt;
         if (L::kOwnP) {
@@ -574,7 +588,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const bool whole = !mask && (j + 1) * kKeys <= it.klen;
         Live live{};
         if (!whole) live = live_keys(mask, it.klen, j, lane);
-        if (!warp_wait(&v_full[s], (uint32_t)((j / ST) & 1), err)) break;
+        if (!one_wait(&v_full[s], (uint32_t)((j / ST) & 1), err, lane)) break;
         if (!whole) {
           const int n = covered(j);
           // 8 lanes a row and half, 4 rows at a time
@@ -624,26 +638,33 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const bool whole = !mask && (j + 1) * kKeys <= it.klen;
         Live live{};
         if (!whole) live = live_keys(mask, it.klen, j, lane);
-        if (!(ok = warp_wait(&s_full[x], (uint32_t)j & 1, err))) break;
+        if (!(ok = one_wait(&s_full[x], (uint32_t)j & 1, err, lane))) break;
         tc_after();
         uint32_t s[128];
+        tmem_ld32_raw(tS, s);
+        tmem_ld32_raw(tS + 32, s + 32);
+        tmem_wait_ld();
+        tmem_ld32_raw(tS + 64, s + 64);
+        tmem_ld32_raw(tS + 96, s + 96);
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        auto row_max = [&](int e0) {
+          if (!whole) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) tmem_ld32_raw(tS + 32 * q, s + 32 * q);
+            for (int e = 0; e < 64; ++e)
+              if (!((live.w[(e0 + e) >> 5] >> (e & 31)) & 1)) s[e0 + e] = 0xff800000u;
+          }
+#pragma unroll
+          for (int e = 0; e < 64; e += 2)
+            mx[(e >> 1) & 3] = fmax3(mx[(e >> 1) & 3], __uint_as_float(s[e0 + e]), __uint_as_float(s[e0 + e + 1]));
+        };
+        row_max(0);
         tmem_wait_ld();
         if (L::kOwnP) {
           tc_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&s_free[x]);
         }
-        if (!whole) {
-#pragma unroll
-          for (int e = 0; e < 128; ++e)
-            if (!((live.w[e >> 5] >> (e & 31)) & 1)) s[e] = 0xff800000u;
-        }
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int e = 0; e < 128; e += 2)
-          mx[(e >> 1) & 3] = fmax3(mx[(e >> 1) & 3], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+        row_max(64);
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
         const bool move = (top - m) * sc > 8.0f;  // also at the first attended key (m = -inf)
         float f = 1.0f;
@@ -652,8 +673,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           m = top;
           l *= f;
         }
-        // P_x and O_x are free once PV_x(j-1) is done
-        if (j > 0 && !(ok = warp_wait(&pv_done[x], (uint32_t)(j - 1) & 1, err))) break;
+        const float mc = m == -INFINITY ? 0.0f : m * sc;
+        const uint64_t cc = f2pack(sc, sc), nm = f2pack(-mc, -mc);
+        uint64_t sum = f2pack(0.0f, 0.0f);
+        uint32_t pw[32];
+        weights<T>(s, cc, nm, pw, sum);
+        weights<T>(s + 32, cc, nm, pw + 16, sum);
+        // P_x and O_x are free once PV_x(j-1) is done: half the weights are
+        // computed before they are needed
+        if (j > 0 && !(ok = one_wait(&pv_done[x], (uint32_t)(j - 1) & 1, err, lane))) break;
         tc_after();
         if (j > 0 && __any_sync(0xffffffffu, move)) {
 #pragma unroll 1
@@ -671,13 +699,21 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             tmem_st16(tO + 16 * q, o);
           }
         }
-        l += weights<T>(s, sc, m == -INFINITY ? 0.0f : m * sc, tP);
+        tmem_st16(tP, pw);
+        tmem_st16(tP + 16, pw + 16);
+        weights<T>(s + 64, cc, nm, pw, sum);
+        tmem_st16(tP + 32, pw);
+        weights<T>(s + 96, cc, nm, pw, sum);
+        tmem_st16(tP + 48, pw);
+        float l0, l1;
+        f2unpack(sum, l0, l1);
+        l += l0 + l1;
         tmem_wait_st();
         tc_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[x]);
       }
-      if (ok && nt > 0) ok = warp_wait(&pv_done[x], (uint32_t)(nt - 1) & 1, err);
+      if (ok && nt > 0) ok = one_wait(&pv_done[x], (uint32_t)(nt - 1) & 1, err, lane);
       if (ok) {
         tc_after();
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
@@ -815,10 +851,10 @@ cudaError_t launch_tile(const XAttnItem *items, int n, const XAttnWork &w, const
 
 template <typename T, int DP>
 cudaError_t run(const XAttnWork &w, const XAttnCall &c, int *err, cudaStream_t st) {
-  const XAttnItem *i16 = w.items, *i32 = i16 + w.n16, *it = i32 + w.n32, *groups = it + w.n_tile;
-  cudaError_t e = launch_tile<T, DP>(it, w.n_tile, w, c, err, st);
-  if (e == cudaSuccess) e = launch_few<T, DP, 1>(i16, w.n16, w, c, st);
-  if (e == cudaSuccess) e = launch_few<T, DP, 2>(i32, w.n32, w, c, st);
+  const XAttnItem *few = w.items, *tile = few + w.n_few, *groups = tile + w.n_tile;
+  cudaError_t e = launch_tile<T, DP>(tile, w.n_tile, w, c, err, st);
+  if (e == cudaSuccess)
+    e = w.few_rows <= 16 ? launch_few<T, DP, 1>(few, w.n_few, w, c, st) : launch_few<T, DP, 2>(few, w.n_few, w, c, st);
   if (e != cudaSuccess || w.n_groups == 0) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)w.n_groups, (unsigned)((w.group_rows + 7) / 8));
@@ -857,7 +893,7 @@ int64_t choose_chunk(const std::vector<int64_t> &keys, int unit, double fixed, d
     if (t < best) best = t, chunk = c;
     if (c <= 1 || n > 8 * (int64_t)slots + (int64_t)units.size()) break;
   }
-  return chunk * unit;
+  return std::min<int64_t>(chunk * unit, 1 << 24);  // an item's key arithmetic is 32-bit
 }
 
 }  // namespace
@@ -865,10 +901,11 @@ int64_t choose_chunk(const std::vector<int64_t> &keys, int unit, double fixed, d
 XAttnSplit cross_attn_split(const XAttnShape &s, const uint64_t *q_start, const uint64_t *q_len, const uint64_t *k_start,
                             const uint64_t *k_len, size_t n_seq, int sms) {
   const int G = s.H / s.KVH, DP = s.D <= 64 ? 64 : 128;
-  std::vector<XAttnItem> whole[3];  // up to 16 rows, up to 32, tiles
+  std::vector<XAttnItem> whole[2];  // few rows, tiles
+  XAttnSplit out;
   for (size_t i = 0; i < n_seq; ++i) {
     const int64_t rows = (int64_t)q_len[i] * G;
-    const int kind = rows <= 16 ? 0 : rows <= 32 ? 1 : 2, step = kind == 2 ? 2 * kRows : 32;
+    const int kind = rows <= kFewMaxRows ? 0 : 1, step = kind == 0 ? kFewRows : 2 * kRows;
     for (int64_t r0 = 0; r0 < rows; r0 += step)
       for (int g = 0; g < s.KVH; ++g) {
         XAttnItem it{};
@@ -880,11 +917,11 @@ XAttnSplit cross_attn_split(const XAttnShape &s, const uint64_t *q_start, const 
         it.kvh = g;
         it.nsplit = 1;
         whole[kind].push_back(it);
+        if (kind == 0) out.few_rows = std::max(out.few_rows, it.rows);
       }
   }
-  XAttnSplit out;
   std::vector<XAttnItem> groups;
-  for (int kind = 0; kind < 3; ++kind) {
+  for (int kind = 0; kind < 2; ++kind) {
     std::vector<int64_t> keys;
     for (const XAttnItem &it : whole[kind]) keys.push_back(it.klen);
     std::vector<XAttnItem> items;
@@ -892,9 +929,9 @@ XAttnSplit cross_attn_split(const XAttnShape &s, const uint64_t *q_start, const 
       // few rows: a unit is 64 keys (16 a warp); a CTA's start and end cost
       // about as much as 8 of them, a join as 8.  Tiles: units of 128 keys, 2 each.
       const int occ = DP == 64 ? 4 : 2;
-      const int64_t chunk = kind < 2 ? choose_chunk(keys, 64, 8.0, 8.0, sms * occ) : choose_chunk(keys, kKeys, 2.0, 3.0, sms);
+      const int64_t chunk = kind == 0 ? choose_chunk(keys, 64, 8.0, 8.0, sms * occ) : choose_chunk(keys, kKeys, 2.0, 3.0, sms);
       for (XAttnItem it : whole[kind]) {
-        const int klen = it.klen, unit = kind < 2 ? 64 : kKeys;
+        const int klen = it.klen, unit = kind == 0 ? 64 : kKeys;
         it.nsplit = (int)std::max<int64_t>(1, (klen + chunk - 1) / chunk);
         if (it.nsplit > 1) {
           it.ws = out.ws_floats;
@@ -916,7 +953,7 @@ XAttnSplit cross_attn_split(const XAttnShape &s, const uint64_t *q_start, const 
         return (int64_t)a.klen * (a.rows > kRows ? 2 : 1) > (int64_t)b.klen * (b.rows > kRows ? 2 : 1);
       });
     }
-    (kind == 0 ? out.n16 : kind == 1 ? out.n32 : out.n_tile) = (int64_t)items.size();
+    (kind == 0 ? out.n_few : out.n_tile) = (int64_t)items.size();
     out.items.insert(out.items.end(), items.begin(), items.end());
   }
   out.n_groups = (int64_t)groups.size();

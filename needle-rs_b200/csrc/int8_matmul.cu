@@ -395,21 +395,20 @@ cudaError_t product(const Int8Args &a, bool pdl, int *err, cudaStream_t st) {
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e != cudaSuccess) return e;
   const int num_n = (a.N + BN - 1) / BN, nkb = (a.K + BK - 1) / BK;
-  // Tokens of a tile: the fewest waves of tiles, each weighed by the bytes
-  // a stage brings in (an SM takes in about 64 a clock from L2, which is what
-  // binds); wider tiles win ties.
-  int bt = 16;
+  // Tokens of a tile and CTAs that share one: the least estimated time, in
+  // clocks of an SM that takes in about 64 bytes each from L2, which is what
+  // binds: the waves of tiles, each the bytes of its stages and a start and end of
+  // about 2,000 clocks, and as much again for the CTAs of a cluster to meet.
+  int bt = 16, split = 1;
   int64_t best = INT64_MAX;
   for (int b = 256; b >= 16; b /= 2) {
     const int64_t tiles = (int64_t)num_n * ((a.M + b - 1) / b);
-    const int64_t cost = (tiles + sms - 1) / sms * (BN + b);
-    if (cost < best) best = cost, bt = b;
+    for (int s = 1; s <= (b <= 128 ? 8 : 1) && s <= nkb && (s == 1 || tiles * s <= sms); s *= 2) {
+      const int64_t waves = (tiles * s + sms - 1) / sms;
+      const int64_t cost = waves * ((BN + b) * 2 * ((nkb + s - 1) / s)) + 2000 + (s > 1 ? 1000 + b * 16 / s : 0) + b * 8;
+      if (cost < best) best = cost, bt = b, split = s;
+    }
   }
-  // Fewer tiles than half the SMs: a cluster for each tile, its CTAs
-  // sharing K.
-  const int64_t tiles = (int64_t)num_n * ((a.M + bt - 1) / bt);
-  int split = 1;
-  while (bt <= 128 && split < 8 && tiles * split * 2 <= sms && split * 2 <= nkb) split *= 2;
   switch (bt) {
     case 16: return launch_tc<16, TY>(a, split, sms, pdl, err, st);
     case 32: return launch_tc<32, TY>(a, split, sms, pdl, err, st);

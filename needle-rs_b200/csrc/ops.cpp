@@ -355,8 +355,8 @@ NeedleCrossAttnPlan *needle_cross_attn_plan_create(const uint64_t *q_start, cons
     plan->flag = (int *)((char *)plan->buf + ib);
     plan->work.items = (const XAttnItem *)plan->buf;
     plan->work.ws = (float *)((char *)plan->flag + 256);
-    plan->work.n16 = (int)split.n16;
-    plan->work.n32 = (int)split.n32;
+    plan->work.n_few = (int)split.n_few;
+    plan->work.few_rows = split.few_rows;
     plan->work.n_tile = (int)split.n_tile;
     plan->work.n_groups = (int)split.n_groups;
     plan->work.group_rows = split.group_rows;

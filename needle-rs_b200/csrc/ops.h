@@ -83,13 +83,13 @@ struct XAttnCall {
   int64_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head;
   float scale;
 };
-// A plan's work (host): items of up to 16 rows, up to 32 and up to 256, then
-// one entry for each group of items that share rows, to be joined.
+// A plan's work (host): items of few rows, tiles of up to 256, then one entry
+// for each group of items that share rows, to be joined.
 struct XAttnSplit {
   std::vector<XAttnItem> items;
-  int64_t n16 = 0, n32 = 0, n_tile = 0, n_groups = 0;
+  int64_t n_few = 0, n_tile = 0, n_groups = 0;
   int64_t ws_floats = 0;
-  int group_rows = 0;  // most rows of a group
+  int few_rows = 0, group_rows = 0;  // most rows of a few-row item, of a group
 };
 XAttnSplit cross_attn_split(const XAttnShape &s, const uint64_t *q_start, const uint64_t *q_len, const uint64_t *k_start,
                             const uint64_t *k_len, size_t n_seq, int sms);
@@ -98,7 +98,7 @@ struct XAttnWork {
   XAttnShape s;
   const XAttnItem *items = nullptr;
   float *ws = nullptr;
-  int n16 = 0, n32 = 0, n_tile = 0, n_groups = 0, group_rows = 0;
+  int n_few = 0, n_tile = 0, n_groups = 0, few_rows = 0, group_rows = 0;
 };
 cudaError_t cross_attn(const XAttnWork &w, const XAttnCall &c, int *err, cudaStream_t st);
 
