@@ -335,23 +335,18 @@ __global__ void __launch_bounds__(kFewWarps * 32) xattn_few_kernel(const XAttnIt
 
 // ── many rows ───────────────────────────────────────────────────────────────
 
-constexpr int kRows = 128, kKeys = 128, kTileThreads = 384;
-// Registers a thread, as the launch gives them and after setmaxnreg.
-constexpr int kRegLaunch = 168, kRegOther = 56, kRegSoftmax = 224;
-static_assert(128 * kRegOther + 256 * kRegSoftmax == kTileThreads * kRegLaunch, "the split adds up to the launch's");
+constexpr int kRows = 128, kKeys = 64, kTileThreads = 256;
 
 template <int DP>
 struct Tile {
-  static constexpr int kAtoms = DP / 64;                    // 64-dimension halves of a row (128 bytes each)
-  static constexpr int kAtom = kKeys * 128;                 // bytes of 128 rows of one half
-  static constexpr int kBytes = kAtoms * kAtom;             // a tile of Q, K or V
-  static constexpr int kStages = DP == 64 ? 4 : 2;          // K tiles, and V tiles, in flight
-  static constexpr int kQ = 0, kK = 2 * kBytes, kV = kK + kStages * kBytes, kBar = kV + kStages * kBytes;
+  static constexpr int kAtoms = DP / 64;  // 64-dimension parts of a row (128 bytes each)
+  static constexpr int kQAtom = kRows * 128, kAtom = kKeys * 128, kQBytes = kAtoms * kQAtom, kBytes = kAtoms * kAtom;
+  static constexpr int kStages = DP == 64 ? 4 : 2;  // K tiles, and V tiles, in flight
+  static constexpr int kQ = 0, kK = kQBytes, kV = kK + kStages * kBytes, kBar = kV + kStages * kBytes;
   static constexpr int kSmem = kBar + 256 + 1024;
-  // TMEM columns: S of both slots, their O; P beside them where there is room, else over S
-  static constexpr int kO = 256;
-  static constexpr bool kOwnP = DP == 64;
-  __host__ __device__ static constexpr int p_col(int x) { return kOwnP ? 384 + 64 * x : 128 * x; }
+  // TMEM columns: two S (P over each), then O
+  static constexpr int kO = 2 * kKeys, kCols = 256;
+  static_assert(kO + DP <= kCols, "S and O fit half of TMEM");
 };
 
 template <typename T>
@@ -398,15 +393,15 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   return d;
 }
 
-// Which keys of tile j of an item are attended to: bit i of word i / 32
-// (the whole warp calls it).
+// Which keys of tile j of an item are attended to: bit i of word i / 32 (the
+// whole warp calls it).
 struct Live {
-  uint32_t w[4];
+  uint32_t w[kKeys / 32];
 };
 __device__ __forceinline__ Live live_keys(const uint8_t *mask, int klen, int j, int lane) {
   Live v;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
+  for (int q = 0; q < kKeys / 32; ++q) {
     const int i = j * kKeys + 32 * q + lane;
     v.w[q] = __ballot_sync(0xffffffffu, i < klen && (!mask || mask[i] != 0));
   }
@@ -427,30 +422,22 @@ __device__ __forceinline__ void weights(const uint32_t *s, uint64_t cc, uint64_t
   }
 }
 
-// Bounded wait of a converged warp through one lane: 32 lanes polling one
-// barrier take about 200 clocks even when its phase is complete.
-__device__ __forceinline__ bool one_wait(uint64_t *b, uint32_t parity, int *err, int lane) {
-  bool ok = true;
-  if (lane == 0) ok = mbar_wait(b, parity, err);
-  ok = __all_sync(0xffffffffu, ok);
-  __syncwarp();  // orders what lane 0 has seen before the other lanes' reads
-  return ok;
-}
-
-// Up to 256 rows (two slots of 128) of one request and KV head.  Warp 0
-// loads K and V tiles of 128 keys (TMA, a ring each), warp 1 issues the MMAs,
-// warp 2 zeroes the V rows of keys that are not attended to (their weights are
-// zero, but zero times NaN is not), and a warpgroup for each slot turns scores
-// into weights, a thread a row.  For slot x and tile j:
-//   S_x = Q_x K_j^T   M128 N128, both K-major in shared memory
-//   P_x = weights     TMEM, 16 bits
-//   O_x += P_x V_j    M128 N DP, P from TMEM, V MN-major
-// m moves only when a row's maximum passes it by 2^8, and O_x is rescaled
-// then: a weight is at most 256.  With D <= 64 P has TMEM columns of its own and
-// S_x(j+1) is issued as soon as the softmax has read S_x(j); with D > 64 P lies over S
-// and S_x(j+1) follows PV_x(j), while the other slot's softmax runs.
+// Up to 128 rows of one request and KV head, tiles of 64 keys.  Warp 0 loads K
+// and V (TMA, a ring each), warp 1 issues the MMAs, warp 2 zeroes the V rows of keys
+// that are not attended to (their weights are zero, but zero times NaN is not), and
+// warps 4-7 turn scores into weights, a thread a row.  For tile j:
+//   S(j) = Q K_j^T    M128 N64, both K-major in shared memory
+//   P(j) = weights    TMEM, 16 bits, over S(j)
+//   O += P(j) V_j     M128 N DP, P from TMEM, V MN-major
+// S has two buffers: S(j+1) is multiplied while the softmax works on S(j).  m
+// moves only when a row's maximum passes it by 2^8, and O is rescaled then: a
+// weight is at most 256.
+//
+// The exponentials bind (4 a clock on each SM partition).  Half of TMEM and of
+// the registers make two CTAs an SM: one loads, reduces, starts or ends while the other is
+// at its exponentials.
 template <typename T, int DP>
-__global__ void __launch_bounds__(kTileThreads, 1)
+__global__ void __launch_bounds__(kTileThreads, 2)
     xattn_tile_kernel(const XAttnItem *items, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                       XAttnWork w, XAttnCall c, int *err) {
   using L = Tile<DP>;
@@ -458,15 +445,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t *sm = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint64_t *k_full = (uint64_t *)(sm + L::kBar), *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST;
-  uint64_t *v_ok = v_empty + ST, *q_full = v_ok + ST;
-  uint64_t *s_full = q_full + 1, *s_free = s_full + 2, *p_full = s_free + 2, *pv_done = p_full + 2;
-  uint32_t *tmem_slot = (uint32_t *)(pv_done + 2);
+  uint64_t *v_ok = v_empty + ST, *q_full = v_ok + ST, *s_full = q_full + 1, *p_full = s_full + 2, *pv_done = p_full + 1;
+  uint32_t *tmem_slot = (uint32_t *)(pv_done + 1);
   pdl_trigger();
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const XAttnItem it = items[blockIdx.x];
   const int nt = (it.klen + kKeys - 1) / kKeys;
-  const bool two = it.rows > kRows;
   const uint8_t *mask = c.mask ? c.mask + it.k0 : nullptr;
   // keys of tile j that the MMAs cover: a multiple of 16
   auto covered = [&](int j) { return min(kKeys, (it.klen - j * kKeys + 15) & ~15); };
@@ -479,17 +464,16 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       mbar_init(&v_empty[s], 1);
       mbar_init(&v_ok[s], 1);
     }
-    mbar_init(q_full, 8);
-    for (int x = 0; x < 2; ++x) {
-      mbar_init(&s_full[x], 1);
-      mbar_init(&s_free[x], 4);
-      mbar_init(&p_full[x], 4);
-      mbar_init(&pv_done[x], 1);
-    }
+    mbar_init(q_full, 4);
+    mbar_init(&s_full[0], 1);
+    mbar_init(&s_full[1], 1);
+    mbar_init(p_full, 4);
+    mbar_init(pv_done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512));
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(L::kCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   tc_before();
@@ -497,261 +481,215 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   tc_after();
   const uint32_t tmem = *(volatile uint32_t *)tmem_slot;
 
-  if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegOther));
-    if (warp == 0) {
-      if (lane == 0) {
-        int k_done = 0, v_done = 0;
-        bool ok = true;
-        for (int j = 0; j < nt && ok; ++j) {
-          const int s = j % ST, row = (int)it.k0 + j * kKeys;
-          const uint32_t ph = (uint32_t)((j / ST) & 1) ^ 1;
-          if (!(ok = mbar_wait(&k_empty[s], ph, err))) break;
-          mbar_expect_tx(&k_full[s], L::kBytes);
-          for (int a = 0; a < L::kAtoms; ++a)
-            tma_load_3d(sm + L::kK + s * L::kBytes + a * L::kAtom, &mk, &k_full[s], 64 * a, it.kvh, row);
-          ++k_done;
-          if (!(ok = mbar_wait(&v_empty[s], ph, err))) break;
-          mbar_expect_tx(&v_full[s], L::kBytes);
-          for (int a = 0; a < L::kAtoms; ++a)
-            tma_load_3d(sm + L::kV + s * L::kBytes + a * L::kAtom, &mv, &v_full[s], 64 * a, it.kvh, row);
-          ++v_done;
-        }
-        // no copy may be in flight when the CTA leaves
-        for (int j = max(0, k_done - ST); j < k_done; ++j) mbar_drain(&k_full[j % ST], (uint32_t)((j / ST) & 1));
-        for (int j = max(0, v_done - ST); j < v_done; ++j) mbar_drain(&v_full[j % ST], (uint32_t)((j / ST) & 1));
-      }
-      __syncwarp();
-    } else if (warp == 1 && nt > 0) {
-      // descriptors share their high word; the low one is the address / 16
-      // (and, MN-major, the distance of the 64-dimension halves)
-      const uint32_t s16 = smem_u32(sm) >> 4;
-      const uint64_t hi = umma_desc(sm) & 0xFFFFFFFF00000000ull;
-      auto kmaj = [&](uint32_t a16) { return hi | (uint64_t)(a16 | (1u << 16)); };
-      auto mnmaj = [&](uint32_t a16) { return hi | (uint64_t)(a16 | ((uint32_t)(L::kAtom >> 4) << 16)); };
-      const int steps = (w.s.D + 15) / 16;
-      auto issue_s = [&](int x, int j) {
-        const int s = j % ST;
-        const uint32_t id = f16_idesc<T>(covered(j), false), d = tmem + 128u * x;
-        const uint32_t q = s16 + (uint32_t)((L::kQ + x * L::kBytes) >> 4), k = s16 + (uint32_t)((L::kK + s * L::kBytes) >> 4);
-#pragma unroll 1
-        for (int i = 0; i < steps; ++i) {
-          const uint32_t at = (uint32_t)((i >> 2) * (L::kAtom >> 4) + (i & 3) * 2);
-          umma_bf16_e(d, kmaj(q + at), kmaj(k + at), id, i ? 1u : 0u);
-        }
-        umma_commit_e(&s_full[x]);
-      };
-      auto issue_pv = [&](int x, int j) {
-        const int s = j % ST, n = covered(j) >> 4;
-        const uint32_t id = f16_idesc<T>(DP, true), d = tmem + (uint32_t)(L::kO + DP * x);
-        const uint32_t v = s16 + (uint32_t)((L::kV + s * L::kBytes) >> 4), p = tmem + (uint32_t)L::p_col(x);
-#pragma unroll 1
-        for (int i = 0; i < n; ++i) umma_bf16_ts_e(d, p + 8 * i, mnmaj(v + 128 * i), id, (j | i) ? 1u : 0u);
-        umma_commit_e(&pv_done[x]);
-      };
-      // S_x(j), once S_x(j-1) has been read and, where P lies over S, used
-      auto next_s = [&](int x, int j) -> bool {
-        if (j > 0) {
-          if (L::kOwnP ? !one_wait(&s_free[x], (uint32_t)(j - 1) & 1, err, lane) : !one_wait(&pv_done[x], (uint32_t)(j - 1) & 1, err, lane))
-            return false;
-        }
-        if (x == 0 && !one_wait(&k_full[j % ST], (uint32_t)((j / ST) & 1), err, lane)) return false;
-        tc_after();
-        issue_s(x, j);
-        if (x == (two ? 1 : 0)) umma_commit_e(&k_empty[j % ST]);
-        return true;
-      };
-      auto next_pv = [&](int x, int j) -> bool {
-        if (!one_wait(&p_full[x], (uint32_t)j & 1, err, lane)) return false;
-        if (x == 0 && (!one_wait(&v_full[j % ST], (uint32_t)((j / ST) & 1), err, lane) ||
-                       !one_wait(&v_ok[j % ST], (uint32_t)((j / ST) & 1), err, lane)))
-          return false;
-        tc_after();
-        issue_pv(x, j);
-        if (x == (two ? 1 : 0)) umma_commit_e(&v_empty[j % ST]);
-        return true;
-      };
-      bool ok = one_wait(q_full, 0, err, lane) && next_s(0, 0) && (!two || next_s(1, 0));
+  if (warp == 0) {
+    if (lane == 0) {
+      int k_done = 0, v_done = 0;
+      bool ok = true;
       for (int j = 0; j < nt && ok; ++j) {
-        const bool more = j + 1 < nt;
-        if (L::kOwnP) {
-          ok = (!more || next_s(0, j + 1)) && (!more || !two || next_s(1, j + 1)) && next_pv(0, j) &&
-               (!two || next_pv(1, j));
-        } else {
-          ok = next_pv(0, j) && (!more || next_s(0, j + 1)) && (!two || next_pv(1, j)) &&
-               (!more || !two || next_s(1, j + 1));
-        }
+        const int s = j % ST, row = (int)it.k0 + j * kKeys;
+        const uint32_t ph = (uint32_t)((j / ST) & 1) ^ 1;
+        if (!(ok = mbar_wait(&k_empty[s], ph, err))) break;
+        mbar_expect_tx(&k_full[s], L::kBytes);
+        for (int a = 0; a < L::kAtoms; ++a)
+          tma_load_3d(sm + L::kK + s * L::kBytes + a * L::kAtom, &mk, &k_full[s], 64 * a, it.kvh, row);
+        ++k_done;
+        if (!(ok = mbar_wait(&v_empty[s], ph, err))) break;
+        mbar_expect_tx(&v_full[s], L::kBytes);
+        for (int a = 0; a < L::kAtoms; ++a)
+          tma_load_3d(sm + L::kV + s * L::kBytes + a * L::kAtom, &mv, &v_full[s], 64 * a, it.kvh, row);
+        ++v_done;
       }
-    } else if (warp == 2) {
-      for (int j = 0; j < nt; ++j) {
-        const int s = j % ST;
-        const bool whole = !mask && (j + 1) * kKeys <= it.klen;
-        Live live{};
-        if (!whole) live = live_keys(mask, it.klen, j, lane);
-        if (!one_wait(&v_full[s], (uint32_t)((j / ST) & 1), err, lane)) break;
-        if (!whole) {
-          const int n = covered(j);
-          // 8 lanes a row and half, 4 rows at a time
-          for (int r0 = 0; r0 < n; r0 += 4) {
-            const int r = r0 + (lane >> 3);
-            if ((live.w[r >> 5] >> (r & 31)) & 1) continue;
-#pragma unroll
-            for (int a = 0; a < L::kAtoms; ++a)
-              *reinterpret_cast<uint4 *>(sm + L::kV + s * L::kBytes + a * L::kAtom + r * 128 + (lane & 7) * 16) =
-                  make_uint4(0, 0, 0, 0);
-          }
-          fence_async_smem();
-          __syncwarp();
-        }
-        if (lane == 0) mbar_arrive(&v_ok[s]);
-      }
+      // no copy may be in flight when the CTA leaves
+      for (int j = max(0, k_done - ST); j < k_done; ++j) mbar_drain(&k_full[j % ST], (uint32_t)((j / ST) & 1));
+      for (int j = max(0, v_done - ST); j < v_done; ++j) mbar_drain(&v_full[j % ST], (uint32_t)((j / ST) & 1));
     }
-  } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegSoftmax));
-    const int quarter = warp & 3, x = (warp - 4) >> 2;
-    const int i = x * kRows + quarter * 32 + lane, r = it.r0 + i;  // this thread's row
+    __syncwarp();
+  } else if (warp == 1 && nt > 0) {
+    // descriptors share their high word; the low one is the address / 16 (and,
+    // MN-major, the distance of the 64-dimension parts)
+    const uint32_t s16 = smem_u32(sm) >> 4;
+    const uint64_t hi = umma_desc(sm) & 0xFFFFFFFF00000000ull;
+    const uint32_t q16 = (s16 + (uint32_t)(L::kQ >> 4)) | (1u << 16), k16 = s16 + (uint32_t)(L::kK >> 4),
+                   v16 = (s16 + (uint32_t)(L::kV >> 4)) | ((uint32_t)(L::kAtom >> 4) << 16);
+    const int steps = (w.s.D + 15) / 16;
+    auto score = [&](int j) -> bool {  // S(j)
+      const int s = j % ST;
+      if (!warp_wait(&k_full[s], (uint32_t)((j / ST) & 1), err)) return false;
+      tc_after();
+      const uint32_t id = f16_idesc<T>(covered(j), false), k = (k16 + (uint32_t)(s * (L::kBytes >> 4))) | (1u << 16);
+      const uint32_t d = tmem + (uint32_t)((j & 1) * kKeys);
+#pragma unroll
+      for (int i = 0; i < DP / 16; ++i) {
+        const uint32_t in = (uint32_t)((i & 3) * 2), qa = (i >> 2) * (L::kQAtom >> 4) + in, ka = (i >> 2) * (L::kAtom >> 4) + in;
+        if (i < steps) umma_bf16_e(d, hi | (q16 + qa), hi | (k + ka), id, i ? 1u : 0u);
+      }
+      umma_commit_e(&s_full[j & 1]);
+      umma_commit_e(&k_empty[s]);
+      return true;
+    };
+    bool ok = warp_wait(q_full, 0, err) && score(0);
+    for (int j = 0; j < nt && ok; ++j) {
+      // S(j+1) goes where P(j-1) was
+      if (j + 1 < nt) ok = (j == 0 || warp_wait(pv_done, (uint32_t)(j - 1) & 1, err)) && score(j + 1);
+      const int s = j % ST, n = covered(j) >> 4;
+      ok = ok && warp_wait(&v_ok[s], (uint32_t)((j / ST) & 1), err) && warp_wait(p_full, (uint32_t)j & 1, err);
+      if (!ok) break;
+      tc_after();
+      const uint32_t id = f16_idesc<T>(DP, true), v = v16 + (uint32_t)(s * (L::kBytes >> 4));
+#pragma unroll
+      for (int i = 0; i < kKeys / 16; ++i)
+        if (i < n)
+          umma_bf16_ts_e(tmem + L::kO, tmem + (uint32_t)((j & 1) * kKeys + 8 * i), hi | (v + 128 * i), id, (j | i) ? 1u : 0u);
+      umma_commit_e(pv_done);
+      umma_commit_e(&v_empty[s]);
+    }
+  } else if (warp == 2) {
+    for (int j = 0; j < nt; ++j) {
+      const int s = j % ST;
+      const bool whole = !mask && (j + 1) * kKeys <= it.klen;
+      Live live{};
+      if (!whole) live = live_keys(mask, it.klen, j, lane);
+      if (!warp_wait(&v_full[s], (uint32_t)((j / ST) & 1), err)) break;
+      if (!whole) {
+        const int n = covered(j);
+        // 8 lanes a row, 4 rows at a time
+        for (int r0 = 0; r0 < n; r0 += 4) {
+          const int r = r0 + (lane >> 3);
+          if ((live.w[r >> 5] >> (r & 31)) & 1) continue;
+#pragma unroll
+          for (int a = 0; a < L::kAtoms; ++a)
+            *reinterpret_cast<uint4 *>(sm + L::kV + s * L::kBytes + a * L::kAtom + r * 128 + (lane & 7) * 16) =
+                make_uint4(0, 0, 0, 0);
+        }
+        fence_async_smem();
+        __syncwarp();
+      }
+      if (lane == 0) mbar_arrive(&v_ok[s]);
+    }
+  } else if (warp >= 4) {
+    const int quarter = warp & 3, i = quarter * 32 + lane, r = it.r0 + i;  // this thread's row
     const int G = w.s.H / w.s.KVH, D = w.s.D;
     const int h = it.kvh * G + r % G;
     const int64_t row = it.q0 + r / G;
-    const bool mine = i < it.rows, slot = x == 0 || two;
-    if (slot) {  // the row of Q, K-major with the 128-byte swizzle
+    const bool mine = i < it.rows;
+    {  // the row of Q, K-major with the 128-byte swizzle
       const T *q = (const T *)c.q + row * c.q_row + (int64_t)h * c.q_head;
-      uint8_t *dst = sm + L::kQ + x * L::kBytes + (quarter * 32 + lane) * 128;
+      uint8_t *dst = sm + L::kQ + i * 128;
 #pragma unroll
       for (int ch = 0; ch < DP / 8; ++ch) {
         uint4 v = make_uint4(0, 0, 0, 0);
         if (mine && ch * 8 < D) v = *reinterpret_cast<const uint4 *>(q + ch * 8);
-        *reinterpret_cast<uint4 *>(dst + (ch >> 3) * L::kAtom + (((ch & 7) ^ (lane & 7)) << 4)) = v;
+        *reinterpret_cast<uint4 *>(dst + (ch >> 3) * L::kQAtom + (((ch & 7) ^ (lane & 7)) << 4)) = v;
       }
       fence_async_smem();
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(q_full);
-    if (slot) {
-      const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-      const uint32_t tS = tmem + lanes + 128u * x, tP = tmem + lanes + (uint32_t)L::p_col(x);
-      const uint32_t tO = tmem + lanes + (uint32_t)(L::kO + DP * x);
-      const float sc = c.scale * kLog2e;
-      float m = -INFINITY, l = 0.0f;
-      bool ok = true;
-      for (int j = 0; j < nt; ++j) {
-        const bool whole = !mask && (j + 1) * kKeys <= it.klen;
-        Live live{};
-        if (!whole) live = live_keys(mask, it.klen, j, lane);
-        if (!(ok = one_wait(&s_full[x], (uint32_t)j & 1, err, lane))) break;
-        tc_after();
-        uint32_t s[128];
-        tmem_ld32_raw(tS, s);
-        tmem_ld32_raw(tS + 32, s + 32);
-        tmem_wait_ld();
-        tmem_ld32_raw(tS + 64, s + 64);
-        tmem_ld32_raw(tS + 96, s + 96);
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        auto row_max = [&](int e0) {
-          if (!whole) {
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16, tO = tmem + lanes + (uint32_t)L::kO;
+    const float sc = c.scale * kLog2e;
+    float m = -INFINITY, l = 0.0f;
+    bool ok = true;
+    for (int j = 0; j < nt; ++j) {
+      const bool whole = !mask && (j + 1) * kKeys <= it.klen;
+      Live live{};
+      if (!whole) live = live_keys(mask, it.klen, j, lane);
+      if (!(ok = warp_wait(&s_full[j & 1], (uint32_t)(j >> 1) & 1, err))) break;
+      tc_after();
+      const uint32_t tS = tmem + lanes + (uint32_t)((j & 1) * kKeys);
+      uint32_t s[kKeys];
+      tmem_ld32_raw(tS, s);
+      tmem_ld32_raw(tS + 32, s + 32);
+      tmem_wait_ld();
+      if (!whole) {
 #pragma unroll
-            for (int e = 0; e < 64; ++e)
-              if (!((live.w[(e0 + e) >> 5] >> (e & 31)) & 1)) s[e0 + e] = 0xff800000u;
-          }
-#pragma unroll
-          for (int e = 0; e < 64; e += 2)
-            mx[(e >> 1) & 3] = fmax3(mx[(e >> 1) & 3], __uint_as_float(s[e0 + e]), __uint_as_float(s[e0 + e + 1]));
-        };
-        row_max(0);
-        tmem_wait_ld();
-        if (L::kOwnP) {
-          tc_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&s_free[x]);
-        }
-        row_max(64);
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        const bool move = (top - m) * sc > 8.0f;  // also at the first attended key (m = -inf)
-        float f = 1.0f;
-        if (move) {
-          f = ex2((m - top) * sc);
-          m = top;
-          l *= f;
-        }
-        const float mc = m == -INFINITY ? 0.0f : m * sc;
-        const uint64_t cc = f2pack(sc, sc), nm = f2pack(-mc, -mc);
-        uint64_t sum = f2pack(0.0f, 0.0f);
-        uint32_t pw[32];
-        weights<T>(s, cc, nm, pw, sum);
-        weights<T>(s + 32, cc, nm, pw + 16, sum);
-        // P_x and O_x are free once PV_x(j-1) is done: half the weights are
-        // computed before they are needed
-        if (j > 0 && !(ok = one_wait(&pv_done[x], (uint32_t)(j - 1) & 1, err, lane))) break;
-        tc_after();
-        if (j > 0 && __any_sync(0xffffffffu, move)) {
-#pragma unroll 1
-          for (int q = 0; q < DP / 16; ++q) {
-            uint32_t o[16];
-            asm volatile(
-                "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-                "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-                : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]), "=r"(o[4]), "=r"(o[5]), "=r"(o[6]), "=r"(o[7]),
-                  "=r"(o[8]), "=r"(o[9]), "=r"(o[10]), "=r"(o[11]), "=r"(o[12]), "=r"(o[13]), "=r"(o[14]), "=r"(o[15])
-                : "r"(tO + 16 * q));
-            tmem_wait_ld();
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            tmem_st16(tO + 16 * q, o);
-          }
-        }
-        tmem_st16(tP, pw);
-        tmem_st16(tP + 16, pw + 16);
-        weights<T>(s + 64, cc, nm, pw, sum);
-        tmem_st16(tP + 32, pw);
-        weights<T>(s + 96, cc, nm, pw, sum);
-        tmem_st16(tP + 48, pw);
-        float l0, l1;
-        f2unpack(sum, l0, l1);
-        l += l0 + l1;
-        tmem_wait_st();
-        tc_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[x]);
+        for (int e = 0; e < kKeys; ++e)
+          if (!((live.w[e >> 5] >> (e & 31)) & 1)) s[e] = 0xff800000u;
       }
-      if (ok && nt > 0) ok = one_wait(&pv_done[x], (uint32_t)(nt - 1) & 1, err, lane);
-      if (ok) {
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int e = 0; e < kKeys; e += 2)
+        mx[(e >> 1) & 3] = fmax3(mx[(e >> 1) & 3], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      const bool move = (top - m) * sc > 8.0f;  // also at the first attended key (m = -inf)
+      float f = 1.0f;
+      if (move) {
+        f = ex2((m - top) * sc);
+        m = top;
+        l *= f;
+      }
+      if (j > 0 && __any_sync(0xffffffffu, move)) {
+        if (!(ok = warp_wait(pv_done, (uint32_t)(j - 1) & 1, err))) break;
         tc_after();
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
-        T *out = (T *)c.out + row * c.o_row + (int64_t)h * c.o_head;
-        float *p = partial(w, it, it.split, DP);
+#pragma unroll 1
+        for (int q = 0; q < DP / 16; ++q) {
+          uint32_t o[16];
+          asm volatile(
+              "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+              "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+              : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]), "=r"(o[4]), "=r"(o[5]), "=r"(o[6]), "=r"(o[7]),
+                "=r"(o[8]), "=r"(o[9]), "=r"(o[10]), "=r"(o[11]), "=r"(o[12]), "=r"(o[13]), "=r"(o[14]), "=r"(o[15])
+              : "r"(tO + 16 * q));
+          tmem_wait_ld();
 #pragma unroll
-        for (int q = 0; q < DP / 32; ++q) {
-          uint32_t o[32];
+          for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+          tmem_st16(tO + 16 * q, o);
+        }
+      }
+      const float mc = m == -INFINITY ? 0.0f : m * sc;
+      const uint64_t cc = f2pack(sc, sc), nm = f2pack(-mc, -mc);
+      uint64_t sum = f2pack(0.0f, 0.0f);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0;
-          if (nt > 0) {
-            tmem_ld32_raw(tO + 32 * q, o);
-            tmem_wait_ld();
-          }
-          if (!mine) continue;
-          if (it.nsplit > 1) {
+      for (int q = 0; q < kKeys / 32; ++q) {
+        uint32_t pw[16];
+        weights<T>(s + 32 * q, cc, nm, pw, sum);
+        tmem_st16(tS + 16 * q, pw);
+      }
+      float l0, l1;
+      f2unpack(sum, l0, l1);
+      l += l0 + l1;
+      tmem_wait_st();
+      tc_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full);
+    }
+    if (ok && nt > 0) ok = warp_wait(pv_done, (uint32_t)(nt - 1) & 1, err);
+    if (ok) {
+      tc_after();
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
+      T *out = (T *)c.out + row * c.o_row + (int64_t)h * c.o_head;
+      float *p = partial(w, it, it.split, DP);
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<uint4 *>(p + (int64_t)i * DP + 32 * q + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-          } else {
+      for (int q = 0; q < DP / 32; ++q) {
+        uint32_t o[32];
 #pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-              if (32 * q + e >= D) break;
-              uint32_t u[4];
+        for (int e = 0; e < 32; ++e) o[e] = 0;
+        if (nt > 0) {
+          tmem_ld32_raw(tO + 32 * q, o);
+          tmem_wait_ld();
+        }
+        if (!mine) continue;
+        if (it.nsplit > 1) {
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                u[k] = pack2<T>(__uint_as_float(o[e + 2 * k]) * inv, __uint_as_float(o[e + 2 * k + 1]) * inv);
-              *reinterpret_cast<uint4 *>(out + 32 * q + e) = make_uint4(u[0], u[1], u[2], u[3]);
-            }
+          for (int e = 0; e < 32; e += 4)
+            *reinterpret_cast<uint4 *>(p + (int64_t)i * DP + 32 * q + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            if (32 * q + e >= D) break;
+            uint32_t u[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              u[k] = pack2<T>(__uint_as_float(o[e + 2 * k]) * inv, __uint_as_float(o[e + 2 * k + 1]) * inv);
+            *reinterpret_cast<uint4 *>(out + 32 * q + e) = make_uint4(u[0], u[1], u[2], u[3]);
           }
         }
-        if (mine) {
-          if (it.nsplit > 1) {
-            p[it.rows * DP + i] = m * sc;
-            p[it.rows * (DP + 1) + i] = l;
-          } else if (c.lse) {
-            c.lse[row * w.s.H + h] = l == 0.0f ? -INFINITY : fmaf(m * sc, kLn2, logf(l));
-          }
+      }
+      if (mine) {
+        if (it.nsplit > 1) {
+          p[it.rows * DP + i] = m * sc;
+          p[it.rows * (DP + 1) + i] = l;
+        } else if (c.lse) {
+          c.lse[row * w.s.H + h] = l == 0.0f ? -INFINITY : fmaf(m * sc, kLn2, logf(l));
         }
       }
     }
@@ -761,7 +699,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   __syncthreads();
   if (warp == 1) {
     tc_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::kCols));
   }
 }
 
@@ -905,7 +843,7 @@ XAttnSplit cross_attn_split(const XAttnShape &s, const uint64_t *q_start, const 
   XAttnSplit out;
   for (size_t i = 0; i < n_seq; ++i) {
     const int64_t rows = (int64_t)q_len[i] * G;
-    const int kind = rows <= kFewMaxRows ? 0 : 1, step = kind == 0 ? kFewRows : 2 * kRows;
+    const int kind = rows <= kFewMaxRows ? 0 : 1, step = kind == 0 ? kFewRows : kRows;
     for (int64_t r0 = 0; r0 < rows; r0 += step)
       for (int g = 0; g < s.KVH; ++g) {
         XAttnItem it{};
@@ -927,11 +865,11 @@ XAttnSplit cross_attn_split(const XAttnShape &s, const uint64_t *q_start, const 
     std::vector<XAttnItem> items;
     if (!keys.empty()) {
       // few rows: a unit is 64 keys (16 a warp); a CTA's start and end cost
-      // about as much as 8 of them, a join as 8.  Tiles: units of 128 keys, 2 each.
+      // about as much as 8 of them, a join as 8.  Tiles: 4 of 64 keys, a join 6.
       const int occ = DP == 64 ? 4 : 2;
-      const int64_t chunk = kind == 0 ? choose_chunk(keys, 64, 8.0, 8.0, sms * occ) : choose_chunk(keys, kKeys, 2.0, 3.0, sms);
+      const int64_t chunk = kind == 0 ? choose_chunk(keys, 64, 8.0, 8.0, sms * occ) : choose_chunk(keys, kKeys, 4.0, 6.0, sms * 2);
       for (XAttnItem it : whole[kind]) {
-        const int klen = it.klen, unit = kind == 0 ? 64 : kKeys;
+        const int klen = it.klen, unit = 64;
         it.nsplit = (int)std::max<int64_t>(1, (klen + chunk - 1) / chunk);
         if (it.nsplit > 1) {
           it.ws = out.ws_floats;
@@ -950,7 +888,7 @@ XAttnSplit cross_attn_split(const XAttnShape &s, const uint64_t *q_start, const 
       }
       // the longest first
       std::stable_sort(items.begin(), items.end(), [](const XAttnItem &a, const XAttnItem &b) {
-        return (int64_t)a.klen * (a.rows > kRows ? 2 : 1) > (int64_t)b.klen * (b.rows > kRows ? 2 : 1);
+        return a.klen > b.klen;
       });
     }
     (kind == 0 ? out.n_few : out.n_tile) = (int64_t)items.size();

@@ -83,7 +83,7 @@ struct XAttnCall {
   int64_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head;
   float scale;
 };
-// A plan's work (host): items of few rows, tiles of up to 256, then one entry
+// A plan's work (host): items of few rows, tiles of up to 128, then one entry
 // for each group of items that share rows, to be joined.
 struct XAttnSplit {
   std::vector<XAttnItem> items;
