@@ -652,6 +652,9 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       __syncwarp();
       if (lane == 0) mbar_arrive(p_full);
     }
+    // S(nt - 1) says that PV(nt - 3) is done: the last two phases are waited for in
+    // order, since a wait for one alone would take its predecessor's parity for it
+    if (ok && nt > 1) ok = warp_wait(pv_done, (uint32_t)(nt - 2) & 1, err);
     if (ok && nt > 0) ok = warp_wait(pv_done, (uint32_t)(nt - 1) & 1, err);
     if (ok) {
       tc_after();
