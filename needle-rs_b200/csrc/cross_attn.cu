@@ -408,24 +408,72 @@ __device__ __forceinline__ Live live_keys(const uint8_t *mask, int klen, int j, 
   return v;
 }
 
+// 2^t for a pair of t on the FMA units: t = j + f with j = round(t), 2^f on
+// [-1/2, 1/2] by a polynomial of degree 5 fitted here to the least relative
+// error with a constant term of 1 (1.1e-7 with these coefficients), times 2^j put together
+// from its exponent.  t at or below -127 gives 0, NaN stays NaN.
+__device__ __forceinline__ uint64_t ex2_fma(uint64_t t) {
+  const float magic = 12582912.0f + 127.0f;  // its sum with t holds j + 127 in the low bits
+  const uint64_t m2 = f2pack(magic, magic);
+  float a, b;
+  f2unpack(t, a, b);
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(a));  // -127
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(b));
+  t = f2pack(a, b);
+  const uint64_t z = fadd2(t, m2), f = fsub2(t, fsub2(z, m2));
+  uint64_t p = ffma2(f, f2pack(0.001326472731307149f, 0.001326472731307149f), f2pack(0.009671512991189957f, 0.009671512991189957f));
+  p = ffma2(p, f, f2pack(0.05550733581185341f, 0.05550733581185341f));
+  p = ffma2(p, f, f2pack(0.24022242426872253f, 0.24022242426872253f));
+  p = ffma2(p, f, f2pack(0.6931470036506653f, 0.6931470036506653f));
+  p = ffma2(p, f, f2pack(1.0f, 1.0f));
+  f2unpack(z, a, b);
+  return fmul2(p, f2pack(__uint_as_float(__float_as_uint(a) << 23), __uint_as_float(__float_as_uint(b) << 23)));
+}
+
 // 32 weights of a row: p = 2^(s c - m c), rounded and packed into w, their sum
-// added to `sum`.
+// added to `sum`.  The exponential unit gives 4 results a clock on an SM
+// partition and binds the kernel, so a quarter of the exponentials run on the FMA units.
+// The groups of 8 pairs, each one's arguments ahead of the previous one's
+// results, keep one warp at the unit's rate: alone / two warps a partition, a
+// clocked loop of 64 exponentials takes 534 / 887 clocks, without the polynomial 603 / 1067,
+// written pair by pair 1066 / 1194 (the unit: 512 / 1024).
 template <typename T>
-__device__ __forceinline__ void weights(const uint32_t *s, uint64_t cc, uint64_t nm, uint32_t *w, uint64_t &sum) {
+__device__ __forceinline__ void weights(const uint32_t *s, uint64_t cc, uint64_t nm, uint32_t *w, uint64_t *sum) {
+  constexpr int G = 8, FMA = 2;  // pairs of a group, those on the FMA units
+  uint64_t t[G];
+  auto arguments = [&](int g) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    float t0, t1;
-    f2unpack(ffma2(f2pack(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), cc, nm), t0, t1);
-    const float p0 = ex2(t0), p1 = ex2(t1);
-    sum = fadd2(sum, f2pack(p0, p1));
-    w[i] = pack2<T>(p0, p1);
+    for (int i = 0; i < G; ++i)
+      t[i] = ffma2(f2pack(__uint_as_float(s[2 * (g * G + i)]), __uint_as_float(s[2 * (g * G + i) + 1])), cc, nm);
+  };
+  arguments(0);
+#pragma unroll
+  for (int g = 0; g < 16 / G; ++g) {
+    float p[2 * G];
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      if (i < G - FMA) {
+        f2unpack(t[i], p[2 * i], p[2 * i + 1]);
+        p[2 * i] = ex2(p[2 * i]);
+        p[2 * i + 1] = ex2(p[2 * i + 1]);
+      } else {
+        f2unpack(ex2_fma(t[i]), p[2 * i], p[2 * i + 1]);
+      }
+    }
+    if (g + 1 < 16 / G) arguments(g + 1);
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      sum[i & 1] = fadd2(sum[i & 1], f2pack(p[2 * i], p[2 * i + 1]));
+      w[g * G + i] = pack2<T>(p[2 * i], p[2 * i + 1]);
+    }
   }
 }
 
 // Up to 128 rows of one request and KV head, tiles of 64 keys.  Warp 0 loads K
-// and V (TMA, a ring each), warp 1 issues the MMAs, warp 2 zeroes the V rows of keys
-// that are not attended to (their weights are zero, but zero times NaN is not), and
-// warps 4-7 turn scores into weights, a thread a row.  For tile j:
+// and V (TMA, a ring each), warps 1 and 3 issue the MMAs of S and of O (waits and issue of both
+// in one warp took longer than a tile's exponentials), warp 2 zeroes the V rows of
+// keys that are not attended to (their weights are zero, but zero times NaN is not),
+// and warps 4-7 turn scores into weights, a thread a row.  For tile j:
 //   S(j) = Q K_j^T    M128 N64, both K-major in shared memory
 //   P(j) = weights    TMEM, 16 bits, over S(j)
 //   O += P(j) V_j     M128 N DP, P from TMEM, V MN-major
@@ -445,8 +493,8 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t *sm = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint64_t *k_full = (uint64_t *)(sm + L::kBar), *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST;
-  uint64_t *v_ok = v_empty + ST, *q_full = v_ok + ST, *s_full = q_full + 1, *p_full = s_full + 2, *pv_done = p_full + 1;
-  uint32_t *tmem_slot = (uint32_t *)(pv_done + 1);
+  uint64_t *v_ok = v_empty + ST, *q_full = v_ok + ST, *s_full = q_full + 1, *p_full = s_full + 2, *pv_done = p_full + 2;
+  uint32_t *tmem_slot = (uint32_t *)(pv_done + 2);
   pdl_trigger();
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -465,10 +513,11 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       mbar_init(&v_ok[s], 1);
     }
     mbar_init(q_full, 4);
-    mbar_init(&s_full[0], 1);
-    mbar_init(&s_full[1], 1);
-    mbar_init(p_full, 4);
-    mbar_init(pv_done, 1);
+    for (int b = 0; b < 2; ++b) {  // of even and odd tiles: a wait never lags by two phases
+      mbar_init(&s_full[b], 1);
+      mbar_init(&p_full[b], 4);
+      mbar_init(&pv_done[b], 1);
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
@@ -504,43 +553,44 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       for (int j = max(0, v_done - ST); j < v_done; ++j) mbar_drain(&v_full[j % ST], (uint32_t)((j / ST) & 1));
     }
     __syncwarp();
-  } else if (warp == 1 && nt > 0) {
-    // descriptors share their high word; the low one is the address / 16 (and,
-    // MN-major, the distance of the 64-dimension parts)
+  } else if (warp == 1) {
+    // S(j), where P(j-2) was.  Descriptors share their high word; the low one is
+    // the address / 16 (and, MN-major, the distance of the 64-dimension parts).
+    const uint32_t s16 = smem_u32(sm) >> 4, q16 = (s16 + (uint32_t)(L::kQ >> 4)) | (1u << 16);
+    const uint64_t hi = umma_desc(sm) & 0xFFFFFFFF00000000ull;
+    const int steps = (w.s.D + 15) / 16;
+    if (nt == 0 || warp_wait(q_full, 0, err)) {
+      for (int j = 0; j < nt; ++j) {
+        const int s = j % ST;
+        if (!warp_wait(&k_full[s], (uint32_t)((j / ST) & 1), err)) break;
+        if (j >= 2 && !warp_wait(&pv_done[j & 1], (uint32_t)((j - 2) >> 1) & 1, err)) break;
+        tc_after();
+        const uint32_t k = (s16 + (uint32_t)((L::kK + s * L::kBytes) >> 4)) | (1u << 16);
+        const uint32_t id = f16_idesc<T>(covered(j), false), d = tmem + (uint32_t)((j & 1) * kKeys);
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+          const uint32_t in = (uint32_t)((i & 3) * 2), qa = (i >> 2) * (L::kQAtom >> 4) + in, ka = (i >> 2) * (L::kAtom >> 4) + in;
+          if (i < steps) umma_bf16_e(d, hi | (q16 + qa), hi | (k + ka), id, i ? 1u : 0u);
+        }
+        umma_commit_e(&s_full[j & 1]);
+        umma_commit_e(&k_empty[s]);
+      }
+    }
+  } else if (warp == 3) {
+    // O += P(j) V_j
     const uint32_t s16 = smem_u32(sm) >> 4;
     const uint64_t hi = umma_desc(sm) & 0xFFFFFFFF00000000ull;
-    const uint32_t q16 = (s16 + (uint32_t)(L::kQ >> 4)) | (1u << 16), k16 = s16 + (uint32_t)(L::kK >> 4),
-                   v16 = (s16 + (uint32_t)(L::kV >> 4)) | ((uint32_t)(L::kAtom >> 4) << 16);
-    const int steps = (w.s.D + 15) / 16;
-    auto score = [&](int j) -> bool {  // S(j)
-      const int s = j % ST;
-      if (!warp_wait(&k_full[s], (uint32_t)((j / ST) & 1), err)) return false;
-      tc_after();
-      const uint32_t id = f16_idesc<T>(covered(j), false), k = (k16 + (uint32_t)(s * (L::kBytes >> 4))) | (1u << 16);
-      const uint32_t d = tmem + (uint32_t)((j & 1) * kKeys);
-#pragma unroll
-      for (int i = 0; i < DP / 16; ++i) {
-        const uint32_t in = (uint32_t)((i & 3) * 2), qa = (i >> 2) * (L::kQAtom >> 4) + in, ka = (i >> 2) * (L::kAtom >> 4) + in;
-        if (i < steps) umma_bf16_e(d, hi | (q16 + qa), hi | (k + ka), id, i ? 1u : 0u);
-      }
-      umma_commit_e(&s_full[j & 1]);
-      umma_commit_e(&k_empty[s]);
-      return true;
-    };
-    bool ok = warp_wait(q_full, 0, err) && score(0);
-    for (int j = 0; j < nt && ok; ++j) {
-      // S(j+1) goes where P(j-1) was
-      if (j + 1 < nt) ok = (j == 0 || warp_wait(pv_done, (uint32_t)(j - 1) & 1, err)) && score(j + 1);
+    const uint32_t id = f16_idesc<T>(DP, true);
+    for (int j = 0; j < nt; ++j) {
       const int s = j % ST, n = covered(j) >> 4;
-      ok = ok && warp_wait(&v_ok[s], (uint32_t)((j / ST) & 1), err) && warp_wait(p_full, (uint32_t)j & 1, err);
-      if (!ok) break;
+      if (!warp_wait(&v_ok[s], (uint32_t)((j / ST) & 1), err) || !warp_wait(&p_full[j & 1], (uint32_t)(j >> 1) & 1, err)) break;
       tc_after();
-      const uint32_t id = f16_idesc<T>(DP, true), v = v16 + (uint32_t)(s * (L::kBytes >> 4));
+      const uint32_t v = (s16 + (uint32_t)((L::kV + s * L::kBytes) >> 4)) | ((uint32_t)(L::kAtom >> 4) << 16);
 #pragma unroll
       for (int i = 0; i < kKeys / 16; ++i)
         if (i < n)
           umma_bf16_ts_e(tmem + L::kO, tmem + (uint32_t)((j & 1) * kKeys + 8 * i), hi | (v + 128 * i), id, (j | i) ? 1u : 0u);
-      umma_commit_e(pv_done);
+      umma_commit_e(&pv_done[j & 1]);
       umma_commit_e(&v_empty[s]);
     }
   } else if (warp == 2) {
@@ -618,7 +668,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         l *= f;
       }
       if (j > 0 && __any_sync(0xffffffffu, move)) {
-        if (!(ok = warp_wait(pv_done, (uint32_t)(j - 1) & 1, err))) break;
+        if (!(ok = warp_wait(&pv_done[(j - 1) & 1], (uint32_t)((j - 1) >> 1) & 1, err))) break;
         tc_after();
 #pragma unroll 1
         for (int q = 0; q < DP / 16; ++q) {
@@ -637,7 +687,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       }
       const float mc = m == -INFINITY ? 0.0f : m * sc;
       const uint64_t cc = f2pack(sc, sc), nm = f2pack(-mc, -mc);
-      uint64_t sum = f2pack(0.0f, 0.0f);
+      uint64_t sum[2] = {f2pack(0.0f, 0.0f), f2pack(0.0f, 0.0f)};
 #pragma unroll
       for (int q = 0; q < kKeys / 32; ++q) {
         uint32_t pw[16];
@@ -645,17 +695,14 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         tmem_st16(tS + 16 * q, pw);
       }
       float l0, l1;
-      f2unpack(sum, l0, l1);
+      f2unpack(fadd2(sum[0], sum[1]), l0, l1);
       l += l0 + l1;
       tmem_wait_st();
       tc_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_full);
+      if (lane == 0) mbar_arrive(&p_full[j & 1]);
     }
-    // S(nt - 1) says that PV(nt - 3) is done: the last two phases are waited for in
-    // order, since a wait for one alone would take its predecessor's parity for it
-    if (ok && nt > 1) ok = warp_wait(pv_done, (uint32_t)(nt - 2) & 1, err);
-    if (ok && nt > 0) ok = warp_wait(pv_done, (uint32_t)(nt - 1) & 1, err);
+    if (ok && nt > 0) ok = warp_wait(&pv_done[(nt - 1) & 1], (uint32_t)((nt - 1) >> 1) & 1, err);
     if (ok) {
       tc_after();
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
