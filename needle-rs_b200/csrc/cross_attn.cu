@@ -537,12 +537,12 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       for (int j = 0; j < nt && ok; ++j) {
         const int s = j % ST, row = (int)it.k0 + j * kKeys;
         const uint32_t ph = (uint32_t)((j / ST) & 1) ^ 1;
-        if (!(ok = mbar_wait(&k_empty[s], ph, err))) break;
+        if (!(ok = mbar_sleep_wait(&k_empty[s], ph, err))) break;
         mbar_expect_tx(&k_full[s], L::kBytes);
         for (int a = 0; a < L::kAtoms; ++a)
           tma_load_3d(sm + L::kK + s * L::kBytes + a * L::kAtom, &mk, &k_full[s], 64 * a, it.kvh, row);
         ++k_done;
-        if (!(ok = mbar_wait(&v_empty[s], ph, err))) break;
+        if (!(ok = mbar_sleep_wait(&v_empty[s], ph, err))) break;
         mbar_expect_tx(&v_full[s], L::kBytes);
         for (int a = 0; a < L::kAtoms; ++a)
           tma_load_3d(sm + L::kV + s * L::kBytes + a * L::kAtom, &mv, &v_full[s], 64 * a, it.kvh, row);
@@ -559,11 +559,11 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     const uint32_t s16 = smem_u32(sm) >> 4, q16 = (s16 + (uint32_t)(L::kQ >> 4)) | (1u << 16);
     const uint64_t hi = umma_desc(sm) & 0xFFFFFFFF00000000ull;
     const int steps = (w.s.D + 15) / 16;
-    if (nt == 0 || warp_wait(q_full, 0, err)) {
+    if (nt == 0 || warp_sleep_wait(q_full, 0, err)) {
       for (int j = 0; j < nt; ++j) {
         const int s = j % ST;
-        if (!warp_wait(&k_full[s], (uint32_t)((j / ST) & 1), err)) break;
-        if (j >= 2 && !warp_wait(&pv_done[j & 1], (uint32_t)((j - 2) >> 1) & 1, err)) break;
+        if (!warp_sleep_wait(&k_full[s], (uint32_t)((j / ST) & 1), err)) break;
+        if (j >= 2 && !warp_sleep_wait(&pv_done[j & 1], (uint32_t)((j - 2) >> 1) & 1, err)) break;
         tc_after();
         const uint32_t k = (s16 + (uint32_t)((L::kK + s * L::kBytes) >> 4)) | (1u << 16);
         const uint32_t id = f16_idesc<T>(covered(j), false), d = tmem + (uint32_t)((j & 1) * kKeys);
@@ -583,7 +583,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     const uint32_t id = f16_idesc<T>(DP, true);
     for (int j = 0; j < nt; ++j) {
       const int s = j % ST, n = covered(j) >> 4;
-      if (!warp_wait(&v_ok[s], (uint32_t)((j / ST) & 1), err) || !warp_wait(&p_full[j & 1], (uint32_t)(j >> 1) & 1, err)) break;
+      if (!warp_sleep_wait(&v_ok[s], (uint32_t)((j / ST) & 1), err) || !warp_sleep_wait(&p_full[j & 1], (uint32_t)(j >> 1) & 1, err)) break;
       tc_after();
       const uint32_t v = (s16 + (uint32_t)((L::kV + s * L::kBytes) >> 4)) | ((uint32_t)(L::kAtom >> 4) << 16);
 #pragma unroll
@@ -599,7 +599,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       const bool whole = !mask && (j + 1) * kKeys <= it.klen;
       Live live{};
       if (!whole) live = live_keys(mask, it.klen, j, lane);
-      if (!warp_wait(&v_full[s], (uint32_t)((j / ST) & 1), err)) break;
+      if (!warp_sleep_wait(&v_full[s], (uint32_t)((j / ST) & 1), err)) break;
       if (!whole) {
         const int n = covered(j);
         // 8 lanes a row, 4 rows at a time
@@ -643,7 +643,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       const bool whole = !mask && (j + 1) * kKeys <= it.klen;
       Live live{};
       if (!whole) live = live_keys(mask, it.klen, j, lane);
-      if (!(ok = warp_wait(&s_full[j & 1], (uint32_t)(j >> 1) & 1, err))) break;
+      if (!(ok = warp_sleep_wait(&s_full[j & 1], (uint32_t)(j >> 1) & 1, err))) break;
       tc_after();
       const uint32_t tS = tmem + lanes + (uint32_t)((j & 1) * kKeys);
       uint32_t s[kKeys];
@@ -668,7 +668,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         l *= f;
       }
       if (j > 0 && __any_sync(0xffffffffu, move)) {
-        if (!(ok = warp_wait(&pv_done[(j - 1) & 1], (uint32_t)((j - 1) >> 1) & 1, err))) break;
+        if (!(ok = warp_sleep_wait(&pv_done[(j - 1) & 1], (uint32_t)((j - 1) >> 1) & 1, err))) break;
         tc_after();
 #pragma unroll 1
         for (int q = 0; q < DP / 16; ++q) {
@@ -702,7 +702,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[j & 1]);
     }
-    if (ok && nt > 0) ok = warp_wait(&pv_done[(nt - 1) & 1], (uint32_t)((nt - 1) >> 1) & 1, err);
+    if (ok && nt > 0) ok = warp_sleep_wait(&pv_done[(nt - 1) & 1], (uint32_t)((nt - 1) >> 1) & 1, err);
     if (ok) {
       tc_after();
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
