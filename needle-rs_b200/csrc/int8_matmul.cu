@@ -167,18 +167,43 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, int *v) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+// y = sum * scale + bias, rounded once to the type.
 template <typename TY>
-__device__ __forceinline__ void finish(const Int8Args &a, TY *y, int acc, float s, float bias) {
+__device__ __forceinline__ void finish(TY *y, int acc, float s, float bias) {
   *y = from_f32<TY>(fmaf(__int2float_rn(acc), s, bias));
 }
 
-// Stages of operand tiles in flight: as many as fit 196 KB.
-template <int BT>
-constexpr int kStages = BT <= 64 ? 8 : BT == 128 ? 6 : 4;
-template <int BT>
-constexpr int kStageBytes = (BN + BT) * BK;
-template <int BT>
-constexpr size_t kSmem = (size_t)kStages<BT> * kStageBytes<BT> + 1024 + 256;
+// Stages of operand tiles in flight: as many as fit 196 KB.  The fused form holds
+// only weights in its ring, and the tokens of all of its K beside it.
+template <int BT, bool FUSED>
+constexpr int kStages = FUSED ? 7 : BT <= 64 ? 8 : BT == 128 ? 6 : 4;
+template <int BT, bool FUSED>
+constexpr int kStageBytes = (BN + (FUSED ? 0 : BT)) * BK;
+constexpr int kFusedBlocks = 40;  // blocks of K whose tokens fit beside the ring
+template <int BT, bool FUSED>
+constexpr size_t kSmem = (size_t)kStages<BT, FUSED> * kStageBytes<BT, FUSED> + (FUSED ? kFusedBlocks * 16 * BK : 0) + 1024 + 512;
+
+// 8 elements of a row from k on, as f32, zero past K.
+__device__ __forceinline__ void load8(const Int8Args &a, int64_t row, int k, float *v) {
+  const int64_t at = row * a.ldx + k;
+  if (a.x_vec && k + 8 <= a.K) {
+    if (a.x_dtype == DT_F32)
+      load<8>((const float *)a.x + at, v);
+    else if (a.x_dtype == DT_F16)
+      load<8>((const __half *)a.x + at, v);
+    else
+      load<8>((const __nv_bfloat16 *)a.x + at, v);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    v[j] = 0.0f;
+    if (k + j < a.K)
+      v[j] = a.x_dtype == DT_F32   ? ((const float *)a.x)[at + j]
+             : a.x_dtype == DT_F16 ? (float)((const __half *)a.x)[at + j]
+                                   : (float)((const __nv_bfloat16 *)a.x)[at + j];
+  }
+}
 
 // Warp 0 loads (TMA, a ring of stages), warp 1 allocates TMEM and issues the
 // MMAs, warps 4.. turn sums into results from one of two accumulators while
@@ -187,20 +212,30 @@ constexpr size_t kSmem = (size_t)kStages<BT> * kStageBytes<BT> + 1024 + 256;
 // partial tiles meet in distributed shared memory, CTA r finishing the r-th
 // part of the tokens: the grid then has a cluster for each tile.
 //
-// Under programmatic dependent launch (behind the kernel that rounds the
-// tokens) the set-up and the first weight tiles do not wait for it.
-template <int BT, typename TY>
+// Small products are a chain of latencies, so nothing waits that need not: the
+// thread that initialises the barriers requests the first weight tiles at once,
+// before TMEM is allocated and before the kernel that rounds the tokens is done
+// (programmatic dependent launch), and scales and biases are fetched before the sums.
+//
+// FUSED (up to 16 tokens): no such kernel.  Every CTA finds the rows' maxima
+// itself and rounds its part of K into the MMA's operand layout while its
+// weights arrive: the tokens are few enough to be read by every CTA, and a
+// launch costs more.
+template <int BT, typename TY, bool FUSED>
 __global__ void __launch_bounds__(384, 1)
     int8_tc_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ CUtensorMap mq, Int8Args a, int split,
                    int *err) {
-  constexpr int STAGES = kStages<BT>, BYTES = kStageBytes<BT>, W_BYTES = BN * BK;
+  constexpr int STAGES = kStages<BT, FUSED>, BYTES = kStageBytes<BT, FUSED>, W_BYTES = BN * BK;
   constexpr uint32_t IDESC = i8_idesc(BN, BT);
   constexpr int COLS = 2 * BT;  // TMEM columns: two accumulators
+  constexpr int HALF = BT / 2 < 16 ? 16 : BT / 2;  // tokens of an epilogue warpgroup (16: the second has none)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  uint64_t *full = (uint64_t *)(smem + STAGES * BYTES), *empty = full + STAGES;
+  uint8_t *tokens = smem + STAGES * BYTES;  // FUSED: [block of K][16 rows][128 bytes]
+  uint64_t *full = (uint64_t *)(tokens + (FUSED ? kFusedBlocks * 16 * BK : 0)), *empty = full + STAGES;
   uint64_t *tfull = empty + STAGES, *tempty = tfull + 2;
-  uint32_t *tmem_slot = (uint32_t *)(tempty + 2);
+  uint32_t *tmem_slot = (uint32_t *)(tempty + 2), *tops = tmem_slot + 2;  // tops: [12 warps]
+  float *scales = (float *)(tops + 12);                                   // FUSED: [16]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = split > 1 ? (int)cluster_ctarank() : 0;
@@ -209,8 +244,11 @@ __global__ void __launch_bounds__(384, 1)
   const int first = blockIdx.x / split, step = gridDim.x / split;
   const int nkb = (a.K + BK - 1) / BK;
   const int kb0 = (int)((int64_t)nkb * rank / split), kb1 = (int)((int64_t)nkb * (rank + 1) / split);
+  const int burst = min(STAGES, kb1 - kb0);
 
   if (threadIdx.x == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mw) : "memory");
+    if (!FUSED) asm volatile("prefetch.tensormap [%0];" ::"l"(&mq) : "memory");
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
@@ -220,11 +258,58 @@ __global__ void __launch_bounds__(384, 1)
       mbar_init(&tempty[b], 8);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_smem();
+    for (int i = 0; i < burst; ++i) {
+      mbar_expect_tx(&full[i], BYTES);
+      tma_load_2d(smem + i * BYTES, &mw, &full[i], (kb0 + i) * BK, (first % num_n) * BN);
+    }
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                  "r"(COLS));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  __syncwarp();
+  if (FUSED) {
+    // the rows' maxima: a row by as many warps as there are for each
+    const int wpr = max(1, 12 / a.M), groups = 12 / wpr, group = warp / wpr;
+    for (int r0 = 0; r0 < a.M; r0 += groups) {
+      const int r = r0 + group;
+      uint32_t top = 0;
+      if (group < groups && r < a.M)
+        for (int k = (warp % wpr * 32 + lane) * 8; k < a.K; k += wpr * 256) {
+          float v[8];
+          load8(a, r, k, v);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) top = max(top, abs_bits(v[j]));
+        }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (lane == 0) tops[warp] = top;
+      __syncthreads();
+      if (threadIdx.x < groups && r0 + (int)threadIdx.x < a.M) {
+        uint32_t t = 0;
+        for (int i = 0; i < wpr; ++i) t = max(t, tops[threadIdx.x * wpr + i]);
+        const RowScale rs = int8_row_scale(t);
+        scales[r0 + threadIdx.x] = rs.scale;
+        scales[16 + r0 + threadIdx.x] = rs.inv;
+      }
+      __syncthreads();
+    }
+    // this CTA's part of K, rows past M zero, in the swizzled layout
+    const int chunks = (kb1 - kb0) * (BK / 8);  // of 8 values
+    for (int u = threadIdx.x; u < 16 * chunks; u += blockDim.x) {
+      const int r = u / chunks, c = u % chunks, blk = c / (BK / 8), in = c % (BK / 8);
+      uint2 w = make_uint2(0, 0);
+      if (r < a.M) {
+        float v[8];
+        load8(a, r, kb0 * BK + c * 8, v);
+        const float inv = scales[16 + r];
+        w = make_uint2(int8_pack4(v, inv), int8_pack4(v + 4, inv));
+      }
+      *reinterpret_cast<uint2 *>(tokens + blk * 16 * BK + r * BK + (((in >> 1) ^ (r & 7)) << 4) + (in & 1) * 8) = w;
+    }
+    fence_async_smem();
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
@@ -233,87 +318,93 @@ __global__ void __launch_bounds__(384, 1)
 
   if (warp == 0) {
     if (lane == 0) {
-      int64_t issued = 0;  // stages requested so far
-      bool ok = true, waited = false;
-      for (int64_t t = first; t < tiles && ok; t += step) {
+      if (!FUSED) {
+        pdl_wait();  // the tokens
+        for (int i = 0; i < burst; ++i)
+          tma_load_2d(smem + i * BYTES + W_BYTES, &mq, &full[i], (kb0 + i) * BK, (first / num_n) * BT);
+      }
+      int s = burst == STAGES ? 0 : burst, issued = burst;  // issued: up to STAGES
+      uint32_t ph = burst == STAGES ? 1 : 0;
+      int kb = kb0 + burst;
+      bool ok = true;
+      for (int64_t t = first; t < tiles && ok; t += step, kb = kb0) {
         const int n0 = (int)(t % num_n) * BN, m0 = (int)(t / num_n) * BT;
-        for (int kb = kb0; kb < kb1;) {
-          // the weight tiles of as many stages as are free at the start; then one stage at a time
-          const int burst = waited ? 1 : min(STAGES, kb1 - kb);
-          for (int i = 0; i < burst && ok; ++i) {
-            const int s = (int)((issued + i) % STAGES);
-            ok = mbar_wait(&empty[s], (uint32_t)(((issued + i) / STAGES) & 1) ^ 1, err);
-            if (!ok) break;
-            mbar_expect_tx(&full[s], BYTES);
-            tma_load_2d(smem + s * BYTES, &mw, &full[s], (kb + i) * BK, n0);
-          }
-          if (!ok) break;
-          if (!waited) pdl_wait();  // the tokens
-          waited = true;
-          for (int i = 0; i < burst; ++i) {
-            const int s = (int)((issued + i) % STAGES);
-            tma_load_2d(smem + s * BYTES + W_BYTES, &mq, &full[s], (kb + i) * BK, m0);
-          }
-          kb += burst;
-          issued += burst;
+        for (; kb < kb1; ++kb) {
+          if (!(ok = mbar_wait(&empty[s], ph ^ 1, err))) break;
+          mbar_expect_tx(&full[s], BYTES);
+          tma_load_2d(smem + s * BYTES, &mw, &full[s], kb * BK, n0);
+          if (!FUSED) tma_load_2d(smem + s * BYTES + W_BYTES, &mq, &full[s], kb * BK, m0);
+          issued = min(issued + 1, STAGES);
+          if (++s == STAGES) s = 0, ph ^= 1;
         }
       }
       // no copy may be in flight when the CTA leaves
-      for (int64_t i = max((int64_t)0, issued - STAGES); i < issued; ++i)
-        mbar_drain(&full[i % STAGES], (uint32_t)((i / STAGES) & 1));
+      for (int i = 0; i < issued; ++i) {
+        if (s-- == 0) s = STAGES - 1, ph ^= 1;
+        mbar_drain(&full[s], ph);
+      }
     }
     __syncwarp();
   } else if (warp == 1) {
-    int64_t used = 0;
-    int i = 0;
+    int s = 0, i = 0;
+    uint32_t ph = 0;
     bool ok = true;
     for (int64_t t = first; t < tiles && ok; t += step, ++i) {
       const int buf = i & 1;
-      if (!(ok = warp_wait(&tempty[buf], ((i >> 1) & 1) ^ 1, err))) break;
+      if (i >= 2 && !(ok = warp_wait(&tempty[buf], ((i >> 1) & 1) ^ 1, err))) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t d = tmem + (uint32_t)(buf * BT);
-      for (int kb = kb0; kb < kb1; ++kb, ++used) {
-        const int s = (int)(used % STAGES);
-        if (!(ok = warp_wait(&full[s], (uint32_t)((used / STAGES) & 1), err))) break;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!(ok = warp_wait(&full[s], ph, err))) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint64_t dw = umma_desc(smem + s * BYTES), dq = umma_desc(smem + s * BYTES + W_BYTES);
+        const uint64_t dw = umma_desc(smem + s * BYTES);
+        const uint64_t dq = umma_desc(FUSED ? tokens + (kb - kb0) * 16 * BK : smem + s * BYTES + W_BYTES);
 #pragma unroll
         for (int k = 0; k < BK / 32; ++k)
           mma_i8(d, dw + 2 * k, dq + 2 * k, IDESC, (kb > kb0 || k) ? 1u : 0u);  // 32 bytes: 2 in descriptor units
         umma_commit_e(&empty[s]);
+        if (++s == STAGES) s = 0, ph ^= 1;
       }
       if (ok) umma_commit_e(&tfull[buf]);
     }
   } else if (warp >= 4) {
-    const int quarter = warp & 3, half = (warp - 4) >> 2;  // TMEM lanes, columns
-    constexpr int HALF = BT / 2 < 16 ? 16 : BT / 2;        // 16 columns leave the second warpgroup idle
-    pdl_wait();                                            // the tokens' scales
+    const int quarter = warp & 3, half = (warp - 4) >> 2;  // TMEM lanes, tokens
+    if (!FUSED) pdl_wait();                                // the tokens' scales
     int i = 0;
     for (int64_t t = first; t < tiles; t += step, ++i) {
       const int buf = i & 1;
-      const int n = (int)(t % num_n) * BN + quarter * 32 + lane, m0 = (int)(t / num_n) * BT;
+      const int n = (int)(t % num_n) * BN + quarter * 32 + lane, m0 = (int)(t / num_n) * BT + half * HALF;
       const bool in = n < a.N;
       const float sw = in ? a.w_scales[n] : 0.0f, bias = in && a.bias ? a.bias[n] : 0.0f;
+      float sq[(HALF + 31) / 32];
+#pragma unroll
+      for (int q = 0; q < (HALF + 31) / 32; ++q) {
+        const int m = m0 + 32 * q + lane;
+        sq[q] = 32 * q + lane < HALF && m < a.M ? (FUSED ? scales[m] : a.q_scales[m]) : 0.0f;
+      }
       if (!warp_wait(&tfull[buf], (uint32_t)((i >> 1) & 1), err)) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint32_t base = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BT);
-      for (int c = half * HALF; c < min((half + 1) * HALF, BT); c += 16) {
-        int v[16];
-        tmem_ld16(base + c, v);
-        if (split == 1) {
-          const int m = m0 + c;
-          if (m >= a.M) break;
-          const float sq = lane < 16 && m + lane < a.M ? a.q_scales[m + lane] : 0.0f;
-          TY *y = (TY *)a.y + (int64_t)m * a.ldy + n;
+      const uint32_t base = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BT + half * HALF);
+      if (half * HALF < BT) {
+        const int left = a.M - m0;  // tokens from here on
+        TY *y = (TY *)a.y + (int64_t)m0 * a.ldy + n;
+#pragma unroll
+        for (int c = 0; c < HALF; c += 16) {
+          if (c >= left && split == 1) break;
+          int v[16];
+          tmem_ld16(base + c, v);
+          if (split > 1) {  // over the operand ring, which is drained: every MMA that read it has completed
+            int *part = reinterpret_cast<int *>(smem) + (half * HALF + c) * BN + quarter * 32 + lane;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) part[j * BN] = v[j];
+            continue;
+          }
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            const float s = __shfl_sync(0xffffffffu, sq, j) * sw;
-            if (in && m + j < a.M) finish(a, y + j * a.ldy, v[j], s, bias);
+            const float s = __shfl_sync(0xffffffffu, sq[c >> 5], (c & 31) + j) * sw;
+            if (in && c + j < left) finish(y, v[j], s, bias);
+            y += a.ldy;
           }
-        } else {  // over the operand ring, which is drained: every MMA that read it has completed
-          int *part = reinterpret_cast<int *>(smem);
-#pragma unroll
-          for (int j = 0; j < 16; ++j) part[(c + j) * BN + quarter * 32 + lane] = v[j];
         }
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -325,23 +416,43 @@ __global__ void __launch_bounds__(384, 1)
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if (split > 1) {
-    cluster_sync();
+    // this CTA's tokens of the tile: 4 channels a thread, all CTAs' parts at once
     const int n0 = (first % num_n) * BN, m0 = (first / num_n) * BT;
-    const int c0 = BT * rank / split, c1 = BT * (rank + 1) / split;
+    const int c0 = BT * rank / split, units = (BT / split) * (BN / 4);
     const uint32_t mine = smem_u32(smem);
-    for (int u = c0 * BN + threadIdx.x; u < c1 * BN; u += blockDim.x) {
-      const int c = u / BN, n = n0 + u % BN, m = m0 + c;
-      int acc = 0;
-      for (int r = 0; r < split; ++r) {
-        uint32_t at;
-        int v;
-        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(mine + 4u * (uint32_t)u), "r"(r));
-        asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
-        acc += v;
+    cluster_sync();
+    for (int u = threadIdx.x; u < units; u += blockDim.x) {
+      const int c = c0 + u / (BN / 4), in = u % (BN / 4) * 4, n = n0 + in, m = m0 + c;
+      if (m >= a.M) break;  // the later units are of later tokens
+      int4 part[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r < split) {
+          uint32_t at;
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(mine + 4u * (uint32_t)(c * BN + in)), "r"(r));
+          asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(part[r].x), "=r"(part[r].y), "=r"(part[r].z), "=r"(part[r].w)
+                       : "r"(at)
+                       : "memory");
+        }
+      const float sq = FUSED ? scales[m] : a.q_scales[m];
+      float sw[4], bias[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        sw[j] = n + j < a.N ? a.w_scales[n + j] : 0.0f;
+        bias[j] = n + j < a.N && a.bias ? a.bias[n + j] : 0.0f;
       }
-      if (n < a.N && m < a.M)
-        finish(a, (TY *)a.y + (int64_t)m * a.ldy + n, acc, a.q_scales[m] * a.w_scales[n], a.bias ? a.bias[n] : 0.0f);
+      int4 acc = part[0];
+#pragma unroll
+      for (int r = 1; r < 8; ++r)
+        if (r < split) acc.x += part[r].x, acc.y += part[r].y, acc.z += part[r].z, acc.w += part[r].w;
+      const int sums[4] = {acc.x, acc.y, acc.z, acc.w};
+      TY *y = (TY *)a.y + (int64_t)m * a.ldy + n;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (n + j < a.N) finish(y + j, sums[j], sq * sw[j], bias[j]);
     }
+    __syncwarp();
     cluster_sync();  // no CTA leaves while another reads its part
   }
   if (warp == 1) {
@@ -356,24 +467,24 @@ cudaError_t row_map(CUtensorMap *map, const int8_t *p, int64_t rows, int K, int 
   return tma_map_tiled(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, p, dims, strides, box);
 }
 
-template <int BT, typename TY>
+template <int BT, typename TY, bool FUSED>
 cudaError_t launch_tc(const Int8Args &a, int split, int sms, bool pdl, int *err, cudaStream_t st) {
   static thread_local int ready = -1;  // device whose kernel attributes are set
-  auto *kernel = int8_tc_kernel<BT, TY>;
+  auto *kernel = int8_tc_kernel<BT, TY, FUSED>;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && ready != dev) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem<BT>);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem<BT, FUSED>);
     if (e == cudaSuccess) ready = dev;
   }
-  CUtensorMap mq;
-  if (e == cudaSuccess) e = row_map(&mq, a.q, a.M, a.K, BT);
+  CUtensorMap mq = *a.w_map;
+  if (e == cudaSuccess && !FUSED) e = row_map(&mq, a.q, a.M, a.K, BT);
   if (e != cudaSuccess) return e;
   const int64_t tiles = (int64_t)((a.N + BN - 1) / BN) * ((a.M + BT - 1) / BT);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(split > 1 ? tiles * split : std::min<int64_t>(tiles, sms)));
   cfg.blockDim = dim3(384);
-  cfg.dynamicSmemBytes = kSmem<BT>;
+  cfg.dynamicSmemBytes = kSmem<BT, FUSED>;
   cfg.stream = st;
   cudaLaunchAttribute at[2];
   if (split > 1) {
@@ -388,33 +499,52 @@ cudaError_t launch_tc(const Int8Args &a, int split, int sms, bool pdl, int *err,
   return cudaLaunchKernelEx(&cfg, kernel, *a.w_map, mq, a, split, err);
 }
 
+// Tokens of a tile and CTAs that share one: the least estimated time, in
+// clocks of an SM that takes in about 64 bytes each from L2, which is what
+// binds: the waves of tiles, each the bytes of its stages and a start and end of
+// about 2,000 clocks, and as much again for the CTAs of a cluster to meet.
+struct Shape {
+  int bt, split;
+};
+Shape choose_shape(int M, int N, int K, int sms) {
+  const int num_n = (N + BN - 1) / BN, nkb = (K + BK - 1) / BK;
+  Shape best{16, 1};
+  int64_t least = INT64_MAX;
+  for (int b = 256; b >= 16; b /= 2) {
+    const int64_t tiles = (int64_t)num_n * ((M + b - 1) / b);
+    for (int s = 1; s <= (b <= 128 ? 8 : 1) && s <= nkb && (s == 1 || tiles * s <= sms); s *= 2) {
+      const int64_t waves = (tiles * s + sms - 1) / sms;
+      const int64_t cost = waves * ((BN + b) * 2 * ((nkb + s - 1) / s)) + 2000 + (s > 1 ? 1000 + b * 16 / s : 0) + b * 8;
+      if (cost < least) least = cost, best = Shape{b, s};
+    }
+  }
+  return best;
+}
+
+// Whether a product of unrounded tokens takes the fused kernel: one tile of 16
+// tokens, few enough bytes for every CTA to read them all (one token's 32,768
+// f32), and a part of K that fits beside the weights' ring.
+bool fuses(const Shape &sh, int M, int K, int dtype) {
+  const int nkb = (K + BK - 1) / BK;
+  return sh.bt == 16 && M <= 16 && (int64_t)M * K * (int64_t)dtype_size(dtype) <= (128 << 10) &&
+         (nkb + sh.split - 1) / sh.split <= kFusedBlocks;
+}
+
 template <typename TY>
 cudaError_t product(const Int8Args &a, bool pdl, int *err, cudaStream_t st) {
   int dev = 0, sms = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e != cudaSuccess) return e;
-  const int num_n = (a.N + BN - 1) / BN, nkb = (a.K + BK - 1) / BK;
-  // Tokens of a tile and CTAs that share one: the least estimated time, in
-  // clocks of an SM that takes in about 64 bytes each from L2, which is what
-  // binds: the waves of tiles, each the bytes of its stages and a start and end of
-  // about 2,000 clocks, and as much again for the CTAs of a cluster to meet.
-  int bt = 16, split = 1;
-  int64_t best = INT64_MAX;
-  for (int b = 256; b >= 16; b /= 2) {
-    const int64_t tiles = (int64_t)num_n * ((a.M + b - 1) / b);
-    for (int s = 1; s <= (b <= 128 ? 8 : 1) && s <= nkb && (s == 1 || tiles * s <= sms); s *= 2) {
-      const int64_t waves = (tiles * s + sms - 1) / sms;
-      const int64_t cost = waves * ((BN + b) * 2 * ((nkb + s - 1) / s)) + 2000 + (s > 1 ? 1000 + b * 16 / s : 0) + b * 8;
-      if (cost < best) best = cost, bt = b, split = s;
-    }
-  }
-  switch (bt) {
-    case 16: return launch_tc<16, TY>(a, split, sms, pdl, err, st);
-    case 32: return launch_tc<32, TY>(a, split, sms, pdl, err, st);
-    case 64: return launch_tc<64, TY>(a, split, sms, pdl, err, st);
-    case 128: return launch_tc<128, TY>(a, split, sms, pdl, err, st);
-    default: return launch_tc<256, TY>(a, split, sms, pdl, err, st);
+  const Shape sh = choose_shape(a.M, a.N, a.K, sms);
+  switch (sh.bt) {
+    case 16:
+      return a.x ? launch_tc<16, TY, true>(a, sh.split, sms, false, err, st)
+                 : launch_tc<16, TY, false>(a, sh.split, sms, pdl, err, st);
+    case 32: return launch_tc<32, TY, false>(a, sh.split, sms, pdl, err, st);
+    case 64: return launch_tc<64, TY, false>(a, sh.split, sms, pdl, err, st);
+    case 128: return launch_tc<128, TY, false>(a, sh.split, sms, pdl, err, st);
+    default: return launch_tc<256, TY, false>(a, sh.split, sms, pdl, err, st);
   }
 }
 
@@ -442,6 +572,13 @@ cudaError_t int8_quantize_cols(const void *w, int dtype, int64_t K, int64_t N, i
 }
 
 cudaError_t int8_weight_map(CUtensorMap *map, const int8_t *w, int64_t N, int K) { return row_map(map, w, N, K, BN); }
+
+bool int8_matmul_fuses(int M, int N, int K, int x_dtype) {
+  int dev = 0, sms = 0;
+  return cudaGetDevice(&dev) == cudaSuccess &&
+         cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess &&
+         fuses(choose_shape(M, N, K, sms), M, K, x_dtype);
+}
 
 cudaError_t int8_matmul(const Int8Args &a, bool pdl, int *err, cudaStream_t st) {
   if (a.y_dtype == DT_F32) return product<float>(a, pdl, err, st);

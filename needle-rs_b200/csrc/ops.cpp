@@ -224,6 +224,14 @@ int needle_int8_plan_matmul(NeedleInt8Plan *p, const void *x, int x_dtype, size_
     OnDevice on(p->device);
     if (!on.good() || !all_on(p->device, {{"x", x}, {"y", y}, {"bias", bias}})) return false;
     cudaStream_t st = (cudaStream_t)stream;
+    if (int8_matmul_fuses((int)M, p->N, p->K, x_dtype)) {
+      Int8Args a{nullptr, &p->w_map, nullptr, p->w_scales, bias, y, (int64_t)ldy, (int)M, p->N, p->K, y_dtype};
+      a.x = x;
+      a.ldx = (int64_t)ldx;
+      a.x_dtype = x_dtype;
+      a.x_vec = aligned(x, 16) && ldx * dtype_size(x_dtype) % 16 == 0;
+      return ok(int8_matmul(a, false, p->flag, st));
+    }
     return ok(int8_quantize_rows(x, x_dtype, (int64_t)M, p->K, (int64_t)ldx, p->q, p->q_scales, st)) &&
            int8_product(p, p->q, p->q_scales, M, bias, y, y_dtype, ldy, true, st);
   }) ? 0 : -1;

@@ -28,14 +28,21 @@ cudaError_t int8_quantize_rows(const void *x, int dtype, int64_t M, int64_t K, i
 cudaError_t int8_quantize_cols(const void *w, int dtype, int64_t K, int64_t N, int8_t *data, float *scales,
                                cudaStream_t st);
 struct Int8Args {
-  const int8_t *q;                   // [M][Kp]
+  const int8_t *q;                   // [M][Kp], or NULL with x set
   const CUtensorMap *w_map;          // of the weight [N][Kp] (host)
   const float *q_scales, *w_scales;  // [M], [N]
   const float *bias;                 // [N] or NULL
   void *y;                           // [M][ldy] of y_dtype
   int64_t ldy;
   int M, N, K, y_dtype;
+  // unrounded tokens [M][ldx] for the kernel that rounds them itself
+  const void *x = nullptr;
+  int64_t ldx = 0;
+  int x_dtype = 0;
+  bool x_vec = false;  // rows on 16-byte boundaries
 };
+// Whether int8_matmul takes unrounded tokens of these sizes (few of them).
+bool int8_matmul_fuses(int M, int N, int K, int x_dtype);
 // TMA descriptor of a weight [N][Kp], 16-byte aligned.
 cudaError_t int8_weight_map(CUtensorMap *map, const int8_t *w, int64_t N, int K);
 // *err is set if a bounded wait inside the kernel expired.  pdl: the kernel
