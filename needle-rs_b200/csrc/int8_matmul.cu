@@ -156,6 +156,17 @@ __device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint3
       "l"(a), "l"(b), "r"(idesc), "r"(acc));
 }
 
+// The same over a CTA pair: rows of A and of B split between the CTAs' shared
+// memory at the same offsets, rows of D between their TMEM.
+__device__ __forceinline__ void mma_i8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+
 // 16 columns of this warp's TMEM lanes.
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, int *v) {
   asm volatile(
@@ -171,6 +182,38 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, int *v) {
 template <typename TY>
 __device__ __forceinline__ void finish(TY *y, int acc, float s, float bias) {
   *y = from_f32<TY>(fmaf(__int2float_rn(acc), s, bias));
+}
+
+// Scales of the NC tokens from m0 on: lane l holds tokens l, l + 32, ...
+template <int NC>
+__device__ __forceinline__ void token_scales(const float *scales, int m0, int M, int lane, float *sq) {
+#pragma unroll
+  for (int q = 0; q < (NC + 31) / 32; ++q) {
+    const int m = m0 + 32 * q + lane;
+    sq[q] = 32 * q + lane < NC && m < M ? scales[m] : 0.0f;
+  }
+}
+
+// Results of NC tokens from m0 on and this lane's channel n, from NC columns of its
+// TMEM lane.
+template <int NC, typename TY>
+__device__ __forceinline__ void store_tokens(const Int8Args &a, uint32_t taddr, int m0, int n, float sw, float bias,
+                                             const float *sq) {
+  const int left = a.M - m0;
+  const bool in = n < a.N;
+  TY *y = (TY *)a.y + (int64_t)m0 * a.ldy + n;
+#pragma unroll
+  for (int c = 0; c < NC; c += 16) {
+    if (c >= left) break;
+    int v[16];
+    tmem_ld16(taddr + c, v);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const float s = __shfl_sync(0xffffffffu, sq[c >> 5], (c & 31) + j) * sw;
+      if (in && c + j < left) finish(y, v[j], s, bias);
+      y += a.ldy;
+    }
+  }
 }
 
 // Stages of operand tiles in flight: as many as fit 196 KB.  The fused form holds
@@ -223,7 +266,7 @@ __device__ __forceinline__ void load8(const Int8Args &a, int64_t row, int k, flo
 // launch costs more.
 template <int BT, typename TY, bool FUSED>
 __global__ void __launch_bounds__(384, 1)
-    int8_tc_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ CUtensorMap mq, Int8Args a, int split,
+    int8_tc_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ CUtensorMap mq, Int8Args a, int lg,
                    int *err) {
   constexpr int STAGES = kStages<BT, FUSED>, BYTES = kStageBytes<BT, FUSED>, W_BYTES = BN * BK;
   constexpr uint32_t IDESC = i8_idesc(BN, BT);
@@ -238,12 +281,12 @@ __global__ void __launch_bounds__(384, 1)
   float *scales = (float *)(tops + 12);                                   // FUSED: [16]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = split > 1 ? (int)cluster_ctarank() : 0;
+  const int split = 1 << lg, rank = lg ? (int)cluster_ctarank() : 0;
   const int num_n = (a.N + BN - 1) / BN, num_t = (a.M + BT - 1) / BT;
-  const int64_t tiles = (int64_t)num_n * num_t;
-  const int first = blockIdx.x / split, step = gridDim.x / split;
+  const int tiles = num_n * num_t;
+  const int first = (int)blockIdx.x >> lg, step = (int)gridDim.x >> lg;
   const int nkb = (a.K + BK - 1) / BK;
-  const int kb0 = (int)((int64_t)nkb * rank / split), kb1 = (int)((int64_t)nkb * (rank + 1) / split);
+  const int kb0 = (nkb * rank) >> lg, kb1 = (nkb * (rank + 1)) >> lg;
   const int burst = min(STAGES, kb1 - kb0);
 
   if (threadIdx.x == 0) {
@@ -296,19 +339,17 @@ __global__ void __launch_bounds__(384, 1)
       }
       __syncthreads();
     }
-    // this CTA's part of K, rows past M zero, in the swizzled layout
+    // this CTA's part of K in the swizzled layout; the rows past M hold anything,
+    // which reaches no token that is stored
     const int chunks = (kb1 - kb0) * (BK / 8);  // of 8 values
-    for (int u = threadIdx.x; u < 16 * chunks; u += blockDim.x) {
-      const int r = u / chunks, c = u % chunks, blk = c / (BK / 8), in = c % (BK / 8);
-      uint2 w = make_uint2(0, 0);
-      if (r < a.M) {
+    for (int r = 0; r < a.M; ++r)
+      for (int c = threadIdx.x; c < chunks; c += blockDim.x) {
         float v[8];
         load8(a, r, kb0 * BK + c * 8, v);
         const float inv = scales[16 + r];
-        w = make_uint2(int8_pack4(v, inv), int8_pack4(v + 4, inv));
+        *reinterpret_cast<uint2 *>(tokens + (c / 16) * 16 * BK + r * BK + (((c % 16 >> 1) ^ (r & 7)) << 4) + (c & 1) * 8) =
+            make_uint2(int8_pack4(v, inv), int8_pack4(v + 4, inv));
       }
-      *reinterpret_cast<uint2 *>(tokens + blk * 16 * BK + r * BK + (((in >> 1) ^ (r & 7)) << 4) + (in & 1) * 8) = w;
-    }
     fence_async_smem();
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -327,8 +368,8 @@ __global__ void __launch_bounds__(384, 1)
       uint32_t ph = burst == STAGES ? 1 : 0;
       int kb = kb0 + burst;
       bool ok = true;
-      for (int64_t t = first; t < tiles && ok; t += step, kb = kb0) {
-        const int n0 = (int)(t % num_n) * BN, m0 = (int)(t / num_n) * BT;
+      for (int t = first; t < tiles && ok; t += step, kb = kb0) {
+        const int n0 = t % num_n * BN, m0 = t / num_n * BT;
         for (; kb < kb1; ++kb) {
           if (!(ok = mbar_wait(&empty[s], ph ^ 1, err))) break;
           mbar_expect_tx(&full[s], BYTES);
@@ -349,7 +390,11 @@ __global__ void __launch_bounds__(384, 1)
     int s = 0, i = 0;
     uint32_t ph = 0;
     bool ok = true;
-    for (int64_t t = first; t < tiles && ok; t += step, ++i) {
+    // descriptors: a common high word, the address / 16 in the low one (a block
+    // of 16 tokens is 16 * BK / 16 = BK units)
+    const uint64_t hi = umma_desc(smem) & 0xFFFFFFFF00000000ull;
+    const uint32_t w16 = (smem_u32(smem) >> 4) | (1u << 16), t16 = (smem_u32(tokens) >> 4) | (1u << 16);
+    for (int t = first; t < tiles && ok; t += step, ++i) {
       const int buf = i & 1;
       if (i >= 2 && !(ok = warp_wait(&tempty[buf], ((i >> 1) & 1) ^ 1, err))) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -357,11 +402,10 @@ __global__ void __launch_bounds__(384, 1)
       for (int kb = kb0; kb < kb1; ++kb) {
         if (!(ok = warp_wait(&full[s], ph, err))) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint64_t dw = umma_desc(smem + s * BYTES);
-        const uint64_t dq = umma_desc(FUSED ? tokens + (kb - kb0) * 16 * BK : smem + s * BYTES + W_BYTES);
+        const uint32_t dw = w16 + (uint32_t)(s * (BYTES >> 4)), dq = FUSED ? t16 + (uint32_t)((kb - kb0) * BK) : dw + (W_BYTES >> 4);
 #pragma unroll
         for (int k = 0; k < BK / 32; ++k)
-          mma_i8(d, dw + 2 * k, dq + 2 * k, IDESC, (kb > kb0 || k) ? 1u : 0u);  // 32 bytes: 2 in descriptor units
+          mma_i8(d, hi | (dw + 2 * k), hi | (dq + 2 * k), IDESC, (kb > kb0 || k) ? 1u : 0u);  // 32 bytes: 2 units
         umma_commit_e(&empty[s]);
         if (++s == STAGES) s = 0, ph ^= 1;
       }
@@ -371,40 +415,27 @@ __global__ void __launch_bounds__(384, 1)
     const int quarter = warp & 3, half = (warp - 4) >> 2;  // TMEM lanes, tokens
     if (!FUSED) pdl_wait();                                // the tokens' scales
     int i = 0;
-    for (int64_t t = first; t < tiles; t += step, ++i) {
+    for (int t = first; t < tiles; t += step, ++i) {
       const int buf = i & 1;
-      const int n = (int)(t % num_n) * BN + quarter * 32 + lane, m0 = (int)(t / num_n) * BT + half * HALF;
+      const int n = t % num_n * BN + quarter * 32 + lane, m0 = t / num_n * BT + half * HALF;
       const bool in = n < a.N;
       const float sw = in ? a.w_scales[n] : 0.0f, bias = in && a.bias ? a.bias[n] : 0.0f;
       float sq[(HALF + 31) / 32];
-#pragma unroll
-      for (int q = 0; q < (HALF + 31) / 32; ++q) {
-        const int m = m0 + 32 * q + lane;
-        sq[q] = 32 * q + lane < HALF && m < a.M ? (FUSED ? scales[m] : a.q_scales[m]) : 0.0f;
-      }
+      token_scales<HALF>(FUSED ? scales : a.q_scales, m0, a.M, lane, sq);
       if (!warp_wait(&tfull[buf], (uint32_t)((i >> 1) & 1), err)) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t base = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BT + half * HALF);
-      if (half * HALF < BT) {
-        const int left = a.M - m0;  // tokens from here on
-        TY *y = (TY *)a.y + (int64_t)m0 * a.ldy + n;
+      if (half * HALF >= BT) {
+      } else if (split == 1) {
+        store_tokens<HALF, TY>(a, base, m0, n, sw, bias, sq);
+      } else {  // over the operand ring, which is drained: every MMA that read it has completed
 #pragma unroll
         for (int c = 0; c < HALF; c += 16) {
-          if (c >= left && split == 1) break;
           int v[16];
           tmem_ld16(base + c, v);
-          if (split > 1) {  // over the operand ring, which is drained: every MMA that read it has completed
-            int *part = reinterpret_cast<int *>(smem) + (half * HALF + c) * BN + quarter * 32 + lane;
+          int *part = reinterpret_cast<int *>(smem) + (half * HALF + c) * BN + quarter * 32 + lane;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) part[j * BN] = v[j];
-            continue;
-          }
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float s = __shfl_sync(0xffffffffu, sq[c >> 5], (c & 31) + j) * sw;
-            if (in && c + j < left) finish(y, v[j], s, bias);
-            y += a.ldy;
-          }
+          for (int j = 0; j < 16; ++j) part[j * BN] = v[j];
         }
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -418,12 +449,20 @@ __global__ void __launch_bounds__(384, 1)
   if (split > 1) {
     // this CTA's tokens of the tile: 4 channels a thread, all CTAs' parts at once
     const int n0 = (first % num_n) * BN, m0 = (first / num_n) * BT;
-    const int c0 = BT * rank / split, units = (BT / split) * (BN / 4);
+    const int c0 = (BT * rank) >> lg, units = (BT >> lg) * (BN / 4);
     const uint32_t mine = smem_u32(smem);
+    const int in = (int)threadIdx.x % (BN / 4) * 4, n = n0 + in;  // the same channels in every turn
+    float sw[4], bias[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      sw[j] = n + j < a.N ? a.w_scales[n + j] : 0.0f;
+      bias[j] = n + j < a.N && a.bias ? a.bias[n + j] : 0.0f;
+    }
     cluster_sync();
     for (int u = threadIdx.x; u < units; u += blockDim.x) {
-      const int c = c0 + u / (BN / 4), in = u % (BN / 4) * 4, n = n0 + in, m = m0 + c;
+      const int c = c0 + u / (BN / 4), m = m0 + c;
       if (m >= a.M) break;  // the later units are of later tokens
+      const float sq = FUSED ? scales[m] : a.q_scales[m];
       int4 part[8];
 #pragma unroll
       for (int r = 0; r < 8; ++r)
@@ -435,13 +474,6 @@ __global__ void __launch_bounds__(384, 1)
                        : "r"(at)
                        : "memory");
         }
-      const float sq = FUSED ? scales[m] : a.q_scales[m];
-      float sw[4], bias[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        sw[j] = n + j < a.N ? a.w_scales[n + j] : 0.0f;
-        bias[j] = n + j < a.N && a.bias ? a.bias[n + j] : 0.0f;
-      }
       int4 acc = part[0];
 #pragma unroll
       for (int r = 1; r < 8; ++r)
@@ -461,6 +493,133 @@ __global__ void __launch_bounds__(384, 1)
   }
 }
 
+// Many tokens: a cluster of two CTAs computes 256 channels x 256 tokens with
+// tcgen05.mma.cta_group::2 M256 N256.  Each CTA loads its own 128 channels and
+// its own 128 tokens (32 KB a stage of 128 bytes of K); the leader's MMAs read both
+// CTAs' tiles and leave each its 128 channels' sums of all 256 tokens.  A stage is
+// 512 clocks of MMA and 512 of L2 intake at 64 bytes a clock; one CTA alone
+// takes in 768 for 128 channels x 256 tokens.
+// Synchronisation: both CTAs' loads complete on the leader's `full`; an
+// MMA's completion is signalled to both CTAs' `empty` and `tfull`; both CTAs' epilogue
+// warps arrive on the leader's `tempty`.
+constexpr int kPairStages = 6, kPairBytes = 2 * BN * BK;
+constexpr size_t kPairSmem = (size_t)kPairStages * kPairBytes + 1024 + 256;
+
+template <typename TY>
+__global__ void __launch_bounds__(384, 1)
+    int8_pair_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ CUtensorMap mq, Int8Args a, int *err) {
+  constexpr int STAGES = kPairStages, W_BYTES = BN * BK, BT = 256, HALF = 128;
+  constexpr uint32_t IDESC = i8_idesc(2 * BN, BT);
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t *full = (uint64_t *)(smem + STAGES * kPairBytes), *empty = full + STAGES;
+  uint64_t *tfull = empty + STAGES, *tempty = tfull + 2;
+  uint32_t *tmem_slot = (uint32_t *)(tempty + 2);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)cluster_ctarank(), pair = (int)blockIdx.x >> 1, pairs = (int)gridDim.x >> 1;
+  const int num_n = (a.N + 2 * BN - 1) / (2 * BN), num_t = (a.M + BT - 1) / BT, tiles = num_n * num_t;
+  const int nkb = (a.K + BK - 1) / BK;
+
+  if (threadIdx.x == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mw) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mq) : "memory");
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&tfull[b], 1);
+      mbar_init(&tempty[b], 16);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(2 * BT));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  cluster_sync();  // both CTAs' barriers are initialised before either is signalled
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = *(volatile uint32_t *)tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      pdl_wait();  // the tokens
+      int s = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int t = pair; t < tiles && ok; t += pairs) {
+        const int n0 = t % num_n * 2 * BN + rank * BN, m0 = t / num_n * BT + rank * BN;
+        for (int kb = 0; kb < nkb; ++kb) {
+          if (!(ok = mbar_wait(&empty[s], ph ^ 1, err))) break;
+          if (rank == 0) mbar_expect_tx(&full[s], 2 * kPairBytes);  // both CTAs' bytes
+          const uint32_t fb = pair_leader_addr(&full[s]);
+          tma_load_2d_pair(smem + s * kPairBytes, &mw, fb, kb * BK, n0);
+          tma_load_2d_pair(smem + s * kPairBytes + W_BYTES, &mq, fb, kb * BK, m0);
+          if (++s == STAGES) s = 0, ph ^= 1;
+        }
+      }
+      // every requested stage has been multiplied before the CTA leaves
+      for (int i = 0; i < STAGES && ok; ++i) {
+        ok = mbar_wait(&empty[s], ph ^ 1, err);
+        if (++s == STAGES) s = 0, ph ^= 1;
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1 && rank == 0) {
+    int s = 0, i = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    const uint64_t hi = umma_desc(smem) & 0xFFFFFFFF00000000ull;
+    const uint32_t w16 = (smem_u32(smem) >> 4) | (1u << 16);
+    for (int t = pair; t < tiles && ok; t += pairs, ++i) {
+      const int buf = i & 1;
+      if (i >= 2 && !(ok = warp_wait(&tempty[buf], ((i >> 1) & 1) ^ 1, err))) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t d = tmem + (uint32_t)(buf * BT);
+      for (int kb = 0; kb < nkb; ++kb) {
+        if (!(ok = warp_wait(&full[s], ph, err))) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t dw = w16 + (uint32_t)(s * (kPairBytes >> 4)), dq = dw + (W_BYTES >> 4);
+#pragma unroll
+        for (int k = 0; k < BK / 32; ++k) mma_i8_pair(d, hi | (dw + 2 * k), hi | (dq + 2 * k), IDESC, (kb | k) ? 1u : 0u);
+        umma_commit_pair_e(&empty[s]);
+        if (++s == STAGES) s = 0, ph ^= 1;
+      }
+      if (ok) umma_commit_pair_e(&tfull[buf]);
+    }
+  } else if (warp >= 4) {
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    pdl_wait();  // the tokens' scales
+    int i = 0;
+    for (int t = pair; t < tiles; t += pairs, ++i) {
+      const int buf = i & 1;
+      const int n = t % num_n * 2 * BN + rank * BN + quarter * 32 + lane, m0 = t / num_n * BT + half * HALF;
+      const float sw = n < a.N ? a.w_scales[n] : 0.0f, bias = n < a.N && a.bias ? a.bias[n] : 0.0f;
+      float sq[HALF / 32];
+      token_scales<HALF>(a.q_scales, m0, a.M, lane, sq);
+      if (!warp_wait(&tfull[buf], (uint32_t)((i >> 1) & 1), err)) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      store_tokens<HALF, TY>(a, tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BT + half * HALF), m0, n, sw, bias,
+                             sq);
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(&tempty[buf], 0);
+    }
+  }
+  __syncwarp();
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  cluster_sync();  // no arrive or MMA reaches a CTA that has left
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BT));
+  }
+}
+
 cudaError_t row_map(CUtensorMap *map, const int8_t *p, int64_t rows, int K, int box_rows) {
   const uint64_t dims[2] = {(uint64_t)K, (uint64_t)rows}, strides[1] = {(uint64_t)int8_row_bytes(K)};
   const uint32_t box[2] = {BK, (uint32_t)box_rows};
@@ -468,7 +627,7 @@ cudaError_t row_map(CUtensorMap *map, const int8_t *p, int64_t rows, int K, int 
 }
 
 template <int BT, typename TY, bool FUSED>
-cudaError_t launch_tc(const Int8Args &a, int split, int sms, bool pdl, int *err, cudaStream_t st) {
+cudaError_t launch_tc(const Int8Args &a, int lg, int sms, bool pdl, int *err, cudaStream_t st) {
   static thread_local int ready = -1;  // device whose kernel attributes are set
   auto *kernel = int8_tc_kernel<BT, TY, FUSED>;
   int dev = 0;
@@ -482,6 +641,7 @@ cudaError_t launch_tc(const Int8Args &a, int split, int sms, bool pdl, int *err,
   if (e != cudaSuccess) return e;
   const int64_t tiles = (int64_t)((a.N + BN - 1) / BN) * ((a.M + BT - 1) / BT);
   cudaLaunchConfig_t cfg = {};
+  const int split = 1 << lg;
   cfg.gridDim = dim3((unsigned)(split > 1 ? tiles * split : std::min<int64_t>(tiles, sms)));
   cfg.blockDim = dim3(384);
   cfg.dynamicSmemBytes = kSmem<BT, FUSED>;
@@ -496,28 +656,64 @@ cudaError_t launch_tc(const Int8Args &a, int split, int sms, bool pdl, int *err,
     at[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
   }
   cfg.attrs = at;
-  return cudaLaunchKernelEx(&cfg, kernel, *a.w_map, mq, a, split, err);
+  return cudaLaunchKernelEx(&cfg, kernel, *a.w_map, mq, a, lg, err);
+}
+
+template <typename TY>
+cudaError_t launch_pair(const Int8Args &a, int sms, bool pdl, int *err, cudaStream_t st) {
+  static thread_local int ready = -1;
+  auto *kernel = int8_pair_kernel<TY>;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && ready != dev) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPairSmem);
+    if (e == cudaSuccess) ready = dev;
+  }
+  CUtensorMap mq;
+  if (e == cudaSuccess) e = row_map(&mq, a.q, a.M, a.K, BN);
+  if (e != cudaSuccess) return e;
+  const int64_t tiles = (int64_t)((a.N + 2 * BN - 1) / (2 * BN)) * ((a.M + 255) / 256);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, sms / 2)));
+  cfg.blockDim = dim3(384);
+  cfg.dynamicSmemBytes = kPairSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim = {2, 1, 1};
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = pdl ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, *a.w_map, mq, a, err);
 }
 
 // Tokens of a tile and CTAs that share one: the least estimated time, in
 // clocks of an SM that takes in about 64 bytes each from L2, which is what
 // binds: the waves of tiles, each the bytes of its stages and a start and end of
 // about 2,000 clocks, and as much again for the CTAs of a cluster to meet.
+// A CTA pair's tile of 256 channels x 256 tokens (bt 512) takes in 512 clocks a
+// stage instead of the 768 of one CTA's 128 x 256.
 struct Shape {
-  int bt, split;
+  int bt, lg;  // tokens (512: a pair's tile), log2 of the CTAs
 };
 Shape choose_shape(int M, int N, int K, int sms) {
   const int num_n = (N + BN - 1) / BN, nkb = (K + BK - 1) / BK;
-  Shape best{16, 1};
+  Shape best{16, 0};
   int64_t least = INT64_MAX;
   for (int b = 256; b >= 16; b /= 2) {
     const int64_t tiles = (int64_t)num_n * ((M + b - 1) / b);
-    for (int s = 1; s <= (b <= 128 ? 8 : 1) && s <= nkb && (s == 1 || tiles * s <= sms); s *= 2) {
+    for (int lg = 0; lg <= (b <= 128 ? 3 : 0); ++lg) {
+      const int s = 1 << lg;
+      if (lg && (s > nkb || tiles * s > sms)) break;
       const int64_t waves = (tiles * s + sms - 1) / sms;
       const int64_t cost = waves * ((BN + b) * 2 * ((nkb + s - 1) / s)) + 2000 + (s > 1 ? 1000 + b * 16 / s : 0) + b * 8;
-      if (cost < least) least = cost, best = Shape{b, s};
+      if (cost < least) least = cost, best = Shape{b, lg};
     }
   }
+  const int64_t pair_tiles = (int64_t)((N + 2 * BN - 1) / (2 * BN)) * ((M + 255) / 256);
+  const int64_t cost = (pair_tiles + sms / 2 - 1) / (sms / 2) * (2 * BN * 2 * nkb) + 4000 + 256 * 8;
+  if (cost < least) best = Shape{512, 0};
   return best;
 }
 
@@ -527,7 +723,7 @@ Shape choose_shape(int M, int N, int K, int sms) {
 bool fuses(const Shape &sh, int M, int K, int dtype) {
   const int nkb = (K + BK - 1) / BK;
   return sh.bt == 16 && M <= 16 && (int64_t)M * K * (int64_t)dtype_size(dtype) <= (128 << 10) &&
-         (nkb + sh.split - 1) / sh.split <= kFusedBlocks;
+         (nkb + (1 << sh.lg) - 1) >> sh.lg <= kFusedBlocks;
 }
 
 template <typename TY>
@@ -539,12 +735,13 @@ cudaError_t product(const Int8Args &a, bool pdl, int *err, cudaStream_t st) {
   const Shape sh = choose_shape(a.M, a.N, a.K, sms);
   switch (sh.bt) {
     case 16:
-      return a.x ? launch_tc<16, TY, true>(a, sh.split, sms, false, err, st)
-                 : launch_tc<16, TY, false>(a, sh.split, sms, pdl, err, st);
-    case 32: return launch_tc<32, TY, false>(a, sh.split, sms, pdl, err, st);
-    case 64: return launch_tc<64, TY, false>(a, sh.split, sms, pdl, err, st);
-    case 128: return launch_tc<128, TY, false>(a, sh.split, sms, pdl, err, st);
-    default: return launch_tc<256, TY, false>(a, sh.split, sms, pdl, err, st);
+      return a.x ? launch_tc<16, TY, true>(a, sh.lg, sms, false, err, st)
+                 : launch_tc<16, TY, false>(a, sh.lg, sms, pdl, err, st);
+    case 32: return launch_tc<32, TY, false>(a, sh.lg, sms, pdl, err, st);
+    case 64: return launch_tc<64, TY, false>(a, sh.lg, sms, pdl, err, st);
+    case 128: return launch_tc<128, TY, false>(a, sh.lg, sms, pdl, err, st);
+    case 512: return launch_pair<TY>(a, sms, pdl, err, st);
+    default: return launch_tc<256, TY, false>(a, sh.lg, sms, pdl, err, st);
   }
 }
 
