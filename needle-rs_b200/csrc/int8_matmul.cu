@@ -35,37 +35,66 @@ __device__ __forceinline__ uint32_t abs_bits(T v) {
   return __float_as_uint((float)v) & 0x7fffffffu;
 }
 
+// Largest |x| of a thread's vectors of 8, as the bits of an f32.  16-bit types
+// compare as pairs of 16-bit integers: their bits without the sign order as the
+// values do, infinities and NaN on top.
+template <typename T>
+struct TopOf {
+  uint32_t top = 0;
+  __device__ __forceinline__ void see(const uint4 *raw) {
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(raw);
+#pragma unroll
+    for (int j = 0; j < 2 * (int)sizeof(T); ++j)
+      top = sizeof(T) == 4 ? max(top, w[j] & 0x7fffffffu) : __vmaxu2(top, w[j] & 0x7fff7fffu);
+  }
+  __device__ __forceinline__ uint32_t bits() const {
+    if constexpr (sizeof(T) == 4) {
+      return top;
+    } else {
+      const uint16_t h = (uint16_t)max(top & 0xffffu, top >> 16);
+      return __float_as_uint((float)*reinterpret_cast<const T *>(&h));
+    }
+  }
+};
+
 // Rows on 16-byte boundaries: read once, 8 elements a load, and kept in
 // registers between the maximum and the rounding.
 template <typename T, int CH>
-__global__ void __launch_bounds__(CH <= 2 ? 256 : 1024)
+__global__ void __launch_bounds__(CH == 1 ? 512 : 1024)
     quantize_rows_kernel(const T *x, int64_t M, int K, int64_t ldx, int8_t *q, int Kp, float *scales) {
   __shared__ uint32_t sm[32];
+  constexpr int V = sizeof(T) / 2;  // 16-byte pieces of 8 elements
   pdl_trigger();
-  const int T_ = blockDim.x;
+  const int threads = blockDim.x;
   const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   if (row >= M) return;  // blockDim.y > 1 only when a warp owns a row: no barrier is skipped
   x += row * ldx;
   q += row * Kp;
-  float v[CH][8];
-  uint32_t top = 0;
+  uint4 raw[CH][V];
+  TopOf<T> top;
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
-    const int i = (c * T_ + threadIdx.x) * 8;
+    const int i = (c * threads + threadIdx.x) * 8;
     if (i < K) {
-      load<8>(x + i, v[c]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) top = max(top, abs_bits(v[c][j]));
+      for (int p = 0; p < V; ++p) raw[c][p] = reinterpret_cast<const uint4 *>(x + i)[p];
     }
   }
-  const RowScale rs = int8_row_scale(row_max_bits(top, T_ >> 5, sm));
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+    if ((c * threads + (int)threadIdx.x) * 8 < K) top.see(raw[c]);
+  const RowScale rs = int8_row_scale(row_max_bits(top.bits(), threads >> 5, sm));
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
-    const int i = (c * T_ + threadIdx.x) * 8;
-    if (i < K)
-      *reinterpret_cast<uint2 *>(q + i) = make_uint2(int8_pack4(v[c], rs.inv), int8_pack4(v[c] + 4, rs.inv));
-    else if (i < Kp)
+    const int i = (c * threads + threadIdx.x) * 8;
+    if (i < K) {
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = (float)reinterpret_cast<const T *>(raw[c])[j];
+      *reinterpret_cast<uint2 *>(q + i) = make_uint2(int8_pack4(v, rs.inv), int8_pack4(v + 4, rs.inv));
+    } else if (i < Kp) {
       *reinterpret_cast<uint2 *>(q + i) = make_uint2(0, 0);
+    }
   }
   if (threadIdx.x == 0) scales[row] = rs.scale;
 }
@@ -82,7 +111,7 @@ __global__ void quantize_any_kernel(const T *x, int64_t K, int64_t ldx, int8_t *
   for (int64_t i = threadIdx.x; i < K; i += blockDim.x) top = max(top, abs_bits(x[i]));
   const RowScale rs = int8_row_scale(row_max_bits(top, blockDim.x >> 5, sm));
   for (int64_t i = threadIdx.x; i < Kp; i += blockDim.x)
-    q[i] = i < K ? (int8_t)int8_round((float)x[i], rs.inv) : (int8_t)0;
+    q[i] = i < K ? int8_round((float)x[i], rs.inv) : (int8_t)0;
   if (threadIdx.x == 0) scales[row] = rs.scale;
 }
 
@@ -94,7 +123,7 @@ cudaError_t quantize_rows(const T *x, int64_t M, int64_t K, int64_t ldx, int8_t 
     quantize_any_kernel<T><<<(unsigned)M, 256, 0, st>>>(x, K, ldx, q, Kp, scales);
     return cudaGetLastError();
   }
-  const int CH = K <= 256 ? 1 : K <= 4096 ? 2 : 4;
+  const int CH = K <= 4096 ? 1 : K <= 16384 ? 2 : 4;
   const int threads = (int)((Kp + 8 * CH - 1) / (8 * CH) + 31) / 32 * 32, rows = threads == 32 ? 8 : 1;
   const unsigned grid = (unsigned)((M + rows - 1) / rows);
   const dim3 block(threads, rows);
@@ -127,7 +156,7 @@ __global__ void quantize_cols_kernel(const T *w, int64_t K, int64_t N, int8_t *d
   for (int64_t k0 = 0; k0 < Kp; k0 += 32) {
     for (int j = ty; j < 32; j += 8) {
       const int64_t k = k0 + j;
-      tile[j][tx] = n < N && k < K ? (int8_t)int8_round((float)w[k * N + n], rs.inv) : (int8_t)0;
+      tile[j][tx] = n < N && k < K ? int8_round((float)w[k * N + n], rs.inv) : (int8_t)0;
     }
     __syncthreads();
     for (int j = ty; j < 32; j += 8) {

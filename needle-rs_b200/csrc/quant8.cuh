@@ -31,15 +31,19 @@ __device__ __forceinline__ RowScale int8_row_scale(uint32_t top) {
 }
 
 // |x * inv| is at most 127 (1 + 2^-23), which rounds to 127: no clamp.  A row
-// with an infinity or NaN has inv = 0 and becomes zeros: infinity * 0 is NaN,
-// which __float2int_rn turns into 0.
-__device__ __forceinline__ int int8_round(float x, float inv) { return __float2int_rn(__fmul_rn(x, inv)); }
-
+// with inv = 0 (all zero, or with an infinity or NaN) becomes zeros.  Adding
+// 1.5 * 2^23 to a product rounds it to an integer, half to even, and leaves that
+// integer's low bits in the sum's: one addition instead of a conversion.
+__device__ __forceinline__ uint32_t int8_low(float x, float inv) {
+  return __float_as_uint(__fadd_rn(__fmul_rn(x, inv), 12582912.0f));
+}
+__device__ __forceinline__ int8_t int8_round(float x, float inv) {
+  return inv == 0.0f ? (int8_t)0 : (int8_t)(int8_low(x, inv) & 0xffu);
+}
 __device__ __forceinline__ uint32_t int8_pack4(const float *x, float inv) {
-  uint32_t w = 0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) w |= ((uint32_t)int8_round(x[j], inv) & 0xffu) << (8 * j);
-  return w;
+  const uint32_t a = __byte_perm(int8_low(x[0], inv), int8_low(x[1], inv), 0x0040);
+  const uint32_t b = __byte_perm(int8_low(x[2], inv), int8_low(x[3], inv), 0x0040);
+  return inv == 0.0f ? 0u : __byte_perm(a, b, 0x5410);
 }
 
 }  // namespace ndl
