@@ -13,9 +13,10 @@
 // elements a warp owns a row and reduces with shuffles alone; above, a block
 // does.
 //
-// Many aligned rows are streamed by persistent blocks (residual_norm_stream_kernel);
-// fewer rows than blocks, or rows off 16-byte boundaries, take
-// residual_norm_kernel, a block or warp for each row.
+// Many rows are streamed by persistent blocks (residual_norm_stream_kernel, and
+// residual_norm_any_kernel off 16-byte boundaries); fewer rows than blocks, and
+// rows above 8,192 elements, take residual_norm_kernel, a block or warp for each
+// row.
 #include <algorithm>
 
 #include "common.cuh"
@@ -262,7 +263,7 @@ __global__ void __launch_bounds__(512) residual_norm_stream_kernel(ResidualNormA
   __shared__ __align__(16) float sm[2][3][16];  // of even and odd rows: a row's writes follow a barrier of the row between
   const int T = blockDim.x, warps = T >> 5, d = a.d, threads = T * blockDim.y;
   if (warps > 1) {
-    if (threadIdx.x < 96) (&sm[0][0][0])[threadIdx.x] = 0.0f;
+    for (int i = threadIdx.x; i < 96; i += T) (&sm[0][0][0])[i] = 0.0f;
     __syncthreads();
   }
   const int64_t step = (int64_t)gridDim.x * blockDim.y;
@@ -438,6 +439,139 @@ __global__ void __launch_bounds__(512) residual_norm_stream_kernel(ResidualNormA
   }
 }
 
+// Many rows off 16-byte boundaries (odd d).  As the streaming kernel, but a row
+// crosses between global and shared memory in whole 16-byte pieces (row_in,
+// row_out) and its elements are read and written there one by one, a thread every
+// T-th column: element accesses to global memory left the memory idle (14,785 x
+// 6,738 bf16 took 847 us).
+constexpr int kAnyCols = 16;  // columns a thread
+template <typename TX, typename TY, int MODE>
+__global__ void __launch_bounds__(512, 2) residual_norm_any_kernel(ResidualNormArgs a, int bx, int by) {
+  constexpr int CH = kAnyCols, S = kStreamStages;
+  // a row group's shared memory: S stages of x, y and gate rows, then r and h
+  extern __shared__ __align__(16) uint8_t buf[];
+  __shared__ __align__(16) float sm[3][16];
+  const int T = blockDim.x, warps = T >> 5, t = threadIdx.x, d = a.d;
+  if (warps > 1) {
+    for (int i = t; i < 48; i += T) (&sm[0][0])[i] = 0.0f;
+    __syncthreads();
+  }
+  auto sync = [&] {
+    if (warps > 1)
+      __syncthreads();
+    else
+      __syncwarp();
+  };
+  const int64_t step = (int64_t)gridDim.x * blockDim.y;
+  int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  if (row >= a.M) return;  // blockDim.y > 1 only when a warp owns a row: no barrier is skipped
+  const int stage = bx + MODE * by;
+  uint8_t *in = buf + (size_t)threadIdx.y * (S * stage + bx + by), *out_r = in + S * stage, *out_h = out_r + bx;
+  auto fetch = [&](int64_t at, int s) {
+    if (at < a.M) {
+      row_in(in + s * stage, (const TX *)a.x + at * a.ldx, d * (int)sizeof(TX), t, T);
+      if (MODE >= 1) row_in(in + s * stage + bx, (const TY *)a.y + at * a.ldy, d * (int)sizeof(TY), t, T);
+      if (MODE == 2) row_in(in + s * stage + bx + by, (const TY *)a.gate + at * a.ldg, d * (int)sizeof(TY), t, T);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) fetch(row + s * step, s);
+  float g = 1.0f;  // scalar gate
+  if (a.gate_kind == 1) {
+    g = *(const float *)a.gate;
+    if (a.sigmoid) g = logistic(g);
+  }
+  // factor of column i, a token gate left out (read from L1 every row: registers
+  // for them would halve the blocks on an SM)
+  auto post_factor = [&](int i) {
+    float f = a.post ? g * (1.0f + a.post[i]) : g;
+    if (a.gate_kind == 2) f *= a.sigmoid ? logistic16(((const float *)a.gate)[i]) : ((const float *)a.gate)[i];
+    return f;
+  };
+  const float over_d = 1.0f / (float)d;
+  auto element = [](const void *p, int64_t at, auto type, const uint8_t *b) {  // where row `at`'s elements lie in b
+    (void)type;
+    return b + ((uintptr_t)p + (uintptr_t)at * sizeof(type) & 15);
+  };
+  int s = 0;
+  for (; row < a.M; row += step) {
+    fetch(row + (S - 1) * step, s == 0 ? S - 1 : s - 1);
+    asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
+    sync();  // the whole row has arrived, and the last one has left out_r and out_h
+    const uint8_t *at = in + s * stage;
+    if (++s == S) s = 0;
+    const TX *px = (const TX *)element(a.x, row * a.ldx, TX{}, at);
+    const TY *py = (const TY *)element(a.y, row * a.ldy, TY{}, at + bx);
+    const TY *pg = (const TY *)element(a.gate, row * a.ldg, TY{}, at + bx + by);
+    float r[CH], ss = 0.0f;
+    if (MODE >= 1) {
+      float inv = 1.0f;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int i = c * T + t;
+        r[c] = i < d ? (float)py[i] : 0.0f;
+        ss = fmaf(r[c], r[c], ss);
+      }
+      if (a.post) inv = rsqrtf(fmaf(stream_sum(f2pack(ss, 0.0f), warps, sm[0]), over_d, kEps));
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int i = c * T + t;
+        if (i >= d) continue;
+        r[c] = r[c] * inv * post_factor(i);
+        if (MODE == 2) {
+          const float gv = (float)pg[i];
+          r[c] *= a.sigmoid ? (sizeof(TY) == 2 ? logistic16(gv) : logistic(gv)) : gv;
+        }
+      }
+    }
+    ss = 0.0f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int i = c * T + t;
+      const float xv = i < d ? (float)px[i] : 0.0f;
+      r[c] = MODE >= 1 ? fmaf(a.scale, xv, r[c]) : a.scale * xv;
+      ss = fmaf(r[c], r[c], ss);
+    }
+    if (MODE >= 1 && a.r) {
+      TX *to = (TX *)element(a.r, row * a.ldr, TX{}, out_r);
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+        if (c * T + t < d) to[c * T + t] = from_f32<TX>(r[c]);
+    }
+    if (a.h) {
+      const float inv = rsqrtf(fmaf(stream_sum(f2pack(ss, 0.0f), warps, sm[1]), over_d, kEps));
+      uint32_t top = 0;  // largest |h| as bits: infinities and NaN order above every number
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        if (c * T + t < d) r[c] = r[c] * inv * (1.0f + a.pre[c * T + t]);
+        top = max(top, __float_as_uint(r[c]) & 0x7fffffffu);
+      }
+      if (a.h_dtype == DT_I8) {
+        const RowScale rs = int8_row_scale(row_max_bits(top, warps, reinterpret_cast<uint32_t *>(sm[2])));
+        int8_t *to = (int8_t *)out_h;  // rows of 8-bit values start on 16-byte boundaries
+        const int dp = (d + 15) / 16 * 16;
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+          if (c * T + t < d) to[c * T + t] = int8_round(r[c], rs.inv);
+        if (t < dp - d) to[d + t] = 0;
+        if (t == 0) a.h_scales[row] = rs.scale;
+      } else {
+        TY *to = (TY *)element(a.h, row * a.ldh, TY{}, out_h);
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+          if (c * T + t < d) to[c * T + t] = from_f32<TY>(r[c]);
+      }
+    }
+    sync();
+    if (MODE >= 1 && a.r) row_out((TX *)a.r + row * a.ldr, out_r, d * (int)sizeof(TX), t, T);
+    if (a.h && a.h_dtype == DT_I8)
+      row_out((int8_t *)a.h + row * a.ldh, out_h, (d + 15) / 16 * 16, t, T);
+    else if (a.h)
+      row_out((TY *)a.h + row * a.ldh, out_h, d * (int)sizeof(TY), t, T);
+  }
+}
+
 template <typename TX, typename TY, int VEC, int CH>
 cudaError_t launch_rows(const ResidualNormArgs &a, cudaStream_t st) {
   const int need = (a.d + VEC * CH - 1) / (VEC * CH);
@@ -490,6 +624,31 @@ cudaError_t stream_rows(const ResidualNormArgs &a, bool *done, cudaStream_t st) 
   return a.gate_kind == 3 ? stream_mode<TX, TY, 2>(a, done, st) : stream_mode<TX, TY, 1>(a, done, st);
 }
 
+// The same for rows at any alignment; from one row a block on.
+template <typename TX, typename TY, int MODE>
+cudaError_t launch_any(const ResidualNormArgs &a, bool *done, cudaStream_t st) {
+  const int T = ((a.d + kAnyCols - 1) / kAnyCols + 31) / 32 * 32, rows = T == 32 ? 4 : 1;
+  // bytes of a row and its offset, to the next 16-byte boundary
+  const int bx = (a.d * (int)sizeof(TX) + 31) / 16 * 16, by = (a.d * (int)sizeof(TY) + 31) / 16 * 16;
+  const size_t smem = (size_t)rows * (kStreamStages * (bx + MODE * by) + bx + by);
+  auto *kernel = residual_norm_any_kernel<TX, TY, MODE>;
+  static thread_local int last_dev = -1, last_d = 0, fit = 0;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (last_dev != dev || last_d != a.d)) {
+    int sms = 0, each = 0;
+    e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+    if (e == cudaSuccess && smem <= 200 * 1024)
+      e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&each, kernel, T * rows, smem);
+    if (e == cudaSuccess) last_dev = dev, last_d = a.d, fit = sms * each;
+  }
+  *done = e != cudaSuccess || (fit > 0 && a.M >= (int64_t)fit * rows);
+  if (e != cudaSuccess || !*done) return e;
+  kernel<<<dim3((unsigned)fit), dim3(T, rows), smem, st>>>(a, bx, by);
+  return cudaGetLastError();
+}
+
 template <typename TX, typename TY>
 cudaError_t dispatch(const ResidualNormArgs &a, cudaStream_t st) {
   auto al = [](const void *p) { return ((uintptr_t)p & 15) == 0; };
@@ -505,6 +664,13 @@ cudaError_t dispatch(const ResidualNormArgs &a, cudaStream_t st) {
     if (a.d <= 256) return launch_rows<TX, TY, 8, 1>(a, st);
     if (a.d <= 4096) return launch_rows<TX, TY, 8, 2>(a, st);
     return launch_rows<TX, TY, 8, 4>(a, st);
+  }
+  if (a.d <= 8192) {
+    bool done = false;
+    const cudaError_t e = !a.y               ? launch_any<TX, TY, 0>(a, &done, st)
+                          : a.gate_kind == 3 ? launch_any<TX, TY, 2>(a, &done, st)
+                                             : launch_any<TX, TY, 1>(a, &done, st);
+    if (done) return e;
   }
   if (a.d <= 8192) return launch_rows<TX, TY, 1, 8>(a, st);
   return launch_rows<TX, TY, 1, 32>(a, st);

@@ -152,6 +152,45 @@ def test_strides_and_alignment(d, off):
     assert (rd[:, d:] == 5).all() and (hd[:, d:] == 5).all()
 
 
+MANY = [(20000, 33), (20000, 64), (9000, 264), (9000, 257), (9001, 512), (8000, 777), (6000, 1000), (5000, 1024), (4001, 2048),
+        (3000, 2054), (2500, 4096), (2000, 4099), (1500, 4360), (1500, 6738), (1300, 8192), (1200, 8191)]
+
+
+@pytest.mark.parametrize("gate", ["none", "scalar", "channel", "token", "no block"])
+@pytest.mark.parametrize("M,d", MANY)
+def test_many_rows(M, d, gate):
+    """Enough rows for every block to take several, in whole vectors and off 16-byte boundaries; every row is checked."""
+    k = MANY.index((M, d)) + ["none", "scalar", "channel", "token", "no block"].index(gate)
+    ty = (nb.BF16, nb.F16, nb.F32)[k % 3]
+    tx = nb.F32 if k % 2 else ty
+    sigmoid, post, i8 = k % 4 != 1, k % 5 != 2, k % 2 == 0
+    x, y, g, ps, pre = inputs(M, d, tx, ty, "none" if gate == "no block" else gate, post, k)
+    xd, prd = cuda(x, pre)
+    Kp = nb.int8_row_bytes(d)
+    hd = torch.full((M + 1, Kp), 9, dtype=torch.int8, device="cuda") if i8 else torch.full((M + 1, d), 7.0, dtype=TYPES[ty], device="cuda")
+    hs = torch.full((M + 1,), 7.0, device="cuda") if i8 else None
+    if gate == "no block":
+        r, h, er, eh = reference(x, None, None, None, False, 0.75, pre)
+        nb.residual_norm(p(xd), tx, None, ty, M, d, p(prd), None, p(hd), nb.I8 if i8 else ty, residual_scale=0.75, h_scales_ptr=p(hs))
+    else:
+        r, h, er, eh = reference(x, y, ps, g, sigmoid, 0.75, pre)
+        yd, gd, pd = cuda(y, g, ps)
+        rd = torch.full((M + 1, d), 7.0, dtype=TYPES[tx], device="cuda")
+        flags = KINDS[gate] | (nb.GATE_SIGMOID if gate != "none" and sigmoid else 0)
+        nb.residual_norm(p(xd), tx, p(yd), ty, M, d, p(prd), p(rd), p(hd), nb.I8 if i8 else ty, post_scale_ptr=p(pd), gate_ptr=p(gd),
+                         gate_flags=flags, residual_scale=0.75, h_scales_ptr=p(hs))
+        close(rd[:M], r, rounded(er, r, tx))
+        assert (rd[M] == 7).all()
+    if i8:
+        s, q, etop = hs[:M].double().cpu(), hd[:M].double().cpu(), eh.max(dim=1).values
+        assert (q[:, d:] == 0).all() and (hd[M] == 9).all() and hs[M] == 7
+        assert ((s - h.abs().max(dim=1).values / 127).abs() <= etop / 127 + 2 * U * s).all()
+        close(q[:, :d] * s[:, None], h, eh + s[:, None] * (0.5 + 4 * 127 * U) + etop[:, None])
+    else:
+        close(hd[:M], h, rounded(eh, h, ty))
+        assert (hd[M] == 7).all()
+
+
 def test_zero_rows_infinities_and_nan():
     M, d = 4, 96
     x, y, _, ps, pre = inputs(M, d, nb.F32, nb.F32, "none", True, 1)
