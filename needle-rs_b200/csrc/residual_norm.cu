@@ -22,12 +22,12 @@
 #include "common.cuh"
 #include "ops.h"
 #include "quant8.cuh"
+#include "residual_norm.cuh"
 #include "rowio.cuh"
 
 namespace ndl {
 namespace {
 
-constexpr float kEps = 1e-6f;
 constexpr int kWarpRows = 8;  // rows of a block whose warps own a row each
 
 // Sum over the threads of a row; `warps` of them when the block owns the row,
@@ -156,48 +156,8 @@ __global__ void __launch_bounds__(kMaxThreads<VEC, CH>) residual_norm_kernel(Res
   if (threadIdx.x == 0) a.h_scales[row] = rs.scale;
 }
 
-__device__ __forceinline__ float logistic(float v) { return 1.0f / (1.0f + expf(-v)); }
-
-// The same for a gate read from 16 bits, by the approximate instructions (a few
-// ulp and one more for each unit of |v|).
-__device__ __forceinline__ float logistic16(float v) {
-  float e;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * -1.4426950408889634f));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(1.0f + e));
-  return e;
-}
-
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-
-// Two elements of a 32-bit word as packed f32.
-template <typename T>
-__device__ __forceinline__ uint64_t pair_f32(uint32_t w);
-template <>
-__device__ __forceinline__ uint64_t pair_f32<__nv_bfloat16>(uint32_t w) {
-  return f2pack(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-}
-template <>
-__device__ __forceinline__ uint64_t pair_f32<__half>(uint32_t w) {
-  const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
-  return f2pack(f.x, f.y);
-}
-template <typename T>
-__device__ __forceinline__ uint32_t pair_bits(uint64_t v);
-template <>
-__device__ __forceinline__ uint32_t pair_bits<__nv_bfloat16>(uint64_t v) {
-  float a, b;
-  f2unpack(v, a, b);
-  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t *>(&h);
-}
-template <>
-__device__ __forceinline__ uint32_t pair_bits<__half>(uint64_t v) {
-  float a, b;
-  f2unpack(v, a, b);
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t *>(&h);
 }
 
 // 8 elements as four packed pairs, from pieces of 16 bytes `stride` apart, and
@@ -222,23 +182,6 @@ __device__ __forceinline__ void put8(T *p, const uint64_t *v) {
   }
 }
 
-// Sum over a row's threads: its warp, or all `warps` of the block through sm
-// (16-byte aligned, zero past the warps).
-__device__ __forceinline__ float stream_sum(uint64_t v, int warps, float *sm) {
-  float a, b;
-  f2unpack(v, a, b);
-  a = warp_sum(a + b);
-  if (warps == 1) return a;
-  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = a;
-  __syncthreads();
-  float t = 0.0f;
-  for (int i = 0; i < warps; i += 4) {
-    const float4 f = *reinterpret_cast<const float4 *>(sm + i);
-    t += (f.x + f.y) + (f.z + f.w);
-  }
-  return t;
-}
-
 // Persistent blocks over many rows.  A thread owns CH vectors of 8 columns of
 // every row of its block (or warp): their factors ((1 + s_post) g and
 // 1 + s_pre, f32) stay in registers, since reading 12 bytes of them an element from L1
@@ -254,7 +197,6 @@ __device__ __forceinline__ float stream_sum(uint64_t v, int warps, float *sm) {
 // quotient (its 2 ulp are part of the row factor's few), and what is known before the
 // first row as a template: MODE 0 no y, 1 y, 2 y and a token gate; FULL: every
 // thread has all its vectors.  177 us now: 6.1 TB/s.
-constexpr int kStreamStages = 2;
 template <typename TX, typename TY, int MODE, bool FULL, int CH>
 __global__ void __launch_bounds__(512) residual_norm_stream_kernel(ResidualNormArgs a) {
   constexpr int S = kStreamStages, PX = sizeof(TX) / 2, PY = sizeof(TY) / 2;  // 16-byte pieces of 8 elements
@@ -439,139 +381,6 @@ __global__ void __launch_bounds__(512) residual_norm_stream_kernel(ResidualNormA
   }
 }
 
-// Many rows off 16-byte boundaries (odd d).  As the streaming kernel, but a row
-// crosses between global and shared memory in whole 16-byte pieces (row_in,
-// row_out) and its elements are read and written there one by one, a thread every
-// T-th column: element accesses to global memory left the memory idle (14,785 x
-// 6,738 bf16 took 847 us).
-constexpr int kAnyCols = 16;  // columns a thread
-template <typename TX, typename TY, int MODE>
-__global__ void __launch_bounds__(512, 2) residual_norm_any_kernel(ResidualNormArgs a, int bx, int by) {
-  constexpr int CH = kAnyCols, S = kStreamStages;
-  // a row group's shared memory: S stages of x, y and gate rows, then r and h
-  extern __shared__ __align__(16) uint8_t buf[];
-  __shared__ __align__(16) float sm[3][16];
-  const int T = blockDim.x, warps = T >> 5, t = threadIdx.x, d = a.d;
-  if (warps > 1) {
-    for (int i = t; i < 48; i += T) (&sm[0][0])[i] = 0.0f;
-    __syncthreads();
-  }
-  auto sync = [&] {
-    if (warps > 1)
-      __syncthreads();
-    else
-      __syncwarp();
-  };
-  const int64_t step = (int64_t)gridDim.x * blockDim.y;
-  int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-  if (row >= a.M) return;  // blockDim.y > 1 only when a warp owns a row: no barrier is skipped
-  const int stage = bx + MODE * by;
-  uint8_t *in = buf + (size_t)threadIdx.y * (S * stage + bx + by), *out_r = in + S * stage, *out_h = out_r + bx;
-  auto fetch = [&](int64_t at, int s) {
-    if (at < a.M) {
-      row_in(in + s * stage, (const TX *)a.x + at * a.ldx, d * (int)sizeof(TX), t, T);
-      if (MODE >= 1) row_in(in + s * stage + bx, (const TY *)a.y + at * a.ldy, d * (int)sizeof(TY), t, T);
-      if (MODE == 2) row_in(in + s * stage + bx + by, (const TY *)a.gate + at * a.ldg, d * (int)sizeof(TY), t, T);
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-#pragma unroll
-  for (int s = 0; s < S - 1; ++s) fetch(row + s * step, s);
-  float g = 1.0f;  // scalar gate
-  if (a.gate_kind == 1) {
-    g = *(const float *)a.gate;
-    if (a.sigmoid) g = logistic(g);
-  }
-  // factor of column i, a token gate left out (read from L1 every row: registers
-  // for them would halve the blocks on an SM)
-  auto post_factor = [&](int i) {
-    float f = a.post ? g * (1.0f + a.post[i]) : g;
-    if (a.gate_kind == 2) f *= a.sigmoid ? logistic16(((const float *)a.gate)[i]) : ((const float *)a.gate)[i];
-    return f;
-  };
-  const float over_d = 1.0f / (float)d;
-  auto element = [](const void *p, int64_t at, auto type, const uint8_t *b) {  // where row `at`'s elements lie in b
-    (void)type;
-    return b + ((uintptr_t)p + (uintptr_t)at * sizeof(type) & 15);
-  };
-  int s = 0;
-  for (; row < a.M; row += step) {
-    fetch(row + (S - 1) * step, s == 0 ? S - 1 : s - 1);
-    asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
-    sync();  // the whole row has arrived, and the last one has left out_r and out_h
-    const uint8_t *at = in + s * stage;
-    if (++s == S) s = 0;
-    const TX *px = (const TX *)element(a.x, row * a.ldx, TX{}, at);
-    const TY *py = (const TY *)element(a.y, row * a.ldy, TY{}, at + bx);
-    const TY *pg = (const TY *)element(a.gate, row * a.ldg, TY{}, at + bx + by);
-    float r[CH], ss = 0.0f;
-    if (MODE >= 1) {
-      float inv = 1.0f;
-#pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        const int i = c * T + t;
-        r[c] = i < d ? (float)py[i] : 0.0f;
-        ss = fmaf(r[c], r[c], ss);
-      }
-      if (a.post) inv = rsqrtf(fmaf(stream_sum(f2pack(ss, 0.0f), warps, sm[0]), over_d, kEps));
-#pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        const int i = c * T + t;
-        if (i >= d) continue;
-        r[c] = r[c] * inv * post_factor(i);
-        if (MODE == 2) {
-          const float gv = (float)pg[i];
-          r[c] *= a.sigmoid ? (sizeof(TY) == 2 ? logistic16(gv) : logistic(gv)) : gv;
-        }
-      }
-    }
-    ss = 0.0f;
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      const int i = c * T + t;
-      const float xv = i < d ? (float)px[i] : 0.0f;
-      r[c] = MODE >= 1 ? fmaf(a.scale, xv, r[c]) : a.scale * xv;
-      ss = fmaf(r[c], r[c], ss);
-    }
-    if (MODE >= 1 && a.r) {
-      TX *to = (TX *)element(a.r, row * a.ldr, TX{}, out_r);
-#pragma unroll
-      for (int c = 0; c < CH; ++c)
-        if (c * T + t < d) to[c * T + t] = from_f32<TX>(r[c]);
-    }
-    if (a.h) {
-      const float inv = rsqrtf(fmaf(stream_sum(f2pack(ss, 0.0f), warps, sm[1]), over_d, kEps));
-      uint32_t top = 0;  // largest |h| as bits: infinities and NaN order above every number
-#pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        if (c * T + t < d) r[c] = r[c] * inv * (1.0f + a.pre[c * T + t]);
-        top = max(top, __float_as_uint(r[c]) & 0x7fffffffu);
-      }
-      if (a.h_dtype == DT_I8) {
-        const RowScale rs = int8_row_scale(row_max_bits(top, warps, reinterpret_cast<uint32_t *>(sm[2])));
-        int8_t *to = (int8_t *)out_h;  // rows of 8-bit values start on 16-byte boundaries
-        const int dp = (d + 15) / 16 * 16;
-#pragma unroll
-        for (int c = 0; c < CH; ++c)
-          if (c * T + t < d) to[c * T + t] = int8_round(r[c], rs.inv);
-        if (t < dp - d) to[d + t] = 0;
-        if (t == 0) a.h_scales[row] = rs.scale;
-      } else {
-        TY *to = (TY *)element(a.h, row * a.ldh, TY{}, out_h);
-#pragma unroll
-        for (int c = 0; c < CH; ++c)
-          if (c * T + t < d) to[c * T + t] = from_f32<TY>(r[c]);
-      }
-    }
-    sync();
-    if (MODE >= 1 && a.r) row_out((TX *)a.r + row * a.ldr, out_r, d * (int)sizeof(TX), t, T);
-    if (a.h && a.h_dtype == DT_I8)
-      row_out((int8_t *)a.h + row * a.ldh, out_h, (d + 15) / 16 * 16, t, T);
-    else if (a.h)
-      row_out((TY *)a.h + row * a.ldh, out_h, d * (int)sizeof(TY), t, T);
-  }
-}
-
 template <typename TX, typename TY, int VEC, int CH>
 cudaError_t launch_rows(const ResidualNormArgs &a, cudaStream_t st) {
   const int need = (a.d + VEC * CH - 1) / (VEC * CH);
@@ -624,31 +433,6 @@ cudaError_t stream_rows(const ResidualNormArgs &a, bool *done, cudaStream_t st) 
   return a.gate_kind == 3 ? stream_mode<TX, TY, 2>(a, done, st) : stream_mode<TX, TY, 1>(a, done, st);
 }
 
-// The same for rows at any alignment; from one row a block on.
-template <typename TX, typename TY, int MODE>
-cudaError_t launch_any(const ResidualNormArgs &a, bool *done, cudaStream_t st) {
-  const int T = ((a.d + kAnyCols - 1) / kAnyCols + 31) / 32 * 32, rows = T == 32 ? 4 : 1;
-  // bytes of a row and its offset, to the next 16-byte boundary
-  const int bx = (a.d * (int)sizeof(TX) + 31) / 16 * 16, by = (a.d * (int)sizeof(TY) + 31) / 16 * 16;
-  const size_t smem = (size_t)rows * (kStreamStages * (bx + MODE * by) + bx + by);
-  auto *kernel = residual_norm_any_kernel<TX, TY, MODE>;
-  static thread_local int last_dev = -1, last_d = 0, fit = 0;
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess && (last_dev != dev || last_d != a.d)) {
-    int sms = 0, each = 0;
-    e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
-    if (e == cudaSuccess && smem <= 200 * 1024)
-      e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&each, kernel, T * rows, smem);
-    if (e == cudaSuccess) last_dev = dev, last_d = a.d, fit = sms * each;
-  }
-  *done = e != cudaSuccess || (fit > 0 && a.M >= (int64_t)fit * rows);
-  if (e != cudaSuccess || !*done) return e;
-  kernel<<<dim3((unsigned)fit), dim3(T, rows), smem, st>>>(a, bx, by);
-  return cudaGetLastError();
-}
-
 template <typename TX, typename TY>
 cudaError_t dispatch(const ResidualNormArgs &a, cudaStream_t st) {
   auto al = [](const void *p) { return ((uintptr_t)p & 15) == 0; };
@@ -667,9 +451,7 @@ cudaError_t dispatch(const ResidualNormArgs &a, cudaStream_t st) {
   }
   if (a.d <= 8192) {
     bool done = false;
-    const cudaError_t e = !a.y               ? launch_any<TX, TY, 0>(a, &done, st)
-                          : a.gate_kind == 3 ? launch_any<TX, TY, 2>(a, &done, st)
-                                             : launch_any<TX, TY, 1>(a, &done, st);
+    const cudaError_t e = residual_norm_any(a, &done, st);
     if (done) return e;
   }
   if (a.d <= 8192) return launch_rows<TX, TY, 1, 8>(a, st);

@@ -53,32 +53,32 @@ __device__ __forceinline__ void store(T *p, const float *v) {
 // Rows at any byte offset, moved in 16-byte pieces.  A row of n bytes at p lies in
 // shared memory from buf + (p & 15) on, so that its whole 16-byte pieces are
 // aligned on both sides; the bytes before the first and behind the last whole
-// piece move as elements of E.  `t` of `T` threads each take a share.
+// piece (under 32) move as elements of E, one a thread of the last 32.  `t` of `T`
+// threads each take a share.
 template <typename E>
 __device__ __forceinline__ void row_in(uint8_t *buf, const E *p, int n, int t, int T) {
-  const int o = (int)((uintptr_t)p & 15), head = min((16 - o) & 15, n), whole = (n - head) / 16 * 16;
-  const uint8_t *g = (const uint8_t *)p;
-  uint8_t *s = buf + o;
-  const uint32_t su = (uint32_t)__cvta_generic_to_shared(s);
-  for (int i = head + 16 * t; i < head + whole; i += 16 * T)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(su + i), "l"(g + i) : "memory");
-  const int edge = head + (n - head - whole);
-  for (int i = t * (int)sizeof(E); i < edge; i += T * (int)sizeof(E)) {
-    const int at = i < head ? i : i + whole;
-    *reinterpret_cast<E *>(s + at) = *reinterpret_cast<const E *>(g + at);
+  const int o = (int)((uintptr_t)p & 15), head = min((16 - o) & 15, n), whole = (n - head) & ~15;
+  const uint8_t *g = (const uint8_t *)p + head + 16 * t;
+  uint32_t s = (uint32_t)__cvta_generic_to_shared(buf) + o + head + 16 * t;
+  for (int i = 16 * t; i < whole; i += 16 * T, g += 16 * T, s += 16 * T)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s), "l"(g) : "memory");
+  const int e = (t - T + 32) * (int)sizeof(E);
+  if (e >= 0 && e < n - whole) {
+    const int at = e < head ? e : e + whole;
+    *reinterpret_cast<E *>(buf + o + at) = *reinterpret_cast<const E *>((const uint8_t *)p + at);
   }
 }
 template <typename E>
 __device__ __forceinline__ void row_out(E *p, const uint8_t *buf, int n, int t, int T) {
-  const int o = (int)((uintptr_t)p & 15), head = min((16 - o) & 15, n), whole = (n - head) / 16 * 16;
-  uint8_t *g = (uint8_t *)p;
-  const uint8_t *s = buf + o;
-  for (int i = head + 16 * t; i < head + whole; i += 16 * T)
-    *reinterpret_cast<uint4 *>(g + i) = *reinterpret_cast<const uint4 *>(s + i);
-  const int edge = head + (n - head - whole);
-  for (int i = t * (int)sizeof(E); i < edge; i += T * (int)sizeof(E)) {
-    const int at = i < head ? i : i + whole;
-    *reinterpret_cast<E *>(g + at) = *reinterpret_cast<const E *>(s + at);
+  const int o = (int)((uintptr_t)p & 15), head = min((16 - o) & 15, n), whole = (n - head) & ~15;
+  uint8_t *g = (uint8_t *)p + head + 16 * t;
+  const uint8_t *s = buf + o + head + 16 * t;
+  for (int i = 16 * t; i < whole; i += 16 * T, g += 16 * T, s += 16 * T)
+    *reinterpret_cast<uint4 *>(g) = *reinterpret_cast<const uint4 *>(s);
+  const int e = (t - T + 32) * (int)sizeof(E);
+  if (e >= 0 && e < n - whole) {
+    const int at = e < head ? e : e + whole;
+    *reinterpret_cast<E *>((uint8_t *)p + at) = *reinterpret_cast<const E *>(buf + o + at);
   }
 }
 
