@@ -766,21 +766,31 @@ __global__ void xattn_join_kernel(const XAttnItem *groups, XAttnWork w, XAttnCal
   const int G = w.s.H / w.s.KVH, D = w.s.D, r = it.r0 + i, h = it.kvh * G + r % G;
   const int64_t row = it.q0 + r / G, stride = (int64_t)it.rows * (DP + 4);
   const float *p = partial(w, it, 0, DP), *pm = p + it.rows * DP + i, *pl = pm + it.rows;
+  // lane s holds split s's m and l of 32 splits at a time; their sums are fetched 8 at once
   float M = -INFINITY;
   for (int s = lane; s < it.nsplit; s += 32) M = fmaxf(M, pm[s * stride]);
   M = warp_max(M);
   const float base = M == -INFINITY ? 0.0f : M;
   float L = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   const bool own = 4 * lane < D;
-  for (int s = 0; s < it.nsplit; ++s) {
-    const float f = ex2(pm[s * stride] - base);
-    L += f * pl[s * stride];
-    if (own) {
-      const float4 v = *reinterpret_cast<const float4 *>(p + s * stride + (int64_t)i * DP + 4 * lane);
-      o[0] += f * v.x;
-      o[1] += f * v.y;
-      o[2] += f * v.z;
-      o[3] += f * v.w;
+  const float *po = p + (int64_t)i * DP + (own ? 4 * lane : 0);
+  for (int s0 = 0; s0 < it.nsplit; s0 += 32) {
+    const int n = min(32, it.nsplit - s0);
+    const float f = lane < n ? ex2(pm[(s0 + lane) * stride] - base) : 0.0f;
+    L += warp_sum(lane < n ? f * pl[(s0 + lane) * stride] : 0.0f);
+    for (int s1 = 0; s1 < n; s1 += 8) {
+      float4 v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        v[u] = s1 + u < n ? *reinterpret_cast<const float4 *>(po + (s0 + s1 + u) * stride) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float w = __shfl_sync(0xffffffffu, f, s1 + u);
+        o[0] += w * v[u].x;
+        o[1] += w * v[u].y;
+        o[2] += w * v[u].z;
+        o[3] += w * v[u].w;
+      }
     }
   }
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;

@@ -60,7 +60,7 @@ struct TopOf {
 // Rows on 16-byte boundaries: read once, 8 elements a load, and kept in
 // registers between the maximum and the rounding.
 template <typename T, int CH>
-__global__ void __launch_bounds__(CH == 1 ? 512 : 1024)
+__global__ void __launch_bounds__(CH == 4 ? 1024 : 512)
     quantize_rows_kernel(const T *x, int64_t M, int K, int64_t ldx, int8_t *q, int Kp, float *scales) {
   __shared__ uint32_t sm[32];
   constexpr int V = sizeof(T) / 2;  // 16-byte pieces of 8 elements
@@ -99,9 +99,47 @@ __global__ void __launch_bounds__(CH == 1 ? 512 : 1024)
   if (threadIdx.x == 0) scales[row] = rs.scale;
 }
 
-// Any alignment and length: a block a row, in two passes.
+// Rows at any alignment: a thread's columns are `threads` apart, so that a warp
+// reads neighbours, and stay in registers; the values leave through shared memory
+// in whole words.
+template <typename T, int CH>
+__global__ void __launch_bounds__(1024)
+    quantize_any_kernel(const T *x, int64_t M, int K, int64_t ldx, int8_t *q, int Kp, float *scales) {
+  extern __shared__ __align__(16) int8_t line[];  // [rows of the block][Kp]
+  __shared__ uint32_t sm[32];
+  pdl_trigger();
+  const int threads = blockDim.x;
+  const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  if (row >= M) return;  // blockDim.y > 1 only when a warp owns a row: no barrier is skipped
+  x += row * ldx;
+  T v[CH];
+  uint32_t top = 0;
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+    if (c * threads + (int)threadIdx.x < K) v[c] = x[c * threads + threadIdx.x];
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+    if (c * threads + (int)threadIdx.x < K) top = max(top, abs_bits(v[c]));
+  const RowScale rs = int8_row_scale(row_max_bits(top, threads >> 5, sm));
+  int8_t *mine = line + threadIdx.y * Kp;
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int i = c * threads + threadIdx.x;
+    if (i < K) mine[i] = int8_round((float)v[c], rs.inv);
+  }
+  if (threadIdx.x < Kp - K) mine[K + threadIdx.x] = 0;
+  if (threads > 32)
+    __syncthreads();
+  else
+    __syncwarp();
+  uint32_t *out = reinterpret_cast<uint32_t *>(q + row * Kp);
+  for (int i = threadIdx.x; i < Kp / 4; i += threads) out[i] = reinterpret_cast<const uint32_t *>(mine)[i];
+  if (threadIdx.x == 0) scales[row] = rs.scale;
+}
+
+// Any length: a block a row, in two passes.
 template <typename T>
-__global__ void quantize_any_kernel(const T *x, int64_t K, int64_t ldx, int8_t *q, int64_t Kp, float *scales) {
+__global__ void quantize_long_kernel(const T *x, int64_t K, int64_t ldx, int8_t *q, int64_t Kp, float *scales) {
   __shared__ uint32_t sm[32];
   pdl_trigger();
   const int64_t row = blockIdx.x;
@@ -118,12 +156,21 @@ __global__ void quantize_any_kernel(const T *x, int64_t K, int64_t ldx, int8_t *
 template <typename T>
 cudaError_t quantize_rows(const T *x, int64_t M, int64_t K, int64_t ldx, int8_t *q, float *scales, cudaStream_t st) {
   const int64_t Kp = int8_row_bytes(K);
-  const bool vec = K % 8 == 0 && ldx % 8 == 0 && ((uintptr_t)x & 15) == 0 && K <= 32768;
-  if (!vec) {
-    quantize_any_kernel<T><<<(unsigned)M, 256, 0, st>>>(x, K, ldx, q, Kp, scales);
+  if (K > 32768) {
+    quantize_long_kernel<T><<<(unsigned)M, 1024, 0, st>>>(x, K, ldx, q, Kp, scales);
     return cudaGetLastError();
   }
-  const int CH = K <= 4096 ? 1 : K <= 16384 ? 2 : 4;
+  if (K % 8 || ldx % 8 || ((uintptr_t)x & 15)) {
+    // 16 columns a thread, 32 above 16,384
+    const int each = K <= 16384 ? 16 : 32, threads = (int)((K + each - 1) / each + 31) / 32 * 32, rows = threads == 32 ? 8 : 1;
+    const unsigned grid = (unsigned)((M + rows - 1) / rows);
+    if (each == 16)
+      quantize_any_kernel<T, 16><<<grid, dim3(threads, rows), rows * Kp, st>>>(x, M, (int)K, ldx, q, (int)Kp, scales);
+    else
+      quantize_any_kernel<T, 32><<<grid, dim3(threads, rows), rows * Kp, st>>>(x, M, (int)K, ldx, q, (int)Kp, scales);
+    return cudaGetLastError();
+  }
+  const int CH = K <= 2048 ? 1 : K <= 8192 ? 2 : 4;
   const int threads = (int)((Kp + 8 * CH - 1) / (8 * CH) + 31) / 32 * 32, rows = threads == 32 ? 8 : 1;
   const unsigned grid = (unsigned)((M + rows - 1) / rows);
   const dim3 block(threads, rows);

@@ -53,66 +53,72 @@ __global__ void __launch_bounds__(kMaxThreads<VEC, CH>) residual_norm_kernel(Res
   const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   if (row >= a.M) return;  // blockDim.y > 1 only when a warp owns a row: no barrier is skipped
   const TX *x = (const TX *)a.x + row * a.ldx;
+  // a row here and there is a chain of latencies: x is on its way while y is reduced
   float r[CH][VEC];
+  alignas(16) TX xraw[CH][VEC];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int i = (c * T + threadIdx.x) * VEC;
+    if (i >= d) continue;
+    if constexpr (VEC == 1) {
+      xraw[c][0] = x[i];
+    } else {
+#pragma unroll
+      for (int p = 0; p < VEC * (int)sizeof(TX) / 16; ++p)
+        reinterpret_cast<uint4 *>(xraw[c])[p] = reinterpret_cast<const uint4 *>(x + i)[p];
+    }
+  }
   if (a.y) {
     const TY *y = (const TY *)a.y + row * a.ldy;
     float ss = 0.0f;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int i = (c * T + threadIdx.x) * VEC;
-      if (i < d) {
-        load<VEC>(y + i, r[c]);
-      } else {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) r[c][j] = 0.0f;
-      }
+      for (int j = 0; j < VEC; ++j) r[c][j] = 0.0f;
+      if (i < d) load<VEC>(y + i, r[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
 #pragma unroll
       for (int j = 0; j < VEC; ++j) ss += r[c][j] * r[c][j];
-    }
-    float inv = 1.0f;
-    if (a.post) inv = 1.0f / sqrtf(row_sum(ss, warps, sm[0]) / (float)d + kEps);
     float g = 1.0f;
     if (a.gate_kind == 1) {
       g = *(const float *)a.gate;
-      if (a.sigmoid) g = 1.0f / (1.0f + expf(-g));
+      if (a.sigmoid) g = logistic(g);
     }
+    if (a.post) g *= 1.0f / sqrtf(row_sum(ss, warps, sm[0]) / (float)d + kEps);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int i = (c * T + threadIdx.x) * VEC;
-      if (i < d) {
-        float xv[VEC];
-        load<VEC>(x + i, xv);
-        if (a.post) {
-          float s[VEC];
-          load<VEC>(a.post + i, s);
+      if (i >= d) continue;
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) r[c][j] = ((1.0f + s[j]) * r[c][j]) * inv;
-        }
-        if (a.gate_kind >= 2) {
-          float gv[VEC];
-          if (a.gate_kind == 2)
-            load<VEC>((const float *)a.gate + i, gv);
-          else
-            load<VEC>((const TY *)a.gate + row * a.ldg + i, gv);
+      for (int j = 0; j < VEC; ++j) r[c][j] *= g;
+      if (a.post) {
+        float s[VEC];
+        load<VEC>(a.post + i, s);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) r[c][j] *= a.sigmoid ? 1.0f / (1.0f + expf(-gv[j])) : gv[j];
-        } else {
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) r[c][j] *= g;
-        }
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) r[c][j] += a.scale * xv[j];
-        if (a.r) store<VEC>((TX *)a.r + row * a.ldr + i, r[c]);
+        for (int j = 0; j < VEC; ++j) r[c][j] *= 1.0f + s[j];
       }
+      if (a.gate_kind >= 2) {
+        float gv[VEC];
+        if (a.gate_kind == 2)
+          load<VEC>((const float *)a.gate + i, gv);
+        else
+          load<VEC>((const TY *)a.gate + row * a.ldg + i, gv);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) r[c][j] *= a.sigmoid ? logistic(gv[j]) : gv[j];
+      }
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) r[c][j] = fmaf(a.scale, (float)xraw[c][j], r[c][j]);
+      if (a.r) store<VEC>((TX *)a.r + row * a.ldr + i, r[c]);
     }
   } else {
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      const int i = (c * T + threadIdx.x) * VEC;
-      if (i < d) load<VEC>(x + i, r[c]);
+    for (int c = 0; c < CH; ++c)
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) r[c][j] = i < d ? a.scale * r[c][j] : 0.0f;
-    }
+      for (int j = 0; j < VEC; ++j)
+        r[c][j] = (c * T + (int)threadIdx.x) * VEC < d ? a.scale * (float)xraw[c][j] : 0.0f;
   }
   if (!a.h) return;
   float ss = 0.0f;
@@ -455,6 +461,7 @@ cudaError_t dispatch(const ResidualNormArgs &a, cudaStream_t st) {
     if (done) return e;
   }
   if (a.d <= 8192) return launch_rows<TX, TY, 1, 8>(a, st);
+  if (a.d <= 16384) return launch_rows<TX, TY, 1, 16>(a, st);
   return launch_rows<TX, TY, 1, 32>(a, st);
 }
 
