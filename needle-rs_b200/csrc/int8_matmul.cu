@@ -170,7 +170,11 @@ cudaError_t quantize_rows(const T *x, int64_t M, int64_t K, int64_t ldx, int8_t 
       quantize_any_kernel<T, 32><<<grid, dim3(threads, rows), rows * Kp, st>>>(x, M, (int)K, ldx, q, (int)Kp, scales);
     return cudaGetLastError();
   }
-  const int CH = K <= 2048 ? 1 : K <= 8192 ? 2 : 4;
+  // A row's reductions and two divisions are the same work for every thread: 32
+  // elements a thread from 512 on (8192 x 4096 bf16: 28.6 us with 8 a thread, 21.0 with 16,
+  // 18.6 with 32; 16384 x 4096 f32: 51 us, the copy rate.  Persistent blocks that
+  // fetch rows ahead took 19.1 and 87 us.)
+  const int CH = K <= 256 ? 1 : K <= 512 ? 2 : 4;
   const int threads = (int)((Kp + 8 * CH - 1) / (8 * CH) + 31) / 32 * 32, rows = threads == 32 ? 8 : 1;
   const unsigned grid = (unsigned)((M + rows - 1) / rows);
   const dim3 block(threads, rows);

@@ -13,10 +13,9 @@
 // elements a warp owns a row and reduces with shuffles alone; above, a block
 // does.
 //
-// Many rows are streamed by persistent blocks (residual_norm_stream_kernel, and
-// residual_norm_any_kernel off 16-byte boundaries); fewer rows than blocks, and
-// rows above 8,192 elements, take residual_norm_kernel, a block or warp for each
-// row.
+// Many rows up to 8,192 elements are streamed by persistent blocks where that is
+// faster (residual_norm_stream_kernel, and residual_norm_any_kernel off 16-byte
+// boundaries); the others take residual_norm_kernel, a block or warp for each row.
 #include <algorithm>
 
 #include "common.cuh"
@@ -107,7 +106,8 @@ __global__ void __launch_bounds__(kMaxThreads<VEC, CH>) residual_norm_kernel(Res
         else
           load<VEC>((const TY *)a.gate + row * a.ldg + i, gv);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) r[c][j] *= a.sigmoid ? logistic(gv[j]) : gv[j];
+        for (int j = 0; j < VEC; ++j)
+          r[c][j] *= !a.sigmoid ? gv[j] : a.gate_kind == 3 && sizeof(TY) == 2 ? logistic16(gv[j]) : logistic(gv[j]);
       }
 #pragma unroll
       for (int j = 0; j < VEC; ++j) r[c][j] = fmaf(a.scale, (float)xraw[c][j], r[c][j]);
@@ -162,8 +162,14 @@ __global__ void __launch_bounds__(kMaxThreads<VEC, CH>) residual_norm_kernel(Res
   if (threadIdx.x == 0) a.h_scales[row] = rs.scale;
 }
 
+// f32 vectors are two pieces of 16 bytes: through L1, so that the second finds the
+// 32-byte sector there that the first has fetched.
+template <typename T>
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  if constexpr (sizeof(T) == 4)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
 // 8 elements as four packed pairs, from pieces of 16 bytes `stride` apart, and
@@ -202,7 +208,7 @@ __device__ __forceinline__ void put8(T *p, const uint64_t *v) {
 // throughout, the reciprocal square root of CUDA instead of an exact root and
 // quotient (its 2 ulp are part of the row factor's few), and what is known before the
 // first row as a template: MODE 0 no y, 1 y, 2 y and a token gate; FULL: every
-// thread has all its vectors.  177 us now: 6.1 TB/s.
+// thread has all its vectors.  169 us now: 6.4 TB/s.
 template <typename TX, typename TY, int MODE, bool FULL, int CH>
 __global__ void __launch_bounds__(512) residual_norm_stream_kernel(ResidualNormArgs a) {
   constexpr int S = kStreamStages, PX = sizeof(TX) / 2, PY = sizeof(TY) / 2;  // 16-byte pieces of 8 elements
@@ -236,13 +242,13 @@ __global__ void __launch_bounds__(512) residual_norm_stream_kernel(ResidualNormA
       for (int c = 0; c < CH; ++c) {
         if (!in[c]) continue;
 #pragma unroll
-        for (int p = 0; p < PX; ++p) copy16(dst + (c * PER + p) * piece, (const uint8_t *)(fx + c * T * 8) + 16 * p);
+        for (int p = 0; p < PX; ++p) copy16<TX>(dst + (c * PER + p) * piece, (const uint8_t *)(fx + c * T * 8) + 16 * p);
 #pragma unroll
         for (int p = 0; p < PY && MODE >= 1; ++p)
-          copy16(dst + (c * PER + PX + p) * piece, (const uint8_t *)(fy + c * T * 8) + 16 * p);
+          copy16<TY>(dst + (c * PER + PX + p) * piece, (const uint8_t *)(fy + c * T * 8) + 16 * p);
 #pragma unroll
         for (int p = 0; p < PY && MODE == 2; ++p)
-          copy16(dst + (c * PER + PX + PY + p) * piece, (const uint8_t *)(fg + c * T * 8) + 16 * p);
+          copy16<TY>(dst + (c * PER + PX + PY + p) * piece, (const uint8_t *)(fg + c * T * 8) + 16 * p);
       }
       next += step;
       fx += step * a.ldx;
@@ -428,15 +434,21 @@ cudaError_t stream_vectors(const ResidualNormArgs &a, bool *done, cudaStream_t s
 }
 // One vector of 8 a thread, two above 4,096 elements: more warps with fewer
 // columns each cover each other's reductions better (65,536 x 2,048 bf16:
-// 177 us with one, 193 with two).
+// 169 us with one, 190 with two).
 template <typename TX, typename TY, int MODE>
 cudaError_t stream_mode(const ResidualNormArgs &a, bool *done, cudaStream_t st) {
   return a.d <= 4096 ? stream_vectors<TX, TY, MODE, 1>(a, done, st) : stream_vectors<TX, TY, MODE, 2>(a, done, st);
 }
+// An f32 x has twice the bytes for the same instructions, and a block for each row
+// then keeps up (32,768 x 2,048 with a bf16 y: 131 us, streamed 147; 16-bit x
+// 65,536 x 2,048: 231, streamed 169), unless a token gate adds to them
+// (4,096 x 4,096: 49, streamed 43).
 template <typename TX, typename TY>
 cudaError_t stream_rows(const ResidualNormArgs &a, bool *done, cudaStream_t st) {
-  if (!a.y) return stream_mode<TX, TY, 0>(a, done, st);
-  return a.gate_kind == 3 ? stream_mode<TX, TY, 2>(a, done, st) : stream_mode<TX, TY, 1>(a, done, st);
+  if (a.gate_kind == 3) return stream_mode<TX, TY, 2>(a, done, st);
+  if constexpr (sizeof(TX) == 2) return a.y ? stream_mode<TX, TY, 1>(a, done, st) : stream_mode<TX, TY, 0>(a, done, st);
+  *done = false;
+  return cudaSuccess;
 }
 
 template <typename TX, typename TY>

@@ -75,6 +75,21 @@ def test_quantize_tokens(M, K, pad, dtype):
     assert np.array_equal(q[:, :K], want) and np.array_equal(s.cpu().numpy(), ws) and not q[:, K:].any()
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("M,K", [(20001, 40), (20000, 72), (9000, 512), (6000, 1000), (4000, 2056), (3001, 4096), (2500, 4104), (1300, 8192),
+                                 (3000, 617), (70000, 8), (1000, 20001)])
+def test_quantize_many_tokens(M, K, dtype):
+    g = torch.Generator(device="cuda").manual_seed(M + K)
+    x = (torch.randn((M, K), generator=g, device="cuda") * torch.exp(torch.randn((M, 1), generator=g, device="cuda"))).to(TYPES[dtype])
+    Kp = nb.int8_row_bytes(K)
+    q, s = torch.full((M + 1, Kp), 99, dtype=torch.int8, device="cuda"), torch.full((M + 1,), 5.0, device="cuda")
+    nb.int8_quantize_tokens(x.data_ptr(), M, K, q.data_ptr(), s.data_ptr(), dtype)
+    want, ws = quantized(x.cpu())
+    q = q.cpu().numpy()
+    assert np.array_equal(q[:M, :K], want) and not q[:M, K:].any() and (q[M] == 99).all()
+    assert np.array_equal(s.cpu().numpy()[:M], ws) and s[M] == 5
+
+
 def test_quantize_odd_rows():
     # zeros, subnormals, the largest values, ties, an infinity and NaN
     x = torch.zeros((8, 40))
