@@ -63,14 +63,20 @@ __device__ __forceinline__ float *partial(const XAttnWork &w, const XAttnItem &i
 
 // ── few rows ────────────────────────────────────────────────────────────────
 
-constexpr int kFewWarps = 4, kFewKeys = 16, kFewStages = 3;
+constexpr int kFewWarps = 4, kFewKeys = 16;
+// Stages of a warp's ring: two, and 5 CTAs an SM, where registers allow that
+// many (256 decode requests: 16.6 us, with three 17.7), else three.
+template <int DP, int MT>
+constexpr int kFewStages = DP == 64 && MT == 1 ? 2 : 3;
+template <int DP, int MT>
+constexpr int kFewCtas = DP == 64 ? (MT == 1 ? 5 : 3) : 2;
 // Rows of an item, and of a request and KV head that this kernel takes.
 constexpr int kFewRows = 32, kFewMaxRows = 64;
 
 template <int DP>
 constexpr int kFewStageBytes = 2 * kFewKeys * DP * 2;  // K and V rows of 16 keys
-template <int DP>
-constexpr int kFewSmem = kFewWarps * kFewStages * kFewStageBytes<DP> + kFewWarps * kFewStages * 4;
+template <int DP, int MT>
+constexpr int kFewSmem = kFewWarps * kFewStages<DP, MT> * (kFewStageBytes<DP> + 4);
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool take) {
   const int n = take ? 16 : 0;  // 0: the 16 bytes become zero and src is not read
@@ -113,17 +119,17 @@ __device__ __forceinline__ void mma16<__nv_bfloat16>(float *d, const uint32_t *a
 // hold can reach a product.  Ring rows are swizzled (16-byte chunk c of row r
 // at c ^ (r & 7)): ldmatrix reads them without bank conflicts.
 template <typename T, int DP, int MT>
-__global__ void __launch_bounds__(kFewWarps * 32) xattn_few_kernel(const XAttnItem *items, XAttnWork w, XAttnCall c) {
-  constexpr int CH = DP / 8, KS = DP / 16;  // 16-byte chunks of a row, MMA steps over the dimensions
+__global__ void __launch_bounds__(kFewWarps * 32, kFewCtas<DP, MT>) xattn_few_kernel(const XAttnItem *items, XAttnWork w, XAttnCall c) {
+  constexpr int ST = kFewStages<DP, MT>, CH = DP / 8, KS = DP / 16;  // 16-byte chunks of a row, MMA steps over the dimensions
   extern __shared__ __align__(128) uint8_t sm[];
-  uint32_t *live_of = reinterpret_cast<uint32_t *>(sm + kFewWarps * kFewStages * kFewStageBytes<DP>);
+  uint32_t *live_of = reinterpret_cast<uint32_t *>(sm + kFewWarps * ST * kFewStageBytes<DP>);
   pdl_trigger();
   const XAttnItem it = items[blockIdx.x];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int G = w.s.H / w.s.KVH, D = w.s.D;
   const int nblk = (it.klen + kFewKeys - 1) / kFewKeys;
   const uint8_t *mask = c.mask ? c.mask + it.k0 : nullptr;
-  const uint32_t ring = smem_u32(sm) + warp * kFewStages * kFewStageBytes<DP>;
+  const uint32_t ring = smem_u32(sm) + warp * ST * kFewStageBytes<DP>;
   // this lane's 16-byte chunk of the first rows of the warp's next block: the
   // other rows follow RS rows apart, the next block 64 rows on
   constexpr int RS = 32 / CH;
@@ -153,7 +159,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) xattn_few_kernel(const XAttnIt
   };
   auto issue = [&](int n, int stage) {  // the warp's n-th block, in order
     const uint32_t live = live_block(n);
-    if (lane == 0) live_of[warp * kFewStages + stage] = live;
+    if (lane == 0) live_of[warp * ST + stage] = live;
     const uint32_t dst = ring + stage * kFewStageBytes<DP>;
 #pragma unroll
     for (int i = 0; i < CH / 2; ++i) {
@@ -169,7 +175,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) xattn_few_kernel(const XAttnIt
   const int mine = (nblk - warp + kFewWarps - 1) / kFewWarps;  // blocks of this warp
 
 #pragma unroll
-  for (int n = 0; n < kFewStages - 1; ++n) {
+  for (int n = 0; n < ST - 1; ++n) {
     if (n < mine) issue(n, n);
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
@@ -205,13 +211,13 @@ __global__ void __launch_bounds__(kFewWarps * 32) xattn_few_kernel(const XAttnIt
 
   int stage = 0;
   for (int n = 0; n < mine; ++n) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(kFewStages - 2) : "memory");
+    asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
     __syncwarp();  // every lane's copies of this stage, and the reads of the stage refilled next
-    if (n + kFewStages - 1 < mine) issue(n + kFewStages - 1, stage == 0 ? kFewStages - 1 : stage - 1);
+    if (n + ST - 1 < mine) issue(n + ST - 1, stage == 0 ? ST - 1 : stage - 1);
     asm volatile("cp.async.commit_group;" ::: "memory");
-    const uint32_t live = live_of[warp * kFewStages + stage];
+    const uint32_t live = live_of[warp * ST + stage];
     const uint32_t K = ring + stage * kFewStageBytes<DP>, V = K + kFewKeys * DP * 2;
-    if (++stage == kFewStages) stage = 0;
+    if (++stage == ST) stage = 0;
     if (!live) continue;
     float s[MT][2][4];
 #pragma unroll
@@ -281,7 +287,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) xattn_few_kernel(const XAttnIt
   // the four warps' results: sums [warp][row][DP], m and l [warp][row]
   constexpr int R = 16 * MT;
   float *so = reinterpret_cast<float *>(sm), *smm = so + kFewWarps * R * DP, *sl = smm + kFewWarps * R;
-  static_assert(kFewWarps * R * (DP + 2) * 4 <= kFewWarps * kFewStages * kFewStageBytes<DP>, "the rings hold the results");
+  static_assert(kFewWarps * R * (DP + 2) * 4 <= kFewWarps * ST * kFewStageBytes<DP>, "the rings hold the results");
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -470,9 +476,10 @@ __device__ __forceinline__ void weights(const uint32_t *s, uint64_t cc, uint64_t
 }
 
 // Up to 128 rows of one request and KV head, tiles of 64 keys.  Warp 0 loads K
-// and V (TMA, a ring each), warps 1 and 3 issue the MMAs of S and of O (waits and issue of both
-// in one warp took longer than a tile's exponentials), warp 2 zeroes the V rows of
-// keys that are not attended to (their weights are zero, but zero times NaN is not),
+// and V (TMA, a ring each), warps 1 and 3 issue the MMAs of S and of O (in one warp
+// their waits delay each other: 157 us on 16 x 1024 x 2048 targets, 146 in two), warp 2
+// (only with a mask) zeroes the V rows of keys that are not attended to (their weights
+// are zero, but zero times NaN is not; without a mask warp 3 does that for the last tile),
 // and warps 4-7 turn scores into weights, a thread a row.  For tile j:
 //   S(j) = Q K_j^T    M128 N64, both K-major in shared memory
 //   P(j) = weights    TMEM, 16 bits, over S(j)
@@ -559,11 +566,11 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     const uint32_t s16 = smem_u32(sm) >> 4, q16 = (s16 + (uint32_t)(L::kQ >> 4)) | (1u << 16);
     const uint64_t hi = umma_desc(sm) & 0xFFFFFFFF00000000ull;
     const int steps = (w.s.D + 15) / 16;
-    if (nt == 0 || warp_sleep_wait(q_full, 0, err)) {
+    if (nt == 0 || warp_wait(q_full, 0, err)) {
       for (int j = 0; j < nt; ++j) {
         const int s = j % ST;
-        if (!warp_sleep_wait(&k_full[s], (uint32_t)((j / ST) & 1), err)) break;
-        if (j >= 2 && !warp_sleep_wait(&pv_done[j & 1], (uint32_t)((j - 2) >> 1) & 1, err)) break;
+        if (!warp_wait(&k_full[s], (uint32_t)((j / ST) & 1), err)) break;
+        if (j >= 2 && !warp_wait(&pv_done[j & 1], (uint32_t)((j - 2) >> 1) & 1, err)) break;
         tc_after();
         const uint32_t k = (s16 + (uint32_t)((L::kK + s * L::kBytes) >> 4)) | (1u << 16);
         const uint32_t id = f16_idesc<T>(covered(j), false), d = tmem + (uint32_t)((j & 1) * kKeys);
@@ -583,7 +590,16 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     const uint32_t id = f16_idesc<T>(DP, true);
     for (int j = 0; j < nt; ++j) {
       const int s = j % ST, n = covered(j) >> 4;
-      if (!warp_sleep_wait(&v_ok[s], (uint32_t)((j / ST) & 1), err) || !warp_sleep_wait(&p_full[j & 1], (uint32_t)(j >> 1) & 1, err)) break;
+      if (!warp_wait(mask ? &v_ok[s] : &v_full[s], (uint32_t)((j / ST) & 1), err)) break;
+      if (!mask && (j + 1) * kKeys > it.klen) {  // the last tile's rows past the item
+        for (int u = lane; u < (16 * n - (it.klen - j * kKeys)) * 8 * L::kAtoms; u += 32) {
+          const int a = u / 8 % L::kAtoms, r = it.klen - j * kKeys + u / (8 * L::kAtoms);
+          *reinterpret_cast<uint4 *>(sm + L::kV + s * L::kBytes + a * L::kAtom + r * 128 + u % 8 * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_async_smem();
+        __syncwarp();
+      }
+      if (!warp_wait(&p_full[j & 1], (uint32_t)(j >> 1) & 1, err)) break;
       tc_after();
       const uint32_t v = (s16 + (uint32_t)((L::kV + s * L::kBytes) >> 4)) | ((uint32_t)(L::kAtom >> 4) << 16);
 #pragma unroll
@@ -593,27 +609,23 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       umma_commit_e(&pv_done[j & 1]);
       umma_commit_e(&v_empty[s]);
     }
-  } else if (warp == 2) {
+  } else if (warp == 2 && mask) {
     for (int j = 0; j < nt; ++j) {
       const int s = j % ST;
-      const bool whole = !mask && (j + 1) * kKeys <= it.klen;
-      Live live{};
-      if (!whole) live = live_keys(mask, it.klen, j, lane);
+      const Live live = live_keys(mask, it.klen, j, lane);
       if (!warp_sleep_wait(&v_full[s], (uint32_t)((j / ST) & 1), err)) break;
-      if (!whole) {
-        const int n = covered(j);
-        // 8 lanes a row, 4 rows at a time
-        for (int r0 = 0; r0 < n; r0 += 4) {
-          const int r = r0 + (lane >> 3);
-          if ((live.w[r >> 5] >> (r & 31)) & 1) continue;
+      const int n = covered(j);
+      // 8 lanes a row, 4 rows at a time
+      for (int r0 = 0; r0 < n; r0 += 4) {
+        const int r = r0 + (lane >> 3);
+        if ((live.w[r >> 5] >> (r & 31)) & 1) continue;
 #pragma unroll
-          for (int a = 0; a < L::kAtoms; ++a)
-            *reinterpret_cast<uint4 *>(sm + L::kV + s * L::kBytes + a * L::kAtom + r * 128 + (lane & 7) * 16) =
-                make_uint4(0, 0, 0, 0);
-        }
-        fence_async_smem();
-        __syncwarp();
+        for (int a = 0; a < L::kAtoms; ++a)
+          *reinterpret_cast<uint4 *>(sm + L::kV + s * L::kBytes + a * L::kAtom + r * 128 + (lane & 7) * 16) =
+              make_uint4(0, 0, 0, 0);
       }
+      fence_async_smem();
+      __syncwarp();
       if (lane == 0) mbar_arrive(&v_ok[s]);
     }
   } else if (warp >= 4) {
@@ -643,7 +655,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       const bool whole = !mask && (j + 1) * kKeys <= it.klen;
       Live live{};
       if (!whole) live = live_keys(mask, it.klen, j, lane);
-      if (!(ok = warp_sleep_wait(&s_full[j & 1], (uint32_t)(j >> 1) & 1, err))) break;
+      if (!(ok = warp_wait(&s_full[j & 1], (uint32_t)(j >> 1) & 1, err))) break;
       tc_after();
       const uint32_t tS = tmem + lanes + (uint32_t)((j & 1) * kKeys);
       uint32_t s[kKeys];
@@ -668,7 +680,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         l *= f;
       }
       if (j > 0 && __any_sync(0xffffffffu, move)) {
-        if (!(ok = warp_sleep_wait(&pv_done[(j - 1) & 1], (uint32_t)((j - 1) >> 1) & 1, err))) break;
+        if (!(ok = warp_wait(&pv_done[(j - 1) & 1], (uint32_t)((j - 1) >> 1) & 1, err))) break;
         tc_after();
 #pragma unroll 1
         for (int q = 0; q < DP / 16; ++q) {
@@ -702,7 +714,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[j & 1]);
     }
-    if (ok && nt > 0) ok = warp_sleep_wait(&pv_done[(nt - 1) & 1], (uint32_t)((nt - 1) >> 1) & 1, err);
+    if (ok && nt > 0) ok = warp_wait(&pv_done[(nt - 1) & 1], (uint32_t)((nt - 1) >> 1) & 1, err);
     if (ok) {
       tc_after();
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
@@ -810,11 +822,11 @@ cudaError_t launch_few(const XAttnItem *items, int n, const XAttnWork &w, const 
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && ready != dev) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem<DP>);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem<DP, MT>);
     if (e == cudaSuccess) ready = dev;
   }
   if (e != cudaSuccess) return e;
-  kernel<<<n, kFewWarps * 32, kFewSmem<DP>, st>>>(items, w, c);
+  kernel<<<n, kFewWarps * 32, kFewSmem<DP, MT>, st>>>(items, w, c);
   return cudaGetLastError();
 }
 
@@ -926,7 +938,7 @@ XAttnSplit cross_attn_split(const XAttnShape &s, const uint64_t *q_start, const 
     if (!keys.empty()) {
       // few rows: a unit is 64 keys (16 a warp); a CTA's start and end cost
       // about as much as 8 of them, a join as 8.  Tiles: 4 of 64 keys, a join 6.
-      const int occ = DP == 64 ? 4 : 2;
+      const int occ = DP == 64 ? out.few_rows <= 16 ? 5 : 3 : 2;
       const int64_t chunk = kind == 0 ? choose_chunk(keys, 64, 8.0, 8.0, sms * occ) : choose_chunk(keys, kKeys, 4.0, 6.0, sms * 2);
       for (XAttnItem it : whole[kind]) {
         const int klen = it.klen, unit = 64;

@@ -55,28 +55,20 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *b, uint32_t parity, int *err
   }
 }
 
-// The same waits for kernels whose waiting warps share the issue slots with busy
-// ones: each poll after the first lets the thread sleep in the barrier unit for up to
-// kHintNs, instead of the short default after which a spinning warp takes
-// issue slots again.
-constexpr uint32_t kHintNs = 20000;
+// The same waits for warps that have time to spare beside busy ones: they sleep
+// between polls and leave the issue slots to the others.
 __device__ __forceinline__ bool mbar_sleep_wait(uint64_t *b, uint32_t parity, int *err) {
   if (mbar_try_wait(b, parity)) return true;
   const uint64_t t0 = globaltimer_ns();
-  for (;;) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(b)), "r"(parity), "r"(kHintNs)
-        : "memory");
-    if (ok) return true;
-    if (*(volatile int *)err) return false;
-    if (globaltimer_ns() - t0 > kWaitNs) {
-      atomicExch(err, 1);
-      return false;
+  for (uint32_t i = 1;; ++i) {
+    __nanosleep(100);
+    if (mbar_try_wait(b, parity)) return true;
+    if ((i & 255) == 0) {
+      if (*(volatile int *)err) return false;
+      if (globaltimer_ns() - t0 > kWaitNs) {
+        atomicExch(err, 1);
+        return false;
+      }
     }
   }
 }
