@@ -489,27 +489,36 @@ __device__ __forceinline__ void weights(const uint32_t *s, uint64_t cc, uint64_t
 // weight is at most 256.
 //
 // The exponentials bind (4 a clock on each SM partition).  Half of TMEM and of
-// the registers make two CTAs an SM: one loads, reduces, starts or ends while the other is
-// at its exponentials.
+// the registers make two CTAs an SM: one loads, reduces or ends while the other
+// is at its exponentials.  CTAs are persistent: K and V tiles keep coming across
+// items, and the next item's Q is fetched while O is waited for and its first S
+// multiplied while O is stored.  Against a CTA for each item: 31 us for 44 on 64 requests
+// of 256 to 512 x 64 to 128 keys (8 heads), 141 for 148 on 16 of 512 to 1024 x 1024 to
+// 2048 (16 heads, 64 dimensions), 62 for 70 on 8 of 1024 x 1500 (8 heads, 128).  Items
+// come longest first and are dealt in snake order.  Barriers of S, P and O count tiles
+// through all items.
 template <typename T, int DP>
 __global__ void __launch_bounds__(kTileThreads, 2)
-    xattn_tile_kernel(const XAttnItem *items, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
-                      XAttnWork w, XAttnCall c, int *err) {
+    xattn_tile_kernel(const XAttnItem *items, int n_items, const __grid_constant__ CUtensorMap mk,
+                      const __grid_constant__ CUtensorMap mv, XAttnWork w, XAttnCall c, int *err) {
   using L = Tile<DP>;
   constexpr int ST = L::kStages;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t *sm = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint64_t *k_full = (uint64_t *)(sm + L::kBar), *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST;
-  uint64_t *v_ok = v_empty + ST, *q_full = v_ok + ST, *s_full = q_full + 1, *p_full = s_full + 2, *pv_done = p_full + 2;
+  uint64_t *v_ok = v_empty + ST, *q_full = v_ok + ST, *o_free = q_full + 1, *s_full = o_free + 1, *p_full = s_full + 2,
+           *pv_done = p_full + 2;
   uint32_t *tmem_slot = (uint32_t *)(pv_done + 2);
   pdl_trigger();
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const XAttnItem it = items[blockIdx.x];
-  const int nt = (it.klen + kKeys - 1) / kKeys;
-  const uint8_t *mask = c.mask ? c.mask + it.k0 : nullptr;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = w.s.H / w.s.KVH, D = w.s.D;
+  // this CTA's item of a round; n_items or more: none
+  auto item_of = [&](int round) {
+    return round * (int)gridDim.x + (int)(round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+  };
+  auto tiles = [](int klen) { return (klen + kKeys - 1) / kKeys; };
   // keys of tile j that the MMAs cover: a multiple of 16
-  auto covered = [&](int j) { return min(kKeys, (it.klen - j * kKeys + 15) & ~15); };
+  auto covered = [](int klen, int j) { return min(kKeys, (klen - j * kKeys + 15) & ~15); };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
@@ -520,6 +529,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       mbar_init(&v_ok[s], 1);
     }
     mbar_init(q_full, 4);
+    mbar_init(o_free, 4);
     for (int b = 0; b < 2; ++b) {  // of even and odd tiles: a wait never lags by two phases
       mbar_init(&s_full[b], 1);
       mbar_init(&p_full[b], 4);
@@ -536,190 +546,231 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   __syncthreads();
   tc_after();
   const uint32_t tmem = *(volatile uint32_t *)tmem_slot;
+  bool ok = true;
 
   if (warp == 0) {
     if (lane == 0) {
-      int k_done = 0, v_done = 0;
-      bool ok = true;
-      for (int j = 0; j < nt && ok; ++j) {
-        const int s = j % ST, row = (int)it.k0 + j * kKeys;
-        const uint32_t ph = (uint32_t)((j / ST) & 1) ^ 1;
-        if (!(ok = mbar_sleep_wait(&k_empty[s], ph, err))) break;
-        mbar_expect_tx(&k_full[s], L::kBytes);
-        for (int a = 0; a < L::kAtoms; ++a)
-          tma_load_3d(sm + L::kK + s * L::kBytes + a * L::kAtom, &mk, &k_full[s], 64 * a, it.kvh, row);
-        ++k_done;
-        if (!(ok = mbar_sleep_wait(&v_empty[s], ph, err))) break;
-        mbar_expect_tx(&v_full[s], L::kBytes);
-        for (int a = 0; a < L::kAtoms; ++a)
-          tma_load_3d(sm + L::kV + s * L::kBytes + a * L::kAtom, &mv, &v_full[s], 64 * a, it.kvh, row);
-        ++v_done;
+      int s = 0, k_done = 0, v_done = 0;  // tiles requested, up to ST
+      uint32_t ph = 0;
+      for (int round = 0, i; ok && (i = item_of(round)) < n_items; ++round) {
+        const int kvh = items[i].kvh, nt = tiles(items[i].klen), row0 = (int)items[i].k0;
+        for (int j = 0; j < nt; ++j) {
+          const int row = row0 + j * kKeys;
+          if (!(ok = mbar_sleep_wait(&k_empty[s], ph ^ 1, err))) break;
+          mbar_expect_tx(&k_full[s], L::kBytes);
+          for (int a = 0; a < L::kAtoms; ++a)
+            tma_load_3d(sm + L::kK + s * L::kBytes + a * L::kAtom, &mk, &k_full[s], 64 * a, kvh, row);
+          k_done = min(k_done + 1, ST);
+          if (!(ok = mbar_sleep_wait(&v_empty[s], ph ^ 1, err))) {
+            mbar_drain(&k_full[s], ph);
+            k_done = min(k_done, ST - 1);
+            break;
+          }
+          mbar_expect_tx(&v_full[s], L::kBytes);
+          for (int a = 0; a < L::kAtoms; ++a)
+            tma_load_3d(sm + L::kV + s * L::kBytes + a * L::kAtom, &mv, &v_full[s], 64 * a, kvh, row);
+          v_done = min(v_done + 1, ST);
+          if (++s == ST) s = 0, ph ^= 1;
+        }
       }
       // no copy may be in flight when the CTA leaves
-      for (int j = max(0, k_done - ST); j < k_done; ++j) mbar_drain(&k_full[j % ST], (uint32_t)((j / ST) & 1));
-      for (int j = max(0, v_done - ST); j < v_done; ++j) mbar_drain(&v_full[j % ST], (uint32_t)((j / ST) & 1));
+      for (int u = 0; u < ST; ++u) {
+        if (s-- == 0) s = ST - 1, ph ^= 1;
+        if (u < k_done) mbar_drain(&k_full[s], ph);
+        if (u < v_done) mbar_drain(&v_full[s], ph);
+      }
     }
     __syncwarp();
   } else if (warp == 1) {
-    // S(j), where P(j-2) was.  Descriptors share their high word; the low one is
+    // S(t), where P(t-2) was.  Descriptors share their high word; the low one is
     // the address / 16 (and, MN-major, the distance of the 64-dimension parts).
     const uint32_t s16 = smem_u32(sm) >> 4, q16 = (s16 + (uint32_t)(L::kQ >> 4)) | (1u << 16);
     const uint64_t hi = umma_desc(sm) & 0xFFFFFFFF00000000ull;
-    const int steps = (w.s.D + 15) / 16;
-    if (nt == 0 || warp_wait(q_full, 0, err)) {
-      for (int j = 0; j < nt; ++j) {
-        const int s = j % ST;
-        if (!warp_wait(&k_full[s], (uint32_t)((j / ST) & 1), err)) break;
-        if (j >= 2 && !warp_wait(&pv_done[j & 1], (uint32_t)((j - 2) >> 1) & 1, err)) break;
+    const int steps = (D + 15) / 16;
+    int t = 0, seen = 0;  // tiles, items with keys
+    for (int round = 0, i; ok && (i = item_of(round)) < n_items; ++round) {
+      const int klen = items[i].klen, nt = tiles(klen);
+      if (nt == 0) continue;
+      ok = warp_wait(q_full, (uint32_t)seen++ & 1, err);
+      for (int j = 0; j < nt && ok; ++j, ++t) {
+        const int s = t % ST;
+        if (!(ok = warp_wait(&k_full[s], (uint32_t)(t / ST) & 1, err))) break;
+        if (t >= 2 && !(ok = warp_wait(&pv_done[t & 1], (uint32_t)((t - 2) >> 1) & 1, err))) break;
         tc_after();
         const uint32_t k = (s16 + (uint32_t)((L::kK + s * L::kBytes) >> 4)) | (1u << 16);
-        const uint32_t id = f16_idesc<T>(covered(j), false), d = tmem + (uint32_t)((j & 1) * kKeys);
+        const uint32_t id = f16_idesc<T>(covered(klen, j), false), d = tmem + (uint32_t)((t & 1) * kKeys);
 #pragma unroll
-        for (int i = 0; i < DP / 16; ++i) {
-          const uint32_t in = (uint32_t)((i & 3) * 2), qa = (i >> 2) * (L::kQAtom >> 4) + in, ka = (i >> 2) * (L::kAtom >> 4) + in;
-          if (i < steps) umma_bf16_e(d, hi | (q16 + qa), hi | (k + ka), id, i ? 1u : 0u);
+        for (int u = 0; u < DP / 16; ++u) {
+          const uint32_t in = (uint32_t)((u & 3) * 2), qa = (u >> 2) * (L::kQAtom >> 4) + in, ka = (u >> 2) * (L::kAtom >> 4) + in;
+          if (u < steps) umma_bf16_e(d, hi | (q16 + qa), hi | (k + ka), id, u ? 1u : 0u);
         }
-        umma_commit_e(&s_full[j & 1]);
+        umma_commit_e(&s_full[t & 1]);
         umma_commit_e(&k_empty[s]);
       }
     }
   } else if (warp == 3) {
-    // O += P(j) V_j
+    // O += P(t) V_j
     const uint32_t s16 = smem_u32(sm) >> 4;
     const uint64_t hi = umma_desc(sm) & 0xFFFFFFFF00000000ull;
     const uint32_t id = f16_idesc<T>(DP, true);
-    for (int j = 0; j < nt; ++j) {
-      const int s = j % ST, n = covered(j) >> 4;
-      if (!warp_wait(mask ? &v_ok[s] : &v_full[s], (uint32_t)((j / ST) & 1), err)) break;
-      if (!mask && (j + 1) * kKeys > it.klen) {  // the last tile's rows past the item
-        for (int u = lane; u < (16 * n - (it.klen - j * kKeys)) * 8 * L::kAtoms; u += 32) {
-          const int a = u / 8 % L::kAtoms, r = it.klen - j * kKeys + u / (8 * L::kAtoms);
-          *reinterpret_cast<uint4 *>(sm + L::kV + s * L::kBytes + a * L::kAtom + r * 128 + u % 8 * 16) = make_uint4(0, 0, 0, 0);
+    int t = 0, seen = 0;
+    for (int round = 0, i; ok && (i = item_of(round)) < n_items; ++round) {
+      const int klen = items[i].klen, nt = tiles(klen);
+      for (int j = 0; j < nt && ok; ++j, ++t) {
+        const int s = t % ST, n = covered(klen, j) >> 4;
+        if (!(ok = warp_wait(c.mask ? &v_ok[s] : &v_full[s], (uint32_t)(t / ST) & 1, err))) break;
+        if (!c.mask && (j + 1) * kKeys > klen) {  // the last tile's rows past the item
+          const int r0 = klen - j * kKeys;
+          for (int u = lane; u < (16 * n - r0) * 8 * L::kAtoms; u += 32)
+            *reinterpret_cast<uint4 *>(sm + L::kV + s * L::kBytes + u / 8 % L::kAtoms * L::kAtom +
+                                       (r0 + u / (8 * L::kAtoms)) * 128 + u % 8 * 16) = make_uint4(0, 0, 0, 0);
+          fence_async_smem();
+          __syncwarp();
+        }
+        if (!(ok = warp_wait(&p_full[t & 1], (uint32_t)(t >> 1) & 1, err))) break;
+        // the last item's O has been read
+        if (j == 0 && seen++ > 0 && !(ok = warp_wait(o_free, (uint32_t)seen & 1, err))) break;
+        tc_after();
+        const uint32_t v = (s16 + (uint32_t)((L::kV + s * L::kBytes) >> 4)) | ((uint32_t)(L::kAtom >> 4) << 16);
+#pragma unroll
+        for (int u = 0; u < kKeys / 16; ++u)
+          if (u < n)
+            umma_bf16_ts_e(tmem + L::kO, tmem + (uint32_t)((t & 1) * kKeys + 8 * u), hi | (v + 128 * u), id, (j | u) ? 1u : 0u);
+        umma_commit_e(&pv_done[t & 1]);
+        umma_commit_e(&v_empty[s]);
+      }
+    }
+  } else if (warp == 2 && c.mask) {
+    int t = 0;
+    for (int round = 0, i; ok && (i = item_of(round)) < n_items; ++round) {
+      const int klen = items[i].klen, nt = tiles(klen);
+      const uint8_t *mask = c.mask + items[i].k0;
+      for (int j = 0; j < nt && ok; ++j, ++t) {
+        const int s = t % ST, n = covered(klen, j);
+        const Live live = live_keys(mask, klen, j, lane);
+        if (!(ok = warp_sleep_wait(&v_full[s], (uint32_t)(t / ST) & 1, err))) break;
+        // 8 lanes a row, 4 rows at a time
+        for (int r0 = 0; r0 < n; r0 += 4) {
+          const int r = r0 + (lane >> 3);
+          if ((live.w[r >> 5] >> (r & 31)) & 1) continue;
+#pragma unroll
+          for (int a = 0; a < L::kAtoms; ++a)
+            *reinterpret_cast<uint4 *>(sm + L::kV + s * L::kBytes + a * L::kAtom + r * 128 + (lane & 7) * 16) =
+                make_uint4(0, 0, 0, 0);
         }
         fence_async_smem();
         __syncwarp();
+        if (lane == 0) mbar_arrive(&v_ok[s]);
       }
-      if (!warp_wait(&p_full[j & 1], (uint32_t)(j >> 1) & 1, err)) break;
-      tc_after();
-      const uint32_t v = (s16 + (uint32_t)((L::kV + s * L::kBytes) >> 4)) | ((uint32_t)(L::kAtom >> 4) << 16);
-#pragma unroll
-      for (int i = 0; i < kKeys / 16; ++i)
-        if (i < n)
-          umma_bf16_ts_e(tmem + L::kO, tmem + (uint32_t)((j & 1) * kKeys + 8 * i), hi | (v + 128 * i), id, (j | i) ? 1u : 0u);
-      umma_commit_e(&pv_done[j & 1]);
-      umma_commit_e(&v_empty[s]);
-    }
-  } else if (warp == 2 && mask) {
-    for (int j = 0; j < nt; ++j) {
-      const int s = j % ST;
-      const Live live = live_keys(mask, it.klen, j, lane);
-      if (!warp_sleep_wait(&v_full[s], (uint32_t)((j / ST) & 1), err)) break;
-      const int n = covered(j);
-      // 8 lanes a row, 4 rows at a time
-      for (int r0 = 0; r0 < n; r0 += 4) {
-        const int r = r0 + (lane >> 3);
-        if ((live.w[r >> 5] >> (r & 31)) & 1) continue;
-#pragma unroll
-        for (int a = 0; a < L::kAtoms; ++a)
-          *reinterpret_cast<uint4 *>(sm + L::kV + s * L::kBytes + a * L::kAtom + r * 128 + (lane & 7) * 16) =
-              make_uint4(0, 0, 0, 0);
-      }
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&v_ok[s]);
     }
   } else if (warp >= 4) {
-    const int quarter = warp & 3, i = quarter * 32 + lane, r = it.r0 + i;  // this thread's row
-    const int G = w.s.H / w.s.KVH, D = w.s.D;
-    const int h = it.kvh * G + r % G;
-    const int64_t row = it.q0 + r / G;
-    const bool mine = i < it.rows;
-    {  // the row of Q, K-major with the 128-byte swizzle
-      const T *q = (const T *)c.q + row * c.q_row + (int64_t)h * c.q_head;
-      uint8_t *dst = sm + L::kQ + i * 128;
-#pragma unroll
-      for (int ch = 0; ch < DP / 8; ++ch) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (mine && ch * 8 < D) v = *reinterpret_cast<const uint4 *>(q + ch * 8);
-        *reinterpret_cast<uint4 *>(dst + (ch >> 3) * L::kQAtom + (((ch & 7) ^ (lane & 7)) << 4)) = v;
-      }
-      fence_async_smem();
-    }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(q_full);
+    const int quarter = warp & 3, i = quarter * 32 + lane;  // this thread's row of an item
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16, tO = tmem + lanes + (uint32_t)L::kO;
     const float sc = c.scale * kLog2e;
-    float m = -INFINITY, l = 0.0f;
-    bool ok = true;
-    for (int j = 0; j < nt; ++j) {
-      const bool whole = !mask && (j + 1) * kKeys <= it.klen;
-      Live live{};
-      if (!whole) live = live_keys(mask, it.klen, j, lane);
-      if (!(ok = warp_wait(&s_full[j & 1], (uint32_t)(j >> 1) & 1, err))) break;
-      tc_after();
-      const uint32_t tS = tmem + lanes + (uint32_t)((j & 1) * kKeys);
-      uint32_t s[kKeys];
-      tmem_ld32_raw(tS, s);
-      tmem_ld32_raw(tS + 32, s + 32);
-      tmem_wait_ld();
-      if (!whole) {
+    // an item's row of Q on its way to shared memory, K-major with the 128-byte swizzle
+    const uint32_t q_to = smem_u32(sm + L::kQ) + i * 128;
+    auto fetch_q = [&](const XAttnItem *it) {
+      const int r = it->r0 + i;
+      const bool mine = i < it->rows;
+      const T *q = (const T *)c.q + (it->q0 + r / G) * c.q_row + (int64_t)(it->kvh * G + r % G) * c.q_head;
 #pragma unroll
-        for (int e = 0; e < kKeys; ++e)
-          if (!((live.w[e >> 5] >> (e & 31)) & 1)) s[e] = 0xff800000u;
+      for (int ch = 0; ch < DP / 8; ++ch) {
+        const bool take = mine && ch * 8 < D;
+        cp16(q_to + (ch >> 3) * L::kQAtom + (((ch & 7) ^ (lane & 7)) << 4), take ? q + ch * 8 : (const T *)c.q, take);
       }
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int e = 0; e < kKeys; e += 2)
-        mx[(e >> 1) & 3] = fmax3(mx[(e >> 1) & 3], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-      const bool move = (top - m) * sc > 8.0f;  // also at the first attended key (m = -inf)
-      float f = 1.0f;
-      if (move) {
-        f = ex2((m - top) * sc);
-        m = top;
-        l *= f;
-      }
-      if (j > 0 && __any_sync(0xffffffffu, move)) {
-        if (!(ok = warp_wait(&pv_done[(j - 1) & 1], (uint32_t)((j - 1) >> 1) & 1, err))) break;
-        tc_after();
-#pragma unroll 1
-        for (int q = 0; q < DP / 16; ++q) {
-          uint32_t o[16];
-          asm volatile(
-              "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-              "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-              : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]), "=r"(o[4]), "=r"(o[5]), "=r"(o[6]), "=r"(o[7]),
-                "=r"(o[8]), "=r"(o[9]), "=r"(o[10]), "=r"(o[11]), "=r"(o[12]), "=r"(o[13]), "=r"(o[14]), "=r"(o[15])
-              : "r"(tO + 16 * q));
-          tmem_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-          tmem_st16(tO + 16 * q, o);
-        }
-      }
-      const float mc = m == -INFINITY ? 0.0f : m * sc;
-      const uint64_t cc = f2pack(sc, sc), nm = f2pack(-mc, -mc);
-      uint64_t sum[2] = {f2pack(0.0f, 0.0f), f2pack(0.0f, 0.0f)};
-#pragma unroll
-      for (int q = 0; q < kKeys / 32; ++q) {
-        uint32_t pw[16];
-        weights<T>(s + 32 * q, cc, nm, pw, sum);
-        tmem_st16(tS + 16 * q, pw);
-      }
-      float l0, l1;
-      f2unpack(fadd2(sum[0], sum[1]), l0, l1);
-      l += l0 + l1;
-      tmem_wait_st();
-      tc_before();
+    };
+    auto have_q = [&] {
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      fence_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[j & 1]);
+      if (lane == 0) mbar_arrive(q_full);
+    };
+    if (item_of(0) < n_items && items[item_of(0)].klen > 0) {
+      fetch_q(items + item_of(0));
+      have_q();
     }
-    if (ok && nt > 0) ok = warp_wait(&pv_done[(nt - 1) & 1], (uint32_t)((nt - 1) >> 1) & 1, err);
-    if (ok) {
+    int t = 0;
+    for (int round = 0, at; ok && (at = item_of(round)) < n_items; ++round) {
+      const int klen = items[at].klen, nt = tiles(klen), next = item_of(round + 1);
+      const uint8_t *mask = c.mask ? c.mask + items[at].k0 : nullptr;
+      float m = -INFINITY, l = 0.0f;
+      for (int j = 0; j < nt; ++j, ++t) {
+        const bool whole = !mask && (j + 1) * kKeys <= klen;
+        Live live{};
+        if (!whole) live = live_keys(mask, klen, j, lane);
+        if (!(ok = warp_wait(&s_full[t & 1], (uint32_t)(t >> 1) & 1, err))) break;
+        tc_after();
+        const uint32_t tS = tmem + lanes + (uint32_t)((t & 1) * kKeys);
+        uint32_t s[kKeys];
+        tmem_ld32_raw(tS, s);
+        tmem_ld32_raw(tS + 32, s + 32);
+        tmem_wait_ld();
+        if (!whole) {
+#pragma unroll
+          for (int e = 0; e < kKeys; ++e)
+            if (!((live.w[e >> 5] >> (e & 31)) & 1)) s[e] = 0xff800000u;
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < kKeys; e += 2)
+          mx[(e >> 1) & 3] = fmax3(mx[(e >> 1) & 3], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        const bool move = (top - m) * sc > 8.0f;  // also at the first attended key (m = -inf)
+        float f = 1.0f;
+        if (move) {
+          f = ex2((m - top) * sc);
+          m = top;
+          l *= f;
+        }
+        if (j > 0 && __any_sync(0xffffffffu, move)) {
+          if (!(ok = warp_wait(&pv_done[(t - 1) & 1], (uint32_t)((t - 1) >> 1) & 1, err))) break;
+          tc_after();
+#pragma unroll 1
+          for (int q = 0; q < DP / 16; ++q) {
+            uint32_t o[16];
+            asm volatile(
+                "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+                "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]), "=r"(o[4]), "=r"(o[5]), "=r"(o[6]), "=r"(o[7]),
+                  "=r"(o[8]), "=r"(o[9]), "=r"(o[10]), "=r"(o[11]), "=r"(o[12]), "=r"(o[13]), "=r"(o[14]), "=r"(o[15])
+                : "r"(tO + 16 * q));
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tmem_st16(tO + 16 * q, o);
+          }
+        }
+        const float mc = m == -INFINITY ? 0.0f : m * sc;
+        const uint64_t cc = f2pack(sc, sc), nm = f2pack(-mc, -mc);
+        uint64_t sum[2] = {f2pack(0.0f, 0.0f), f2pack(0.0f, 0.0f)};
+#pragma unroll
+        for (int q = 0; q < kKeys / 32; ++q) {
+          uint32_t pw[16];
+          weights<T>(s + 32 * q, cc, nm, pw, sum);
+          tmem_st16(tS + 16 * q, pw);
+        }
+        float l0, l1;
+        f2unpack(fadd2(sum[0], sum[1]), l0, l1);
+        l += l0 + l1;
+        tmem_wait_st();
+        tc_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t & 1]);
+      }
+      if (!ok) break;
+      // every S of this item is done: the next one's Q may take its place
+      const bool more = next < n_items && items[next].klen > 0;
+      if (more) fetch_q(items + next);
+      if (nt > 0 && !(ok = warp_wait(&pv_done[(t - 1) & 1], (uint32_t)((t - 1) >> 1) & 1, err))) break;
       tc_after();
+      if (more) have_q();
+      const XAttnItem *it = items + at;
+      const int r = it->r0 + i, h = it->kvh * G + r % G, nsplit = it->nsplit, rows = it->rows;
+      const int64_t row = it->q0 + r / G;
+      const bool mine = i < rows;
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
       T *out = (T *)c.out + row * c.o_row + (int64_t)h * c.o_head;
-      float *p = partial(w, it, it.split, DP);
+      float *p = partial(w, *it, it->split, DP);
 #pragma unroll
       for (int q = 0; q < DP / 32; ++q) {
         uint32_t o[32];
@@ -728,9 +779,14 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         if (nt > 0) {
           tmem_ld32_raw(tO + 32 * q, o);
           tmem_wait_ld();
+          if (q == DP / 32 - 1) {
+            tc_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(o_free);
+          }
         }
         if (!mine) continue;
-        if (it.nsplit > 1) {
+        if (nsplit > 1) {
 #pragma unroll
           for (int e = 0; e < 32; e += 4)
             *reinterpret_cast<uint4 *>(p + (int64_t)i * DP + 32 * q + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
@@ -747,14 +803,15 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         }
       }
       if (mine) {
-        if (it.nsplit > 1) {
-          p[it.rows * DP + i] = m * sc;
-          p[it.rows * (DP + 1) + i] = l;
+        if (nsplit > 1) {
+          p[rows * DP + i] = m * sc;
+          p[rows * (DP + 1) + i] = l;
         } else if (c.lse) {
           c.lse[row * w.s.H + h] = l == 0.0f ? -INFINITY : fmaf(m * sc, kLn2, logf(l));
         }
       }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   }
   __syncwarp();
   tc_before();
@@ -855,7 +912,10 @@ cudaError_t launch_tile(const XAttnItem *items, int n, const XAttnWork &w, const
   if (e == cudaSuccess) e = kv_map(&mk, c.k, s, c.k_row, c.k_head);
   if (e == cudaSuccess) e = kv_map(&mv, c.v, s, c.v_row, c.v_head);
   if (e != cudaSuccess) return e;
-  kernel<<<n, kTileThreads, Tile<DP>::kSmem, st>>>(items, mk, mv, w, c, err);
+  int sms = 0;
+  e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return e;
+  kernel<<<std::min(n, 2 * sms), kTileThreads, Tile<DP>::kSmem, st>>>(items, n, mk, mv, w, c, err);
   return cudaGetLastError();
 }
 

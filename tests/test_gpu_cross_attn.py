@@ -145,6 +145,27 @@ def test_against_64_bits(i, dtype):
     run(q, k, v, mask, qs, ql, ks, kl, dtype, D ** -0.5, layout)
 
 
+@pytest.mark.parametrize("mask", ["none", "random", "padding"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_more_tiles_of_rows_than_fit_at_once(D, mask):
+    """Hundreds of tiles of 128 rows, so that each CTA works through several: of
+    different lengths, some without keys, some wholly masked."""
+    ql = [150 + 7 * i % 90 for i in range(40)]
+    kl = [0 if i % 11 == 3 else (37 * i) % 400 + 1 for i in range(40)]
+    dtype = nb.F16 if D == 64 else nb.BF16
+    q, k, v, m, qs, ks = make(ql, kl, 16, 4, D, dtype, D, 0.6 if mask == "random" else 1.0, gap=2)
+    if mask == "padding":  # what is behind a document's end inside its row, from none of it to all
+        m = torch.ones(k.shape[0], dtype=torch.uint8)
+        for i, (b, n) in enumerate(zip(ks, kl)):
+            m[b + n * (i % 6) // 5:b + n] = 0
+        v[m == 0] = float("nan")
+        k[m == 0] = float("inf")
+    od, ld = run(q, k, torch.nan_to_num(v), m, qs, ql, ks, kl, dtype, D ** -0.5)
+    if mask == "padding":
+        again, _ = run(q, k, v, m, qs, ql, ks, kl, dtype, D ** -0.5, check=False)
+        assert torch.equal(again.view(torch.int16), od.view(torch.int16))
+
+
 @pytest.mark.parametrize("n", [1, 40])
 def test_what_is_masked_changes_nothing(n):
     """NaN, infinities and the lowest value in masked keys, in the rows between requests and behind the last."""
