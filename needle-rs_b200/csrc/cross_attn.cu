@@ -404,14 +404,29 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
 struct Live {
   uint32_t w[kKeys / 32];
 };
-__device__ __forceinline__ Live live_keys(const uint8_t *mask, int klen, int j, int lane) {
-  Live v;
+struct LiveBytes {  // on their way, a lane's
+  uint8_t b[kKeys / 32];
+};
+__device__ __forceinline__ LiveBytes live_load(const uint8_t *mask, int klen, int j, int lane) {
+  LiveBytes v;
 #pragma unroll
   for (int q = 0; q < kKeys / 32; ++q) {
     const int i = j * kKeys + 32 * q + lane;
-    v.w[q] = __ballot_sync(0xffffffffu, i < klen && (!mask || mask[i] != 0));
+    v.b[q] = i >= klen ? 0 : mask ? mask[i] : 1;
   }
   return v;
+}
+__device__ __forceinline__ Live live_bits(const LiveBytes &b) {
+  Live v;
+#pragma unroll
+  for (int q = 0; q < kKeys / 32; ++q) v.w[q] = __ballot_sync(0xffffffffu, b.b[q] != 0);
+  return v;
+}
+__device__ __forceinline__ bool all_live(const Live &v) {
+  uint32_t a = 0xffffffffu;
+#pragma unroll
+  for (int q = 0; q < kKeys / 32; ++q) a &= v.w[q];
+  return a == 0xffffffffu;
 }
 
 // 2^t for a pair of t on the FMA units: t = j + f with j = round(t), 2^f on
@@ -479,7 +494,9 @@ __device__ __forceinline__ void weights(const uint32_t *s, uint64_t cc, uint64_t
 // and V (TMA, a ring each), warps 1 and 3 issue the MMAs of S and of O (in one warp
 // their waits delay each other: 157 us on 16 x 1024 x 2048 targets, 146 in two), warp 2
 // (only with a mask) zeroes the V rows of keys that are not attended to (their weights
-// are zero, but zero times NaN is not; without a mask warp 3 does that for the last tile),
+// are zero, but zero times NaN is not; without a mask warp 3 does that for the last tile;
+// its mask bytes come a tile ahead and its stores are predicated, not looped over: with
+// half of 1024 to 2048 keys masked 171 us for 220),
 // and warps 4-7 turn scores into weights, a thread a row.  For tile j:
 //   S(j) = Q K_j^T    M128 N64, both K-major in shared memory
 //   P(j) = weights    TMEM, 16 bits, over S(j)
@@ -645,18 +662,24 @@ __global__ void __launch_bounds__(kTileThreads, 2)
     for (int round = 0, i; ok && (i = item_of(round)) < n_items; ++round) {
       const int klen = items[i].klen, nt = tiles(klen);
       const uint8_t *mask = c.mask + items[i].k0;
+      LiveBytes ahead = live_load(mask, klen, 0, lane);
       for (int j = 0; j < nt && ok; ++j, ++t) {
-        const int s = t % ST, n = covered(klen, j);
-        const Live live = live_keys(mask, klen, j, lane);
-        if (!(ok = warp_sleep_wait(&v_full[s], (uint32_t)(t / ST) & 1, err))) break;
-        // 8 lanes a row, 4 rows at a time
-        for (int r0 = 0; r0 < n; r0 += 4) {
-          const int r = r0 + (lane >> 3);
-          if ((live.w[r >> 5] >> (r & 31)) & 1) continue;
+        const int s = t % ST;
+        const Live live = live_bits(ahead);
+        ahead = live_load(mask, klen, j + 1, lane);
+        if (!(ok = warp_wait(&v_full[s], (uint32_t)(t / ST) & 1, err))) break;
+        if (!all_live(live)) {  // 8 lanes a row, 4 rows at a time
+          uint8_t *to = sm + L::kV + s * L::kBytes + lane * 16;
 #pragma unroll
-          for (int a = 0; a < L::kAtoms; ++a)
-            *reinterpret_cast<uint4 *>(sm + L::kV + s * L::kBytes + a * L::kAtom + r * 128 + (lane & 7) * 16) =
-                make_uint4(0, 0, 0, 0);
+          for (int q = 0; q < kKeys / 32; ++q) {
+            const uint32_t bits = live.w[q] >> (lane >> 3);
+#pragma unroll
+            for (int r = 0; r < 32; r += 4)
+              if (!((bits >> r) & 1))
+#pragma unroll
+                for (int a = 0; a < L::kAtoms; ++a)
+                  *reinterpret_cast<uint4 *>(to + a * L::kAtom + (32 * q + r) * 128) = make_uint4(0, 0, 0, 0);
+          }
         }
         fence_async_smem();
         __syncwarp();
@@ -694,10 +717,11 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       const int klen = items[at].klen, nt = tiles(klen), next = item_of(round + 1);
       const uint8_t *mask = c.mask ? c.mask + items[at].k0 : nullptr;
       float m = -INFINITY, l = 0.0f;
+      // the bytes of a tile's mask are fetched a tile ahead
+      Live live = live_bits(live_load(mask, klen, 0, lane));
       for (int j = 0; j < nt; ++j, ++t) {
-        const bool whole = !mask && (j + 1) * kKeys <= klen;
-        Live live{};
-        if (!whole) live = live_keys(mask, klen, j, lane);
+        const bool whole = all_live(live);
+        const LiveBytes ahead = live_load(mask, klen, j + 1, lane);
         if (!(ok = warp_wait(&s_full[t & 1], (uint32_t)(t >> 1) & 1, err))) break;
         tc_after();
         const uint32_t tS = tmem + lanes + (uint32_t)((t & 1) * kKeys);
@@ -754,6 +778,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         l += l0 + l1;
         tmem_wait_st();
         tc_before();
+        live = live_bits(ahead);
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[t & 1]);
       }
