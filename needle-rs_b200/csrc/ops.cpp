@@ -26,14 +26,19 @@ bool fail(const std::string &msg) {
   return false;
 }
 
+// An error that is reported here must not come back as the result of a later
+// call's launch.
 bool ok(cudaError_t e) {
+  if (e != cudaSuccess) cudaGetLastError();
   return e == cudaSuccess || fail(std::string("CUDA error: ") + cudaGetErrorString(e));
 }
 
-// Makes `device` current for a call and puts the caller's device back.
+// Makes `device` current for a call and puts the caller's device back.  What an
+// earlier call of the library left as the thread's last error is dropped.
 class OnDevice {
  public:
   explicit OnDevice(int device) {
+    cudaGetLastError();
     good_ = ok(cudaGetDevice(&before_));
     if (good_ && before_ != device) {
       good_ = ok(cudaSetDevice(device));

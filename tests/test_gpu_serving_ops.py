@@ -144,3 +144,15 @@ def test_two_layers_on_two_streams():
         layer.verify()
         for a, b in zip(w, layer.results()):
             assert torch.equal(a, b)
+
+
+def test_an_error_is_reported_once():
+    """A failed allocation is not the next call's result."""
+    w, s = torch.zeros((16, 1 << 17), dtype=torch.int8, device="cuda"), torch.zeros(16, device="cuda")
+    x, pre, h = torch.ones((2, 64), device="cuda"), torch.zeros(64, device="cuda"), torch.empty((2, 64), device="cuda")
+    for _ in range(2):
+        with pytest.raises(nb.NeedleError, match="CUDA error"):
+            nb.Int8Plan(w.data_ptr(), s.data_ptr(), 131071, 16, 1 << 30)  # 128 TiB of rows
+        nb.residual_norm(x.data_ptr(), nb.F32, None, nb.F32, 2, 64, pre.data_ptr(), None, h.data_ptr(), nb.F32)
+    torch.cuda.synchronize()
+    assert torch.isfinite(h).all()
