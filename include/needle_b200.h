@@ -274,7 +274,9 @@ void needle_ffn_plan_free(NeedleFfnPlan *plan);
  * device), whatever device is current, and restore the current one.  `stream`
  * (cudaStream_t or NULL) must belong to that device.  Every call but the
  * plans' creation is asynchronous, allocates nothing and can be captured into
- * a CUDA graph.  Sizes of zero are refused unless a comment says otherwise. */
+ * a CUDA graph.  Sizes of zero are refused unless a comment says otherwise;
+ * counts of rows and channels go up to 2^31 - 256.  A graph that captured a
+ * plan's calls must not be replayed after the plan is freed. */
 
 /* Element types of the operands below. */
 #define NEEDLE_F32 0
@@ -369,7 +371,8 @@ int needle_residual_norm(const void *x, int x_dtype, size_t ldx, const void *y, 
  * to dtype for the product with V); head_dim a multiple of 8 up to 128.
  * The plan holds the split of the requests over the device and the
  * workspace: lengths stay fixed while a prompt is decoded, so one plan serves
- * every layer and step. */
+ * every layer and step.  It belongs to the device that is current when it is
+ * created. */
 typedef struct NeedleCrossAttnPlan NeedleCrossAttnPlan;
 NeedleCrossAttnPlan *needle_cross_attn_plan_create(const uint64_t *q_start, const uint64_t *q_len,
                                                    const uint64_t *k_start, const uint64_t *k_len, size_t n_seq,

@@ -993,6 +993,11 @@ int64_t choose_chunk(const std::vector<int64_t> &keys, int unit, double fixed, d
 
 }  // namespace
 
+// rows of a work item of a request with `rows` rows for each KV head
+static int step_of(int64_t rows) { return rows <= kFewMaxRows ? kFewRows : kRows; }
+
+int64_t cross_attn_items(int64_t rows) { return (rows + step_of(rows) - 1) / step_of(rows); }
+
 XAttnSplit cross_attn_split(const XAttnShape &s, const uint64_t *q_start, const uint64_t *q_len, const uint64_t *k_start,
                             const uint64_t *k_len, size_t n_seq, int sms) {
   const int G = s.H / s.KVH, DP = s.D <= 64 ? 64 : 128;
@@ -1000,7 +1005,7 @@ XAttnSplit cross_attn_split(const XAttnShape &s, const uint64_t *q_start, const 
   XAttnSplit out;
   for (size_t i = 0; i < n_seq; ++i) {
     const int64_t rows = (int64_t)q_len[i] * G;
-    const int kind = rows <= kFewMaxRows ? 0 : 1, step = kind == 0 ? kFewRows : kRows;
+    const int kind = rows <= kFewMaxRows ? 0 : 1, step = step_of(rows);
     for (int64_t r0 = 0; r0 < rows; r0 += step)
       for (int g = 0; g < s.KVH; ++g) {
         XAttnItem it{};

@@ -86,7 +86,8 @@ bool aligned(const void *p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 // Natural alignment of an operand of element type t.
 bool natural(const void *p, int t) { return aligned(p, dtype_size(t)); }
 
-constexpr size_t kMaxRows = 0x7fffffff;
+constexpr size_t kMaxRows = 0x7fffff00;  // whole tiles of 256 rows still count in 31 bits
+constexpr int64_t kMaxItems = 1 << 26;    // of a cross attention plan: 3 GB
 constexpr size_t kMaxStride = (size_t)1 << 36;  // elements
 
 // Runs f, turning a C++ exception into an error.
@@ -339,12 +340,14 @@ NeedleCrossAttnPlan *needle_cross_attn_plan_create(const uint64_t *q_start, cons
     if (D == 0 || D > 128 || D % 8) return fail("cross attention: head_dim must be a multiple of 8 up to 128");
     if (KVH == 0 || H == 0 || H % KVH || H > 4096)
       return fail("cross attention: num_heads must be a multiple of num_kv_heads, up to 4096");
-    int64_t q_rows = 0, k_rows = 0;
+    int64_t q_rows = 0, k_rows = 0, items = 0;
     std::vector<std::pair<uint64_t, uint64_t>> spans;
     for (size_t i = 0; i < n_seq; ++i) {
       if (q_start[i] > kMaxRows || q_len[i] > kMaxRows - q_start[i] || k_start[i] > kMaxRows ||
           k_len[i] > kMaxRows - k_start[i] || q_len[i] * (H / KVH) > kMaxRows)
-        return fail("cross attention: request " + std::to_string(i) + " has rows past 2^31 - 1");
+        return fail("cross attention: request " + std::to_string(i) + " has rows past 2^31 - 256");
+      items += cross_attn_items((int64_t)(q_len[i] * (H / KVH))) * (int64_t)KVH;
+      if (items > kMaxItems) return fail("cross attention: too many rows and heads for one plan");
       if (q_len[i]) {
         spans.emplace_back(q_start[i], q_start[i] + q_len[i]);
         q_rows = std::max(q_rows, (int64_t)(q_start[i] + q_len[i]));
@@ -362,7 +365,6 @@ NeedleCrossAttnPlan *needle_cross_attn_plan_create(const uint64_t *q_start, cons
       return false;
     plan->work.s = XAttnShape{(int)H, (int)KVH, (int)D, dtype, k_rows};
     const XAttnSplit split = cross_attn_split(plan->work.s, q_start, q_len, k_start, k_len, n_seq, sms);
-    if (split.items.size() > kMaxRows) return fail("cross attention: too many rows for one plan");
     const size_t ib = (split.items.size() * sizeof(XAttnItem) + 255) / 256 * 256;
     if (!ok(cudaMalloc(&plan->buf, ib + (size_t)split.ws_floats * sizeof(float) + 256))) return false;
     plan->flag = (int *)((char *)plan->buf + ib);

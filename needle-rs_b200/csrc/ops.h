@@ -98,6 +98,8 @@ struct XAttnSplit {
   int64_t ws_floats = 0;
   int few_rows = 0, group_rows = 0;  // most rows of a few-row item, of a group
 };
+// Items, before splits, of a KV head of a request with `rows` rows for each.
+int64_t cross_attn_items(int64_t rows);
 XAttnSplit cross_attn_split(const XAttnShape &s, const uint64_t *q_start, const uint64_t *q_len, const uint64_t *k_start,
                             const uint64_t *k_len, size_t n_seq, int sms);
 // The same on the device, with its workspace.

@@ -100,3 +100,18 @@ def test_cross_attn_plan_lists_of_one_length():
     a = np.zeros(1, np.uint64)
     p = a.ctypes.data_as(C.c_void_p)
     assert not L.needle_cross_attn_plan_create(None, p, p, p, 1, 8, 4, 64, nb.BF16, None)
+
+
+@pytest.mark.parametrize("ql,n,H,KVH", [([(1 << 31) - 4096], 1, 64, 64), ([64] * 20000, 20000, 4096, 4096)])
+def test_cross_attn_plan_refuses_more_rows_than_it_can_list(ql, n, H, KVH):
+    """Before the list is made: it would not fit the host's memory."""
+    at = list(np.cumsum([0] + ql[:-1]))
+    refused("too many rows", nb.CrossAttnPlan, at, ql, [0] * n, [9] * n, H, KVH, 64, nb.BF16)
+
+
+def test_rows_stop_at_whole_tiles_below_31_bits():
+    """Counts of rows are rounded up to tiles of 256 in 32 bits."""
+    refused("invalid plan", nb.Int8Plan, P, P, 64, 8, (1 << 31) - 255)
+    refused("invalid plan", nb.Int8Plan, P, P, 64, (1 << 31) - 255, 8)
+    refused("invalid quantize", nb.int8_quantize_tokens, P, (1 << 31) - 255, 64, P, P, nb.F32)
+    refused("past 2", nb.CrossAttnPlan, [0], [4], [0], [(1 << 31) - 255], 8, 4, 64, nb.BF16)
