@@ -73,6 +73,8 @@ constexpr int kFewCtas = DP == 64 ? (MT == 1 ? 5 : 3) : 2;
 // Rows of an item, and of a request and KV head that this kernel takes.
 constexpr int kFewRows = 32, kFewMaxRows = 64;
 
+__host__ __device__ constexpr int few_dp(int ks) { return ks <= 4 ? 64 : 128; }
+
 template <int DP>
 constexpr int kFewStageBytes = 2 * kFewKeys * DP * 2;  // K and V rows of 16 keys
 template <int DP, int MT>
@@ -118,9 +120,13 @@ __device__ __forceinline__ void mma16<__nv_bfloat16>(float *d, const uint32_t *a
 // past D are written as zeros by the copies themselves, so nothing that they
 // hold can reach a product.  Ring rows are swizzled (16-byte chunk c of row r
 // at c ^ (r & 7)): ldmatrix reads them without bank conflicts.
-template <typename T, int DP, int MT>
-__global__ void __launch_bounds__(kFewWarps * 32, kFewCtas<DP, MT>) xattn_few_kernel(const XAttnItem *items, XAttnWork w, XAttnCall c) {
-  constexpr int ST = kFewStages<DP, MT>, CH = DP / 8, KS = DP / 16;  // 16-byte chunks of a row, MMA steps over the dimensions
+// KS: steps of 16 dimensions, 4, 6 or 8; a stage's rows have 64 or 128.  (24 requests of
+// 1 to 17 tokens x 3 heads of 80 dimensions over up to 511 keys: 14.3 us in 6 steps and
+// with the warps' results 8 floats apart in shared memory, 18.6 in 8 steps and
+// without, 18.4 with steps that end at D: branches keep loads and products apart.)
+template <typename T, int KS, int MT>
+__global__ void __launch_bounds__(kFewWarps * 32, kFewCtas<few_dp(KS), MT>) xattn_few_kernel(const XAttnItem *items, XAttnWork w, XAttnCall c) {
+  constexpr int DP = few_dp(KS), ST = kFewStages<DP, MT>, CH = DP / 8;  // CH: 16-byte chunks of a row
   extern __shared__ __align__(128) uint8_t sm[];
   uint32_t *live_of = reinterpret_cast<uint32_t *>(sm + kFewWarps * ST * kFewStageBytes<DP>);
   pdl_trigger();
@@ -198,11 +204,11 @@ __global__ void __launch_bounds__(kFewWarps * 32, kFewCtas<DP, MT>) xattn_few_ke
     }
 
   const float sc = c.scale * kLog2e;
-  float o[MT][DP / 8][4], m[MT][2], l[MT][2];
+  float o[MT][2 * KS][4], m[MT][2], l[MT][2];
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
-    for (int n = 0; n < DP / 8; ++n)
+    for (int n = 0; n < 2 * KS; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[mt][n][i] = 0.0f;
     m[mt][0] = m[mt][1] = -INFINITY;
@@ -256,7 +262,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, kFewCtas<DP, MT>) xattn_few_ke
           m[mt][h] = mx;
           l[mt][h] *= f;
 #pragma unroll
-          for (int n = 0; n < DP / 8; ++n) {
+          for (int n = 0; n < 2 * KS; ++n) {
             o[mt][n][2 * h] *= f;
             o[mt][n][2 * h + 1] *= f;
           }
@@ -284,10 +290,11 @@ __global__ void __launch_bounds__(kFewWarps * 32, kFewCtas<DP, MT>) xattn_few_ke
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();  // the rings are free
 
-  // the four warps' results: sums [warp][row][DP], m and l [warp][row]
-  constexpr int R = 16 * MT;
-  float *so = reinterpret_cast<float *>(sm), *smm = so + kFewWarps * R * DP, *sl = smm + kFewWarps * R;
-  static_assert(kFewWarps * R * (DP + 2) * 4 <= kFewWarps * ST * kFewStageBytes<DP>, "the rings hold the results");
+  // the four warps' results: sums [warp][row][DP] (rows 8 floats apart in banks:
+  // a quarter of a warp's stores meet no other's), m and l [warp][row]
+  constexpr int R = 16 * MT, LD = DP + 8;
+  float *so = reinterpret_cast<float *>(sm), *smm = so + kFewWarps * R * LD, *sl = smm + kFewWarps * R;
+  static_assert(kFewWarps * R * (LD + 2) * 4 <= kFewWarps * ST * kFewStageBytes<DP>, "the rings hold the results");
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -302,29 +309,32 @@ __global__ void __launch_bounds__(kFewWarps * 32, kFewCtas<DP, MT>) xattn_few_ke
         sl[warp * R + i] = lr;
       }
 #pragma unroll
-      for (int n = 0; n < DP / 8; ++n)
-        *reinterpret_cast<float2 *>(so + (warp * R + i) * DP + n * 8 + 2 * t) =
+      for (int n = 0; n < 2 * KS; ++n)
+        *reinterpret_cast<float2 *>(so + (warp * R + i) * LD + n * 8 + 2 * t) =
             make_float2(o[mt][n][2 * h], o[mt][n][2 * h + 1]);
     }
   __syncthreads();
-  for (int u = threadIdx.x; u < it.rows * (DP / 2); u += kFewWarps * 32) {
-    const int i = u / (DP / 2), d = u % (DP / 2) * 2;
-    if (d >= D) continue;
-    float M = -INFINITY, L = 0.0f, x0 = 0.0f, x1 = 0.0f;
+  const int quads = D / 4;  // 4 dimensions a thread
+  for (int u = threadIdx.x; u < it.rows * quads; u += kFewWarps * 32) {
+    const int i = u / quads, d = u % quads * 4;
+    float mw[kFewWarps], M = -INFINITY, L = 0.0f;
 #pragma unroll
-    for (int a = 0; a < kFewWarps; ++a) M = fmaxf(M, smm[a * R + i]);
+    for (int a = 0; a < kFewWarps; ++a) M = fmaxf(M, mw[a] = smm[a * R + i]);
     const float base = M == -INFINITY ? 0.0f : M;
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
     for (int a = 0; a < kFewWarps; ++a) {
-      const float f = ex2(smm[a * R + i] - base);
-      const float2 v = *reinterpret_cast<const float2 *>(so + (a * R + i) * DP + d);
+      const float f = ex2(mw[a] - base);
+      const float4 v = *reinterpret_cast<const float4 *>(so + (a * R + i) * LD + d);
       L += f * sl[a * R + i];
-      x0 += f * v.x;
-      x1 += f * v.y;
+      x.x += f * v.x;
+      x.y += f * v.y;
+      x.z += f * v.z;
+      x.w += f * v.w;
     }
     if (it.nsplit > 1) {
       float *p = partial(w, it, it.split, DP);
-      *reinterpret_cast<float2 *>(p + i * DP + d) = make_float2(x0, x1);
+      *reinterpret_cast<float4 *>(p + i * DP + d) = x;
       if (d == 0) {
         p[it.rows * DP + i] = M;
         p[it.rows * (DP + 1) + i] = L;
@@ -334,7 +344,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, kFewCtas<DP, MT>) xattn_few_ke
     const int r = it.r0 + i, h = it.kvh * G + r % G;
     const int64_t row = it.q0 + r / G;
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;  // no key: zeros
-    *reinterpret_cast<uint32_t *>((T *)c.out + row * c.o_row + (int64_t)h * c.o_head + d) = pack2<T>(x0 * inv, x1 * inv);
+    *reinterpret_cast<uint2 *>((T *)c.out + row * c.o_row + (int64_t)h * c.o_head + d) =
+        make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
     if (d == 0 && c.lse) c.lse[row * w.s.H + h] = L == 0.0f ? -INFINITY : fmaf(M, kLn2, logf(L));
   }
 }
@@ -896,10 +907,10 @@ __global__ void xattn_join_kernel(const XAttnItem *groups, XAttnWork w, XAttnCal
 
 // ── launches ────────────────────────────────────────────────────────────────
 
-template <typename T, int DP, int MT>
+template <typename T, int KS, int MT>
 cudaError_t launch_few(const XAttnItem *items, int n, const XAttnWork &w, const XAttnCall &c, cudaStream_t st) {
-  if (n == 0) return cudaSuccess;
-  auto *kernel = xattn_few_kernel<T, DP, MT>;
+  auto *kernel = xattn_few_kernel<T, KS, MT>;
+  constexpr int DP = few_dp(KS);
   static thread_local int ready = -1;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -948,8 +959,14 @@ template <typename T, int DP>
 cudaError_t run(const XAttnWork &w, const XAttnCall &c, int *err, cudaStream_t st) {
   const XAttnItem *few = w.items, *tile = few + w.n_few, *groups = tile + w.n_tile;
   cudaError_t e = launch_tile<T, DP>(tile, w.n_tile, w, c, err, st);
-  if (e == cudaSuccess)
-    e = w.few_rows <= 16 ? launch_few<T, DP, 1>(few, w.n_few, w, c, st) : launch_few<T, DP, 2>(few, w.n_few, w, c, st);
+  if (e == cudaSuccess && w.n_few) {
+    if (DP == 128 && w.s.D <= 96)
+      e = w.few_rows <= 16 ? launch_few<T, DP == 128 ? 6 : 4, 1>(few, w.n_few, w, c, st)
+                           : launch_few<T, DP == 128 ? 6 : 4, 2>(few, w.n_few, w, c, st);
+    else
+      e = w.few_rows <= 16 ? launch_few<T, DP / 16, 1>(few, w.n_few, w, c, st)
+                           : launch_few<T, DP / 16, 2>(few, w.n_few, w, c, st);
+  }
   if (e != cudaSuccess || w.n_groups == 0) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)w.n_groups, (unsigned)((w.group_rows + 7) / 8));
