@@ -65,11 +65,13 @@ __device__ __forceinline__ float *partial(const XAttnWork &w, const XAttnItem &i
 
 constexpr int kFewWarps = 4, kFewKeys = 16;
 // Stages of a warp's ring: two, and 5 CTAs an SM, where registers allow that
-// many (256 decode requests: 16.6 us, with three 17.7), else three.
-template <int DP, int MT>
-constexpr int kFewStages = DP == 64 && MT == 1 ? 2 : 3;
-template <int DP, int MT>
-constexpr int kFewCtas = DP == 64 ? (MT == 1 ? 5 : 3) : 2;
+// many (256 decode requests: 16.6 us, with three 17.7), else three.  LONE, a CTA an SM
+// at most: five, since nothing else covers a load's latency (8 heads of 64 over 512 keys:
+// one request 7.4 us for 8.5, 32 requests 8.0 for 9.4; four stages and six the same).
+template <int DP, int MT, bool LONE>
+constexpr int kFewStages = LONE ? 5 : DP == 64 && MT == 1 ? 2 : 3;
+template <int DP, int MT, bool LONE>
+constexpr int kFewCtas = LONE ? 1 : DP == 64 ? (MT == 1 ? 5 : 3) : 2;
 // Rows of an item, and of a request and KV head that this kernel takes.
 constexpr int kFewRows = 32, kFewMaxRows = 64;
 
@@ -77,8 +79,8 @@ __host__ __device__ constexpr int few_dp(int ks) { return ks <= 4 ? 64 : 128; }
 
 template <int DP>
 constexpr int kFewStageBytes = 2 * kFewKeys * DP * 2;  // K and V rows of 16 keys
-template <int DP, int MT>
-constexpr int kFewSmem = kFewWarps * kFewStages<DP, MT> * (kFewStageBytes<DP> + 4);
+template <int DP, int MT, bool LONE>
+constexpr int kFewSmem = kFewWarps * kFewStages<DP, MT, LONE> * (kFewStageBytes<DP> + 4);
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool take) {
   const int n = take ? 16 : 0;  // 0: the 16 bytes become zero and src is not read
@@ -124,9 +126,10 @@ __device__ __forceinline__ void mma16<__nv_bfloat16>(float *d, const uint32_t *a
 // 1 to 17 tokens x 3 heads of 80 dimensions over up to 511 keys: 14.3 us in 6 steps and
 // with the warps' results 8 floats apart in shared memory, 18.6 in 8 steps and
 // without, 18.4 with steps that end at D: branches keep loads and products apart.)
-template <typename T, int KS, int MT>
-__global__ void __launch_bounds__(kFewWarps * 32, kFewCtas<few_dp(KS), MT>) xattn_few_kernel(const XAttnItem *items, XAttnWork w, XAttnCall c) {
-  constexpr int DP = few_dp(KS), ST = kFewStages<DP, MT>, CH = DP / 8;  // CH: 16-byte chunks of a row
+template <typename T, int KS, int MT, bool LONE>
+__global__ void __launch_bounds__(kFewWarps * 32, kFewCtas<few_dp(KS), MT, LONE>)
+    xattn_few_kernel(const XAttnItem *items, XAttnWork w, XAttnCall c) {
+  constexpr int DP = few_dp(KS), ST = kFewStages<DP, MT, LONE>, CH = DP / 8;  // CH: 16-byte chunks of a row
   extern __shared__ __align__(128) uint8_t sm[];
   uint32_t *live_of = reinterpret_cast<uint32_t *>(sm + kFewWarps * ST * kFewStageBytes<DP>);
   pdl_trigger();
@@ -907,20 +910,28 @@ __global__ void xattn_join_kernel(const XAttnItem *groups, XAttnWork w, XAttnCal
 
 // ── launches ────────────────────────────────────────────────────────────────
 
-template <typename T, int KS, int MT>
-cudaError_t launch_few(const XAttnItem *items, int n, const XAttnWork &w, const XAttnCall &c, cudaStream_t st) {
-  auto *kernel = xattn_few_kernel<T, KS, MT>;
-  constexpr int DP = few_dp(KS);
+template <typename T, int KS, int MT, bool LONE>
+cudaError_t launch_few(const XAttnItem *items, const XAttnWork &w, const XAttnCall &c, int dev, cudaStream_t st) {
+  constexpr int kSmem = kFewSmem<few_dp(KS), MT, LONE>;
+  auto *kernel = xattn_few_kernel<T, KS, MT, LONE>;
   static thread_local int ready = -1;
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess && ready != dev) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem<DP, MT>);
-    if (e == cudaSuccess) ready = dev;
+  if (ready != dev) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e != cudaSuccess) return e;
+    ready = dev;
   }
-  if (e != cudaSuccess) return e;
-  kernel<<<n, kFewWarps * 32, kFewSmem<DP, MT>, st>>>(items, w, c);
+  kernel<<<w.n_few, kFewWarps * 32, kSmem, st>>>(items, w, c);
   return cudaGetLastError();
+}
+template <typename T, int KS>
+cudaError_t few_rows(const XAttnItem *items, const XAttnWork &w, const XAttnCall &c, cudaStream_t st) {
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return e;
+  if (w.n_few <= sms)
+    return w.few_rows <= 16 ? launch_few<T, KS, 1, true>(items, w, c, dev, st) : launch_few<T, KS, 2, true>(items, w, c, dev, st);
+  return w.few_rows <= 16 ? launch_few<T, KS, 1, false>(items, w, c, dev, st) : launch_few<T, KS, 2, false>(items, w, c, dev, st);
 }
 
 cudaError_t kv_map(CUtensorMap *map, const void *p, const XAttnShape &s, int64_t row, int64_t head) {
@@ -959,14 +970,8 @@ template <typename T, int DP>
 cudaError_t run(const XAttnWork &w, const XAttnCall &c, int *err, cudaStream_t st) {
   const XAttnItem *few = w.items, *tile = few + w.n_few, *groups = tile + w.n_tile;
   cudaError_t e = launch_tile<T, DP>(tile, w.n_tile, w, c, err, st);
-  if (e == cudaSuccess && w.n_few) {
-    if (DP == 128 && w.s.D <= 96)
-      e = w.few_rows <= 16 ? launch_few<T, DP == 128 ? 6 : 4, 1>(few, w.n_few, w, c, st)
-                           : launch_few<T, DP == 128 ? 6 : 4, 2>(few, w.n_few, w, c, st);
-    else
-      e = w.few_rows <= 16 ? launch_few<T, DP / 16, 1>(few, w.n_few, w, c, st)
-                           : launch_few<T, DP / 16, 2>(few, w.n_few, w, c, st);
-  }
+  if (e == cudaSuccess && w.n_few)
+    e = DP == 128 && w.s.D <= 96 ? few_rows<T, DP == 128 ? 6 : 4>(few, w, c, st) : few_rows<T, DP / 16>(few, w, c, st);
   if (e != cudaSuccess || w.n_groups == 0) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)w.n_groups, (unsigned)((w.group_rows + 7) / 8));
