@@ -9,9 +9,9 @@
 // maximum m and sum l for each row (f32); weights are e^(s - m), rounded to the
 // operands' type for the product with V, whose sums are f32.
 //
-// Two kernels.  Up to 32 rows read K and V from HBM faster than any tensor
+// Two kernels.  Up to 16 rows read K and V from HBM faster than any tensor
 // core needs them: xattn_few_kernel streams them through a ring for each warp
-// and multiplies with mma.sync (16 rows an instruction).  More rows are bound by the
+// and multiplies with mma.sync.  More rows are bound by the
 // exponentials and the products: xattn_tile_kernel runs both on tcgen05 with
 // 128-row tiles in TMEM.
 //
@@ -64,23 +64,27 @@ __device__ __forceinline__ float *partial(const XAttnWork &w, const XAttnItem &i
 // ── few rows ────────────────────────────────────────────────────────────────
 
 constexpr int kFewWarps = 4, kFewKeys = 16;
+// Rows of an item: what one MMA takes.  Two MMAs' rows (17 to 32) were up to a quarter
+// slower than a tile of 128 that is mostly empty (24 requests of 16 tokens x 2 heads of 128
+// over 512 keys: 16.6 us, tile 12.5; 256 of 16 x 2 heads of 64 over 64 to 512: 32.6 and 29.5;
+// 8 of 12 x 2 heads of 64 over 8k to 20k: 35 and 38), two items of 32 half as fast
+// (64 requests of 32 x 2 heads of 64 over 2000 keys: 68 and 37).
+constexpr int kFewRows = 16;
 // Stages of a warp's ring: two, and 5 CTAs an SM, where registers allow that
 // many (256 decode requests: 16.6 us, with three 17.7), else three.  LONE, a CTA an SM
 // at most: five, since nothing else covers a load's latency (8 heads of 64 over 512 keys:
 // one request 7.4 us for 8.5, 32 requests 8.0 for 9.4; four stages and six the same).
-template <int DP, int MT, bool LONE>
-constexpr int kFewStages = LONE ? 5 : DP == 64 && MT == 1 ? 2 : 3;
-template <int DP, int MT, bool LONE>
-constexpr int kFewCtas = LONE ? 1 : DP == 64 ? (MT == 1 ? 5 : 3) : 2;
-// Rows of an item, and of a request and KV head that this kernel takes.
-constexpr int kFewRows = 32, kFewMaxRows = 64;
+template <int DP, bool LONE>
+constexpr int kFewStages = LONE ? 5 : DP == 64 ? 2 : 3;
+template <int DP, bool LONE>
+constexpr int kFewCtas = LONE ? 1 : DP == 64 ? 5 : 2;
 
 __host__ __device__ constexpr int few_dp(int ks) { return ks <= 4 ? 64 : 128; }
 
 template <int DP>
 constexpr int kFewStageBytes = 2 * kFewKeys * DP * 2;  // K and V rows of 16 keys
-template <int DP, int MT, bool LONE>
-constexpr int kFewSmem = kFewWarps * kFewStages<DP, MT, LONE> * (kFewStageBytes<DP> + 4);
+template <int DP, bool LONE>
+constexpr int kFewSmem = kFewWarps * kFewStages<DP, LONE> * (kFewStageBytes<DP> + 4);
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool take) {
   const int n = take ? 16 : 0;  // 0: the 16 bytes become zero and src is not read
@@ -115,7 +119,7 @@ __device__ __forceinline__ void mma16<__nv_bfloat16>(float *d, const uint32_t *a
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Up to 16 * MT rows of one request and KV head.  Each of four warps takes
+// Up to 16 rows of one request and KV head.  Each of four warps takes
 // every fourth block of 16 keys through its own ring of cp.async stages, with
 // its own running maxima: no barrier until the warps' results meet in shared
 // memory at the end.  Rows of masked keys, of keys past the item and dimensions
@@ -126,10 +130,10 @@ __device__ __forceinline__ void mma16<__nv_bfloat16>(float *d, const uint32_t *a
 // 1 to 17 tokens x 3 heads of 80 dimensions over up to 511 keys: 14.3 us in 6 steps and
 // with the warps' results 8 floats apart in shared memory, 18.6 in 8 steps and
 // without, 18.4 with steps that end at D: branches keep loads and products apart.)
-template <typename T, int KS, int MT, bool LONE>
-__global__ void __launch_bounds__(kFewWarps * 32, kFewCtas<few_dp(KS), MT, LONE>)
+template <typename T, int KS, bool LONE>
+__global__ void __launch_bounds__(kFewWarps * 32, kFewCtas<few_dp(KS), LONE>)
     xattn_few_kernel(const XAttnItem *items, XAttnWork w, XAttnCall c) {
-  constexpr int DP = few_dp(KS), ST = kFewStages<DP, MT, LONE>, CH = DP / 8;  // CH: 16-byte chunks of a row
+  constexpr int DP = few_dp(KS), ST = kFewStages<DP, LONE>, CH = DP / 8;  // CH: 16-byte chunks of a row
   extern __shared__ __align__(128) uint8_t sm[];
   uint32_t *live_of = reinterpret_cast<uint32_t *>(sm + kFewWarps * ST * kFewStageBytes<DP>);
   pdl_trigger();
@@ -189,34 +193,27 @@ __global__ void __launch_bounds__(kFewWarps * 32, kFewCtas<few_dp(KS), MT, LONE>
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
 
-  // Q as MMA fragments (rows g and g + 8 of each 16)
-  uint32_t qf[MT][KS][4];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
+  // Q as MMA fragments (rows g and g + 8)
+  uint32_t qf[KS][4];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int i = mt * 16 + h * 8 + g, r = it.r0 + i;
+      const int i = h * 8 + g, r = it.r0 + i;
       const T *q = (const T *)c.q + (it.q0 + r / G) * c.q_row + (int64_t)(it.kvh * G + r % G) * c.q_head;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const int d = ks * 16 + u * 8 + 2 * t;
-          qf[mt][ks][2 * u + h] = i < it.rows && d < D ? *reinterpret_cast<const uint32_t *>(q + d) : 0u;
+          qf[ks][2 * u + h] = i < it.rows && d < D ? *reinterpret_cast<const uint32_t *>(q + d) : 0u;
         }
     }
 
   const float sc = c.scale * kLog2e;
-  float o[MT][2 * KS][4], m[MT][2], l[MT][2];
+  float o[2 * KS][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
+  for (int n = 0; n < 2 * KS; ++n)
 #pragma unroll
-    for (int n = 0; n < 2 * KS; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[mt][n][i] = 0.0f;
-    m[mt][0] = m[mt][1] = -INFINITY;
-    l[mt][0] = l[mt][1] = 0.0f;
-  }
+    for (int i = 0; i < 4; ++i) o[n][i] = 0.0f;
 
   int stage = 0;
   for (int n = 0; n < mine; ++n) {
@@ -228,66 +225,56 @@ __global__ void __launch_bounds__(kFewWarps * 32, kFewCtas<few_dp(KS), MT, LONE>
     const uint32_t K = ring + stage * kFewStageBytes<DP>, V = K + kFewKeys * DP * 2;
     if (++stage == ST) stage = 0;
     if (!live) continue;
-    float s[MT][2][4];
+    float s[2][4];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s[mt][i >> 2][i & 3] = 0.0f;
+    for (int i = 0; i < 8; ++i) s[i >> 2][i & 3] = 0.0f;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       uint32_t kf[4];
       const int row = (lane >> 4) * 8 + (lane & 7), ch = 2 * ks + ((lane >> 3) & 1);
       ldm4(kf, K + row * (DP * 2) + ((ch ^ (row & 7)) << 4));
+      mma16<T>(s[0], qf[ks], kf[0], kf[1]);
+      mma16<T>(s[1], qf[ks], kf[2], kf[3]);
+    }
+    uint32_t pf[4];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        mma16<T>(s[mt][0], qf[mt][ks], kf[0], kf[1]);
-        mma16<T>(s[mt][1], qf[mt][ks], kf[2], kf[3]);
+    for (int h = 0; h < 2; ++h) {  // row g, then g + 8
+      float mx = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          float &x = s[n][2 * h + u];
+          if (!((live >> (n * 8 + 2 * t + u)) & 1)) x = -INFINITY;
+          mx = fmaxf(mx, x);
+        }
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      if (mx > m[h]) {
+        const float f = ex2((m[h] - mx) * sc);
+        m[h] = mx;
+        l[h] *= f;
+#pragma unroll
+        for (int n = 0; n < 2 * KS; ++n) {
+          o[n][2 * h] *= f;
+          o[n][2 * h + 1] *= f;
+        }
+      }
+      const float base = m[h] == -INFINITY ? 0.0f : m[h] * sc;
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const float p0 = ex2(fmaf(s[n][2 * h], sc, -base)), p1 = ex2(fmaf(s[n][2 * h + 1], sc, -base));
+        l[h] += p0 + p1;
+        pf[2 * n + h] = pack2<T>(p0, p1);
       }
     }
-    uint32_t pf[MT][4];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {  // row g, then g + 8
-        float mx = -INFINITY;
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            float &x = s[mt][n][2 * h + u];
-            if (!((live >> (n * 8 + 2 * t + u)) & 1)) x = -INFINITY;
-            mx = fmaxf(mx, x);
-          }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        if (mx > m[mt][h]) {
-          const float f = ex2((m[mt][h] - mx) * sc);
-          m[mt][h] = mx;
-          l[mt][h] *= f;
-#pragma unroll
-          for (int n = 0; n < 2 * KS; ++n) {
-            o[mt][n][2 * h] *= f;
-            o[mt][n][2 * h + 1] *= f;
-          }
-        }
-        const float base = m[mt][h] == -INFINITY ? 0.0f : m[mt][h] * sc;
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const float p0 = ex2(fmaf(s[mt][n][2 * h], sc, -base)), p1 = ex2(fmaf(s[mt][n][2 * h + 1], sc, -base));
-          l[mt][h] += p0 + p1;
-          pf[mt][2 * n + h] = pack2<T>(p0, p1);
-        }
-      }
 #pragma unroll
     for (int nb = 0; nb < KS; ++nb) {
       uint32_t vf[4];
       const int row = ((lane >> 3) & 1) * 8 + (lane & 7), ch = 2 * nb + (lane >> 4);
       ldm4t(vf, V + row * (DP * 2) + ((ch ^ (row & 7)) << 4));
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        mma16<T>(o[mt][2 * nb], pf[mt], vf[0], vf[1]);
-        mma16<T>(o[mt][2 * nb + 1], pf[mt], vf[2], vf[3]);
-      }
+      mma16<T>(o[2 * nb], pf, vf[0], vf[1]);
+      mma16<T>(o[2 * nb + 1], pf, vf[2], vf[3]);
     }
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -295,27 +282,24 @@ __global__ void __launch_bounds__(kFewWarps * 32, kFewCtas<few_dp(KS), MT, LONE>
 
   // the four warps' results: sums [warp][row][DP] (rows 8 floats apart in banks:
   // a quarter of a warp's stores meet no other's), m and l [warp][row]
-  constexpr int R = 16 * MT, LD = DP + 8;
+  constexpr int R = kFewRows, LD = DP + 8;
   float *so = reinterpret_cast<float *>(sm), *smm = so + kFewWarps * R * LD, *sl = smm + kFewWarps * R;
   static_assert(kFewWarps * R * (LD + 2) * 4 <= kFewWarps * ST * kFewStageBytes<DP>, "the rings hold the results");
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int i = mt * 16 + h * 8 + g;
-      float lr = l[mt][h];
-      lr += __shfl_xor_sync(0xffffffffu, lr, 1);
-      lr += __shfl_xor_sync(0xffffffffu, lr, 2);
-      if (i >= it.rows) continue;
-      if (t == 0) {
-        smm[warp * R + i] = m[mt][h] * sc;
-        sl[warp * R + i] = lr;
-      }
-#pragma unroll
-      for (int n = 0; n < 2 * KS; ++n)
-        *reinterpret_cast<float2 *>(so + (warp * R + i) * LD + n * 8 + 2 * t) =
-            make_float2(o[mt][n][2 * h], o[mt][n][2 * h + 1]);
+  for (int h = 0; h < 2; ++h) {
+    const int i = h * 8 + g;
+    float lr = l[h];
+    lr += __shfl_xor_sync(0xffffffffu, lr, 1);
+    lr += __shfl_xor_sync(0xffffffffu, lr, 2);
+    if (i >= it.rows) continue;
+    if (t == 0) {
+      smm[warp * R + i] = m[h] * sc;
+      sl[warp * R + i] = lr;
     }
+#pragma unroll
+    for (int n = 0; n < 2 * KS; ++n)
+      *reinterpret_cast<float2 *>(so + (warp * R + i) * LD + n * 8 + 2 * t) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+  }
   __syncthreads();
   const int quads = D / 4;  // 4 dimensions a thread
   for (int u = threadIdx.x; u < it.rows * quads; u += kFewWarps * 32) {
@@ -910,10 +894,10 @@ __global__ void xattn_join_kernel(const XAttnItem *groups, XAttnWork w, XAttnCal
 
 // ── launches ────────────────────────────────────────────────────────────────
 
-template <typename T, int KS, int MT, bool LONE>
+template <typename T, int KS, bool LONE>
 cudaError_t launch_few(const XAttnItem *items, const XAttnWork &w, const XAttnCall &c, int dev, cudaStream_t st) {
-  constexpr int kSmem = kFewSmem<few_dp(KS), MT, LONE>;
-  auto *kernel = xattn_few_kernel<T, KS, MT, LONE>;
+  constexpr int kSmem = kFewSmem<few_dp(KS), LONE>;
+  auto *kernel = xattn_few_kernel<T, KS, LONE>;
   static thread_local int ready = -1;
   if (ready != dev) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
@@ -929,9 +913,7 @@ cudaError_t few_rows(const XAttnItem *items, const XAttnWork &w, const XAttnCall
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e != cudaSuccess) return e;
-  if (w.n_few <= sms)
-    return w.few_rows <= 16 ? launch_few<T, KS, 1, true>(items, w, c, dev, st) : launch_few<T, KS, 2, true>(items, w, c, dev, st);
-  return w.few_rows <= 16 ? launch_few<T, KS, 1, false>(items, w, c, dev, st) : launch_few<T, KS, 2, false>(items, w, c, dev, st);
+  return w.n_few <= sms ? launch_few<T, KS, true>(items, w, c, dev, st) : launch_few<T, KS, false>(items, w, c, dev, st);
 }
 
 cudaError_t kv_map(CUtensorMap *map, const void *p, const XAttnShape &s, int64_t row, int64_t head) {
@@ -1015,19 +997,29 @@ int64_t choose_chunk(const std::vector<int64_t> &keys, int unit, double fixed, d
 
 }  // namespace
 
-// rows of a work item of a request with `rows` rows for each KV head
-static int step_of(int64_t rows) { return rows <= kFewMaxRows ? kFewRows : kRows; }
-
-int64_t cross_attn_items(int64_t rows) { return (rows + step_of(rows) - 1) / step_of(rows); }
+int64_t cross_attn_items(int64_t rows) { return (rows + kRows - 1) / kRows; }
 
 XAttnSplit cross_attn_split(const XAttnShape &s, const uint64_t *q_start, const uint64_t *q_len, const uint64_t *k_start,
                             const uint64_t *k_len, size_t n_seq, int sms) {
   const int G = s.H / s.KVH, DP = s.D <= 64 ? 64 : 128;
   std::vector<XAttnItem> whole[2];  // few rows, tiles
   XAttnSplit out;
+  // Requests of few rows beside others join them in tiles, which saves a launch that would
+  // wait for theirs, while that adds at most 25 tiles of 64 keys (about as many
+  // microseconds, an item's start and end counted as 4) to each of the CTAs.  24 requests of 1
+  // to 17 tokens x 3 heads of 80 dimensions, up to 511 keys (2 tiles a CTA): 12.6 us, apart
+  // 22.8; nine in ten of 1 token x 2 heads of 64, else 16: 100 requests of 64 to 511 keys (10)
+  // 16.6 and 21.7, 200 (20) 24.4 and 26.8, 400 (41) 43 and 35; 100 of 64 to 4000 (44) 61 and 53.
+  int64_t tiles = 0, added = 0;
   for (size_t i = 0; i < n_seq; ++i) {
     const int64_t rows = (int64_t)q_len[i] * G;
-    const int kind = rows <= kFewMaxRows ? 0 : 1, step = step_of(rows);
+    if (rows > kFewRows) tiles += s.KVH;
+    else if (rows > 0) added += s.KVH * (((int64_t)k_len[i] + kKeys - 1) / kKeys + 4);
+  }
+  const int64_t few_rows = tiles > 0 && added <= 25 * 2 * (int64_t)sms ? 0 : kFewRows;
+  for (size_t i = 0; i < n_seq; ++i) {
+    const int64_t rows = (int64_t)q_len[i] * G;
+    const int kind = rows <= few_rows ? 0 : 1, step = kind == 0 ? kFewRows : kRows;
     for (int64_t r0 = 0; r0 < rows; r0 += step)
       for (int g = 0; g < s.KVH; ++g) {
         XAttnItem it{};
@@ -1039,7 +1031,6 @@ XAttnSplit cross_attn_split(const XAttnShape &s, const uint64_t *q_start, const 
         it.kvh = g;
         it.nsplit = 1;
         whole[kind].push_back(it);
-        if (kind == 0) out.few_rows = std::max(out.few_rows, it.rows);
       }
   }
   std::vector<XAttnItem> groups;
@@ -1050,7 +1041,7 @@ XAttnSplit cross_attn_split(const XAttnShape &s, const uint64_t *q_start, const 
     if (!keys.empty()) {
       // few rows: a unit is 64 keys (16 a warp); a CTA's start and end cost
       // about as much as 8 of them, a join as 8.  Tiles: 4 of 64 keys, a join 6.
-      const int occ = DP == 64 ? out.few_rows <= 16 ? 5 : 3 : 2;
+      const int occ = DP == 64 ? 5 : 2;
       const int64_t chunk = kind == 0 ? choose_chunk(keys, 64, 8.0, 8.0, sms * occ) : choose_chunk(keys, kKeys, 4.0, 6.0, sms * 2);
       for (XAttnItem it : whole[kind]) {
         const int klen = it.klen, unit = 64;

@@ -371,7 +371,6 @@ NeedleCrossAttnPlan *needle_cross_attn_plan_create(const uint64_t *q_start, cons
     plan->work.items = (const XAttnItem *)plan->buf;
     plan->work.ws = (float *)((char *)plan->flag + 256);
     plan->work.n_few = (int)split.n_few;
-    plan->work.few_rows = split.few_rows;
     plan->work.n_tile = (int)split.n_tile;
     plan->work.n_groups = (int)split.n_groups;
     plan->work.group_rows = split.group_rows;

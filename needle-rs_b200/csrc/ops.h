@@ -96,7 +96,7 @@ struct XAttnSplit {
   std::vector<XAttnItem> items;
   int64_t n_few = 0, n_tile = 0, n_groups = 0;
   int64_t ws_floats = 0;
-  int few_rows = 0, group_rows = 0;  // most rows of a few-row item, of a group
+  int group_rows = 0;  // most rows of a group
 };
 // Items, before splits, of a KV head of a request with `rows` rows for each.
 int64_t cross_attn_items(int64_t rows);
@@ -107,7 +107,7 @@ struct XAttnWork {
   XAttnShape s;
   const XAttnItem *items = nullptr;
   float *ws = nullptr;
-  int n_few = 0, n_tile = 0, n_groups = 0, few_rows = 0, group_rows = 0;
+  int n_few = 0, n_tile = 0, n_groups = 0, group_rows = 0;
 };
 cudaError_t cross_attn(const XAttnWork &w, const XAttnCall &c, int *err, cudaStream_t st);
 

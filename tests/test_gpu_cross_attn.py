@@ -166,6 +166,17 @@ def test_more_tiles_of_rows_than_fit_at_once(D, mask):
         assert torch.equal(again.view(torch.int16), od.view(torch.int16))
 
 
+@pytest.mark.parametrize("n,D", [(6, 64), (6, 80), (70, 64), (70, 128)])
+def test_single_tokens_beside_longer_queries(n, D):
+    """Requests of few rows and of many in one plan: few requests, whose tiles fit
+    the GPU at once, and more."""
+    ql = [(1, 40, 3, 0, 9, 130)[i % 6] for i in range(n)]
+    kl = [(53 * i) % 300 for i in range(n)]
+    dtype = nb.BF16 if D == 64 else nb.F16
+    q, k, v, mask, qs, ks = make(ql, kl, 8, 4, D, dtype, n + D, 0.7, gap=1)
+    run(q, k, v, mask, qs, ql, ks, kl, dtype, D ** -0.5)
+
+
 @pytest.mark.parametrize("n", [1, 40])
 def test_what_is_masked_changes_nothing(n):
     """NaN, infinities and the lowest value in masked keys, in the rows between requests and behind the last."""
