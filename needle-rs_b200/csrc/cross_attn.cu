@@ -79,8 +79,6 @@ constexpr int kFewStages = LONE ? 5 : DP == 64 ? 2 : 3;
 template <int DP, bool LONE>
 constexpr int kFewCtas = LONE ? 1 : DP == 64 ? 5 : 2;
 
-__host__ __device__ constexpr int few_dp(int ks) { return ks <= 4 ? 64 : 128; }
-
 template <int DP>
 constexpr int kFewStageBytes = 2 * kFewKeys * DP * 2;  // K and V rows of 16 keys
 template <int DP, bool LONE>
@@ -126,14 +124,10 @@ __device__ __forceinline__ void mma16<__nv_bfloat16>(float *d, const uint32_t *a
 // past D are written as zeros by the copies themselves, so nothing that they
 // hold can reach a product.  Ring rows are swizzled (16-byte chunk c of row r
 // at c ^ (r & 7)): ldmatrix reads them without bank conflicts.
-// KS: steps of 16 dimensions, 4, 6 or 8; a stage's rows have 64 or 128.  (24 requests of
-// 1 to 17 tokens x 3 heads of 80 dimensions over up to 511 keys: 14.3 us in 6 steps and
-// with the warps' results 8 floats apart in shared memory, 18.6 in 8 steps and
-// without, 18.4 with steps that end at D: branches keep loads and products apart.)
-template <typename T, int KS, bool LONE>
-__global__ void __launch_bounds__(kFewWarps * 32, kFewCtas<few_dp(KS), LONE>)
+template <typename T, int DP, bool LONE>
+__global__ void __launch_bounds__(kFewWarps * 32, kFewCtas<DP, LONE>)
     xattn_few_kernel(const XAttnItem *items, XAttnWork w, XAttnCall c) {
-  constexpr int DP = few_dp(KS), ST = kFewStages<DP, LONE>, CH = DP / 8;  // CH: 16-byte chunks of a row
+  constexpr int ST = kFewStages<DP, LONE>, CH = DP / 8, KS = DP / 16;  // 16-byte chunks of a row, MMA steps over the dimensions
   extern __shared__ __align__(128) uint8_t sm[];
   uint32_t *live_of = reinterpret_cast<uint32_t *>(sm + kFewWarps * ST * kFewStageBytes<DP>);
   pdl_trigger();
@@ -894,10 +888,10 @@ __global__ void xattn_join_kernel(const XAttnItem *groups, XAttnWork w, XAttnCal
 
 // ── launches ────────────────────────────────────────────────────────────────
 
-template <typename T, int KS, bool LONE>
+template <typename T, int DP, bool LONE>
 cudaError_t launch_few(const XAttnItem *items, const XAttnWork &w, const XAttnCall &c, int dev, cudaStream_t st) {
-  constexpr int kSmem = kFewSmem<few_dp(KS), LONE>;
-  auto *kernel = xattn_few_kernel<T, KS, LONE>;
+  constexpr int kSmem = kFewSmem<DP, LONE>;
+  auto *kernel = xattn_few_kernel<T, DP, LONE>;
   static thread_local int ready = -1;
   if (ready != dev) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
@@ -907,13 +901,13 @@ cudaError_t launch_few(const XAttnItem *items, const XAttnWork &w, const XAttnCa
   kernel<<<w.n_few, kFewWarps * 32, kSmem, st>>>(items, w, c);
   return cudaGetLastError();
 }
-template <typename T, int KS>
+template <typename T, int DP>
 cudaError_t few_rows(const XAttnItem *items, const XAttnWork &w, const XAttnCall &c, cudaStream_t st) {
   int dev = 0, sms = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e != cudaSuccess) return e;
-  return w.n_few <= sms ? launch_few<T, KS, true>(items, w, c, dev, st) : launch_few<T, KS, false>(items, w, c, dev, st);
+  return w.n_few <= sms ? launch_few<T, DP, true>(items, w, c, dev, st) : launch_few<T, DP, false>(items, w, c, dev, st);
 }
 
 cudaError_t kv_map(CUtensorMap *map, const void *p, const XAttnShape &s, int64_t row, int64_t head) {
@@ -952,8 +946,7 @@ template <typename T, int DP>
 cudaError_t run(const XAttnWork &w, const XAttnCall &c, int *err, cudaStream_t st) {
   const XAttnItem *few = w.items, *tile = few + w.n_few, *groups = tile + w.n_tile;
   cudaError_t e = launch_tile<T, DP>(tile, w.n_tile, w, c, err, st);
-  if (e == cudaSuccess && w.n_few)
-    e = DP == 128 && w.s.D <= 96 ? few_rows<T, DP == 128 ? 6 : 4>(few, w, c, st) : few_rows<T, DP / 16>(few, w, c, st);
+  if (e == cudaSuccess && w.n_few) e = few_rows<T, DP>(few, w, c, st);
   if (e != cudaSuccess || w.n_groups == 0) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)w.n_groups, (unsigned)((w.group_rows + 7) / 8));

@@ -343,7 +343,11 @@ __device__ __forceinline__ void load8(const Int8Args &a, int64_t row, int k, flo
 // FUSED (up to 16 tokens): no such kernel.  Every CTA finds the rows' maxima
 // itself and rounds its part of K into the MMA's operand layout while its
 // weights arrive: the tokens are few enough to be read by every CTA, and a
-// launch costs more.
+// launch costs more (1 x 512 x 2048: 6.1 us, rounded by a launch before it 8.2).
+//
+// Bound by latency and then by the weights' bytes: 64 x 4096 x 4096 takes 10.3 us with the
+// rounding of its tokens (13.3 with weights requested after TMEM and scales after the
+// sums, 17.7 without the split by estimate), its 16.8 MB alone 2.6 at the copy rate.
 template <int BT, typename TY, bool FUSED>
 __global__ void __launch_bounds__(384, 1)
     int8_tc_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ CUtensorMap mq, Int8Args a, int lg,
@@ -578,7 +582,9 @@ __global__ void __launch_bounds__(384, 1)
 // its own 128 tokens (32 KB a stage of 128 bytes of K); the leader's MMAs read both
 // CTAs' tiles and leave each its 128 channels' sums of all 256 tokens.  A stage is
 // 512 clocks of MMA and 512 of L2 intake at 64 bytes a clock; one CTA alone
-// takes in 768 for 128 channels x 256 tokens.
+// takes in 768 for 128 channels x 256 tokens.  8192 x 4096 x 4096: 87 us, 3.15 POP/s, 0.93
+// of twice the measured bf16 rate, the tensor pipe busy 88% of the time that SMs run; with the
+// rounding of the tokens 128 us where one CTA's tiles took 138.
 // Synchronisation: both CTAs' loads complete on the leader's `full`; an
 // MMA's completion is signalled to both CTAs' `empty` and `tfull`; both CTAs' epilogue
 // warps arrive on the leader's `tempty`.
