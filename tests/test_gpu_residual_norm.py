@@ -191,6 +191,21 @@ def test_many_rows(M, d, gate):
         assert (hd[M] == 7).all()
 
 
+@pytest.mark.parametrize("M,d,tx,ty,gate", [(20000, 33, nb.F16, nb.F16, "channel"), (9000, 257, nb.F32, nb.BF16, "token"),
+                                            (9000, 512, nb.BF16, nb.BF16, "none"), (5000, 1024, nb.F16, nb.F16, "token"),
+                                            (2500, 4096, nb.F32, nb.BF16, "token"), (1500, 6738, nb.BF16, nb.BF16, "scalar")])
+def test_many_rows_in_place(M, d, tx, ty, gate):
+    """r in the place of x and h in that of y, where rows are fetched ahead and pieces of 16 bytes hold parts of two rows."""
+    x, y, g, ps, pre = inputs(M, d, tx, ty, gate, True, 3)
+    xd, yd, gd, pd, prd = cuda(x, y, g, ps, pre)
+    rd, hd = torch.empty_like(xd), torch.empty_like(yd)
+    call = lambda r, h: nb.residual_norm(p(xd), tx, p(yd), ty, M, d, p(prd), p(r), p(h), ty, post_scale_ptr=p(pd), gate_ptr=p(gd),  # noqa: E731
+                                         gate_flags=KINDS[gate])
+    call(rd, hd)
+    call(xd, yd)
+    assert torch.equal(rd, xd) and torch.equal(hd, yd)
+
+
 def test_zero_rows_infinities_and_nan():
     M, d = 4, 96
     x, y, _, ps, pre = inputs(M, d, nb.F32, nb.F32, "none", True, 1)
