@@ -11,18 +11,18 @@
 namespace ndl {
 namespace {
 
-constexpr int kAnyPairs = 8;  // pairs of columns a thread
+constexpr int kAnyPairs = 8;  // pairs of columns a thread, up to
 
 // The pairs of columns t, t + T, ... of a row that starts `off` bytes into a
 // 16-byte aligned buffer, read and written as words: lanes that hold neighbouring
 // pairs touch neighbouring words.  Pairs from the
 // `nc`-th on lie past the row: they are zero and not written.
-template <typename E, int T>
+template <typename E, int T, int P>
 __device__ __forceinline__ void pairs_in(const uint8_t *buf, int off, int t, int nc, uint64_t *v) {
   const uint32_t *w = reinterpret_cast<const uint32_t *>(buf) + (off >> 2) + t * (int)(sizeof(E) / 2);
   const int sh = (off & 2) << 3;
 #pragma unroll
-  for (int c = 0; c < kAnyPairs; ++c) {
+  for (int c = 0; c < P; ++c) {
     uint32_t a = 0, b = 0;
     if (c < nc) {
       a = w[c * T * (int)(sizeof(E) / 2)];
@@ -34,12 +34,12 @@ __device__ __forceinline__ void pairs_in(const uint8_t *buf, int off, int t, int
       v[c] = pair_f32<E>(__funnelshift_r(a, b, sh));
   }
 }
-template <typename E, int T>
+template <typename E, int T, int P>
 __device__ __forceinline__ void pairs_out(uint8_t *buf, int off, int t, int nc, const uint64_t *v) {
   uint32_t *w = reinterpret_cast<uint32_t *>(buf) + (off >> 2) + t * (int)(sizeof(E) / 2);
   if constexpr (sizeof(E) == 4) {
 #pragma unroll
-    for (int c = 0; c < kAnyPairs; ++c) {
+    for (int c = 0; c < P; ++c) {
       float a, b;
       f2unpack(v[c], a, b);
       if (c < nc) {
@@ -50,7 +50,7 @@ __device__ __forceinline__ void pairs_out(uint8_t *buf, int off, int t, int nc, 
   } else if (off & 2) {
     uint16_t *h = reinterpret_cast<uint16_t *>(w) + 1;
 #pragma unroll
-    for (int c = 0; c < kAnyPairs; ++c) {
+    for (int c = 0; c < P; ++c) {
       const uint32_t bits = pair_bits<E>(v[c]);
       if (c < nc) {
         h[2 * c * T] = (uint16_t)bits;
@@ -59,7 +59,7 @@ __device__ __forceinline__ void pairs_out(uint8_t *buf, int off, int t, int nc, 
     }
   } else {
 #pragma unroll
-    for (int c = 0; c < kAnyPairs; ++c)
+    for (int c = 0; c < P; ++c)
       if (c < nc) w[c * T] = pair_bits<E>(v[c]);
   }
 }
@@ -70,9 +70,9 @@ __device__ __forceinline__ void pairs_out(uint8_t *buf, int off, int t, int nc, 
 // starts; T is a template, so that a pair's place is a constant.  Element by element in
 // global memory 14,785 x 6,738 bf16 took 847 us, element by element in shared memory 431
 // (92 instructions an element and warp), by pairs with T a variable 320.
-template <typename TX, typename TY, bool TOKEN, int T>
+template <typename TX, typename TY, bool TOKEN, int T, int P>
 __global__ void __launch_bounds__(T < 128 ? 128 : T, 1024 / (T < 128 ? 128 : T)) residual_norm_any_kernel(ResidualNormArgs a, int bx, int by) {
-  constexpr int CH = kAnyPairs, S = kStreamStages, warps = T / 32;
+  constexpr int S = kStreamStages, warps = T / 32;
   // a row group's shared memory: S stages of x, y and gate rows, then r and h
   extern __shared__ __align__(16) uint8_t buf[];
   __shared__ __align__(16) float sm[3][16];
@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T, 1024 / (T < 128 ? 128 : T))
   const int nc = ((d + 1) / 2 - t + T - 1) / T;
   auto times = [&](uint64_t *r, const float *p, float one, bool logi) {  // r *= one + p
 #pragma unroll
-    for (int c = 0; c < kAnyPairs; ++c) {
+    for (int c = 0; c < P; ++c) {
       float u = 0.0f, v = 0.0f;
       if (c < nc) u = p[2 * (c * T + t)], v = p[min(2 * (c * T + t) + 1, d - 1)];
       u = logi ? logistic16(u) : one + u;
@@ -143,25 +143,25 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T, 1024 / (T < 128 ? 128 : T))
       if (TOKEN) *reinterpret_cast<TY *>(at + bx + by + og + d * sizeof(TY)) = from_f32<TY>(0.0f);
     }
     sync();  // the whole row has arrived, and the last one has left out_r and out_h
-    uint64_t r[CH], v[CH], ss = zero;
+    uint64_t r[P], v[P], ss = zero;
 #pragma unroll
-    for (int c = 0; c < CH; ++c) r[c] = zero;
+    for (int c = 0; c < P; ++c) r[c] = zero;
     if (have_y) {
       float inv = g;
-      pairs_in<TY, T>(at + bx, oy, t, nc, r);
+      pairs_in<TY, T, P>(at + bx, oy, t, nc, r);
       if (a.post) {
 #pragma unroll
-        for (int c = 0; c < kAnyPairs; ++c) ss = ffma2(r[c], r[c], ss);
+        for (int c = 0; c < P; ++c) ss = ffma2(r[c], r[c], ss);
         inv *= rsqrtf(fmaf(stream_sum(ss, warps, sm[0]), over_d, kEps));
       }
 #pragma unroll
-      for (int c = 0; c < kAnyPairs; ++c) r[c] = fmul2(r[c], f2pack(inv, inv));
+      for (int c = 0; c < P; ++c) r[c] = fmul2(r[c], f2pack(inv, inv));
       if (a.post) times(r, a.post, 1.0f, false);
       if (!TOKEN && channel) times(r, channel, 0.0f, a.sigmoid);
       if (TOKEN) {
-        pairs_in<TY, T>(at + bx + by, og, t, nc, v);
+        pairs_in<TY, T, P>(at + bx + by, og, t, nc, v);
 #pragma unroll
-        for (int c = 0; c < kAnyPairs; ++c) {
+        for (int c = 0; c < P; ++c) {
           if (a.sigmoid) {
             float x0, x1;
             f2unpack(v[c], x0, x1);
@@ -172,22 +172,22 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T, 1024 / (T < 128 ? 128 : T))
       }
     }
     ss = zero;
-    pairs_in<TX, T>(at, ox, t, nc, v);
+    pairs_in<TX, T, P>(at, ox, t, nc, v);
 #pragma unroll
-    for (int c = 0; c < kAnyPairs; ++c) {
+    for (int c = 0; c < P; ++c) {
       r[c] = ffma2(v[c], sc, r[c]);
       ss = ffma2(r[c], r[c], ss);
     }
-    if (a.r) pairs_out<TX, T>(out_r, offset(a.r, row, a.ldr, sizeof(TX)), t, nc, r);
+    if (a.r) pairs_out<TX, T, P>(out_r, offset(a.r, row, a.ldr, sizeof(TX)), t, nc, r);
     if (a.h) {
       const float inv = rsqrtf(fmaf(stream_sum(ss, warps, sm[1]), over_d, kEps));
 #pragma unroll
-      for (int c = 0; c < kAnyPairs; ++c) r[c] = fmul2(r[c], f2pack(inv, inv));
+      for (int c = 0; c < P; ++c) r[c] = fmul2(r[c], f2pack(inv, inv));
       times(r, a.pre, 1.0f, false);
       if (a.h_dtype == DT_I8) {
         uint32_t top = 0;  // largest |h| as bits: infinities and NaN order above every number
 #pragma unroll
-        for (int c = 0; c < kAnyPairs; ++c) {
+        for (int c = 0; c < P; ++c) {
           float x0, x1;
           f2unpack(r[c], x0, x1);
           top = max(top, max(__float_as_uint(x0) & 0x7fffffffu, __float_as_uint(x1) & 0x7fffffffu));
@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T, 1024 / (T < 128 ? 128 : T))
         const RowScale rs = int8_row_scale(row_max_bits(top, warps, reinterpret_cast<uint32_t *>(sm[2])));
         const int dp = (d + 15) / 16 * 16;  // rows of 8-bit values start on 16-byte boundaries
 #pragma unroll
-        for (int c = 0; c < kAnyPairs; ++c) {
+        for (int c = 0; c < P; ++c) {
           float x0, x1;
           f2unpack(r[c], x0, x1);
           if (c < nc)
@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T, 1024 / (T < 128 ? 128 : T))
         if (t < dp - d) out_h[d + t] = 0;
         if (t == 0) a.h_scales[row] = rs.scale;
       } else {
-        pairs_out<TY, T>(out_h, offset(a.h, row, a.ldh, sizeof(TY)), t, nc, r);
+        pairs_out<TY, T, P>(out_h, offset(a.h, row, a.ldh, sizeof(TY)), t, nc, r);
       }
     }
     sync();
@@ -217,13 +217,13 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T, 1024 / (T < 128 ? 128 : T))
 }
 
 // The same for rows at any alignment; from one row a block on.
-template <typename TX, typename TY, bool TOKEN, int T>
+template <typename TX, typename TY, bool TOKEN, int T, int P = kAnyPairs>
 cudaError_t launch_any(const ResidualNormArgs &a, bool *done, cudaStream_t st) {
   const int rows = T == 32 ? 4 : 1;  // blocks of several rows only where no barrier spans them
   // bytes of a row and its offset, to the next 16-byte boundary
   const int bx = (a.d * (int)sizeof(TX) + 31) / 16 * 16, by = (a.d * (int)sizeof(TY) + 31) / 16 * 16;
   const size_t smem = (size_t)rows * (kStreamStages * (bx + (TOKEN ? 2 : 1) * by) + bx + by);
-  auto *kernel = residual_norm_any_kernel<TX, TY, TOKEN, T>;
+  auto *kernel = residual_norm_any_kernel<TX, TY, TOKEN, T, P>;
   static thread_local int last_dev = -1, last_d = 0, fit = 0;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -241,10 +241,14 @@ cudaError_t launch_any(const ResidualNormArgs &a, bool *done, cudaStream_t st) {
   return cudaGetLastError();
 }
 
-// The fewest threads, a power of two, whose pairs cover a row.
+// The fewest threads, a power of two, whose pairs cover a row; for less than a
+// warp's 512 columns fewer pairs a thread, 2 or 4 (60,000 rows, with 8 in brackets:
+// 63 f32 and f16 43 us (70), 117 f16 with a token gate 50 (72), 201 bf16 52 (62), 255 f32 62 (69)).
 template <typename TX, typename TY, bool TOKEN>
 cudaError_t launch_threads(const ResidualNormArgs &a, bool *done, cudaStream_t st) {
   const int need = (a.d + 2 * kAnyPairs - 1) / (2 * kAnyPairs);
+  if (need <= 8) return launch_any<TX, TY, TOKEN, 32, 2>(a, done, st);
+  if (need <= 16) return launch_any<TX, TY, TOKEN, 32, 4>(a, done, st);
   if (need <= 32) return launch_any<TX, TY, TOKEN, 32>(a, done, st);
   if (need <= 64) return launch_any<TX, TY, TOKEN, 64>(a, done, st);
   if (need <= 128) return launch_any<TX, TY, TOKEN, 128>(a, done, st);

@@ -153,7 +153,7 @@ def test_strides_and_alignment(d, off):
 
 
 MANY = [(20000, 33), (20000, 64), (9000, 264), (9000, 257), (9001, 512), (8000, 777), (6000, 1000), (5000, 1024), (4001, 2048),
-        (3000, 2054), (2500, 4096), (2000, 4099), (1500, 4360), (1500, 6738), (1300, 8192), (1200, 8191)]
+        (3000, 2054), (2500, 4096), (2000, 4099), (1500, 4360), (1500, 6738), (1300, 8192), (1200, 8191), (20000, 131), (15000, 255)]
 
 
 @pytest.mark.parametrize("gate", ["none", "scalar", "channel", "token", "no block"])
