@@ -302,7 +302,7 @@ template <int BT, bool FUSED>
 constexpr int kStages = FUSED ? 7 : BT <= 64 ? 8 : BT == 128 ? 6 : 4;
 template <int BT, bool FUSED>
 constexpr int kStageBytes = (BN + (FUSED ? 0 : BT)) * BK;
-constexpr int kFusedBlocks = 40;  // blocks of K whose tokens fit beside the ring
+constexpr int kFusedBlocks = 32;  // blocks of K of the most values that a kernel rounds itself
 template <int BT, bool FUSED>
 constexpr size_t kSmem = (size_t)kStages<BT, FUSED> * kStageBytes<BT, FUSED> + (FUSED ? kFusedBlocks * 16 * BK : 0) + 1024 + 512;
 
@@ -342,7 +342,7 @@ __device__ __forceinline__ void load8(const Int8Args &a, int64_t row, int k, flo
 //
 // FUSED (up to 16 tokens): no such kernel.  Every CTA finds the rows' maxima
 // itself and rounds its part of K into the MMA's operand layout while its
-// weights arrive: the tokens are few enough to be read by every CTA, and a
+// weights arrive: the values are few enough to be read by every CTA, and a
 // launch costs more (1 x 512 x 2048: 6.1 us, rounded by a launch before it 8.2).
 //
 // Bound by latency and then by the weights' bytes: 64 x 4096 x 4096 takes 10.3 us with the
@@ -425,15 +425,15 @@ __global__ void __launch_bounds__(384, 1)
     }
     // this CTA's part of K in the swizzled layout; the rows past M hold anything,
     // which reaches no token that is stored
-    const int chunks = (kb1 - kb0) * (BK / 8);  // of 8 values
-    for (int r = 0; r < a.M; ++r)
-      for (int c = threadIdx.x; c < chunks; c += blockDim.x) {
-        float v[8];
-        load8(a, r, kb0 * BK + c * 8, v);
-        const float inv = scales[16 + r];
-        *reinterpret_cast<uint2 *>(tokens + (c / 16) * 16 * BK + r * BK + (((c % 16 >> 1) ^ (r & 7)) << 4) + (c & 1) * 8) =
-            make_uint2(int8_pack4(v, inv), int8_pack4(v + 4, inv));
-      }
+    const int blocks = kb1 - kb0;
+    for (int i = threadIdx.x; i < a.M * blocks * (BK / 8); i += blockDim.x) {  // 8 values: chunk c % 16 of a row's block
+      const int c = i % (BK / 8), r = i / (BK / 8) % a.M, block = i / (BK / 8) / a.M;
+      float v[8];
+      load8(a, r, (kb0 + block) * BK + c * 8, v);
+      const float inv = scales[16 + r];
+      *reinterpret_cast<uint2 *>(tokens + block * 16 * BK + r * BK + (((c >> 1) ^ (r & 7)) << 4) + (c & 1) * 8) =
+          make_uint2(int8_pack4(v, inv), int8_pack4(v + 4, inv));
+    }
     fence_async_smem();
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -803,14 +803,11 @@ Shape choose_shape(int M, int N, int K, int sms) {
   return best;
 }
 
-// Whether a product of unrounded tokens takes the fused kernel: one tile of 16
-// tokens, few enough bytes for every CTA to read them all (one token's 32,768
-// f32), and a part of K that fits beside the weights' ring.
-bool fuses(const Shape &sh, int M, int K, int dtype) {
-  const int nkb = (K + BK - 1) / BK;
-  return sh.bt == 16 && M <= 16 && (int64_t)M * K * (int64_t)dtype_size(dtype) <= (128 << 10) &&
-         (nkb + (1 << sh.lg) - 1) >> sh.lg <= kFusedBlocks;
-}
+// Whether a product of unrounded tokens takes the fused kernel: one tile of up to 16
+// tokens, 4,096 values in all (fused and with a launch to round them, us, bf16: 8 x 512 x 512
+// 6.3 and 8.0, 1 x 4096 x 4096 8.6 and 9.0, 16 x 512 x 512 8.3 and 8.0, 4 x 2048 x 2048 14.0
+// and 12.2, 16 x 2048 x 2048 22.6 and 12.4: every CTA reads all of them).
+bool fuses(const Shape &sh, int M, int K) { return sh.bt == 16 && M <= 16 && (int64_t)M * K <= kFusedBlocks * BK; }
 
 template <typename TY>
 cudaError_t product(const Int8Args &a, bool pdl, int *err, cudaStream_t st) {
@@ -856,11 +853,11 @@ cudaError_t int8_quantize_cols(const void *w, int dtype, int64_t K, int64_t N, i
 
 cudaError_t int8_weight_map(CUtensorMap *map, const int8_t *w, int64_t N, int K) { return row_map(map, w, N, K, BN); }
 
-bool int8_matmul_fuses(int M, int N, int K, int x_dtype) {
+bool int8_matmul_fuses(int M, int N, int K) {
   int dev = 0, sms = 0;
   return cudaGetDevice(&dev) == cudaSuccess &&
          cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess &&
-         fuses(choose_shape(M, N, K, sms), M, K, x_dtype);
+         fuses(choose_shape(M, N, K, sms), M, K);
 }
 
 cudaError_t int8_matmul(const Int8Args &a, bool pdl, int *err, cudaStream_t st) {

@@ -230,7 +230,7 @@ int needle_int8_plan_matmul(NeedleInt8Plan *p, const void *x, int x_dtype, size_
     OnDevice on(p->device);
     if (!on.good() || !all_on(p->device, {{"x", x}, {"y", y}, {"bias", bias}})) return false;
     cudaStream_t st = (cudaStream_t)stream;
-    if (int8_matmul_fuses((int)M, p->N, p->K, x_dtype)) {
+    if (int8_matmul_fuses((int)M, p->N, p->K)) {
       Int8Args a{nullptr, &p->w_map, nullptr, p->w_scales, bias, y, (int64_t)ldy, (int)M, p->N, p->K, y_dtype};
       a.x = x;
       a.ldx = (int64_t)ldx;

@@ -42,7 +42,7 @@ struct Int8Args {
   bool x_vec = false;  // rows on 16-byte boundaries
 };
 // Whether int8_matmul takes unrounded tokens of these sizes (few of them).
-bool int8_matmul_fuses(int M, int N, int K, int x_dtype);
+bool int8_matmul_fuses(int M, int N, int K);
 // TMA descriptor of a weight [N][Kp], 16-byte aligned.
 cudaError_t int8_weight_map(CUtensorMap *map, const int8_t *w, int64_t N, int K);
 // *err is set if a bounded wait inside the kernel expired.  pdl: the kernel
