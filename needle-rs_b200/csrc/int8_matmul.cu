@@ -774,6 +774,33 @@ cudaError_t launch_pair(const Int8Args &a, int sms, bool pdl, int *err, cudaStre
   return cudaLaunchKernelEx(&cfg, kernel, *a.w_map, mq, a, err);
 }
 
+// Clusters of 2^lg CTAs that run at once on the current device: fewer than its SMs
+// would hold, since a cluster stays within one of their groups (15 of 8 CTAs on 148 SMs; a
+// sixteenth waits for a second round: 64 x 2048 x 2048 14.5 us, split by four instead 8.6).
+cudaError_t clusters_at_once(int dev, int sms, int *fit) {
+  static thread_local int last_dev = -1, last[4];
+  if (last_dev != dev) {
+    auto *kernel = int8_tc_kernel<16, float, false>;  // as the others, a CTA an SM
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem<16, false>);
+    for (int lg = 0; lg < 4 && e == cudaSuccess; ++lg) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3((unsigned)(sms >> lg << lg));
+      cfg.blockDim = dim3(384);
+      cfg.dynamicSmemBytes = kSmem<16, false>;
+      cudaLaunchAttribute at[1];
+      at[0].id = cudaLaunchAttributeClusterDimension;
+      at[0].val.clusterDim = {1u << lg, 1, 1};
+      cfg.attrs = at;
+      cfg.numAttrs = 1;
+      e = cudaOccupancyMaxActiveClusters(&last[lg], kernel, &cfg);
+    }
+    if (e != cudaSuccess) return e;
+    last_dev = dev;
+  }
+  for (int lg = 0; lg < 4; ++lg) fit[lg] = last[lg];
+  return cudaSuccess;
+}
+
 // Tokens of a tile and CTAs that share one: the least estimated time, in
 // clocks of an SM that takes in about 64 bytes each from L2, which is what
 // binds: the waves of tiles, each the bytes of its stages and a start and end of
@@ -783,7 +810,7 @@ cudaError_t launch_pair(const Int8Args &a, int sms, bool pdl, int *err, cudaStre
 struct Shape {
   int bt, lg;  // tokens (512: a pair's tile), log2 of the CTAs
 };
-Shape choose_shape(int M, int N, int K, int sms) {
+Shape choose_shape(int M, int N, int K, int sms, const int *fit) {
   const int num_n = (N + BN - 1) / BN, nkb = (K + BK - 1) / BK;
   Shape best{16, 0};
   int64_t least = INT64_MAX;
@@ -791,7 +818,7 @@ Shape choose_shape(int M, int N, int K, int sms) {
     const int64_t tiles = (int64_t)num_n * ((M + b - 1) / b);
     for (int lg = 0; lg <= (b <= 128 ? 3 : 0); ++lg) {
       const int s = 1 << lg;
-      if (lg && (s > nkb || tiles * s > sms)) break;
+      if (lg && (s > nkb || tiles > fit[lg])) break;
       const int64_t waves = (tiles * s + sms - 1) / sms;
       const int64_t cost = waves * ((BN + b) * 2 * ((nkb + s - 1) / s)) + 2000 + (s > 1 ? 1000 + b * 16 / s : 0) + b * 8;
       if (cost < least) least = cost, best = Shape{b, lg};
@@ -811,11 +838,12 @@ bool fuses(const Shape &sh, int M, int K) { return sh.bt == 16 && M <= 16 && (in
 
 template <typename TY>
 cudaError_t product(const Int8Args &a, bool pdl, int *err, cudaStream_t st) {
-  int dev = 0, sms = 0;
+  int dev = 0, sms = 0, fit[4];
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e == cudaSuccess) e = clusters_at_once(dev, sms, fit);
   if (e != cudaSuccess) return e;
-  const Shape sh = choose_shape(a.M, a.N, a.K, sms);
+  const Shape sh = choose_shape(a.M, a.N, a.K, sms, fit);
   switch (sh.bt) {
     case 16:
       return a.x ? launch_tc<16, TY, true>(a, sh.lg, sms, false, err, st)
@@ -854,10 +882,10 @@ cudaError_t int8_quantize_cols(const void *w, int dtype, int64_t K, int64_t N, i
 cudaError_t int8_weight_map(CUtensorMap *map, const int8_t *w, int64_t N, int K) { return row_map(map, w, N, K, BN); }
 
 bool int8_matmul_fuses(int M, int N, int K) {
-  int dev = 0, sms = 0;
+  int dev = 0, sms = 0, fit[4];
   return cudaGetDevice(&dev) == cudaSuccess &&
          cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess &&
-         fuses(choose_shape(M, N, K, sms), M, K);
+         clusters_at_once(dev, sms, fit) == cudaSuccess && fuses(choose_shape(M, N, K, sms, fit), M, K);
 }
 
 cudaError_t int8_matmul(const Int8Args &a, bool pdl, int *err, cudaStream_t st) {
