@@ -518,7 +518,6 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   uint64_t *v_ok = v_empty + ST, *q_full = v_ok + ST, *o_free = q_full + 1, *s_full = o_free + 1, *p_full = s_full + 2,
            *pv_done = p_full + 2;
   uint32_t *tmem_slot = (uint32_t *)(pv_done + 2);
-  pdl_trigger();
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = w.s.H / w.s.KVH, D = w.s.D;
   // this CTA's item of a round; n_items or more: none
@@ -555,6 +554,8 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   __syncthreads();
   tc_after();
   const uint32_t tmem = *(volatile uint32_t *)tmem_slot;
+  // not before TMEM is held: a kernel behind this one could take it and wait for this one's end
+  pdl_trigger();
   bool ok = true;
 
   if (warp == 0) {
