@@ -587,7 +587,8 @@ __global__ void __launch_bounds__(384, 1)
 // rounding of the tokens 128 us where one CTA's tiles took 138.
 // Synchronisation: both CTAs' loads complete on the leader's `full`; an
 // MMA's completion is signalled to both CTAs' `empty` and `tfull`; both CTAs' epilogue
-// warps arrive on the leader's `tempty`.
+// warps arrive on the leader's `tempty`.  After a wait that ran out the leader waits for
+// the copies that either CTA has in flight: `asked` tells it how far both came.
 constexpr int kPairStages = 6, kPairBytes = 2 * BN * BK;
 constexpr size_t kPairSmem = (size_t)kPairStages * kPairBytes + 1024 + 256;
 
@@ -601,6 +602,7 @@ __global__ void __launch_bounds__(384, 1)
   uint64_t *full = (uint64_t *)(smem + STAGES * kPairBytes), *empty = full + STAGES;
   uint64_t *tfull = empty + STAGES, *tempty = tfull + 2;
   uint32_t *tmem_slot = (uint32_t *)(tempty + 2);
+  uint32_t *asked = tmem_slot + 2;  // of each CTA: stages requested * 2, and 1 if a wait of its loader ran out
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_ctarank(), pair = (int)blockIdx.x >> 1, pairs = (int)gridDim.x >> 1;
@@ -635,7 +637,7 @@ __global__ void __launch_bounds__(384, 1)
     if (lane == 0) {
       pdl_wait();  // the tokens
       int s = 0;
-      uint32_t ph = 0;
+      uint32_t ph = 0, requested = 0;
       bool ok = true;
       for (int t = pair; t < tiles && ok; t += pairs) {
         const int n0 = t % num_n * 2 * BN + rank * BN, m0 = t / num_n * BT + rank * BN;
@@ -645,6 +647,7 @@ __global__ void __launch_bounds__(384, 1)
           const uint32_t fb = pair_leader_addr(&full[s]);
           tma_load_2d_pair(smem + s * kPairBytes, &mw, fb, kb * BK, n0);
           tma_load_2d_pair(smem + s * kPairBytes + W_BYTES, &mq, fb, kb * BK, m0);
+          ++requested;
           if (++s == STAGES) s = 0, ph ^= 1;
         }
       }
@@ -653,6 +656,7 @@ __global__ void __launch_bounds__(384, 1)
         ok = mbar_wait(&empty[s], ph ^ 1, err);
         if (++s == STAGES) s = 0, ph ^= 1;
       }
+      for (uint32_t r = 0; r < 2; ++r) store_cluster(&asked[rank], r, requested << 1 | (ok ? 0u : 1u));
     }
     __syncwarp();
   } else if (warp == 1 && rank == 0) {
@@ -700,6 +704,25 @@ __global__ void __launch_bounds__(384, 1)
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   cluster_sync();  // no arrive or MMA reaches a CTA that has left
+  if ((asked[0] | asked[1]) & 1u) {  // the same in both CTAs
+    if (rank == 0 && threadIdx.x == 0) {
+      // The stages from `both` on were requested by one CTA alone.  Where that is the
+      // leader, `full` was told to expect the other's bytes too: it copies once more in its place.
+      const uint32_t n0 = asked[0] >> 1, n1 = asked[1] >> 1, most = max(n0, n1), both = min(n0, n1);
+      for (uint32_t k = most > STAGES ? most - STAGES : 0; k < most; ++k) {
+        const int s = (int)(k % STAGES);
+        if (k >= both && n1 > n0) mbar_expect_tx(&full[s], kPairBytes);
+        if (k >= both && n0 > n1) {
+          const uint32_t fb = pair_leader_addr(&full[s]);
+          tma_load_2d_pair(smem + s * kPairBytes, &mw, fb, 0, 0);
+          tma_load_2d_pair(smem + s * kPairBytes + W_BYTES, &mq, fb, 0, 0);
+        }
+        mbar_drain(&full[s], k / STAGES & 1);
+      }
+    }
+    __syncthreads();
+    cluster_sync();  // no copy is in flight when a CTA leaves
+  }
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BT));

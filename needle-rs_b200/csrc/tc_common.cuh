@@ -164,6 +164,13 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint64_t *b, uint32_t rank) 
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
 }
 
+// Store to the same word in CTA `rank` of the cluster.
+__device__ __forceinline__ void store_cluster(uint32_t *p, uint32_t rank, uint32_t v) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(remote), "r"(v) : "memory");
+}
+
 // UMMA shared-memory descriptor: K-major operand, 128-byte swizzle, 8-row
 // atoms of 1024 bytes stacked along M/N (SBO = 1024 B), version 1 (sm100).
 __device__ __forceinline__ uint64_t umma_desc(const void *smem) {

@@ -41,3 +41,19 @@ def test_tmem_is_held_before_the_next_kernel_may_start(name):
             continue
         between = body[body.rindex("tcgen05.alloc"):body.index("pdl_trigger()")] if body.rindex("tcgen05.alloc") < body.index("pdl_trigger()") else ""
         assert "__syncthreads()" in between, kernel
+
+
+@pytest.mark.parametrize("name", ["cross_attn.cu", "int8_matmul.cu"])
+def test_a_wait_that_ran_out_leaves_no_copy_in_flight(name):
+    """A block that leaves while a TMA copy is on its way lets it write the shared
+    memory of the next one: behind the loading loop every kernel waits for the
+    stages it has requested, whether a wait ran out before that or not."""
+    for kernel, body in kernels(name).items():
+        loads = [m.start() for m in re.finditer(r"\btma_load_\dd(_pair)?\(", body)]
+        drains = [m.start() for m in re.finditer(r"\bmbar_drain\(", body)]
+        if loads:
+            assert drains and drains[-1] > loads[-1], kernel
+        if any("tma_load_2d_pair" in body[at:at + 16] for at in loads):
+            # the copies of both blocks of a pair: after they have met, and they meet again
+            met = [m.start() for m in re.finditer(r"\bcluster_sync\(\)", body)]
+            assert any(a < drains[-1] < b for a, b in zip(met[1:], met[2:])), kernel
