@@ -516,8 +516,8 @@ __global__ void __launch_bounds__(kTileThreads, 2)
   uint8_t *sm = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint64_t *k_full = (uint64_t *)(sm + L::kBar), *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST;
   uint64_t *v_ok = v_empty + ST, *q_full = v_ok + ST, *o_free = q_full + 1, *s_full = o_free + 1, *p_full = s_full + 2,
-           *pv_done = p_full + 2;
-  uint32_t *tmem_slot = (uint32_t *)(pv_done + 2);
+           *pv_done = p_full + 2, *done = pv_done + 2;  // done: of a warp's MMAs in flight, after a wait that ran out
+  uint32_t *tmem_slot = (uint32_t *)(done + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = w.s.H / w.s.KVH, D = w.s.D;
   // this CTA's item of a round; n_items or more: none
@@ -542,6 +542,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
       mbar_init(&s_full[b], 1);
       mbar_init(&p_full[b], 4);
       mbar_init(&pv_done[b], 1);
+      mbar_init(&done[b], 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -618,6 +619,10 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         umma_commit_e(&k_empty[s]);
       }
     }
+    if (!ok) {
+      umma_commit_e(&done[0]);
+      mbar_drain(&done[0], 0);
+    }
   } else if (warp == 3) {
     // O += P(t) V_j
     const uint32_t s16 = smem_u32(sm) >> 4;
@@ -649,6 +654,10 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         umma_commit_e(&pv_done[t & 1]);
         umma_commit_e(&v_empty[s]);
       }
+    }
+    if (!ok) {
+      umma_commit_e(&done[1]);
+      mbar_drain(&done[1], 0);
     }
   } else if (warp == 2 && c.mask) {
     int t = 0;

@@ -361,7 +361,8 @@ __global__ void __launch_bounds__(384, 1)
   uint8_t *tokens = smem + STAGES * BYTES;  // FUSED: [block of K][16 rows][128 bytes]
   uint64_t *full = (uint64_t *)(tokens + (FUSED ? kFusedBlocks * 16 * BK : 0)), *empty = full + STAGES;
   uint64_t *tfull = empty + STAGES, *tempty = tfull + 2;
-  uint32_t *tmem_slot = (uint32_t *)(tempty + 2), *tops = tmem_slot + 2;  // tops: [12 warps]
+  uint64_t *done = tempty + 2;  // of MMAs in flight, after a wait that ran out
+  uint32_t *tmem_slot = (uint32_t *)(done + 1), *tops = tmem_slot + 2;  // tops: [12 warps]
   float *scales = (float *)(tops + 12);                                   // FUSED: [16]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -384,6 +385,7 @@ __global__ void __launch_bounds__(384, 1)
       mbar_init(&tfull[b], 1);
       mbar_init(&tempty[b], 8);
     }
+    mbar_init(done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_smem();
     for (int i = 0; i < burst; ++i) {
@@ -495,6 +497,10 @@ __global__ void __launch_bounds__(384, 1)
       }
       if (ok) umma_commit_e(&tfull[buf]);
     }
+    if (!ok) {
+      umma_commit_e(done);
+      mbar_drain(done, 0);
+    }
   } else if (warp >= 4) {
     const int quarter = warp & 3, half = (warp - 4) >> 2;  // TMEM lanes, tokens
     if (!FUSED) pdl_wait();                                // the tokens' scales
@@ -601,7 +607,8 @@ __global__ void __launch_bounds__(384, 1)
   uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint64_t *full = (uint64_t *)(smem + STAGES * kPairBytes), *empty = full + STAGES;
   uint64_t *tfull = empty + STAGES, *tempty = tfull + 2;
-  uint32_t *tmem_slot = (uint32_t *)(tempty + 2);
+  uint64_t *done = tempty + 2;  // of MMAs in flight, after a wait that ran out
+  uint32_t *tmem_slot = (uint32_t *)(done + 1);
   uint32_t *asked = tmem_slot + 2;  // of each CTA: stages requested * 2, and 1 if a wait of its loader ran out
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -620,6 +627,7 @@ __global__ void __launch_bounds__(384, 1)
       mbar_init(&tfull[b], 1);
       mbar_init(&tempty[b], 16);
     }
+    mbar_init(done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
@@ -680,6 +688,10 @@ __global__ void __launch_bounds__(384, 1)
         if (++s == STAGES) s = 0, ph ^= 1;
       }
       if (ok) umma_commit_pair_e(&tfull[buf]);
+    }
+    if (!ok) {
+      umma_commit_pair_e(done);
+      mbar_drain(done, 0);
     }
   } else if (warp >= 4) {
     const int quarter = warp & 3, half = (warp - 4) >> 2;

@@ -57,3 +57,13 @@ def test_a_wait_that_ran_out_leaves_no_copy_in_flight(name):
             # the copies of both blocks of a pair: after they have met, and they meet again
             met = [m.start() for m in re.finditer(r"\bcluster_sync\(\)", body)]
             assert any(a < drains[-1] < b for a, b in zip(met[1:], met[2:])), kernel
+
+
+@pytest.mark.parametrize("name", ["cross_attn.cu", "int8_matmul.cu"])
+def test_a_wait_that_ran_out_leaves_no_product_in_flight(name):
+    """TMEM that is freed under a running MMA may be another block's when the sums
+    arrive: a warp that gives up commits what it has issued and waits for that."""
+    for kernel, body in kernels(name).items():
+        issuers = len(re.findall(r"\bumma_commit(?:_pair)?_e\(&(?:tfull|s_full|pv_done)\[", body))
+        given_up = len(re.findall(r"if \(!ok\) \{\s*umma_commit(?:_pair)?_e\((&?done[^)]*)\);\s*mbar_drain\(\1, 0\);", body))
+        assert given_up == issuers, kernel
