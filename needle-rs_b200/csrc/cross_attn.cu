@@ -215,6 +215,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, kFewCtas<DP, LONE>)
     __syncwarp();  // every lane's copies of this stage, and the reads of the stage refilled next
     if (n + ST - 1 < mine) issue(n + ST - 1, stage == 0 ? ST - 1 : stage - 1);
     asm volatile("cp.async.commit_group;" ::: "memory");
+    __syncwarp();  // the matrix loads below take a whole warp
     const uint32_t live = live_of[warp * ST + stage];
     const uint32_t K = ring + stage * kFewStageBytes<DP>, V = K + kFewKeys * DP * 2;
     if (++stage == ST) stage = 0;
@@ -262,6 +263,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, kFewCtas<DP, LONE>)
         pf[2 * n + h] = pack2<T>(p0, p1);
       }
     }
+    __syncwarp();
 #pragma unroll
     for (int nb = 0; nb < KS; ++nb) {
       uint32_t vf[4];
@@ -769,6 +771,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         const float mc = m == -INFINITY ? 0.0f : m * sc;
         const uint64_t cc = f2pack(sc, sc), nm = f2pack(-mc, -mc);
         uint64_t sum[2] = {f2pack(0.0f, 0.0f), f2pack(0.0f, 0.0f)};
+        __syncwarp();  // TMEM is read and written by whole warps
 #pragma unroll
         for (int q = 0; q < kKeys / 32; ++q) {
           uint32_t pw[16];
@@ -803,6 +806,7 @@ __global__ void __launch_bounds__(kTileThreads, 2)
         uint32_t o[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) o[e] = 0;
+        __syncwarp();  // rows past the item's left the last turn early
         if (nt > 0) {
           tmem_ld32_raw(tO + 32 * q, o);
           tmem_wait_ld();

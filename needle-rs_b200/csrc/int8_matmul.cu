@@ -285,6 +285,7 @@ __device__ __forceinline__ void store_tokens(const Int8Args &a, uint32_t taddr, 
 #pragma unroll
   for (int c = 0; c < NC; c += 16) {
     if (c >= left) break;
+    __syncwarp();  // channels past the last stored nothing; TMEM is read by whole warps
     int v[16];
     tmem_ld16(taddr + c, v);
 #pragma unroll
@@ -548,6 +549,7 @@ __global__ void __launch_bounds__(384, 1)
       sw[j] = n + j < a.N ? a.w_scales[n + j] : 0.0f;
       bias[j] = n + j < a.N && a.bias ? a.bias[n + j] : 0.0f;
     }
+    __syncwarp();
     cluster_sync();
     for (int u = threadIdx.x; u < units; u += blockDim.x) {
       const int c = c0 + u / (BN / 4), m = m0 + c;

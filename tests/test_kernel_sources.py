@@ -67,3 +67,54 @@ def test_a_wait_that_ran_out_leaves_no_product_in_flight(name):
         issuers = len(re.findall(r"\bumma_commit(?:_pair)?_e\(&(?:tfull|s_full|pv_done)\[", body))
         given_up = len(re.findall(r"if \(!ok\) \{\s*umma_commit(?:_pair)?_e\((&?done[^)]*)\);\s*mbar_drain\(\1, 0\);", body))
         assert given_up == issuers, kernel
+
+
+MEET = r"__syncwarp\(\)|__syncthreads\(\)|warp_wait\(|warp_sleep_wait\(|__any_sync\("
+LANES = r"if \((?:!?mine|in\b|!in\b|move|mx > |lane == 0|i >= it\.rows|n \+ j)|n \+ j < a\.N \?"
+
+
+def enclosing_loops(text, at):
+    """Starts and ends of the braced loop bodies around a place, the innermost first."""
+    found, depth, i = [], 0, at
+    while i > 0:
+        i -= 1
+        if text[i] == "}":
+            depth += 1
+        elif text[i] == "{" and depth:
+            depth -= 1
+        elif text[i] == "{":
+            if re.search(r"for \([^{};]*;[^{};]*;[^{};]*\)\s*$", text[max(0, i - 200):i]):
+                end, d = i + 1, 1
+                while d:
+                    d += {"{": 1, "}": -1}.get(text[end], 0)
+                    end += 1
+                found.append((i, end))
+    return found
+
+
+@pytest.mark.parametrize("name,calls", [("cross_attn.cu", r"\b(?:tmem_ld32_raw|tmem_st16|ldm4t?)\("),
+                                        ("int8_matmul.cu", r"\btmem_ld16\(|\bcluster_sync\(\)")])
+def test_warps_are_whole_where_an_instruction_takes_one(name, calls):
+    """Matrix loads, TMEM accesses and cluster barriers are executed by whole
+    warps.  Behind a branch that lanes take apart, in the text before them or
+    in an earlier turn of their loop, the lanes meet first; that the compiler brings
+    them together there is not its duty."""
+    text = source(name)
+    seen = 0
+    for m in re.finditer(calls, text):
+        if text[text.rindex("\n", 0, m.start()):m.start()].strip().startswith("__device__"):
+            continue  # the helper itself
+        seen += 1
+        before = text[:m.start()]
+        body = before.rindex("\n}\n")  # the end of the function before this one
+        met = max((x.end() for x in re.finditer(MEET, before)), default=-1)
+        apart = max((x.end() for x in re.finditer(LANES, before)), default=-1)
+        assert met > body and (apart < body or met > apart), before[-400:]
+        for a, b in enclosing_loops(text, m.start()):
+            if a < body:
+                break
+            last = [x.start() for x in re.finditer(LANES, text[a:b])]
+            meets = [x.start() for x in re.finditer(MEET, text[a:b])]
+            if last and last[-1] > m.start() - a:  # a branch behind it, before its next turn
+                assert any(x < m.start() - a or x > last[-1] for x in meets), text[a:m.start()][-400:]
+    assert seen
