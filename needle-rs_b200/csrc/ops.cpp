@@ -398,7 +398,7 @@ int needle_cross_attn_plan_run(NeedleCrossAttnPlan *p, const void *q, size_t q_r
       if (s < D || s % 8 || s > kMaxStride)
         return fail("cross attention: strides must be multiples of 8 elements and at least head_dim");
     const size_t H = (size_t)p->work.s.H, rows = (size_t)p->q_rows;
-    if (out_row < (H - 1) * out_head + D && (rows == 0 || out_head < (rows - 1) * out_row + D))
+    if (rows > 0 && out_row < (H - 1) * out_head + D && out_head < (rows - 1) * out_row + D)
       return fail("cross attention: rows and heads of out overlap");
     OnDevice on(p->device);
     if (!on.good() || !all_on(p->device, {{"q", q}, {"k", k}, {"v", v}, {"out", out}, {"key_mask", key_mask},

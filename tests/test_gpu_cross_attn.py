@@ -298,3 +298,10 @@ def test_run_refuses():
     at = (host.ctypes.data + 15) // 16 * 16
     with pytest.raises(nb.NeedleError, match="device memory|CUDA error"):
         plan.run(at, p, p, p, 0.125)
+
+
+@pytest.mark.parametrize("layout", ["token", "head", "fused"])
+def test_no_queries_in_any_layout(layout):
+    q, k, v, _, qs, ks = make([0, 0], [5, 6], 4, 2, 32, nb.F16, 1, gap=1)
+    od, ld = run(q, k, v, None, qs, [0, 0], ks, [5, 6], nb.F16, 0.2, layout)
+    assert (od == 7).all() and (ld == 7).all()
