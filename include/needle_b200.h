@@ -380,9 +380,10 @@ NeedleCrossAttnPlan *needle_cross_attn_plan_create(const uint64_t *q_start, cons
                                                    void *stream);
 /* Row r of head h of q is at q + r * q_row + h * q_head (elements), likewise
  * k, v and out: token-major and head-major layouts, and parts of fused rows.
- * Bases must be 16-byte aligned and strides multiples of 8 elements.  out must
- * not overlap the inputs or itself; rows outside the requests are left as
- * they were.  lse, if not NULL, is f32 [rows][num_heads], rows as in q, and
+ * Bases must be 16-byte aligned and strides multiples of 8 elements.  q and out
+ * may be NULL where no request has query rows, k and v where none that has any
+ * has keys.  out must not overlap the inputs or itself; rows outside the
+ * requests are left as they were.  lse, if not NULL, is f32 [rows][num_heads], rows as in q, and
  * receives log(sum_j exp(s_j)) (-infinity for a row without keys).  scale
  * must be positive.  Calls on one plan share its workspace and must be ordered
  * (one stream), and so must the replays of graphs that captured them. */

@@ -389,7 +389,9 @@ int needle_cross_attn_plan_run(NeedleCrossAttnPlan *p, const void *q, size_t q_r
                                const uint8_t *key_mask, float scale, void *out, size_t out_row, size_t out_head,
                                float *lse, void *stream) {
   return guarded([&] {
-    if (!p || !q || !k || !v || !out || !aligned(lse, 4)) return fail("invalid cross attention arguments");
+    // operands of no rows may be NULL, as an empty tensor's pointer is
+    if (!p || (p->q_rows && (!q || !out)) || (p->work.s.k_rows && (!k || !v)) || !aligned(lse, 4))
+      return fail("invalid cross attention arguments");
     if (!(scale > 0.0f) || std::isinf(scale)) return fail("cross attention: scale must be positive and finite");
     const size_t D = (size_t)p->work.s.D;
     for (const void *b : {q, k, v, (const void *)out})
@@ -404,6 +406,7 @@ int needle_cross_attn_plan_run(NeedleCrossAttnPlan *p, const void *q, size_t q_r
     if (!on.good() || !all_on(p->device, {{"q", q}, {"k", k}, {"v", v}, {"out", out}, {"key_mask", key_mask},
                                           {"lse", lse}}))
       return false;
+    if (p->work.s.k_rows == 0) k = v = q;  // any address: nothing is read from it
     XAttnCall c{q, k, v, key_mask, out, lse, (int64_t)q_row, (int64_t)q_head, (int64_t)k_row, (int64_t)k_head,
                 (int64_t)v_row, (int64_t)v_head, (int64_t)out_row, (int64_t)out_head, scale};
     return ok(cross_attn(p->work, c, p->flag, (cudaStream_t)stream));

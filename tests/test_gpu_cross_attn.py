@@ -305,3 +305,23 @@ def test_no_queries_in_any_layout(layout):
     q, k, v, _, qs, ks = make([0, 0], [5, 6], 4, 2, 32, nb.F16, 1, gap=1)
     od, ld = run(q, k, v, None, qs, [0, 0], ks, [5, 6], nb.F16, 0.2, layout)
     assert (od == 7).all() and (ld == 7).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("ql", [[1, 2], [3, 150], [0, 0]])
+def test_operands_of_no_rows_may_be_null(ql, D):
+    """The pointer of an empty tensor: K and V where no request has keys, q and out where none has queries."""
+    H, KVH, rows = 4, 2, sum(ql)
+    plan = nb.CrossAttnPlan([0, ql[0]], ql, [0, 0], [0, 0], H, KVH, D, nb.BF16)
+    q = torch.randn((rows, H, D), device="cuda").bfloat16()
+    empty = torch.empty((0, KVH, D), dtype=torch.bfloat16, device="cuda")
+    out, lse = torch.full_like(q, 7.0), torch.full((rows, H), 7.0, device="cuda")
+    assert empty.data_ptr() == 0 and (rows or q.data_ptr() == 0)
+    plan.run(q.data_ptr(), empty.data_ptr(), empty.data_ptr(), out.data_ptr(), 0.125, lse_ptr=lse.data_ptr())
+    plan.status()
+    assert (out == 0).all() and (lse == -float("inf")).all()
+    one = nb.CrossAttnPlan([0], [1], [0], [1], H, KVH, D, nb.BF16)
+    p = torch.zeros((1, H, D), dtype=torch.bfloat16, device="cuda").data_ptr()
+    for a in ((None, p, p, p), (p, None, p, p), (p, p, None, p), (p, p, p, None)):
+        with pytest.raises(nb.NeedleError, match="invalid"):
+            one.run(*a, 0.125)
