@@ -454,9 +454,10 @@ cudaError_t stream_rows(const ResidualNormArgs &a, bool *done, cudaStream_t st) 
 template <typename TX, typename TY>
 cudaError_t dispatch(const ResidualNormArgs &a, cudaStream_t st) {
   auto al = [](const void *p) { return ((uintptr_t)p & 15) == 0; };
-  const bool vec = a.d % 8 == 0 && al(a.x) && al(a.y) && al(a.gate) && al(a.r) && al(a.h) && al(a.post) && al(a.pre) &&
-                   a.ldx % 8 == 0 && (!a.y || a.ldy % 8 == 0) && (!a.r || a.ldr % 8 == 0) && a.ldh % 8 == 0 &&
-                   (a.gate_kind != 3 || a.ldg % 8 == 0);
+  // a scalar gate is read as one f32, wherever it lies
+  const bool vec = a.d % 8 == 0 && al(a.x) && al(a.y) && (a.gate_kind < 2 || al(a.gate)) && al(a.r) && al(a.h) && al(a.post) &&
+                   al(a.pre) && a.ldx % 8 == 0 && (!a.y || a.ldy % 8 == 0) && (!a.r || a.ldr % 8 == 0) &&
+                   (!a.h || a.ldh % 8 == 0) && (a.gate_kind != 3 || a.ldg % 8 == 0);
   if (vec) {
     bool done = false;
     if (a.d <= 8192) {

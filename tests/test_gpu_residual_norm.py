@@ -234,3 +234,25 @@ def test_graph_on_another_stream():
     r, h, er, eh = reference(x2, y, ps, g, True, 1.0, pre)
     close(rd, r, rounded(er, r, nb.F32))
     close(hd, h, rounded(eh, h, nb.BF16))
+
+
+@pytest.mark.parametrize("M,d,tx,ty", [(1, 512, nb.F32, nb.F32), (7, 2048, nb.F32, nb.BF16), (9000, 512, nb.BF16, nb.BF16), (2500, 4096, nb.F16, nb.F16)])
+def test_a_scalar_gate_lies_anywhere(M, d, tx, ty):
+    """One of an array of gates, a layer each: its address changes nothing, nor does the stride of an h that is not written."""
+    x, y, g, ps, pre = inputs(M, d, tx, ty, "scalar", True, M + d)
+    gates = torch.zeros(8, device="cuda")
+    xd, yd, pd, prd = cuda(x, y, ps, pre)
+    got = []
+    for at in (0, 1, 2, 3):
+        gates.fill_(float("nan"))
+        gates[at] = g[0]
+        rd, hd, r2 = torch.empty_like(xd), torch.empty_like(yd), torch.empty_like(xd)
+        common = dict(post_scale_ptr=p(pd), gate_ptr=p(gates[at:]), gate_flags=nb.GATE_SCALAR | nb.GATE_SIGMOID)
+        nb.residual_norm(p(xd), tx, p(yd), ty, M, d, p(prd), p(rd), p(hd), ty, **common)
+        nb.residual_norm(p(xd), tx, p(yd), ty, M, d, None, p(r2), None, ty, ldh=d + at, **common)
+        got.append((rd, hd, r2))
+    r, h, er, eh = reference(x, y, ps, g, True, 1.0, pre)
+    close(got[1][0], r, rounded(er, r, tx))
+    close(got[1][1], h, rounded(eh, h, ty))
+    for t in got[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(t, got[0]))
