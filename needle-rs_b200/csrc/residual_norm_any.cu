@@ -117,8 +117,8 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T, 1024 / (T < 128 ? 128 : T))
     for (int c = 0; c < P; ++c) {
       float u = 0.0f, v = 0.0f;
       if (c < nc) u = p[2 * (c * T + t)], v = p[min(2 * (c * T + t) + 1, d - 1)];
-      u = logi ? logistic16(u) : one + u;
-      v = logi ? logistic16(v) : one + v;
+      u = logi ? logistic(u) : one + u;
+      v = logi ? logistic(v) : one + v;
       r[c] = fmul2(r[c], f2pack(u, v));
     }
   };

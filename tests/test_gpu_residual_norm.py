@@ -256,3 +256,20 @@ def test_a_scalar_gate_lies_anywhere(M, d, tx, ty):
     close(got[1][1], h, rounded(eh, h, ty))
     for t in got[1:]:
         assert all(torch.equal(a, b) for a, b in zip(t, got[0]))
+
+
+@pytest.mark.parametrize("M,d", [(3, 512), (3, 131), (9000, 512), (9000, 257), (20000, 33), (1500, 4099)])
+def test_wide_f32_gates(M, d):
+    """The logistic function of f32 gates from -90 to 90: a few roundings, however far it is from 1.  x is zero, so
+    that r is the gated y alone; h follows the largest of a row.  (At -90 the function is below the normal range, where
+    exp(90) is infinite: 0 or its value, both within 2^-126.)"""
+    g = torch.Generator().manual_seed(d)
+    x, y = torch.zeros(M, d), torch.randn(M, d, generator=g)
+    gate = (torch.rand(d, generator=g) * 2 - 1) * 90
+    gate[:5] = torch.tensor([-90.0, -87.0, -20.0, 20.0, 90.0])
+    xd, yd, gd = cuda(x, y, gate)
+    rd = torch.empty_like(xd)
+    nb.residual_norm(p(xd), nb.F32, p(yd), nb.F32, M, d, None, p(rd), None, nb.F32, gate_ptr=p(gd), gate_flags=nb.GATE_CHANNEL | nb.GATE_SIGMOID)
+    want = y.double() * torch.sigmoid(gate.double())
+    # exp within 2 units, a unit being 2 U (and its own share of the sum), the sum, the quotient and the product half a unit each
+    close(rd, want, (2 * 2 + 3) * U * (1 + U) ** 8 * want.abs() + y.double().abs() * 2.0 ** -126)
