@@ -109,14 +109,16 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T, 1024 / (T < 128 ? 128 : T))
     if (a.sigmoid) g = logistic(g);
   }
   // pairs of this thread; a row's column behind the last (odd d) is kept zero in
-  // shared memory, so that no pair is a special case; factors of a pair's columns are read
-  // from L1 every row (registers for them would halve the blocks on an SM)
+  // shared memory, and its factor is finite, so that no pair is a special case; factors of a
+  // pair's columns are read from L1 every row (registers for them would halve the blocks on an SM)
   const int nc = ((d + 1) / 2 - t + T - 1) / T;
   auto times = [&](uint64_t *r, const float *p, float one, bool logi) {  // r *= one + p
 #pragma unroll
     for (int c = 0; c < P; ++c) {
       float u = 0.0f, v = 0.0f;
-      if (c < nc) u = p[2 * (c * T + t)], v = p[min(2 * (c * T + t) + 1, d - 1)];
+      const int i = 2 * (c * T + t);
+      if (c < nc) u = p[i];
+      if (i + 1 < d) v = p[i + 1];
       u = logi ? logistic(u) : one + u;
       v = logi ? logistic(v) : one + v;
       r[c] = fmul2(r[c], f2pack(u, v));

@@ -273,3 +273,20 @@ def test_wide_f32_gates(M, d):
     want = y.double() * torch.sigmoid(gate.double())
     # exp within 2 units, a unit being 2 U (and its own share of the sum), the sum, the quotient and the product half a unit each
     close(rd, want, (2 * 2 + 3) * U * (1 + U) ** 8 * want.abs() + y.double().abs() * 2.0 ** -126)
+
+
+@pytest.mark.parametrize("M,d", [(5, 257), (9000, 257), (20000, 33), (9000, 512)])
+@pytest.mark.parametrize("where", ["gate", "post"])
+def test_an_infinite_factor_stays_in_its_column(where, M, d):
+    """r is infinite in the last column alone; the row's mean is then infinite, and h = r / sqrt(infinity) is 0
+    in the other columns and NaN (infinity * 0) in that one."""
+    g = torch.Generator().manual_seed(d)
+    x, y, one = torch.randn(M, d, generator=g), torch.randn(M, d, generator=g), torch.zeros(d)
+    far = torch.zeros(d)
+    far[-1] = float("inf")
+    xd, yd, fd, od = cuda(x, y, far if where == "post" else far + 1, one)
+    rd, hd = torch.empty_like(xd), torch.empty_like(yd)
+    a = dict(post_scale_ptr=p(fd)) if where == "post" else dict(gate_ptr=p(fd), gate_flags=nb.GATE_CHANNEL)
+    nb.residual_norm(p(xd), nb.F32, p(yd), nb.F32, M, d, p(od), p(rd), p(hd), nb.F32, **a)
+    assert torch.isfinite(rd[:, :-1]).all() and torch.isinf(rd[:, -1]).all()
+    assert (hd[:, :-1] == 0).all() and torch.isnan(hd[:, -1]).all()
