@@ -55,8 +55,8 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *b, uint32_t parity, int *err
   }
 }
 
-// The same waits for warps that have time to spare beside busy ones: they sleep
-// between polls and leave the issue slots to the others.
+// The same wait for a warp that has time to spare beside busy ones: it sleeps
+// between polls and leaves the issue slots to the others.
 __device__ __forceinline__ bool mbar_sleep_wait(uint64_t *b, uint32_t parity, int *err) {
   if (mbar_try_wait(b, parity)) return true;
   const uint64_t t0 = globaltimer_ns();
@@ -71,9 +71,6 @@ __device__ __forceinline__ bool mbar_sleep_wait(uint64_t *b, uint32_t parity, in
       }
     }
   }
-}
-__device__ __forceinline__ bool warp_sleep_wait(uint64_t *b, uint32_t parity, int *err) {
-  return __all_sync(0xffffffffu, mbar_sleep_wait(b, parity, err));
 }
 
 // Bounded wait that ignores the error flag: after a wait gave up, lets the
@@ -191,23 +188,6 @@ __host__ __device__ constexpr uint32_t umma_idesc(int M, int N, bool b_mn = fals
          ((uint32_t)(M >> 4) << 24);
 }
 
-// UMMA descriptor of an MN-major operand with 128-byte swizzle whose MN
-// extent is one 64-element atom: rows of 128 bytes = 64 bf16 along MN, one
-// row per K index, 8-row (8 K) groups of 1024 bytes (SBO).
-// lbo: byte stride between consecutive 64-element MN atoms when the operand
-// spans more than one (N = 128 reads the atom at smem + lbo as elements
-// 64..127).
-__device__ __forceinline__ uint64_t umma_desc_mn(const void *smem, uint32_t lbo = 16) {
-  uint64_t addr = smem_u32(smem);
-  uint64_t d = 0;
-  d |= (addr >> 4) & 0x3FFFull;                 // start address
-  d |= (uint64_t)((lbo >> 4) & 0x3FFFu) << 16;  // LBO: stride between 64-element MN atoms
-  d |= (uint64_t)(1024 >> 4) << 32;  // SBO: stride between 8-row K groups
-  d |= (uint64_t)1 << 46;            // version
-  d |= (uint64_t)2 << 61;            // SWIZZLE_128B
-  return d;
-}
-
 // tcgen05.mma issued by the pair leader over both CTAs: A rows and B columns
 // split between the CTAs' shared memory at the same offsets, D split by rows
 // between their TMEM.
@@ -251,15 +231,6 @@ __device__ __forceinline__ void umma_bf16_ts_e(uint32_t d_tmem, uint32_t a_tmem,
       "setp.ne.b32 p, %4, 0;\n\t"
       "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
       "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc));
-}
-__device__ __forceinline__ void umma_bf16_pair_e(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc,
-                                                 uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p, e;\n\t"
-      "elect.sync _|e, 0xffffffff;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc));
 }
 __device__ __forceinline__ void umma_commit_e(uint64_t *bar) {
   asm volatile(

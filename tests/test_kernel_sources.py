@@ -69,7 +69,7 @@ def test_a_wait_that_ran_out_leaves_no_product_in_flight(name):
         assert given_up == issuers, kernel
 
 
-MEET = r"__syncwarp\(\)|__syncthreads\(\)|warp_wait\(|warp_sleep_wait\(|__any_sync\("
+MEET = r"__syncwarp\(\)|__syncthreads\(\)|warp_wait\(|__any_sync\("
 LANES = r"if \((?:!?mine|in\b|!in\b|move|mx > |lane == 0|i >= it\.rows|n \+ j)|n \+ j < a\.N \?"
 
 
@@ -118,3 +118,10 @@ def test_warps_are_whole_where_an_instruction_takes_one(name, calls):
             if last and last[-1] > m.start() - a:  # a branch behind it, before its next turn
                 assert any(x < m.start() - a or x > last[-1] for x in meets), text[a:m.start()][-400:]
     assert seen
+
+
+def test_every_device_function_is_called():
+    text = "\n".join(source(f) for f in sorted(os.listdir(SRC)))
+    made = r"__device__[^;{}()]*?\b%s\("
+    for name in set(re.findall(made % r"(\w+)", text)):
+        assert len(re.findall(r"\b%s\b" % name, text)) > len(re.findall(made % name, text)), name
