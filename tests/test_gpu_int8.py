@@ -237,3 +237,68 @@ def test_plan_refuses():
         plan.matmul(host.ctypes.data, 1, p)
     with pytest.raises(nb.NeedleError, match="invalid plan matmul"):
         plan.matmul_quantized(p + 4, p, 1, p)
+
+
+def launched(call):
+    """Names of the kernels that call(stream) launches, in order, from a graph that captures it."""
+    driver = pytest.importorskip("cuda.bindings.driver")
+    g = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(g, stream=torch.cuda.Stream()):
+        call(torch.cuda.current_stream().cuda_stream)
+    graph = driver.CUgraph(g.raw_cuda_graph())
+    err, _, n = driver.cuGraphGetNodes(graph)
+    err, nodes, n = driver.cuGraphGetNodes(graph, n)
+    assert err == driver.CUresult.CUDA_SUCCESS
+    names = []
+    for node in nodes[:n]:
+        if driver.cuGraphNodeGetType(node)[1] != driver.CUgraphNodeType.CU_GRAPH_NODE_TYPE_KERNEL:
+            continue
+        err, params = driver.cuGraphKernelNodeGetParams(node)
+        assert err == driver.CUresult.CUDA_SUCCESS
+        err, name = driver.cuFuncGetName(params.func) if int(params.func) else driver.cuKernelGetName(params.kern)
+        assert err == driver.CUresult.CUDA_SUCCESS
+        names.append(name.decode())
+    return names
+
+
+# M, K, N and the kernel of the product: tiles of 16 to 256 tokens, and pairs of CTAs with 256 x 256 tiles, whose last
+# tiles have few or odd channels, tokens and values of K; 153 tiles on 74 pairs use both accumulators again
+FORMS = [(1, 512, 2048, "int8_tc_kernelILi16E"), (16, 2048, 2048, "int8_tc_kernelILi16E"), (31, 4096, 4096, "int8_tc_kernelILi32E"),
+         (64, 4096, 4096, "int8_tc_kernelILi64E"), (200, 2050, 5001, "int8_tc_kernelILi128E"), (2100, 70, 8200, "int8_tc_kernelILi256E"),
+         (1025, 2050, 3001, "int8_pair_kernel"), (2049, 2050, 3001, "int8_pair_kernel"), (2049, 1100, 4099, "int8_pair_kernel"),
+         (4096, 512, 4096, "int8_pair_kernel"), (2305, 4097, 2304, "int8_pair_kernel")]
+
+
+@pytest.mark.parametrize("y_dtype", list(TYPES))
+@pytest.mark.parametrize("M,K,N,form", FORMS)
+def test_every_form_of_the_product(M, K, N, form, y_dtype):
+    g = torch.Generator(device="cuda").manual_seed(M + K + N)
+    Kp = nb.int8_row_bytes(K)
+    w = torch.full((N, Kp), 99, dtype=torch.int8, device="cuda")  # past K: never read
+    w[:, :K] = torch.randint(-128, 128, (N, K), generator=g, dtype=torch.int8, device="cuda")
+    ws = torch.rand(N, generator=g, device="cuda") * 0.02 + 0.001
+    bias = torch.randn(N, generator=g, device="cuda")
+    x_dtype = (M + y_dtype) % 3
+    x = torch.randn((M, K + 8), generator=g, device="cuda").to(TYPES[x_dtype])
+    q, qs = quantized(x[:, :K].cpu())
+    qd = torch.full((M, Kp), 55, dtype=torch.int8, device="cuda")
+    qd[:, :K] = torch.from_numpy(q).cuda()
+    qsd = torch.from_numpy(qs).cuda()
+    # exact in 64 bits: the sums stay below 2^53
+    prod = (qd[:, :K].double() @ w[:, :K].double().t()) * (qsd.double()[:, None] * ws.double()[None])
+    want = (prod + bias.double()).cpu()
+    plan = nb.Int8Plan(w.data_ptr(), ws.data_ptr(), K, N, M + 3)
+    y = torch.full((M + 1, N + 3), 7.0, dtype=TYPES[y_dtype], device="cuda")
+
+    def call(st):
+        plan.matmul(x.data_ptr(), M, y.data_ptr(), x_dtype, y_dtype, ldx=K + 8, ldy=N + 3, bias_ptr=bias.data_ptr(), stream=st)
+
+    call(None)
+    plan.status()
+    check(y[:M, :N], prod.cpu(), want, y_dtype)
+    assert (y[M] == 7).all() and (y[:M, N:] == 7).all()
+    y2 = torch.full((M, N), float("nan"), dtype=TYPES[y_dtype], device="cuda")
+    plan.matmul_quantized(qd.data_ptr(), qsd.data_ptr(), M, y2.data_ptr(), y_dtype, bias_ptr=bias.data_ptr())
+    plan.status()
+    assert torch.equal(y2, y[:M, :N])
+    assert form in launched(call)[-1], launched(call)
