@@ -12,6 +12,7 @@ namespace ndl {
 namespace {
 
 constexpr int kAnyPairs = 8;  // pairs of columns a thread, up to
+constexpr size_t kAnySmem = 226 * 1024;
 
 // The pairs of columns t, t + T, ... of a row that starts `off` bytes into a
 // 16-byte aligned buffer, read and written as words: lanes that hold neighbouring
@@ -70,7 +71,7 @@ __device__ __forceinline__ void pairs_out(uint8_t *buf, int off, int t, int nc, 
 // starts; T is a template, so that a pair's place is a constant.  Element by element in
 // global memory 14,785 x 6,738 bf16 took 847 us, element by element in shared memory 431
 // (92 instructions an element and warp), by pairs with T a variable 320.
-template <typename TX, typename TY, bool TOKEN, int T, int P>
+template <typename TX, typename TY, bool TOKEN, bool EACH, int T, int P>
 __global__ void __launch_bounds__(T < 128 ? 128 : T, 1024 / (T < 128 ? 128 : T)) residual_norm_any_kernel(ResidualNormArgs a, int bx, int by) {
   constexpr int S = kStreamStages, warps = T / 32;
   // a row group's shared memory: S stages of x, y and gate rows, then r and h
@@ -78,10 +79,15 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T, 1024 / (T < 128 ? 128 : T))
   __shared__ __align__(16) float sm[3][16];
   const int t = threadIdx.x, d = a.d;
   const bool have_y = TOKEN || a.y != nullptr;
-  if (warps > 1) {
+  // the logistic function of a channel gate: EACH row's work, or found once a block and kept behind the rows
+  const bool logi = !TOKEN && a.gate_kind == 2 && a.sigmoid, keep = !EACH && logi;
+  const int stage = bx + (TOKEN ? 2 : 1) * by;
+  float *gates = reinterpret_cast<float *>(buf + (size_t)blockDim.y * (S * stage + bx + by));
+  if (keep)
+    for (int i = threadIdx.y * T + t; i < d; i += T * blockDim.y) gates[i] = logistic(((const float *)a.gate)[i]);
+  if (warps > 1)
     for (int i = t; i < 48; i += T) (&sm[0][0])[i] = 0.0f;
-    __syncthreads();
-  }
+  if (warps > 1 || keep) __syncthreads();
   auto sync = [&] {
     if (warps > 1)
       __syncthreads();
@@ -91,7 +97,6 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T, 1024 / (T < 128 ? 128 : T))
   const int64_t step = (int64_t)gridDim.x * blockDim.y;
   int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   if (row >= a.M) return;  // blockDim.y > 1 only when a warp owns a row: no barrier is skipped
-  const int stage = bx + (TOKEN ? 2 : 1) * by;
   uint8_t *in = buf + (size_t)threadIdx.y * (S * stage + bx + by), *out_r = in + S * stage, *out_h = out_r + bx;
   auto fetch = [&](int64_t at, int s) {
     if (at < a.M) {
@@ -109,22 +114,21 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T, 1024 / (T < 128 ? 128 : T))
     if (a.sigmoid) g = logistic(g);
   }
   // pairs of this thread; a row's column behind the last (odd d) is kept zero in
-  // shared memory, and its factor is finite, so that no pair is a special case; factors of a
-  // pair's columns are read from L1 every row (registers for them would halve the blocks on an SM)
+  // shared memory, so that no pair is a special case; factors of a pair's columns are read
+  // from L1 every row (registers for them would halve the blocks on an SM)
   const int nc = ((d + 1) / 2 - t + T - 1) / T;
-  auto times = [&](uint64_t *r, const float *p, float one, bool logi) {  // r *= one + p
+  const int odd = (d & 1) && (d >> 1) % T == t ? (d >> 1) / T : -1;  // the pair that holds that column
+  auto times = [&](uint64_t *r, const float *p, float one) {  // r *= one + p; EACH: logistic(p) for the gate
 #pragma unroll
     for (int c = 0; c < P; ++c) {
       float u = 0.0f, v = 0.0f;
-      const int i = 2 * (c * T + t);
-      if (c < nc) u = p[i];
-      if (i + 1 < d) v = p[i + 1];
-      u = logi ? logistic(u) : one + u;
-      v = logi ? logistic(v) : one + v;
+      if (c < nc) u = p[2 * (c * T + t)], v = p[min(2 * (c * T + t) + 1, d - 1)];
+      u = EACH && one == 0.0f ? logistic(u) : one + u;
+      v = EACH && one == 0.0f ? logistic(v) : one + v;
       r[c] = fmul2(r[c], f2pack(u, v));
     }
   };
-  const float *channel = a.gate_kind == 2 ? (const float *)a.gate : nullptr;
+  const float *channel = a.gate_kind != 2 ? nullptr : keep ? gates : (const float *)a.gate;
   const uint64_t zero = f2pack(0.0f, 0.0f), sc = f2pack(a.scale, a.scale);
   const float over_d = 1.0f / (float)d;
   // bytes from the last 16-byte boundary to row `at` of p
@@ -158,8 +162,8 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T, 1024 / (T < 128 ? 128 : T))
       }
 #pragma unroll
       for (int c = 0; c < P; ++c) r[c] = fmul2(r[c], f2pack(inv, inv));
-      if (a.post) times(r, a.post, 1.0f, false);
-      if (!TOKEN && channel) times(r, channel, 0.0f, a.sigmoid);
+      if (a.post) times(r, a.post, 1.0f);
+      if (!TOKEN && channel) times(r, channel, 0.0f);
       if (TOKEN) {
         pairs_in<TY, T, P>(at + bx + by, og, t, nc, v);
 #pragma unroll
@@ -170,6 +174,14 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T, 1024 / (T < 128 ? 128 : T))
             v[c] = f2pack(sizeof(TY) == 2 ? logistic16(x0) : logistic(x0), sizeof(TY) == 2 ? logistic16(x1) : logistic(x1));
           }
           r[c] = fmul2(r[c], v[c]);
+        }
+      }
+      if (odd >= 0) {  // the last column's factor, which that column was multiplied by, may be infinite
+#pragma unroll
+        for (int c = 0; c < P; ++c) {
+          float x0, x1;
+          f2unpack(r[c], x0, x1);
+          if (c == odd) r[c] = f2pack(x0, 0.0f);
         }
       }
     }
@@ -185,7 +197,7 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T, 1024 / (T < 128 ? 128 : T))
       const float inv = rsqrtf(fmaf(stream_sum(ss, warps, sm[1]), over_d, kEps));
 #pragma unroll
       for (int c = 0; c < P; ++c) r[c] = fmul2(r[c], f2pack(inv, inv));
-      times(r, a.pre, 1.0f, false);
+      times(r, a.pre, 1.0f);
       if (a.h_dtype == DT_I8) {
         uint32_t top = 0;  // largest |h| as bits: infinities and NaN order above every number
 #pragma unroll
@@ -225,21 +237,32 @@ cudaError_t launch_any(const ResidualNormArgs &a, bool *done, cudaStream_t st) {
   // bytes of a row and its offset, to the next 16-byte boundary
   const int bx = (a.d * (int)sizeof(TX) + 31) / 16 * 16, by = (a.d * (int)sizeof(TY) + 31) / 16 * 16;
   const size_t smem = (size_t)rows * (kStreamStages * (bx + (TOKEN ? 2 : 1) * by) + bx + by);
-  auto *kernel = residual_norm_any_kernel<TX, TY, TOKEN, T, P>;
-  static thread_local int last_dev = -1, last_d = 0, fit = 0;
+  const size_t kept_smem = smem + 4 * (size_t)a.d;
+  auto *kernel = residual_norm_any_kernel<TX, TY, TOKEN, false, T, P>;
+  // the form that finds a channel gate's logistic function for each row: where one block would be left of two
+  constexpr bool kEach = !TOKEN && T == 512;
+  auto *each_row = residual_norm_any_kernel<TX, TY, TOKEN, kEach, T, P>;
+  static thread_local int last_dev = -1, last_d = 0, fit = 0, fit_kept = 0;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && (last_dev != dev || last_d != a.d)) {
-    int sms = 0, each = 0;
+    int sms = 0, each = 0, kept = 0;
     e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
-    if (e == cudaSuccess && smem <= 200 * 1024)
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kAnySmem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(each_row, cudaFuncAttributeMaxDynamicSharedMemorySize, kAnySmem);
+    if (e == cudaSuccess && smem <= kAnySmem)
       e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&each, kernel, T * rows, smem);
-    if (e == cudaSuccess) last_dev = dev, last_d = a.d, fit = sms * each;
+    if (e == cudaSuccess && kept_smem <= kAnySmem)
+      e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&kept, kernel, T * rows, kept_smem);
+    if (e == cudaSuccess) last_dev = dev, last_d = a.d, fit = sms * each, fit_kept = sms * kept;
   }
-  *done = e != cudaSuccess || (fit > 0 && a.M >= (int64_t)fit * rows);
+  // 9,001 x 2,050, f32 and bf16, a sigmoid channel gate: 94 us kept, 119 for each row; 9,001 x 8,190
+  // bf16, where one block would be left of two: 333 and 283
+  const bool logi = a.gate_kind == 2 && a.sigmoid, keep = logi && !(kEach && fit_kept < fit);
+  const int blocks = keep ? fit_kept : fit;
+  *done = e != cudaSuccess || (blocks > 0 && a.M >= (int64_t)blocks * rows);
   if (e != cudaSuccess || !*done) return e;
-  kernel<<<dim3((unsigned)fit), dim3(T, rows), smem, st>>>(a, bx, by);
+  (logi && !keep ? each_row : kernel)<<<dim3((unsigned)blocks), dim3(T, rows), keep ? kept_smem : smem, st>>>(a, bx, by);
   return cudaGetLastError();
 }
 

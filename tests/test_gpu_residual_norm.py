@@ -258,7 +258,7 @@ def test_a_scalar_gate_lies_anywhere(M, d, tx, ty):
         assert all(torch.equal(a, b) for a, b in zip(t, got[0]))
 
 
-@pytest.mark.parametrize("M,d", [(3, 512), (3, 131), (9000, 512), (9000, 257), (20000, 33), (1500, 4099)])
+@pytest.mark.parametrize("M,d", [(3, 512), (3, 131), (9000, 512), (9000, 257), (20000, 33), (2500, 2051), (1500, 4099), (1300, 8191)])
 def test_wide_f32_gates(M, d):
     """The logistic function of f32 gates from -90 to 90: a few roundings, however far it is from 1.  x is zero, so
     that r is the gated y alone; h follows the largest of a row.  (At -90 the function is below the normal range, where
