@@ -325,3 +325,67 @@ def test_operands_of_no_rows_may_be_null(ql, D):
     for a in ((None, p, p, p), (p, None, p, p), (p, p, None, p), (p, p, p, None)):
         with pytest.raises(nb.NeedleError, match="invalid"):
             one.run(*a, 0.125)
+
+
+VISIBLE = [([1], [20000], 8, 4, 64), ([1, 3], [9000, 70], 4, 4, 64), ([2], [4097], 2, 1, 128), ([40], [5000], 4, 2, 64),
+           ([130, 1], [3001, 641], 2, 2, 128), ([300, 17], [700, 385], 4, 2, 80), ([1] * 40, [500 + 13 * i for i in range(40)], 4, 2, 64)]
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("i", range(len(VISIBLE)))
+def test_every_block_of_keys_is_seen_by_itself(i, dtype, masked):
+    """Each column of V is zero but for one block of 64 keys, with a value of its own for each key of it, so that an
+    output is that block's share of the weights: a key that is left out, taken twice or from elsewhere, in a tile, in the last
+    part of one or where a range is cut, moves it by about a sixty-fourth.  Scores are small, so that every block has a share.
+
+    Relative to a share: the errors of the scores and exponentials (as above), half a step of the type for each
+    weight, n + 4 U of the sums, and the row's sum with the same but for the step.  A row's sum is at least 1 in units of
+    its largest weight, and no weight was rounded in smaller units than that (a running maximum is never above
+    the final one), so f16 adds at most half of its smallest step, 2^-25, for each key of the block."""
+    ql, kl, H, KVH, D = VISIBLE[i]
+    q, k, _, mask, qs, ks = make(ql, kl, H, KVH, D, dtype, 100 + i, 0.7 if masked else 1.0, gap=1, width=0.3)
+    t, scale, eps = TYPES[dtype], D ** -0.5, torch.finfo(TYPES[dtype]).eps
+    tiny = 2.0 ** -25 if dtype == nb.F16 else 0.0
+    cols = KVH * D
+    plan = nb.CrossAttnPlan(qs, ql, ks, kl, H, KVH, D, dtype)
+    qd, kd, md = q.cuda(), k.cuda(), None if mask is None else mask.cuda()
+    od = torch.empty_like(qd)
+    for first in range(0, (max(kl) + 63) // 64, cols):
+        v = torch.zeros((k.shape[0], cols), dtype=t)
+        for b, m in zip(ks, kl):
+            j = torch.arange(m)
+            at = j // 64 - first
+            ok = (at >= 0) & (at < cols)
+            v[b + j[ok], at[ok]] = (1 + (j[ok] % 64) / 64).to(t)  # exact in 8 bits
+        vd = v.view(-1, KVH, D).cuda()
+        plan.run(qd.data_ptr(), kd.data_ptr(), vd.data_ptr(), od.data_ptr(), scale, key_mask_ptr=None if md is None else md.data_ptr())
+        plan.status()
+        for a, n, b, m in zip(qs, ql, ks, kl):
+            seen = torch.arange(b, b + m, device="cuda")
+            if md is not None:
+                seen = seen[md[b:b + m] != 0]
+            kk, vv = (x[seen].double().repeat_interleave(H // KVH, dim=1) for x in (kd, vd))
+            qq = qd[a:a + n].double()
+            s = torch.einsum("qhd,khd->hqk", qq, kk) * scale
+            es = torch.einsum("qhd,khd->hqk", qq.abs(), kk.abs()) * (scale * 2 * (D + 8) * U)
+            pr = torch.softmax(s, -1)
+            top = s.amax(-1, keepdim=True)
+            ep = es + (8 + (s - top).abs() * 2) * U
+            rel = ((pr * ep).sum(-1) + (seen.numel() + 4) * U).t()[..., None]
+            want = torch.einsum("hqk,khd->qhd", pr, vv)
+            e = torch.einsum("hqk,khd->qhd", pr * (ep + eps / 2 * (1 + eps)), vv) + want * (rel + (seen.numel() + 4) * U)
+            e = e + tiny * (vv.sum(0)[None] / torch.exp(s - top).sum(-1).t()[..., None])
+            close(od[a:a + n], want.cpu(), e.cpu(), dtype)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n", [1, 40, 200])
+def test_values_of_one(n, dtype):
+    """All values 1: an output is the sum of the rounded weights over the sum of the weights."""
+    m, H, KVH, D = 7001, 4, 2, 64
+    q, k, v, mask, qs, ks = make([n], [m], H, KVH, D, dtype, n, 0.9)
+    od, _ = run(q, k, torch.ones_like(v), mask, qs, [n], ks, [m], dtype, 0.125, check=False)
+    half = torch.finfo(TYPES[dtype]).eps / 2
+    tiny = 2.0 ** -25 * m if dtype == nb.F16 else 0.0
+    assert ((od.double() - 1).abs() <= half + tiny + 2 * (m + 4) * U + half * (1 + 2 * half)).all()
