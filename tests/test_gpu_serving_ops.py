@@ -156,3 +156,37 @@ def test_an_error_is_reported_once():
         nb.residual_norm(x.data_ptr(), nb.F32, None, nb.F32, 2, 64, pre.data_ptr(), None, h.data_ptr(), nb.F32)
     torch.cuda.synchronize()
     assert torch.isfinite(h).all()
+
+
+@pytest.mark.parametrize("ql,kl,H,KVH,D", [([1] * 9, [400, 31, 0, 512, 7, 300, 1000, 64, 65], 8, 4, 64), ([3, 130], [700, 2500], 6, 2, 40)])
+def test_attention_behind_norms_of_heads(ql, kl, H, KVH, D):
+    """As the shipped model has it: query heads and key heads are normed between their product and the attention,
+    by the residual norm without a block's output on a row for each token and head."""
+    d, M, R = 512, sum(ql), sum(kl)
+    qs, ks = ([sum(n[:i]) for i in range(len(n))] for n in (ql, kl))
+    g = torch.Generator().manual_seed(D)
+    p = lambda t: t.data_ptr()  # noqa: E731
+    e = lambda *s: torch.zeros(s, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    h, enc = (torch.randn(n, d, generator=g).bfloat16().cuda() for n in (M, R))
+    q_scale, k_scale = ((torch.randn(D, generator=g) * 0.1).cuda() for _ in range(2))
+    w = {n: random_weight(heads * D, d, seed) for n, heads, seed in (("q", H, 1), ("k", KVH, 2), ("v", KVH, 3))}
+    wd = {n: (a.cuda(), (s / 16).cuda()) for n, (a, s) in w.items()}
+    plan = {n: nb.Int8Plan(p(a), p(s), d, a.shape[0], M if n == "q" else R) for n, (a, s) in wd.items()}
+    attn = nb.CrossAttnPlan(qs, ql, ks, kl, H, KVH, D, nb.BF16)
+    q, qn, a, k, kn, v = e(M, H, D), e(M, H, D), e(M, H, D), e(R, KVH, D), e(R, KVH, D), e(R, KVH, D)
+    plan["k"].matmul(p(enc), R, p(k), nb.BF16, nb.BF16)  # once a prompt
+    plan["v"].matmul(p(enc), R, p(v), nb.BF16, nb.BF16)
+    nb.residual_norm(p(k), nb.BF16, None, nb.BF16, R * KVH, D, p(k_scale), None, p(kn), nb.BF16)
+    plan["q"].matmul(p(h), M, p(q), nb.BF16, nb.BF16)
+    nb.residual_norm(p(q), nb.BF16, None, nb.BF16, M * H, D, p(q_scale), None, p(qn), nb.BF16)
+    attn.run(p(qn), p(kn), p(v), p(a), D ** -0.5)
+    for plan_ in [*plan.values(), attn]:
+        plan_.status()
+    for n, x, got in (("q", h, q), ("k", enc, k), ("v", enc, v)):
+        x8, xs = quantized(x.cpu())
+        check(got.view(got.shape[0], -1), *expected(torch.from_numpy(x8), torch.from_numpy(xs), w[n][0], wd[n][1].cpu(), None, d), nb.BF16)
+    for x, s, got in ((q, q_scale, qn), (k, k_scale, kn)):
+        _, want, _, err = norm_reference(x.view(-1, D).cpu(), None, None, None, False, 1.0, s.cpu())
+        close(got.view(-1, D), want, rounded(err, want, nb.BF16))
+    out, _, eo, _ = attn_reference(qn.cpu(), kn.cpu(), v.cpu(), None, qs, ql, ks, kl, D ** -0.5)
+    attn_close(a, out, eo, nb.BF16)
