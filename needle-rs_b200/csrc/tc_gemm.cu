@@ -503,7 +503,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int num_m = (M + TC_BM - 1) / TC_BM, num_n = (N + BN - 1) / BN;
   const int tiles = num_m * num_n, nkb = Kp / TC_BK;
-  pdl_trigger();
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < TC_STAGES; ++s) {
@@ -525,6 +524,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *(volatile uint32_t *)tmem_slot;
+  // not before TMEM is held: a kernel behind this one could take it and wait for this one's end
+  pdl_trigger();
   // under programmatic dependent launch the setup above overlaps the previous
   // kernel's tail; global memory is touched only after it has completed
   pdl_wait();
@@ -890,7 +891,6 @@ __global__ void __launch_bounds__(TC_SPLITK_THREADS, 1)
   const int mt = tile / num_n, nt = tile - mt * num_n;
   const int kper = Kp / TC_BK / S, kb0 = (int)rank * kper;
   float *tile_ws = e.o.splitk_ws + (size_t)tile * S * (128 * BN);
-  pdl_trigger();
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -909,6 +909,7 @@ __global__ void __launch_bounds__(TC_SPLITK_THREADS, 1)
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *(volatile uint32_t *)tmem_slot;
+  pdl_trigger();  // not before TMEM is held: a kernel behind this one could take it and wait for this one's end
 
   if (warp == 0 && lane == 0) {
     // ── TMA producer: this CTA's K slice.  The weight (B) tiles of the first

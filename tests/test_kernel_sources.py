@@ -30,7 +30,7 @@ def kernels(name):
     return found
 
 
-@pytest.mark.parametrize("name", ["cross_attn.cu", "int8_matmul.cu"])
+@pytest.mark.parametrize("name", ["cross_attn.cu", "int8_matmul.cu", "tc_gemm.cu", "tc_attn.cu"])
 def test_tmem_is_held_before_the_next_kernel_may_start(name):
     """griddepcontrol.launch_dependents counts for a block from its first
     thread on.  A dependent kernel that starts before the block holds its TMEM
