@@ -276,7 +276,10 @@ void needle_ffn_plan_free(NeedleFfnPlan *plan);
  * plans' creation is asynchronous, allocates nothing and can be captured into
  * a CUDA graph.  Sizes of zero are refused unless a comment says otherwise;
  * counts of rows and channels go up to 2^31 - 256.  A graph that captured a
- * plan's calls must not be replayed after the plan is freed. */
+ * plan's calls must not be replayed after the plan is freed.  A kernel of the
+ * caller that is launched programmatically behind a call may start before
+ * that has ended: it waits (griddepcontrol.wait) before it touches what the
+ * call reads or writes. */
 
 /* Element types of the operands below. */
 #define NEEDLE_F32 0
@@ -337,7 +340,12 @@ void needle_int8_plan_free(NeedleInt8Plan *plan);
  * The gate g is 1 (gate_flags 0, gate NULL), one f32 (NEEDLE_GATE_SCALAR), f32[d]
  * (NEEDLE_GATE_CHANNEL) or a [M][ldg] matrix of y's type
  * (NEEDLE_GATE_TOKEN); with NEEDLE_GATE_SIGMOID added, the logistic function
- * of that.  All arithmetic is f32.
+ * of that.  All arithmetic is f32.  How many rows come together and whether they
+ * start on 16-byte boundaries decides the order of a row's sums and whether its
+ * factor is a root's quotient or a reciprocal root, so a row's last bits may
+ * depend on them; the same call gives the same bits.  The logistic function of a
+ * token gate of 16 bits is off by a few f32 units and one more for each unit of
+ * its argument.
  *   y NULL: r is x * residual_scale and only h is written (r must be NULL):
  *     the norm before the first block; post_scale and gate must be NULL.
  *   h NULL: only r is written; pre_scale must be NULL then.
@@ -368,11 +376,13 @@ int needle_residual_norm(const void *x, int x_dtype, size_t ldx, const void *y, 
  * is not zero; what masked keys and rows outside the request hold, NaN
  * and infinity included, changes nothing.  A row without keys gives zeros.
  * dtype: f16 or bf16 for q, k, v and out (sums in f32; the weights are rounded
- * to dtype for the product with V); head_dim a multiple of 8 up to 128.
+ * to dtype for the product with V); head_dim a multiple of 8 up to 128;
+ * num_heads a multiple of num_kv_heads up to 4096.
  * The plan holds the split of the requests over the device and the
  * workspace: lengths stay fixed while a prompt is decoded, so one plan serves
- * every layer and step.  It belongs to the device that is current when it is
- * created. */
+ * every layer and step.  Other lengths take another plan: creating one splits the
+ * requests on the host, allocates, copies and waits for the stream.  It belongs
+ * to the device that is current when it is created. */
 typedef struct NeedleCrossAttnPlan NeedleCrossAttnPlan;
 NeedleCrossAttnPlan *needle_cross_attn_plan_create(const uint64_t *q_start, const uint64_t *q_len,
                                                    const uint64_t *k_start, const uint64_t *k_len, size_t n_seq,
@@ -380,12 +390,13 @@ NeedleCrossAttnPlan *needle_cross_attn_plan_create(const uint64_t *q_start, cons
                                                    void *stream);
 /* Row r of head h of q is at q + r * q_row + h * q_head (elements), likewise
  * k, v and out: token-major and head-major layouts, and parts of fused rows.
- * Bases must be 16-byte aligned and strides multiples of 8 elements.  q and out
+ * Bases must be 16-byte aligned and strides multiples of 8 elements, head_dim or
+ * more (also that of a single head).  q and out
  * may be NULL where no request has query rows, k and v where none that has any
  * has keys.  out must not overlap the inputs or itself; rows outside the
  * requests are left as they were.  lse, if not NULL, is f32 [rows][num_heads], rows as in q, and
  * receives log(sum_j exp(s_j)) (-infinity for a row without keys).  scale
- * must be positive.  Calls on one plan share its workspace and must be ordered
+ * must be positive and finite.  Calls on one plan share its workspace and must be ordered
  * (one stream), and so must the replays of graphs that captured them. */
 int needle_cross_attn_plan_run(NeedleCrossAttnPlan *plan, const void *q, size_t q_row, size_t q_head, const void *k,
                                size_t k_row, size_t k_head, const void *v, size_t v_row, size_t v_head,

@@ -208,7 +208,8 @@ __device__ __forceinline__ void put8(T *p, const uint64_t *v) {
 // throughout, the reciprocal square root of CUDA instead of an exact root and
 // quotient (its 2 ulp are part of the row factor's few), and what is known before the
 // first row as a template: MODE 0 no y, 1 y, 2 y and a token gate; FULL: every
-// thread has all its vectors.  169 us now: 6.4 TB/s.
+// thread has all its vectors.  172 us now, 6.2 TB/s; calls one behind the other whose
+// outputs rotate over four buffers take 185 (5.8 TB/s), as they do for any writer.
 template <typename TX, typename TY, int MODE, bool FULL, int CH>
 __global__ void __launch_bounds__(512) residual_norm_stream_kernel(ResidualNormArgs a) {
   constexpr int S = kStreamStages, PX = sizeof(TX) / 2, PY = sizeof(TY) / 2;  // 16-byte pieces of 8 elements
@@ -433,8 +434,8 @@ cudaError_t stream_vectors(const ResidualNormArgs &a, bool *done, cudaStream_t s
                            : launch_stream<TX, TY, MODE, false, CH>(a, T, done, st);
 }
 // One vector of 8 a thread, two above 4,096 elements: more warps with fewer
-// columns each cover each other's reductions better (65,536 x 2,048 bf16:
-// 169 us with one, 190 with two).
+// columns each cover each other's reductions better (65,536 x 2,048 bf16 into one
+// buffer: 169 us with one, 190 with two).
 template <typename TX, typename TY, int MODE>
 cudaError_t stream_mode(const ResidualNormArgs &a, bool *done, cudaStream_t st) {
   return a.d <= 4096 ? stream_vectors<TX, TY, MODE, 1>(a, done, st) : stream_vectors<TX, TY, MODE, 2>(a, done, st);
