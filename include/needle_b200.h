@@ -310,8 +310,8 @@ int needle_int8_quantize_weight(const void *w, int w_dtype, size_t K, size_t N, 
 /* A prepared 8-bit weight (data [N][row_bytes(K)], 16-byte aligned, and
  * scales[N], both kept by the caller while the plan lives) for
  *   y[m][n] = (sum_k q[m][k] w[n][k]) * (q_scales[m] * w_scales[n]) + bias[n]
- * with an exact 32-bit integer sum (K <= 131,071), rounded once to y_dtype
- * (f32, f16 or bf16).  needle_int8_plan_matmul quantises the tokens
+ * with an exact 32-bit integer sum (K <= 131,071), the rest in f32, rounded
+ * once to y_dtype (f32, f16 or bf16).  needle_int8_plan_matmul quantises the tokens
  * x[M][ldx] first (the same values as needle_int8_quantize_tokens), into the
  * plan's workspace of max_m rows; needle_int8_plan_matmul_quantized takes rows
  * that are quantised already (q 16-byte aligned).  M <= max_m; bias (f32[N])

@@ -11,8 +11,9 @@ constexpr int kStreamStages = 2;  // rows in shared memory: the current one and 
 
 __device__ __forceinline__ float logistic(float v) { return 1.0f / (1.0f + expf(-v)); }
 
-// The same for a gate read from 16 bits, by the approximate instructions (a few
-// ulp and one more for each unit of |v|).
+// The same for a token gate read from 16 bits, by the approximate instructions (a few
+// ulp and one more for each unit of |v|, below half a step of the gate's own type up to
+// |v| = 90); gates of f32 take the form above.
 __device__ __forceinline__ float logistic16(float v) {
   float e;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * -1.4426950408889634f));
