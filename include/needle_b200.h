@@ -406,6 +406,109 @@ int needle_cross_attn_plan_run(NeedleCrossAttnPlan *plan, const void *q, size_t 
 int needle_cross_attn_plan_status(NeedleCrossAttnPlan *plan);
 void needle_cross_attn_plan_free(NeedleCrossAttnPlan *plan);
 
+/* A decoder's keys and values in 4 bits, in pages.  A page holds page_tokens
+ * (a multiple of 16) tokens of a request for all KV heads,
+ * needle_kv4_page_bytes bytes; `pages` is an array of n_pages of them on the device, on a
+ * 128-byte boundary, one for each layer, kept by the caller.  A page's bytes are
+ * the library's own order.
+ * A head's dimensions are held in groups of 32 (the last one may be shorter):
+ *   minimum = f16(min x), scale = f16((max x - min x) / 15)
+ *   code = rint((x - minimum) * (1 / scale)) within 0 to 15 (0 for scale 0)
+ *   x stands for minimum + scale * code
+ * each operation but the roundings to f16 rounded to f32, rint to even: 5 bits a
+ * value.  A token and head whose key or value holds an infinity, NaN
+ * or a magnitude above 32,768 reads as NaN, key and value, and makes the rows that attend to it
+ * NaN; others are not touched by it.  Groups whose range is below 15 * 2^-14
+ * are rounded as f16's subnormal scales allow.
+ *
+ * The plan holds the shapes and the workspace; it serves every layer.  It belongs to the device that is
+ * current when it is created.  dtype (f16 or bf16) is that of keys, values,
+ * queries and outputs; head_dim a multiple of 8 up to 128; num_heads a
+ * multiple of num_kv_heads up to 4096.
+ *
+ * The requests of a call are arrays on the device, so that a captured call
+ * sees the lengths of its replay: request i has rows
+ * [row_start[i], row_start[i + 1]) of the operands (which have `rows` rows; rows of no
+ * request are left alone), kv_len[i] tokens in its cache, and its token t is
+ * in page page_table[i * table_width + t / page_tokens].  A request may have no rows and no
+ * tokens.  Entries of the table behind a request's tokens are not read.  Kernels
+ * check the numbers: row starts that fall or pass `rows`, lengths below zero or past
+ * table_width pages, and pages outside the array are found by
+ * needle_kv4_plan_status.  Such a request's results are undefined then (where
+ * row starts fall, those of all), and nothing outside the operands and the
+ * pages is touched. */
+typedef struct NeedleKv4Plan NeedleKv4Plan;
+typedef struct NeedleKv4Batch {
+  const int32_t *row_start;  /* [n_seq + 1] */
+  const int32_t *kv_len;     /* [n_seq] */
+  const int32_t *page_table; /* [n_seq][table_width] */
+  size_t n_seq, rows, table_width;
+} NeedleKv4Batch;
+size_t needle_kv4_page_bytes(size_t num_kv_heads, size_t head_dim, size_t page_tokens);
+NeedleKv4Plan *needle_kv4_plan_create(size_t num_heads, size_t num_kv_heads, size_t head_dim, size_t page_tokens,
+                                      size_t n_pages, size_t max_seqs, size_t max_rows, int dtype, void *stream);
+/* Row r of head h of an operand is at base + r * row + h * head (elements):
+ * bases on 16-byte boundaries, strides multiples of 8 elements and at least head_dim.
+ * append: a request's rows of k and v become its last tokens, kv_len[i]
+ * counts them already.  A page that two requests of a call write, at the same token, holds either.
+ * read: the values of a request's last tokens, as many as it has
+ * rows, rounded once to dtype; k_out or v_out may be NULL. */
+int needle_kv4_append(NeedleKv4Plan *plan, void *pages, const NeedleKv4Batch *batch, const void *k, size_t k_row,
+                      size_t k_head, const void *v, size_t v_row, size_t v_head, void *stream);
+int needle_kv4_read(NeedleKv4Plan *plan, const void *pages, const NeedleKv4Batch *batch, void *k_out, size_t k_row,
+                    size_t k_head, void *v_out, size_t v_row, size_t v_head, void *stream);
+/* Attention of a request's rows of q to its cache: out, lse and the order of heads as
+ * needle_cross_attn_plan_run.  With NEEDLE_KV4_CAUSAL the rows are the
+ * request's last tokens (appended before): row j of n sees the first
+ * kv_len - n + j + 1.  Without it every row sees all kv_len tokens, which may be none: zeros.
+ * Sums are f32; the weights of the sum over values, and the values, are rounded to f16.
+ * out must not overlap q or itself.  Calls of a plan's attention share its workspace and must be ordered (one
+ * stream), and so must the replays of graphs that captured them. */
+#define NEEDLE_KV4_CAUSAL 1u
+int needle_kv4_attn(NeedleKv4Plan *plan, const void *pages, const NeedleKv4Batch *batch, const void *q, size_t q_row,
+                    size_t q_head, float scale, uint32_t flags, void *out, size_t out_row, size_t out_head, float *lse,
+                    void *stream);
+/* As needle_int8_plan_status; also -1 if a batch's numbers did not fit since the last check. */
+int needle_kv4_plan_status(NeedleKv4Plan *plan);
+void needle_kv4_plan_free(NeedleKv4Plan *plan);
+
+/* Drafted tokens against the target's logits.  Request i has the drafts
+ * [draft_start[i], draft_start[i + 1]) of draft_ids (draft_start on the device, [n_seq + 1], from
+ * n_drafts drafts in all; a request may have none) and one row of logits [ldl] more than drafts: row
+ * draft_start[i] + i + j belongs to its token j.  With
+ *   p = softmax(logits / temperature[i])    over the row's allowed entries
+ * draft t is taken while accept_u[t] * q < p[draft], q = draft_probs[t][draft] (f32
+ * rows [ldp] that the draft was drawn from), or 1 where draft_probs is NULL.
+ * The first one that is not is replaced by an entry of max(p - q, 0) (NULL:
+ * of p without the draft; where that leaves nothing, of p); behind the last draft follows an
+ * entry of p.  The entry of weights w is the first v with w_0 + .. + w_v > final_u[i] * sum(w):
+ * the random numbers are the caller's, in [0, 1).  Weights and sums are 64-bit there.
+ * temperature NULL is 1.  Zero (or less) is greedy: a draft is taken while it
+ * is the row's largest logit, which follows else; of equal ones the lowest
+ * index, with NEEDLE_VERIFY_LAST_TIE the highest (as the engine's own head).
+ * An entry is allowed if its bit in mask (64-bit words as
+ * needle_batch_set_step_mask takes them, [rows][ld_mask], or NULL) is set and its logit is
+ * above minus infinity; what other entries hold changes nothing.  A row without
+ * allowed entries, or with NaN or plus infinity among them, ends its request
+ * without a token.
+ * out_ids[i][0 ..] receives the taken drafts and the token behind them, out_len[i] their
+ * number, logprobs (may be NULL) log p of each (greedy: of temperature 1); both have rows of ld_out entries, at
+ * least a request's drafts + 1, and are filled up with 0xffffffff and 0.
+ * What the kernels find out of range (draft_start that falls or passes n_drafts, more drafts than ld_out - 1) gives
+ * that request no token and is reported by needle_verify_plan_status.
+ * A draft outside the vocabulary is not taken.
+ * dtype: f32, f16 or bf16 logits.  Calls on one plan share its workspace and must be ordered. */
+#define NEEDLE_VERIFY_LAST_TIE 1u
+typedef struct NeedleVerifyPlan NeedleVerifyPlan;
+NeedleVerifyPlan *needle_verify_plan_create(size_t vocab, size_t max_seqs, size_t max_drafts, int dtype, void *stream);
+int needle_verify_plan_run(NeedleVerifyPlan *plan, const void *logits, size_t ldl, const uint64_t *mask, size_t ld_mask,
+                           const int32_t *draft_start, const uint32_t *draft_ids, const float *draft_probs, size_t ldp,
+                           const float *temperature, const float *accept_u, const float *final_u, size_t n_seq,
+                           size_t n_drafts, uint32_t flags, uint32_t *out_ids, float *logprobs, size_t ld_out,
+                           uint32_t *out_len, void *stream);
+int needle_verify_plan_status(NeedleVerifyPlan *plan);
+void needle_verify_plan_free(NeedleVerifyPlan *plan);
+
 /* ── SafeTensors reader (crates/needle-infer/src/safetensors.rs:43-128) ── */
 /* The weight-file reader needle_load uses, on a host buffer: header JSON with
  * a string-valued __metadata__ object, dtypes F32 / BF16 / F16 / I8 and the

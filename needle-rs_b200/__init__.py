@@ -122,6 +122,17 @@ def lib():
             "needle_cross_attn_plan_run": (I, [P, P, S, S, P, S, S, P, S, S, P, C.c_float, P, S, S, P, P]),
             "needle_cross_attn_plan_status": (I, [P]),
             "needle_cross_attn_plan_free": (None, [P]),
+            "needle_kv4_page_bytes": (S, [S, S, S]),
+            "needle_kv4_plan_create": (P, [S, S, S, S, S, S, S, I, P]),
+            "needle_kv4_append": (I, [P, P, P, P, S, S, P, S, S, P]),
+            "needle_kv4_read": (I, [P, P, P, P, S, S, P, S, S, P]),
+            "needle_kv4_attn": (I, [P, P, P, P, S, S, C.c_float, U32, P, S, S, P, P]),
+            "needle_kv4_plan_status": (I, [P]),
+            "needle_kv4_plan_free": (None, [P]),
+            "needle_verify_plan_create": (P, [S, S, S, I, P]),
+            "needle_verify_plan_run": (I, [P, P, S, P, S, P, P, P, S, P, P, P, S, S, U32, P, P, S, P, P]),
+            "needle_verify_plan_status": (I, [P]),
+            "needle_verify_plan_free": (None, [P]),
             "needle_safetensors_parse": (P, [P, S]),
             "needle_safetensors_metadata": (C.c_char_p, [P, C.c_char_p]),
             "needle_safetensors_get_f32": (S, [P, C.c_char_p, P, S]),
@@ -577,6 +588,112 @@ class CrossAttnPlan:
     def close(self):
         if getattr(self, "_h", None):
             lib().needle_cross_attn_plan_free(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+# ── a decoder's cache in 4 bits, and the check of drafts ──
+KV4_CAUSAL = 1
+VERIFY_LAST_TIE = 1
+
+
+def kv4_page_bytes(num_kv_heads, head_dim, page_tokens):
+    """Bytes of a page of page_tokens tokens (a multiple of 16) in 4 bits."""
+    return lib().needle_kv4_page_bytes(num_kv_heads, head_dim, page_tokens)
+
+
+class Kv4Batch(C.Structure):
+    """The requests of a call (device pointers to int32): rows
+    [row_start[i], row_start[i + 1]) of `rows`, kv_len[i] cached tokens, pages
+    page_table[i][0 ..] of table_width entries."""
+    _fields_ = [("row_start", C.c_void_p), ("kv_len", C.c_void_p), ("page_table", C.c_void_p), ("n_seq", C.c_size_t),
+                ("rows", C.c_size_t), ("table_width", C.c_size_t)]
+
+    def __init__(self, row_start_ptr, kv_len_ptr, page_table_ptr, n_seq, rows, table_width):
+        super().__init__(row_start_ptr, kv_len_ptr, page_table_ptr, n_seq, rows, table_width)
+        self._ref = C.addressof(self)
+
+
+class Kv4Plan:
+    """A decoder's keys and values in 4 bits (needle_kv4_*), in n_pages pages of
+    page_tokens tokens that the caller holds, an array for each layer.
+    Strides are (row, head) in elements; by default [rows][heads][head_dim]."""
+
+    def __init__(self, num_heads, num_kv_heads, head_dim, page_tokens, n_pages, max_seqs, max_rows, dtype=BF16, stream=None):
+        self.num_heads, self.num_kv_heads, self.head_dim = num_heads, num_kv_heads, head_dim
+        self._qs = (num_heads * head_dim, head_dim)
+        self._ks = (num_kv_heads * head_dim, head_dim)
+        self._h = lib().needle_kv4_plan_create(num_heads, num_kv_heads, head_dim, page_tokens, n_pages, max_seqs, max_rows,
+                                               dtype, stream)
+        if not self._h:
+            raise NeedleError(last_error() or "needle_kv4_plan_create failed")
+
+    def append(self, pages_ptr, batch, k_ptr, v_ptr, k_strides=None, v_strides=None, stream=None):
+        """Writes a request's rows as its last tokens (kv_len counts them already)."""
+        kr, kh = k_strides or self._ks
+        vr, vh = v_strides or self._ks
+        _check(_lib.needle_kv4_append(self._h, pages_ptr, batch._ref, k_ptr, kr, kh, v_ptr, vr, vh, stream))
+
+    def read(self, pages_ptr, batch, k_ptr, v_ptr, k_strides=None, v_strides=None, stream=None):
+        """The values of a request's last tokens, as many as it has rows."""
+        kr, kh = k_strides or self._ks
+        vr, vh = v_strides or self._ks
+        _check(_lib.needle_kv4_read(self._h, pages_ptr, batch._ref, k_ptr, kr, kh, v_ptr, vr, vh, stream))
+
+    def attn(self, pages_ptr, batch, q_ptr, out_ptr, scale, causal=True, q_strides=None, out_strides=None, lse_ptr=None,
+             stream=None):
+        """Attention of a request's rows to its cache; causal: they are its last tokens."""
+        qr, qh = q_strides or self._qs
+        orow, oh = out_strides or self._qs
+        _check(_lib.needle_kv4_attn(self._h, pages_ptr, batch._ref, q_ptr, qr, qh, scale, KV4_CAUSAL if causal else 0, out_ptr,
+                                    orow, oh, lse_ptr, stream))
+
+    def status(self):
+        _check(lib().needle_kv4_plan_status(self._h))
+
+    def close(self):
+        if getattr(self, "_h", None):
+            lib().needle_kv4_plan_free(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class VerifyPlan:
+    """Drafted tokens against the target's logits (needle_verify_plan_*), with
+    random numbers that the caller gives."""
+
+    def __init__(self, vocab, max_seqs, max_drafts, dtype=F32, stream=None):
+        self.vocab = vocab
+        self._h = lib().needle_verify_plan_create(vocab, max_seqs, max_drafts, dtype, stream)
+        if not self._h:
+            raise NeedleError(last_error() or "needle_verify_plan_create failed")
+
+    def run(self, logits_ptr, draft_start_ptr, draft_ids_ptr, accept_u_ptr, final_u_ptr, out_ids_ptr, out_len_ptr, n_seq,
+            n_drafts, ld_out, draft_probs_ptr=None, temperature_ptr=None, mask_ptr=None, logprobs_ptr=None, ldl=None, ldp=None,
+            ld_mask=None, flags=0, stream=None):
+        """Row strides default to the vocabulary, that of the mask to its 64-bit words."""
+        V = self.vocab
+        _check(_lib.needle_verify_plan_run(self._h, logits_ptr, V if ldl is None else ldl, mask_ptr,
+                                           (V + 63) // 64 if ld_mask is None else ld_mask, draft_start_ptr, draft_ids_ptr,
+                                           draft_probs_ptr, V if ldp is None else ldp, temperature_ptr, accept_u_ptr, final_u_ptr,
+                                           n_seq, n_drafts, flags, out_ids_ptr, logprobs_ptr, ld_out, out_len_ptr, stream))
+
+    def status(self):
+        _check(lib().needle_verify_plan_status(self._h))
+
+    def close(self):
+        if getattr(self, "_h", None):
+            lib().needle_verify_plan_free(self._h)
             self._h = None
 
     def __del__(self):

@@ -1,0 +1,89 @@
+// kv4.cuh — the cache of keys and values in 4 bits: its layout, and the
+// requests of a call.
+//
+// A page holds page_tokens tokens of one request, for each KV head one after
+// another in tiles of 16 tokens.  A tile is 640 bytes for each group of 32
+// dimensions (NG groups: head_dim rounded up):
+//   K codes  [NG][32][2] words    V codes [NG][32][2] words
+//   K (scale, minimum) [16][NG] pairs of f16
+//   V scales, minima   [NG][2][16] f16
+// The order inside is that of the operands of a 16 x 8 x 16 matrix
+// instruction, so that a lane fetches what it multiplies in 8 bytes and needs no
+// shuffle, and a token's codes share no byte with another's:
+//   K as its rows (16 tokens) by dimensions: lane 4 r + q has tokens m = r and
+//   m = r + 8, words of 8 dimensions 32 g + 8 q .., where token t is row
+//   m = 2 (t / 4) + t % 2 + 8 (t / 2 % 2) and dimension d of a word sits in
+//   nibble d / 2 + 4 (d % 2): a mask leaves a pair of neighbours in the
+//   halves of a word.
+//   V transposed (dimensions by 16 tokens): lane 4 r + q has dimensions
+//   32 g + 4 r .. + 3 of tokens 4 q, 4 q + 1 (low and high half of word 0)
+//   and 4 q + 2, 4 q + 3 (word 1), a nibble each.
+#pragma once
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "ops.h"
+
+namespace ndl {
+namespace kv4 {
+
+constexpr int kTokens = 16, kGroup = 32;
+constexpr float kLargest = 32768.0f;  // magnitudes above it do not fit: 15 steps of f16 from there may pass f16's range
+
+__host__ __device__ constexpr int tile_bytes(int ng) { return 640 * ng; }
+// Offsets inside a tile.
+__host__ __device__ constexpr int v_codes(int ng) { return 256 * ng; }
+__host__ __device__ constexpr int k_params(int ng) { return 512 * ng; }
+__host__ __device__ constexpr int v_params(int ng) { return 576 * ng; }
+
+__host__ __device__ __forceinline__ int row_of(int t) { return 2 * (t >> 2) + (t & 1) + 8 * ((t >> 1) & 1); }
+// Word (4 bytes) of dimensions 32 g + 8 q .. of token t's key.
+__host__ __device__ __forceinline__ int k_word(int t, int g, int q) {
+  const int m = row_of(t);
+  return ((g * 32 + (m & 7) * 4 + q) * 2 + (m >> 3)) * 4;
+}
+// Half word (2 bytes) of dimensions 32 g + 4 r .. of token t's value.
+__host__ __device__ __forceinline__ int v_half(int ng, int t, int g, int r) {
+  return v_codes(ng) + ((g * 32 + r * 4 + (t >> 2)) * 2 + ((t >> 1) & 1)) * 4 + (t & 1) * 2;
+}
+__host__ __device__ __forceinline__ int k_param(int ng, int t, int g) { return k_params(ng) + (row_of(t) * ng + g) * 4; }
+__host__ __device__ __forceinline__ int v_param(int ng, int t, int g, int which) {
+  return v_params(ng) + ((g * 2 + which) * 16 + t) * 2;
+}
+
+// A request of a call.
+struct Seq {
+  int row0, n, len;  // its rows of the operands, tokens in its cache
+};
+
+// Request i; one whose numbers do not fit the operands has no rows and no
+// tokens, and the plan's flag says so.  `inside`: its rows are its last tokens.
+__host__ __device__ __forceinline__ Seq sequence(const Kv4Rows &b, const Kv4Shape &s, int i, bool inside, int *bad) {
+  const int a = b.row_start[i], e = b.row_start[i + 1], len = b.kv_len[i];
+  const bool ok = a >= 0 && a <= e && e <= b.rows && len >= 0 && len <= (int64_t)b.width * s.page_tokens &&
+                  !(inside && e - a > len);
+  if (!ok) *bad = 1;
+  return ok ? Seq{a, e - a, len} : Seq{0, 0, 0};
+}
+
+// The first block looks at every request, those without rows as well.
+__device__ __forceinline__ void check_all(const Kv4Rows &b, const Kv4Shape &s, bool inside, int *bad) {
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < b.n_seq; i += blockDim.x) sequence(b, s, i, inside, bad);
+}
+
+// Tile `t` (of 16 tokens) of request i's cache for a KV head; NULL (flag set)
+// where the table names a page that is not there.
+__host__ __device__ __forceinline__ uint8_t *tile_at(uint8_t *pages, const Kv4Rows &b, const Kv4Shape &s, int i, int64_t t, int kvh,
+                                            int *bad) {
+  const int per = s.page_tokens / kTokens, in = (int)(t % per);
+  const int page = b.table[(int64_t)i * b.width + t / per];
+  if (page < 0 || page >= s.n_pages) {
+    *bad = 1;
+    return nullptr;
+  }
+  return pages + (int64_t)page * s.page_bytes + ((int64_t)kvh * per + in) * tile_bytes(s.ng);
+}
+
+}  // namespace kv4
+}  // namespace ndl

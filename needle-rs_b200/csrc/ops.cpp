@@ -1,5 +1,6 @@
 // ops.cpp — entry points of the serving operators: the 8-bit product, the
-// residual norm and cross attention (declared in needle_b200.h).
+// residual norm, cross attention, the 4-bit cache with its attention, and the
+// verification of drafts (declared in needle_b200.h).
 //
 // No counterpart in the reference.  Every argument is checked before the
 // first CUDA call, and no C++ exception leaves an entry point.
@@ -88,6 +89,7 @@ bool natural(const void *p, int t) { return aligned(p, dtype_size(t)); }
 
 constexpr size_t kMaxRows = 0x7fffff00;  // whole tiles of 256 rows still count in 31 bits
 constexpr int64_t kMaxItems = 1 << 26;    // of a cross attention plan: 3 GB
+constexpr size_t kMaxSeqs = 1 << 20;      // requests of a call to the 4-bit cache or the verification
 constexpr size_t kMaxStride = (size_t)1 << 36;  // elements
 
 // Runs f, turning a C++ exception into an error.
@@ -106,14 +108,16 @@ bool guarded(F f) {
 }
 
 // Reads and clears a plan's flag of expired waits; synchronises the device.
-bool check_flag(int device, int *flag, const char *what) {
+// `numbers`: a second flag follows it, of numbers in device memory that did not fit.
+bool check_flag(int device, int *flag, const char *what, const char *numbers = nullptr) {
   OnDevice on(device);
-  int e = 0;
-  if (!on.good() || !ok(cudaDeviceSynchronize()) || !ok(cudaMemcpy(&e, flag, sizeof e, cudaMemcpyDeviceToHost)))
+  int e[2] = {0, 0};
+  if (!on.good() || !ok(cudaDeviceSynchronize()) ||
+      !ok(cudaMemcpy(e, flag, numbers ? sizeof e : sizeof e[0], cudaMemcpyDeviceToHost)))
     return false;
-  if (!e) return true;
-  cudaMemset(flag, 0, sizeof e);
-  return fail(std::string(what) + ": a wait inside a launch timed out");
+  if (!e[0] && !e[1]) return true;
+  cudaMemset(flag, 0, numbers ? sizeof e : sizeof e[0]);
+  return fail(std::string(what) + ": " + (e[0] ? "a wait inside a launch timed out" : numbers));
 }
 
 void free_buffer(int device, void *buf) {
@@ -144,12 +148,62 @@ struct NeedleCrossAttnPlan {
   int *flag = nullptr;
 };
 
+struct NeedleKv4Plan {
+  int device = 0;
+  Kv4Shape s;
+  size_t max_seqs = 0, max_rows = 0;
+  void *buf = nullptr;
+  Kv4Work work;
+};
+
+struct NeedleVerifyPlan {
+  int device = 0;
+  VerifyShape s;
+  size_t max_seqs = 0, max_drafts = 0;
+  void *buf = nullptr;
+  VerifyWork work;
+};
+
 namespace {
 
 bool int8_product(NeedleInt8Plan *p, const int8_t *q, const float *qs, size_t M, const float *bias, void *y, int y_dtype,
                   size_t ldy, bool pdl, cudaStream_t st) {
   Int8Args a{q, &p->w_map, qs, p->w_scales, bias, y, (int64_t)ldy, (int)M, p->N, p->K, y_dtype};
   return ok(int8_matmul(a, pdl, p->flag, st));
+}
+
+// The checks that the calls on a 4-bit cache share.
+bool kv4_batch(const NeedleKv4Plan *p, const void *pages, const NeedleKv4Batch *b, Kv4Rows *rows) {
+  if (!p || !pages || !b || !b->row_start || !b->kv_len || !b->page_table || b->n_seq == 0 || b->n_seq > p->max_seqs ||
+      b->rows > p->max_rows || b->table_width == 0 || b->table_width > kMaxRows || !aligned(pages, 128) ||
+      !aligned(b->row_start, 4) || !aligned(b->kv_len, 4) || !aligned(b->page_table, 4))
+    return fail("invalid 4-bit cache arguments");
+  *rows = Kv4Rows{b->row_start, b->kv_len, b->page_table, (int)b->n_seq, (int)b->table_width, (int64_t)b->rows};
+  return true;
+}
+
+bool kv4_on_device(const NeedleKv4Plan *p, const void *pages, const NeedleKv4Batch *b) {
+  return all_on(p->device, {{"pages", pages}, {"row_start", b->row_start}, {"kv_len", b->kv_len}, {"page_table", b->page_table}});
+}
+
+struct Heads {
+  const void *p;
+  size_t row, head;
+};
+bool kv4_operands(const NeedleKv4Plan *p, std::initializer_list<Heads> operands) {
+  for (const Heads &o : operands) {
+    if (!aligned(o.p, 16)) return fail("4-bit cache: operands must start on 16-byte boundaries");
+    for (size_t s : {o.row, o.head})
+      if (s < (size_t)p->s.D || s % 8 || s > kMaxStride)
+        return fail("4-bit cache: strides must be multiples of 8 elements and at least head_dim");
+  }
+  return true;
+}
+
+// Whether the elements of `rows` rows of `heads` heads are different ones.
+bool apart(const NeedleKv4Plan *p, size_t rows, size_t row, size_t head, int heads) {
+  const size_t D = (size_t)p->s.D;
+  return rows == 0 || row >= (size_t)(heads - 1) * head + D || head >= (rows - 1) * row + D;
 }
 
 }  // namespace
@@ -418,6 +472,159 @@ int needle_cross_attn_plan_status(NeedleCrossAttnPlan *p) {
 }
 
 void needle_cross_attn_plan_free(NeedleCrossAttnPlan *p) {
+  if (!p) return;
+  if (p->buf) free_buffer(p->device, p->buf);
+  delete p;
+}
+
+size_t needle_kv4_page_bytes(size_t KVH, size_t D, size_t page_tokens) {
+  return KVH * (page_tokens / 16) * ((D + 31) / 32 * 640);
+}
+
+NeedleKv4Plan *needle_kv4_plan_create(size_t H, size_t KVH, size_t D, size_t page_tokens, size_t n_pages, size_t max_seqs,
+                                      size_t max_rows, int dtype, void *stream) {
+  NeedleKv4Plan *plan = nullptr;
+  const bool good = guarded([&] {
+    if (dtype != NEEDLE_F16 && dtype != NEEDLE_BF16) return fail("4-bit cache takes f16 or bf16");
+    if (D == 0 || D > 128 || D % 8) return fail("4-bit cache: head_dim must be a multiple of 8 up to 128");
+    if (KVH == 0 || H == 0 || H % KVH || H > 4096)
+      return fail("4-bit cache: num_heads must be a multiple of num_kv_heads, up to 4096");
+    if (page_tokens == 0 || page_tokens % 16 || page_tokens > 65536)
+      return fail("4-bit cache: page_tokens must be a multiple of 16 up to 65536");
+    if (n_pages == 0 || n_pages > kMaxRows || max_seqs == 0 || max_seqs > kMaxSeqs || max_rows == 0 || max_rows > kMaxRows ||
+        max_rows * (H / KVH) > kMaxRows)
+      return fail("4-bit cache: invalid number of pages, sequences or rows");
+    plan = new NeedleKv4Plan();
+    plan->s = Kv4Shape{(int)H, (int)KVH, (int)D, (int)((D + 31) / 32), (int)page_tokens, dtype, (int64_t)n_pages,
+                       (int64_t)needle_kv4_page_bytes(KVH, D, page_tokens)};
+    plan->max_seqs = max_seqs;
+    plan->max_rows = max_rows;
+    if (!ok(cudaGetDevice(&plan->device)) || !ok(cudaMalloc(&plan->buf, 256))) return false;
+    plan->work.err = (int *)plan->buf;
+    plan->work.bad = plan->work.err + 1;
+    cudaStream_t st = (cudaStream_t)stream;
+    return ok(cudaMemsetAsync(plan->buf, 0, 256, st)) && ok(cudaStreamSynchronize(st));
+  });
+  if (good) return plan;
+  needle_kv4_plan_free(plan);
+  return nullptr;
+}
+
+int needle_kv4_append(NeedleKv4Plan *p, void *pages, const NeedleKv4Batch *b, const void *k, size_t k_row, size_t k_head,
+                      const void *v, size_t v_row, size_t v_head, void *stream) {
+  return guarded([&] {
+    Kv4Rows rows;
+    if (!kv4_batch(p, pages, b, &rows) || !kv4_operands(p, {{k, k_row, k_head}, {v, v_row, v_head}})) return false;
+    if (b->rows && (!k || !v)) return fail("invalid 4-bit cache arguments");
+    OnDevice on(p->device);
+    if (!on.good() || !kv4_on_device(p, pages, b) || !all_on(p->device, {{"k", k}, {"v", v}})) return false;
+    Kv4Call c{(uint8_t *)pages, k, v, nullptr, nullptr, (int64_t)k_row, (int64_t)k_head, (int64_t)v_row, (int64_t)v_head};
+    return ok(kv4_append(p->s, rows, c, p->work.bad, (cudaStream_t)stream));
+  }) ? 0 : -1;
+}
+
+int needle_kv4_read(NeedleKv4Plan *p, const void *pages, const NeedleKv4Batch *b, void *k, size_t k_row, size_t k_head,
+                    void *v, size_t v_row, size_t v_head, void *stream) {
+  return guarded([&] {
+    Kv4Rows rows;
+    if (!kv4_batch(p, pages, b, &rows) || !kv4_operands(p, {{k, k_row, k_head}, {v, v_row, v_head}})) return false;
+    if (b->rows && !k && !v) return fail("invalid 4-bit cache arguments");
+    if ((k && !apart(p, b->rows, k_row, k_head, p->s.KVH)) || (v && !apart(p, b->rows, v_row, v_head, p->s.KVH)))
+      return fail("4-bit cache: rows and heads of an output overlap");
+    OnDevice on(p->device);
+    if (!on.good() || !kv4_on_device(p, pages, b) || !all_on(p->device, {{"k_out", k}, {"v_out", v}})) return false;
+    Kv4Call c{(uint8_t *)pages, nullptr, nullptr, k, v, (int64_t)k_row, (int64_t)k_head, (int64_t)v_row, (int64_t)v_head};
+    return ok(kv4_read(p->s, rows, c, p->work.bad, (cudaStream_t)stream));
+  }) ? 0 : -1;
+}
+
+int needle_kv4_attn(NeedleKv4Plan *p, const void *pages, const NeedleKv4Batch *b, const void *q, size_t q_row, size_t q_head,
+                    float scale, uint32_t flags, void *out, size_t o_row, size_t o_head, float *lse, void *stream) {
+  return guarded([&] {
+    Kv4Rows rows;
+    if (!kv4_batch(p, pages, b, &rows) || !kv4_operands(p, {{q, q_row, q_head}, {out, o_row, o_head}})) return false;
+    if ((b->rows && (!q || !out)) || !aligned(lse, 4) || (flags & ~NEEDLE_KV4_CAUSAL)) return fail("invalid 4-bit cache arguments");
+    if (!(scale > 0.0f) || std::isinf(scale)) return fail("4-bit cache: scale must be positive and finite");
+    if (!apart(p, b->rows, o_row, o_head, p->s.H)) return fail("4-bit cache: rows and heads of an output overlap");
+    OnDevice on(p->device);
+    if (!on.good() || !kv4_on_device(p, pages, b) || !all_on(p->device, {{"q", q}, {"out", out}, {"lse", lse}})) return false;
+    Kv4AttnCall c{(const uint8_t *)pages, q, out, lse, (int64_t)q_row, (int64_t)q_head, (int64_t)o_row, (int64_t)o_head, scale,
+                  (flags & NEEDLE_KV4_CAUSAL) != 0};
+    return ok(kv4_attn(p->s, rows, c, p->work, (cudaStream_t)stream));
+  }) ? 0 : -1;
+}
+
+int needle_kv4_plan_status(NeedleKv4Plan *p) {
+  return guarded([&] {
+    return p ? check_flag(p->device, p->work.err, "4-bit cache",
+                          "a row start, a length or a page index of a batch was out of range")
+             : fail("null plan");
+  }) ? 0 : -1;
+}
+
+void needle_kv4_plan_free(NeedleKv4Plan *p) {
+  if (!p) return;
+  if (p->buf) free_buffer(p->device, p->buf);
+  delete p;
+}
+
+NeedleVerifyPlan *needle_verify_plan_create(size_t vocab, size_t max_seqs, size_t max_drafts, int dtype, void *stream) {
+  NeedleVerifyPlan *plan = nullptr;
+  const bool good = guarded([&] {
+    if (!float_type(dtype)) return fail("verification takes f32, f16 or bf16 logits");
+    if (vocab == 0 || vocab > (1u << 24) || max_seqs == 0 || max_seqs > kMaxSeqs || max_drafts > kMaxRows - kMaxSeqs)
+      return fail("invalid verification plan arguments");
+    plan = new NeedleVerifyPlan();
+    plan->s = VerifyShape{(int)vocab, dtype};
+    plan->max_seqs = max_seqs;
+    plan->max_drafts = max_drafts;
+    if (!ok(cudaGetDevice(&plan->device)) || !ok(cudaMalloc(&plan->buf, 256))) return false;
+    plan->work.bad = (int *)plan->buf + 1;
+    cudaStream_t st = (cudaStream_t)stream;
+    return ok(cudaMemsetAsync(plan->buf, 0, 256, st)) && ok(cudaStreamSynchronize(st));
+  });
+  if (good) return plan;
+  needle_verify_plan_free(plan);
+  return nullptr;
+}
+
+int needle_verify_plan_run(NeedleVerifyPlan *p, const void *logits, size_t ldl, const uint64_t *mask, size_t ld_mask,
+                           const int32_t *draft_start, const uint32_t *draft_ids, const float *draft_probs, size_t ldp,
+                           const float *temperature, const float *accept_u, const float *final_u, size_t n_seq,
+                           size_t n_drafts, uint32_t flags, uint32_t *out_ids, float *logprobs, size_t ld_out,
+                           uint32_t *out_len, void *stream) {
+  return guarded([&] {
+    if (!p || !logits || !draft_start || !final_u || !out_ids || !out_len || n_seq == 0 || n_seq > p->max_seqs ||
+        n_drafts > p->max_drafts || (n_drafts && (!draft_ids || !accept_u)) || ld_out == 0 || ld_out > kMaxRows ||
+        (flags & ~NEEDLE_VERIFY_LAST_TIE) || !natural(logits, p->s.dtype) || !aligned(mask, 8))
+      return fail("invalid verification arguments");
+    for (const void *o : {(const void *)draft_start, (const void *)draft_ids, (const void *)draft_probs,
+                          (const void *)temperature, (const void *)accept_u, (const void *)final_u, (const void *)out_ids,
+                          (const void *)logprobs, (const void *)out_len})
+      if (!aligned(o, 4)) return fail("invalid verification arguments");
+    const size_t V = (size_t)p->s.V;
+    if (ldl < V || ldl > kMaxStride || (mask && (ld_mask < (V + 63) / 64 || ld_mask > kMaxStride)) ||
+        (draft_probs && (ldp < V || ldp > kMaxStride)))
+      return fail("verification: a row stride is below the vocabulary");
+    OnDevice on(p->device);
+    if (!on.good() ||
+        !all_on(p->device, {{"logits", logits}, {"mask", mask}, {"draft_start", draft_start}, {"draft_ids", draft_ids},
+                            {"draft_probs", draft_probs}, {"temperature", temperature}, {"accept_u", accept_u},
+                            {"final_u", final_u}, {"out_ids", out_ids}, {"logprobs", logprobs}, {"out_len", out_len}}))
+      return false;
+    VerifyCall c{logits, mask, draft_start, draft_ids, draft_probs, temperature, accept_u, final_u, out_ids, out_len,
+                 logprobs, (int64_t)ldl, (int64_t)ld_mask, (int64_t)ldp, (int64_t)ld_out, (int)n_seq, (int)n_drafts, flags};
+    return ok(verify_drafts(p->s, c, p->work, (cudaStream_t)stream));
+  }) ? 0 : -1;
+}
+
+int needle_verify_plan_status(NeedleVerifyPlan *p) {
+  return guarded([&] {
+    return p ? check_flag(p->device, p->work.bad - 1, "verification", "a request's drafts were out of range") : fail("null plan");
+  }) ? 0 : -1;
+}
+
+void needle_verify_plan_free(NeedleVerifyPlan *p) {
   if (!p) return;
   if (p->buf) free_buffer(p->device, p->buf);
   delete p;

@@ -1,5 +1,6 @@
 // ops.h — launchers of the serving operators (int8_matmul.cu,
-// residual_norm.cu, cross_attn.cu) behind the entry points in ops.cpp.
+// residual_norm.cu, cross_attn.cu, kv4_cache.cu, kv4_attn.cu, verify.cu)
+// behind the entry points in ops.cpp.
 //
 // All pointers are device pointers unless a name says host.  Launchers enqueue
 // on `st` and return the launch status.
@@ -110,5 +111,61 @@ struct XAttnWork {
   int n_few = 0, n_tile = 0, n_groups = 0, group_rows = 0;
 };
 cudaError_t cross_attn(const XAttnWork &w, const XAttnCall &c, int *err, cudaStream_t st);
+
+// ── cache of keys and values in 4 bits (its layout: kv4.cuh) ──
+struct Kv4Shape {
+  int H, KVH, D, ng, page_tokens, dtype;
+  int64_t n_pages, page_bytes;
+};
+// The requests of a call (device arrays).  Kernels check every number in
+// them; what does not fit sets the plan's `bad` flag and is left out.
+struct Kv4Rows {
+  const int32_t *row_start, *kv_len, *table;
+  int n_seq, width;
+  int64_t rows;
+};
+struct Kv4Call {
+  uint8_t *pages;
+  const void *k, *v;    // append
+  void *k_out, *v_out;  // read
+  int64_t k_row, k_head, v_row, v_head;
+};
+cudaError_t kv4_append(const Kv4Shape &s, const Kv4Rows &b, const Kv4Call &c, int *bad, cudaStream_t st);
+cudaError_t kv4_read(const Kv4Shape &s, const Kv4Rows &b, const Kv4Call &c, int *bad, cudaStream_t st);
+
+struct Kv4AttnCall {
+  const uint8_t *pages;
+  const void *q;
+  void *out;
+  float *lse;
+  int64_t q_row, q_head, o_row, o_head;
+  float scale;
+  bool causal;
+};
+struct Kv4Work {
+  int *err, *bad;  // a wait that ran out; a request that does not fit
+};
+cudaError_t kv4_attn(const Kv4Shape &s, const Kv4Rows &b, const Kv4AttnCall &c, const Kv4Work &w, cudaStream_t st);
+
+// ── verification of drafts ──
+struct VerifyShape {
+  int V, dtype;
+};
+struct VerifyCall {
+  const void *logits;
+  const uint64_t *mask;
+  const int32_t *start;
+  const uint32_t *ids;
+  const float *probs, *temperature, *accept_u, *final_u;
+  uint32_t *out_ids, *out_len;
+  float *logprobs;
+  int64_t ldl, ld_mask, ldp, ld_out;
+  int n_seq, n_drafts;
+  uint32_t flags;
+};
+struct VerifyWork {
+  int *bad;
+};
+cudaError_t verify_drafts(const VerifyShape &s, const VerifyCall &c, const VerifyWork &w, cudaStream_t st);
 
 }  // namespace ndl
