@@ -188,14 +188,14 @@ def prepare_kv(case, g, seed):
         s["plan"] = n.Kv4Plan(H, KVH, D, page, n_pages, B, max(sum(new), 1), code(t))
         s["pages"] = torch.empty(n_pages * n.kv4_page_bytes(KVH, D, page), dtype=torch.uint8, device="cuda")
         s["held"] = [table, i32(starts(new)), i32(total), i32(starts(total))]
-        s["batch"] = n.Kv4Batch(s["held"][1].data_ptr(), s["held"][2].data_ptr(), table.data_ptr(), B, sum(new), width)
+        s["batch"] = n.Kv4Batch(s["held"][1].data_ptr(), s["held"][2].data_ptr(), table.data_ptr(), B, sum(new), width, max(new))
         if case["op"] == "attn":
             s["out"] = torch.empty_like(s["q"])
             s["lse"] = torch.empty((sum(new), H), device="cuda") if case["lse"] else None
         else:
             s["out"] = [torch.empty((sum(new), KVH, D), dtype=TYPES[t], device="cuda") for _ in range(2)]
         if case["op"] != "store":
-            whole = n.Kv4Batch(s["held"][3].data_ptr(), s["held"][2].data_ptr(), table.data_ptr(), B, sum(total), width)
+            whole = n.Kv4Batch(s["held"][3].data_ptr(), s["held"][2].data_ptr(), table.data_ptr(), B, sum(total), width, max(total))
             s["plan"].append(s["pages"].data_ptr(), whole, k.data_ptr(), v.data_ptr(), k.stride()[:2], v.stride()[:2])
             torch.cuda.synchronize()
     elif case["op"] != "store":
