@@ -432,8 +432,8 @@ void needle_cross_attn_plan_free(NeedleCrossAttnPlan *plan);
  * request are left alone), kv_len[i] tokens in its cache, and its token t is
  * in page page_table[i * table_width + t / page_tokens].  A request may have no rows and no
  * tokens.  Entries of the table behind a request's tokens are not read.  Kernels
- * check the numbers: row starts that fall or pass `rows`, lengths below zero or past
- * table_width pages, and pages outside the array are found by
+ * check the numbers: row starts that fall or pass `rows`, more rows than max_new, lengths below zero, past
+ * table_width pages or 2^30, and pages outside the array are found by
  * needle_kv4_plan_status.  Such a request's results are undefined then (where
  * row starts fall, those of all), and nothing outside the operands and the
  * pages is touched. */
@@ -443,6 +443,7 @@ typedef struct NeedleKv4Batch {
   const int32_t *kv_len;     /* [n_seq] */
   const int32_t *page_table; /* [n_seq][table_width] */
   size_t n_seq, rows, table_width;
+  size_t max_new; /* no request has more rows: `rows` where nothing better is known */
 } NeedleKv4Batch;
 size_t needle_kv4_page_bytes(size_t num_kv_heads, size_t head_dim, size_t page_tokens);
 NeedleKv4Plan *needle_kv4_plan_create(size_t num_heads, size_t num_kv_heads, size_t head_dim, size_t page_tokens,

@@ -610,12 +610,12 @@ def kv4_page_bytes(num_kv_heads, head_dim, page_tokens):
 class Kv4Batch(C.Structure):
     """The requests of a call (device pointers to int32): rows
     [row_start[i], row_start[i + 1]) of `rows`, kv_len[i] cached tokens, pages
-    page_table[i][0 ..] of table_width entries."""
+    page_table[i][0 ..] of table_width entries; max_new bounds a request's rows."""
     _fields_ = [("row_start", C.c_void_p), ("kv_len", C.c_void_p), ("page_table", C.c_void_p), ("n_seq", C.c_size_t),
-                ("rows", C.c_size_t), ("table_width", C.c_size_t)]
+                ("rows", C.c_size_t), ("table_width", C.c_size_t), ("max_new", C.c_size_t)]
 
-    def __init__(self, row_start_ptr, kv_len_ptr, page_table_ptr, n_seq, rows, table_width):
-        super().__init__(row_start_ptr, kv_len_ptr, page_table_ptr, n_seq, rows, table_width)
+    def __init__(self, row_start_ptr, kv_len_ptr, page_table_ptr, n_seq, rows, table_width, max_new=None):
+        super().__init__(row_start_ptr, kv_len_ptr, page_table_ptr, n_seq, rows, table_width, rows if max_new is None else max_new)
         self._ref = C.addressof(self)
 
 

@@ -6,7 +6,7 @@
 // dimensions (NG groups: head_dim rounded up):
 //   K codes  [NG][32][2] words    V codes [NG][32][2] words
 //   K (scale, minimum) [16][NG] pairs of f16
-//   V scales, minima   [NG][2][16] f16
+//   V scales and minima  [NG][4 tokens' quads][2][4] f16
 // The order inside is that of the operands of a 16 x 8 x 16 matrix
 // instruction, so that a lane fetches what it multiplies in 8 bytes and needs no
 // shuffle, and a token's codes share no byte with another's:
@@ -28,6 +28,7 @@ namespace ndl {
 namespace kv4 {
 
 constexpr int kTokens = 16, kGroup = 32;
+constexpr int kMaxTokens = 1 << 30;  // of a request
 constexpr float kLargest = 32768.0f;  // magnitudes above it do not fit: 15 steps of f16 from there may pass f16's range
 
 __host__ __device__ constexpr int tile_bytes(int ng) { return 640 * ng; }
@@ -48,7 +49,7 @@ __host__ __device__ __forceinline__ int v_half(int ng, int t, int g, int r) {
 }
 __host__ __device__ __forceinline__ int k_param(int ng, int t, int g) { return k_params(ng) + (row_of(t) * ng + g) * 4; }
 __host__ __device__ __forceinline__ int v_param(int ng, int t, int g, int which) {
-  return v_params(ng) + ((g * 2 + which) * 16 + t) * 2;
+  return v_params(ng) + (((g * 4 + (t >> 2)) * 2 + which) * 4 + (t & 3)) * 2;
 }
 
 // A request of a call.
@@ -60,7 +61,7 @@ struct Seq {
 // tokens, and the plan's flag says so.  `inside`: its rows are its last tokens.
 __host__ __device__ __forceinline__ Seq sequence(const Kv4Rows &b, const Kv4Shape &s, int i, bool inside, int *bad) {
   const int a = b.row_start[i], e = b.row_start[i + 1], len = b.kv_len[i];
-  const bool ok = a >= 0 && a <= e && e <= b.rows && len >= 0 && len <= (int64_t)b.width * s.page_tokens &&
+  const bool ok = a >= 0 && a <= e && e <= b.rows && e - a <= b.max_new && len >= 0 && len <= kMaxTokens && len <= (int64_t)b.width * s.page_tokens &&
                   !(inside && e - a > len);
   if (!ok) *bad = 1;
   return ok ? Seq{a, e - a, len} : Seq{0, 0, 0};
@@ -72,17 +73,24 @@ __device__ __forceinline__ void check_all(const Kv4Rows &b, const Kv4Shape &s, b
     for (int i = threadIdx.x; i < b.n_seq; i += blockDim.x) sequence(b, s, i, inside, bad);
 }
 
-// Tile `t` (of 16 tokens) of request i's cache for a KV head; NULL (flag set)
-// where the table names a page that is not there.
-__host__ __device__ __forceinline__ uint8_t *tile_at(uint8_t *pages, const Kv4Rows &b, const Kv4Shape &s, int i, int64_t t, int kvh,
-                                            int *bad) {
-  const int per = s.page_tokens / kTokens, in = (int)(t % per);
+// Where tile `t` (of 16 tokens) of request i's cache for a KV head begins, in
+// units of 128 bytes; kNoPlace (flag set) where the table names a page that is
+// not there.
+constexpr uint32_t kNoPlace = 0xffffffffu;
+__host__ __device__ __forceinline__ uint32_t place_of(const Kv4Rows &b, const Kv4Shape &s, int i, int t, int kvh, int *bad) {
+  const int per = s.page_tokens / kTokens, in = t % per;
   const int page = b.table[(int64_t)i * b.width + t / per];
   if (page < 0 || page >= s.n_pages) {
     *bad = 1;
-    return nullptr;
+    return kNoPlace;
   }
-  return pages + (int64_t)page * s.page_bytes + ((int64_t)kvh * per + in) * tile_bytes(s.ng);
+  return (uint32_t)(((int64_t)page * s.page_bytes + ((int64_t)kvh * per + in) * tile_bytes(s.ng)) >> 7);
+}
+// The same as an address, or NULL.
+__host__ __device__ __forceinline__ uint8_t *tile_at(uint8_t *pages, const Kv4Rows &b, const Kv4Shape &s, int i, int t, int kvh,
+                                                     int *bad) {
+  const uint32_t p = place_of(b, s, i, t, kvh, bad);
+  return p == kNoPlace ? nullptr : pages + (int64_t)p * 128;
 }
 
 }  // namespace kv4

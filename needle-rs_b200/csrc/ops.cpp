@@ -175,10 +175,11 @@ bool int8_product(NeedleInt8Plan *p, const int8_t *q, const float *qs, size_t M,
 // The checks that the calls on a 4-bit cache share.
 bool kv4_batch(const NeedleKv4Plan *p, const void *pages, const NeedleKv4Batch *b, Kv4Rows *rows) {
   if (!p || !pages || !b || !b->row_start || !b->kv_len || !b->page_table || b->n_seq == 0 || b->n_seq > p->max_seqs ||
-      b->rows > p->max_rows || b->table_width == 0 || b->table_width > kMaxRows || !aligned(pages, 128) ||
+      b->rows > p->max_rows || b->max_new > b->rows || b->table_width == 0 || b->table_width > kMaxRows || !aligned(pages, 128) ||
       !aligned(b->row_start, 4) || !aligned(b->kv_len, 4) || !aligned(b->page_table, 4))
     return fail("invalid 4-bit cache arguments");
-  *rows = Kv4Rows{b->row_start, b->kv_len, b->page_table, (int)b->n_seq, (int)b->table_width, (int64_t)b->rows};
+  *rows = Kv4Rows{b->row_start, b->kv_len, b->page_table, (int)b->n_seq, (int)b->table_width, (int64_t)b->rows,
+                  (int)b->max_new};
   return true;
 }
 
@@ -494,16 +495,26 @@ NeedleKv4Plan *needle_kv4_plan_create(size_t H, size_t KVH, size_t D, size_t pag
     if (n_pages == 0 || n_pages > kMaxRows || max_seqs == 0 || max_seqs > kMaxSeqs || max_rows == 0 || max_rows > kMaxRows ||
         max_rows * (H / KVH) > kMaxRows)
       return fail("4-bit cache: invalid number of pages, sequences or rows");
+    if (n_pages * needle_kv4_page_bytes(KVH, D, page_tokens) >= (size_t)1 << 39)
+      return fail("4-bit cache: an array of pages must stay below 512 GiB");
     plan = new NeedleKv4Plan();
     plan->s = Kv4Shape{(int)H, (int)KVH, (int)D, (int)((D + 31) / 32), (int)page_tokens, dtype, (int64_t)n_pages,
                        (int64_t)needle_kv4_page_bytes(KVH, D, page_tokens)};
     plan->max_seqs = max_seqs;
     plan->max_rows = max_rows;
-    if (!ok(cudaGetDevice(&plan->device)) || !ok(cudaMalloc(&plan->buf, 256))) return false;
+    int sms = 0;
+    if (!ok(cudaGetDevice(&plan->device)) ||
+        !ok(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, plan->device)))
+      return false;
+    const size_t cb = (256 + (size_t)kv4_attn_blocks(sms) * sizeof(int) + 255) / 256 * 256;
+    if (!ok(cudaMalloc(&plan->buf, cb + (size_t)kv4_attn_floats(plan->s, sms) * sizeof(float)))) return false;
     plan->work.err = (int *)plan->buf;
     plan->work.bad = plan->work.err + 1;
+    plan->work.counters = plan->work.err + 64;
+    plan->work.ws = (float *)((char *)plan->buf + cb);
+    plan->work.sms = sms;
     cudaStream_t st = (cudaStream_t)stream;
-    return ok(cudaMemsetAsync(plan->buf, 0, 256, st)) && ok(cudaStreamSynchronize(st));
+    return ok(cudaMemsetAsync(plan->buf, 0, cb, st)) && ok(cudaStreamSynchronize(st));
   });
   if (good) return plan;
   needle_kv4_plan_free(plan);

@@ -123,6 +123,7 @@ struct Kv4Rows {
   const int32_t *row_start, *kv_len, *table;
   int n_seq, width;
   int64_t rows;
+  int max_new;  // no request has more rows
 };
 struct Kv4Call {
   uint8_t *pages;
@@ -143,8 +144,13 @@ struct Kv4AttnCall {
   bool causal;
 };
 struct Kv4Work {
-  int *err, *bad;  // a wait that ran out; a request that does not fit
+  int *err = nullptr, *bad = nullptr;  // a wait that ran out; a request that does not fit
+  int *counters = nullptr;             // kv4_attn_blocks of them, zero between calls
+  float *ws = nullptr;                 // kv4_attn_floats
+  int sms = 0;
 };
+int64_t kv4_attn_blocks(int sms);
+int64_t kv4_attn_floats(const Kv4Shape &s, int sms);
 cudaError_t kv4_attn(const Kv4Shape &s, const Kv4Rows &b, const Kv4AttnCall &c, const Kv4Work &w, cudaStream_t st);
 
 // ── verification of drafts ──

@@ -185,7 +185,7 @@ def prepare_kv(case, g, seed):
         at = starts(used)
         table = i32([order[at[i]:at[i + 1]] + [-1] * (width - used[i]) for i in range(B)])
         n_pages = max(sum(used), 1)
-        s["plan"] = n.Kv4Plan(H, KVH, D, page, n_pages, B, max(sum(new), 1), code(t))
+        s["plan"] = n.Kv4Plan(H, KVH, D, page, n_pages, B, max(sum(new), sum(total), 1), code(t))
         s["pages"] = torch.empty(n_pages * n.kv4_page_bytes(KVH, D, page), dtype=torch.uint8, device="cuda")
         s["held"] = [table, i32(starts(new)), i32(total), i32(starts(total))]
         s["batch"] = n.Kv4Batch(s["held"][1].data_ptr(), s["held"][2].data_ptr(), table.data_ptr(), B, sum(new), width, max(new))

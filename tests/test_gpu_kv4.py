@@ -233,7 +233,8 @@ class Attn:
         self.lse = torch.full((self.R, H), 7.0, device="cuda")
         self.lens = cache.lens()
         self.held = i32(self.start), i32(self.lens)
-        self.batch = nb.Kv4Batch(self.held[0].data_ptr(), self.held[1].data_ptr(), cache.table.data_ptr(), cache.B, self.R, cache.width)
+        self.batch = nb.Kv4Batch(self.held[0].data_ptr(), self.held[1].data_ptr(), cache.table.data_ptr(), cache.B, self.R, cache.width,
+                                 max(new))
 
     def run(self, scale, causal, stream=None, plan=None):
         (plan or self.c.plan).attn(self.c.pages.data_ptr(), self.batch, self.q.data_ptr(), self.out.data_ptr(), scale, causal,

@@ -28,7 +28,7 @@ def test_page_bytes():
     (dict(D=136), "head_dim"), (dict(H=6), "num_heads"), (dict(H=0), "num_heads"), (dict(KVH=0), "num_heads"), (dict(H=8192), "num_heads"),
     (dict(page=0), "page_tokens"), (dict(page=24), "page_tokens"), (dict(page=65552), "page_tokens"), (dict(pages=0), "invalid number"),
     (dict(pages=1 << 31), "invalid number"), (dict(seqs=0), "invalid number"), (dict(seqs=(1 << 20) + 1), "invalid number"),
-    (dict(rows=0), "invalid number"), (dict(rows=1 << 31), "invalid number"),
+    (dict(page=65536, pages=100000), "512 GiB"), (dict(rows=0), "invalid number"), (dict(rows=1 << 31), "invalid number"),
 ])
 def test_kv4_plan_refuses(bad, match):
     a = dict(H=8, KVH=4, D=64, page=16, pages=10, seqs=4, rows=64, dtype=nb.BF16)
@@ -96,7 +96,7 @@ int main() {
   Kv4Shape s{8, 4, 64, 2, 32, 1, 10, 4 * 2 * 1280};
   const int32_t start[] = {0, 3, 3, 2, 9, 12, -1, 5, 2147483647}, len[] = {64, 10, 10, 10, 97, -1, 10, 10};
   std::vector<int32_t> table(8 * 3, 0);
-  Kv4Rows b{start, len, table.data(), 8, 3, 11};
+  Kv4Rows b{start, len, table.data(), 8, 3, 11, 7};
   struct { int i; bool inside; int n, len, bad; } want[] = {
       {0, true, 3, 64, 0}, {0, false, 3, 64, 0}, {1, true, 0, 10, 0}, {2, true, 0, 0, 1} /* falls */, {3, true, 7, 10, 0},
       {4, true, 0, 0, 1} /* 97 tokens in 3 pages of 32, and row 12 of 11 */, {5, false, 0, 0, 1} /* falls, length -1 */,
@@ -109,11 +109,14 @@ int main() {
   }
   const int32_t few[] = {2, 10};
   const int32_t two[] = {0, 3, 6};
-  Kv4Rows c{two, few, table.data(), 2, 3, 6};
+  Kv4Rows c{two, few, table.data(), 2, 3, 6, 6};
   int bad = 0;
   CHECK(sequence(c, s, 0, true, &bad).n == 0 && bad == 1);  // three rows among two tokens
   bad = 0;
   CHECK(sequence(c, s, 0, false, &bad).n == 3 && bad == 0);
+
+  c.max_new = 2;
+  CHECK(sequence(c, s, 0, false, &bad).n == 0 && bad == 1);  // three rows where two are the most
 
   // pages outside the array are not addressed
   for (int32_t page : {-1, 10, 2147483647, (int32_t)0x80000000}) {
