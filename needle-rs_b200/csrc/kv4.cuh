@@ -5,8 +5,8 @@
 // another in tiles of 16 tokens.  A tile is 640 bytes for each group of 32
 // dimensions (NG groups: head_dim rounded up):
 //   K codes  [NG][32][2] words    V codes [NG][32][2] words
-//   K (scale, minimum) [16][NG] pairs of f16
-//   V scales and minima  [NG][4 tokens' quads][2][4] f16
+//   K scales [NG][8][2], minima [NG][8][2]: f16 of rows r and r + 8
+//   V scales and minima [NG][4][2][4]: f16 of tokens 4 q .. 4 q + 3
 // The order inside is that of the operands of a 16 x 8 x 16 matrix
 // instruction, so that a lane fetches what it multiplies in 8 bytes and needs no
 // shuffle, and a token's codes share no byte with another's:
@@ -47,7 +47,10 @@ __host__ __device__ __forceinline__ int k_word(int t, int g, int q) {
 __host__ __device__ __forceinline__ int v_half(int ng, int t, int g, int r) {
   return v_codes(ng) + ((g * 32 + r * 4 + (t >> 2)) * 2 + ((t >> 1) & 1)) * 4 + (t & 1) * 2;
 }
-__host__ __device__ __forceinline__ int k_param(int ng, int t, int g) { return k_params(ng) + (row_of(t) * ng + g) * 4; }
+__host__ __device__ __forceinline__ int k_param(int ng, int t, int g, int which) {
+  const int m = row_of(t);
+  return k_params(ng) + (((which * ng + g) * 8 + (m & 7)) * 2 + (m >> 3)) * 2;
+}
 __host__ __device__ __forceinline__ int v_param(int ng, int t, int g, int which) {
   return v_params(ng) + (((g * 4 + (t >> 2)) * 2 + which) * 4 + (t & 3)) * 2;
 }

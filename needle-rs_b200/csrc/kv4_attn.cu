@@ -13,7 +13,8 @@
 // low four bits of a half, a subnormal) or c * 2^-20 (the next four), which
 // tensor cores multiply exactly.
 //   K: q . k = sum over groups of s (q . c) + m (sum of q): products with the
-//      codes, exact in f32, then two FMAs a group for each score.  No key is rounded.
+//      codes, then an FMA a group for each score; the second terms are one small
+//      product of the minima with the sums, each in two f16.  No key is rounded.
 //   V: 1024 + c (or 64 + c) by an OR, minus 1024, times s plus m on pairs of
 //      f16: a value is rounded to f16 once.
 // q is brought to a largest value of 2^10 .. 2^11 by a power of two for each row and
@@ -44,14 +45,37 @@ __device__ __forceinline__ float ex2(float x) {
 }
 __device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
 __device__ __forceinline__ __half2 halves(uint32_t u) { return *reinterpret_cast<__half2 *>(&u); }
-__device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool take) {
+  const int n = take ? 16 : 0;  // 0: the 16 bytes become zero and src is not read
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+// (u & mask) | c in one instruction: c in a register
+__device__ __forceinline__ uint32_t and_or(uint32_t u, uint32_t mask, uint32_t c) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(u), "r"(mask), "r"(c));
+  return d;
+}
+__device__ __forceinline__ uint32_t in_register(uint32_t c) {
+  uint32_t d;
+  asm volatile("mov.b32 %0, %1;" : "=r"(d) : "r"(c));
+  return d;
+}
+// a / b for a below 2^63, b above 0: mostly both fit 32 bits
+__device__ __forceinline__ int64_t divided(int64_t a, int64_t b) {
+  return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
 }
 __device__ __forceinline__ void mma(float *d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// d = a (16 x 8) b (8 x 8)
+__device__ __forceinline__ void mma8(float *d, uint32_t a0, uint32_t a1, uint32_t b0) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%7, %7, %7, %7};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(b0), "f"(0.0f));
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
@@ -60,8 +84,10 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 }
 
 // How the units of a call fall to the blocks: request i has KVH heads x blocks
-// of ROWS rows x units of 64 keys, block b of n takes units
-// [total * b / n, total * (b + 1) / n) of all requests' in order.
+// of ROWS rows ("items") x units of 64 keys, and block b of n takes units
+// [total * b / n, total * (b + 1) / n) of all requests' in order.  A border inside
+// an item of at most a block's share moves to that item's nearer end: such items stay
+// whole, and longer ones are cut and joined.
 struct Share {
   int64_t total, begin, end, base;  // base: units before request `seq`, the one that `begin` falls in
   int blocks, seq;
@@ -69,7 +95,7 @@ struct Share {
 struct Units {
   Seq q;
   int row_blocks;
-  int64_t keys;  // units of a row block and head
+  int64_t keys;  // units of an item
 
   __device__ int64_t all(int KVH) const { return (int64_t)row_blocks * KVH * keys; }
 };
@@ -93,7 +119,7 @@ __device__ __forceinline__ float *slot_of(const Kv4Work &w, int64_t block, int w
 template <int ROWS>
 __device__ Share share_of(const Kv4Rows &b, const Kv4Shape &s, bool causal, const Kv4Work &w) {
   __shared__ int64_t sums[kWarps], items[kWarps];
-  __shared__ int64_t found_base;
+  __shared__ int64_t border[2], found_base;
   __shared__ int found;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int per = (b.n_seq + kThreads - 1) / kThreads, i0 = min((int)threadIdx.x * per, b.n_seq), i1 = min(i0 + per, b.n_seq);
@@ -124,46 +150,54 @@ __device__ Share share_of(const Kv4Rows &b, const Kv4Shape &s, bool causal, cons
   const int64_t blocks = min(min((int64_t)gridDim.x, (r.total + 1) / 2), n * 128);
   r.blocks = (int)blocks;
   if (blockIdx.x >= blocks) return r;
-  r.begin = r.total * blockIdx.x / blocks;
-  r.end = r.total * (blockIdx.x + 1) / blocks;
-  if (upto - mine <= r.begin && r.begin < upto) {
-    int64_t base = upto - mine;
-    for (int i = i0;; ++i) {
-      const int64_t x = units_of<ROWS>(b, s, i, causal, w.bad).all(s.KVH);
-      if (r.begin < base + x) {
-        found = i;
-        found_base = base;
-        break;
+  const int64_t whole = divided(r.total, blocks);
+  const int rest = (int)(r.total - whole * blocks);
+#pragma unroll 1
+  for (int e = 0; e < 2; ++e) {
+    const int64_t x = whole * (blockIdx.x + e) + (uint32_t)rest * (blockIdx.x + e) / (uint32_t)blocks;
+    if (x == r.total && threadIdx.x == 0) border[e] = x;
+    if (upto - mine <= x && x < upto) {
+      int64_t base = upto - mine;
+      int i = i0;
+      Units u = units_of<ROWS>(b, s, i, causal, w.bad);
+      while (x >= base + u.all(s.KVH)) {
+        base += u.all(s.KVH);
+        u = units_of<ROWS>(b, s, ++i, causal, w.bad);
       }
-      base += x;
+      const int64_t in = x - base - divided(x - base, u.keys) * u.keys, to = u.keys * blocks > r.total ? x : in * 2 < u.keys ? x - in : x - in + u.keys;
+      border[e] = to;
+      if (e == 0) found = i, found_base = base;
     }
   }
   __syncthreads();
+  r.begin = border[0];
+  r.end = border[1];
   r.seq = found;
   r.base = found_base;
   return r;
 }
 
-// Stages of a warp's ring, and blocks an SM.
-__host__ __device__ constexpr int few_stages(int ng) { return ng == 4 ? 5 : ng == 3 ? 6 : 8; }
+// A warp's ring holds pairs of tiles (32 keys a turn); stages of it, and blocks an SM.
+__host__ __device__ constexpr int few_stages(int ng) { return ng == 4 ? 2 : ng == 3 ? 3 : 4; }
 __host__ __device__ constexpr int few_blocks(int nb) { return nb == 1 ? 4 : nb == 2 ? 3 : 2; }
 template <int NG, int NB>
 constexpr int few_smem() {
-  constexpr int ring = kWarps * few_stages(NG) * tile_bytes(NG), merge = kWarps * NB * 8 * (NG * 32 + 4 + 2) * 4;
+  constexpr int ring = kWarps * few_stages(NG) * 2 * tile_bytes(NG), merge = kWarps * NB * 8 * (NG * 32 + 4 + 2) * 4;
   return ring > merge ? ring : merge;
 }
 
 template <typename T, int NG, int NB>
 __global__ void __launch_bounds__(kThreads, few_blocks(NB))
     few_kernel(Kv4AttnCall c, Kv4Shape s, Kv4Rows b, Kv4Work w) {
-  constexpr int ST = few_stages(NG), TB = tile_bytes(NG), ROWS = NB * 8, DP = NG * 32;
+  constexpr int ST = few_stages(NG), TB = tile_bytes(NG), ROWS = NB * 8, DP = NG * 32, PAIR = 2 * kTokens;
+  constexpr uint32_t kLo = 0x000f000fu, kHi = 0x00f000f0u;
   extern __shared__ __align__(128) uint8_t sm[];
   __shared__ int last_one;
   const Share share = share_of<ROWS>(b, s, c.causal, w);
   if (blockIdx.x >= share.blocks) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, q4 = lane & 3;
   const int G = s.H / s.KVH, D = s.D;
-  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(sm) + warp * ST * TB;
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(sm) + warp * ST * 2 * TB;
 
   int seq = share.seq;
   int64_t base = share.base, at = share.begin;
@@ -183,66 +217,70 @@ __global__ void __launch_bounds__(kThreads, few_blocks(NB))
       }
       un = units_of<ROWS>(b, s, seq, c.causal, w.bad);
     }
-    const int64_t item = (at - base) / un.keys, first = base + item * un.keys;
+    const int64_t item = divided(at - base, un.keys), first = base + item * un.keys;
     const int u0 = (int)(at - first), u1 = (int)min(un.keys, share.end - first);
     at = first + u1;
-    const int kvh = (int)(item % s.KVH), r0 = (int)(item / s.KVH) * ROWS;
+    const int rb = (int)divided(item, s.KVH), kvh = (int)(item - (int64_t)rb * s.KVH), r0 = rb * ROWS;
     const int rows = min(ROWS, un.q.n * G - r0), len = un.q.len;
     // keys that row x of the block sees
     auto limit = [&](int x) { return c.causal ? len - un.q.n + (r0 + min(x, rows - 1)) / G + 1 : len; };
-    const int k_all = limit(0);                                         // every row sees these
+    const int k_all = limit(0);  // every row sees these
     const int t0 = u0 * (kUnit / kTokens);
     const int t1 = min(u1 * (kUnit / kTokens), (limit(rows - 1) + kTokens - 1) / kTokens);
-    const int mine = max(0, (t1 - t0 - warp + kWarps - 1) / kWarps);  // tiles of this warp
-
-    // tiles' places in units of 128 bytes, of 32 of the warp's tiles (a lane each) and of the next 32
-    auto places = [&](int n) {
-      const int t = t0 + warp + (n + lane) * kWarps;
-      if (n + lane >= mine) return kNoPlace;
-      return place_of(b, s, seq, t, kvh, w.bad);
-    };
-    uint32_t window = places(0), ahead = places(32);
-    auto issue = [&](int n, int stage) {
-      if ((n & 31) == 0 && n > 0) {
-        window = ahead;
-        ahead = places(n + 32);
-      }
-      const uint32_t place = __shfl_sync(0xffffffffu, window, n & 31);
-      if (place != kNoPlace) {
-        const uint8_t *src = c.pages + (int64_t)place * 128;
-#pragma unroll
-        for (int i = 0; i < (TB / 16 + 31) / 32; ++i)
-          if (i * 32 + lane < TB / 16) cp16(ring + stage * TB + (i * 32 + lane) * 16, src + (i * 32 + lane) * 16);
-      }
-      return place != kNoPlace;
-    };
-    uint32_t there = 0;  // bit `stage`: its tile exists
-#pragma unroll
-    for (int n = 0; n < ST - 1; ++n) {
-      if (n < mine && issue(n, n)) there |= 1u << n;
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    }
+    // turns of this warp: it takes every fourth pair of tiles
+    const int pairs = max(0, (t1 - t0 + 1) >> 1), mine = max(0, (pairs - warp + kWarps - 1) / kWarps);
 
     // q: lane 4 n + q4 has dimensions 32 g + 8 q4 .. of row n, as its column of the matrix product
-    uint32_t qf[NB][NG][4];
-    float qs[NB][NG][2], sc[NB][2];  // sums of a group (* 2^-24), and the score's factor, of rows 2 q4 and 2 q4 + 1
-    int lim[NB][2];
+    uint4 raw[NB][NG];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       const int x = nb * 8 + r, row = r0 + x;
-      const bool have = x < rows;
       const T *q = (const T *)c.q + (un.q.row0 + row / G) * c.q_row + (int64_t)(kvh * G + row % G) * c.q_head;
-      float v[NG][8], top = 0.0f;
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         const int d = g * 32 + q4 * 8;
+        raw[nb][g] = x < rows && d < D ? *reinterpret_cast<const uint4 *>(q + d) : make_uint4(0, 0, 0, 0);
+      }
+    }
+
+    // places of 32 of the warp's tiles (a lane each: two for each turn) and of the next 32
+    auto places = [&](int n) {
+      const int t = t0 + 2 * (warp + (n + (lane >> 1)) * kWarps) + (lane & 1);
+      return n + (lane >> 1) < mine && t < t1 ? place_of(b, s, seq, t, kvh, w.bad) : kNoPlace;
+    };
+    uint32_t window = places(0), ahead = places(16);
+    auto issue = [&](int n, int stage) {  // tiles that are not there become zeros
+      if ((n & 15) == 0 && n > 0) {
+        window = ahead;
+        ahead = places(n + 16);
+      }
+      const uint32_t p0 = __shfl_sync(0xffffffffu, window, (n & 15) * 2), p1 = __shfl_sync(0xffffffffu, window, (n & 15) * 2 + 1);
+      const bool h0 = p0 != kNoPlace, h1 = p1 != kNoPlace;
+      const uint8_t *s0 = c.pages + (h0 ? (int64_t)p0 * 128 : 0) + lane * 16, *s1 = c.pages + (h1 ? (int64_t)p1 * 128 : 0) + lane * 16;
+      const uint32_t to = ring + stage * 2 * TB + lane * 16;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[g][i] = 0.0f;
-        if (have && d < D) load<8>(q + d, v[g]);
+      for (int i = 0; i < (TB + 511) / 512; ++i) {
+        if (i * 512 + lane * 16 >= TB) break;
+        cp16(to + i * 512, s0 + i * 512, h0);
+        cp16(to + TB + i * 512, s1 + i * 512, h1);
+      }
+    };
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(v[g][i])));
-        }
+    for (int n = 0; n < ST - 1; ++n) {
+      if (n < mine) issue(n, n);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+
+    uint32_t qf[NB][NG][4], qm[NB];
+    float sc[NB][2], step[NB][2];  // a score's factor, and 2^8 in a score's units, of rows 2 q4 and 2 q4 + 1
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      float top = 0.0f;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const T *e = reinterpret_cast<const T *>(&raw[nb][g]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf((float)e[i])));
       }
 #pragma unroll
       for (int o = 1; o < 4; o <<= 1) {
@@ -250,107 +288,141 @@ __global__ void __launch_bounds__(kThreads, few_blocks(NB))
         asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(other));
       }
       // 2^e brings the largest value to [2^10, 2^11); infinities and NaN make the row NaN
-      const int e = min(100, 137 - (int)(__float_as_uint(top) >> 23));
-      const float up = __uint_as_float((uint32_t)(e + 127) << 23);
-      const float mul = top <= 3.402823466e38f ? up : __uint_as_float(0x7fc00000u);
-      const float factor = c.scale * kLog2e * 16777216.0f * __uint_as_float((uint32_t)(127 - e) << 23);
+      const int e2 = min(100, 137 - (int)(__float_as_uint(top) >> 23));
+      const float mul = top <= 3.402823466e38f ? __uint_as_float((uint32_t)(e2 + 127) << 23) : __uint_as_float(0x7fc00000u);
+      const float factor = c.scale * kLog2e * 16777216.0f * __uint_as_float((uint32_t)(127 - e2) << 23);
+      float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        float sum = 0.0f;
+        const T *e = reinterpret_cast<const T *>(&raw[nb][g]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const __half2 h = __floats2half2_rn(v[g][2 * i] * mul, v[g][2 * i + 1] * mul);
+          const __half2 h = __floats2half2_rn((float)e[2 * i] * mul, (float)e[2 * i + 1] * mul);
           const float2 f = __half22float2(h);
-          sum += f.x + f.y;
+          sums[g] += f.x + f.y;
           // pairs 1 and 3 meet codes that are 16 times as large
           qf[nb][g][i] = bits(i & 1 ? __hmul2(h, __float2half2_rn(0.0625f)) : h);
         }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        sum *= 5.9604644775390625e-8f;  // 2^-24
-        qs[nb][g][0] = __shfl_sync(0xffffffffu, sum, 8 * q4);
-        qs[nb][g][1] = __shfl_sync(0xffffffffu, sum, 8 * q4 + 4);
+        sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 1);
+        sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 2);
+        sums[g] *= 0.015625f;  // 2^-6: at most 2^10
       }
+      // the sums as f16 and what is left over: the operand that meets the groups' minima
+      const float a = q4 & 1 ? sums[2] : sums[0], b2 = q4 & 1 ? sums[3] : sums[1];
+      __half2 h = __floats2half2_rn(a, b2);
+      if (q4 >= 2) {
+        const float2 f = __half22float2(h);
+        h = __floats2half2_rn(a - f.x, b2 - f.y);
+      }
+      qm[nb] = bits(h);
       sc[nb][0] = __shfl_sync(0xffffffffu, factor, 8 * q4);
       sc[nb][1] = __shfl_sync(0xffffffffu, factor, 8 * q4 + 4);
-      lim[nb][0] = limit(nb * 8 + 2 * q4);
-      lim[nb][1] = limit(nb * 8 + 2 * q4 + 1);
+      step[nb][0] = 8.0f / sc[nb][0];
+      step[nb][1] = 8.0f / sc[nb][1];
     }
 
-    float o[NB][NG][8], m[NB][2], l[NB][2];  // m: in units of log2
+    // weights are 2^(x sc - from); a score above `past` moves `from`
+    float o[NB][NG][8], from[NB][2], past[NB][2], l[NB][2];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
       for (int g = 0; g < NG; ++g)
 #pragma unroll
         for (int i = 0; i < 8; ++i) o[nb][g][i] = 0.0f;
-      m[nb][0] = m[nb][1] = -INFINITY;
-      l[nb][0] = l[nb][1] = 0.0f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) past[nb][h] = -INFINITY, from[nb][h] = l[nb][h] = 0.0f;
     }
 
+    const uint32_t i1024 = in_register(0x64006400u), i64 = in_register(0x54005400u);
+    const __half2 c1024 = halves(i1024), c64 = halves(i64);
+    auto low = [&](uint32_t u, __half2 sc, __half2 mi) { return bits(__hfma2(__hsub2(halves(and_or(u, kLo, i1024)), c1024), sc, mi)); };
+    auto high = [&](uint32_t u, __half2 sc, __half2 mi) { return bits(__hfma2(__hsub2(halves(and_or(u, kHi, i64)), c64), sc, mi)); };
     int stage = 0;
     for (int n = 0; n < mine; ++n) {
       asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
       __syncwarp();  // every lane's copies of this stage, and the reads of the stage refilled next
-      if (n + ST - 1 < mine) {
-        const int to = stage == 0 ? ST - 1 : stage - 1;
-        there = issue(n + ST - 1, to) ? there | 1u << to : there & ~(1u << to);
-      }
+      if (n + ST - 1 < mine) issue(n + ST - 1, stage == 0 ? ST - 1 : stage - 1);
       asm volatile("cp.async.commit_group;" ::: "memory");
-      const uint8_t *tile = sm + (warp * ST + stage) * TB;
-      const bool have = (there >> stage) & 1;
+      const int j = (t0 + 2 * (warp + n * kWarps)) * kTokens;
+      uint8_t *tile = sm + (warp * ST + stage) * 2 * TB;
       if (++stage == ST) stage = 0;
-      if (!have) continue;
-      const int j = (t0 + warp + n * kWarps) * kTokens;
-      __syncwarp();  // the products below take a whole warp
-
-      // scores
-      float x[NB][4];
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[nb][i] = 0.0f;
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        const uint2 k = *reinterpret_cast<const uint2 *>(tile + g * 256 + lane * 8);
-        const float2 p0 = __half22float2(*reinterpret_cast<const __half2 *>(tile + k_params(NG) + (r * NG + g) * 4));
-        const float2 p1 = __half22float2(*reinterpret_cast<const __half2 *>(tile + k_params(NG) + ((r + 8) * NG + g) * 4));
-        const uint32_t lo = 0x000f000fu, hi = 0x00f000f0u, kx = k.x >> 8, ky = k.y >> 8;
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          mma(a, k.x & lo, k.y & lo, k.x & hi, k.y & hi, qf[nb][g][0], qf[nb][g][1]);
-          mma(a, kx & lo, ky & lo, kx & hi, ky & hi, qf[nb][g][2], qf[nb][g][3]);
-          x[nb][0] = fmaf(p0.x, a[0], fmaf(p0.y, qs[nb][g][0], x[nb][0]));
-          x[nb][1] = fmaf(p0.x, a[1], fmaf(p0.y, qs[nb][g][1], x[nb][1]));
-          x[nb][2] = fmaf(p1.x, a[2], fmaf(p1.y, qs[nb][g][0], x[nb][2]));
-          x[nb][3] = fmaf(p1.x, a[3], fmaf(p1.y, qs[nb][g][1], x[nb][3]));
+      if (j + PAIR > len) {  // behind the last token the page may hold anything
+        for (int u = lane; u < 2 * 32 * NG; u += 32) {
+          const int half = u / (32 * NG), in = u % (32 * NG), t = ((in >> 3) & 3) * 4 + (in & 3);
+          if (j + half * kTokens + t >= len) *reinterpret_cast<uint16_t *>(tile + half * TB + v_params(NG) + in * 2) = 0;
         }
       }
-      const bool cut = j + kTokens > k_all;
-      const int ja = j + 4 * (r >> 1) + (r & 1);  // the token of the matrix's row r; that of r + 8 is 2 on
+      __syncwarp();  // the products below take a whole warp
+      // scores, minima first
+      float x[NB][2][4];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int g0 = 2 * (q4 & 1);
+        const uint8_t *p = tile + half * TB + k_params(NG) + ((NG + g0) * 8 + r) * 4;
+        const uint32_t y0 = g0 < NG ? *reinterpret_cast<const uint32_t *>(p) : 0u;
+        const uint32_t y1 = g0 + 1 < NG ? *reinterpret_cast<const uint32_t *>(p + 32) : 0u;
+        const uint32_t a0 = __byte_perm(y0, y1, 0x5410), a1 = __byte_perm(y0, y1, 0x7632);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          mma8(x[nb][half], a0, a1, qm[nb]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[nb][half][i] *= 3.814697265625e-06f;  // 2^-18
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint2 k = *reinterpret_cast<const uint2 *>(tile + half * TB + g * 256 + lane * 8);
+          const float2 p = __half22float2(*reinterpret_cast<const __half2 *>(tile + half * TB + k_params(NG) + (g * 8 + r) * 4));
+          const uint32_t kx = k.x >> 8, ky = k.y >> 8;
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            mma(a, k.x & kLo, k.y & kLo, k.x & kHi, k.y & kHi, qf[nb][g][0], qf[nb][g][1]);
+            mma(a, kx & kLo, ky & kLo, kx & kHi, ky & kHi, qf[nb][g][2], qf[nb][g][3]);
+            float *y = x[nb][half];
+            y[0] = fmaf(p.x, a[0], y[0]);
+            y[1] = fmaf(p.x, a[1], y[1]);
+            y[2] = fmaf(p.y, a[2], y[2]);
+            y[3] = fmaf(p.y, a[3], y[3]);
+          }
+        }
+      if (j + PAIR > k_all) {
+        const int ja = j + 4 * (r >> 1) + (r & 1);  // the token of the matrix's row r; that of r + 8 is 2 on
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int lim = limit(nb * 8 + 2 * q4 + h);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              if (ja + half * kTokens >= lim) x[nb][half][h] = -INFINITY;
+              if (ja + half * kTokens + 2 >= lim) x[nb][half][h + 2] = -INFINITY;
+            }
+          }
+      }
       bool move = false;
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[nb][i] *= sc[nb][i & 1];
-          if (cut && ja + (i & 2) >= lim[nb][i & 1]) x[nb][i] = -INFINITY;
-          move = move || x[nb][i] > m[nb][i & 1] + 8.0f;
-        }
-      // m moves only when a score passes it by 2^8: a weight is at most 256
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) move = move || x[nb][half][i] > past[nb][i & 1];
+      // only when a score passes it by 2^8: a weight is at most 256
       if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            float top = fmaxf(x[nb][h], x[nb][2 + h]);
+            float top = fmaxf(fmaxf(x[nb][0][h], x[nb][0][2 + h]), fmaxf(x[nb][1][h], x[nb][1][2 + h]));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-            if (top > m[nb][h]) {
-              const float f = ex2(m[nb][h] - top);
-              m[nb][h] = top;
+            if (top > past[nb][h]) {
+              const float m = top * sc[nb][h], f = past[nb][h] == -INFINITY ? 0.0f : ex2(from[nb][h] - m);
+              from[nb][h] = m;
+              past[nb][h] = top + step[nb][h];
               l[nb][h] *= f;
 #pragma unroll
               for (int g = 0; g < NG; ++g)
@@ -360,47 +432,38 @@ __global__ void __launch_bounds__(kThreads, few_blocks(NB))
           }
         __syncwarp();
       }
-      uint32_t pf[NB][2];
+      uint32_t pf[NB][2][2];
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const float b0 = m[nb][0] == -INFINITY ? 0.0f : m[nb][0], b1 = m[nb][1] == -INFINITY ? 0.0f : m[nb][1];
-        const float w0 = ex2(x[nb][0] - b0), w1 = ex2(x[nb][1] - b1), w2 = ex2(x[nb][2] - b0), w3 = ex2(x[nb][3] - b1);
-        l[nb][0] += w0 + w2;
-        l[nb][1] += w1 + w3;
-        // keys by rows -> rows by keys: the other operand of the product with V
-        pf[nb][0] = transpose8(bits(__floats2half2_rn(w0, w1)));
-        pf[nb][1] = transpose8(bits(__floats2half2_rn(w2, w3)));
-      }
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          float p[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) p[i] = ex2(fmaf(x[nb][half][i], sc[nb][i & 1], -from[nb][i & 1]));
+          l[nb][0] += p[0] + p[2];
+          l[nb][1] += p[1] + p[3];
+          // keys by rows -> rows by keys: the other operand of the product with V
+          pf[nb][half][0] = transpose8(bits(__floats2half2_rn(p[0], p[1])));
+          pf[nb][half][1] = transpose8(bits(__floats2half2_rn(p[2], p[3])));
+        }
 
       // O^T += V^T P^T
 #pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        const uint2 v = *reinterpret_cast<const uint2 *>(tile + v_codes(NG) + g * 256 + lane * 8);
-        uint4 p = *reinterpret_cast<const uint4 *>(tile + v_params(NG) + (g * 4 + q4) * 16);
-        if (cut) {  // behind the last token the page may hold anything
-          const int left = len - j - 4 * q4;
-          p.x &= left >= 2 ? 0xffffffffu : left == 1 ? 0xffffu : 0u;
-          p.z &= left >= 2 ? 0xffffffffu : left == 1 ? 0xffffu : 0u;
-          p.y &= left >= 4 ? 0xffffffffu : left == 3 ? 0xffffu : 0u;
-          p.w &= left >= 4 ? 0xffffffffu : left == 3 ? 0xffffu : 0u;
-        }
-        const __half2 s0 = halves(p.x), s1 = halves(p.y), m0 = halves(p.z), m1 = halves(p.w);
-        const __half2 c1024 = halves(0x64006400u), c64 = halves(0x54005400u);
-        auto low = [&](uint32_t u, __half2 sc, __half2 mi) {
-          return bits(__hfma2(__hsub2(halves((u & 0x000f000fu) | 0x64006400u), c1024), sc, mi));
-        };
-        auto high = [&](uint32_t u, __half2 sc, __half2 mi) {
-          return bits(__hfma2(__hsub2(halves((u & 0x00f000f0u) | 0x54005400u), c64), sc, mi));
-        };
-        const uint32_t a0 = low(v.x, s0, m0), a1 = high(v.x, s0, m0), a2 = low(v.y, s1, m1), a3 = high(v.y, s1, m1);
-        const uint32_t vx = v.x >> 8, vy = v.y >> 8;
-        const uint32_t b0 = low(vx, s0, m0), b1 = high(vx, s0, m0), b2 = low(vy, s1, m1), b3 = high(vy, s1, m1);
+      for (int g = 0; g < NG; ++g)
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          mma(o[nb][g], a0, a1, a2, a3, pf[nb][0], pf[nb][1]);
-          mma(o[nb][g] + 4, b0, b1, b2, b3, pf[nb][0], pf[nb][1]);
+        for (int half = 0; half < 2; ++half) {
+          const uint2 v = *reinterpret_cast<const uint2 *>(tile + half * TB + v_codes(NG) + g * 256 + lane * 8);
+          const uint4 p = *reinterpret_cast<const uint4 *>(tile + half * TB + v_params(NG) + (g * 4 + q4) * 16);
+          const __half2 s0 = halves(p.x), s1 = halves(p.y), m0 = halves(p.z), m1 = halves(p.w);
+          const uint32_t vx = v.x >> 8, vy = v.y >> 8;
+          const uint32_t a0 = low(v.x, s0, m0), a1 = high(v.x, s0, m0), a2 = low(v.y, s1, m1), a3 = high(v.y, s1, m1);
+          const uint32_t b0 = low(vx, s0, m0), b1 = high(vx, s0, m0), b2 = low(vy, s1, m1), b3 = high(vy, s1, m1);
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            mma(o[nb][g], a0, a1, a2, a3, pf[nb][half][0], pf[nb][half][1]);
+            mma(o[nb][g] + 4, b0, b1, b2, b3, pf[nb][half][0], pf[nb][half][1]);
+          }
         }
-      }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();  // the rings are free
@@ -418,7 +481,7 @@ __global__ void __launch_bounds__(kThreads, few_blocks(NB))
         lr += __shfl_xor_sync(0xffffffffu, lr, 16);
         const int x = warp * ROWS + nb * 8 + 2 * q4 + h;
         if (r == 0) {
-          smm[x] = m[nb][h];
+          smm[x] = past[nb][h] == -INFINITY ? -INFINITY : from[nb][h];
           sl[x] = lr;
         }
 #pragma unroll
@@ -467,7 +530,7 @@ __global__ void __launch_bounds__(kThreads, few_blocks(NB))
     }
     if (!whole) {
       // the blocks that hold parts of this item; the last to arrive joins them in their order
-      auto block_of = [&](int64_t unit) { return ((unit + 1) * share.blocks - 1) / share.total; };
+      auto block_of = [&](int64_t unit) { return divided((unit + 1) * share.blocks - 1, share.total); };
       const int64_t b0 = block_of(first), b1 = block_of(first + un.keys - 1);
       __threadfence();
       __syncthreads();

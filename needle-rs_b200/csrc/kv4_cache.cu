@@ -77,7 +77,7 @@ __global__ void append_kernel(Kv4Call c, Kv4Shape s, Kv4Rows b, int *bad) {
       w |= __shfl_xor_sync(0xffffffffu, w, 2);
       w |= __shfl_xor_sync(0xffffffffu, w, 4);
       if ((lane & 7) == 0) *(uint32_t *)(tile + k_word(t, g, lane >> 3)) = w;
-      if (lane == 0) *(__half2 *)(tile + k_param(ng, t, g)) = __halves2half2(scale, least);
+      if (lane < 2) *(__half *)(tile + k_param(ng, t, g, lane)) = lane ? least : scale;
     }
   }
 }
@@ -97,7 +97,8 @@ __global__ void read_kernel(Kv4Call c, Kv4Shape s, Kv4Rows b, int *bad) {
   const int t = at.pos % kTokens;
   for (int d = lane; d < s.D; d += 32) {
     const int g = d >> 5, i = d & 31;
-    const float2 kp = __half22float2(*(const __half2 *)(tile + k_param(ng, t, g)));
+    const float2 kp = make_float2(__half2float(*(const __half *)(tile + k_param(ng, t, g, 0))),
+                                  __half2float(*(const __half *)(tile + k_param(ng, t, g, 1))));
     if (c.k_out) {
       const uint32_t w = *(const uint32_t *)(tile + k_word(t, g, i >> 3));
       k[d] = from_f32<T>(fmaf(kp.x, (float)((w >> (4 * (((i & 7) >> 1) + 4 * (i & 1)))) & 15u), kp.y));

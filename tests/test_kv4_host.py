@@ -85,9 +85,8 @@ int main() {
       for (int g = 0; g < ng; ++g) {
         for (int q = 0; q < 4; ++q) claim(k_word(t, g, q), 4, t);
         for (int r = 0; r < 8; ++r) claim(v_half(ng, t, g, r), 2, t);
-        claim(k_param(ng, t, g), 4, t);
-        for (int w = 0; w < 2; ++w) claim(v_param(ng, t, g, w), 2, t);
-        CHECK(k_word(t, g, 0) % 4 == 0 && v_half(ng, t, g, 0) % 2 == 0 && k_param(ng, t, g) % 4 == 0);
+        for (int w = 0; w < 2; ++w) claim(k_param(ng, t, g, w), 2, t), claim(v_param(ng, t, g, w), 2, t);
+        CHECK(k_word(t, g, 0) % 4 == 0 && v_half(ng, t, g, 0) % 2 == 0 && k_param(ng, t, g, 0) % 2 == 0);
       }
     for (int b : owner) CHECK(b >= 0);
   }
