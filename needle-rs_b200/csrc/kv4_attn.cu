@@ -15,8 +15,8 @@
 //   K: q . k = sum over groups of s (q . c) + m (sum of q): products with the
 //      codes, then an FMA a group for each score; the second terms are one small
 //      product of the minima with the sums, each in two f16.  No key is rounded.
-//   V: 1024 + c (or 64 + c) by an OR, minus 1024, times s plus m on pairs of
-//      f16: a value is rounded to f16 once.
+//   V: the weights (f16) times a group's s, rounded to f16 again, multiply the
+//      codes; the second terms are one small product of the minima with the weights.
 // q is brought to a largest value of 2^10 .. 2^11 by a power of two for each row and
 // taken as f16 (exact, but for values below 2^-24 of the row's largest).
 #include <cuda_bf16.h>
@@ -49,21 +49,6 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool take) {
   const int n = take ? 16 : 0;  // 0: the 16 bytes become zero and src is not read
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
-// (u & mask) | c in one instruction: c in a register
-__device__ __forceinline__ uint32_t and_or(uint32_t u, uint32_t mask, uint32_t c) {
-  uint32_t d;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(u), "r"(mask), "r"(c));
-  return d;
-}
-__device__ __forceinline__ uint32_t in_register(uint32_t c) {
-  uint32_t d;
-  asm volatile("mov.b32 %0, %1;" : "=r"(d) : "r"(c));
-  return d;
-}
-// a / b for a below 2^63, b above 0: mostly both fit 32 bits
-__device__ __forceinline__ int64_t divided(int64_t a, int64_t b) {
-  return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
-}
 __device__ __forceinline__ void mma(float *d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -87,101 +72,103 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 // of ROWS rows ("items") x units of 64 keys, and block b of n takes units
 // [total * b / n, total * (b + 1) / n) of all requests' in order.  A border inside
 // an item of at most a block's share moves to that item's nearer end: such items stay
-// whole, and longer ones are cut and joined.
-struct Share {
-  int64_t total, begin, end, base;  // base: units before request `seq`, the one that `begin` falls in
-  int blocks, seq;
-};
+// whole, and longer ones are cut and joined.  Units count in 32 bits: a thread's
+// requests have less than 2^25.
 struct Units {
   Seq q;
-  int row_blocks;
-  int64_t keys;  // units of an item
+  int row_blocks, keys;  // `keys`: units of an item
 
-  __device__ int64_t all(int KVH) const { return (int64_t)row_blocks * KVH * keys; }
+  __device__ uint32_t all(int KVH) const { return (uint32_t)row_blocks * KVH * keys; }
 };
 template <int ROWS>
 __device__ __forceinline__ Units units_of(const Kv4Rows &b, const Kv4Shape &s, int i, bool causal, int *bad) {
   Units u;
   u.q = sequence(b, s, i, causal, bad);
-  u.row_blocks = (int)(((int64_t)u.q.n * (s.H / s.KVH) + ROWS - 1) / ROWS);
+  u.row_blocks = (u.q.n * (s.H / s.KVH) + ROWS - 1) / ROWS;
   u.keys = max(1, (u.q.len + kUnit - 1) / kUnit);
+  if ((int64_t)u.row_blocks * s.KVH * u.keys >= 1 << 25) {
+    *bad = 1;
+    u.row_blocks = 0;
+  }
   return u;
 }
+struct Share {
+  uint32_t total, begin, end, base;  // base: units before request `seq`, the one that `begin` falls in
+  int blocks, seq;
+  Units un;  // of request `seq`
+};
 
 // Partial results of items that are cut between blocks: two slots a block (the
 // item that it starts in the middle of, the one that it leaves unfinished) of
 // ROWS x (DP + 2) floats, and a counter of arrivals for each block where such an item begins.
 template <int ROWS, int DP>
-__device__ __forceinline__ float *slot_of(const Kv4Work &w, int64_t block, int which) {
-  return w.ws + (block * 2 + which) * (ROWS * (DP + 2));
+__device__ __forceinline__ float *slot_of(const Kv4Work &w, int block, int which) {
+  return w.ws + ((int64_t)block * 2 + which) * (ROWS * (DP + 2));
 }
 
 template <int ROWS>
-__device__ Share share_of(const Kv4Rows &b, const Kv4Shape &s, bool causal, const Kv4Work &w) {
-  __shared__ int64_t sums[kWarps], items[kWarps];
-  __shared__ int64_t border[2], found_base;
-  __shared__ int found;
+__device__ __forceinline__ void share_of(const Kv4Rows &b, const Kv4Shape &s, bool causal, const Kv4Work &w, Share *share) {
+  __shared__ uint32_t sums[kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int per = (b.n_seq + kThreads - 1) / kThreads, i0 = min((int)threadIdx.x * per, b.n_seq), i1 = min(i0 + per, b.n_seq);
-  int64_t mine = 0, n = 0;
+  uint32_t mine = 0;
+  Units u;
   for (int i = i0; i < i1; ++i) {
-    const Units u = units_of<ROWS>(b, s, i, causal, w.bad);
-    mine += u.all(s.KVH);
-    n += (int64_t)u.row_blocks * s.KVH;
+    u = units_of<ROWS>(b, s, i, causal, w.bad);
+    mine = min(mine + u.all(s.KVH), (1u << 25) - 1);
   }
-  int64_t upto = mine;
+  uint32_t upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+    const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= o) upto += x;
-    n += __shfl_xor_sync(0xffffffffu, n, o);
   }
   if (lane == 31) sums[warp] = upto;
-  if (lane == 0) items[warp] = n;
   __syncthreads();
-  Share r;
-  r.total = n = 0;
+  uint32_t total = 0;
+#pragma unroll
   for (int k = 0; k < kWarps; ++k) {
     if (k < warp) upto += sums[k];
-    r.total += sums[k];
-    n += items[k];
+    total += sums[k];
   }
-  // an item is cut into 128 pieces at most, and a block has two units at least
-  const int64_t blocks = min(min((int64_t)gridDim.x, (r.total + 1) / 2), n * 128);
-  r.blocks = (int)blocks;
-  if (blockIdx.x >= blocks) return r;
-  const int64_t whole = divided(r.total, blocks);
-  const int rest = (int)(r.total - whole * blocks);
-#pragma unroll 1
-  for (int e = 0; e < 2; ++e) {
-    const int64_t x = whole * (blockIdx.x + e) + (uint32_t)rest * (blockIdx.x + e) / (uint32_t)blocks;
-    if (x == r.total && threadIdx.x == 0) border[e] = x;
-    if (upto - mine <= x && x < upto) {
-      int64_t base = upto - mine;
-      int i = i0;
-      Units u = units_of<ROWS>(b, s, i, causal, w.bad);
-      while (x >= base + u.all(s.KVH)) {
-        base += u.all(s.KVH);
-        u = units_of<ROWS>(b, s, ++i, causal, w.bad);
+  const uint32_t blocks = min(gridDim.x, (total + 1) / 2), me = blockIdx.x;  // a block has two units at least
+  if (threadIdx.x == 0) {
+    share->total = total;
+    share->blocks = (int)blocks;
+    share->end = total;
+  }
+  __syncthreads();
+  if (me >= blocks) return;
+  const uint32_t whole = total / blocks, rest = total - whole * blocks;
+  const uint32_t lo = whole * me + rest * me / blocks, hi = whole * (me + 1) + rest * (me + 1) / blocks;
+  const uint32_t before = upto - mine;
+  if (before <= hi && lo < upto) {
+    uint32_t base = before;
+    for (int i = i0; i < i1; ++i) {
+      if (per > 1) u = units_of<ROWS>(b, s, i, causal, w.bad);
+      const uint32_t next = min(base + u.all(s.KVH), upto);
+      auto border = [&](uint32_t x) {
+        const uint32_t in = (x - base) % u.keys;
+        return u.keys > whole ? x : in * 2 < (uint32_t)u.keys ? x - in : x - in + u.keys;
+      };
+      if (base <= lo && lo < next) {
+        share->begin = border(lo);
+        share->base = base;
+        share->seq = i;
+        share->un = u;
       }
-      const int64_t in = x - base - divided(x - base, u.keys) * u.keys, to = u.keys * blocks > r.total ? x : in * 2 < u.keys ? x - in : x - in + u.keys;
-      border[e] = to;
-      if (e == 0) found = i, found_base = base;
+      if (base <= hi && hi < next) share->end = border(hi);
+      base = next;
     }
   }
   __syncthreads();
-  r.begin = border[0];
-  r.end = border[1];
-  r.seq = found;
-  r.base = found_base;
-  return r;
 }
 
 // A warp's ring holds pairs of tiles (32 keys a turn); stages of it, and blocks an SM.
 __host__ __device__ constexpr int few_stages(int ng) { return ng == 4 ? 2 : ng == 3 ? 3 : 4; }
 __host__ __device__ constexpr int few_blocks(int nb) { return nb == 1 ? 4 : nb == 2 ? 3 : 2; }
 template <int NG, int NB>
-constexpr int few_smem() {
+__host__ __device__ constexpr int few_smem() {
   constexpr int ring = kWarps * few_stages(NG) * 2 * tile_bytes(NG), merge = kWarps * NB * 8 * (NG * 32 + 4 + 2) * 4;
   return ring > merge ? ring : merge;
 }
@@ -193,34 +180,39 @@ __global__ void __launch_bounds__(kThreads, few_blocks(NB))
   constexpr uint32_t kLo = 0x000f000fu, kHi = 0x00f000f0u;
   extern __shared__ __align__(128) uint8_t sm[];
   __shared__ int last_one;
-  const Share share = share_of<ROWS>(b, s, c.causal, w);
+  __shared__ Share share;
+  share_of<ROWS>(b, s, c.causal, w, &share);
   if (blockIdx.x >= share.blocks) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, q4 = lane & 3;
   const int G = s.H / s.KVH, D = s.D;
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(sm) + warp * ST * 2 * TB;
 
   int seq = share.seq;
-  int64_t base = share.base, at = share.begin;
-  Units un = units_of<ROWS>(b, s, seq, c.causal, w.bad);
+  uint32_t base = share.base, at = share.begin;
+  Units un = share.un;
   while (at < share.end) {
     if (at >= base + un.all(s.KVH)) {  // on to the next request with rows, 32 at a time
       base += un.all(s.KVH);
-      for (;;) {
-        const int i = seq + 1 + lane;
-        const bool some = i < b.n_seq && units_of<ROWS>(b, s, min(i, b.n_seq - 1), c.causal, w.bad).row_blocks > 0;
-        const uint32_t any = __ballot_sync(0xffffffffu, some);
+      for (++seq; seq < b.n_seq; seq += 32) {
+        const Units next = units_of<ROWS>(b, s, min(seq + lane, b.n_seq - 1), c.causal, w.bad);
+        const uint32_t any = __ballot_sync(0xffffffffu, seq + lane < b.n_seq && next.row_blocks > 0);
         if (any) {
-          seq += __ffs(any);
+          const int from = __ffs(any) - 1;
+          seq += from;
+          un.q.row0 = __shfl_sync(0xffffffffu, next.q.row0, from);
+          un.q.n = __shfl_sync(0xffffffffu, next.q.n, from);
+          un.q.len = __shfl_sync(0xffffffffu, next.q.len, from);
+          un.row_blocks = __shfl_sync(0xffffffffu, next.row_blocks, from);
+          un.keys = __shfl_sync(0xffffffffu, next.keys, from);
           break;
         }
-        seq += 32;
       }
-      un = units_of<ROWS>(b, s, seq, c.causal, w.bad);
+      if (seq >= b.n_seq) break;
     }
-    const int64_t item = divided(at - base, un.keys), first = base + item * un.keys;
-    const int u0 = (int)(at - first), u1 = (int)min(un.keys, share.end - first);
+    const uint32_t item = (at - base) / un.keys, first = base + item * un.keys;
+    const int u0 = (int)(at - first), u1 = (int)min((uint32_t)un.keys, share.end - first);
     at = first + u1;
-    const int rb = (int)divided(item, s.KVH), kvh = (int)(item - (int64_t)rb * s.KVH), r0 = rb * ROWS;
+    const int rb = (int)item / s.KVH, kvh = (int)item - rb * s.KVH, r0 = rb * ROWS;
     const int rows = min(ROWS, un.q.n * G - r0), len = un.q.len;
     // keys that row x of the block sees
     auto limit = [&](int x) { return c.causal ? len - un.q.n + (r0 + min(x, rows - 1)) / G + 1 : len; };
@@ -272,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, few_blocks(NB))
     }
 
     uint32_t qf[NB][NG][4], qm[NB];
-    float sc[NB][2], step[NB][2];  // a score's factor, and 2^8 in a score's units, of rows 2 q4 and 2 q4 + 1
+    float sc[NB][2], step[NB][2];  // a score's factor, and 2^3 in a score's units, of rows 2 q4 and 2 q4 + 1
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       float top = 0.0f;
@@ -317,12 +309,12 @@ __global__ void __launch_bounds__(kThreads, few_blocks(NB))
       qm[nb] = bits(h);
       sc[nb][0] = __shfl_sync(0xffffffffu, factor, 8 * q4);
       sc[nb][1] = __shfl_sync(0xffffffffu, factor, 8 * q4 + 4);
-      step[nb][0] = 8.0f / sc[nb][0];
-      step[nb][1] = 8.0f / sc[nb][1];
+      step[nb][0] = 3.0f / sc[nb][0];
+      step[nb][1] = 3.0f / sc[nb][1];
     }
 
     // weights are 2^(x sc - from); a score above `past` moves `from`
-    float o[NB][NG][8], from[NB][2], past[NB][2], l[NB][2];
+    float o[NB][NG][8], om[NB][4], from[NB][2], past[NB][2], l[NB][2];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
@@ -330,13 +322,9 @@ __global__ void __launch_bounds__(kThreads, few_blocks(NB))
 #pragma unroll
         for (int i = 0; i < 8; ++i) o[nb][g][i] = 0.0f;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) past[nb][h] = -INFINITY, from[nb][h] = l[nb][h] = 0.0f;
+      for (int h = 0; h < 2; ++h) past[nb][h] = -INFINITY, from[nb][h] = l[nb][h] = om[nb][h] = om[nb][2 + h] = 0.0f;
     }
 
-    const uint32_t i1024 = in_register(0x64006400u), i64 = in_register(0x54005400u);
-    const __half2 c1024 = halves(i1024), c64 = halves(i64);
-    auto low = [&](uint32_t u, __half2 sc, __half2 mi) { return bits(__hfma2(__hsub2(halves(and_or(u, kLo, i1024)), c1024), sc, mi)); };
-    auto high = [&](uint32_t u, __half2 sc, __half2 mi) { return bits(__hfma2(__hsub2(halves(and_or(u, kHi, i64)), c64), sc, mi)); };
     int stage = 0;
     for (int n = 0; n < mine; ++n) {
       asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
@@ -409,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, few_blocks(NB))
         for (int half = 0; half < 2; ++half)
 #pragma unroll
           for (int i = 0; i < 4; ++i) move = move || x[nb][half][i] > past[nb][i & 1];
-      // only when a score passes it by 2^8: a weight is at most 256
+      // only when a score passes it by 2^3: a weight times a scale stays in f16's range
       if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
@@ -424,6 +412,7 @@ __global__ void __launch_bounds__(kThreads, few_blocks(NB))
               from[nb][h] = m;
               past[nb][h] = top + step[nb][h];
               l[nb][h] *= f;
+              om[nb][h] *= f;
 #pragma unroll
               for (int g = 0; g < NG; ++g)
 #pragma unroll
@@ -447,23 +436,27 @@ __global__ void __launch_bounds__(kThreads, few_blocks(NB))
           pf[nb][half][1] = transpose8(bits(__floats2half2_rn(p[2], p[3])));
         }
 
-      // O^T += V^T P^T
+      // O^T += codes^T (weights times scales), and minima (a row for each group) times weights
 #pragma unroll
-      for (int g = 0; g < NG; ++g)
+      for (int half = 0; half < 2; ++half) {
+        const uint8_t *p = tile + half * TB + v_params(NG) + q4 * 16;
+        const uint2 y = r < NG ? *reinterpret_cast<const uint2 *>(p + r * 64 + 8) : make_uint2(0, 0);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
+        for (int nb = 0; nb < NB; ++nb) mma(om[nb], y.x, 0, y.y, 0, pf[nb][half][0], pf[nb][half][1]);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
           const uint2 v = *reinterpret_cast<const uint2 *>(tile + half * TB + v_codes(NG) + g * 256 + lane * 8);
-          const uint4 p = *reinterpret_cast<const uint4 *>(tile + half * TB + v_params(NG) + (g * 4 + q4) * 16);
-          const __half2 s0 = halves(p.x), s1 = halves(p.y), m0 = halves(p.z), m1 = halves(p.w);
+          const uint2 sv = *reinterpret_cast<const uint2 *>(p + g * 64);
           const uint32_t vx = v.x >> 8, vy = v.y >> 8;
-          const uint32_t a0 = low(v.x, s0, m0), a1 = high(v.x, s0, m0), a2 = low(v.y, s1, m1), a3 = high(v.y, s1, m1);
-          const uint32_t b0 = low(vx, s0, m0), b1 = high(vx, s0, m0), b2 = low(vy, s1, m1), b3 = high(vy, s1, m1);
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb) {
-            mma(o[nb][g], a0, a1, a2, a3, pf[nb][half][0], pf[nb][half][1]);
-            mma(o[nb][g] + 4, b0, b1, b2, b3, pf[nb][half][0], pf[nb][half][1]);
+            const uint32_t p0 = bits(__hmul2(halves(pf[nb][half][0]), halves(sv.x)));
+            const uint32_t p1 = bits(__hmul2(halves(pf[nb][half][1]), halves(sv.y)));
+            mma(o[nb][g], v.x & kLo, v.x & kHi, v.y & kLo, v.y & kHi, p0, p1);
+            mma(o[nb][g] + 4, vx & kLo, vx & kHi, vy & kLo, vy & kHi, p0, p1);
           }
         }
+      }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();  // the rings are free
@@ -486,8 +479,13 @@ __global__ void __launch_bounds__(kThreads, few_blocks(NB))
         }
 #pragma unroll
         for (int g = 0; g < NG; ++g)
+        {
+          // codes were c * 2^-24 on rows r of a product, c * 2^-20 on rows r + 8
+          const float least = __shfl_sync(0xffffffffu, om[nb][h], 4 * g + q4);
           *reinterpret_cast<float4 *>(so + x * LD + g * 32 + r * 4) =
-              make_float4(o[nb][g][h], o[nb][g][2 + h], o[nb][g][4 + h], o[nb][g][6 + h]);
+              make_float4(fmaf(o[nb][g][h], 16777216.0f, least), fmaf(o[nb][g][2 + h], 1048576.0f, least),
+                          fmaf(o[nb][g][4 + h], 16777216.0f, least), fmaf(o[nb][g][6 + h], 1048576.0f, least));
+        }
       }
     __syncthreads();
     const bool whole = u0 == 0 && u1 == un.keys;
@@ -530,38 +528,66 @@ __global__ void __launch_bounds__(kThreads, few_blocks(NB))
     }
     if (!whole) {
       // the blocks that hold parts of this item; the last to arrive joins them in their order
-      auto block_of = [&](int64_t unit) { return divided((unit + 1) * share.blocks - 1, share.total); };
-      const int64_t b0 = block_of(first), b1 = block_of(first + un.keys - 1);
+      auto block_of = [&](uint32_t unit) { return (int)((((uint64_t)unit + 1) * share.blocks - 1) / share.total); };
+      const int b0 = block_of(first), parts = block_of(first + un.keys - 1) - b0 + 1;
       __threadfence();
       __syncthreads();
       if (threadIdx.x == 0) {
-        const int arrived = atomicAdd(w.counters + b0, 1);
-        last_one = arrived == (int)(b1 - b0);
+        last_one = atomicAdd(w.counters + b0, 1) == parts - 1;
         if (last_one) w.counters[b0] = 0;
         __threadfence();
       }
       __syncthreads();
       if (last_one) {
-        const int parts = (int)(b1 - b0) + 1;
-        auto part = [&](int p) { return slot_of<ROWS, DP>(w, b0 + p, p == 0 ? 1 : 0); };
-        for (int u = threadIdx.x; u < rows * quads; u += kThreads) {
-          const int x = u / quads, d = u % quads * 4;
-          float M = -INFINITY, L = 0.0f;
-          for (int p = 0; p < parts; ++p) M = fmaxf(M, __ldcg(part(p) + ROWS * DP + x));
-          const float from = M == -INFINITY ? 0.0f : M;
-          float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-          for (int p = 0; p < parts; ++p) {
-            const float *sp = part(p);
-            const float f = ex2(__ldcg(sp + ROWS * DP + x) - from);
-            const float4 y = __ldcg(reinterpret_cast<const float4 *>(sp + x * DP + d));
-            L += f * __ldcg(sp + ROWS * (DP + 1) + x);
-            v.x += f * y.x;
-            v.y += f * y.y;
-            v.z += f * y.z;
-            v.w += f * y.w;
+        // rounds of 64 parts: their m and l come together, then their sums, eight loads in flight
+        constexpr int kRound = 64;
+        float *fm = reinterpret_cast<float *>(sm), *fl = fm + kRound * ROWS;  // [part][row]
+        static_assert(2 * kRound * ROWS * 4 <= few_smem<NG, NB>(), "a round fits the rings");
+        constexpr int PER = (ROWS * (DP / 4) + kThreads - 1) / kThreads;
+        float4 acc[PER];
+        float M[PER], L[PER];
+#pragma unroll
+        for (int k = 0; k < PER; ++k) acc[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f), M[k] = -INFINITY, L[k] = 0.0f;
+        auto slot_at = [&](int p) { return slot_of<ROWS, DP>(w, b0 + p, p == 0 ? 1 : 0); };
+        for (int p0 = 0; p0 < parts; p0 += kRound) {
+          const int n = min(kRound, parts - p0);
+          for (int u = threadIdx.x; u < n * ROWS; u += kThreads) {
+            const float *sp = slot_at(p0 + u / ROWS) + ROWS * DP + u % ROWS;
+            fm[u] = __ldcg(sp);
+            fl[u] = __ldcg(sp + ROWS);
           }
-          finish(x, d, v, M, L);
+          __syncthreads();
+#pragma unroll
+          for (int k = 0; k < PER; ++k) {
+            const int u = threadIdx.x + k * kThreads, x = u / quads, d = u % quads * 4;
+            if (u >= rows * quads) break;
+            float top = M[k];
+            for (int p = 0; p < n; ++p) top = fmaxf(top, fm[p * ROWS + x]);
+            const float ref = top == -INFINITY ? 0.0f : top, f = ex2(M[k] - ref);
+            M[k] = top;
+            L[k] *= f;
+            acc[k].x *= f, acc[k].y *= f, acc[k].z *= f, acc[k].w *= f;
+            for (int q = 0; q < n; q += 8) {
+              float4 y[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                y[i] = q + i < n ? __ldcg(reinterpret_cast<const float4 *>(slot_at(p0 + q + i) + x * DP + d))
+                                 : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                if (q + i >= n) break;
+                const float g = ex2(fm[(q + i) * ROWS + x] - ref);
+                L[k] += g * fl[(q + i) * ROWS + x];
+                acc[k].x += g * y[i].x, acc[k].y += g * y[i].y, acc[k].z += g * y[i].z, acc[k].w += g * y[i].w;
+              }
+            }
+          }
+          __syncthreads();
+        }
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+          const int u = threadIdx.x + k * kThreads;
+          if (u < rows * quads) finish(u / quads, u % quads * 4, acc[k], M[k], L[k]);
         }
       }
     }
@@ -581,7 +607,9 @@ cudaError_t launch_few(const Kv4Shape &s, const Kv4Rows &b, const Kv4AttnCall &c
     if (e == cudaSuccess) ready = dev;
   }
   if (e != cudaSuccess) return e;
-  kernel<<<w.sms * few_blocks(NB), kThreads, smem, st>>>(c, s, b, w);
+  // an item is cut into 128 pieces at most while every request has rows
+  const int64_t most = (int64_t)b.n_seq * s.KVH * 128;
+  kernel<<<(unsigned)std::min<int64_t>(most, (int64_t)w.sms * few_blocks(NB)), kThreads, smem, st>>>(c, s, b, w);
   return cudaGetLastError();
 }
 
