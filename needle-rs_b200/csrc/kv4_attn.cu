@@ -357,25 +357,49 @@ __global__ void __launch_bounds__(kThreads, few_blocks(NB))
           for (int i = 0; i < 4; ++i) x[nb][half][i] *= 3.814697265625e-06f;  // 2^-18
         }
       }
+      // the products of two groups and both tiles side by side: their chains hide each other
+      constexpr int SIDE = NG < 2 ? 1 : 2;
 #pragma unroll
-      for (int g = 0; g < NG; ++g)
+      for (int g0 = 0; g0 < NG; g0 += SIDE) {
+        uint2 k[SIDE][2];
+        float2 p[SIDE][2];
+        float a[SIDE][2][NB][4];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint2 k = *reinterpret_cast<const uint2 *>(tile + half * TB + g * 256 + lane * 8);
-          const float2 p = __half22float2(*reinterpret_cast<const __half2 *>(tile + half * TB + k_params(NG) + (g * 8 + r) * 4));
-          const uint32_t kx = k.x >> 8, ky = k.y >> 8;
+        for (int u = 0; u < SIDE * 2; ++u) {
+          const int g = g0 + u / 2, half = u % 2;
+          if (g >= NG) break;
+          k[u / 2][half] = *reinterpret_cast<const uint2 *>(tile + half * TB + g * 256 + lane * 8);
+          p[u / 2][half] = __half22float2(*reinterpret_cast<const __half2 *>(tile + half * TB + k_params(NG) + (g * 8 + r) * 4));
+        }
+#pragma unroll
+        for (int step = 0; step < 2; ++step)
+#pragma unroll
+          for (int u = 0; u < SIDE * 2; ++u) {
+            const int g = g0 + u / 2, half = u % 2;
+            if (g >= NG) break;
+            const uint32_t x0 = step ? k[u / 2][half].x >> 8 : k[u / 2][half].x, y0 = step ? k[u / 2][half].y >> 8 : k[u / 2][half].y;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+              float *d = a[u / 2][half][nb];
+              if (step == 0) d[0] = d[1] = d[2] = d[3] = 0.0f;
+              mma(d, x0 & kLo, y0 & kLo, x0 & kHi, y0 & kHi, qf[nb][g][2 * step], qf[nb][g][2 * step + 1]);
+            }
+          }
+#pragma unroll
+        for (int u = 0; u < SIDE * 2; ++u) {
+          const int half = u % 2;
+          if (g0 + u / 2 >= NG) break;
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb) {
-            float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            mma(a, k.x & kLo, k.y & kLo, k.x & kHi, k.y & kHi, qf[nb][g][0], qf[nb][g][1]);
-            mma(a, kx & kLo, ky & kLo, kx & kHi, ky & kHi, qf[nb][g][2], qf[nb][g][3]);
             float *y = x[nb][half];
-            y[0] = fmaf(p.x, a[0], y[0]);
-            y[1] = fmaf(p.x, a[1], y[1]);
-            y[2] = fmaf(p.y, a[2], y[2]);
-            y[3] = fmaf(p.y, a[3], y[3]);
+            const float *d = a[u / 2][half][nb];
+            y[0] = fmaf(p[u / 2][half].x, d[0], y[0]);
+            y[1] = fmaf(p[u / 2][half].x, d[1], y[1]);
+            y[2] = fmaf(p[u / 2][half].y, d[2], y[2]);
+            y[3] = fmaf(p[u / 2][half].y, d[3], y[3]);
           }
         }
+      }
       if (j + PAIR > k_all) {
         const int ja = j + 4 * (r >> 1) + (r & 1);  // the token of the matrix's row r; that of r + 8 is 2 on
 #pragma unroll
