@@ -589,8 +589,12 @@ NeedleVerifyPlan *needle_verify_plan_create(size_t vocab, size_t max_seqs, size_
     plan->s = VerifyShape{(int)vocab, dtype};
     plan->max_seqs = max_seqs;
     plan->max_drafts = max_drafts;
-    if (!ok(cudaGetDevice(&plan->device)) || !ok(cudaMalloc(&plan->buf, 256))) return false;
+    plan->work.pieces = verify_pieces(plan->s);
+    const size_t pieces = (max_drafts + max_seqs) * (size_t)plan->work.pieces;
+    if (pieces > kMaxRows) return fail("verification: too many rows of this vocabulary for one plan");
+    if (!ok(cudaGetDevice(&plan->device)) || !ok(cudaMalloc(&plan->buf, 256 + pieces * sizeof(float4)))) return false;
     plan->work.bad = (int *)plan->buf + 1;
+    plan->work.piece = (float4 *)((char *)plan->buf + 256);
     cudaStream_t st = (cudaStream_t)stream;
     return ok(cudaMemsetAsync(plan->buf, 0, 256, st)) && ok(cudaStreamSynchronize(st));
   });

@@ -170,8 +170,11 @@ struct VerifyCall {
   uint32_t flags;
 };
 struct VerifyWork {
-  int *bad;
+  int *bad = nullptr;
+  float4 *piece = nullptr;  // [rows][pieces]: largest logit (NaN: none to be had), sum, its index
+  int pieces = 0;
 };
+int verify_pieces(const VerifyShape &s);
 cudaError_t verify_drafts(const VerifyShape &s, const VerifyCall &c, const VerifyWork &w, cudaStream_t st);
 
 }  // namespace ndl
