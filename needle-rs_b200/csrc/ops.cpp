@@ -583,15 +583,13 @@ NeedleVerifyPlan *needle_verify_plan_create(size_t vocab, size_t max_seqs, size_
   NeedleVerifyPlan *plan = nullptr;
   const bool good = guarded([&] {
     if (!float_type(dtype)) return fail("verification takes f32, f16 or bf16 logits");
-    if (vocab == 0 || vocab > (1u << 24) || max_seqs == 0 || max_seqs > kMaxSeqs || max_drafts > kMaxRows - kMaxSeqs)
+    if (vocab == 0 || vocab > (1u << 24) || max_seqs == 0 || max_seqs > kMaxSeqs || max_drafts > kMaxRows - 2 * kMaxSeqs)
       return fail("invalid verification plan arguments");
     plan = new NeedleVerifyPlan();
     plan->s = VerifyShape{(int)vocab, dtype};
     plan->max_seqs = max_seqs;
     plan->max_drafts = max_drafts;
-    plan->work.pieces = verify_pieces(plan->s);
-    const size_t pieces = (max_drafts + max_seqs) * (size_t)plan->work.pieces;
-    if (pieces > kMaxRows) return fail("verification: too many rows of this vocabulary for one plan");
+    const size_t pieces = (size_t)verify_work_pieces((int64_t)(max_drafts + max_seqs));
     if (!ok(cudaGetDevice(&plan->device)) || !ok(cudaMalloc(&plan->buf, 256 + pieces * sizeof(float4)))) return false;
     plan->work.bad = (int *)plan->buf + 1;
     plan->work.piece = (float4 *)((char *)plan->buf + 256);

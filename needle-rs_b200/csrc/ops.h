@@ -171,10 +171,9 @@ struct VerifyCall {
 };
 struct VerifyWork {
   int *bad = nullptr;
-  float4 *piece = nullptr;  // [rows][pieces]: largest logit (NaN: none to be had), sum, its index
-  int pieces = 0;
+  float4 *piece = nullptr;  // of rows: largest logit (NaN: none to be had), sum, its index
 };
-int verify_pieces(const VerifyShape &s);
+int64_t verify_work_pieces(int64_t rows);
 cudaError_t verify_drafts(const VerifyShape &s, const VerifyCall &c, const VerifyWork &w, cudaStream_t st);
 
 }  // namespace ndl

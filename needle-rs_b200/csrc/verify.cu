@@ -24,7 +24,6 @@ namespace ndl {
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kVectors = 4;  // 16-byte pieces of a row that a thread of the first kernel holds
 constexpr float kLog2e = 1.4426950408889634f;
 // Relative error of a row's sum as the first kernel finds it: a weight's argument t (base 2) is rounded three times
 // (3 |t| 2^-24), where the mean of |t| over a row is at most log2 of its entries (24); its exponential is
@@ -58,7 +57,6 @@ __device__ __forceinline__ float temperature(const VerifyCall &c, int i) {
 
 // 8 bits of a row's mask from entry v on (the row has `words` 64-bit words).
 __device__ __forceinline__ uint32_t mask_bits(const uint64_t *mask, int v, int words) {
-  if (!mask) return 0xffu;
   const int w = v >> 6, o = v & 63;
   uint64_t x = mask[w] >> o;
   if (o > 56 && w + 1 < words) x |= mask[w + 1] << (64 - o);
@@ -90,17 +88,24 @@ struct Row {
   __device__ int units() const { return vectors + 2; }
   __device__ int first(int u) const { return u == 0 ? 0 : lead + (u - 1) * E; }
   __device__ int count(int u) const { return u == 0 ? lead : u <= vectors ? E : V - lead - vectors * E; }
-  __device__ void load(int u, float *x) const {
+  // Their values; entries that are not there or masked: minus infinity.
+  __device__ __forceinline__ void load(int u, float *x) const {
     const int n = count(u), v0 = first(u);
     if (n == E) {
-      const uint4 raw = *reinterpret_cast<const uint4 *>(p + v0);
-      const T *e = reinterpret_cast<const T *>(&raw);
-      const uint32_t open = mask_bits(mask, v0, words);
-#pragma unroll
-      for (int i = 0; i < E; ++i) x[i] = (open >> i) & 1 ? (float)e[i] : -INFINITY;
+      values(*reinterpret_cast<const uint4 *>(p + v0), mask ? mask_bits(mask, v0, words) : 0xffu, x);
     } else {
 #pragma unroll
       for (int i = 0; i < E; ++i) x[i] = i < n ? at(v0 + i) : -INFINITY;
+    }
+  }
+  __device__ __forceinline__ void values(const uint4 &raw, uint32_t open, float *x) const {
+    const T *e = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+    for (int i = 0; i < E; ++i) x[i] = (float)e[i];
+    if (mask) {
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (!((open >> i) & 1)) x[i] = -INFINITY;
     }
   }
 };
@@ -110,62 +115,103 @@ __device__ __forceinline__ void better(float &x, int &i, float y, int j, bool la
   if (y > x || (y == x && (last ? j > i : j < i))) x = y, i = j;
 }
 
+// A block for each piece of a row.  A warp's weights are relative to the
+// largest value that it has met; a turn that passes it rescales the sums and looks for
+// the index, which is rare behind the first few (a maximum for each lane was passed
+// by some lane in nearly every turn: 45 us for 320 rows of 131,072, where this takes 20).
 template <typename T>
-__global__ void __launch_bounds__(kThreads) verify_rows_kernel(VerifyCall c, VerifyShape s, VerifyWork w) {
+__global__ void __launch_bounds__(kThreads) verify_rows_kernel(VerifyCall c, VerifyShape s, VerifyWork w, int pieces) {
   pdl_trigger();
-  constexpr int E = Row<T>::E;
+  constexpr int E = Row<T>::E, AHEAD = 4;
   __shared__ float tops[kWarps], sums[kWarps];
   __shared__ int bests[kWarps], owner;
-  const int64_t row = blockIdx.x / w.pieces;
-  const int piece = (int)(blockIdx.x % w.pieces), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t row = blockIdx.x / pieces;
+  const int piece = (int)(blockIdx.x % pieces), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Row<T> r(c, s, row);
-  // every load at once; the row's request is looked up meanwhile
-  float x[kVectors][E];
-  const int u0 = piece * kThreads * kVectors;
-#pragma unroll
-  for (int k = 0; k < kVectors; ++k) {
-    const int u = u0 + k * kThreads + tid;
-    if (u < r.units()) {
-      r.load(u, x[k]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < E; ++i) x[k][i] = -INFINITY;
-    }
-  }
+  const int u0 = (int)((int64_t)r.units() * piece / pieces), u1 = (int)((int64_t)r.units() * (piece + 1) / pieces);
   if (tid == 0) owner = -1;
   __syncthreads();
   for (int i = tid; i < c.n_seq; i += kThreads) {
     const Request q = request(c, i);
     if (q.ok && row >= (int64_t)q.first + i && row <= (int64_t)q.first + i + q.n) owner = i;
   }
+  __syncthreads();
+  if (owner < 0) return;
   const bool last = c.flags & 1;
+  const float cc = kLog2e / temperature(c, owner);
+  const uint64_t cc2 = f2pack(cc, cc);
   float top = -INFINITY;
   int best = last ? -1 : s.V;
   bool broken = false;
+  uint64_t sum2 = f2pack(0.0f, 0.0f);
+  auto take = [&](const float *x, int v0) {
+    float m = x[0];
 #pragma unroll
-  for (int k = 0; k < kVectors; ++k) {
-    const int u = u0 + k * kThreads + tid, v0 = r.first(u);
+    for (int i = 1; i < E; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(x[i]));
+    broken = broken || !(m < INFINITY);  // NaN or plus infinity
+    if (__any_sync(0xffffffffu, m > top || (last && m == top && m > -INFINITY))) {
+      const float most = warp_max(fmaxf(top, m));
+      int at = 0;
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      broken = broken || !(x[k][i] < INFINITY);  // NaN or plus infinity
-      if (x[k][i] > -INFINITY) better(top, best, x[k][i], v0 + i, last);
+      for (int i = 0; i < E; ++i) {
+        const int k = last ? i : E - 1 - i;  // the last, or the first, of the vector's largest
+        if (x[k] == most) at = k;
+      }
+      // the warp's units come in order: lower lanes have lower indexes
+      const uint32_t here = __ballot_sync(0xffffffffu, m == most);
+      if (here) best = __shfl_sync(0xffffffffu, v0 + at, last ? 31 - __clz(here) : __ffs(here) - 1);
+      const float f = ex2((top - most) * cc);
+      sum2 = fmul2(sum2, f2pack(f, f));
+      top = most;
+    }
+    const float from = top == -INFINITY ? 0.0f : top;
+    const uint64_t from2 = f2pack(from, from);
+#pragma unroll
+    for (int i = 0; i < E; i += 2) {
+      float a, b;
+      f2unpack(fmul2(fsub2(f2pack(x[i], x[i + 1]), from2), cc2), a, b);
+      sum2 = fadd2(sum2, f2pack(ex2(a), ex2(b)));
+    }
+  };
+  for (int turn = u0 + warp * 32; turn < u1; turn += AHEAD * kThreads) {
+    const int u = turn + lane;
+    uint4 raw[AHEAD];
+    uint32_t open[AHEAD];
+    bool whole[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int at = u + k * kThreads;
+      whole[k] = at < u1 && at > 0 && at <= r.vectors;
+      if (whole[k]) {
+        raw[k] = *reinterpret_cast<const uint4 *>(r.p + r.first(at));
+        if (r.mask) open[k] = mask_bits(r.mask, r.first(at), r.words);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int at = u + k * kThreads;
+      float x[E];
+      if (whole[k]) {
+        r.values(raw[k], open[k], x);
+      } else if (at < u1) {
+        r.load(at, x);
+      } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) x[i] = -INFINITY;
+      }
+      __syncwarp();
+      take(x, r.first(at));
     }
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    better(top, best, __shfl_xor_sync(0xffffffffu, top, o), __shfl_xor_sync(0xffffffffu, best, o), last);
+  float lo, hi;
+  f2unpack(sum2, lo, hi);
+  float sum = lo + hi;
+  const float own = top;
   if (lane == 0) tops[warp] = top, bests[warp] = best;
   broken = __syncthreads_or(broken);
-  if (owner < 0) return;
 #pragma unroll
   for (int k = 0; k < kWarps; ++k) better(top, best, tops[k], bests[k], last);
-  const float cc = kLog2e / temperature(c, owner), from = top == -INFINITY ? 0.0f : top;
-  float sum = 0.0f;
-#pragma unroll
-  for (int k = 0; k < kVectors; ++k)
-#pragma unroll
-    for (int i = 0; i < E; ++i) sum += ex2((x[k][i] - from) * cc);
-  sum = warp_sum(sum);
+  sum = warp_sum(own == -INFINITY ? 0.0f : sum * ex2((own - top) * cc));
   if (lane == 0) sums[warp] = sum;
   __syncthreads();
   if (tid == 0) {
@@ -201,7 +247,7 @@ constexpr int kSegments = kCluster * kWarps;
 // The weights of a row's entries: of p (unnormalised), or of max(p - q, 0).
 template <typename T>
 struct Weights {
-  const Row<T> &r;
+  Row<T> r;
   float top, c_hi, c_lo;
   double top64, inv_t, inv_w;  // of the 64-bit form
   float inv_w32;
@@ -217,15 +263,24 @@ struct Weights {
     r.load(u, x);
     const int v0 = r.first(u), n = r.count(u);
     double sum = 0.0;
+    float qs[E];
+    if (rest) {
+      if (n == E && ((uintptr_t)(q + v0) & 15) == 0) {
+#pragma unroll
+        for (int i = 0; i < E; i += 4) *reinterpret_cast<float4 *>(qs + i) = *reinterpret_cast<const float4 *>(q + v0 + i);
+      } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) qs[i] = i < n ? q[v0 + i] : 0.0f;
+      }
+    }
     if (EXACT) {
-#pragma unroll 1
-      for (int i = 0; i < n; ++i) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
         double e = x[i] == -INFINITY ? 0.0 : exp(((double)x[i] - top64) * inv_t);
-        if (rest) e = fmax(e * inv_w - (double)q[v0 + i], 0.0);
+        if (rest) e = i < n ? fmax(e * inv_w - (double)qs[i], 0.0) : 0.0;
         if (v0 + i == hole) e = 0.0;
         sum += y[i] = e;
       }
-      for (int i = n; i < E; ++i) y[i] = 0.0;
       return sum;
     }
     float part = 0.0f;
@@ -236,7 +291,7 @@ struct Weights {
       const float a = d * c_hi, b = fmaf(d, c_hi, -a) + fmaf(rest_d, c_hi, d * c_lo);
       float e = ex2(a);
       e = x[i] == -INFINITY ? 0.0f : fmaf(e, b * 0.6931471805599453f, e);
-      if (rest) e = i < n ? fmaxf(fmaf(e, inv_w32, -q[v0 + i]), 0.0f) : 0.0f;
+      if (rest) e = i < n ? fmaxf(fmaf(e, inv_w32, -qs[i]), 0.0f) : 0.0f;
       if (v0 + i == hole) e = 0.0f;
       part += e;
       y[i] = e;
@@ -247,97 +302,128 @@ struct Weights {
 
 struct Shared {
   double seg[2][kSegments];  // sums of the segments, of two turns
-  double top_of[kWarps];
-  int token, sure;
-  double logp;
+  double part[kWarps];       // of a segment's eighths
+  double answer;
+  int sure;
 };
 
+// Where a cumulative sum of 64 numbers (lane l has the 2l-th and the next) passes `want`: the number's index
+// and the sum before it; the last one above zero where rounding leaves none.
+struct Place {
+  int at;
+  double before, total;
+  bool passed;
+};
+__device__ __forceinline__ Place place_in(double a, double b, double want) {
+  const int lane = threadIdx.x & 31;
+  double upto = a + b;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double x = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += x;
+  }
+  const double before = upto - (a + b);
+  const bool pa = a > 0.0 && before + a > want, pb = b > 0.0 && upto > want;
+  const uint32_t passed = __ballot_sync(0xffffffffu, pa || pb), some = __ballot_sync(0xffffffffu, a > 0.0 || b > 0.0);
+  Place r;
+  r.total = __shfl_sync(0xffffffffu, upto, 31);
+  r.passed = passed != 0;
+  const int from = passed ? __ffs(passed) - 1 : some ? 31 - __clz(some) : -1;
+  const bool second = passed ? !pa : b > 0.0;
+  r.at = from < 0 ? -1 : __shfl_sync(0xffffffffu, 2 * lane + (second ? 1 : 0), max(from, 0));
+  r.before = __shfl_sync(0xffffffffu, second ? before + a : before, max(from, 0));
+  return r;
+}
+
+__device__ __forceinline__ double warp_sum64(double x) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+
 // Sums of the cluster's segments of a row (a warp's units lie side by side), in
-// their order, into sm.seg[turn]; returns the total.
+// their order, into sm.seg[turn] of every block; returns the total.
 template <bool EXACT, typename T>
-__device__ double segment_sums(const Weights<T> &w, Shared &sm, int turn) {
+__device__ __noinline__ double segment_sums(const Weights<T> w, Shared &sm, int turn) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, size = (int)cluster_size(), me = (int)cluster_rank();
   const int segments = size * kWarps, seg = me * kWarps + warp, units = w.r.units();
   const int u0 = (int)((int64_t)units * seg / segments), u1 = (int)((int64_t)units * (seg + 1) / segments);
   double sum = 0.0, y[Row<T>::E];
-#pragma unroll 2
+#pragma unroll (EXACT ? 1 : 4)
   for (int u = u0 + lane; u < u1; u += 32) sum += w.template unit<EXACT>(u, y);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  sum = warp_sum64(sum);
   if (lane < size) store_there(&sm.seg[turn][seg], (uint32_t)lane, sum);
   cluster_meet();
-  double total = 0.0;
-  for (int k = 0; k < segments; ++k) total += sm.seg[turn][k];
-  return total;
+  const double a = 2 * lane < segments ? sm.seg[turn][2 * lane] : 0.0, b = 2 * lane < segments ? sm.seg[turn][2 * lane + 1] : 0.0;
+  return warp_sum64(a + b);
 }
 
 // The first entry at which the sum of the weights passes `want` (the last of
-// any weight, if rounding leaves none), by the warp whose segment it is; the
-// others learn nothing.  `off`: how far the sums may be off; *sure: the entry is further than that from
+// any weight, if rounding leaves none), by one warp of the block whose segment it is; -1 for the
+// others.  `off`: how far the sums may be off; *sure: the entry is further than that from
 // its borders.
 template <bool EXACT, typename T>
-__device__ void find(const Weights<T> &w, Shared &sm, int turn, double want, double off, int *token, bool *sure) {
+__device__ __noinline__ int find(const Weights<T> w, Shared &sm, int turn, double want, double off, bool *sure) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, size = (int)cluster_size(), me = (int)cluster_rank();
   const int segments = size * kWarps, units = w.r.units();
-  int seg = -1, some = -1;
-  double before = 0.0;
-  for (int k = 0; k < segments && seg < 0; ++k) {
-    const double x = sm.seg[turn][k];
-    if (x > 0.0) some = k;
-    if (x > 0.0 && before + x > want) seg = k;
-    else before += x;
-  }
-  *token = -1;
-  *sure = true;
-  if (seg < 0) {
-    seg = some;  // rounding: the last entry of the last segment of any weight
-    before = want;
-    *sure = false;
-  }
-  if (seg != me * kWarps + warp) return;
-  const int u0 = (int)((int64_t)units * seg / segments), u1 = (int)((int64_t)units * (seg + 1) / segments);
+  const bool some = 2 * lane < segments;
+  Place p = place_in(some ? sm.seg[turn][2 * lane] : 0.0, some ? sm.seg[turn][2 * lane + 1] : 0.0, want);
+  *sure = false;
+  if (p.at < 0 || p.at / kWarps != me) return -1;
+  // the block's warps take an eighth of the segment each, then one of them that eighth
+  const int s0 = (int)((int64_t)units * p.at / segments), s1 = (int)((int64_t)units * (p.at + 1) / segments);
+  auto border = [&](int k) { return s0 + (int)((int64_t)(s1 - s0) * k / kWarps); };
+  double sum = 0.0, y[Row<T>::E];
+  for (int u = border(warp) + lane; u < border(warp + 1); u += 32) sum += w.template unit<EXACT>(u, y);
+  sum = warp_sum64(sum);
+  if (lane == 0) sm.part[warp] = sum;
+  __syncthreads();
+  double before = p.passed ? p.before : want;
+  bool passed = p.passed;
+  p = place_in(2 * lane < kWarps ? sm.part[2 * lane] : 0.0, 2 * lane < kWarps ? sm.part[2 * lane + 1] : 0.0, want - before);
+  passed = passed && p.passed;
+  if (p.at != warp) return -1;
+  before += p.before;
   int last = -1;
-  for (int a = u0; a < u1; a += 32) {
+  for (int a = border(warp); a < border(warp + 1); a += 32) {
     constexpr int E = Row<T>::E;
     const int u = a + lane;
-    double y[E], own = u < u1 ? w.template unit<EXACT>(u, y) : 0.0, upto = own;
+    const double own = u < border(warp + 1) ? w.template unit<EXACT>(u, y) : 0.0;
+    double upto = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const double x = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += x;
     }
-    const uint32_t some = __ballot_sync(0xffffffffu, own > 0.0), here = __ballot_sync(0xffffffffu, own > 0.0 && before + upto > want);
-    const int from = here ? __ffs(here) - 1 : some ? 31 - __clz(some) : -1;
-    int pick = -1;
-    bool fine = false;
-    if (lane == from) {
-      double at = before + upto - own;
-#pragma unroll
-      for (int i = 0; i < E; ++i) {
-        if (!(y[i] > 0.0) || (here && pick >= 0 && at > want)) continue;
-        fine = want >= at + off && want < at + y[i] - off;
-        at += y[i];
-        pick = w.r.first(u) + i;
-      }
-    }
+    const uint32_t any = __ballot_sync(0xffffffffu, own > 0.0);
+    const uint32_t here = __ballot_sync(0xffffffffu, passed && own > 0.0 && before + upto > want);
+    const int from = here ? __ffs(here) - 1 : any ? 31 - __clz(any) : -1;
     if (from >= 0) {
-      pick = __shfl_sync(0xffffffffu, pick, from);
-      fine = __shfl_sync(0xffffffffu, (int)fine, from);
-      last = pick;
+      int pick = -1;
+      bool fine = false;
+      if (lane == from) {
+        double at = before + upto - own;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          if (!(y[i] > 0.0) || (here && pick >= 0 && at > want)) continue;
+          fine = want >= at + off && want < at + y[i] - off;
+          at += y[i];
+          pick = w.r.first(u) + i;
+        }
+      }
+      last = __shfl_sync(0xffffffffu, pick, from);
       if (here) {
-        *token = pick;
-        *sure = *sure && fine;
-        return;
+        *sure = __shfl_sync(0xffffffffu, (int)fine, from);
+        return last;
       }
     }
     before += __shfl_sync(0xffffffffu, upto, 31);
   }
-  *token = last;
-  *sure = false;
+  return last;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) verify_pick_kernel(VerifyCall c, VerifyShape s, VerifyWork w) {
+__global__ void __launch_bounds__(kThreads, 3) verify_pick_kernel(VerifyCall c, VerifyShape s, VerifyWork w, int pieces) {
   __shared__ Shared sm;
   __shared__ float tops[kThreads], sums[kThreads];
   __shared__ int bests[kThreads], found;
@@ -370,11 +456,11 @@ __global__ void __launch_bounds__(kThreads) verify_pick_kernel(VerifyCall c, Ver
   for (int base = 0; len < 0; base += kThreads) {
     const int rows = min(kThreads, rq.n + 1 - base);
     for (int j = warp; j < rows; j += kWarps) {
-      const float4 *p = w.piece + ((int64_t)rq.first + i + base + j) * w.pieces;
+      const float4 *p = w.piece + ((int64_t)rq.first + i + base + j) * pieces;
       float top = -INFINITY, sum = 0.0f;
       int best = last ? -1 : s.V;
       bool broken = false;
-      for (int k = lane; k < w.pieces; k += 32) {
+      for (int k = lane; k < pieces; k += 32) {
         const float4 x = p[k];
         broken = broken || x.x != x.x;
         better(top, best, x.x, __float_as_int(x.z), last);
@@ -384,7 +470,7 @@ __global__ void __launch_bounds__(kThreads) verify_pick_kernel(VerifyCall c, Ver
         better(top, best, __shfl_xor_sync(0xffffffffu, top, o), __shfl_xor_sync(0xffffffffu, best, o), last);
       const float cc = kLog2e / temp;
       if (top > -INFINITY)
-        for (int k = lane; k < w.pieces; k += 32) {
+        for (int k = lane; k < pieces; k += 32) {
           const float4 x = p[k];
           sum += x.y * ex2((x.x - top) * cc);
         }
@@ -480,7 +566,7 @@ __global__ void __launch_bounds__(kThreads) verify_pick_kernel(VerifyCall c, Ver
       for (int exact = 0; exact < 2; ++exact) {
         wt.rest = false;
         wt.hole = -1;
-        if (tid == 0) sm.top_of[0] = 0.0;
+        if (tid == 0) sm.answer = 0.0;
         W = exact ? segment_sums<true>(wt, sm, 0) : segment_sums<false>(wt, sm, 0);
         double total = W, off = exact ? 0.0 : 2.0 * kDraw * W;
         int turn = 0;
@@ -504,14 +590,13 @@ __global__ void __launch_bounds__(kThreads) verify_pick_kernel(VerifyCall c, Ver
             wt.hole = -1;
           }
         }
-        if (exact) find<true>(wt, sm, turn, u * total, 0.0, &pick, &sure);
-        else find<false>(wt, sm, turn, u * total, off, &pick, &sure);
+        pick = exact ? find<true>(wt, sm, turn, u * total, 0.0, &sure) : find<false>(wt, sm, turn, u * total, off, &sure);
         mine = pick >= 0 && lane == 0;
         if (exact) break;
         // one warp of the cluster knows: it tells all
-        if (pick >= 0 && lane < size) store_there(&sm.top_of[0], (uint32_t)lane, sure && !close ? 1.0 : 0.0);
+        if (pick >= 0 && lane < size) store_there(&sm.answer, (uint32_t)lane, sure && !close ? 1.0 : 0.0);
         cluster_meet();
-        const bool good = sm.top_of[0] == 1.0;
+        const bool good = sm.answer == 1.0;
         cluster_meet();  // sm.seg and the answer may be written again
         if (good) break;
         mine = false;
@@ -531,10 +616,18 @@ __global__ void __launch_bounds__(kThreads) verify_pick_kernel(VerifyCall c, Ver
   if (me == 0 && tid == 0) c.out_len[i] = (uint32_t)len;
 }
 
+// Pieces of a row: enough for some turns of the device's blocks, of two vectors a thread or more.
+constexpr int64_t kBlocks = 4096;
+int verify_pieces(const VerifyShape &s, int64_t rows) {
+  const int64_t most = (s.V / (s.dtype == DT_F32 ? 4 : 8) + 2 + 2 * kThreads - 1) / (2 * kThreads);
+  return (int)std::max<int64_t>(1, std::min(most, (kBlocks + rows - 1) / rows));
+}
+
 template <typename T>
 cudaError_t run(const VerifyShape &s, const VerifyCall &c, const VerifyWork &w, cudaStream_t st) {
   const int64_t rows = (int64_t)c.n_drafts + c.n_seq;
-  verify_rows_kernel<T><<<(unsigned)(rows * w.pieces), kThreads, 0, st>>>(c, s, w);
+  const int pieces = verify_pieces(s, rows);
+  verify_rows_kernel<T><<<(unsigned)(rows * pieces), kThreads, 0, st>>>(c, s, w, pieces);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   const int size = s.V <= 4096 ? 1 : s.V <= 16384 ? 2 : kCluster;
@@ -550,16 +643,12 @@ cudaError_t run(const VerifyShape &s, const VerifyCall &c, const VerifyWork &w, 
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, verify_pick_kernel<T>, c, s, w);
+  return cudaLaunchKernelEx(&cfg, verify_pick_kernel<T>, c, s, w, pieces);
 }
 
 }  // namespace
 
-// A row's units (vectors and two ends) over those of a block.
-int verify_pieces(const VerifyShape &s) {
-  const int e = s.dtype == DT_F32 ? 4 : 8;
-  return (s.V / e + 2 + kThreads * kVectors - 1) / (kThreads * kVectors);
-}
+int64_t verify_work_pieces(int64_t rows) { return rows + kBlocks; }
 
 cudaError_t verify_drafts(const VerifyShape &s, const VerifyCall &c, const VerifyWork &w, cudaStream_t st) {
   if (s.dtype == DT_F32) return run<float>(s, c, w, st);
