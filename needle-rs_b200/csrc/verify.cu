@@ -6,11 +6,11 @@
 // takes drafts while u q < p, and draws the token behind them.
 //
 // The definition is in 64 bits: a token is where a cumulative sum passes a
-// random number.  Both kernels work in f32 and know how far they may be off
-// (kAccept, kDraw below); where a comparison falls within that bound, the cluster repeats
-// the row with 64-bit exponentials (about one draw in ten over 131,072 entries, next to
-// no draft), so that results are those of the definition.  All draws in 64 bits take twice
-// the time of the second kernel.
+// random number, and over 131,072 entries two neighbouring borders are often closer
+// than sums of f32 exponentials are sure to be (a first pass in f32 left four draws in
+// ten to be repeated: 280 us for the second kernel on 256 requests).  Draws therefore take 64-bit exponentials, by a
+// table and a short polynomial.  A draft's test needs the row's sum alone: f32, and in 64 bits
+// where u q is within the f32 sum's error of p.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -29,8 +29,6 @@ constexpr float kLog2e = 1.4426950408889634f;
 // (3 |t| 2^-24), where the mean of |t| over a row is at most log2 of its entries (24); its exponential is
 // off by 2^-22, the sum by a few units.
 constexpr double kAccept = 1e-5;
-// The same in the second kernel, which carries what the argument's roundings leave out: an exponential's 2^-22 and a few units.
-constexpr double kDraw = 5e-7;
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -244,27 +242,49 @@ __device__ __forceinline__ void store_there(double *p, uint32_t rank, double v) 
 constexpr int kCluster = 8;  // blocks of a request, at most
 constexpr int kSegments = kCluster * kWarps;
 
-// The weights of a row's entries: of p (unnormalised), or of max(p - q, 0).
+// 2^(t / 128) for t <= 0 (minus infinity: 0) in 64 bits: 128 values in a table, and a polynomial of degree 4
+// on the rest, at most 1/256 of a binary order away (the Taylor series of the exponential: its next term is below
+// 2e-15); the method is P. Tang's (table-driven exponentials, 1989).
+constexpr int kTable = 128;
+__device__ __forceinline__ double exp2_table(double t, const double *table) {
+  const double magic = 6755399441055744.0;  // 1.5 * 2^52: a sum with it holds round(t) in the low bits
+  const double big = fmax(t, -128.0 * 1000.0) + magic;
+  const int n = __double2loint(big);
+  const double r = t - (big - magic), h = 0.6931471805599453094 / kTable;
+  double y = fma(r, h * h * h * h / 24.0, h * h * h / 6.0);
+  y = fma(y, r, h * h / 2.0);
+  y = fma(y, r, h);
+  y = fma(y, r, 1.0) * table[n & (kTable - 1)];
+  const double e = __hiloint2double(__double2hiint(y) + ((n >> 7) << 20), __double2loint(y));
+  return t < -128.0 * 1000.0 ? 0.0 : e;
+}
+// An f32 number in 64 bits without the conversion unit; zeros and subnormals become 2^-127 (nothing beside a logit
+// or a probability).
+__device__ __forceinline__ double widened(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + 0x38000000u)), (int)(b << 29));
+}
+
+// The weights of a row's entries: of p (times its sum), or of max(p - q, 0).
 template <typename T>
 struct Weights {
   Row<T> r;
-  float top, c_hi, c_lo;
-  double top64, inv_t, inv_w;  // of the 64-bit form
-  float inv_w32;
-  const float *q;  // NULL: none
+  double scale, shift;  // a weight is 2^((x scale - shift) / 128)
+  double inv_w;
+  const float *q;  // NULL: weights of p
   int hole;        // an entry of weight zero, or -1
-  bool rest;       // max(p - q, 0)
 
-  // Weights of unit u's entries in 32 or 64 bits; returns their sum.
-  template <bool EXACT>
-  __device__ __forceinline__ double unit(int u, double *y) const {
+  __device__ Weights(const Row<T> &row, float top, double inv_t) : r(row), inv_w(0.0), q(nullptr), hole(-1) {
+    scale = 1.4426950408889634074 * kTable * inv_t;
+    shift = (double)top * scale;
+  }
+  // Weights of unit u's entries; returns their sum.
+  __device__ __forceinline__ double unit(int u, double *y, const double *table) const {
     constexpr int E = Row<T>::E;
-    float x[E];
+    float x[E], qs[E];
     r.load(u, x);
     const int v0 = r.first(u), n = r.count(u);
-    double sum = 0.0;
-    float qs[E];
-    if (rest) {
+    if (q) {
       if (n == E && ((uintptr_t)(q + v0) & 15) == 0) {
 #pragma unroll
         for (int i = 0; i < E; i += 4) *reinterpret_cast<float4 *>(qs + i) = *reinterpret_cast<const float4 *>(q + v0 + i);
@@ -273,38 +293,23 @@ struct Weights {
         for (int i = 0; i < E; ++i) qs[i] = i < n ? q[v0 + i] : 0.0f;
       }
     }
-    if (EXACT) {
-#pragma unroll
-      for (int i = 0; i < E; ++i) {
-        double e = x[i] == -INFINITY ? 0.0 : exp(((double)x[i] - top64) * inv_t);
-        if (rest) e = i < n ? fmax(e * inv_w - (double)qs[i], 0.0) : 0.0;
-        if (v0 + i == hole) e = 0.0;
-        sum += y[i] = e;
-      }
-      return sum;
-    }
-    float part = 0.0f;
+    double sum = 0.0;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      // (x - top) * c as a sum of two f32: 2^(a + b) = 2^a (1 + b ln 2)
-      const float d = x[i] - top, back = x[i] - d, rest_d = (x[i] - (d + back)) + (back - top);
-      const float a = d * c_hi, b = fmaf(d, c_hi, -a) + fmaf(rest_d, c_hi, d * c_lo);
-      float e = ex2(a);
-      e = x[i] == -INFINITY ? 0.0f : fmaf(e, b * 0.6931471805599453f, e);
-      if (rest) e = i < n ? fmaxf(fmaf(e, inv_w32, -qs[i]), 0.0f) : 0.0f;
-      if (v0 + i == hole) e = 0.0f;
-      part += e;
-      y[i] = e;
+      double e = exp2_table(fma(widened(x[i]), scale, -shift), table);
+      if (x[i] == -INFINITY || v0 + i == hole) e = 0.0;
+      if (q) e = fmax(fma(e, inv_w, -widened(qs[i])), 0.0);
+      sum += y[i] = e;
     }
-    return (double)part;
+    return sum;
   }
 };
 
 struct Shared {
   double seg[2][kSegments];  // sums of the segments, of two turns
   double part[kWarps];       // of a segment's eighths
-  double answer;
-  int sure;
+  double table[kTable];      // 2^(i / 128)
+  int verdict;
 };
 
 // Where a cumulative sum of 64 numbers (lane l has the 2l-th and the next) passes `want`: the number's index
@@ -343,14 +348,14 @@ __device__ __forceinline__ double warp_sum64(double x) {
 
 // Sums of the cluster's segments of a row (a warp's units lie side by side), in
 // their order, into sm.seg[turn] of every block; returns the total.
-template <bool EXACT, typename T>
+template <typename T>
 __device__ __noinline__ double segment_sums(const Weights<T> w, Shared &sm, int turn) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, size = (int)cluster_size(), me = (int)cluster_rank();
   const int segments = size * kWarps, seg = me * kWarps + warp, units = w.r.units();
   const int u0 = (int)((int64_t)units * seg / segments), u1 = (int)((int64_t)units * (seg + 1) / segments);
   double sum = 0.0, y[Row<T>::E];
-#pragma unroll (EXACT ? 1 : 4)
-  for (int u = u0 + lane; u < u1; u += 32) sum += w.template unit<EXACT>(u, y);
+#pragma unroll 2
+  for (int u = u0 + lane; u < u1; u += 32) sum += w.unit(u, y, sm.table);
   sum = warp_sum64(sum);
   if (lane < size) store_there(&sm.seg[turn][seg], (uint32_t)lane, sum);
   cluster_meet();
@@ -359,28 +364,27 @@ __device__ __noinline__ double segment_sums(const Weights<T> w, Shared &sm, int 
 }
 
 // The first entry at which the sum of the weights passes `want` (the last of
-// any weight, if rounding leaves none), by one warp of the block whose segment it is; -1 for the
-// others.  `off`: how far the sums may be off; *sure: the entry is further than that from
-// its borders.
-template <bool EXACT, typename T>
-__device__ __noinline__ int find(const Weights<T> w, Shared &sm, int turn, double want, double off, bool *sure) {
+// any weight, if rounding leaves none), by one warp of the block whose segment it
+// is; -1 for the others.
+template <typename T>
+__device__ __noinline__ int find(const Weights<T> w, Shared &sm, int turn, double want) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, size = (int)cluster_size(), me = (int)cluster_rank();
   const int segments = size * kWarps, units = w.r.units();
   const bool some = 2 * lane < segments;
   Place p = place_in(some ? sm.seg[turn][2 * lane] : 0.0, some ? sm.seg[turn][2 * lane + 1] : 0.0, want);
-  *sure = false;
   if (p.at < 0 || p.at / kWarps != me) return -1;
   // the block's warps take an eighth of the segment each, then one of them that eighth
   const int s0 = (int)((int64_t)units * p.at / segments), s1 = (int)((int64_t)units * (p.at + 1) / segments);
   auto border = [&](int k) { return s0 + (int)((int64_t)(s1 - s0) * k / kWarps); };
   double sum = 0.0, y[Row<T>::E];
-  for (int u = border(warp) + lane; u < border(warp + 1); u += 32) sum += w.template unit<EXACT>(u, y);
+  for (int u = border(warp) + lane; u < border(warp + 1); u += 32) sum += w.unit(u, y, sm.table);
   sum = warp_sum64(sum);
   if (lane == 0) sm.part[warp] = sum;
   __syncthreads();
-  double before = p.passed ? p.before : want;
+  double before = p.before;
   bool passed = p.passed;
-  p = place_in(2 * lane < kWarps ? sm.part[2 * lane] : 0.0, 2 * lane < kWarps ? sm.part[2 * lane + 1] : 0.0, want - before);
+  p = place_in(2 * lane < kWarps ? sm.part[2 * lane] : 0.0, 2 * lane < kWarps ? sm.part[2 * lane + 1] : 0.0,
+               passed ? want - before : INFINITY);
   passed = passed && p.passed;
   if (p.at != warp) return -1;
   before += p.before;
@@ -388,7 +392,7 @@ __device__ __noinline__ int find(const Weights<T> w, Shared &sm, int turn, doubl
   for (int a = border(warp); a < border(warp + 1); a += 32) {
     constexpr int E = Row<T>::E;
     const int u = a + lane;
-    const double own = u < border(warp + 1) ? w.template unit<EXACT>(u, y) : 0.0;
+    const double own = u < border(warp + 1) ? w.unit(u, y, sm.table) : 0.0;
     double upto = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -400,22 +404,17 @@ __device__ __noinline__ int find(const Weights<T> w, Shared &sm, int turn, doubl
     const int from = here ? __ffs(here) - 1 : any ? 31 - __clz(any) : -1;
     if (from >= 0) {
       int pick = -1;
-      bool fine = false;
       if (lane == from) {
         double at = before + upto - own;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
           if (!(y[i] > 0.0) || (here && pick >= 0 && at > want)) continue;
-          fine = want >= at + off && want < at + y[i] - off;
           at += y[i];
           pick = w.r.first(u) + i;
         }
       }
       last = __shfl_sync(0xffffffffu, pick, from);
-      if (here) {
-        *sure = __shfl_sync(0xffffffffu, (int)fine, from);
-        return last;
-      }
+      if (here) return last;
     }
     before += __shfl_sync(0xffffffffu, upto, 31);
   }
@@ -441,6 +440,7 @@ __global__ void __launch_bounds__(kThreads, 3) verify_pick_kernel(VerifyCall c, 
     if (me == 0 && tid == 0) *w.bad = 1, c.out_len[i] = 0;
     return;
   }
+  for (int k = tid; k < kTable; k += kThreads) sm.table[k] = exp2((double)k / kTable);
   const bool greedy = is_greedy(c, i), last = c.flags & 1;
   const float temp = temperature(c, i);
   const double inv_t = 1.0 / (double)temp;
@@ -451,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, 3) verify_pick_kernel(VerifyCall c, 
   int taken = 0;           // drafts taken before this round
   int len = -1;            // tokens, when the request has ended
   uint32_t token = 0xffffffffu;
-  float row_top = 0.0f;
+  float row_top = 0.0f, row_sum = 0.0f;
   bool draw = false;
   for (int base = 0; len < 0; base += kThreads) {
     const int rows = min(kThreads, rq.n + 1 - base);
@@ -516,12 +516,11 @@ __global__ void __launch_bounds__(kThreads, 3) verify_pick_kernel(VerifyCall c, 
     // drafts too close to tell, in order: the row's sum in 64 bits
     for (;;) {
       const int f = found;
-      if (tid == f && f < rows) sm.sure = verdict;
+      if (tid == f && f < rows) sm.verdict = verdict;
       __syncthreads();
-      if (f >= rows || sm.sure != 2) break;
+      if (f >= rows || sm.verdict != 2) break;
       const Row<T> r(c, s, (int64_t)rq.first + i + base + f);
-      Weights<T> wt{r, 0.0f, 0.0f, 0.0f, (double)tops[f], inv_t, 0.0, 0.0f, nullptr, -1, false};
-      const double W = segment_sums<true>(wt, sm, 0);
+      const double W = segment_sums(Weights<T>(r, tops[f], inv_t), sm, 0);
       if (tid == 0) found = rows;
       __syncthreads();
       if (tid == f) {
@@ -539,9 +538,10 @@ __global__ void __launch_bounds__(kThreads, 3) verify_pick_kernel(VerifyCall c, 
     if (f < rows) {
       taken = base + f;
       row_top = tops[f];
+      row_sum = sums[f];
       token = (uint32_t)bests[f];
-      len = sm.sure == 3 ? taken : taken + 1;
-      draw = sm.sure != 3;
+      len = sm.verdict == 3 ? taken : taken + 1;
+      draw = sm.verdict != 3;
     }
     __syncthreads();
   }
@@ -549,59 +549,41 @@ __global__ void __launch_bounds__(kThreads, 3) verify_pick_kernel(VerifyCall c, 
   // the token behind the drafts
   if (draw) {
     const Row<T> r(c, s, (int64_t)rq.first + i + taken);
-    const bool replaced = taken < rq.n;
-    const int t = rq.first + taken;
-    const double c64 = 1.4426950408889634074 * inv_t;
-    Weights<T> wt{r, row_top, (float)c64, (float)(c64 - (double)(float)c64), (double)row_top, inv_t, 0.0, 0.0f, nullptr, -1, false};
-    double W = 0.0;
-    bool mine = false;
-    if (greedy) {
-      if (logp) W = segment_sums<false>(wt, sm, 0);
-      mine = me == 0 && tid == 0;
-    } else {
-      const double u = (double)c.final_u[i];
-      int pick = -1;
-      bool sure = true;
-      // in f32; again in 64 bits if that is too close to tell
-      for (int exact = 0; exact < 2; ++exact) {
-        wt.rest = false;
-        wt.hole = -1;
-        if (tid == 0) sm.answer = 0.0;
-        W = exact ? segment_sums<true>(wt, sm, 0) : segment_sums<false>(wt, sm, 0);
-        double total = W, off = exact ? 0.0 : 2.0 * kDraw * W;
-        int turn = 0;
-        bool close = false;
-        if (replaced) {
-          wt.rest = probs != nullptr;
-          wt.q = probs ? probs + (int64_t)t * c.ldp : nullptr;
-          wt.inv_w = 1.0 / W;
-          wt.inv_w32 = (float)wt.inv_w;
-          const uint32_t d = c.ids[t];
-          wt.hole = probs ? -1 : d < (uint32_t)s.V ? (int)d : -1;
-          const double left = exact ? segment_sums<true>(wt, sm, 1) : segment_sums<false>(wt, sm, 1);
-          const double bound = probs ? 4.0 * kDraw : 2.0 * kDraw * W;  // p has the error of W as well
-          close = !exact && left <= 2.0 * bound;
-          if (left > 0.0) {
-            turn = 1;
-            total = left;
-            off = exact ? 0.0 : bound;
-          } else {  // nothing left over: p itself
-            wt.rest = false;
+    double W = (double)row_sum;
+    bool mine = me == 0 && tid == 0;
+    if (!greedy) {
+      Weights<T> wt(r, row_top, inv_t);
+      const int t = rq.first + taken;
+      int turn = 0;
+      double total;
+      if (taken < rq.n && probs) {  // a replaced draft: of what p has more than q
+        W = segment_sums(wt, sm, 0);
+        wt.q = probs + (int64_t)t * c.ldp;
+        wt.inv_w = 1.0 / W;
+        total = segment_sums(wt, sm, 1);
+        turn = 1;
+        if (!(total > 0.0)) {  // nothing: of p itself
+          wt.q = nullptr;
+          total = W;
+          turn = 0;
+        }
+      } else {
+        const uint32_t d = taken < rq.n ? c.ids[t] : 0xffffffffu;
+        wt.hole = d < (uint32_t)s.V ? (int)d : -1;
+        total = W = segment_sums(wt, sm, 0);
+        if (wt.hole >= 0) {
+          const float x = r.at(wt.hole);
+          if (x > -INFINITY) W += exp(((double)x - (double)row_top) * inv_t);
+          if (!(total > 0.0)) {  // the draft has all of the row's weight
             wt.hole = -1;
+            total = segment_sums(wt, sm, 1);
+            turn = 1;
           }
         }
-        pick = exact ? find<true>(wt, sm, turn, u * total, 0.0, &sure) : find<false>(wt, sm, turn, u * total, off, &sure);
-        mine = pick >= 0 && lane == 0;
-        if (exact) break;
-        // one warp of the cluster knows: it tells all
-        if (pick >= 0 && lane < size) store_there(&sm.answer, (uint32_t)lane, sure && !close ? 1.0 : 0.0);
-        cluster_meet();
-        const bool good = sm.answer == 1.0;
-        cluster_meet();  // sm.seg and the answer may be written again
-        if (good) break;
-        mine = false;
       }
+      const int pick = find(wt, sm, turn, (double)c.final_u[i] * total);
       token = (uint32_t)pick;
+      mine = pick >= 0 && lane == 0;
     }
     if (mine) {
       out[taken] = token;
@@ -630,7 +612,12 @@ cudaError_t run(const VerifyShape &s, const VerifyCall &c, const VerifyWork &w, 
   verify_rows_kernel<T><<<(unsigned)(rows * pieces), kThreads, 0, st>>>(c, s, w, pieces);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  const int size = s.V <= 4096 ? 1 : s.V <= 16384 ? 2 : kCluster;
+  // blocks of a request: as many as are on the device at once, 2048 entries each or more
+  int dev = 0, sms = 0, size = 1;
+  e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return e;
+  while (size < kCluster && (int64_t)c.n_seq * size * 2 <= 3 * sms && size * 4096 <= s.V) size *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(c.n_seq * size));
   cfg.blockDim = dim3(kThreads);
