@@ -171,39 +171,48 @@ __global__ void __launch_bounds__(kThreads) verify_rows_kernel(VerifyCall c, Ver
       sum2 = fadd2(sum2, f2pack(ex2(a), ex2(b)));
     }
   };
-  for (int turn = u0 + warp * 32; turn < u1; turn += AHEAD * kThreads) {
-    const int u = turn + lane;
+  const int v0 = max(u0, 1), v1 = min(u1, r.vectors + 1);  // whole vectors
+  int turn = v0 + warp * 32;
+  for (; turn + (AHEAD - 1) * kThreads + 32 <= v1; turn += AHEAD * kThreads) {
     uint4 raw[AHEAD];
     uint32_t open[AHEAD];
-    bool whole[AHEAD];
+    const T *p = r.p + r.first(turn + lane);
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) {
-      const int at = u + k * kThreads;
-      whole[k] = at < u1 && at > 0 && at <= r.vectors;
-      if (whole[k]) {
-        raw[k] = *reinterpret_cast<const uint4 *>(r.p + r.first(at));
-        if (r.mask) open[k] = mask_bits(r.mask, r.first(at), r.words);
-      }
+      raw[k] = *reinterpret_cast<const uint4 *>(p + k * kThreads * E);
+      if (r.mask) open[k] = mask_bits(r.mask, r.first(turn + lane + k * kThreads), r.words);
     }
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) {
-      const int at = u + k * kThreads;
       float x[E];
-      if (whole[k]) {
-        r.values(raw[k], open[k], x);
-      } else if (at < u1) {
-        r.load(at, x);
-      } else {
-#pragma unroll
-        for (int i = 0; i < E; ++i) x[i] = -INFINITY;
-      }
-      __syncwarp();
-      take(x, r.first(at));
+      r.values(raw[k], open[k], x);
+      take(x, r.first(turn + lane + k * kThreads));
     }
+  }
+  for (; turn < v1; turn += kThreads) {
+    float x[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) x[i] = -INFINITY;
+    if (turn + lane < v1) r.load(turn + lane, x);
+    __syncwarp();
+    take(x, r.first(turn + lane));
   }
   float lo, hi;
   f2unpack(sum2, lo, hi);
   float sum = lo + hi;
+  if (warp == 0) {  // the entries before and behind the whole vectors, a lane each
+    const int tail = r.first(r.vectors + 1), n = u0 == 0 ? r.lead : 0, m = u1 == r.units() ? r.V - tail : 0;
+    int at = lane < n ? lane : lane - n < m ? tail + lane - n : -1;
+    float x = at < 0 ? -INFINITY : r.at(at), most = x;
+    broken = broken || !(x < INFINITY);
+    if (!(x > -INFINITY)) most = -INFINITY, at = last ? -1 : s.V;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+      better(most, at, __shfl_xor_sync(0xffffffffu, most, o), __shfl_xor_sync(0xffffffffu, at, o), last);
+    const float old = top;
+    better(top, best, most, at, last);
+    if (top > -INFINITY) sum = (old == -INFINITY ? 0.0f : sum * ex2((old - top) * cc)) + ex2((x - top) * cc);
+  }
   const float own = top;
   if (lane == 0) tops[warp] = top, bests[warp] = best;
   broken = __syncthreads_or(broken);
@@ -242,41 +251,43 @@ __device__ __forceinline__ void store_there(double *p, uint32_t rank, double v) 
 constexpr int kCluster = 8;  // blocks of a request, at most
 constexpr int kSegments = kCluster * kWarps;
 
-// 2^(t / 128) for t <= 0 (minus infinity: 0) in 64 bits: 128 values in a table, and a polynomial of degree 4
-// on the rest, at most 1/256 of a binary order away (the Taylor series of the exponential: its next term is below
-// 2e-15); the method is P. Tang's (table-driven exponentials, 1989).
-constexpr int kTable = 128;
+// 2^(t / 512) for -1000 < t / 512 <= 0 in 64 bits: 512 values in a table, and a polynomial of degree 3 on the
+// rest, at most 1/1024 of a binary order away (the exponential's Taylor series; its next term is
+// below 1e-14).  The method is P. Tang's (table-driven exponentials, 1989).
+constexpr int kTable = 512;
 __device__ __forceinline__ double exp2_table(double t, const double *table) {
   const double magic = 6755399441055744.0;  // 1.5 * 2^52: a sum with it holds round(t) in the low bits
-  const double big = fmax(t, -128.0 * 1000.0) + magic;
+  const double big = t + magic;
   const int n = __double2loint(big);
   const double r = t - (big - magic), h = 0.6931471805599453094 / kTable;
-  double y = fma(r, h * h * h * h / 24.0, h * h * h / 6.0);
-  y = fma(y, r, h * h / 2.0);
+  double y = fma(r, h * h * h / 6.0, h * h / 2.0);
   y = fma(y, r, h);
   y = fma(y, r, 1.0) * table[n & (kTable - 1)];
-  const double e = __hiloint2double(__double2hiint(y) + ((n >> 7) << 20), __double2loint(y));
-  return t < -128.0 * 1000.0 ? 0.0 : e;
+  return __hiloint2double(__double2hiint(y) + (n & ~(kTable - 1)) * ((1 << 20) / kTable), __double2loint(y));
 }
-// An f32 number in 64 bits without the conversion unit; zeros and subnormals become 2^-127 (nothing beside a logit
-// or a probability).
+// An f32 number in 64 bits without the conversion unit; zeros and subnormals become about 2^-127 (nothing beside a
+// logit or a probability).
+template <typename T>
 __device__ __forceinline__ double widened(float x) {
   const uint32_t b = __float_as_uint(x);
-  return __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + 0x38000000u)), (int)(b << 29));
+  const uint32_t hi = (b >> 3) + 0x38000000u + (b >> 31) * 0x70000000u;
+  return __hiloint2double((int)hi, sizeof(T) == 2 ? 0 : (int)(b << 29));  // 16-bit types have no bits there
 }
 
 // The weights of a row's entries: of p (times its sum), or of max(p - q, 0).
 template <typename T>
 struct Weights {
   Row<T> r;
-  double scale, shift;  // a weight is 2^((x scale - shift) / 128)
+  double scale, shift;  // a weight is 2^((x scale - shift) / 512)
   double inv_w;
-  const float *q;  // NULL: weights of p
-  int hole;        // an entry of weight zero, or -1
+  float top, least;  // no weight for x - top at or below it: 2^-1000
+  const float *q;    // NULL: weights of p
+  int hole;          // an entry of weight zero, or -1
 
-  __device__ Weights(const Row<T> &row, float top, double inv_t) : r(row), inv_w(0.0), q(nullptr), hole(-1) {
+  __device__ Weights(const Row<T> &row, float largest, double inv_t) : r(row), inv_w(0.0), top(largest), q(nullptr), hole(-1) {
     scale = 1.4426950408889634074 * kTable * inv_t;
-    shift = (double)top * scale;
+    shift = (double)largest * scale;
+    least = (float)(-693.0 / inv_t);
   }
   // Weights of unit u's entries; returns their sum.
   __device__ __forceinline__ double unit(int u, double *y, const double *table) const {
@@ -293,12 +304,21 @@ struct Weights {
         for (int i = 0; i < E; ++i) qs[i] = i < n ? q[v0 + i] : 0.0f;
       }
     }
+    if ((unsigned)(hole - v0) < (unsigned)E) {
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (v0 + i == hole) x[i] = -INFINITY;
+    }
     double sum = 0.0;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      double e = exp2_table(fma(widened(x[i]), scale, -shift), table);
-      if (x[i] == -INFINITY || v0 + i == hole) e = 0.0;
-      if (q) e = fmax(fma(e, inv_w, -widened(qs[i])), 0.0);
+      double e = exp2_table(fma(widened<T>(x[i]), scale, -shift), table);
+      if (!(x[i] - top > least)) e = 0.0;
+      if (q) {
+        e = fma(e, inv_w, -widened<float>(qs[i]));
+        const int keep = ~(__double2hiint(e) >> 31);  // zero for what is below zero
+        e = __hiloint2double(__double2hiint(e) & keep, __double2loint(e) & keep);
+      }
       sum += y[i] = e;
     }
     return sum;
@@ -308,7 +328,7 @@ struct Weights {
 struct Shared {
   double seg[2][kSegments];  // sums of the segments, of two turns
   double part[kWarps];       // of a segment's eighths
-  double table[kTable];      // 2^(i / 128)
+  double table[kTable];      // 2^(i / 512)
   int verdict;
 };
 
@@ -598,8 +618,9 @@ __global__ void __launch_bounds__(kThreads, 3) verify_pick_kernel(VerifyCall c, 
   if (me == 0 && tid == 0) c.out_len[i] = (uint32_t)len;
 }
 
-// Pieces of a row: enough for some turns of the device's blocks, of two vectors a thread or more.
-constexpr int64_t kBlocks = 4096;
+// Pieces of a row: enough for some turns of the device's blocks (of rows of 131,072 entries, two for 1280 rows), of two vectors a
+// thread or more.
+constexpr int64_t kBlocks = 2048;
 int verify_pieces(const VerifyShape &s, int64_t rows) {
   const int64_t most = (s.V / (s.dtype == DT_F32 ? 4 : 8) + 2 + 2 * kThreads - 1) / (2 * kThreads);
   return (int)std::max<int64_t>(1, std::min(most, (kBlocks + rows - 1) / rows));
@@ -612,12 +633,12 @@ cudaError_t run(const VerifyShape &s, const VerifyCall &c, const VerifyWork &w, 
   verify_rows_kernel<T><<<(unsigned)(rows * pieces), kThreads, 0, st>>>(c, s, w, pieces);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  // blocks of a request: as many as are on the device at once, 2048 entries each or more
+  // blocks of a request: as many as the device takes in two turns, 2048 entries each or more
   int dev = 0, sms = 0, size = 1;
   e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e != cudaSuccess) return e;
-  while (size < kCluster && (int64_t)c.n_seq * size * 2 <= 3 * sms && size * 4096 <= s.V) size *= 2;
+  while (size < kCluster && (int64_t)c.n_seq * size * 2 <= 6 * sms && size * 4096 <= s.V) size *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(c.n_seq * size));
   cfg.blockDim = dim3(kThreads);
