@@ -274,6 +274,10 @@ __device__ __forceinline__ double widened(float x) {
   return __hiloint2double((int)hi, sizeof(T) == 2 ? 0 : (int)(b << 29));  // 16-bit types have no bits there
 }
 
+__device__ __forceinline__ double masked(double x, int keep) {
+  return __hiloint2double(__double2hiint(x) & keep, __double2loint(x) & keep);
+}
+
 // The weights of a row's entries: of p (times its sum), or of max(p - q, 0).
 template <typename T>
 struct Weights {
@@ -312,14 +316,20 @@ struct Weights {
     double sum = 0.0;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      double e = exp2_table(fma(widened<T>(x[i]), scale, -shift), table);
-      if (!(x[i] - top > least)) e = 0.0;
-      if (q) {
-        e = fma(e, inv_w, -widened<float>(qs[i]));
-        const int keep = ~(__double2hiint(e) >> 31);  // zero for what is below zero
-        e = __hiloint2double(__double2hiint(e) & keep, __double2loint(e) & keep);
+      // weights of zero by bits, not by a branch: the chains of a unit's entries hide each other
+      const double e = exp2_table(fma(widened<T>(x[i]), scale, -shift), table);
+      y[i] = masked(e, -(int)(x[i] - top > least));
+    }
+    if (q) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const double e = fma(y[i], inv_w, -widened<float>(qs[i]));
+        y[i] = masked(e, ~(__double2hiint(e) >> 31));  // zero for what is below zero
       }
-      sum += y[i] = e;
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      sum += y[i];
     }
     return sum;
   }
@@ -442,7 +452,7 @@ __device__ __noinline__ int find(const Weights<T> w, Shared &sm, int turn, doubl
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 3) verify_pick_kernel(VerifyCall c, VerifyShape s, VerifyWork w, int pieces) {
+__global__ void __launch_bounds__(kThreads, 4) verify_pick_kernel(VerifyCall c, VerifyShape s, VerifyWork w, int pieces) {
   __shared__ Shared sm;
   __shared__ float tops[kThreads], sums[kThreads];
   __shared__ int bests[kThreads], found;
@@ -633,12 +643,12 @@ cudaError_t run(const VerifyShape &s, const VerifyCall &c, const VerifyWork &w, 
   verify_rows_kernel<T><<<(unsigned)(rows * pieces), kThreads, 0, st>>>(c, s, w, pieces);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  // blocks of a request: as many as the device takes in two turns, 2048 entries each or more
+  // blocks of a request: as many as are on the device at once, 2048 entries each or more
   int dev = 0, sms = 0, size = 1;
   e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e != cudaSuccess) return e;
-  while (size < kCluster && (int64_t)c.n_seq * size * 2 <= 6 * sms && size * 4096 <= s.V) size *= 2;
+  while (size < kCluster && (int64_t)c.n_seq * size * 2 <= 4 * sms && size * 4096 <= s.V) size *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(c.n_seq * size));
   cfg.blockDim = dim3(kThreads);
