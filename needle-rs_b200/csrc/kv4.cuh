@@ -70,12 +70,6 @@ __host__ __device__ __forceinline__ Seq sequence(const Kv4Rows &b, const Kv4Shap
   return ok ? Seq{a, e - a, len} : Seq{0, 0, 0};
 }
 
-// The first block looks at every request, those without rows as well.
-__device__ __forceinline__ void check_all(const Kv4Rows &b, const Kv4Shape &s, bool inside, int *bad) {
-  if (blockIdx.x == 0)
-    for (int i = threadIdx.x; i < b.n_seq; i += blockDim.x) sequence(b, s, i, inside, bad);
-}
-
 // Where tile `t` (of 16 tokens) of request i's cache for a KV head begins, in
 // units of 128 bytes; kNoPlace (flag set) where the table names a page that is
 // not there.

@@ -7,6 +7,10 @@
 // every other operation rounded to f32, so that any program that follows the
 // formula gets the same codes.  The codes are of the rounded scale and
 // minimum: what their rounding to f16 moves is within the codes' rounding.
+//
+// Both directions are bound by the bytes of the 16-bit side.  A warp takes a
+// tile of 16 tokens of a request and head.  Blocks share a call's tiles evenly: each
+// counts the requests' tiles by itself (one look at the lengths) and takes its part of them.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -22,113 +26,310 @@ namespace {
 
 using namespace kv4;
 
-// The request and the token of row `row` of a call (n = 0: none).
-struct Row {
-  int seq, pos;
-  bool there;
-};
-__device__ __forceinline__ Row row_at(const Kv4Rows &b, const Kv4Shape &s, int64_t row, int *bad) {
-  int lo = 0, hi = b.n_seq;  // the last request that starts at or before the row
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (b.row_start[mid] <= row) lo = mid; else hi = mid;
-  }
-  const Seq q = sequence(b, s, lo, true, bad);
-  const bool there = row >= q.row0 && row < q.row0 + q.n;
-  return Row{lo, there ? q.len - q.n + (int)(row - q.row0) : 0, there};
+constexpr int kWarps = 8, kThreads = kWarps * 32;
+
+// Tiles of 16 tokens that hold rows of a request, times KV heads.
+__device__ __forceinline__ uint32_t units_of(const Seq &q, int KVH) {
+  return q.n ? (uint32_t)((q.len - 1) / kTokens - (q.len - q.n) / kTokens + 1) * KVH : 0u;
 }
 
-template <typename T>
-__global__ void append_kernel(Kv4Call c, Kv4Shape s, Kv4Rows b, int *bad) {
-  check_all(b, s, true, bad);
-  const int64_t unit = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  const int64_t row = unit / s.KVH;
-  const int kvh = (int)(unit % s.KVH), lane = threadIdx.x & 31, ng = s.ng;
-  if (row >= b.rows) return;
-  const Row at = row_at(b, s, row, bad);
-  if (!at.there) return;
-  uint8_t *tile = tile_at(c.pages, b, s, at.seq, at.pos / kTokens, kvh, bad);
-  if (!tile) return;
-  const T *k = (const T *)c.k + row * c.k_row + (int64_t)kvh * c.k_head;
-  const T *v = (const T *)c.v + row * c.v_row + (int64_t)kvh * c.v_head;
-  const int t = at.pos % kTokens;
-  bool ok = true;
-  for (int d = lane; d < s.D; d += 32) ok = ok && fabsf((float)k[d]) <= kLargest && fabsf((float)v[d]) <= kLargest;
-  ok = __all_sync(0xffffffffu, ok);
-  for (int u = 0; u < 2 * ng; ++u) {
-    const int g = u >> 1, d = g * 32 + lane;
-    const bool is_v = u & 1, in = d < s.D;
-    const float x = in ? (float)(is_v ? v : k)[d] : 0.0f;
-    const float lo = -warp_max(in ? -x : -INFINITY), hi = warp_max(in ? x : -INFINITY);
-    __half scale = __float2half_rn(__fdiv_rn(hi - lo, 15.0f)), least = __float2half_rn(lo);
-    if (!ok) scale = least = __ushort_as_half(is_v ? 0 : 0x7fff);
-    const float sc = __half2float(scale), inv = sc > 0.0f ? __fdiv_rn(1.0f, sc) : 0.0f;
-    const float q = rintf(__fmul_rn(__fsub_rn(x, __half2float(least)), inv));
-    const uint32_t code = ok && in ? (uint32_t)fminf(fmaxf(q, 0.0f), 15.0f) : 0u;
-    if (is_v) {
-      uint32_t w = code << (4 * (lane & 3));
-      w |= __shfl_xor_sync(0xffffffffu, w, 1);
-      w |= __shfl_xor_sync(0xffffffffu, w, 2);
-      if ((lane & 3) == 0) *(uint16_t *)(tile + v_half(ng, t, g, lane >> 2)) = (uint16_t)w;
-      if (lane < 2) *(__half *)(tile + v_param(ng, t, g, lane)) = lane ? least : scale;
-    } else {
-      uint32_t w = code << (4 * (((lane & 7) >> 1) + 4 * (lane & 1)));
-      w |= __shfl_xor_sync(0xffffffffu, w, 1);
-      w |= __shfl_xor_sync(0xffffffffu, w, 2);
-      w |= __shfl_xor_sync(0xffffffffu, w, 4);
-      if ((lane & 7) == 0) *(uint32_t *)(tile + k_word(t, g, lane >> 3)) = w;
-      if (lane < 2) *(__half *)(tile + k_param(ng, t, g, lane)) = lane ? least : scale;
+// A warp's walk over its block's part of a call's units.
+struct Walk {
+  uint32_t at, end;     // this warp's next unit, the block's last + 1
+  uint32_t base, upto;  // units before the window's first request, and a lane's request's end (exclusive sum + own)
+  int first;            // request of lane 0
+  Seq q;                // a lane's request
+
+  __device__ void window(const Kv4Rows &b, const Kv4Shape &s, int *bad) {
+    const int lane = threadIdx.x & 31;
+    q = first + lane < b.n_seq ? sequence(b, s, first + lane, true, bad) : Seq{0, 0, 0};
+    upto = units_of(q, s.KVH);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+  }
+  __device__ void start(const Kv4Rows &b, const Kv4Shape &s, int *bad) {
+    __shared__ uint32_t sums[kWarps], found_base;
+    __shared__ int found;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int per = (b.n_seq + kThreads - 1) / kThreads, i0 = min((int)threadIdx.x * per, b.n_seq), i1 = min(i0 + per, b.n_seq);
+    uint32_t mine = 0;
+    for (int i = i0; i < i1; ++i) mine += units_of(sequence(b, s, i, true, bad), s.KVH);
+    uint32_t sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t x = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += x;
+    }
+    if (lane == 31) sums[warp] = sum;
+    if (threadIdx.x == 0) found = b.n_seq, found_base = 0;
+    __syncthreads();
+    uint32_t total = 0;
+#pragma unroll
+    for (int k = 0; k < kWarps; ++k) {
+      if (k < warp) sum += sums[k];
+      total += sums[k];
+    }
+    const uint32_t begin = (uint32_t)((uint64_t)total * blockIdx.x / gridDim.x);
+    end = (uint32_t)((uint64_t)total * (blockIdx.x + 1) / gridDim.x);
+    uint32_t before = sum - mine;
+    if (before <= begin && begin < sum) {
+      int i = i0;
+      for (;; ++i) {
+        const uint32_t n = per > 1 ? units_of(sequence(b, s, i, true, bad), s.KVH) : mine;
+        if (begin < before + n || i + 1 >= i1) break;
+        before += n;
+      }
+      found = i;
+      found_base = before;
+    }
+    __syncthreads();
+    first = found;
+    base = found_base;
+    at = begin + warp;
+    if (at < end) window(b, s, bad);
+  }
+  // The request and the place in it of the warp's next unit; false at the end.
+  __device__ bool next(const Kv4Rows &b, const Kv4Shape &s, int *bad, int *seq, Seq *of, int *unit) {
+    while (at < end && first < b.n_seq) {
+      const uint32_t here = __ballot_sync(0xffffffffu, at < base + upto);
+      if (here) {
+        const int lane = __ffs(here) - 1;
+        *seq = first + lane;
+        of->row0 = __shfl_sync(0xffffffffu, q.row0, lane);
+        of->n = __shfl_sync(0xffffffffu, q.n, lane);
+        of->len = __shfl_sync(0xffffffffu, q.len, lane);
+        const uint32_t before = lane ? __shfl_sync(0xffffffffu, upto, lane - 1) : 0u;
+        *unit = (int)(at - base - before);
+        at += kWarps;
+        return true;
+      }
+      base += __shfl_sync(0xffffffffu, upto, 31);
+      first += 32;
+      window(b, s, bad);
+    }
+    return false;
+  }
+};
+
+// Lanes take 16-byte pieces (8 dimensions) of K and of V: 8 NG pieces a token.  A tile whose 16 tokens are
+// all new is put together in shared memory (groups 272 bytes apart: no
+// two lanes of a quarter meet in a bank) and leaves in whole vectors; else a token's words go to the page one by
+// one.  By words alone, 32,768 tokens of 8 heads of 128 took 3 times as long.
+constexpr int kPad = 272;
+__host__ __device__ constexpr int staged_bytes(int ng) { return ng * (2 * kPad + 128); }
+
+template <typename T, int NG>
+__global__ void __launch_bounds__(kThreads) append_kernel(Kv4Call c, Kv4Shape s, Kv4Rows b, int *bad) {
+  constexpr int PIECES = 8 * NG, TP = PIECES <= 16 ? 32 / PIECES : 1, PASSES = kTokens / TP;  // tokens of a pass
+  constexpr int BATCH = PASSES < 8 ? PASSES : 8;
+  __shared__ __align__(16) uint8_t stage[kWarps][staged_bytes(NG)];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int sub = lane / PIECES, piece = lane % PIECES, g = (piece % (4 * NG)) >> 2, q4 = piece & 3, d = g * 32 + q4 * 8;
+  const bool is_v = piece >= 4 * NG, lane_in = lane < TP * PIECES, in = lane_in && d < s.D;
+  const uint32_t token_lanes = PIECES == 32 ? 0xffffffffu : ((1u << PIECES) - 1) << (sub * PIECES % 32);
+  Walk walk;
+  walk.start(b, s, bad);
+  int seq, unit;
+  Seq q;
+  while (walk.next(b, s, bad, &seq, &q, &unit)) {
+    const int t = (q.len - q.n) / kTokens + unit / s.KVH, kvh = unit % s.KVH;
+    uint8_t *page = tile_at(c.pages, b, s, seq, t, kvh, bad);
+    if (!page) continue;
+    const int first = max(0, q.len - q.n - t * kTokens), last = min(kTokens, q.len - t * kTokens);  // its new tokens
+    const bool whole = last - first == kTokens;
+    // row of token i of the tile: row0 + i
+    const int64_t row0 = (int64_t)q.row0 + t * kTokens - (q.len - q.n);
+    const T *src = (const T *)(is_v ? c.v : c.k) + row0 * (is_v ? c.v_row : c.k_row) + (int64_t)kvh * (is_v ? c.v_head : c.k_head) + d;
+    const int64_t step = is_v ? c.v_row : c.k_row;
+    __syncwarp();  // the copies out of the last tile are done
+#pragma unroll
+    for (int p0 = 0; p0 < PASSES; p0 += BATCH) {
+      uint4 raw[BATCH];
+#pragma unroll
+      for (int p = 0; p < BATCH; ++p) {
+        const int tok = (p0 + p) * TP + sub;
+        raw[p] = in && tok >= first && tok < last ? *reinterpret_cast<const uint4 *>(src + tok * step) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int p = 0; p < BATCH; ++p) {
+        const int tok = (p0 + p) * TP + sub;
+        const T *e = reinterpret_cast<const T *>(&raw[p]);
+        float x[8], lo = INFINITY, hi = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          x[i] = (float)e[i];
+          if (in) {  // NaN stays
+            asm("min.NaN.f32 %0, %0, %1;" : "+f"(lo) : "f"(x[i]));
+            asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi) : "f"(x[i]));
+          }
+        }
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+          const float l = __shfl_xor_sync(0xffffffffu, lo, o), h = __shfl_xor_sync(0xffffffffu, hi, o);
+          asm("min.NaN.f32 %0, %0, %1;" : "+f"(lo) : "f"(l));
+          asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi) : "f"(h));
+        }
+        const bool fits = !lane_in || (lo >= -kLargest && hi <= kLargest) || d - q4 * 8 >= s.D;
+        const bool ok = (__ballot_sync(0xffffffffu, !fits) & token_lanes) == 0;
+        __half scale = __float2half_rn(__fdiv_rn(hi - lo, 15.0f)), least = __float2half_rn(lo);
+        if (!ok) scale = least = __ushort_as_half(is_v ? 0 : 0x7fff);
+        const float sc = __half2float(scale), mi = __half2float(least), inv = sc > 0.0f ? __fdiv_rn(1.0f, sc) : 0.0f;
+        uint32_t code[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float y = fminf(fmaxf(__fmul_rn(__fsub_rn(x[i], mi), inv), 0.0f), 15.0f);
+          // a sum with 1.5 * 2^23 is rounded to an integer, half to even, in the low bits; NaN became 0 above
+          code[i] = ok && in ? __float_as_uint(__fadd_rn(y, 12582912.0f)) & 15u : 0u;
+        }
+        if (lane_in && tok >= first && tok < last) {
+          uint8_t *to = whole ? stage[warp] : page;
+          const int gap = whole ? kPad - 256 : 0;  // the staged groups lie further apart
+          if (is_v) {
+            const uint32_t w0 = code[0] | code[1] << 4 | code[2] << 8 | code[3] << 12;
+            const uint32_t w1 = code[4] | code[5] << 4 | code[6] << 8 | code[7] << 12;
+            *(uint16_t *)(to + v_half(NG, tok, g, 2 * q4) + (NG + g) * gap) = (uint16_t)w0;
+            *(uint16_t *)(to + v_half(NG, tok, g, 2 * q4 + 1) + (NG + g) * gap) = (uint16_t)w1;
+          } else {
+            // neighbours in the halves of a word
+            *(uint32_t *)(to + k_word(tok, g, q4) + g * gap) = code[0] | code[1] << 16 | code[2] << 4 | code[3] << 20 | code[4] << 8 |
+                                                             code[5] << 24 | code[6] << 12 | code[7] << 28;
+          }
+          if (q4 < 2) {
+            const int at = is_v ? v_param(NG, tok, g, q4) : k_param(NG, tok, g, q4);
+            *(__half *)(to + at + 2 * NG * gap) = q4 ? least : scale;
+          }
+        }
+      }
+    }
+    if (whole) {
+      __syncwarp();
+      for (int i = lane; i < 40 * NG; i += 32) {
+        const int at = i < 32 * NG ? (i >> 4) * kPad + (i & 15) * 16 : 2 * NG * kPad + (i - 32 * NG) * 16;
+        reinterpret_cast<uint4 *>(page)[i] = *reinterpret_cast<const uint4 *>(stage[warp] + at);
+      }
     }
   }
 }
 
-template <typename T>
-__global__ void read_kernel(Kv4Call c, Kv4Shape s, Kv4Rows b, int *bad) {
-  check_all(b, s, true, bad);
-  const int64_t unit = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  const int64_t row = unit / s.KVH;
-  const int kvh = (int)(unit % s.KVH), lane = threadIdx.x & 31, ng = s.ng;
-  if (row >= b.rows) return;
-  const Row at = row_at(b, s, row, bad);
-  if (!at.there) return;
-  const uint8_t *tile = tile_at(c.pages, b, s, at.seq, at.pos / kTokens, kvh, bad);
-  if (!tile) return;
-  T *k = (T *)c.k_out + row * c.k_row + (int64_t)kvh * c.k_head, *v = (T *)c.v_out + row * c.v_row + (int64_t)kvh * c.v_head;
-  const int t = at.pos % kTokens;
-  for (int d = lane; d < s.D; d += 32) {
-    const int g = d >> 5, i = d & 31;
-    const float2 kp = make_float2(__half2float(*(const __half *)(tile + k_param(ng, t, g, 0))),
-                                  __half2float(*(const __half *)(tile + k_param(ng, t, g, 1))));
+// minimum + scale * code for code nibble `n` of w.
+__device__ __forceinline__ float value_of(uint32_t w, int n, float scale, float least) {
+  const float c = __uint_as_float(((w >> (4 * n)) & 15u) | 0x4b000000u) - 8388608.0f;
+  return fmaf(scale, c, least);
+}
+
+// A lane reads what an attention would give it: for K words of two tokens (rows r and
+// r + 8 of a matrix operand), for V four dimensions of four tokens; eight bytes a group each.  Rows leave in 64-byte
+// runs.
+template <typename T, int NG>
+__global__ void __launch_bounds__(kThreads) read_kernel(Kv4Call c, Kv4Shape s, Kv4Rows b, int *bad) {
+  const int lane = threadIdx.x & 31, r = lane >> 2, q4 = lane & 3;
+  Walk walk;
+  walk.start(b, s, bad);
+  int seq, unit;
+  Seq q;
+  while (walk.next(b, s, bad, &seq, &q, &unit)) {
+    const int t = (q.len - q.n) / kTokens + unit / s.KVH, kvh = unit % s.KVH;
+    const uint8_t *page = tile_at(c.pages, b, s, seq, t, kvh, bad);
+    if (!page) continue;
+    const int first = max(0, q.len - q.n - t * kTokens), last = min(kTokens, q.len - t * kTokens);
+    const int64_t row0 = (int64_t)q.row0 + t * kTokens - (q.len - q.n);
+    uint2 kc[NG], vc[NG], vs[NG], vm[NG];
+    uint32_t ks[NG], km[NG];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      if (c.k_out) {
+        kc[g] = *reinterpret_cast<const uint2 *>(page + g * 256 + lane * 8);
+        ks[g] = *reinterpret_cast<const uint32_t *>(page + k_params(NG) + (g * 8 + r) * 4);
+        km[g] = *reinterpret_cast<const uint32_t *>(page + k_params(NG) + ((NG + g) * 8 + r) * 4);
+      }
+      if (c.v_out) {
+        vc[g] = *reinterpret_cast<const uint2 *>(page + v_codes(NG) + g * 256 + lane * 8);
+        const uint4 p = *reinterpret_cast<const uint4 *>(page + v_params(NG) + (g * 4 + q4) * 16);
+        vs[g] = make_uint2(p.x, p.y);
+        vm[g] = make_uint2(p.z, p.w);
+      }
+    }
+    // a key's scale of NaN marks a token that did not fit: of tokens 4 q4, 4 q4 + 2, 4 q4 + 1, 4 q4 + 3
+    const uint2 mark = *reinterpret_cast<const uint2 *>(page + k_params(NG) + 2 * q4 * 4);
     if (c.k_out) {
-      const uint32_t w = *(const uint32_t *)(tile + k_word(t, g, i >> 3));
-      k[d] = from_f32<T>(fmaf(kp.x, (float)((w >> (4 * (((i & 7) >> 1) + 4 * (i & 1)))) & 15u), kp.y));
+      const int ta = 4 * (r >> 1) + (r & 1);
+      T *out = (T *)c.k_out + row0 * c.k_row + (int64_t)kvh * c.k_head + q4 * 8;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const float2 sc = __half22float2(*reinterpret_cast<const __half2 *>(&ks[g]));
+        const float2 mi = __half22float2(*reinterpret_cast<const __half2 *>(&km[g]));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t w = h ? kc[g].y : kc[g].x;
+          float x[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = value_of(w, (i >> 1) + 4 * (i & 1), h ? sc.y : sc.x, h ? mi.y : mi.x);
+          const int tok = ta + 2 * h;
+          if (tok >= first && tok < last && g * 32 + q4 * 8 < s.D) store<8>(out + tok * c.k_row + g * 32, x);
+        }
+      }
     }
     if (c.v_out) {
-      const uint32_t w = *(const uint16_t *)(tile + v_half(ng, t, g, i >> 2));
-      const float sc = __half2float(*(const __half *)(tile + v_param(ng, t, g, 0)));
-      const float least = __half2float(*(const __half *)(tile + v_param(ng, t, g, 1)));
-      // a key of NaN marks a token that did not fit
-      v[d] = from_f32<T>(isnan(kp.x) ? kp.x : fmaf(sc, (float)((w >> (4 * (i & 3))) & 15u), least));
+      T *out = (T *)c.v_out + row0 * c.v_row + (int64_t)kvh * c.v_head + r * 4;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int tok = 4 * q4 + i;
+        const uint32_t m = i & 1 ? mark.y : mark.x;
+        const bool lost = (((i < 2 ? m : m >> 16) & 0x7fffu)) > 0x7c00u;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          const uint32_t w = (i < 2 ? vc[g].x : vc[g].y) >> (16 * (i & 1));
+          const uint32_t su = (i < 2 ? vs[g].x : vs[g].y) >> (16 * (i & 1)), mu = (i < 2 ? vm[g].x : vm[g].y) >> (16 * (i & 1));
+          const float sc = __half2float(__ushort_as_half((unsigned short)su)), mi = __half2float(__ushort_as_half((unsigned short)mu));
+          alignas(8) T e[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) e[k] = from_f32<T>(lost ? __uint_as_float(0x7fc00000u) : value_of(w, k, sc, mi));
+          if (tok >= first && tok < last && g * 32 + r * 4 < s.D)
+            *reinterpret_cast<uint2 *>(out + tok * c.v_row + g * 32) = *reinterpret_cast<const uint2 *>(e);
+        }
+      }
     }
   }
+}
+
+// Blocks: a warp for each tile that there can be, up to `most` of them.
+unsigned grid_of(const Kv4Shape &s, const Kv4Rows &b, int64_t most) {
+  const int64_t tiles = std::min<int64_t>(b.rows, b.rows / kTokens + 2 * (int64_t)b.n_seq);
+  return (unsigned)std::max<int64_t>(1, std::min(most, (tiles * s.KVH + kWarps - 1) / kWarps));
+}
+
+template <typename T, int NG>
+cudaError_t launch(bool append, const Kv4Shape &s, const Kv4Rows &b, const Kv4Call &c, int *bad, int sms, cudaStream_t st) {
+  const unsigned grid = grid_of(s, b, (int64_t)sms * 4);
+  if (append) append_kernel<T, NG><<<grid, kThreads, 0, st>>>(c, s, b, bad);
+  else read_kernel<T, NG><<<grid, kThreads, 0, st>>>(c, s, b, bad);
+  return cudaGetLastError();
+}
+template <typename T>
+cudaError_t launch(bool append, const Kv4Shape &s, const Kv4Rows &b, const Kv4Call &c, int *bad, int sms, cudaStream_t st) {
+  switch (s.ng) {
+    case 1: return launch<T, 1>(append, s, b, c, bad, sms, st);
+    case 2: return launch<T, 2>(append, s, b, c, bad, sms, st);
+    case 3: return launch<T, 3>(append, s, b, c, bad, sms, st);
+    default: return launch<T, 4>(append, s, b, c, bad, sms, st);
+  }
+}
+cudaError_t launch(bool append, const Kv4Shape &s, const Kv4Rows &b, const Kv4Call &c, const Kv4Work &w, cudaStream_t st) {
+  if (b.rows == 0) return cudaSuccess;
+  return s.dtype == DT_F16 ? launch<__half>(append, s, b, c, w.bad, w.sms, st)
+                           : launch<__nv_bfloat16>(append, s, b, c, w.bad, w.sms, st);
 }
 
 }  // namespace
 
-cudaError_t kv4_append(const Kv4Shape &s, const Kv4Rows &b, const Kv4Call &c, int *bad, cudaStream_t st) {
-  if (b.rows == 0) return cudaSuccess;
-  const unsigned grid = (unsigned)((b.rows * s.KVH + 7) / 8);
-  if (s.dtype == DT_F16) append_kernel<__half><<<grid, 256, 0, st>>>(c, s, b, bad);
-  else append_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(c, s, b, bad);
-  return cudaGetLastError();
+cudaError_t kv4_append(const Kv4Shape &s, const Kv4Rows &b, const Kv4Call &c, const Kv4Work &w, cudaStream_t st) {
+  return launch(true, s, b, c, w, st);
 }
-
-cudaError_t kv4_read(const Kv4Shape &s, const Kv4Rows &b, const Kv4Call &c, int *bad, cudaStream_t st) {
-  if (b.rows == 0) return cudaSuccess;
-  const unsigned grid = (unsigned)((b.rows * s.KVH + 7) / 8);
-  if (s.dtype == DT_F16) read_kernel<__half><<<grid, 256, 0, st>>>(c, s, b, bad);
-  else read_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(c, s, b, bad);
-  return cudaGetLastError();
+cudaError_t kv4_read(const Kv4Shape &s, const Kv4Rows &b, const Kv4Call &c, const Kv4Work &w, cudaStream_t st) {
+  return launch(false, s, b, c, w, st);
 }
 
 }  // namespace ndl

@@ -493,7 +493,7 @@ NeedleKv4Plan *needle_kv4_plan_create(size_t H, size_t KVH, size_t D, size_t pag
     if (page_tokens == 0 || page_tokens % 16 || page_tokens > 65536)
       return fail("4-bit cache: page_tokens must be a multiple of 16 up to 65536");
     if (n_pages == 0 || n_pages > kMaxRows || max_seqs == 0 || max_seqs > kMaxSeqs || max_rows == 0 || max_rows > kMaxRows ||
-        max_rows * (H / KVH) > kMaxRows)
+        max_rows * std::max(KVH, H / KVH) > kMaxRows)
       return fail("4-bit cache: invalid number of pages, sequences or rows");
     if (n_pages * needle_kv4_page_bytes(KVH, D, page_tokens) >= (size_t)1 << 39)
       return fail("4-bit cache: an array of pages must stay below 512 GiB");
@@ -530,7 +530,7 @@ int needle_kv4_append(NeedleKv4Plan *p, void *pages, const NeedleKv4Batch *b, co
     OnDevice on(p->device);
     if (!on.good() || !kv4_on_device(p, pages, b) || !all_on(p->device, {{"k", k}, {"v", v}})) return false;
     Kv4Call c{(uint8_t *)pages, k, v, nullptr, nullptr, (int64_t)k_row, (int64_t)k_head, (int64_t)v_row, (int64_t)v_head};
-    return ok(kv4_append(p->s, rows, c, p->work.bad, (cudaStream_t)stream));
+    return ok(kv4_append(p->s, rows, c, p->work, (cudaStream_t)stream));
   }) ? 0 : -1;
 }
 
@@ -545,7 +545,7 @@ int needle_kv4_read(NeedleKv4Plan *p, const void *pages, const NeedleKv4Batch *b
     OnDevice on(p->device);
     if (!on.good() || !kv4_on_device(p, pages, b) || !all_on(p->device, {{"k_out", k}, {"v_out", v}})) return false;
     Kv4Call c{(uint8_t *)pages, nullptr, nullptr, k, v, (int64_t)k_row, (int64_t)k_head, (int64_t)v_row, (int64_t)v_head};
-    return ok(kv4_read(p->s, rows, c, p->work.bad, (cudaStream_t)stream));
+    return ok(kv4_read(p->s, rows, c, p->work, (cudaStream_t)stream));
   }) ? 0 : -1;
 }
 

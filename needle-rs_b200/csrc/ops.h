@@ -131,8 +131,6 @@ struct Kv4Call {
   void *k_out, *v_out;  // read
   int64_t k_row, k_head, v_row, v_head;
 };
-cudaError_t kv4_append(const Kv4Shape &s, const Kv4Rows &b, const Kv4Call &c, int *bad, cudaStream_t st);
-cudaError_t kv4_read(const Kv4Shape &s, const Kv4Rows &b, const Kv4Call &c, int *bad, cudaStream_t st);
 
 struct Kv4AttnCall {
   const uint8_t *pages;
@@ -151,6 +149,8 @@ struct Kv4Work {
 };
 int64_t kv4_attn_blocks(int sms);
 int64_t kv4_attn_floats(const Kv4Shape &s, int sms);
+cudaError_t kv4_append(const Kv4Shape &s, const Kv4Rows &b, const Kv4Call &c, const Kv4Work &w, cudaStream_t st);
+cudaError_t kv4_read(const Kv4Shape &s, const Kv4Rows &b, const Kv4Call &c, const Kv4Work &w, cudaStream_t st);
 cudaError_t kv4_attn(const Kv4Shape &s, const Kv4Rows &b, const Kv4AttnCall &c, const Kv4Work &w, cudaStream_t st);
 
 // ── verification of drafts ──
