@@ -114,22 +114,96 @@ struct Walk {
   }
 };
 
-// Lanes take 16-byte pieces (8 dimensions) of K and of V: 8 NG pieces a token.  A tile whose 16 tokens are
-// all new is put together in shared memory (groups 272 bytes apart: no
-// two lanes of a quarter meet in a bank) and leaves in whole vectors; else a token's words go to the page one by
-// one.  By words alone, 32,768 tokens of 8 heads of 128 took 3 times as long.
+__device__ __forceinline__ float least3(float a, float b, float c) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float most3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// x / 15 rounded to f32: the product with 1 / 15 and one step on its remainder (Brisebarre, Muller and Raina, division
+// by constants, 2004; right for every mantissa).
+__device__ __forceinline__ float fifteenth(float x) {
+  const float c = 1.0f / 15.0f, q = __fmul_rn(x, c);
+  return fmaf(fmaf(-15.0f, q, x), c, q);
+}
+
+// A group's least and largest value over the four lanes that have it, NaN if there is one.
+struct Range {
+  float lo, hi;
+  __device__ __forceinline__ bool fits() const { return lo >= -kLargest && hi <= kLargest; }
+};
+template <typename T>
+__device__ __forceinline__ Range range_of(const uint4 &raw, bool in) {
+  const T *e = reinterpret_cast<const T *>(&raw);
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = (float)e[i];
+  Range r;
+  r.lo = least3(least3(x[0], x[1], x[2]), least3(x[3], x[4], x[5]), least3(x[6], x[7], x[7]));
+  r.hi = most3(most3(x[0], x[1], x[2]), most3(x[3], x[4], x[5]), most3(x[6], x[7], x[7]));
+  if (!in) r.lo = INFINITY, r.hi = -INFINITY;
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) {
+    const float l = __shfl_xor_sync(0xffffffffu, r.lo, o), h = __shfl_xor_sync(0xffffffffu, r.hi, o);
+    r.lo = least3(r.lo, l, l);
+    r.hi = most3(r.hi, h, h);
+  }
+  return r;
+}
+
+// Eight codes in a word (nibble i: code i, or neighbours in the halves), their scale and minimum.
+struct Coded {
+  uint32_t word;
+  __half scale, least;
+};
+template <typename T, bool PAIRS>
+__device__ __forceinline__ Coded coded(const uint4 &raw, const Range &r, bool in, bool ok, uint16_t lost) {
+  const T *e = reinterpret_cast<const T *>(&raw);
+  Coded c;
+  c.scale = ok ? __float2half_rn(fifteenth(r.hi - r.lo)) : __ushort_as_half(lost);
+  c.least = ok ? __float2half_rn(r.lo) : __ushort_as_half(lost);
+  const float sc = __half2float(c.scale), mi = __half2float(c.least);
+  const float inv = in && sc > 0.0f ? __frcp_rn(sc) : 0.0f;  // 0: codes of 0, whatever x is
+  const uint64_t mi2 = f2pack(mi, mi), inv2 = f2pack(inv, inv), magic = f2pack(12582912.0f, 12582912.0f);
+  c.word = 0;
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    float a, b;
+    f2unpack(fmul2(fsub2(f2pack((float)e[i], (float)e[i + 1]), mi2), inv2), a, b);
+    a = fminf(fmaxf(a, 0.0f), 15.0f);
+    b = fminf(fmaxf(b, 0.0f), 15.0f);
+    // a sum with 1.5 * 2^23 is rounded to an integer, half to even, in the low bits
+    f2unpack(fadd2(f2pack(a, b), magic), a, b);
+    c.word += __float_as_uint(a) << (PAIRS ? 2 * i : 4 * i);
+    c.word += __float_as_uint(b) << (PAIRS ? 2 * i + 16 : 4 * i + 4);
+  }
+  c.word -= 0x4b400000u * 0x11111111u;  // what the sums hold above the codes
+  return c;
+}
+
+// Lanes take 16-byte pieces (8 dimensions) of a token's key and value: 4 NG lanes a token.  A tile whose 16 tokens
+// are all new is put together in shared memory (groups 272 bytes apart, against bank conflicts) and leaves in whole
+// vectors; else a token's words go to the page one by one.
 constexpr int kPad = 272;
 __host__ __device__ constexpr int staged_bytes(int ng) { return ng * (2 * kPad + 128); }
 
 template <typename T, int NG>
-__global__ void __launch_bounds__(kThreads) append_kernel(Kv4Call c, Kv4Shape s, Kv4Rows b, int *bad) {
-  constexpr int PIECES = 8 * NG, TP = PIECES <= 16 ? 32 / PIECES : 1, PASSES = kTokens / TP;  // tokens of a pass
-  constexpr int BATCH = PASSES < 8 ? PASSES : 8;
+__global__ void __launch_bounds__(kThreads, 3) append_kernel(Kv4Call c, Kv4Shape s, Kv4Rows b, int *bad) {
+  constexpr int PIECES = 4 * NG, TP = NG == 3 ? 2 : 32 / PIECES, PASSES = kTokens / TP;  // tokens of a pass
   __shared__ __align__(16) uint8_t stage[kWarps][staged_bytes(NG)];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int sub = lane / PIECES, piece = lane % PIECES, g = (piece % (4 * NG)) >> 2, q4 = piece & 3, d = g * 32 + q4 * 8;
-  const bool is_v = piece >= 4 * NG, lane_in = lane < TP * PIECES, in = lane_in && d < s.D;
-  const uint32_t token_lanes = PIECES == 32 ? 0xffffffffu : ((1u << PIECES) - 1) << (sub * PIECES % 32);
+  const int sub = lane / PIECES, piece = lane % PIECES, g = piece >> 2, q4 = piece & 3, d = g * 32 + q4 * 8;
+  const bool lane_in = sub < TP, in = lane_in && d < s.D;
+  const uint32_t token_lanes = (PIECES == 32 ? 0xffffffffu : (1u << PIECES) - 1) << (sub * PIECES % 32);
+  // a lane's places in a tile, for token sub * PASSES of it; those of the p-th behind it are a constant away
+  const int t0 = (lane_in ? sub : 0) * PASSES;
+  const int k_at = k_word(t0, g, q4), v_at = v_half(NG, t0, g, 2 * q4);
+  const int kp_at = k_param(NG, t0, g, q4 & 1), vp_at = v_param(NG, t0, g, q4 & 1);
   Walk walk;
   walk.start(b, s, bad);
   int seq, unit;
@@ -141,65 +215,48 @@ __global__ void __launch_bounds__(kThreads) append_kernel(Kv4Call c, Kv4Shape s,
     const int first = max(0, q.len - q.n - t * kTokens), last = min(kTokens, q.len - t * kTokens);  // its new tokens
     const bool whole = last - first == kTokens;
     // row of token i of the tile: row0 + i
-    const int64_t row0 = (int64_t)q.row0 + t * kTokens - (q.len - q.n);
-    const T *src = (const T *)(is_v ? c.v : c.k) + row0 * (is_v ? c.v_row : c.k_row) + (int64_t)kvh * (is_v ? c.v_head : c.k_head) + d;
-    const int64_t step = is_v ? c.v_row : c.k_row;
-    __syncwarp();  // the copies out of the last tile are done
+    const int64_t row0 = (int64_t)q.row0 + t * kTokens - (q.len - q.n) + t0;
+    const T *k = (const T *)c.k + row0 * c.k_row + (int64_t)kvh * c.k_head + d;
+    const T *v = (const T *)c.v + row0 * c.v_row + (int64_t)kvh * c.v_head + d;
+    const int from = lane_in ? first - t0 : PASSES, upto = last - t0;  // passes of this lane that have a token
+    const uint4 none = make_uint4(0, 0, 0, 0);
+    uint4 k_next[2], v_next[2];
+    auto fetch = [&](int p) {
 #pragma unroll
-    for (int p0 = 0; p0 < PASSES; p0 += BATCH) {
-      uint4 raw[BATCH];
-#pragma unroll
-      for (int p = 0; p < BATCH; ++p) {
-        const int tok = (p0 + p) * TP + sub;
-        raw[p] = in && tok >= first && tok < last ? *reinterpret_cast<const uint4 *>(src + tok * step) : make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < 2; ++i) {
+        const bool there = in && p + i >= from && p + i < upto;
+        k_next[i] = there ? *reinterpret_cast<const uint4 *>(k) : none;
+        v_next[i] = there ? *reinterpret_cast<const uint4 *>(v) : none;
+        k += c.k_row;
+        v += c.v_row;
       }
+    };
+    fetch(0);
+    __syncwarp();  // the copies out of the last tile are done
+    // the staged groups lie further apart
+    uint8_t *to = whole ? stage[warp] : page;
+    const int gap = whole ? kPad - 256 : 0;
+    uint8_t *kc = to + k_at + g * gap, *vc = to + v_at + (NG + g) * gap, *kp = to + kp_at + 2 * NG * gap, *vp = to + vp_at + 2 * NG * gap;
+#pragma unroll 1
+    for (int p = 0; p < PASSES; p += 2) {
+      uint4 k_raw[2], v_raw[2];
 #pragma unroll
-      for (int p = 0; p < BATCH; ++p) {
-        const int tok = (p0 + p) * TP + sub;
-        const T *e = reinterpret_cast<const T *>(&raw[p]);
-        float x[8], lo = INFINITY, hi = -INFINITY;
+      for (int i = 0; i < 2; ++i) k_raw[i] = k_next[i], v_raw[i] = v_next[i];
+      if (p + 2 < PASSES) fetch(p + 2);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          x[i] = (float)e[i];
-          if (in) {  // NaN stays
-            asm("min.NaN.f32 %0, %0, %1;" : "+f"(lo) : "f"(x[i]));
-            asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi) : "f"(x[i]));
-          }
-        }
-#pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
-          const float l = __shfl_xor_sync(0xffffffffu, lo, o), h = __shfl_xor_sync(0xffffffffu, hi, o);
-          asm("min.NaN.f32 %0, %0, %1;" : "+f"(lo) : "f"(l));
-          asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi) : "f"(h));
-        }
-        const bool fits = !lane_in || (lo >= -kLargest && hi <= kLargest) || d - q4 * 8 >= s.D;
+      for (int i = 0; i < 2; ++i) {
+        const Range rk = range_of<T>(k_raw[i], in), rv = range_of<T>(v_raw[i], in);
+        const bool fits = !in || (rk.fits() && rv.fits());
         const bool ok = (__ballot_sync(0xffffffffu, !fits) & token_lanes) == 0;
-        __half scale = __float2half_rn(__fdiv_rn(hi - lo, 15.0f)), least = __float2half_rn(lo);
-        if (!ok) scale = least = __ushort_as_half(is_v ? 0 : 0x7fff);
-        const float sc = __half2float(scale), mi = __half2float(least), inv = sc > 0.0f ? __fdiv_rn(1.0f, sc) : 0.0f;
-        uint32_t code[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float y = fminf(fmaxf(__fmul_rn(__fsub_rn(x[i], mi), inv), 0.0f), 15.0f);
-          // a sum with 1.5 * 2^23 is rounded to an integer, half to even, in the low bits; NaN became 0 above
-          code[i] = ok && in ? __float_as_uint(__fadd_rn(y, 12582912.0f)) & 15u : 0u;
-        }
-        if (lane_in && tok >= first && tok < last) {
-          uint8_t *to = whole ? stage[warp] : page;
-          const int gap = whole ? kPad - 256 : 0;  // the staged groups lie further apart
-          if (is_v) {
-            const uint32_t w0 = code[0] | code[1] << 4 | code[2] << 8 | code[3] << 12;
-            const uint32_t w1 = code[4] | code[5] << 4 | code[6] << 8 | code[7] << 12;
-            *(uint16_t *)(to + v_half(NG, tok, g, 2 * q4) + (NG + g) * gap) = (uint16_t)w0;
-            *(uint16_t *)(to + v_half(NG, tok, g, 2 * q4 + 1) + (NG + g) * gap) = (uint16_t)w1;
-          } else {
-            // neighbours in the halves of a word
-            *(uint32_t *)(to + k_word(tok, g, q4) + g * gap) = code[0] | code[1] << 16 | code[2] << 4 | code[3] << 20 | code[4] << 8 |
-                                                             code[5] << 24 | code[6] << 12 | code[7] << 28;
-          }
+        const Coded ck = coded<T, true>(k_raw[i], rk, in, ok, 0x7fff), cv = coded<T, false>(v_raw[i], rv, in, ok, 0);
+        if (p + i >= from && p + i < upto) {
+          const int n = p + i, m = row_of(n), vo = (n >> 2) * 8 + ((n >> 1) & 1) * 4 + (n & 1) * 2;
+          *(uint32_t *)(kc + (m & 7) * 32 + (m >> 3) * 4) = ck.word;
+          *(uint16_t *)(vc + vo) = (uint16_t)cv.word;
+          *(uint16_t *)(vc + vo + 32) = (uint16_t)(cv.word >> 16);
           if (q4 < 2) {
-            const int at = is_v ? v_param(NG, tok, g, q4) : k_param(NG, tok, g, q4);
-            *(__half *)(to + at + 2 * NG * gap) = q4 ? least : scale;
+            *(__half *)(kp + (m & 7) * 4 + (m >> 3) * 2) = q4 ? ck.least : ck.scale;
+            *(__half *)(vp + (n >> 2) * 16 + (n & 3) * 2) = q4 ? cv.least : cv.scale;
           }
         }
       }
@@ -303,9 +360,8 @@ unsigned grid_of(const Kv4Shape &s, const Kv4Rows &b, int64_t most) {
 
 template <typename T, int NG>
 cudaError_t launch(bool append, const Kv4Shape &s, const Kv4Rows &b, const Kv4Call &c, int *bad, int sms, cudaStream_t st) {
-  const unsigned grid = grid_of(s, b, (int64_t)sms * 4);
-  if (append) append_kernel<T, NG><<<grid, kThreads, 0, st>>>(c, s, b, bad);
-  else read_kernel<T, NG><<<grid, kThreads, 0, st>>>(c, s, b, bad);
+  if (append) append_kernel<T, NG><<<grid_of(s, b, (int64_t)sms * 3), kThreads, 0, st>>>(c, s, b, bad);
+  else read_kernel<T, NG><<<grid_of(s, b, (int64_t)sms * 4), kThreads, 0, st>>>(c, s, b, bad);
   return cudaGetLastError();
 }
 template <typename T>
