@@ -17,7 +17,7 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 CU = ["int4_matmul.cu", "attention.cu", "head.cu", "tc_gemm.cu", "tc_attn.cu", "ffn_noalloc.cu", "measure.cu",
       "int8_matmul.cu", "residual_norm.cu", "residual_norm_any.cu", "cross_attn.cu",
-      "kv4_cache.cu", "kv4_attn.cu", "verify.cu"]
+      "kv4_cache.cu", "kv4_attn.cu", "kv4_tile.cu", "verify.cu"]
 CPP = ["safetensors.cpp", "frontend.cpp", "engine.cpp", "capi.cpp", "ops.cpp", "tma_encode.cpp"]
 
 

@@ -1,0 +1,138 @@
+// attn_tile.cuh — pieces of the attention kernels whose products run on tcgen05: instruction
+// descriptors, TMEM accesses, the exponentials of a row.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "common.cuh"
+
+namespace ndl {
+
+// 2^x by the PTX base-2 exponential (a few ulp; results below 2^-126 become 0).
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool take) {
+  const int n = take ? 16 : 0;  // 0: the 16 bytes become zero and src is not read
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+// Instruction descriptor of 128 rows x n columns in 16-bit T with f32 sums, B K-major or MN-major.
+template <typename T>
+__host__ __device__ constexpr uint32_t f16_idesc(int n, bool b_mn) {
+  const uint32_t t = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  return (1u << 4) | (t << 7) | (t << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(128 >> 4) << 24);
+}
+
+__device__ __forceinline__ void tmem_ld32_raw(uint32_t taddr, uint32_t *r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ float fmax3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 2^t for a pair of t on the FMA units: t = j + f with j = round(t), 2^f on
+// [-1/2, 1/2] by a polynomial of degree 5 fitted here to the least relative
+// error with a constant term of 1 (1.1e-7 with these coefficients), times 2^j put together
+// from its exponent.  t at or below -127 gives 0, NaN stays NaN.
+__device__ __forceinline__ uint64_t ex2_fma(uint64_t t) {
+  const float magic = 12582912.0f + 127.0f;  // its sum with t holds j + 127 in the low bits
+  const uint64_t m2 = f2pack(magic, magic);
+  float a, b;
+  f2unpack(t, a, b);
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(a));  // -127
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(b));
+  t = f2pack(a, b);
+  const uint64_t z = fadd2(t, m2), f = fsub2(t, fsub2(z, m2));
+  uint64_t p = ffma2(f, f2pack(0.001326472731307149f, 0.001326472731307149f), f2pack(0.009671512991189957f, 0.009671512991189957f));
+  p = ffma2(p, f, f2pack(0.05550733581185341f, 0.05550733581185341f));
+  p = ffma2(p, f, f2pack(0.24022242426872253f, 0.24022242426872253f));
+  p = ffma2(p, f, f2pack(0.6931470036506653f, 0.6931470036506653f));
+  p = ffma2(p, f, f2pack(1.0f, 1.0f));
+  f2unpack(z, a, b);
+  return fmul2(p, f2pack(__uint_as_float(__float_as_uint(a) << 23), __uint_as_float(__float_as_uint(b) << 23)));
+}
+
+// 32 weights of a row: p = 2^(s c - m c), rounded and packed into w, their sum
+// added to `sum`.  The exponential unit gives 4 results a clock on an SM
+// partition and binds the kernel, so a quarter of the exponentials run on the FMA units.
+// The groups of 8 pairs, each one's arguments ahead of the previous one's
+// results, keep one warp at the unit's rate: alone / two warps a partition, a
+// clocked loop of 64 exponentials takes 534 / 887 clocks, without the polynomial 603 / 1067,
+// written pair by pair 1066 / 1194 (the unit: 512 / 1024).
+template <typename T>
+__device__ __forceinline__ void weights(const uint32_t *s, uint64_t cc, uint64_t nm, uint32_t *w, uint64_t *sum) {
+  constexpr int G = 8, FMA = 2;  // pairs of a group, those on the FMA units
+  uint64_t t[G];
+  auto arguments = [&](int g) {
+#pragma unroll
+    for (int i = 0; i < G; ++i)
+      t[i] = ffma2(f2pack(__uint_as_float(s[2 * (g * G + i)]), __uint_as_float(s[2 * (g * G + i) + 1])), cc, nm);
+  };
+  arguments(0);
+#pragma unroll
+  for (int g = 0; g < 16 / G; ++g) {
+    float p[2 * G];
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      if (i < G - FMA) {
+        f2unpack(t[i], p[2 * i], p[2 * i + 1]);
+        p[2 * i] = ex2(p[2 * i]);
+        p[2 * i + 1] = ex2(p[2 * i + 1]);
+      } else {
+        f2unpack(ex2_fma(t[i]), p[2 * i], p[2 * i + 1]);
+      }
+    }
+    if (g + 1 < 16 / G) arguments(g + 1);
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      sum[i & 1] = fadd2(sum[i & 1], f2pack(p[2 * i], p[2 * i + 1]));
+      w[g * G + i] = pack2<T>(p[2 * i], p[2 * i + 1]);
+    }
+  }
+}
+
+}  // namespace ndl

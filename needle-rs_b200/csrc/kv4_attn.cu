@@ -1,5 +1,5 @@
-// kv4_attn.cu — attention of query rows to a cache of keys and values in 4
-// bits:
+// kv4_attn.cu — attention of a few query rows to a cache of keys and values in
+// 4 bits (many rows: kv4_tile.cu):
 //   s_j = scale * q . k_j     out = sum_j e^(s_j) v_j / sum_j e^(s_j)
 // with k = m + s c and v = m + s c of each group of 32 dimensions.
 //
@@ -24,8 +24,9 @@
 
 #include <algorithm>
 
+#include "attn_tile.cuh"
 #include "common.cuh"
-#include "kv4.cuh"
+#include "kv4_share.cuh"
 #include "ops.h"
 #include "rowio.cuh"
 
@@ -34,21 +35,10 @@ namespace {
 
 using namespace kv4;
 
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kWarps = 4, kThreads = kWarps * 32;
-constexpr int kUnit = 64;  // keys of a unit of work
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
 __device__ __forceinline__ __half2 halves(uint32_t u) { return *reinterpret_cast<__half2 *>(&u); }
-__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool take) {
-  const int n = take ? 16 : 0;  // 0: the 16 bytes become zero and src is not read
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
 __device__ __forceinline__ void mma(float *d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -68,34 +58,17 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   return y;
 }
 
-// How the units of a call fall to the blocks: request i has KVH heads x blocks
-// of ROWS rows ("items") x units of 64 keys, and block b of n takes units
-// [total * b / n, total * (b + 1) / n) of all requests' in order.  A border inside
-// an item of at most a block's share moves to that item's nearer end: such items stay
-// whole, and longer ones are cut and joined.  Units count in 32 bits: a thread's
-// requests have less than 2^25.
-struct Units {
-  Seq q;
-  int row_blocks, keys;  // `keys`: units of an item
+// A request's items: its rows with each KV head.
+struct FewItems {
+  int KVH;
 
-  __device__ uint32_t all(int KVH) const { return (uint32_t)row_blocks * KVH * keys; }
-};
-template <int ROWS>
-__device__ __forceinline__ Units units_of(const Kv4Rows &b, const Kv4Shape &s, int i, bool causal, int *bad) {
-  Units u;
-  u.q = sequence(b, s, i, causal, bad);
-  u.row_blocks = (u.q.n * (s.H / s.KVH) + ROWS - 1) / ROWS;
-  u.keys = max(1, (u.q.len + kUnit - 1) / kUnit);
-  if ((int64_t)u.row_blocks * s.KVH * u.keys >= 1 << 25) {
-    *bad = 1;
-    u.row_blocks = 0;
+  __device__ uint32_t units(const Seq &q) const { return max(1, (q.len + kUnit - 1) / kUnit); }
+  __device__ uint64_t all(const Seq &q) const { return q.n ? (uint64_t)units(q) * KVH : 0; }
+  __device__ void item(const Seq &q, uint32_t at, uint32_t *first, uint32_t *n) const {
+    *n = units(q);
+    *first = at - at % *n;
   }
-  return u;
-}
-struct Share {
-  uint32_t total, begin, end, base;  // base: units before request `seq`, the one that `begin` falls in
-  int blocks, seq;
-  Units un;  // of request `seq`
+  __device__ uint32_t snap(uint32_t share) const { return share; }
 };
 
 // Partial results of items that are cut between blocks: two slots a block (the
@@ -106,67 +79,9 @@ __device__ __forceinline__ float *slot_of(const Kv4Work &w, int block, int which
   return w.ws + ((int64_t)block * 2 + which) * (ROWS * (DP + 2));
 }
 
-template <int ROWS>
-__device__ __forceinline__ void share_of(const Kv4Rows &b, const Kv4Shape &s, bool causal, const Kv4Work &w, Share *share) {
-  __shared__ uint32_t sums[kWarps];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int per = (b.n_seq + kThreads - 1) / kThreads, i0 = min((int)threadIdx.x * per, b.n_seq), i1 = min(i0 + per, b.n_seq);
-  uint32_t mine = 0;
-  Units u;
-  for (int i = i0; i < i1; ++i) {
-    u = units_of<ROWS>(b, s, i, causal, w.bad);
-    mine = min(mine + u.all(s.KVH), (1u << 25) - 1);
-  }
-  uint32_t upto = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += x;
-  }
-  if (lane == 31) sums[warp] = upto;
-  __syncthreads();
-  uint32_t total = 0;
-#pragma unroll
-  for (int k = 0; k < kWarps; ++k) {
-    if (k < warp) upto += sums[k];
-    total += sums[k];
-  }
-  const uint32_t blocks = min(gridDim.x, (total + 1) / 2), me = blockIdx.x;  // a block has two units at least
-  if (threadIdx.x == 0) {
-    share->total = total;
-    share->blocks = (int)blocks;
-    share->end = total;
-  }
-  __syncthreads();
-  if (me >= blocks) return;
-  const uint32_t whole = total / blocks, rest = total - whole * blocks;
-  const uint32_t lo = whole * me + rest * me / blocks, hi = whole * (me + 1) + rest * (me + 1) / blocks;
-  const uint32_t before = upto - mine;
-  if (before <= hi && lo < upto) {
-    uint32_t base = before;
-    for (int i = i0; i < i1; ++i) {
-      if (per > 1) u = units_of<ROWS>(b, s, i, causal, w.bad);
-      const uint32_t next = min(base + u.all(s.KVH), upto);
-      auto border = [&](uint32_t x) {
-        const uint32_t in = (x - base) % u.keys;
-        return u.keys > whole ? x : in * 2 < (uint32_t)u.keys ? x - in : x - in + u.keys;
-      };
-      if (base <= lo && lo < next) {
-        share->begin = border(lo);
-        share->base = base;
-        share->seq = i;
-        share->un = u;
-      }
-      if (base <= hi && hi < next) share->end = border(hi);
-      base = next;
-    }
-  }
-  __syncthreads();
-}
-
 // A warp's ring holds pairs of tiles (32 keys a turn); stages of it, and blocks an SM.
 __host__ __device__ constexpr int few_stages(int ng) { return ng == 4 ? 2 : ng == 3 ? 3 : 4; }
-__host__ __device__ constexpr int few_blocks(int nb) { return nb == 1 ? 4 : nb == 2 ? 3 : 2; }
+__host__ __device__ constexpr int few_blocks(int nb) { return nb == 1 ? 4 : 3; }
 template <int NG, int NB>
 __host__ __device__ constexpr int few_smem() {
   constexpr int ring = kWarps * few_stages(NG) * 2 * tile_bytes(NG), merge = kWarps * NB * 8 * (NG * 32 + 4 + 2) * 4;
@@ -181,7 +96,8 @@ __global__ void __launch_bounds__(kThreads, few_blocks(NB))
   extern __shared__ __align__(128) uint8_t sm[];
   __shared__ int last_one;
   __shared__ Share share;
-  share_of<ROWS>(b, s, c.causal, w, &share);
+  const FewItems few{s.KVH};
+  share_of<FewItems, kWarps>(few, b, s, c.causal, w.bad, &share);
   if (blockIdx.x >= share.blocks) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, q4 = lane & 3;
   const int G = s.H / s.KVH, D = s.D;
@@ -189,33 +105,20 @@ __global__ void __launch_bounds__(kThreads, few_blocks(NB))
 
   int seq = share.seq;
   uint32_t base = share.base, at = share.begin;
-  Units un = share.un;
+  Seq rq = share.q;
   while (at < share.end) {
-    if (at >= base + un.all(s.KVH)) {  // on to the next request with rows, 32 at a time
-      base += un.all(s.KVH);
-      for (++seq; seq < b.n_seq; seq += 32) {
-        const Units next = units_of<ROWS>(b, s, min(seq + lane, b.n_seq - 1), c.causal, w.bad);
-        const uint32_t any = __ballot_sync(0xffffffffu, seq + lane < b.n_seq && next.row_blocks > 0);
-        if (any) {
-          const int from = __ffs(any) - 1;
-          seq += from;
-          un.q.row0 = __shfl_sync(0xffffffffu, next.q.row0, from);
-          un.q.n = __shfl_sync(0xffffffffu, next.q.n, from);
-          un.q.len = __shfl_sync(0xffffffffu, next.q.len, from);
-          un.row_blocks = __shfl_sync(0xffffffffu, next.row_blocks, from);
-          un.keys = __shfl_sync(0xffffffffu, next.keys, from);
-          break;
-        }
-      }
+    const uint32_t all = (uint32_t)few.all(rq);
+    if (at >= base + all) {
+      base += all;
+      seq = next_request(few, b, s, seq, c.causal, w.bad, &rq);
       if (seq >= b.n_seq) break;
     }
-    const uint32_t item = (at - base) / un.keys, first = base + item * un.keys;
-    const int u0 = (int)(at - first), u1 = (int)min((uint32_t)un.keys, share.end - first);
+    const uint32_t units = few.units(rq), item = (at - base) / units, first = base + item * units;
+    const int u0 = (int)(at - first), u1 = (int)min(units, share.end - first);
     at = first + u1;
-    const int rb = (int)item / s.KVH, kvh = (int)item - rb * s.KVH, r0 = rb * ROWS;
-    const int rows = min(ROWS, un.q.n * G - r0), len = un.q.len;
+    const int kvh = (int)item, rows = rq.n * G, len = rq.len;
     // keys that row x of the block sees
-    auto limit = [&](int x) { return c.causal ? len - un.q.n + (r0 + min(x, rows - 1)) / G + 1 : len; };
+    auto limit = [&](int x) { return c.causal ? len - rq.n + min(x, rows - 1) / G + 1 : len; };
     const int k_all = limit(0);  // every row sees these
     const int t0 = u0 * (kUnit / kTokens);
     const int t1 = min(u1 * (kUnit / kTokens), (limit(rows - 1) + kTokens - 1) / kTokens);
@@ -226,8 +129,8 @@ __global__ void __launch_bounds__(kThreads, few_blocks(NB))
     uint4 raw[NB][NG];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const int x = nb * 8 + r, row = r0 + x;
-      const T *q = (const T *)c.q + (un.q.row0 + row / G) * c.q_row + (int64_t)(kvh * G + row % G) * c.q_head;
+      const int x = nb * 8 + r;
+      const T *q = (const T *)c.q + (rq.row0 + x / G) * c.q_row + (int64_t)(kvh * G + x % G) * c.q_head;
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         const int d = g * 32 + q4 * 8;
@@ -280,7 +183,7 @@ __global__ void __launch_bounds__(kThreads, few_blocks(NB))
         asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(other));
       }
       // 2^e brings the largest value to [2^10, 2^11); infinities and NaN make the row NaN
-      const int e2 = min(100, 137 - (int)(__float_as_uint(top) >> 23));
+      const int e2 = min(60, 137 - (int)(__float_as_uint(top) >> 23));
       const float mul = top <= 3.402823466e38f ? __uint_as_float((uint32_t)(e2 + 127) << 23) : __uint_as_float(0x7fc00000u);
       const float factor = c.scale * kLog2e * 16777216.0f * __uint_as_float((uint32_t)(127 - e2) << 23);
       float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -512,11 +415,11 @@ __global__ void __launch_bounds__(kThreads, few_blocks(NB))
         }
       }
     __syncthreads();
-    const bool whole = u0 == 0 && u1 == un.keys;
+    const bool whole = u0 == 0 && u1 == (int)units;
     const int quads = D / 4;
     auto finish = [&](int x, int d, float4 v, float M, float L) {
-      const int row = r0 + x, h = kvh * G + row % G;
-      const int64_t at_row = un.q.row0 + row / G;
+      const int h = kvh * G + x % G;
+      const int64_t at_row = rq.row0 + x / G;
       const float inv = L == 0.0f ? 0.0f : 1.0f / L;  // no key: zeros
       alignas(8) T out[4] = {from_f32<T>(v.x * inv), from_f32<T>(v.y * inv), from_f32<T>(v.z * inv), from_f32<T>(v.w * inv)};
       *reinterpret_cast<uint2 *>((T *)c.out + at_row * c.o_row + (int64_t)h * c.o_head + d) = *reinterpret_cast<uint2 *>(out);
@@ -552,8 +455,7 @@ __global__ void __launch_bounds__(kThreads, few_blocks(NB))
     }
     if (!whole) {
       // the blocks that hold parts of this item; the last to arrive joins them in their order
-      auto block_of = [&](uint32_t unit) { return (int)((((uint64_t)unit + 1) * share.blocks - 1) / share.total); };
-      const int b0 = block_of(first), parts = block_of(first + un.keys - 1) - b0 + 1;
+      const int b0 = block_of(share, first), parts = block_of(share, first + units - 1) - b0 + 1;
       __threadfence();
       __syncthreads();
       if (threadIdx.x == 0) {
@@ -639,10 +541,7 @@ cudaError_t launch_few(const Kv4Shape &s, const Kv4Rows &b, const Kv4AttnCall &c
 
 template <typename T, int NG>
 cudaError_t run(const Kv4Shape &s, const Kv4Rows &b, const Kv4AttnCall &c, const Kv4Work &w, cudaStream_t st) {
-  const int64_t rows = (int64_t)b.max_new * (s.H / s.KVH);
-  if (rows <= 8) return launch_few<T, NG, 1>(s, b, c, w, st);
-  if (rows <= 16) return launch_few<T, NG, 2>(s, b, c, w, st);
-  return launch_few<T, NG, 4>(s, b, c, w, st);
+  return (int64_t)b.max_new * (s.H / s.KVH) <= 8 ? launch_few<T, NG, 1>(s, b, c, w, st) : launch_few<T, NG, 2>(s, b, c, w, st);
 }
 
 template <typename T>
@@ -657,16 +556,18 @@ cudaError_t run(const Kv4Shape &s, const Kv4Rows &b, const Kv4AttnCall &c, const
 
 }  // namespace
 
-int64_t kv4_attn_blocks(int sms) { return (int64_t)sms * few_blocks(1); }
+int64_t kv4_attn_counters(int sms) { return (int64_t)sms * std::max(few_blocks(1), kTileCounters); }
 
 int64_t kv4_attn_floats(const Kv4Shape &s, int sms) {
-  int64_t most = 0;
-  for (int nb : {1, 2, 4}) most = std::max(most, (int64_t)sms * few_blocks(nb) * 2 * nb * 8 * (s.ng * 32 + 2));
+  int64_t most = kv4_tile_floats(s, sms);
+  for (int nb : {1, 2}) most = std::max(most, (int64_t)sms * few_blocks(nb) * 2 * nb * 8 * (s.ng * 32 + 2));
   return most;
 }
 
+// Up to 16 rows of a KV head read the cache faster than tiles would; 17 are a tile.
 cudaError_t kv4_attn(const Kv4Shape &s, const Kv4Rows &b, const Kv4AttnCall &c, const Kv4Work &w, cudaStream_t st) {
   if (b.rows == 0) return cudaSuccess;
+  if ((int64_t)b.max_new * (s.H / s.KVH) > 16) return kv4_attn_tiles(s, b, c, w, st);
   return s.dtype == DT_F16 ? run<__half>(s, b, c, w, st) : run<__nv_bfloat16>(s, b, c, w, st);
 }
 

@@ -1,0 +1,611 @@
+// kv4_tile.cu — attention of many query rows (prompt chunks, longer drafts) to
+// a cache of keys and values in 4 bits, on tcgen05.
+//
+// Up to 256 packed rows of a request and KV head (two tiles of 128) share every
+// key that is read: four warps turn 64 keys and values of 4 bits into f16 operands in shared
+// memory while two others issue the products of the 64 keys before, and eight turn
+// scores into weights, a thread a row:
+//   S = Q K^T     M128 N64, both K-major in shared memory
+//   P = weights   TMEM, f16, over S
+//   O += P V      M128 N 64 or 128, P from TMEM, V MN-major
+// S has two buffers a tile of rows.  m moves only when a row's maximum passes it by 2^8,
+// and O is rescaled then: a weight is at most 256.
+//
+// q is brought to a largest value of 2^10 .. 2^11 by a power of two for each row and
+// taken as f16 (exact, but for values below 2^-24 of the row's largest); keys and values are
+// minimum + scale * code, rounded to f16 once.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "attn_tile.cuh"
+#include "common.cuh"
+#include "kv4_share.cuh"
+#include "ops.h"
+#include "rowio.cuh"
+#include "tc_common.cuh"
+
+namespace ndl {
+namespace {
+
+using namespace kv4;
+using namespace tc;
+
+constexpr int kRows = 256, kHalf = 128, kKeys = kUnit, kWarps = 14, kThreads = kWarps * 32;
+constexpr int kSoftmaxWarps = 8, kCodeWarps = 4;  // then the issuers of S and of O
+
+template <int NG>
+struct Tile {
+  static constexpr int kAtoms = NG <= 2 ? 1 : 2;  // 64-dimension parts of a row (128 bytes each)
+  static constexpr int kQAtom = kHalf * 128, kAtom = kKeys * 128, kQBytes = kAtoms * kQAtom, kBytes = kAtoms * kAtom;
+  static constexpr int kStages = 3;  // of K, and of V
+  static constexpr int kQ = 0, kK = 2 * kQBytes, kV = kK + kStages * kBytes, kBar = kV + kStages * kBytes;
+  static constexpr int kSmem = kBar + 512 + 1024;
+  static constexpr int kDims = 64 * kAtoms;  // columns of O
+  // TMEM columns: two S of each half (P over each), then O of each half
+  static constexpr int kO = 4 * kKeys, kCols = 512;
+};
+
+// A request's items: blocks of 256 of its packed rows, each with every KV head.
+struct TileItems {
+  int KVH, G;
+  bool causal;
+
+  __device__ int blocks(const Seq &q) const { return (int)(((int64_t)q.n * G + kRows - 1) / kRows); }
+  __device__ int rows(const Seq &q, int rb) const { return min(kRows, q.n * G - rb * kRows); }
+  // Keys that row x of a request's packed rows sees.
+  __device__ int keys(const Seq &q, int x) const { return causal ? q.len - q.n + x / G + 1 : q.len; }
+  __device__ uint32_t units(const Seq &q, int rb) const {
+    return max(1, (keys(q, rb * kRows + rows(q, rb) - 1) + kKeys - 1) / kKeys);
+  }
+  __device__ uint64_t all(const Seq &q) const {
+    uint64_t n = 0;
+    for (int rb = 0; rb < blocks(q); ++rb) n += units(q, rb);
+    return n * KVH;
+  }
+  __device__ void place(const Seq &q, uint32_t at, uint32_t *first, uint32_t *n, int *rb, int *kvh) const {
+    uint32_t base = 0;
+    for (int k = 0;; ++k) {
+      const uint32_t u = units(q, k);
+      if (at < base + u * KVH || k + 1 >= blocks(q)) {
+        *n = u;
+        *rb = k;
+        *kvh = (int)min((at - base) / u, (uint32_t)KVH - 1);
+        *first = base + *kvh * u;
+        return;
+      }
+      base += u * KVH;
+    }
+  }
+  __device__ void item(const Seq &q, uint32_t at, uint32_t *first, uint32_t *n) const {
+    int rb, kvh;
+    place(q, at, first, n, &rb, &kvh);
+  }
+  // cutting costs two partial results of 256 rows and their join: some tens of units
+  __device__ uint32_t snap(uint32_t share) const { return min(share, 24u); }
+};
+
+// A block's items one after another; every role of the block walks them by itself.
+struct Walk {
+  TileItems p;
+  uint32_t at, end, base;
+  int seq;
+  Seq q;
+  // the item
+  uint32_t first, units;
+  int u0, u1, kvh, r0, rows;
+
+  __device__ Walk(const TileItems &items, const Share &s) : p(items), at(s.begin), end(s.end), base(s.base), seq(s.seq), q(s.q) {}
+  __device__ bool next(const Kv4Rows &b, const Kv4Shape &s, int *bad) {
+    if (at >= end) return false;
+    const uint32_t all = (uint32_t)p.all(q);
+    if (at >= base + all) {
+      base += all;
+      seq = next_request(p, b, s, seq, p.causal, bad, &q);
+      if (seq >= b.n_seq) return false;
+    }
+    int rb;
+    p.place(q, at - base, &first, &units, &rb, &kvh);
+    first += base;
+    u0 = (int)(at - first);
+    u1 = (int)min(units, end - first);
+    at = first + u1;
+    r0 = rb * kRows;
+    rows = p.rows(q, rb);
+    return true;
+  }
+  __device__ bool no_keys() const { return p.keys(q, r0 + rows - 1) == 0; }
+  __device__ int halves() const { return rows > kHalf ? 2 : 1; }
+  __device__ int tiles() const { return no_keys() ? 0 : u1 - u0; }
+};
+
+// Partial rows of cut items: [256][DP] sums, then m and l of each.
+template <int DP>
+__device__ __forceinline__ float *slot_of(const Kv4Work &w, int block, int which) {
+  return w.ws + ((int64_t)block * 2 + which) * (kRows * (DP + 2));
+}
+
+__device__ __forceinline__ uint32_t and_or(uint32_t u, uint32_t mask, uint32_t c) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(u), "r"(mask), "r"(c));
+  return d;
+}
+__device__ __forceinline__ __half2 pair(uint32_t u) { return *reinterpret_cast<__half2 *>(&u); }
+__device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
+
+// Four pairs of codes of a word (nibbles i and i + 4) as s * c + m: 1024 + c (or 64 + c) by an OR, minus that, exactly;
+// one rounding at the end.
+__device__ __forceinline__ void values(uint32_t w, __half2 s, __half2 m, uint32_t i1024, uint32_t i64, uint32_t *v) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t u = k < 2 ? w : w >> 8;
+    const __half2 c = k & 1 ? __hsub2(pair(and_or(u, 0x00f000f0u, i64)), pair(i64)) : __hsub2(pair(and_or(u, 0x000f000fu, i1024)), pair(i1024));
+    v[k] = bits(__hfma2(c, s, m));
+  }
+}
+
+// 16 tokens of 4 bits on their way, a lane's share.
+template <int NG>
+struct Codes {
+  uint2 k[NG], v[NG];
+  uint32_t ks[NG], km[NG];
+  uint4 vp[NG];
+  int left;  // tokens of the request among them
+
+  __device__ __forceinline__ void fetch(const uint8_t *tile, int lane) {
+    const int r = lane >> 2, q4 = lane & 3;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      k[g] = *reinterpret_cast<const uint2 *>(tile + g * 256 + lane * 8);
+      v[g] = *reinterpret_cast<const uint2 *>(tile + v_codes(NG) + g * 256 + lane * 8);
+      ks[g] = *reinterpret_cast<const uint32_t *>(tile + k_params(NG) + (g * 8 + r) * 4);
+      km[g] = *reinterpret_cast<const uint32_t *>(tile + k_params(NG) + ((NG + g) * 8 + r) * 4);
+      vp[g] = *reinterpret_cast<const uint4 *>(tile + v_params(NG) + (g * 4 + q4) * 16);
+    }
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      k[g] = v[g] = make_uint2(0, 0);
+      ks[g] = km[g] = 0;
+      vp[g] = make_uint4(0, 0, 0, 0);
+    }
+  }
+  // Behind the last token a page may hold anything.
+  __device__ __forceinline__ void cut(int q4) {
+    const int n = left - 4 * q4;
+    const uint32_t a = n >= 2 ? 0xffffffffu : n == 1 ? 0xffffu : 0u, b = n >= 4 ? 0xffffffffu : n == 3 ? 0xffffu : 0u;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      vp[g].x &= a;
+      vp[g].z &= a;
+      vp[g].y &= b;
+      vp[g].w &= b;
+    }
+  }
+};
+
+template <typename T, int NG>
+__global__ void __launch_bounds__(kThreads, 1) tile_kernel(Kv4AttnCall c, Kv4Shape s, Kv4Rows b, Kv4Work w) {
+  using L = Tile<NG>;
+  constexpr int ST = L::kStages, DP = NG * 32;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t *sm = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t *k_full = (uint64_t *)(sm + L::kBar), *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST;
+  uint64_t *q_full = v_empty + ST, *o_free = q_full + 2, *s_full = o_free + 2, *p_full = s_full + 4, *pv_done = p_full + 4,
+           *done = pv_done + 4;  // [half]; [half][buffer]; done: of a warp's MMAs in flight, after a wait that ran out
+  uint32_t *tmem_slot = (uint32_t *)(done + 2);
+  __shared__ Share share;
+  int *err = w.err;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = s.H / s.KVH, D = s.D;
+  const TileItems items{s.KVH, G, c.causal};
+  share_of<TileItems, kWarps>(items, b, s, c.causal, w.bad, &share);
+  if (blockIdx.x >= share.blocks) return;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(&k_full[i], kCodeWarps);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], kCodeWarps);
+      mbar_init(&v_empty[i], 1);
+    }
+    for (int h = 0; h < 2; ++h) {
+      mbar_init(&q_full[h], 4);
+      mbar_init(&o_free[h], 4);
+      mbar_init(&done[h], 1);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&pv_done[i], 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kSoftmaxWarps + kCodeWarps) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(L::kCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const uint32_t tmem = *(volatile uint32_t *)tmem_slot;
+  bool ok = true;
+  Walk walk(items, share);
+
+  if (warp < kSoftmaxWarps) {
+    const int half = warp >> 2, quarter = warp & 3, i = quarter * 32 + lane;  // this thread's row of its half
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16, tO = tmem + lanes + (uint32_t)(L::kO + half * L::kDims);
+    uint8_t *q_to = sm + L::kQ + half * L::kQBytes + i * 128;
+    int t = 0;  // tiles of this half
+    while (ok && walk.next(b, s, w.bad)) {
+      if (half >= walk.halves()) continue;
+      const int nt = walk.tiles(), x = half * kHalf + i, row = walk.r0 + x;
+      const bool mine = x < walk.rows, any = half * kHalf + quarter * 32 < walk.rows;
+      const int64_t token = walk.q.row0 + row / G;
+      const int h = walk.kvh * G + row % G;
+      const int lim = items.keys(walk.q, walk.r0 + min(x, walk.rows - 1));  // keys that the row sees
+      const int lim_least = __shfl_sync(0xffffffffu, lim, 0);
+      float sc = c.scale * kLog2e;
+      if (nt > 0) {
+        // the row of Q, brought to f16's range, K-major with the 128-byte swizzle
+        const T *q = (const T *)c.q + token * c.q_row + (int64_t)h * c.q_head;
+        uint4 raw[DP / 8];
+        float top = 0.0f;
+#pragma unroll
+        for (int ch = 0; ch < DP / 8; ++ch)
+          raw[ch] = mine && ch * 8 < D ? *reinterpret_cast<const uint4 *>(q + ch * 8) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int ch = 0; ch < DP / 8; ++ch) {
+          const T *e = reinterpret_cast<const T *>(&raw[ch]);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf((float)e[k])));
+        }
+        const int e2 = min(60, 137 - (int)(__float_as_uint(top) >> 23));
+        const float mul = top <= 3.402823466e38f ? __uint_as_float((uint32_t)(e2 + 127) << 23) : __uint_as_float(0x7fc00000u);
+        sc *= __uint_as_float((uint32_t)(127 - e2) << 23);
+#pragma unroll
+        for (int ch = 0; ch < DP / 8; ++ch) {
+          const T *e = reinterpret_cast<const T *>(&raw[ch]);
+          uint32_t u[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) u[k] = pack2<__half>((float)e[2 * k] * mul, (float)e[2 * k + 1] * mul);
+          *reinterpret_cast<uint4 *>(q_to + (ch >> 3) * L::kQAtom + (((ch & 7) ^ (lane & 7)) << 4)) = make_uint4(u[0], u[1], u[2], u[3]);
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full[half]);
+      }
+      float m = -INFINITY, l = 0.0f;
+      for (int j = 0; j < nt; ++j, ++t) {
+        const int buf = 2 * half + (t & 1), j0 = (walk.u0 + j) * kKeys;
+        if (!(ok = warp_wait(&s_full[buf], (uint32_t)(t >> 1) & 1, err))) break;
+        tc_after();
+        if (any) {
+          const uint32_t tS = tmem + lanes + (uint32_t)(buf * kKeys);
+          uint32_t x[kKeys];
+          tmem_ld32_raw(tS, x);
+          tmem_ld32_raw(tS + 32, x + 32);
+          tmem_wait_ld();
+          if (j0 + kKeys > lim_least) {
+#pragma unroll
+            for (int e = 0; e < kKeys; ++e)
+              if (j0 + e >= lim) x[e] = 0xff800000u;
+          }
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int e = 0; e < kKeys; e += 2)
+            mx[(e >> 1) & 3] = fmax3(mx[(e >> 1) & 3], __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          const bool move = (top - m) * sc > 8.0f;  // also at the first key that it sees (m = -inf)
+          float f = 1.0f;
+          if (move) {
+            f = ex2((m - top) * sc);
+            m = top;
+            l *= f;
+          }
+          if (j > 0 && __any_sync(0xffffffffu, move)) {
+            if (!(ok = warp_wait(&pv_done[2 * half + ((t - 1) & 1)], (uint32_t)((t - 1) >> 1) & 1, err))) break;
+            tc_after();
+#pragma unroll 1
+            for (int q = 0; q < DP / 16; ++q) {
+              uint32_t o[16];
+              asm volatile(
+                  "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+                  "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                  : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]), "=r"(o[4]), "=r"(o[5]), "=r"(o[6]), "=r"(o[7]),
+                    "=r"(o[8]), "=r"(o[9]), "=r"(o[10]), "=r"(o[11]), "=r"(o[12]), "=r"(o[13]), "=r"(o[14]), "=r"(o[15])
+                  : "r"(tO + 16 * q));
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st16(tO + 16 * q, o);
+            }
+          }
+          const float mc = m == -INFINITY ? 0.0f : m * sc;
+          const uint64_t cc = f2pack(sc, sc), nm = f2pack(-mc, -mc);
+          uint64_t sum[2] = {f2pack(0.0f, 0.0f), f2pack(0.0f, 0.0f)};
+          __syncwarp();  // TMEM is read and written by whole warps
+#pragma unroll
+          for (int q = 0; q < kKeys / 32; ++q) {
+            uint32_t pw[16];
+            weights<__half>(x + 32 * q, cc, nm, pw, sum);
+            tmem_st16(tS + 16 * q, pw);
+          }
+          float l0, l1;
+          f2unpack(fadd2(sum[0], sum[1]), l0, l1);
+          l += l0 + l1;
+          tmem_wait_st();
+        }
+        tc_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[buf]);
+      }
+      if (!ok) break;
+      if (nt > 0 && !(ok = warp_wait(&pv_done[2 * half + ((t - 1) & 1)], (uint32_t)((t - 1) >> 1) & 1, err))) break;
+      tc_after();
+      const bool whole = walk.u0 == 0 && walk.u1 == (int)walk.units;
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
+      T *out = (T *)c.out + token * c.o_row + (int64_t)h * c.o_head;
+      float *p = slot_of<DP>(w, blockIdx.x, walk.u0 == 0 ? 1 : 0);
+#pragma unroll
+      for (int q = 0; q < DP / 32; ++q) {
+        uint32_t o[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = 0;
+        __syncwarp();  // rows past the item's left the last turn early
+        if (nt > 0) {
+          tmem_ld32_raw(tO + 32 * q, o);
+          tmem_wait_ld();
+          if (q == DP / 32 - 1) {
+            tc_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&o_free[half]);
+          }
+        }
+        if (!mine) continue;
+        if (!whole) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            __stcg(reinterpret_cast<uint4 *>(p + (int64_t)x * DP + 32 * q + e), make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            if (32 * q + e >= D) break;
+            uint32_t u[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              u[k] = pack2<T>(__uint_as_float(o[e + 2 * k]) * inv, __uint_as_float(o[e + 2 * k + 1]) * inv);
+            *reinterpret_cast<uint4 *>(out + 32 * q + e) = make_uint4(u[0], u[1], u[2], u[3]);
+          }
+        }
+      }
+      if (mine) {
+        if (!whole) {
+          __stcg(p + kRows * DP + x, m * sc);
+          __stcg(p + kRows * (DP + 1) + x, l);
+        } else if (c.lse) {
+          c.lse[token * s.H + h] = l == 0.0f ? -INFINITY : fmaf(m * sc, kLn2, logf(l));
+        }
+      }
+      if (!whole && any) {
+        // a warp's rows by themselves: the last warp to arrive with a part of them joins the parts in their order
+        const int b0 = block_of(share, walk.first), parts = block_of(share, walk.first + walk.units - 1) - b0 + 1;
+        __threadfence();
+        __syncwarp();
+        int last = 0;
+        if (lane == 0) {
+          int *counter = w.counters + (int64_t)b0 * kTileCounters + warp;
+          last = atomicAdd(counter, 1) == parts - 1;
+          if (last) *counter = 0;
+          __threadfence();
+        }
+        if (__shfl_sync(0xffffffffu, last, 0)) {
+          const int x0 = half * kHalf + quarter * 32, n = min(32, walk.rows - x0), d = lane * 4;
+          for (int k = 0; k < n; ++k) {
+            const int xr = x0 + k, rr = walk.r0 + xr, hr = walk.kvh * G + rr % G;
+            const int64_t tr = walk.q.row0 + rr / G;
+            auto part = [&](int z) { return slot_of<DP>(w, b0 + z, z == 0 ? 1 : 0); };
+            float M = -INFINITY, L = 0.0f;
+            for (int z = 0; z < parts; ++z) M = fmaxf(M, __ldcg(part(z) + kRows * DP + xr));
+            const float from = M == -INFINITY ? 0.0f : M;
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+            for (int z = 0; z < parts; ++z) {
+              const float g = ex2(__ldcg(part(z) + kRows * DP + xr) - from);
+              L += g * __ldcg(part(z) + kRows * (DP + 1) + xr);
+              if (d < D) {
+                const float4 y = __ldcg(reinterpret_cast<const float4 *>(part(z) + (int64_t)xr * DP + d));
+                v.x += g * y.x;
+                v.y += g * y.y;
+                v.z += g * y.z;
+                v.w += g * y.w;
+              }
+            }
+            const float one = L == 0.0f ? 0.0f : 1.0f / L;
+            if (d < D)
+              *reinterpret_cast<uint2 *>((T *)c.out + tr * c.o_row + (int64_t)hr * c.o_head + d) =
+                  make_uint2(pack2<T>(v.x * one, v.y * one), pack2<T>(v.z * one, v.w * one));
+            if (lane == 0 && c.lse) c.lse[tr * s.H + hr] = L == 0.0f ? -INFINITY : fmaf(M, kLn2, logf(L));
+          }
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp < kSoftmaxWarps + kCodeWarps) {
+    // 4 bits to f16: a warp for each 16 tokens of a tile, one tile ahead in registers
+    const int part = warp - kSoftmaxWarps, r = lane >> 2, q4 = lane & 3;
+    const int ta = 16 * part + 4 * (r >> 1) + (r & 1);  // the token of K's row r; that of r + 8 is 2 on
+    uint32_t i1024, i64;  // in registers: an AND and an OR with it are one instruction
+    asm volatile("mov.b32 %0, 0x64006400;" : "=r"(i1024));
+    asm volatile("mov.b32 %0, 0x54005400;" : "=r"(i64));
+    Codes<NG> now, ahead;
+    int j = 0, nt = 0;
+    bool more = true;
+    auto fetch = [&]() {  // the next tile's codes; false behind the last
+      while (more && j >= nt) {
+        more = walk.next(b, s, w.bad);
+        nt = more ? walk.tiles() : 0;
+        j = 0;
+      }
+      if (!more) return false;
+      const int at = (walk.u0 + j++) * kKeys + 16 * part;
+      ahead.left = walk.q.len - at;
+      const uint8_t *tile = ahead.left > 0 ? tile_at((uint8_t *)c.pages, b, s, walk.seq, at / kTokens, walk.kvh, w.bad) : nullptr;
+      if (tile) ahead.fetch(tile, lane);
+      else ahead.clear();
+      return true;
+    };
+    bool have = fetch();
+    for (int t = 0; have; ++t) {
+      now = ahead;
+      have = fetch();
+      const int st = t % ST;
+      const uint32_t ph = (uint32_t)(t / ST) & 1;
+      if (now.left < kTokens) now.cut(q4);
+      if (!(ok = warp_wait(&k_empty[st], ph ^ 1, err))) break;
+      uint8_t *K = sm + L::kK + st * L::kBytes, *V = sm + L::kV + st * L::kBytes;
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t sel = h ? 0x3232 : 0x1010;
+          uint32_t v[4];
+          values(h ? now.k[g].y : now.k[g].x, pair(__byte_perm(now.ks[g], 0, sel)), pair(__byte_perm(now.km[g], 0, sel)), i1024, i64, v);
+          const int row = ta + 2 * h, ch = 4 * g + q4;
+          *reinterpret_cast<uint4 *>(K + (ch >> 3) * L::kAtom + row * 128 + (((ch & 7) ^ (row & 7)) << 4)) =
+              make_uint4(v[0], v[1], v[2], v[3]);
+        }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&k_full[st]);
+      if (!(ok = warp_wait(&v_empty[st], ph ^ 1, err))) break;
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          // dimensions 4 r .. of tokens 4 q4 + 2 h and the next, which are the halves of a pair
+          uint32_t v[4];
+          values(h ? now.v[g].y : now.v[g].x, pair(h ? now.vp[g].y : now.vp[g].x), pair(h ? now.vp[g].w : now.vp[g].z), i1024, i64, v);
+          const int ch = 4 * g + (r >> 1);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int row = 16 * part + 4 * q4 + 2 * h + u;
+            const uint32_t sel = u ? 0x7632 : 0x5410;
+            *reinterpret_cast<uint2 *>(V + (ch >> 3) * L::kAtom + row * 128 + (((ch & 7) ^ (row & 7)) << 4) + (r & 1) * 8) =
+                make_uint2(__byte_perm(v[0], v[1], sel), __byte_perm(v[2], v[3], sel));
+          }
+        }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&v_full[st]);
+    }
+  } else if (warp == kSoftmaxWarps + kCodeWarps) {
+    // S(t), where P(t - 2) was.  Descriptors share their high word; the low one is the address / 16 (and, MN-major,
+    // the distance of the 64-dimension parts).
+    const uint32_t s16 = smem_u32(sm) >> 4;
+    const uint64_t hi = umma_desc(sm) & 0xFFFFFFFF00000000ull;
+    const uint32_t id = f16_idesc<__half>(kKeys, false);
+    int t = 0, th[2] = {0, 0}, seen[2] = {0, 0};
+    while (ok && walk.next(b, s, w.bad)) {
+      const int nt = walk.tiles(), nh = walk.halves();
+      if (nt == 0) continue;
+      for (int h = 0; h < nh && ok; ++h) ok = warp_wait(&q_full[h], (uint32_t)seen[h]++ & 1, err);
+      for (int j = 0; j < nt && ok; ++j, ++t) {
+        const int st = t % ST;
+        if (!(ok = warp_wait(&k_full[st], (uint32_t)(t / ST) & 1, err))) break;
+        const uint32_t k = (s16 + (uint32_t)((L::kK + st * L::kBytes) >> 4)) | (1u << 16);
+        for (int h = 0; h < nh && ok; ++h) {
+          const int n = th[h]++, buf = 2 * h + (n & 1);
+          if (n >= 2 && !(ok = warp_wait(&pv_done[buf], (uint32_t)((n - 2) >> 1) & 1, err))) break;
+          tc_after();
+          const uint32_t q16 = (s16 + (uint32_t)((L::kQ + h * L::kQBytes) >> 4)) | (1u << 16);
+#pragma unroll
+          for (int u = 0; u < DP / 16; ++u) {
+            const uint32_t in = (uint32_t)((u & 3) * 2), qa = (u >> 2) * (L::kQAtom >> 4) + in, ka = (u >> 2) * (L::kAtom >> 4) + in;
+            umma_bf16_e(tmem + (uint32_t)(buf * kKeys), hi | (q16 + qa), hi | (k + ka), id, u ? 1u : 0u);
+          }
+          umma_commit_e(&s_full[buf]);
+        }
+        umma_commit_e(&k_empty[st]);
+      }
+    }
+    if (!ok) {
+      umma_commit_e(&done[0]);
+      mbar_drain(&done[0], 0);
+    }
+  } else {
+    // O += P(t) V
+    const uint32_t s16 = smem_u32(sm) >> 4;
+    const uint64_t hi = umma_desc(sm) & 0xFFFFFFFF00000000ull;
+    const uint32_t id = f16_idesc<__half>(L::kDims, true);
+    int t = 0, th[2] = {0, 0}, seen[2] = {0, 0};
+    while (ok && walk.next(b, s, w.bad)) {
+      const int nt = walk.tiles(), nh = walk.halves();
+      for (int j = 0; j < nt && ok; ++j, ++t) {
+        const int st = t % ST;
+        if (!(ok = warp_wait(&v_full[st], (uint32_t)(t / ST) & 1, err))) break;
+        const uint32_t v = (s16 + (uint32_t)((L::kV + st * L::kBytes) >> 4)) | ((uint32_t)(L::kAtom >> 4) << 16);
+        for (int h = 0; h < nh && ok; ++h) {
+          const int n = th[h]++, buf = 2 * h + (n & 1);
+          if (!(ok = warp_wait(&p_full[buf], (uint32_t)(n >> 1) & 1, err))) break;
+          // the last item's O has been read
+          if (j == 0 && seen[h]++ > 0 && !(ok = warp_wait(&o_free[h], (uint32_t)seen[h] & 1, err))) break;
+          tc_after();
+#pragma unroll
+          for (int u = 0; u < kKeys / 16; ++u)
+            umma_bf16_ts_e(tmem + (uint32_t)(L::kO + h * L::kDims), tmem + (uint32_t)(buf * kKeys + 8 * u), hi | (v + 128 * u), id,
+                           (j | u) ? 1u : 0u);
+          umma_commit_e(&pv_done[buf]);
+        }
+        umma_commit_e(&v_empty[st]);
+      }
+    }
+    if (!ok) {
+      umma_commit_e(&done[1]);
+      mbar_drain(&done[1], 0);
+    }
+  }
+  __syncwarp();
+  tc_before();
+  __syncthreads();
+  if (warp == kSoftmaxWarps + kCodeWarps) {
+    tc_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::kCols));
+  }
+}
+
+template <typename T, int NG>
+cudaError_t launch(const Kv4Shape &s, const Kv4Rows &b, const Kv4AttnCall &c, const Kv4Work &w, cudaStream_t st) {
+  auto *kernel = tile_kernel<T, NG>;
+  static thread_local int ready = -1;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && ready != dev) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<NG>::kSmem);
+    if (e == cudaSuccess) ready = dev;
+  }
+  if (e != cudaSuccess) return e;
+  kernel<<<w.sms, kThreads, Tile<NG>::kSmem, st>>>(c, s, b, w);
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t run(const Kv4Shape &s, const Kv4Rows &b, const Kv4AttnCall &c, const Kv4Work &w, cudaStream_t st) {
+  switch (s.ng) {
+    case 1: return launch<T, 1>(s, b, c, w, st);
+    case 2: return launch<T, 2>(s, b, c, w, st);
+    case 3: return launch<T, 3>(s, b, c, w, st);
+    default: return launch<T, 4>(s, b, c, w, st);
+  }
+}
+
+}  // namespace
+
+int64_t kv4_tile_floats(const Kv4Shape &s, int sms) { return (int64_t)sms * 2 * kRows * (s.ng * 32 + 2); }
+
+cudaError_t kv4_attn_tiles(const Kv4Shape &s, const Kv4Rows &b, const Kv4AttnCall &c, const Kv4Work &w, cudaStream_t st) {
+  return s.dtype == DT_F16 ? run<__half>(s, b, c, w, st) : run<__nv_bfloat16>(s, b, c, w, st);
+}
+
+}  // namespace ndl

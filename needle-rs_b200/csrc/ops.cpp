@@ -506,7 +506,7 @@ NeedleKv4Plan *needle_kv4_plan_create(size_t H, size_t KVH, size_t D, size_t pag
     if (!ok(cudaGetDevice(&plan->device)) ||
         !ok(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, plan->device)))
       return false;
-    const size_t cb = (256 + (size_t)kv4_attn_blocks(sms) * sizeof(int) + 255) / 256 * 256;
+    const size_t cb = (256 + (size_t)kv4_attn_counters(sms) * sizeof(int) + 255) / 256 * 256;
     if (!ok(cudaMalloc(&plan->buf, cb + (size_t)kv4_attn_floats(plan->s, sms) * sizeof(float)))) return false;
     plan->work.err = (int *)plan->buf;
     plan->work.bad = plan->work.err + 1;

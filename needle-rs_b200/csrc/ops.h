@@ -143,15 +143,19 @@ struct Kv4AttnCall {
 };
 struct Kv4Work {
   int *err = nullptr, *bad = nullptr;  // a wait that ran out; a request that does not fit
-  int *counters = nullptr;             // kv4_attn_blocks of them, zero between calls
+  int *counters = nullptr;             // kv4_attn_counters of them, zero between calls
   float *ws = nullptr;                 // kv4_attn_floats
   int sms = 0;
 };
-int64_t kv4_attn_blocks(int sms);
+int64_t kv4_attn_counters(int sms);
 int64_t kv4_attn_floats(const Kv4Shape &s, int sms);
 cudaError_t kv4_append(const Kv4Shape &s, const Kv4Rows &b, const Kv4Call &c, const Kv4Work &w, cudaStream_t st);
 cudaError_t kv4_read(const Kv4Shape &s, const Kv4Rows &b, const Kv4Call &c, const Kv4Work &w, cudaStream_t st);
 cudaError_t kv4_attn(const Kv4Shape &s, const Kv4Rows &b, const Kv4AttnCall &c, const Kv4Work &w, cudaStream_t st);
+// Of many rows: kv4_attn's other half.
+constexpr int kTileCounters = 8;  // of a block
+int64_t kv4_tile_floats(const Kv4Shape &s, int sms);
+cudaError_t kv4_attn_tiles(const Kv4Shape &s, const Kv4Rows &b, const Kv4AttnCall &c, const Kv4Work &w, cudaStream_t st);
 
 // ── verification of drafts ──
 struct VerifyShape {
