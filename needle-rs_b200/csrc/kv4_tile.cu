@@ -40,7 +40,9 @@ struct Tile {
   static constexpr int kAtoms = NG <= 2 ? 1 : 2;  // 64-dimension parts of a row (128 bytes each)
   static constexpr int kQAtom = kHalf * 128, kAtom = kKeys * 128, kQBytes = kAtoms * kQAtom, kBytes = kAtoms * kAtom;
   static constexpr int kStages = 3;  // of K, and of V
-  static constexpr int kQ = 0, kK = 2 * kQBytes, kV = kK + kStages * kBytes, kBar = kV + kStages * kBytes;
+  static constexpr int kAhead = 4;  // tiles of 16 tokens in 4 bits that each of the code warps holds
+  static constexpr int kQ = 0, kK = 2 * kQBytes, kV = kK + kStages * kBytes, kCodes = kV + kStages * kBytes;
+  static constexpr int kBar = kCodes + kCodeWarps * kAhead * tile_bytes(NG);
   static constexpr int kSmem = kBar + 512 + 1024;
   static constexpr int kDims = 64 * kAtoms;  // columns of O
   // TMEM columns: two S of each half (P over each), then O of each half
@@ -145,53 +147,12 @@ __device__ __forceinline__ void values(uint32_t w, __half2 s, __half2 m, uint32_
   }
 }
 
-// 16 tokens of 4 bits on their way, a lane's share.
-template <int NG>
-struct Codes {
-  uint2 k[NG], v[NG];
-  uint32_t ks[NG], km[NG];
-  uint4 vp[NG];
-  int left;  // tokens of the request among them
-
-  __device__ __forceinline__ void fetch(const uint8_t *tile, int lane) {
-    const int r = lane >> 2, q4 = lane & 3;
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      k[g] = *reinterpret_cast<const uint2 *>(tile + g * 256 + lane * 8);
-      v[g] = *reinterpret_cast<const uint2 *>(tile + v_codes(NG) + g * 256 + lane * 8);
-      ks[g] = *reinterpret_cast<const uint32_t *>(tile + k_params(NG) + (g * 8 + r) * 4);
-      km[g] = *reinterpret_cast<const uint32_t *>(tile + k_params(NG) + ((NG + g) * 8 + r) * 4);
-      vp[g] = *reinterpret_cast<const uint4 *>(tile + v_params(NG) + (g * 4 + q4) * 16);
-    }
-  }
-  __device__ __forceinline__ void clear() {
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      k[g] = v[g] = make_uint2(0, 0);
-      ks[g] = km[g] = 0;
-      vp[g] = make_uint4(0, 0, 0, 0);
-    }
-  }
-  // Behind the last token a page may hold anything.
-  __device__ __forceinline__ void cut(int q4) {
-    const int n = left - 4 * q4;
-    const uint32_t a = n >= 2 ? 0xffffffffu : n == 1 ? 0xffffu : 0u, b = n >= 4 ? 0xffffffffu : n == 3 ? 0xffffu : 0u;
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      vp[g].x &= a;
-      vp[g].z &= a;
-      vp[g].y &= b;
-      vp[g].w &= b;
-    }
-  }
-};
-
 template <typename T, int NG>
 __global__ void __launch_bounds__(kThreads, 1) tile_kernel(Kv4AttnCall c, Kv4Shape s, Kv4Rows b, Kv4Work w) {
   using L = Tile<NG>;
   constexpr int ST = L::kStages, DP = NG * 32;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t *sm = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t *sm = smem_raw + (-smem_u32(smem_raw) & 1023);  // an offset: accesses stay known to be shared memory
   uint64_t *k_full = (uint64_t *)(sm + L::kBar), *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST;
   uint64_t *q_full = v_empty + ST, *o_free = q_full + 2, *s_full = o_free + 2, *p_full = s_full + 4, *pv_done = p_full + 4,
            *done = pv_done + 4;  // [half]; [half][buffer]; done: of a warp's MMAs in flight, after a wait that ran out
@@ -402,47 +363,67 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(Kv4AttnCall c, Kv4Sha
         }
         if (__shfl_sync(0xffffffffu, last, 0)) {
           const int x0 = half * kHalf + quarter * 32, n = min(32, walk.rows - x0), d = lane * 4;
-          for (int k = 0; k < n; ++k) {
-            const int xr = x0 + k, rr = walk.r0 + xr, hr = walk.kvh * G + rr % G;
-            const int64_t tr = walk.q.row0 + rr / G;
-            auto part = [&](int z) { return slot_of<DP>(w, b0 + z, z == 0 ? 1 : 0); };
-            float M = -INFINITY, L = 0.0f;
-            for (int z = 0; z < parts; ++z) M = fmaxf(M, __ldcg(part(z) + kRows * DP + xr));
-            const float from = M == -INFINITY ? 0.0f : M;
-            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          auto part = [&](int z) { return slot_of<DP>(w, b0 + z, z == 0 ? 1 : 0); };
+          // a lane's row: its largest m, and its l
+          const int xl = min(x, walk.rows - 1);
+          float M = -INFINITY, sum = 0.0f;
 #pragma unroll 4
+          for (int z = 0; z < parts; ++z) M = fmaxf(M, __ldcg(part(z) + kRows * DP + xl));
+          const float from = M == -INFINITY ? 0.0f : M;
+#pragma unroll 4
+          for (int z = 0; z < parts; ++z)
+            sum += ex2(__ldcg(part(z) + kRows * DP + xl) - from) * __ldcg(part(z) + kRows * (DP + 1) + xl);
+          const float one = sum == 0.0f ? 0.0f : 1.0f / sum;
+          if (mine && c.lse) c.lse[token * s.H + h] = sum == 0.0f ? -INFINITY : fmaf(M, kLn2, logf(sum));
+          // sums: four dimensions a lane, eight rows side by side
+          for (int k0 = 0; k0 < n; k0 += 8) {
+            float4 v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             for (int z = 0; z < parts; ++z) {
-              const float g = ex2(__ldcg(part(z) + kRows * DP + xr) - from);
-              L += g * __ldcg(part(z) + kRows * (DP + 1) + xr);
-              if (d < D) {
-                const float4 y = __ldcg(reinterpret_cast<const float4 *>(part(z) + (int64_t)xr * DP + d));
-                v.x += g * y.x;
-                v.y += g * y.y;
-                v.z += g * y.z;
-                v.w += g * y.w;
+              const float g = ex2(__ldcg(part(z) + kRows * DP + xl) - from) * one;
+              float4 y[8];
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                y[k] = d < D && k0 + k < n ? __ldcg(reinterpret_cast<const float4 *>(part(z) + (int64_t)(x0 + k0 + k) * DP + d))
+                                           : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                const float f = __shfl_sync(0xffffffffu, g, k0 + k);
+                v[k].x += f * y[k].x;
+                v[k].y += f * y[k].y;
+                v[k].z += f * y[k].z;
+                v[k].w += f * y[k].w;
               }
             }
-            const float one = L == 0.0f ? 0.0f : 1.0f / L;
-            if (d < D)
-              *reinterpret_cast<uint2 *>((T *)c.out + tr * c.o_row + (int64_t)hr * c.o_head + d) =
-                  make_uint2(pack2<T>(v.x * one, v.y * one), pack2<T>(v.z * one, v.w * one));
-            if (lane == 0 && c.lse) c.lse[tr * s.H + hr] = L == 0.0f ? -INFINITY : fmaf(M, kLn2, logf(L));
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const int rr = walk.r0 + x0 + k0 + k;
+              if (d < D && k0 + k < n)
+                *reinterpret_cast<uint2 *>((T *)c.out + (walk.q.row0 + rr / G) * c.o_row + (int64_t)(walk.kvh * G + rr % G) * c.o_head + d) =
+                    make_uint2(pack2<T>(v[k].x, v[k].y), pack2<T>(v[k].z, v[k].w));
+            }
           }
         }
         __syncwarp();
       }
     }
   } else if (warp < kSoftmaxWarps + kCodeWarps) {
-    // 4 bits to f16: a warp for each 16 tokens of a tile, one tile ahead in registers
+    // 4 bits to f16: a warp for each 16 tokens of a tile, through a ring of its own (with the next tile alone on its
+    // way, in registers, 64 keys took 3990 clocks instead of KKKK)
     const int part = warp - kSoftmaxWarps, r = lane >> 2, q4 = lane & 3;
     const int ta = 16 * part + 4 * (r >> 1) + (r & 1);  // the token of K's row r; that of r + 8 is 2 on
+    constexpr int TB = tile_bytes(NG), AHEAD = L::kAhead;
+    uint8_t *ring = sm + L::kCodes + part * AHEAD * TB;
+    const uint32_t ring32 = smem_u32(ring);
     uint32_t i1024, i64;  // in registers: an AND and an OR with it are one instruction
     asm volatile("mov.b32 %0, 0x64006400;" : "=r"(i1024));
     asm volatile("mov.b32 %0, 0x54005400;" : "=r"(i64));
-    Codes<NG> now, ahead;
-    int j = 0, nt = 0;
+    int j = 0, nt = 0, next_left = 0, left[AHEAD];
+    uint32_t next_place = kNoPlace;
     bool more = true;
-    auto fetch = [&]() {  // the next tile's codes; false behind the last
+    // the place of the next tile (its table entry is on its way a turn before it is needed); false behind the last
+    auto locate = [&] {
       while (more && j >= nt) {
         more = walk.next(b, s, w.bad);
         nt = more ? walk.tiles() : 0;
@@ -450,28 +431,69 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(Kv4AttnCall c, Kv4Sha
       }
       if (!more) return false;
       const int at = (walk.u0 + j++) * kKeys + 16 * part;
-      ahead.left = walk.q.len - at;
-      const uint8_t *tile = ahead.left > 0 ? tile_at((uint8_t *)c.pages, b, s, walk.seq, at / kTokens, walk.kvh, w.bad) : nullptr;
-      if (tile) ahead.fetch(tile, lane);
-      else ahead.clear();
+      next_left = walk.q.len - at;
+      next_place = next_left > 0 ? place_of(b, s, walk.seq, at / kTokens, walk.kvh, w.bad) : kNoPlace;
       return true;
     };
-    bool have = fetch();
-    for (int t = 0; have; ++t) {
-      now = ahead;
-      have = fetch();
+    bool found = locate();
+    auto fetch = [&](int slot) {  // the copy of that tile (zeros where there is none), and the place of the next
+      if (found) {
+        const bool take = next_place != kNoPlace;
+        const uint8_t *src = c.pages + (take ? (int64_t)next_place * 128 : 0) + lane * 16;
+#pragma unroll
+        for (int i = 0; i < (TB + 511) / 512; ++i)
+          if (i * 512 + lane * 16 < TB) cp16(ring32 + slot * TB + i * 512 + lane * 16, src + i * 512, take);
+        found = locate();
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    int tiles = 0;  // requested
+#pragma unroll
+    for (int k = 0; k < AHEAD - 1; ++k) {
+      left[k] = next_left;
+      if (found) ++tiles;
+      fetch(k);
+    }
+    int slot = 0;
+    for (int t = 0; t < tiles; ++t) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 2) : "memory");
+      __syncwarp();  // every lane's copies of this slot, and the reads of the slot refilled next
+      const int now_left = left[0];
+#pragma unroll
+      for (int k = 0; k < AHEAD - 2; ++k) left[k] = left[k + 1];
+      left[AHEAD - 2] = next_left;
+      if (found) ++tiles;
+      fetch(slot == 0 ? AHEAD - 1 : slot - 1);
+      uint8_t *codes = ring + slot * TB;
+      if (++slot == AHEAD) slot = 0;
+      if (now_left < kTokens) {  // behind the last token the page may hold anything
+        for (int u = lane; u < 32 * NG; u += 32)
+          if (((u >> 3) & 3) * 4 + (u & 3) >= now_left) *reinterpret_cast<uint16_t *>(codes + v_params(NG) + u * 2) = 0;
+        __syncwarp();
+      }
       const int st = t % ST;
       const uint32_t ph = (uint32_t)(t / ST) & 1;
-      if (now.left < kTokens) now.cut(q4);
       if (!(ok = warp_wait(&k_empty[st], ph ^ 1, err))) break;
       uint8_t *K = sm + L::kK + st * L::kBytes, *V = sm + L::kV + st * L::kBytes;
+      // all loads before the stores, which could be of the same bytes for all that the compiler knows
+      uint2 kc[NG], vc[NG];
+      uint32_t ks[NG], km[NG];
+      uint4 vp[NG];
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        kc[g] = *reinterpret_cast<const uint2 *>(codes + g * 256 + lane * 8);
+        ks[g] = *reinterpret_cast<const uint32_t *>(codes + k_params(NG) + (g * 8 + r) * 4);
+        km[g] = *reinterpret_cast<const uint32_t *>(codes + k_params(NG) + ((NG + g) * 8 + r) * 4);
+        vc[g] = *reinterpret_cast<const uint2 *>(codes + v_codes(NG) + g * 256 + lane * 8);
+        vp[g] = *reinterpret_cast<const uint4 *>(codes + v_params(NG) + (g * 4 + q4) * 16);
+      }
 #pragma unroll
       for (int g = 0; g < NG; ++g)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint32_t sel = h ? 0x3232 : 0x1010;
           uint32_t v[4];
-          values(h ? now.k[g].y : now.k[g].x, pair(__byte_perm(now.ks[g], 0, sel)), pair(__byte_perm(now.km[g], 0, sel)), i1024, i64, v);
+          values(h ? kc[g].y : kc[g].x, pair(__byte_perm(ks[g], 0, sel)), pair(__byte_perm(km[g], 0, sel)), i1024, i64, v);
           const int row = ta + 2 * h, ch = 4 * g + q4;
           *reinterpret_cast<uint4 *>(K + (ch >> 3) * L::kAtom + row * 128 + (((ch & 7) ^ (row & 7)) << 4)) =
               make_uint4(v[0], v[1], v[2], v[3]);
@@ -486,7 +508,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(Kv4AttnCall c, Kv4Sha
         for (int h = 0; h < 2; ++h) {
           // dimensions 4 r .. of tokens 4 q4 + 2 h and the next, which are the halves of a pair
           uint32_t v[4];
-          values(h ? now.v[g].y : now.v[g].x, pair(h ? now.vp[g].y : now.vp[g].x), pair(h ? now.vp[g].w : now.vp[g].z), i1024, i64, v);
+          values(h ? vc[g].y : vc[g].x, pair(h ? vp[g].y : vp[g].x), pair(h ? vp[g].w : vp[g].z), i1024, i64, v);
           const int ch = 4 * g + (r >> 1);
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
@@ -500,6 +522,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(Kv4AttnCall c, Kv4Sha
       __syncwarp();
       if (lane == 0) mbar_arrive(&v_full[st]);
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
   } else if (warp == kSoftmaxWarps + kCodeWarps) {
     // S(t), where P(t - 2) was.  Descriptors share their high word; the low one is the address / 16 (and, MN-major,
     // the distance of the 64-dimension parts).
