@@ -70,23 +70,29 @@ __host__ __device__ __forceinline__ Seq sequence(const Kv4Rows &b, const Kv4Shap
   return ok ? Seq{a, e - a, len} : Seq{0, 0, 0};
 }
 
-// Where tile `t` (of 16 tokens) of request i's cache for a KV head begins, in
-// units of 128 bytes; kNoPlace (flag set) where the table names a page that is
-// not there.
+// Which page holds tile `t` (of 16 tokens) of request i's cache, as its table says, and the tile's number in it.  A load: what is
+// done with it can wait a while.
+struct Page {
+  int page, in;
+};
+__host__ __device__ __forceinline__ Page page_of(const Kv4Rows &b, const Kv4Shape &s, int i, int t) {
+  const int per = s.page_tokens / kTokens, n = (int)(((uint64_t)(uint32_t)t * s.per_inverse) >> 38);  // t / per
+  return Page{b.table[(int64_t)i * b.width + n], t - n * per};
+}
+// Where that tile begins for a KV head, in units of 128 bytes; kNoPlace (flag set) where there is no such page.
 constexpr uint32_t kNoPlace = 0xffffffffu;
-__host__ __device__ __forceinline__ uint32_t place_of(const Kv4Rows &b, const Kv4Shape &s, int i, int t, int kvh, int *bad) {
-  const int per = s.page_tokens / kTokens, in = t % per;
-  const int page = b.table[(int64_t)i * b.width + t / per];
-  if (page < 0 || page >= s.n_pages) {
+__host__ __device__ __forceinline__ uint32_t place_of(const Kv4Shape &s, const Page &p, int kvh, int *bad) {
+  if (p.page < 0 || p.page >= s.n_pages) {
     *bad = 1;
     return kNoPlace;
   }
-  return (uint32_t)(((int64_t)page * s.page_bytes + ((int64_t)kvh * per + in) * tile_bytes(s.ng)) >> 7);
+  const int per = s.page_tokens / kTokens;
+  return (uint32_t)(((int64_t)p.page * s.page_bytes + ((int64_t)kvh * per + p.in) * tile_bytes(s.ng)) >> 7);
 }
 // The same as an address, or NULL.
 __host__ __device__ __forceinline__ uint8_t *tile_at(uint8_t *pages, const Kv4Rows &b, const Kv4Shape &s, int i, int t, int kvh,
                                                      int *bad) {
-  const uint32_t p = place_of(b, s, i, t, kvh, bad);
+  const uint32_t p = place_of(s, page_of(b, s, i, t), kvh, bad);
   return p == kNoPlace ? nullptr : pages + (int64_t)p * 128;
 }
 

@@ -139,15 +139,22 @@ __global__ void __launch_bounds__(kThreads, few_blocks(NB))
     }
 
     // places of 32 of the warp's tiles (a lane each: two for each turn) and of the next 32
-    auto places = [&](int n) {
+    auto tile_of = [&](int n) {  // a lane's tile, or one behind the last
       const int t = t0 + 2 * (warp + (n + (lane >> 1)) * kWarps) + (lane & 1);
-      return n + (lane >> 1) < mine && t < t1 ? place_of(b, s, seq, t, kvh, w.bad) : kNoPlace;
+      return n + (lane >> 1) < mine ? t : t1;
     };
-    uint32_t window = places(0), ahead = places(16);
+    auto pages = [&](int n) {
+      const int t = tile_of(n);
+      return t < t1 ? page_of(b, s, seq, t) : Page{0, 0};
+    };
+    auto places = [&](int n, const Page &p) { return tile_of(n) < t1 ? place_of(s, p, kvh, w.bad) : kNoPlace; };
+    const Page now = pages(0);
+    Page ahead = pages(16);  // looked at when its turn comes
+    uint32_t window = places(0, now);
     auto issue = [&](int n, int stage) {  // tiles that are not there become zeros
       if ((n & 15) == 0 && n > 0) {
-        window = ahead;
-        ahead = places(n + 16);
+        window = places(n, ahead);
+        ahead = pages(n + 16);
       }
       const uint32_t p0 = __shfl_sync(0xffffffffu, window, (n & 15) * 2), p1 = __shfl_sync(0xffffffffu, window, (n & 15) * 2 + 1);
       const bool h0 = p0 != kNoPlace, h1 = p1 != kNoPlace;

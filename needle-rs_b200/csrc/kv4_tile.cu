@@ -419,10 +419,10 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(Kv4AttnCall c, Kv4Sha
     uint32_t i1024, i64;  // in registers: an AND and an OR with it are one instruction
     asm volatile("mov.b32 %0, 0x64006400;" : "=r"(i1024));
     asm volatile("mov.b32 %0, 0x54005400;" : "=r"(i64));
-    int j = 0, nt = 0, next_left = 0, left[AHEAD];
-    uint32_t next_place = kNoPlace;
+    int j = 0, nt = 0, next_left = 0, next_kvh = 0, left[AHEAD];
+    Page next_page{0, 0};
     bool more = true;
-    // the place of the next tile (its table entry is on its way a turn before it is needed); false behind the last
+    // the page of the next tile (its table entry is on its way a turn before it is looked at); false behind the last
     auto locate = [&] {
       while (more && j >= nt) {
         more = walk.next(b, s, w.bad);
@@ -432,14 +432,16 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(Kv4AttnCall c, Kv4Sha
       if (!more) return false;
       const int at = (walk.u0 + j++) * kKeys + 16 * part;
       next_left = walk.q.len - at;
-      next_place = next_left > 0 ? place_of(b, s, walk.seq, at / kTokens, walk.kvh, w.bad) : kNoPlace;
+      next_kvh = walk.kvh;
+      if (next_left > 0) next_page = page_of(b, s, walk.seq, at / kTokens);
       return true;
     };
     bool found = locate();
     auto fetch = [&](int slot) {  // the copy of that tile (zeros where there is none), and the place of the next
       if (found) {
-        const bool take = next_place != kNoPlace;
-        const uint8_t *src = c.pages + (take ? (int64_t)next_place * 128 : 0) + lane * 16;
+        const uint32_t place = next_left > 0 ? place_of(s, next_page, next_kvh, w.bad) : kNoPlace;
+        const bool take = place != kNoPlace;
+        const uint8_t *src = c.pages + (take ? (int64_t)place * 128 : 0) + lane * 16;
 #pragma unroll
         for (int i = 0; i < (TB + 511) / 512; ++i)
           if (i * 512 + lane * 16 < TB) cp16(ring32 + slot * TB + i * 512 + lane * 16, src + i * 512, take);

@@ -499,7 +499,7 @@ NeedleKv4Plan *needle_kv4_plan_create(size_t H, size_t KVH, size_t D, size_t pag
       return fail("4-bit cache: an array of pages must stay below 512 GiB");
     plan = new NeedleKv4Plan();
     plan->s = Kv4Shape{(int)H, (int)KVH, (int)D, (int)((D + 31) / 32), (int)page_tokens, dtype, (int64_t)n_pages,
-                       (int64_t)needle_kv4_page_bytes(KVH, D, page_tokens)};
+                       (int64_t)needle_kv4_page_bytes(KVH, D, page_tokens), kv4_inverse((int)page_tokens)};
     plan->max_seqs = max_seqs;
     plan->max_rows = max_rows;
     int sms = 0;

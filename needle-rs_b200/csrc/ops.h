@@ -116,7 +116,9 @@ cudaError_t cross_attn(const XAttnWork &w, const XAttnCall &c, int *err, cudaStr
 struct Kv4Shape {
   int H, KVH, D, ng, page_tokens, dtype;
   int64_t n_pages, page_bytes;
+  uint64_t per_inverse;  // of the tiles of a page: t / per = (t * per_inverse) >> 38 for t below 2^26
 };
+inline uint64_t kv4_inverse(int page_tokens) { return (((uint64_t)1 << 38) + page_tokens / 16 - 1) / (page_tokens / 16); }
 // The requests of a call (device arrays).  Kernels check every number in
 // them; what does not fit sets the plan's `bad` flag and is left out.
 struct Kv4Rows {

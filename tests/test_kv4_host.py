@@ -91,8 +91,18 @@ int main() {
     for (int b : owner) CHECK(b >= 0);
   }
 
+  // the division of a tile's number by a page's tiles
+  for (int per = 1; per <= 4096; per += per < 70 ? 1 : 61) {
+    Kv4Shape d{1, 1, 32, 1, per * 16, 1, 1, 640 * per, kv4_inverse(per * 16)};
+    std::vector<int32_t> one(1 << 20);
+    Kv4Rows e{nullptr, nullptr, one.data(), 1, 1 << 20, 1, 1};
+    for (int64_t t : {0ll, 1ll, per - 1ll, (long long)per, per + 1ll, 1000ll * per - 1, 1000ll * per, (1ll << 26) / per * per - 1, (1ll << 26) - 1})
+      if (t >= 0 && t / per < (1 << 20) && t < 1 << 26) CHECK(page_of(e, d, 0, (int)t).in == t % per);
+    for (uint64_t t : {(1ull << 26) - 1, (1ull << 26) / per * per - 1, (1ull << 25) + 7}) CHECK((t * d.per_inverse) >> 38 == t / per);
+  }
+
   // numbers that do not fit give a request without rows and tokens
-  Kv4Shape s{8, 4, 64, 2, 32, 1, 10, 4 * 2 * 1280};
+  Kv4Shape s{8, 4, 64, 2, 32, 1, 10, 4 * 2 * 1280, kv4_inverse(32)};
   const int32_t start[] = {0, 3, 3, 2, 9, 12, -1, 5, 2147483647}, len[] = {64, 10, 10, 10, 97, -1, 10, 10};
   std::vector<int32_t> table(8 * 3, 0);
   Kv4Rows b{start, len, table.data(), 8, 3, 11, 7};
