@@ -35,6 +35,32 @@ using namespace tc;
 constexpr int kRows = 256, kHalf = 128, kKeys = kUnit, kWarps = 14, kThreads = kWarps * 32;
 constexpr int kSoftmaxWarps = 8, kCodeWarps = 4;  // then the issuers of S and of O
 
+// The bounded wait of a whole warp, suspended in hardware for up to 2 us a try: polling every 80 clocks or so, as the
+// default does, waiting warps took half of the issue slots.
+__device__ __forceinline__ bool long_wait(uint64_t *bar, uint32_t parity, int *err) {
+  bool ok = true;
+  uint64_t t0 = 0;
+  for (uint32_t i = 0;; ++i) {
+    uint32_t there;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 2000;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(there)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    if (there) break;
+    if (i == 0) t0 = globaltimer_ns();
+    if (*(volatile int *)err) ok = false;
+    if (ok && globaltimer_ns() - t0 > kWaitNs) {
+      atomicExch(err, 1);
+      ok = false;
+    }
+    if (!ok) break;
+  }
+  return __all_sync(0xffffffffu, ok);
+}
+
 template <int NG>
 struct Tile {
   static constexpr int kAtoms = NG <= 2 ? 1 : 2;  // 64-dimension parts of a row (128 bytes each)
@@ -240,7 +266,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(Kv4AttnCall c, Kv4Sha
       float m = -INFINITY, l = 0.0f;
       for (int j = 0; j < nt; ++j, ++t) {
         const int buf = 2 * half + (t & 1), j0 = (walk.u0 + j) * kKeys;
-        if (!(ok = warp_wait(&s_full[buf], (uint32_t)(t >> 1) & 1, err))) break;
+        if (!(ok = long_wait(&s_full[buf], (uint32_t)(t >> 1) & 1, err))) break;
         tc_after();
         if (any) {
           const uint32_t tS = tmem + lanes + (uint32_t)(buf * kKeys);
@@ -266,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(Kv4AttnCall c, Kv4Sha
             l *= f;
           }
           if (j > 0 && __any_sync(0xffffffffu, move)) {
-            if (!(ok = warp_wait(&pv_done[2 * half + ((t - 1) & 1)], (uint32_t)((t - 1) >> 1) & 1, err))) break;
+            if (!(ok = long_wait(&pv_done[2 * half + ((t - 1) & 1)], (uint32_t)((t - 1) >> 1) & 1, err))) break;
             tc_after();
 #pragma unroll 1
             for (int q = 0; q < DP / 16; ++q) {
@@ -303,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(Kv4AttnCall c, Kv4Sha
         if (lane == 0) mbar_arrive(&p_full[buf]);
       }
       if (!ok) break;
-      if (nt > 0 && !(ok = warp_wait(&pv_done[2 * half + ((t - 1) & 1)], (uint32_t)((t - 1) >> 1) & 1, err))) break;
+      if (nt > 0 && !(ok = long_wait(&pv_done[2 * half + ((t - 1) & 1)], (uint32_t)((t - 1) >> 1) & 1, err))) break;
       tc_after();
       const bool whole = walk.u0 == 0 && walk.u1 == (int)walk.units;
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
@@ -419,32 +445,38 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(Kv4AttnCall c, Kv4Sha
     uint32_t i1024, i64;  // in registers: an AND and an OR with it are one instruction
     asm volatile("mov.b32 %0, 0x64006400;" : "=r"(i1024));
     asm volatile("mov.b32 %0, 0x54005400;" : "=r"(i64));
-    int j = 0, nt = 0, next_left = 0, next_kvh = 0, left[AHEAD];
-    Page next_page{0, 0};
+    // An item's tiles by 32 (a lane each): their pages come together, those of the next 32 are on their way meanwhile.
+    int j = 0, nt = 0, next_left = 0, left[AHEAD];
+    uint32_t window = kNoPlace;
+    Page ahead{0, 0};
     bool more = true;
-    // the page of the next tile (its table entry is on its way a turn before it is looked at); false behind the last
-    auto locate = [&] {
+    auto at = [&](int n) { return (walk.u0 + n) * kKeys + 16 * part; };  // the first of the 16 tokens
+    auto pages = [&](int n) { return n < nt && at(n) < walk.q.len ? page_of(b, s, walk.seq, at(n) / kTokens) : Page{0, 0}; };
+    auto places = [&](int n, const Page &p) { return n < nt && at(n) < walk.q.len ? place_of(s, p, walk.kvh, w.bad) : kNoPlace; };
+    auto locate = [&] {  // whether there is a next tile
       while (more && j >= nt) {
         more = walk.next(b, s, w.bad);
         nt = more ? walk.tiles() : 0;
         j = 0;
+        ahead = pages(lane);
       }
-      if (!more) return false;
-      const int at = (walk.u0 + j++) * kKeys + 16 * part;
-      next_left = walk.q.len - at;
-      next_kvh = walk.kvh;
-      if (next_left > 0) next_page = page_of(b, s, walk.seq, at / kTokens);
-      return true;
+      return more;
     };
     bool found = locate();
-    auto fetch = [&](int slot) {  // the copy of that tile (zeros where there is none), and the place of the next
+    auto fetch = [&](int slot) {  // its copy (zeros where there is no page)
       if (found) {
-        const uint32_t place = next_left > 0 ? place_of(s, next_page, next_kvh, w.bad) : kNoPlace;
+        if ((j & 31) == 0) {
+          window = places(j + lane, ahead);
+          ahead = pages(j + 32 + lane);
+        }
+        next_left = walk.q.len - at(j);
+        const uint32_t place = __shfl_sync(0xffffffffu, window, j & 31);
         const bool take = place != kNoPlace;
         const uint8_t *src = c.pages + (take ? (int64_t)place * 128 : 0) + lane * 16;
 #pragma unroll
         for (int i = 0; i < (TB + 511) / 512; ++i)
           if (i * 512 + lane * 16 < TB) cp16(ring32 + slot * TB + i * 512 + lane * 16, src + i * 512, take);
+        ++j;
         found = locate();
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
@@ -452,9 +484,9 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(Kv4AttnCall c, Kv4Sha
     int tiles = 0;  // requested
 #pragma unroll
     for (int k = 0; k < AHEAD - 1; ++k) {
-      left[k] = next_left;
       if (found) ++tiles;
       fetch(k);
+      left[k] = next_left;
     }
     int slot = 0;
     for (int t = 0; t < tiles; ++t) {
@@ -463,9 +495,9 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(Kv4AttnCall c, Kv4Sha
       const int now_left = left[0];
 #pragma unroll
       for (int k = 0; k < AHEAD - 2; ++k) left[k] = left[k + 1];
-      left[AHEAD - 2] = next_left;
       if (found) ++tiles;
       fetch(slot == 0 ? AHEAD - 1 : slot - 1);
+      left[AHEAD - 2] = next_left;
       uint8_t *codes = ring + slot * TB;
       if (++slot == AHEAD) slot = 0;
       if (now_left < kTokens) {  // behind the last token the page may hold anything
@@ -475,7 +507,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(Kv4AttnCall c, Kv4Sha
       }
       const int st = t % ST;
       const uint32_t ph = (uint32_t)(t / ST) & 1;
-      if (!(ok = warp_wait(&k_empty[st], ph ^ 1, err))) break;
+      if (!(ok = long_wait(&k_empty[st], ph ^ 1, err))) break;
       uint8_t *K = sm + L::kK + st * L::kBytes, *V = sm + L::kV + st * L::kBytes;
       // all loads before the stores, which could be of the same bytes for all that the compiler knows
       uint2 kc[NG], vc[NG];
@@ -503,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(Kv4AttnCall c, Kv4Sha
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&k_full[st]);
-      if (!(ok = warp_wait(&v_empty[st], ph ^ 1, err))) break;
+      if (!(ok = long_wait(&v_empty[st], ph ^ 1, err))) break;
 #pragma unroll
       for (int g = 0; g < NG; ++g)
 #pragma unroll
@@ -535,14 +567,14 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(Kv4AttnCall c, Kv4Sha
     while (ok && walk.next(b, s, w.bad)) {
       const int nt = walk.tiles(), nh = walk.halves();
       if (nt == 0) continue;
-      for (int h = 0; h < nh && ok; ++h) ok = warp_wait(&q_full[h], (uint32_t)seen[h]++ & 1, err);
+      for (int h = 0; h < nh && ok; ++h) ok = long_wait(&q_full[h], (uint32_t)seen[h]++ & 1, err);
       for (int j = 0; j < nt && ok; ++j, ++t) {
         const int st = t % ST;
-        if (!(ok = warp_wait(&k_full[st], (uint32_t)(t / ST) & 1, err))) break;
+        if (!(ok = long_wait(&k_full[st], (uint32_t)(t / ST) & 1, err))) break;
         const uint32_t k = (s16 + (uint32_t)((L::kK + st * L::kBytes) >> 4)) | (1u << 16);
         for (int h = 0; h < nh && ok; ++h) {
           const int n = th[h]++, buf = 2 * h + (n & 1);
-          if (n >= 2 && !(ok = warp_wait(&pv_done[buf], (uint32_t)((n - 2) >> 1) & 1, err))) break;
+          if (n >= 2 && !(ok = long_wait(&pv_done[buf], (uint32_t)((n - 2) >> 1) & 1, err))) break;
           tc_after();
           const uint32_t q16 = (s16 + (uint32_t)((L::kQ + h * L::kQBytes) >> 4)) | (1u << 16);
 #pragma unroll
@@ -569,13 +601,13 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(Kv4AttnCall c, Kv4Sha
       const int nt = walk.tiles(), nh = walk.halves();
       for (int j = 0; j < nt && ok; ++j, ++t) {
         const int st = t % ST;
-        if (!(ok = warp_wait(&v_full[st], (uint32_t)(t / ST) & 1, err))) break;
+        if (!(ok = long_wait(&v_full[st], (uint32_t)(t / ST) & 1, err))) break;
         const uint32_t v = (s16 + (uint32_t)((L::kV + st * L::kBytes) >> 4)) | ((uint32_t)(L::kAtom >> 4) << 16);
         for (int h = 0; h < nh && ok; ++h) {
           const int n = th[h]++, buf = 2 * h + (n & 1);
-          if (!(ok = warp_wait(&p_full[buf], (uint32_t)(n >> 1) & 1, err))) break;
+          if (!(ok = long_wait(&p_full[buf], (uint32_t)(n >> 1) & 1, err))) break;
           // the last item's O has been read
-          if (j == 0 && seen[h]++ > 0 && !(ok = warp_wait(&o_free[h], (uint32_t)seen[h] & 1, err))) break;
+          if (j == 0 && seen[h]++ > 0 && !(ok = long_wait(&o_free[h], (uint32_t)seen[h] & 1, err))) break;
           tc_after();
 #pragma unroll
           for (int u = 0; u < kKeys / 16; ++u)
