@@ -1,4 +1,4 @@
-// kv4_attn.cu — attention of a few query rows to a cache of keys and values in
+// kv4_attn.cu — attention of few query rows to a cache of keys and values in
 // 4 bits (many rows: kv4_tile.cu):
 //   s_j = scale * q . k_j     out = sum_j e^(s_j) v_j / sum_j e^(s_j)
 // with k = m + s c and v = m + s c of each group of 32 dimensions.
@@ -58,12 +58,14 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   return y;
 }
 
-// A request's items: its rows with each KV head.
+// A request's items: blocks of its rows with each KV head.
 struct FewItems {
-  int KVH;
+  int KVH, G, rows;  // of a block
 
-  __device__ uint32_t units(const Seq &q) const { return max(1, (q.len + kUnit - 1) / kUnit); }
-  __device__ uint64_t all(const Seq &q) const { return q.n ? (uint64_t)units(q) * KVH : 0; }
+  static constexpr int kStart = 5;  // an item's start and end cost about as much as 64 keys five times
+  static constexpr int kLeast = 2;
+  __device__ uint32_t units(const Seq &q) const { return kStart + (q.len + kUnit - 1) / kUnit; }
+  __device__ uint64_t all(const Seq &q) const { return (uint64_t)((q.n * G + rows - 1) / rows) * units(q) * KVH; }
   __device__ void item(const Seq &q, uint32_t at, uint32_t *first, uint32_t *n) const {
     *n = units(q);
     *first = at - at % *n;
@@ -96,7 +98,7 @@ __global__ void __launch_bounds__(kThreads, few_blocks(NB))
   extern __shared__ __align__(128) uint8_t sm[];
   __shared__ int last_one;
   __shared__ Share share;
-  const FewItems few{s.KVH};
+  const FewItems few{s.KVH, s.H / s.KVH, ROWS};
   share_of<FewItems, kWarps>(few, b, s, c.causal, w.bad, &share);
   if (blockIdx.x >= share.blocks) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, q4 = lane & 3;
@@ -116,12 +118,13 @@ __global__ void __launch_bounds__(kThreads, few_blocks(NB))
     const uint32_t units = few.units(rq), item = (at - base) / units, first = base + item * units;
     const int u0 = (int)(at - first), u1 = (int)min(units, share.end - first);
     at = first + u1;
-    const int kvh = (int)item, rows = rq.n * G, len = rq.len;
+    const int rb = (int)item / s.KVH, kvh = (int)item - rb * s.KVH, r0 = rb * ROWS;
+    const int rows = min(ROWS, rq.n * G - r0), len = rq.len;
     // keys that row x of the block sees
-    auto limit = [&](int x) { return c.causal ? len - rq.n + min(x, rows - 1) / G + 1 : len; };
+    auto limit = [&](int x) { return c.causal ? len - rq.n + (r0 + min(x, rows - 1)) / G + 1 : len; };
     const int k_all = limit(0);  // every row sees these
-    const int t0 = u0 * (kUnit / kTokens);
-    const int t1 = min(u1 * (kUnit / kTokens), (limit(rows - 1) + kTokens - 1) / kTokens);
+    const int t0 = max(u0 - FewItems::kStart, 0) * (kUnit / kTokens);
+    const int t1 = min(max(u1 - FewItems::kStart, 0) * (kUnit / kTokens), (limit(rows - 1) + kTokens - 1) / kTokens);
     // turns of this warp: it takes every fourth pair of tiles
     const int pairs = max(0, (t1 - t0 + 1) >> 1), mine = max(0, (pairs - warp + kWarps - 1) / kWarps);
 
@@ -129,8 +132,8 @@ __global__ void __launch_bounds__(kThreads, few_blocks(NB))
     uint4 raw[NB][NG];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const int x = nb * 8 + r;
-      const T *q = (const T *)c.q + (rq.row0 + x / G) * c.q_row + (int64_t)(kvh * G + x % G) * c.q_head;
+      const int x = nb * 8 + r, row = r0 + x;
+      const T *q = (const T *)c.q + (rq.row0 + row / G) * c.q_row + (int64_t)(kvh * G + row % G) * c.q_head;
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         const int d = g * 32 + q4 * 8;
@@ -425,8 +428,8 @@ __global__ void __launch_bounds__(kThreads, few_blocks(NB))
     const bool whole = u0 == 0 && u1 == (int)units;
     const int quads = D / 4;
     auto finish = [&](int x, int d, float4 v, float M, float L) {
-      const int h = kvh * G + x % G;
-      const int64_t at_row = rq.row0 + x / G;
+      const int row = r0 + x, h = kvh * G + row % G;
+      const int64_t at_row = rq.row0 + row / G;
       const float inv = L == 0.0f ? 0.0f : 1.0f / L;  // no key: zeros
       alignas(8) T out[4] = {from_f32<T>(v.x * inv), from_f32<T>(v.y * inv), from_f32<T>(v.z * inv), from_f32<T>(v.w * inv)};
       *reinterpret_cast<uint2 *>((T *)c.out + at_row * c.o_row + (int64_t)h * c.o_head + d) = *reinterpret_cast<uint2 *>(out);
@@ -571,10 +574,12 @@ int64_t kv4_attn_floats(const Kv4Shape &s, int sms) {
   return most;
 }
 
-// Up to 16 rows of a KV head read the cache faster than tiles would; 17 are a tile.
+// Blocks of 16 rows read the cache again for each, tiles of 256 start slowly.  Blocks against tiles, us: 24 requests of 27
+// rows x 4 heads of 80 over up to 2000 keys 21 and 40, of 60 rows 31 and 52; 8 of 64 rows x 8 heads of 128 over 8000 keys 94 and
+// 94, of 128 rows 214 and 100; one of 256 rows x 8 heads over 2000 keys 28 and 46, of 512 rows 39 and 55.
 cudaError_t kv4_attn(const Kv4Shape &s, const Kv4Rows &b, const Kv4AttnCall &c, const Kv4Work &w, cudaStream_t st) {
   if (b.rows == 0) return cudaSuccess;
-  if ((int64_t)b.max_new * (s.H / s.KVH) > 16) return kv4_attn_tiles(s, b, c, w, st);
+  if ((int64_t)b.max_new * (s.H / s.KVH) > 64 && b.rows * s.H > 4096) return kv4_attn_tiles(s, b, c, w, st);
   return s.dtype == DT_F16 ? run<__half>(s, b, c, w, st) : run<__nv_bfloat16>(s, b, c, w, st);
 }
 

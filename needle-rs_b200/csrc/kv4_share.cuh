@@ -6,6 +6,7 @@
 // units of 64 keys; block b of n takes units [total * b / n, total * (b + 1) / n) of all
 // requests' in order.  A border inside a short item moves to that item's nearer end:
 // such items stay whole; longer ones are cut, and their parts joined by the last block to arrive.
+// An item's first units stand for its start and end and hold no keys.
 #pragma once
 #include "kv4.cuh"
 
@@ -21,7 +22,7 @@ struct Share {
 };
 
 // P: all(q): a request's units; item(q, at, &first, &units): the item of unit `at` of a request; snap(share): units of the
-// longest item that stays whole.  A call of 2^31 units or more (2^37 keys) does nothing but say so.
+// longest item that stays whole; kLeast: units of a block at least.  A call of 2^31 units or more (2^37 keys) does nothing but say so.
 template <class P, int W>
 __device__ __forceinline__ void share_of(const P &p, const Kv4Rows &b, const Kv4Shape &s, bool causal, int *bad, Share *share) {
   constexpr int kThreads = W * 32;
@@ -53,7 +54,7 @@ __device__ __forceinline__ void share_of(const P &p, const Kv4Rows &b, const Kv4
     in_all = 0;
   }
   const uint32_t total = (uint32_t)in_all, upto = (uint32_t)sum, mine = (uint32_t)own;
-  const uint32_t blocks = min(gridDim.x, (total + 1) / 2), me = blockIdx.x;  // a block has two units at least
+  const uint32_t blocks = min(gridDim.x, (total + P::kLeast - 1) / P::kLeast), me = blockIdx.x;
   if (threadIdx.x == 0) {
     share->total = total;
     share->blocks = (int)blocks;

@@ -84,8 +84,10 @@ struct TileItems {
   __device__ int rows(const Seq &q, int rb) const { return min(kRows, q.n * G - rb * kRows); }
   // Keys that row x of a request's packed rows sees.
   __device__ int keys(const Seq &q, int x) const { return causal ? q.len - q.n + x / G + 1 : q.len; }
+  static constexpr int kStart = 4;  // an item's start (Q from memory to S) and end, in tiles
+  static constexpr int kLeast = 12;
   __device__ uint32_t units(const Seq &q, int rb) const {
-    return max(1, (keys(q, rb * kRows + rows(q, rb) - 1) + kKeys - 1) / kKeys);
+    return kStart + (keys(q, rb * kRows + rows(q, rb) - 1) + kKeys - 1) / kKeys;
   }
   __device__ uint64_t all(const Seq &q) const {
     uint64_t n = 0;
@@ -143,9 +145,9 @@ struct Walk {
     rows = p.rows(q, rb);
     return true;
   }
-  __device__ bool no_keys() const { return p.keys(q, r0 + rows - 1) == 0; }
   __device__ int halves() const { return rows > kHalf ? 2 : 1; }
-  __device__ int tiles() const { return no_keys() ? 0 : u1 - u0; }
+  __device__ int first_tile() const { return max(u0 - TileItems::kStart, 0); }
+  __device__ int tiles() const { return max(u1 - TileItems::kStart, 0) - first_tile(); }
 };
 
 // Partial rows of cut items: [256][DP] sums, then m and l of each.
@@ -265,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(Kv4AttnCall c, Kv4Sha
       }
       float m = -INFINITY, l = 0.0f;
       for (int j = 0; j < nt; ++j, ++t) {
-        const int buf = 2 * half + (t & 1), j0 = (walk.u0 + j) * kKeys;
+        const int buf = 2 * half + (t & 1), j0 = (walk.first_tile() + j) * kKeys;
         if (!(ok = long_wait(&s_full[buf], (uint32_t)(t >> 1) & 1, err))) break;
         tc_after();
         if (any) {
@@ -450,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(Kv4AttnCall c, Kv4Sha
     uint32_t window = kNoPlace;
     Page ahead{0, 0};
     bool more = true;
-    auto at = [&](int n) { return (walk.u0 + n) * kKeys + 16 * part; };  // the first of the 16 tokens
+    auto at = [&](int n) { return (walk.first_tile() + n) * kKeys + 16 * part; };  // the first of the 16 tokens
     auto pages = [&](int n) { return n < nt && at(n) < walk.q.len ? page_of(b, s, walk.seq, at(n) / kTokens) : Page{0, 0}; };
     auto places = [&](int n, const Page &p) { return n < nt && at(n) < walk.q.len ? place_of(s, p, walk.kvh, w.bad) : kNoPlace; };
     auto locate = [&] {  // whether there is a next tile

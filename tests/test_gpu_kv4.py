@@ -285,7 +285,7 @@ SHAPES = [
     ([2, 2, 2], [50, 51, 52], 24, 1, 16, 16, nb.F16, True), ([70, 300], [2000, 4000], 16, 8, 128, 64, nb.BF16, True),
     ([1] * 40, [37 * i % 611 + 1 for i in range(40)], 64, 2, 112, 32, nb.F16, True),
     ([7] * 30, [90 + 53 * i % 700 for i in range(30)], 9, 3, 48, 16, nb.BF16, True),
-    ([257], [300], 2, 1, 128, 16, nb.F16, True), ([64, 64], [64, 128], 2, 2, 24, 16, nb.F16, False),
+    ([257], [300], 2, 1, 128, 16, nb.F16, True), ([300, 7], [301, 2000], 64, 2, 64, 32, nb.BF16, True), ([64, 64], [64, 128], 2, 2, 24, 16, nb.F16, False),
 ]
 
 
@@ -300,26 +300,38 @@ def test_attention_of_few_rows(G, D, n):
     attend([n] * 3, [n, 100 + G, 530 + D], 2 * G, 2, D, 32, (nb.F16, nb.BF16)[(G + n) % 2], True, seed=G * n)
 
 
-@pytest.mark.parametrize("D", (40, 64, 128))
+@pytest.mark.parametrize("D", (24, 40, 64, 80, 128))
 @pytest.mark.parametrize("n", (20, 65, 128, 129, 300))
 def test_attention_of_many_rows(n, D):
     attend([n, n // 2, 1], [n, 513, 1025], 4, 2, D, 64, nb.BF16, True, seed=n)
     attend([n, n // 2, 0], [777, 1, 40], 3, 1, D, 16, nb.F16, False, seed=n)
 
 
+@pytest.mark.parametrize("G,D,new,lens,page,dtype,causal", [
+    (4, 128, [1024], [1024], 64, nb.BF16, True), (4, 64, [300, 1, 0, 257], [4000, 1, 17, 257], 16, nb.F16, True),
+    (1, 96, [400, 129], [400, 2050], 32, nb.BF16, True), (8, 32, [64, 65, 33], [64, 65, 700], 48, nb.F16, True),
+    (3, 80, [200, 90], [200, 5000], 16, nb.BF16, True), (2, 128, [600, 0, 5], [0, 70, 333], 128, nb.F16, False),
+    (16, 40, [17, 100, 16], [17, 100, 3000], 256, nb.F16, True), (5, 112, [90] * 7, [90 + 131 * i for i in range(7)], 64, nb.BF16, True),
+    (2, 16, [1000], [1030], 16, nb.F16, True), (4, 72, [257, 63], [63, 2111], 32, nb.BF16, False),
+])
+def test_attention_of_whole_chunks(G, D, new, lens, page, dtype, causal):
+    """Enough rows and heads for the tensor cores' tiles, items cut between blocks and joined among them."""
+    attend(new, lens, 8 * G, 8, D, page, dtype, causal, layout=("token", "head", "fused")[D // 8 % 3], seed=D)
+
+
 @pytest.mark.parametrize("width,scale", [(30.0, 0.3), (1e-4, 1.0), (1e4, 1e-5), (0.0, 1.0)])
-@pytest.mark.parametrize("new", [[1, 2], [40, 130]])
+@pytest.mark.parametrize("new", [[1, 2], [40, 130], [300, 290]])
 def test_sharp_flat_and_scaled_rows(new, width, scale):
     """Weights that fall on one key, on all, and q far from one."""
     for dtype in TYPES:
         attend(new, [300, 2500], 8, 2, 64, 64, dtype, True, width=width, scale=scale)
 
 
-@pytest.mark.parametrize("new", [[3, 5], [40, 70]])
-def test_tokens_that_do_not_fit_reach_only_rows_that_see_them(new):
+@pytest.mark.parametrize("new,heads", [([3, 5], 4), ([40, 70], 4), ([200, 90], 32)])
+def test_tokens_that_do_not_fit_reach_only_rows_that_see_them(new, heads):
     """A draft's infinity is behind the rows before it; the page behind the last token holds NaN from the start."""
     lens = [203, 90]
-    c = Cache(2, 256, 4, 2, 64, 16, nb.F16)
+    c = Cache(2, 256, heads, 2, 64, 16, nb.F16)
     n = sum(lens)
     k, v = c.make((n, 2, 64)), c.make((n, 2, 64))
     k[lens[0] - 1, 0, 3] = float("nan")  # only the last row sees it
@@ -328,7 +340,7 @@ def test_tokens_that_do_not_fit_reach_only_rows_that_see_them(new):
     a = Attn(c, new)
     a.run(0.125, True)
     a.check(0.125, True)
-    assert 0 < int(torch.isnan(a.out).any(-1).sum()) == 2 * (1 + 2)
+    assert 0 < int(torch.isnan(a.out).any(-1).sum()) == heads // 2 * (1 + 2)
 
 
 def test_offsets_past_32_bits():
@@ -342,7 +354,7 @@ def test_offsets_past_32_bits():
     c.table = (n_pages - 1 - torch.arange(6, dtype=torch.int32, device="cuda") * 6).view(2, 3)
     c.append([600, 333])
     c.check_read()
-    for new in ([1, 1], [70, 30]):
+    for new in ([1, 1], [70, 30], [600, 333]):
         a = Attn(c, new)
         a.run(0.1, True)
         a.check(0.1, True)
@@ -401,7 +413,7 @@ def test_a_captured_step_replays_on_other_lengths():
 
 def test_two_plans_on_two_streams():
     parts, want = [], []
-    for i, (new, lens) in enumerate((([1] * 6, [900, 5000, 30, 1, 77, 2048]), ([90, 3], [400, 1000]))):
+    for i, (new, lens) in enumerate((([1] * 6, [900, 5000, 30, 1, 77, 2048]), ([390, 400], [400, 1000]))):
         c = Cache(len(lens), max(lens), 8, 2, 128, 64, nb.F16, i, max_rows=sum(lens))
         c.append(lens)
         a = Attn(c, new)
