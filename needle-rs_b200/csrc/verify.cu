@@ -293,30 +293,17 @@ struct Weights {
     shift = (double)largest * scale;
     least = (float)(-693.0 / inv_t);
   }
-  // Weights of unit u's entries; returns their sum.
-  __device__ __forceinline__ double unit(int u, double *y, const double *table) const {
+  // Weights of entries v0 .. from their values x and q's; returns their sum.
+  __device__ __forceinline__ double weigh(float *x, const float *qs, int v0, double *y, const double *table) const {
     constexpr int E = Row<T>::E;
-    float x[E], qs[E];
-    r.load(u, x);
-    const int v0 = r.first(u), n = r.count(u);
-    if (q) {
-      if (n == E && ((uintptr_t)(q + v0) & 15) == 0) {
-#pragma unroll
-        for (int i = 0; i < E; i += 4) *reinterpret_cast<float4 *>(qs + i) = *reinterpret_cast<const float4 *>(q + v0 + i);
-      } else {
-#pragma unroll
-        for (int i = 0; i < E; ++i) qs[i] = i < n ? q[v0 + i] : 0.0f;
-      }
-    }
     if ((unsigned)(hole - v0) < (unsigned)E) {
 #pragma unroll
       for (int i = 0; i < E; ++i)
         if (v0 + i == hole) x[i] = -INFINITY;
     }
-    double sum = 0.0;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      // weights of zero by bits, not by a branch: the chains of a unit's entries hide each other
+      // weights of zero by bits, not by a branch: the chains of the entries hide each other
       const double e = exp2_table(fma(widened<T>(x[i]), scale, -shift), table);
       y[i] = masked(e, -(int)(x[i] - top > least));
     }
@@ -327,9 +314,44 @@ struct Weights {
         y[i] = masked(e, ~(__double2hiint(e) >> 31));  // zero for what is below zero
       }
     }
+    double sum = 0.0;
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      sum += y[i];
+    for (int i = 0; i < E; ++i) sum += y[i];
+    return sum;
+  }
+  __device__ __forceinline__ void load_q(int v0, int n, float *qs) const {
+    constexpr int E = Row<T>::E;
+    if (n == E && ((uintptr_t)(q + v0) & 15) == 0) {
+#pragma unroll
+      for (int i = 0; i < E; i += 4) *reinterpret_cast<float4 *>(qs + i) = __ldg(reinterpret_cast<const float4 *>(q + v0 + i));
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) qs[i] = i < n ? __ldg(q + v0 + i) : 0.0f;
+    }
+  }
+  // Weights of unit u's entries; returns their sum.
+  __device__ __forceinline__ double unit(int u, double *y, const double *table) const {
+    constexpr int E = Row<T>::E;
+    float x[E], qs[E];
+    r.load(u, x);
+    const int v0 = r.first(u);
+    if (q) load_q(v0, r.count(u), qs);
+    return weigh(x, qs, v0, y, table);
+  }
+  // Sum of the weights of whole vectors [a, b) (units), a lane's every 32nd.
+  __device__ __forceinline__ double vectors(int a, int b, const double *table) const {
+    constexpr int E = Row<T>::E;
+    double sum = 0.0;
+    int u = a + (threadIdx.x & 31);
+    const T *p = r.p + r.first(u);
+#pragma unroll 2
+    for (; u < b; u += 32, p += 32 * E) {
+      float x[E], qs[E];
+      double y[E];
+      const int v0 = r.first(u);
+      r.values(__ldg(reinterpret_cast<const uint4 *>(p)), r.mask ? mask_bits(r.mask, v0, r.words) : 0xffu, x);
+      if (q) load_q(v0, E, qs);
+      sum += weigh(x, qs, v0, y, table);
     }
     return sum;
   }
@@ -383,9 +405,10 @@ __device__ __noinline__ double segment_sums(const Weights<T> w, Shared &sm, int 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, size = (int)cluster_size(), me = (int)cluster_rank();
   const int segments = size * kWarps, seg = me * kWarps + warp, units = w.r.units();
   const int u0 = (int)((int64_t)units * seg / segments), u1 = (int)((int64_t)units * (seg + 1) / segments);
-  double sum = 0.0, y[Row<T>::E];
-#pragma unroll 2
-  for (int u = u0 + lane; u < u1; u += 32) sum += w.unit(u, y, sm.table);
+  const int v0 = max(u0, 1), v1 = min(u1, w.r.vectors + 1);  // whole vectors; the ends by a lane
+  double sum = w.vectors(v0, v1, sm.table), y[Row<T>::E];
+  if (lane == 0 && u0 == 0 && u1 > 0) sum += w.unit(0, y, sm.table);
+  if (lane == 1 && u1 == units && u0 < units) sum += w.unit(units - 1, y, sm.table);
   sum = warp_sum64(sum);
   if (lane < size) store_there(&sm.seg[turn][seg], (uint32_t)lane, sum);
   cluster_meet();
