@@ -28,13 +28,14 @@ def quantise(x):
 
 
 def stored(k, v):
-    """(K values, V values, scale * code + |minimum| of K, scale * code of V, |minimum| of V) that a cache of k, v
-    [tokens][KVH][D] holds; values are NaN for a token and head that does not fit."""
+    """(K values, V values, scale * code + |minimum| of K, scale * |code - 8| + |minimum + 8 scales| of V, scale * (code + 8) +
+    |minimum + 8 scales| of V) that a cache of k, v [tokens][KVH][D] holds; values are NaN for a token and head that does not
+    fit."""
     ok = ((k.double().abs() <= 32768) & (v.double().abs() <= 32768)).all(-1, keepdim=True)
     zero = torch.zeros((), dtype=k.dtype, device=k.device)
     (ck, sk, mk), (cv, sv, mv) = quantise(torch.where(ok, k, zero)), quantise(torch.where(ok, v, zero))
     nan = torch.full((), float("nan"), dtype=torch.float64, device=k.device)
-    return torch.where(ok, mk + sk * ck, nan), torch.where(ok, mv + sv * cv, nan), mk.abs() + sk * ck, sv * cv, mv.abs()
+    return torch.where(ok, mk + sk * ck, nan), torch.where(ok, mv + sv * cv, nan), mk.abs() + sk * ck, sv * (cv - 8).abs() + (mv + 8 * sv).abs(), sv * (cv + 8) + (mv + 8 * sv).abs()
 
 
 def attention(q, kv, rows, lens, scale, causal):
@@ -47,19 +48,20 @@ def attention(q, kv, rows, lens, scale, causal):
     of two has brought its row's largest value to 2^10 or above: exact, but for values below 2^-24 of
     that largest, off by 2^-35 of it.  The exponential adds 8 U and U for each unit of its argument.
     A weight p is rounded to f16 (half a step; below the normal range half of the smallest one, against a row's sum
-    of at least one), and so is p * scale, which multiplies codes up to 15, or, where many rows come together, the value instead;
-    sums over n keys, of p * scale * code and of p * minimum apart, add n U.  Numerator and denominator both carry the errors of
+    of at least one), and so are p * scale, whose rounding meets code - 8 (with the smallest step: up to 8), and minimum + 8 scales,
+    or, where many rows come together, the value instead; sums over n keys, of p * scale * code, of 8 p * scale and of p * (minimum
+    + 8 scales), add n U.  Numerator and denominator both carry the errors of
     the weights."""
     H, D = q.shape[1:]
     eps = 2.0 ** -10
     out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
     lse = torch.full(q.shape[:2], -np.inf, dtype=torch.float64, device=q.device)
     eo, el = torch.zeros_like(out), torch.zeros_like(lse)
-    for (a, m), n, (k, v, mag, vc, vm) in zip(rows, lens, kv):
+    for (a, m), n, (k, v, mag, vc, parts) in zip(rows, lens, kv):
         if not m or not n:
             continue
         G = H // k.shape[1]
-        k, v, mag, vc, vm = (t.repeat_interleave(G, dim=1) for t in (k, v, mag, vc, vm))
+        k, v, mag, vc, parts = (t.repeat_interleave(G, dim=1) for t in (k, v, mag, vc, parts))
         qq = q[a:a + m].double()
         s = torch.einsum("qhd,khd->hqk", qq, k) * scale
         es = torch.einsum("qhd,khd->hqk", qq.abs(), mag * (2 * (D + 16) * U) + k.abs() * (eps / 2) + 2.0 ** -25) * scale
@@ -78,7 +80,6 @@ def attention(q, kv, rows, lens, scale, causal):
         # a value that no row of weight sees may be NaN
         vv = torch.where(torch.isnan(v), 0.0, v)
         rel = (pr * ep).sum(-1) + n * U
-        parts = vc + vm
         o = torch.einsum("hqk,khd->qhd", pr, vv)
         w = torch.einsum("hqk,khd->qhd", pr * (ep + eps / 2 * (1 + eps)), vv.abs())
         w = w + torch.einsum("hqk,khd->qhd", pr, torch.maximum(vc, vv.abs()) * (eps / 2) + 2.0 ** -25) * (1 + eps)
