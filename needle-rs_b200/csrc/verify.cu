@@ -50,7 +50,7 @@ __device__ __forceinline__ Request request(const VerifyCall &c, int i) {
 // Zero and below (and NaN): greedy, log-probabilities of temperature 1.
 __device__ __forceinline__ bool is_greedy(const VerifyCall &c, int i) { return c.temperature && !(c.temperature[i] > 0.0f); }
 __device__ __forceinline__ float temperature(const VerifyCall &c, int i) {
-  return c.temperature && c.temperature[i] > 0.0f ? c.temperature[i] : 1.0f;
+  return c.temperature && c.temperature[i] > 0.0f ? fminf(c.temperature[i], 3e38f) : 1.0f;  // infinity is as good as that
 }
 
 // 8 bits of a row's mask from entry v on (the row has `words` 64-bit words).
@@ -282,7 +282,7 @@ __device__ __forceinline__ double masked(double x, int keep) {
 template <typename T>
 struct Weights {
   Row<T> r;
-  double scale, shift;  // a weight is 2^((x scale - shift) / 512)
+  double scale, top64;  // a weight is 2^((x - top) scale / 512), the difference exact: 0 for the largest at any temperature
   double inv_w;
   float top, least;  // no weight for x - top at or below it: 2^-1000
   const float *q;    // NULL: weights of p
@@ -290,7 +290,7 @@ struct Weights {
 
   __device__ Weights(const Row<T> &row, float largest, double inv_t) : r(row), inv_w(0.0), top(largest), q(nullptr), hole(-1) {
     scale = 1.4426950408889634074 * kTable * inv_t;
-    shift = (double)largest * scale;
+    top64 = (double)largest;
     least = (float)(-693.0 / inv_t);
   }
   // Weights of entries v0 .. from their values x and q's; returns their sum.
@@ -304,7 +304,7 @@ struct Weights {
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       // weights of zero by bits, not by a branch: the chains of the entries hide each other
-      const double e = exp2_table(fma(widened<T>(x[i]), scale, -shift), table);
+      const double e = exp2_table((widened<T>(x[i]) - top64) * scale, table);
       y[i] = masked(e, -(int)(x[i] - top > least));
     }
     if (q) {
@@ -485,6 +485,8 @@ __global__ void __launch_bounds__(kThreads, 4) verify_pick_kernel(VerifyCall c, 
   const Request rq = request(c, i);
   uint32_t *out = c.out_ids + (int64_t)i * c.ld_out;
   float *logp = c.logprobs ? c.logprobs + (int64_t)i * c.ld_out : nullptr;
+  for (int k = tid; k < kTable; k += kThreads) sm.table[k] = exp2((double)k / kTable);
+  pdl_wait();
   if (!rq.ok) {
     for (int64_t j = me * kThreads + tid; j < c.ld_out; j += size * kThreads) {
       out[j] = 0xffffffffu;
@@ -493,12 +495,10 @@ __global__ void __launch_bounds__(kThreads, 4) verify_pick_kernel(VerifyCall c, 
     if (me == 0 && tid == 0) *w.bad = 1, c.out_len[i] = 0;
     return;
   }
-  for (int k = tid; k < kTable; k += kThreads) sm.table[k] = exp2((double)k / kTable);
   const bool greedy = is_greedy(c, i), last = c.flags & 1;
   const float temp = temperature(c, i);
   const double inv_t = 1.0 / (double)temp;
   const float *probs = c.probs;
-  pdl_wait();
 
   // rows in rounds of kThreads: a warp joins a row's pieces, a thread checks a draft
   int taken = 0;           // drafts taken before this round

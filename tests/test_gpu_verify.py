@@ -192,6 +192,13 @@ def test_final_numbers_at_the_ends():
         c.go()
 
 
+@pytest.mark.parametrize("temps", [(1e-30, 1e-6, 0.01), (3e38, float("inf"), 1e4)])
+def test_temperatures_far_from_one(temps):
+    for probs in (True, False):
+        Case([3, 0, 2] * 8, 700, nb.F32, 11, probs=probs, temps=temps).go()
+        Case([2] * 9, 4099, nb.BF16, 12, probs=probs, temps=temps, spread=30.0).go()
+
+
 def test_residuals():
     """The drafter's distribution is the target's (nothing is left over but rounding), a single entry, or far off."""
     V = 600
