@@ -179,7 +179,7 @@ bool kv4_batch(const NeedleKv4Plan *p, const void *pages, const NeedleKv4Batch *
       !aligned(b->row_start, 4) || !aligned(b->kv_len, 4) || !aligned(b->page_table, 4))
     return fail("invalid 4-bit cache arguments");
   *rows = Kv4Rows{b->row_start, b->kv_len, b->page_table, (int)b->n_seq, (int)b->table_width, (int64_t)b->rows,
-                  (int)b->max_new};
+                  (int)(b->max_new ? b->max_new : b->rows)};
   return true;
 }
 
@@ -193,6 +193,7 @@ struct Heads {
 };
 bool kv4_operands(const NeedleKv4Plan *p, std::initializer_list<Heads> operands) {
   for (const Heads &o : operands) {
+    if (!o.p) continue;  // nothing is read from it, or written to it
     if (!aligned(o.p, 16)) return fail("4-bit cache: operands must start on 16-byte boundaries");
     for (size_t s : {o.row, o.head})
       if (s < (size_t)p->s.D || s % 8 || s > kMaxStride)

@@ -431,6 +431,21 @@ def test_two_plans_on_two_streams():
         assert torch.equal(a.out, w)
 
 
+def test_parts_that_are_not_there():
+    """Without a bound of rows, and outputs that are NULL with strides of 0."""
+    c = Cache(2, 64, 4, 2, 64, 16, nb.F16)
+    c.append([20, 33])
+    a = Attn(c, [3, 5])
+    a.batch.max_new = 0
+    a.run(0.125, True)
+    a.check(0.125, True)
+    L, o = nb.lib(), torch.zeros((8, 2, 64), dtype=c.t, device="cuda")
+    assert L.needle_kv4_read(c.plan._h, c.pages.data_ptr(), a.batch._ref, None, 0, 0, o.data_ptr(), 128, 64, None) == 0
+    assert L.needle_kv4_read(c.plan._h, c.pages.data_ptr(), a.batch._ref, None, 0, 0, None, 0, 0, None) == -1
+    c.plan.status()
+    assert torch.equal(o[:3].double(), c.stored()[0][1][-3:].half().double())
+
+
 def test_requests_that_share_pages():
     """A prefix of several requests in the same pages."""
     c = Cache(3, 128, 4, 2, 64, 16, nb.BF16)
