@@ -443,7 +443,7 @@ typedef struct NeedleKv4Batch {
   const int32_t *kv_len;     /* [n_seq] */
   const int32_t *page_table; /* [n_seq][table_width] */
   size_t n_seq, rows, table_width;
-  size_t max_new; /* no request has more rows: `rows` where nothing better is known */
+  size_t max_new; /* no request has more rows; 0: not known */
 } NeedleKv4Batch;
 size_t needle_kv4_page_bytes(size_t num_kv_heads, size_t head_dim, size_t page_tokens);
 NeedleKv4Plan *needle_kv4_plan_create(size_t num_heads, size_t num_kv_heads, size_t head_dim, size_t page_tokens,
@@ -462,7 +462,11 @@ int needle_kv4_read(NeedleKv4Plan *plan, const void *pages, const NeedleKv4Batch
  * needle_cross_attn_plan_run.  With NEEDLE_KV4_CAUSAL the rows are the
  * request's last tokens (appended before): row j of n sees the first
  * kv_len - n + j + 1.  Without it every row sees all kv_len tokens, which may be none: zeros.
- * Sums are f32; the weights of the sum over values, and the values, are rounded to f16.
+ * Sums are f32.  Rounded to f16 are: the weights of the sum over values, their products with
+ * a scale, and minimum + 8 scales; with many rows instead the weights, the keys and the
+ * values.  How many rows come together (rows, max_new) and the lengths decide the form and the order of
+ * a row's sums, so its last bits depend on them; the same call gives the same bits.
+ * q may have any size that its type holds; a row with an infinity or NaN gives NaN.
  * out must not overlap q or itself.  Calls of a plan's attention share its workspace and must be ordered (one
  * stream), and so must the replays of graphs that captured them. */
 #define NEEDLE_KV4_CAUSAL 1u
@@ -479,12 +483,12 @@ void needle_kv4_plan_free(NeedleKv4Plan *plan);
  * draft_start[i] + i + j belongs to its token j.  With
  *   p = softmax(logits / temperature[i])    over the row's allowed entries
  * draft t is taken while accept_u[t] * q < p[draft], q = draft_probs[t][draft] (f32
- * rows [ldp] that the draft was drawn from), or 1 where draft_probs is NULL.
+ * rows [ldp] that the draft was drawn from: finite, zero or more), or 1 where draft_probs is NULL.
  * The first one that is not is replaced by an entry of max(p - q, 0) (NULL:
  * of p without the draft; where that leaves nothing, of p); behind the last draft follows an
  * entry of p.  The entry of weights w is the first v with w_0 + .. + w_v > final_u[i] * sum(w):
  * the random numbers are the caller's, in [0, 1).  Weights and sums are 64-bit there.
- * temperature NULL is 1.  Zero (or less) is greedy: a draft is taken while it
+ * temperature NULL is 1.  Zero (or less, or NaN) is greedy: a draft is taken while it
  * is the row's largest logit, which follows else; of equal ones the lowest
  * index, with NEEDLE_VERIFY_LAST_TIE the highest (as the engine's own head).
  * An entry is allowed if its bit in mask (64-bit words as
