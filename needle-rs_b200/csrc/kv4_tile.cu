@@ -13,7 +13,10 @@
 //
 // q is brought to a largest value of 2^10 .. 2^11 by a power of two for each row and
 // taken as f16 (exact, but for values below 2^-24 of the row's largest); keys and values are
-// minimum + scale * code, rounded to f16 once.
+// minimum + scale * code, rounded to f16 once.  A key's rounding moves its score by some 1e-4: outputs are 4.8e-4 off
+// against 64 bits, where f16 rounds them by 2.1e-4 and bf16 by 1.7e-3.  Where lse is asked for (f32, which would be 6e-6 off
+// for 6e-8), K comes as two f16, the value and what its rounding left (SPLIT; S takes two products): outputs are then 3.5e-4
+// off, and 4 x 1024 tokens over 4096 to 16,384 take 1675 us for 970.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -61,13 +64,14 @@ __device__ __forceinline__ bool long_wait(uint64_t *bar, uint32_t parity, int *e
   return __all_sync(0xffffffffu, ok);
 }
 
-template <int NG>
+template <int NG, bool SPLIT>
 struct Tile {
   static constexpr int kAtoms = NG <= 2 ? 1 : 2;  // 64-dimension parts of a row (128 bytes each)
   static constexpr int kQAtom = kHalf * 128, kAtom = kKeys * 128, kQBytes = kAtoms * kQAtom, kBytes = kAtoms * kAtom;
-  static constexpr int kStages = 3;  // of K, and of V
+  static constexpr int kKBytes = SPLIT ? 2 * kBytes : kBytes;  // of a stage of K
+  static constexpr int kStages = SPLIT ? 2 : 3;                // of K, and of V
   static constexpr int kAhead = 4;  // tiles of 16 tokens in 4 bits that each of the code warps holds
-  static constexpr int kQ = 0, kK = 2 * kQBytes, kV = kK + kStages * kBytes, kCodes = kV + kStages * kBytes;
+  static constexpr int kQ = 0, kK = 2 * kQBytes, kV = kK + kStages * kKBytes, kCodes = kV + kStages * kBytes;
   static constexpr int kBar = kCodes + kCodeWarps * kAhead * tile_bytes(NG);
   static constexpr int kSmem = kBar + 512 + 1024;
   static constexpr int kDims = 64 * kAtoms;  // columns of O
@@ -175,9 +179,22 @@ __device__ __forceinline__ void values(uint32_t w, __half2 s, __half2 m, uint32_
   }
 }
 
-template <typename T, int NG>
+// The same as two f16: product and sum with what their roundings leave (two-product, two-sum).
+__device__ __forceinline__ void split_values(uint32_t w, __half2 s, __half2 m, uint32_t i1024, uint32_t i64, uint32_t *v, uint32_t *rest) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t u = k < 2 ? w : w >> 8;
+    const __half2 c = k & 1 ? __hsub2(pair(and_or(u, 0x00f000f0u, i64)), pair(i64)) : __hsub2(pair(and_or(u, 0x000f000fu, i1024)), pair(i1024));
+    const __half2 p = __hmul2_rn(c, s), p_rest = __hfma2(c, s, __hneg2(p)), sum = __hadd2_rn(m, p), back = __hsub2_rn(sum, m);
+    const __half2 s_rest = __hadd2_rn(__hsub2_rn(m, __hsub2_rn(sum, back)), __hsub2_rn(p, back));
+    v[k] = bits(sum);
+    rest[k] = bits(__hadd2_rn(s_rest, p_rest));
+  }
+}
+
+template <typename T, int NG, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1) tile_kernel(Kv4AttnCall c, Kv4Shape s, Kv4Rows b, Kv4Work w) {
-  using L = Tile<NG>;
+  using L = Tile<NG, SPLIT>;
   constexpr int ST = L::kStages, DP = NG * 32;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t *sm = smem_raw + (-smem_u32(smem_raw) & 1023);  // an offset: accesses stay known to be shared memory
@@ -510,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(Kv4AttnCall c, Kv4Sha
       const int st = t % ST;
       const uint32_t ph = (uint32_t)(t / ST) & 1;
       if (!(ok = long_wait(&k_empty[st], ph ^ 1, err))) break;
-      uint8_t *K = sm + L::kK + st * L::kBytes, *V = sm + L::kV + st * L::kBytes;
+      uint8_t *K = sm + L::kK + st * L::kKBytes, *V = sm + L::kV + st * L::kBytes;
       // all loads before the stores, which could be of the same bytes for all that the compiler knows
       uint2 kc[NG], vc[NG];
       uint32_t ks[NG], km[NG];
@@ -528,11 +545,14 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(Kv4AttnCall c, Kv4Sha
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint32_t sel = h ? 0x3232 : 0x1010;
-          uint32_t v[4];
-          values(h ? kc[g].y : kc[g].x, pair(__byte_perm(ks[g], 0, sel)), pair(__byte_perm(km[g], 0, sel)), i1024, i64, v);
+          uint32_t v[4], rest[4];
+          const __half2 sc = pair(__byte_perm(ks[g], 0, sel)), mi = pair(__byte_perm(km[g], 0, sel));
+          if (SPLIT) split_values(h ? kc[g].y : kc[g].x, sc, mi, i1024, i64, v, rest);
+          else values(h ? kc[g].y : kc[g].x, sc, mi, i1024, i64, v);
           const int row = ta + 2 * h, ch = 4 * g + q4;
-          *reinterpret_cast<uint4 *>(K + (ch >> 3) * L::kAtom + row * 128 + (((ch & 7) ^ (row & 7)) << 4)) =
-              make_uint4(v[0], v[1], v[2], v[3]);
+          uint8_t *to = K + (ch >> 3) * L::kAtom + row * 128 + (((ch & 7) ^ (row & 7)) << 4);
+          *reinterpret_cast<uint4 *>(to) = make_uint4(v[0], v[1], v[2], v[3]);
+          if (SPLIT) *reinterpret_cast<uint4 *>(to + L::kBytes) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
         }
       fence_async_smem();
       __syncwarp();
@@ -573,7 +593,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(Kv4AttnCall c, Kv4Sha
       for (int j = 0; j < nt && ok; ++j, ++t) {
         const int st = t % ST;
         if (!(ok = long_wait(&k_full[st], (uint32_t)(t / ST) & 1, err))) break;
-        const uint32_t k = (s16 + (uint32_t)((L::kK + st * L::kBytes) >> 4)) | (1u << 16);
+        const uint32_t k = (s16 + (uint32_t)((L::kK + st * L::kKBytes) >> 4)) | (1u << 16);
         for (int h = 0; h < nh && ok; ++h) {
           const int n = th[h]++, buf = 2 * h + (n & 1);
           if (n >= 2 && !(ok = long_wait(&pv_done[buf], (uint32_t)((n - 2) >> 1) & 1, err))) break;
@@ -583,6 +603,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(Kv4AttnCall c, Kv4Sha
           for (int u = 0; u < DP / 16; ++u) {
             const uint32_t in = (uint32_t)((u & 3) * 2), qa = (u >> 2) * (L::kQAtom >> 4) + in, ka = (u >> 2) * (L::kAtom >> 4) + in;
             umma_bf16_e(tmem + (uint32_t)(buf * kKeys), hi | (q16 + qa), hi | (k + ka), id, u ? 1u : 0u);
+            if (SPLIT) umma_bf16_e(tmem + (uint32_t)(buf * kKeys), hi | (q16 + qa), hi | (k + ka + (uint32_t)(L::kBytes >> 4)), id, 1u);
           }
           umma_commit_e(&s_full[buf]);
         }
@@ -634,19 +655,25 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(Kv4AttnCall c, Kv4Sha
   }
 }
 
-template <typename T, int NG>
+template <typename T, int NG, bool SPLIT>
 cudaError_t launch(const Kv4Shape &s, const Kv4Rows &b, const Kv4AttnCall &c, const Kv4Work &w, cudaStream_t st) {
-  auto *kernel = tile_kernel<T, NG>;
+  constexpr int smem = Tile<NG, SPLIT>::kSmem;
+  static_assert(smem <= 227 * 1024 - 2048, "a block's shared memory");
+  auto *kernel = tile_kernel<T, NG, SPLIT>;
   static thread_local int ready = -1;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && ready != dev) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<NG>::kSmem);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e == cudaSuccess) ready = dev;
   }
   if (e != cudaSuccess) return e;
-  kernel<<<w.sms, kThreads, Tile<NG>::kSmem, st>>>(c, s, b, w);
+  kernel<<<w.sms, kThreads, smem, st>>>(c, s, b, w);
   return cudaGetLastError();
+}
+template <typename T, int NG>
+cudaError_t launch(const Kv4Shape &s, const Kv4Rows &b, const Kv4AttnCall &c, const Kv4Work &w, cudaStream_t st) {
+  return c.lse ? launch<T, NG, true>(s, b, c, w, st) : launch<T, NG, false>(s, b, c, w, st);
 }
 
 template <typename T>
