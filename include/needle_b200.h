@@ -500,7 +500,8 @@ void needle_kv4_plan_free(NeedleKv4Plan *plan);
  * number, logprobs (may be NULL) log p of each (greedy: of temperature 1); both have rows of ld_out entries, at
  * least a request's drafts + 1, and are filled up with 0xffffffff and 0.
  * What the kernels find out of range (draft_start that falls or passes n_drafts, more drafts than ld_out - 1) gives
- * that request no token and is reported by needle_verify_plan_status.
+ * that request no token and is reported by needle_verify_plan_status; where draft_start falls, the other
+ * requests' tokens are undefined. An array of outputs must not overlap another array.
  * A draft outside the vocabulary is not taken.
  * dtype: f32, f16 or bf16 logits.  Calls on one plan share its workspace and must be ordered. */
 #define NEEDLE_VERIFY_LAST_TIE 1u

@@ -202,6 +202,15 @@ bool kv4_operands(const NeedleKv4Plan *p, std::initializer_list<Heads> operands)
   return true;
 }
 
+struct Span {
+  const void *p;
+  size_t bytes;
+};
+bool meet(const Span &a, const Span &b) {
+  const uintptr_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;
+  return x && y && a.bytes && b.bytes && x < y + b.bytes && y < x + a.bytes;
+}
+
 // Whether the elements of `rows` rows of `heads` heads are different ones.
 bool apart(const NeedleKv4Plan *p, size_t rows, size_t row, size_t head, int heads) {
   const size_t D = (size_t)p->s.D;
@@ -620,6 +629,23 @@ int needle_verify_plan_run(NeedleVerifyPlan *p, const void *logits, size_t ldl, 
     if (ldl < V || ldl > kMaxStride || (mask && (ld_mask < (V + 63) / 64 || ld_mask > kMaxStride)) ||
         (draft_probs && (ldp < V || ldp > kMaxStride)))
       return fail("verification: a row stride is below the vocabulary");
+    // the blocks of a request read drafts while one of them writes
+    const size_t rows = n_drafts + n_seq, out = n_seq * ld_out * 4, drafts = n_drafts * 4, seqs = n_seq * 4;
+    const Span inputs[] = {{logits, ((rows - 1) * ldl + V) * dtype_size(p->s.dtype)},
+                           {mask, ((rows - 1) * ld_mask + (V + 63) / 64) * 8},
+                           {draft_start, seqs + 4},
+                           {draft_ids, drafts},
+                           {draft_probs, n_drafts ? ((n_drafts - 1) * ldp + V) * 4 : 0},
+                           {temperature, seqs},
+                           {accept_u, drafts},
+                           {final_u, seqs}};
+    const Span outputs[] = {{out_ids, out}, {logprobs, out}, {out_len, seqs}};
+    for (const Span &o : outputs) {
+      for (const Span &i : inputs)
+        if (meet(i, o)) return fail("verification: an output overlaps an input");
+      for (const Span &other : outputs)
+        if (&other != &o && meet(other, o)) return fail("verification: outputs overlap");
+    }
     OnDevice on(p->device);
     if (!on.good() ||
         !all_on(p->device, {{"logits", logits}, {"mask", mask}, {"draft_start", draft_start}, {"draft_ids", draft_ids},

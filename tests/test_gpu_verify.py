@@ -288,3 +288,25 @@ def test_captured_and_on_other_streams():
         torch.cuda.synchronize()
         for a, b in zip(kept, (c.out, c.len, c.logp)):
             assert torch.equal(a, b)
+
+
+def test_overlapping_outputs_are_refused():
+    c = Case([4], 100, nb.F32, 12)
+    plan = nb.VerifyPlan(100, 1, c.total, nb.F32)
+    c.place()
+    out, logp, lens = c.out, c.logp, c.len
+    kept = [t.clone() for t in (out, logp, lens, c.di, c.dl)]
+    for name, other in (("out", c.di), ("out", c.du), ("len", c.ds), ("len", c.df), ("logp", c.dt), ("logp", c.dp), ("out", c.dl[2:])):
+        setattr(c, name, other)
+        with pytest.raises(nb.NeedleError, match="output overlaps an input"):
+            c.run(plan)
+        c.out, c.logp, c.len = out, logp, lens
+    for name, other in (("out", c.logp), ("len", c.out[0, 4:])):
+        setattr(c, name, other)
+        with pytest.raises(nb.NeedleError, match="outputs overlap"):
+            c.run(plan)
+        c.out, c.logp, c.len = out, logp, lens
+    plan.status()
+    assert all(torch.equal(a, b) for a, b in zip(kept, (out, logp, lens, c.di, c.dl)))
+    c.run(plan)
+    c.check()
