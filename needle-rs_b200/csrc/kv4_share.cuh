@@ -33,7 +33,7 @@ __device__ __forceinline__ void share_of(const P &p, const Kv4Rows &b, const Kv4
   Seq q{0, 0, 0};
   for (int i = i0; i < i1; ++i) {
     q = sequence(b, s, i, causal, bad);
-    own += p.all(q);
+    own += min(p.all(q), (uint64_t)1 << 40);  // 2^20 requests' sum stays in 64 bits, whatever their numbers say
   }
   uint64_t sum = own;
 #pragma unroll
