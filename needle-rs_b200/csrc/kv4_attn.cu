@@ -16,15 +16,19 @@
 //      codes, then an FMA a group for each score; the second terms are one small
 //      product of the minima with the sums, each in two f16.  No key is rounded.
 //   V: the weights (f16) times a group's s, rounded to f16 again, multiply the
-//      codes less 8; what is left, m + 8 s (rounded to f16) times the weights, is one small product of a
-//      row for each group.  With c and m apart, sums over 50,000 keys cancelled to a hundredth and kept the tensor
-//      cores' truncation: 6e-4 off against 64 bits, now 3.5e-4 (rounding the output to f16 alone: 2e-4), for 8% of the time.
+//      codes less 8; what is left, m + 8 s (rounded to f16) times the weights, is one
+//      small product of a row for each group.  For f16 outputs the weights meet s as two f16,
+//      so that their products are rounded once.
+//      Errors against 64 bits over 50,000 keys, where rounding an output to f16 alone is 2.1e-4: codes and minima apart, whose
+//      sums cancel to a hundredth and keep the tensor cores' truncation, 5.6e-4 (63 us for 8 requests of 8k to 50k); codes
+//      less 8 3.5e-4 (69); weights as two f16 3.05e-4 (71); in the small product too 2.98e-4 (73).
 // q is brought to a largest value of 2^10 .. 2^11 by a power of two for each row and
 // taken as f16 (exact, but for values below 2^-24 of the row's largest).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_tile.cuh"
 #include "common.cuh"
@@ -97,6 +101,7 @@ __global__ void __launch_bounds__(kThreads, few_blocks(NB))
     few_kernel(Kv4AttnCall c, Kv4Shape s, Kv4Rows b, Kv4Work w) {
   constexpr int ST = few_stages(NG), TB = tile_bytes(NG), ROWS = NB * 8, DP = NG * 32, PAIR = 2 * kTokens;
   constexpr uint32_t kLo = 0x000f000fu, kHi = 0x00f000f0u;
+  constexpr bool FINE = std::is_same<T, __half>::value;  // outputs of f16: weights times scales are rounded once
   extern __shared__ __align__(128) uint8_t sm[];
   __shared__ int last_one;
   __shared__ Share share;
@@ -360,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, few_blocks(NB))
           }
         __syncwarp();
       }
-      uint32_t pf[NB][2][2];
+      uint32_t pf[NB][2][2], pl[NB][2][2];  // the weights as f16, and what that leaves of them
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -371,8 +376,15 @@ __global__ void __launch_bounds__(kThreads, few_blocks(NB))
           l[nb][0] += p[0] + p[2];
           l[nb][1] += p[1] + p[3];
           // keys by rows -> rows by keys: the other operand of the product with V
-          pf[nb][half][0] = transpose8(bits(__floats2half2_rn(p[0], p[1])));
-          pf[nb][half][1] = transpose8(bits(__floats2half2_rn(p[2], p[3])));
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const __half2 h = __floats2half2_rn(p[2 * k], p[2 * k + 1]);
+            pf[nb][half][k] = transpose8(bits(h));
+            if constexpr (FINE) {
+              const float2 f = __half22float2(h);
+              pl[nb][half][k] = transpose8(bits(__floats2half2_rn(p[2 * k] - f.x, p[2 * k + 1] - f.y)));
+            }
+          }
         }
 
       // O^T += (codes - 8)^T (weights times scales), the 8 by a product of its own; a row for each group of (minima + 8
@@ -392,8 +404,14 @@ __global__ void __launch_bounds__(kThreads, few_blocks(NB))
           const uint32_t vx = v.x >> 8, vy = v.y >> 8, lo8 = 0x80088008u, hi8 = 0x80808080u;  // -8 in a code's places
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb) {
-            const uint32_t p0 = bits(__hmul2(halves(pf[nb][half][0]), halves(sv.x)));
-            const uint32_t p1 = bits(__hmul2(halves(pf[nb][half][1]), halves(sv.y)));
+            uint32_t p0, p1;
+            if constexpr (FINE) {
+              p0 = bits(__hfma2(halves(pf[nb][half][0]), halves(sv.x), __hmul2(halves(pl[nb][half][0]), halves(sv.x))));
+              p1 = bits(__hfma2(halves(pf[nb][half][1]), halves(sv.y), __hmul2(halves(pl[nb][half][1]), halves(sv.y))));
+            } else {
+              p0 = bits(__hmul2(halves(pf[nb][half][0]), halves(sv.x)));
+              p1 = bits(__hmul2(halves(pf[nb][half][1]), halves(sv.y)));
+            }
             mma(o[nb][g], lo8, hi8, lo8, hi8, p0, p1);
             mma(o[nb][g] + 4, lo8, hi8, lo8, hi8, p0, p1);
             mma(o[nb][g], v.x & kLo, v.x & kHi, v.y & kLo, v.y & kHi, p0, p1);
