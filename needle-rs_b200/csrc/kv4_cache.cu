@@ -51,27 +51,33 @@ struct Walk {
     }
   }
   __device__ void start(const Kv4Rows &b, const Kv4Shape &s, int *bad) {
-    __shared__ uint32_t sums[kWarps], found_base;
+    __shared__ uint64_t sums[kWarps];
+    __shared__ uint32_t found_base;
     __shared__ int found;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int per = (b.n_seq + kThreads - 1) / kThreads, i0 = min((int)threadIdx.x * per, b.n_seq), i1 = min(i0 + per, b.n_seq);
-    uint32_t mine = 0;
-    for (int i = i0; i < i1; ++i) mine += units_of(sequence(b, s, i, true, bad), s.KVH);
-    uint32_t sum = mine;
+    uint64_t own = 0;
+    for (int i = i0; i < i1; ++i) own += units_of(sequence(b, s, i, true, bad), s.KVH);
+    uint64_t sum64 = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t x = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += x;
+      const uint64_t x = __shfl_up_sync(0xffffffffu, sum64, o);
+      if (lane >= o) sum64 += x;
     }
-    if (lane == 31) sums[warp] = sum;
+    if (lane == 31) sums[warp] = sum64;
     if (threadIdx.x == 0) found = b.n_seq, found_base = 0;
     __syncthreads();
-    uint32_t total = 0;
+    uint64_t all = 0;
 #pragma unroll
     for (int k = 0; k < kWarps; ++k) {
-      if (k < warp) sum += sums[k];
-      total += sums[k];
+      if (k < warp) sum64 += sums[k];
+      all += sums[k];
     }
+    if (all >> 32) {  // rows of their own make fewer: these requests share them, and nothing is done
+      *bad = 1;
+      all = 0;
+    }
+    const uint32_t total = (uint32_t)all, mine = (uint32_t)own, sum = (uint32_t)sum64;
     const uint32_t begin = (uint32_t)((uint64_t)total * blockIdx.x / gridDim.x);
     end = (uint32_t)((uint64_t)total * (blockIdx.x + 1) / gridDim.x);
     uint32_t before = sum - mine;

@@ -458,3 +458,21 @@ def test_requests_that_share_pages():
     a = Attn(c, [7, 20, 1])
     a.run(0.125, True)
     a.check(0.125, True)
+
+
+def test_requests_that_share_rows_do_nothing():
+    # row starts that rise and fall: 131,073 requests of the same 65,536 rows, 2^32 tiles and more
+    R, n = 65536, 2 * 131073
+    plan = nb.Kv4Plan(8, 8, 8, R, 1, n, R, nb.F16)
+    pages = torch.full((nb.kv4_page_bytes(8, 8, R),), 0xff, dtype=torch.uint8, device="cuda")
+    start, lens, table = i32([0, R] * (n // 2) + [0]), i32([R] * n), i32([0] * n)
+    b = nb.Kv4Batch(start.data_ptr(), lens.data_ptr(), table.data_ptr(), n, R, 1)
+    x = torch.ones((R, 8, 8), dtype=torch.float16, device="cuda")
+    out, ko, vo = (torch.full_like(x, 7.0) for _ in range(3))
+    for f in (lambda: plan.append(pages.data_ptr(), b, x.data_ptr(), x.data_ptr()),
+              lambda: plan.read(pages.data_ptr(), b, ko.data_ptr(), vo.data_ptr()),
+              lambda: plan.attn(pages.data_ptr(), b, x.data_ptr(), out.data_ptr(), 0.1)):
+        f()
+        with pytest.raises(nb.NeedleError, match="out of range"):
+            plan.status()
+    assert (pages == 0xff).all() and all((t == 7.0).all() for t in (out, ko, vo))
