@@ -501,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_pick_kernel(VerifyCall c, 
   const float *probs = c.probs;
 
   // rows in rounds of kThreads: a warp joins a row's pieces, a thread checks a draft
-  int taken = 0;           // drafts taken before this round
+  int taken = 0;           // drafts taken in earlier turns
   int len = -1;            // tokens, when the request has ended
   uint32_t token = 0xffffffffu;
   float row_top = 0.0f, row_sum = 0.0f;
